@@ -1,0 +1,1335 @@
+// Attention over an int8 KV cache for batches whose sequences have lengths of their own
+// (sm_100a): a sliding window with sink tokens for decode steps and prefill chunks, and
+// decode over a prefix that a group of sequences shares.
+//
+//   o = sum_j softmax_j(q . k_j / sqrt(D)) v_j,   k_j[d] = code * k_scale[d],
+//                                                  v_j[d] = code * v_scale[j]
+//
+// A query at position p sees key j when j <= p and (j > p - window or j < sinks); a query
+// over a shared prefix sees all of it and all of its own sequence's tokens.
+//
+// Mathematics.  One pass over the keys with the running maximum and sum of a softmax, in
+// base 2.  Neither cache side is dequantized: the K scales, the softmax scale and log2(e)
+// are folded into q once per row (q' = q k_scale sm_scale log2 e, times a power of two
+// that brings the row's largest |q'| to [2^13, 2^14), rounded to float16; for float16
+// models a second float16 holds what the first leaves over), and the V scale of key j
+// joins the exponent: with t_j = s_j + log2 v_scale_j and m a running maximum of t,
+//   P_j = 2^(t_j - m) (float16),  O += P_j code_j,  l += P_j / v_scale_j (float32),
+// so o = O / l holds for V scales of any size, and P needs no scaling of its own.  The
+// int8 codes are exact in float16.  m moves only when t grows by more than 8 (P <= 256,
+// far inside float16), so O in tensor memory is rarely rescaled.  P rounded to float16 is
+// off by 2^-11 of itself at most, half a step of the coarsest output type below bf16.
+//
+// Work.  Row r of a unit (kv head, sequence or group) is q head kvh * n_rep + r % n_rep of
+// query r / n_rep; 128 rows sit on the 128 lanes of tensor memory, one or two such tiles
+// per block share every key tile (NM).  Keys that no row of the block can see are never
+// read: a block's keys are numbered v = 0 .. nv - 1, the sinks first, then the window's
+// run, and cut into tiles of 128.  Decode kernels (STREAM) lay the tiles of all units in
+// one line and give each block an equal run of it, whatever the lengths; a unit cut by a
+// block border leaves partial states (m, l, O) that combine_kernel joins.  Prefill blocks
+// take one row tile each (split over a few blocks when there are few).
+//
+// Roles of a block (one per SM): softmax warps (4 per row tile, one thread per row), 8
+// warps that read codes from global memory into registers two tiles ahead, turn them into
+// float16 with byte permutes and store them in the 128-byte-swizzled layouts the MMA reads
+// (they also form q'), and one warp whose first lane issues the tcgen05.mma products:
+// S = Q K^T into tensor memory, O += P V with P read from tensor memory, where it
+// overwrites the S it came from.  mbarriers order the roles; every wait is bounded.
+#include <algorithm>
+#include <atomic>
+
+#include "hq_common.cuh"
+#include "umma.cuh"
+
+namespace hq {
+int current_sm_count();
+
+namespace rag {
+using namespace tc;
+
+constexpr int kD = 128;
+constexpr int kBN = 128;                  // keys per tile
+constexpr int kConvThreads = 256;
+constexpr int kTileB = kBN * kD * 2;      // a float16 K, V or Q tile: 32 KB
+constexpr int kStages = 2;                // K and V tiles in shared memory
+constexpr int kLvSlots = 4;               // ring of the keys' log2 V scales and reciprocals
+constexpr int kMaxEntries = 2048;         // sequences plus groups of one call
+constexpr int kPartRow = kD + 4;          // partial rows: m, l, two pad words, o
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColO = 256;           // S buffers at columns 0 and 128
+
+// One set of keys and the rows that read it.
+struct Seg {
+  const int8_t* k;
+  const int8_t* v;
+  int64_t sb, sh, ss;                     // strides of both (b, h, token)
+  const void* ksc;
+  const void* vsc;
+  int64_t kscb, ksch, kscd, vscb, vsch, vscs;
+  const int* lens;                        // tokens held, per entry; null: cap
+  int cap;
+  int nb;                                 // entries (sequences, or groups)
+  int units;                              // queries per entry
+  int step;                               // 1: query u stands u positions after query 0
+  int64_t qsb, qsu;
+  int window, sinks;
+};
+
+struct Params {
+  Seg seg[2];
+  int nseg;
+  const void* q;
+  int64_t qsh;
+  int q_dt, s_dt;
+  int Hkv, nrep;
+  float qk_scale;                         // sm_scale * log2(e)
+  int q_quant;
+  const int* q_lens;                      // prefill: queries per sequence; null: all
+  void* out;                              // rows [b][u][h]
+  int64_t osb, osu, osh;
+  float* part;                            // partial states
+  int* cum;                               // STREAM: first tile of each entry, for combine_kernel
+  int* status;
+  int n_split, n_rt;                      // prefill grid: splits, row tiles
+  int merge_all;                          // every piece goes through combine_kernel
+  int rows_cap[2];                        // partial rows per piece of each segment
+  int64_t part1;                          // float offset of the second segment's pieces
+  int min_tiles;                          // STREAM: least tiles per block
+};
+
+template <int NM, bool LO>
+struct Cfg {
+  static constexpr int kSoft = 128 * NM;
+  static constexpr int kThreads = kSoft + kConvThreads + 32;
+  static constexpr int kParts = LO ? 2 : 1;
+  static constexpr int kQBuf = NM * kParts == 1 ? 2 : 1;
+  static constexpr int kQB = kQBuf * NM * kParts * kTileB;
+  static constexpr int kOffK = kQB;
+  static constexpr int kOffV = kOffK + kStages * kTileB;
+  static constexpr int kOffLv = kOffV + kStages * kTileB;          // [slot][log2, 1/x][128]
+  static constexpr int kOffFac = kOffLv + kLvSlots * 2 * kBN * 4;  // [qbuf][128 NM]
+  static constexpr int kOffBar = kOffFac + kQBuf * 128 * NM * 4;
+  static constexpr int kBars = 2 * kQBuf + 4 * kStages + kLvSlots + 2 + 2 + 2 * NM + 1;
+  static constexpr int kOffMisc = kOffBar + ((kBars * 8 + 15) & ~15);
+  static constexpr int kOffCum = kOffMisc + 16;
+  static constexpr int smem(int entries) { return 1024 + kOffCum + 4 * (entries + 1); }
+  static_assert(1024 + kOffCum + 4 * (kMaxEntries + 1) <= 232448, "one block per SM");
+};
+
+// ---------------------------------------------------------------- small helpers
+__device__ __forceinline__ uint4 ldg_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float load_scale(const void* p, int64_t i, int dt) {
+  return dt == HQ_DTYPE_F16 ? __half2float(static_cast<const __half*>(p)[i])
+                            : static_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// four int8 codes -> two float16 pairs, exact: the biased byte under the exponent of 1024
+__device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t& a, uint32_t& b) {
+  const uint32_t u = w ^ 0x80808080u;
+  const uint32_t k1152 = 0x64806480u;
+  const uint32_t x = prmt(u, 0x64646464u, 0x4140u), y = prmt(u, 0x64646464u, 0x4342u);
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(a) : "r"(x), "r"(k1152));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(b) : "r"(y), "r"(k1152));
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db,
+                                           uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(db), "r"(id), "r"(accumulate));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// Bounded wait (2 s, or as soon as another role of the block has given up).
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63) == 0 && (*abort || global_ns() - t0 > kWaitNs)) {
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- pieces of work
+// The keys of one row tile, numbered v = 0 .. nv - 1: key = v < ns ? v : v + sh.
+struct Keys {
+  int pos0;        // position of the entry's query 0
+  int ns, sh, nv, nt;
+};
+__device__ __forceinline__ int seg_len(const Seg& s, int b) {
+  return s.lens ? min(max(s.lens[b], 0), s.cap) : s.cap;
+}
+// n tokens held, nq queries of which rows u_lo .. u_hi are in the tile
+__device__ __forceinline__ Keys make_keys(const Seg& s, int n, int nq, int u_lo, int u_hi) {
+  Keys k;
+  k.pos0 = s.step ? n - nq : n - 1;
+  const int p_lo = k.pos0 + (s.step ? u_lo : 0), p_hi = k.pos0 + (s.step ? u_hi : 0);
+  const int w0 = max(0, p_lo - s.window + 1);
+  if (w0 <= s.sinks) {
+    k.ns = 0;
+    k.sh = 0;
+    k.nv = p_hi + 1;
+  } else {
+    k.ns = s.sinks;
+    k.sh = w0 - s.sinks;
+    k.nv = p_hi + 1 - k.sh;
+  }
+  k.nv = max(k.nv, 0);
+  k.nt = (k.nv + kBN - 1) / kBN;
+  return k;
+}
+struct Piece {
+  int seg, b, kvh, row0, rows;
+  Keys key;
+  int t0, t1;
+  int slot;        // -1: final output
+};
+
+// STREAM: tiles of entry e, one row tile (0: the call is answered by combine_kernel)
+__device__ __forceinline__ int entry_tiles(const Params& p, int e) {
+  const int si = e < p.seg[0].nb ? 0 : 1;
+  const Seg& s = p.seg[si];
+  const int n = seg_len(s, e - (si ? p.seg[0].nb : 0));
+  const int nt = make_keys(s, n, s.units, 0, 0).nt;
+  return p.merge_all ? nt : max(nt, 1);
+}
+__device__ __host__ __forceinline__ int row_tiles(int rows, int mt) { return (rows + mt - 1) / mt; }
+
+// The pieces of one block, in order.
+template <int MT, bool STREAM>
+struct Walk {
+  int cur, end, e;
+  __device__ __forceinline__ void start(const Params& p, const int* cum) {
+    if constexpr (STREAM) {
+      const int ne = p.seg[0].nb + (p.nseg > 1 ? p.seg[1].nb : 0);
+      const int total = cum[ne];
+      const int per = max(p.min_tiles, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+      cur = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total)));
+      end = static_cast<int>(min(static_cast<int64_t>(cur) + per, static_cast<int64_t>(total)));
+      // the entry that holds tile cur: cum[e] <= cur < cum[e + 1]
+      int lo = 0, hi = ne - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cum[mid] <= cur) lo = mid; else hi = mid - 1;
+      }
+      e = lo;
+    } else {
+      cur = 0;
+      end = 1;
+    }
+  }
+  __device__ __forceinline__ bool next(const Params& p, const int* cum, Piece& w) {
+    if (cur >= end) return false;
+    if constexpr (STREAM) {
+      while (cum[e + 1] <= cur) ++e;
+      w.seg = e < p.seg[0].nb ? 0 : 1;
+      const Seg& s = p.seg[w.seg];
+      w.b = e - (w.seg ? p.seg[0].nb : 0);
+      const int rows = s.units * p.nrep, n_rt = row_tiles(rows, MT), per_e = p.Hkv * n_rt;
+      const int nt = (cum[e + 1] - cum[e]) / per_e;
+      const int idx = (cur - cum[e]) / nt, first = cum[e] + idx * nt;
+      const int rt = idx / p.Hkv;
+      w.kvh = idx - rt * p.Hkv;
+      w.row0 = rt * MT;
+      w.rows = min(MT, rows - w.row0);
+      w.key = make_keys(s, seg_len(s, w.b), s.units, 0, 0);
+      w.t0 = cur - first;
+      w.t1 = min(nt, w.t0 + end - cur);
+      cur = first + w.t1;
+      w.slot = !p.merge_all && w.t0 == 0 && w.t1 == nt ? -1 : w.b * per_e + idx + static_cast<int>(blockIdx.x);
+    } else {
+      cur = 1;
+      // longest row tiles (the last ones of a causal chunk) first
+      const int rt = p.n_rt - 1 - static_cast<int>(blockIdx.y) / p.Hkv;
+      const int b = blockIdx.z, split = blockIdx.x;
+      const Seg& s = p.seg[0];
+      const int nq = p.q_lens ? min(max(p.q_lens[b], 0), s.units) : s.units;
+      w.seg = 0;
+      w.b = b;
+      w.kvh = static_cast<int>(blockIdx.y) % p.Hkv;
+      w.row0 = rt * MT;
+      w.rows = min(MT, nq * p.nrep - w.row0);
+      if (w.rows <= 0) return false;
+      w.key = make_keys(s, seg_len(s, b), nq, w.row0 / p.nrep, (w.row0 + w.rows - 1) / p.nrep);
+      const int nt = max(w.key.nt, 1);
+      w.t0 = static_cast<int>(static_cast<int64_t>(nt) * split / p.n_split);
+      w.t1 = static_cast<int>(static_cast<int64_t>(nt) * (split + 1) / p.n_split);
+      w.slot = p.n_split == 1 ? -1
+                              : ((b * p.Hkv + w.kvh) * p.n_rt + rt) * p.n_split + split;
+    }
+    return true;
+  }
+};
+
+__device__ __forceinline__ float* part_row(const Params& p, int seg, int slot, int r) {
+  return p.part + (seg ? p.part1 : 0) +
+         (static_cast<int64_t>(slot) * p.rows_cap[seg] + r) * kPartRow;
+}
+
+// Stores 4 consecutive values of an output row.
+__device__ __forceinline__ void store4(void* row, int dt, int d, float a, float b, float c, float e) {
+  uint2 w;
+  if (dt == HQ_DTYPE_BF16) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, e);
+    w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  } else {
+    w = make_uint2(pack_h2(a, b), pack_h2(c, e));
+  }
+  *reinterpret_cast<uint2*>(static_cast<char*>(row) + 2 * d) = w;
+}
+__device__ __forceinline__ char* out_row(const Params& p, int b, int u, int h) {
+  return static_cast<char*>(p.out) + 2 * (b * p.osb + u * p.osu + h * p.osh);
+}
+
+// ---------------------------------------------------------------- softmax of one row tile
+struct RowLim {
+  int hi, lo, vsk;  // key v is seen when v <= hi and (v >= lo or v < vsk)
+};
+// t = s * fac + log2(v_scale) of 32 keys, masked; returns into f (pairs)
+template <bool MASK>
+__device__ __forceinline__ void row_t(const float (&s)[32], const float* lv, float fac, int v0,
+                                      const RowLim& lim, float (&t)[32]) {
+  const F2 f2 = f2_make(fac, fac);
+#pragma unroll
+  for (int e = 0; e < 32; e += 4) {
+    const float4 l4 = *reinterpret_cast<const float4*>(lv + e);
+    const F2 a = f2_fma(f2_make(s[e], s[e + 1]), f2, f2_make(l4.x, l4.y));
+    const F2 b = f2_fma(f2_make(s[e + 2], s[e + 3]), f2, f2_make(l4.z, l4.w));
+    f2_split(a, t[e], t[e + 1]);
+    f2_split(b, t[e + 2], t[e + 3]);
+  }
+  if constexpr (MASK) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const int v = v0 + e;
+      if (!(v <= lim.hi && (v >= lim.lo || v < lim.vsk))) t[e] = -INFINITY;
+    }
+  }
+}
+
+template <bool MASK>
+__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, const float* lv,
+                                             float fac, int v0, const RowLim& lim, bool first,
+                                             uint64_t* pv_bar, int cnt, volatile int* abort,
+                                             float& m, float& l, bool& ok) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    float s[32], t[32];
+    tmem_ld32(s_addr + 32 * c, s);
+    row_t<MASK>(s, lv + 32 * c, fac, v0 + 32 * c, lim, t);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(t[e], t[e + 1]));
+  }
+  float a = 1.0f;
+  if (mx > m + 8.0f || (m == -INFINITY && mx != -INFINITY)) {
+    a = ex2_ftz(m - mx);
+    m = mx;
+    l *= a;
+  }
+  // The previous P V is in O.  Every tile waits here, whether it rescales or not: a wait by
+  // parity tells neighbouring completions apart, so none may be skipped.
+  if (cnt > 0) {
+    ok = wait_bar(pv_bar, (cnt - 1) & 1, abort);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) return;
+    tc_fence_after();
+  }
+  if (!first && __any_sync(0xffffffffu, a != 1.0f)) {
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+      float o[32];
+      tmem_ld32(o_addr + 32 * c, o);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] *= a;
+      tmem_st32(o_addr + 32 * c, o);
+    }
+  }
+  const float nb = m == -INFINITY ? 0.0f : -m;
+  const F2 nb2 = f2_make(nb, nb);
+  F2 ls0 = f2_make(0.0f, 0.0f), ls1 = ls0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    float s[32], t[32];
+    tmem_ld32(s_addr + 32 * c, s);
+    row_t<MASK>(s, lv + 32 * c, fac, v0 + 32 * c, lim, t);
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      const float4 r4 = *reinterpret_cast<const float4*>(lv + kBN + 32 * c + e);
+      float x0, x1, x2, x3;
+      f2_split(f2_add(f2_make(t[e], t[e + 1]), nb2), x0, x1);
+      f2_split(f2_add(f2_make(t[e + 2], t[e + 3]), nb2), x2, x3);
+      x0 = ex2_ftz(x0);
+      x1 = ex2_ftz(x1);
+      x2 = ex2_ftz(x2);
+      x3 = ex2_ftz(x3);
+      ls0 = f2_fma(f2_make(x0, x1), f2_make(r4.x, r4.y), ls0);
+      ls1 = f2_fma(f2_make(x2, x3), f2_make(r4.z, r4.w), ls1);
+      w[e / 2] = pack_h2(x0, x1);
+      w[e / 2 + 1] = pack_h2(x2, x3);
+    }
+    // P of keys 32 c .. over S columns 16 c .., which are read
+    tmem_st16(s_addr + 16 * c, w);
+  }
+  float x0, x1;
+  f2_split(f2_add(ls0, ls1), x0, x1);
+  l += x0 + x1;
+  tmem_wait_st();
+}
+
+// ---------------------------------------------------------------- the kernel
+template <int NM, bool LO, bool STREAM>
+__global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const Params p) {
+  using C = Cfg<NM, LO>;
+  constexpr int MT = 128 * NM;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* lvb = reinterpret_cast<float*>(smem + C::kOffLv);
+  float* facb = reinterpret_cast<float*>(smem + C::kOffFac);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = q_full + C::kQBuf;
+  uint64_t* k_full = q_empty + C::kQBuf;
+  uint64_t* k_empty = k_full + kStages;
+  uint64_t* v_full = k_empty + kStages;
+  uint64_t* v_empty = v_full + kStages;
+  uint64_t* lv_full = v_empty + kStages;
+  uint64_t* s_full = lv_full + kLvSlots;  // per S buffer
+  uint64_t* p_ready = s_full + 2;
+  uint64_t* pv_done = p_ready + 2;        // per row tile
+  uint64_t* o_empty = pv_done + NM;
+  uint64_t* drain = o_empty + NM;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+  int* cum = reinterpret_cast<int*>(smem + C::kOffCum);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int kMmaWarp = (C::kSoft + kConvThreads) / 32;
+  // combine_kernel's blocks may be scheduled; they wait for this grid
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (lane == 0) {
+      *abort = 0;
+      for (int i = 0; i < C::kQBuf; ++i) {
+        mbar_init(&q_full[i], kConvThreads / 32);
+        mbar_init(&q_empty[i], 1 + C::kSoft / 32);  // the products' commit, each softmax warp
+      }
+      for (int i = 0; i < kStages; ++i) {
+        mbar_init(&k_full[i], kConvThreads / 32);
+        mbar_init(&k_empty[i], 1);
+        mbar_init(&v_full[i], kConvThreads / 32);
+        mbar_init(&v_empty[i], 1);
+      }
+      for (int i = 0; i < kLvSlots; ++i) mbar_init(&lv_full[i], kConvThreads / 32);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_ready[i], 4);
+      }
+      for (int i = 0; i < NM; ++i) {
+        mbar_init(&pv_done[i], 1);
+        mbar_init(&o_empty[i], 4);
+      }
+      mbar_init(drain, 1);
+      fence_mbar_init();
+    }
+  }
+  if constexpr (STREAM) {  // cum[e]: first tile of entry e in the line of all tiles
+    const int ne = p.seg[0].nb + (p.nseg > 1 ? p.seg[1].nb : 0);
+    for (int e = tid; e < ne; e += C::kThreads) {
+      const int si = e < p.seg[0].nb ? 0 : 1;
+      cum[e + 1] = entry_tiles(p, e) * p.Hkv * row_tiles(p.seg[si].units * p.nrep, MT);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      int run = 0;
+      if (lane == 0) cum[0] = 0;
+      for (int e0 = 0; e0 < ne; e0 += 32) {
+        int x = e0 + lane < ne ? cum[e0 + lane + 1] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        if (e0 + lane < ne) cum[e0 + lane + 1] = run + x;
+        run += __shfl_sync(0xffffffffu, x, 31);
+      }
+      __syncwarp();
+      if (blockIdx.x == 0)
+        for (int e = lane; e <= ne; e += 32) p.cum[e] = cum[e];
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t q_base = smem_u32(smem), k_base = smem_u32(smem + C::kOffK),
+                 v_base = smem_u32(smem + C::kOffV);
+  Walk<MT, STREAM> walk;
+  walk.start(p, cum);
+  Piece w;
+
+  if (warp < C::kSoft / 32) {
+    // ================= softmax: one thread per row
+    const int mt = warp >> 2, r = tid;  // row of the piece
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t o_addr = tmem + kColO + 128 * mt + lane_base;
+    int pc = 0, gt = 0, cnt = 0;        // pieces, tiles of the block, tiles of this row tile
+    bool ok = true;
+    for (; ok && walk.next(p, cum, w); ++pc) {
+      const int n_tiles = w.t1 - w.t0;
+      const int qb = pc % C::kQBuf;
+      float m = -INFINITY, l = 0.0f, fac = 0.0f;
+      if (n_tiles > 0) {
+        ok = wait_bar(&q_full[qb], (pc / C::kQBuf) & 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (r < w.rows) fac = facb[qb * MT + r];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_empty[qb]);
+      }
+      if (w.rows <= 128 * mt) {         // nothing for this row tile
+        gt += n_tiles;
+        continue;
+      }
+      const Seg& s = p.seg[w.seg];
+      const bool live = r < w.rows;
+      const bool warp_live = 32 * warp < w.rows;
+      const int u = (w.row0 + r) / p.nrep;
+      const int pos = w.key.pos0 + (s.step ? u : 0);
+      const RowLim lim = {live ? pos - w.key.sh : 1 << 30,
+                          live ? pos - s.window + 1 - w.key.sh : 0,
+                          w.key.sh > 0 ? w.key.ns : s.sinks};
+      for (int t = w.t0; ok && t < w.t1; ++t, ++gt, ++cnt) {
+        const int buf = NM == 1 ? (cnt & 1) : mt;
+        const uint32_t par = NM == 1 ? ((cnt >> 1) & 1) : (cnt & 1);
+        const int slot = gt % kLvSlots;
+        ok = wait_bar(&lv_full[slot], (gt / kLvSlots) & 1, abort) &&
+             wait_bar(&s_full[buf], par, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (warp_live) {
+          const float* lv = lvb + slot * 2 * kBN;
+          const uint32_t s_addr = tmem + 128 * buf + lane_base;
+          const int v0 = t * kBN;
+          const bool need = v0 + kBN - 1 > lim.hi || (v0 < lim.lo && v0 + kBN > lim.vsk && lim.lo > lim.vsk);
+          if (__any_sync(0xffffffffu, need))
+            softmax_tile<true>(s_addr, o_addr, lv, fac, v0, lim, t == w.t0, &pv_done[mt], cnt,
+                               abort, m, l, ok);
+          else
+            softmax_tile<false>(s_addr, o_addr, lv, fac, v0, lim, t == w.t0, &pv_done[mt], cnt,
+                                abort, m, l, ok);
+        } else if (cnt > 0) {
+          ok = wait_bar(&pv_done[mt], (cnt - 1) & 1, abort);
+          ok = __all_sync(0xffffffffu, ok);
+        }
+        if (!ok) break;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[buf]);
+      }
+      if (!ok) break;
+      // ---- the rows' results
+      if (n_tiles > 0) {
+        ok = wait_bar(&pv_done[mt], (cnt - 1) & 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      if (warp_live) {
+        const bool have = live && l > 0.0f;
+        const int h = w.kvh * p.nrep + (w.row0 + r) % p.nrep;
+        char* dst = nullptr;
+        float* prt = nullptr;
+        float scale = 1.0f;
+        if (w.slot < 0) {
+          dst = out_row(p, w.b, u, h);
+          scale = have ? 1.0f / l : 0.0f;
+        } else {
+          prt = part_row(p, w.seg, w.slot, r);
+          if (live) {
+            prt[0] = have ? m : -INFINITY;
+            prt[1] = have ? l : 0.0f;
+          }
+        }
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          if (n_tiles > 0) {
+            tmem_ld32(o_addr + 32 * c, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+          }
+          if (!live) continue;
+          if (dst) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              store4(dst, p.q_dt, 32 * c + e, have ? o[e] * scale : 0.0f, have ? o[e + 1] * scale : 0.0f,
+                     have ? o[e + 2] * scale : 0.0f, have ? o[e + 3] * scale : 0.0f);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(prt + 4 + 32 * c + e) =
+                  have ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3])
+                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+        }
+      }
+      if (n_tiles > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[mt]);
+      }
+    }
+    if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
+  } else if (warp < kMmaWarp) {
+    // ================= codes -> float16 tiles, q -> q'
+    const int ct = tid - C::kSoft;
+    const int c16 = ct & 7, row = ct >> 3;  // 16 codes of rows row + 32 i
+    // where this thread's two 16-byte chunks go; the upper half of each 8 lanes stores its
+    // second chunk first, so that 8 lanes write 8 different chunk columns
+    const int first = c16 >> 2;
+    const uint32_t blk = static_cast<uint32_t>(c16 >> 2) * (kBN * 128);
+    const int ch = (2 * c16) & 7;
+    struct Buf {
+      uint4 k[4], v[4];
+      float vs[4];
+    } bufs[2];
+    // cursor of the loads
+    Walk<MT, STREAM> lw = walk;
+    Piece lp;
+    lp.t0 = lp.t1 = 0;
+    int lt = 0;
+    const int8_t *kp = nullptr, *vp = nullptr;
+    int64_t vs0 = 0;
+    auto advance = [&]() -> bool {  // to the next tile to load
+      if (++lt < lp.t1) return true;
+      do {
+        if (!lw.next(p, cum, lp)) return false;
+      } while (lp.t0 >= lp.t1);
+      lt = lp.t0;
+      const Seg& s = p.seg[lp.seg];
+      const int64_t o = lp.b * s.sb + lp.kvh * s.sh + 16 * c16;
+      kp = s.k + o;
+      vp = s.v + o;
+      vs0 = lp.b * s.vscb + lp.kvh * s.vsch;
+      return true;
+    };
+    auto key_of = [&](int i, bool& in) -> int64_t {
+      const int v = lt * kBN + row + 32 * i;
+      in = v < lp.key.nv;
+      return v < lp.key.ns ? v : v + lp.key.sh;
+    };
+    auto load_k = [&](Buf& b) {
+      const Seg& s = p.seg[lp.seg];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        bool in;
+        const int64_t key = key_of(i, in);
+        b.k[i] = in ? ldg_stream(kp + key * s.ss) : make_uint4(0, 0, 0, 0);
+        b.vs[i] = in ? load_scale(s.vsc, vs0 + key * s.vscs, p.s_dt) : 0.0f;
+      }
+    };
+    auto load_v = [&](Buf& b) {
+      const Seg& s = p.seg[lp.seg];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        bool in;
+        const int64_t key = key_of(i, in);
+        b.v[i] = in ? ldg_stream(vp + key * s.ss) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto put = [&](unsigned char* tile, int rr, const uint4& x) {
+      uint4 a, b;
+      codes_to_h2(x.x, a.x, a.y);
+      codes_to_h2(x.y, a.z, a.w);
+      codes_to_h2(x.z, b.x, b.y);
+      codes_to_h2(x.w, b.z, b.w);
+      *reinterpret_cast<uint4*>(tile + blk + sw128(rr, ch + first)) = first ? b : a;
+      *reinterpret_cast<uint4*>(tile + blk + sw128(rr, ch + 1 - first)) = first ? a : b;
+    };
+    int pc = 0, gt = 0, ct0 = 0, ct1 = 0;  // pieces, tiles; tiles of the piece at hand
+    bool ok = true;
+    // q' of the rows of piece w into buffer pc % kQBuf
+    auto make_q = [&]() {
+      const int qb = pc % C::kQBuf;
+      if (pc >= C::kQBuf) ok = wait_bar(&q_empty[qb], ((pc / C::kQBuf) - 1) & 1, abort);
+      if (!ok) return;
+      const Seg& s = p.seg[w.seg];
+      const int l16 = ct & 15, rg = ct >> 4;
+      float ks[8];
+      const int64_t k0 = w.b * s.kscb + w.kvh * s.ksch;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        ks[e] = load_scale(s.ksc, k0 + (8 * l16 + e) * s.kscd, p.s_dt) * p.qk_scale;
+#pragma unroll 2
+      for (int r0 = 0; r0 < w.rows; r0 += kConvThreads / 16) {
+        const int r = r0 + rg;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < w.rows) {
+          const int u = (w.row0 + r) / p.nrep, h = w.kvh * p.nrep + (w.row0 + r) % p.nrep;
+          x = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) +
+                                              2 * (w.b * s.qsb + u * s.qsu + h * p.qsh + 8 * l16));
+        }
+        float f[8];
+        if (p.q_dt == HQ_DTYPE_BF16) Vec16<HQ_DTYPE_BF16>::unpack(x, f);
+        else Vec16<HQ_DTYPE_F16>::unpack(x, f);
+        if (p.q_quant) {  // per-token int8 fake quantization, rounded back to the model dtype
+          float am = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(f[e]));
+#pragma unroll
+          for (int o = 8; o >= 1; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+          const Quantizer qz = Quantizer::from_amax(am);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y = static_cast<float>(qz.code(f[e])) * qz.scale;
+            f[e] = p.q_dt == HQ_DTYPE_BF16 ? __bfloat162float(__float2bfloat16_rn(y))
+                                           : __half2float(__float2half_rn(y));
+          }
+        }
+        float am = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          f[e] *= ks[e];
+          am = fmaxf(am, fabsf(f[e]));
+        }
+#pragma unroll
+        for (int o = 8; o >= 1; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+        // 2^ex brings am to [2^13, 2^14)
+        const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am) >> 23) - 127), -100), 100);
+        const float mul = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
+        if (r >= w.rows) continue;
+        if (l16 == 0)
+          facb[qb * MT + r] = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = f[2 * e] * mul, b = f[2 * e + 1] * mul;
+          hi[e] = pack_h2(a, b);
+          if constexpr (LO) {
+            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+            lo[e] = pack_h2(a - g.x, b - g.y);
+          }
+        }
+        unsigned char* tile = smem + (qb * NM + (r >> 7)) * C::kParts * kTileB;
+        const uint32_t at = static_cast<uint32_t>(l16 >> 3) * (kBN * 128) + sw128(r & 127, l16 & 7);
+        *reinterpret_cast<uint4*>(tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (LO)
+          *reinterpret_cast<uint4*>(tile + kTileB + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[qb]);
+      ++pc;
+    };
+    // tile gt from b into shared memory; b then takes the next tile to load
+    auto step = [&](Buf& b, bool& have) {
+      if (ct0 >= ct1) {  // a new piece (pieces without tiles have no q)
+        do {
+          if (!walk.next(p, cum, w)) {
+            ok = false;
+            return;
+          }
+          if (w.t0 >= w.t1) ++pc;
+        } while (w.t0 >= w.t1);
+        ct0 = w.t0;
+        ct1 = w.t1;
+        make_q();
+        if (!ok) return;
+      }
+      ++ct0;
+      const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
+      if (use > 0) ok = wait_bar(&k_empty[st], (use - 1) & 1, abort);
+      if (!ok) return;
+      unsigned char* kt = smem + C::kOffK + st * kTileB;
+      unsigned char* vt = smem + C::kOffV + st * kTileB;
+      bool zero[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        put(kt, row + 32 * i, b.k[i]);
+        zero[i] = b.vs[i] < 8.6736174e-19f;  // 2^-60: such a token's values are zeros
+        if (c16 == 0) {
+          const float x = zero[i] ? 8.6736174e-19f : b.vs[i];
+          lvb[slot * 2 * kBN + row + 32 * i] = __log2f(x);
+          lvb[slot * 2 * kBN + kBN + row + 32 * i] = 1.0f / x;
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&k_full[st]);
+        mbar_arrive(&lv_full[slot]);
+      }
+      have = advance();
+      if (have) load_k(b);
+      if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1, abort);
+      if (!ok) return;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        put(vt, row + 32 * i, zero[i] ? make_uint4(0, 0, 0, 0) : b.v[i]);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[st]);
+      if (have) load_v(b);
+      ++gt;
+    };
+    lt = -1;
+    bool have[2];
+    have[0] = advance();
+    if (have[0]) {
+      load_k(bufs[0]);
+      load_v(bufs[0]);
+    }
+    have[1] = have[0] && advance();
+    if (have[1]) {
+      load_k(bufs[1]);
+      load_v(bufs[1]);
+    }
+    while (ok && have[0]) {
+      step(bufs[0], have[0]);
+      if (!ok || !have[1]) break;
+      step(bufs[1], have[1]);
+    }
+    if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
+  } else {
+    // ================= tensor-core products, issued by one thread
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc<HQ_DTYPE_F16>(128, 128, false);
+      constexpr uint32_t id_o = idesc<HQ_DTYPE_F16>(128, 128, true);
+      bool ok = true;
+      int cntq[NM], cntp[NM], pieces[NM];  // S products, P V products, pieces of each row tile
+      for (int i = 0; i < NM; ++i) cntq[i] = cntp[i] = pieces[i] = 0;
+      // S = Q K^T of tile g for row tile m
+      auto qk = [&](int m, int qb, int g) {
+        const uint32_t buf = NM == 1 ? (cntq[m] & 1) : m;
+        const uint32_t ka = k_base + (g % kStages) * kTileB;
+        const uint32_t qa = q_base + (qb * NM + m) * C::kParts * kTileB;
+#pragma unroll
+        for (int part = 0; part < C::kParts; ++part)
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t off = (kk >> 2) * (kBN * 128) + (kk & 3) * 32;
+            mma_f16(tmem + 128 * buf, sdesc(qa + part * kTileB + off, 16, 1024),
+                    sdesc(ka + off, 16, 1024), id_s, part + kk > 0);
+          }
+        mma_commit(&s_full[buf]);
+        ++cntq[m];
+      };
+      auto pv = [&](int m, int g, bool first) {
+        const uint32_t buf = NM == 1 ? (cntp[m] & 1) : m;
+        const uint32_t par = NM == 1 ? ((cntp[m] >> 1) & 1) : (cntp[m] & 1);
+        ok = ok && wait_bar(&p_ready[buf], par, abort);
+        if (first && pieces[m] > 0) ok = ok && wait_bar(&o_empty[m], (pieces[m] - 1) & 1, abort);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t va = v_base + (g % kStages) * kTileB;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          mma_f16_ts(tmem + kColO + 128 * m, tmem + 128 * buf + 8 * kk,
+                     sdesc(va + kk * 16 * 128, kBN * 128, 1024), id_o, !first || kk > 0);
+        mma_commit(&pv_done[m]);
+        ++cntp[m];
+        if (first) ++pieces[m];
+      };
+      // cursor of the S products, one tile ahead of the P V products
+      Walk<MT, STREAM> qw = walk;
+      Piece qp, cp;
+      int qpc = -1, qt = 0, qg = 0;
+      qp.t0 = qp.t1 = 0;
+      bool more = true;
+      auto q_next = [&]() {  // qp, qt: the next tile's piece and index; waits for its q and K
+        if (++qt >= qp.t1) {
+          do {
+            if (!qw.next(p, cum, qp)) {
+              more = false;
+              return;
+            }
+            ++qpc;
+          } while (qp.t0 >= qp.t1);
+          qt = qp.t0;
+          ok = ok && wait_bar(&q_full[qpc % C::kQBuf], (qpc / C::kQBuf) & 1, abort);
+        }
+        ok = ok && wait_bar(&k_full[qg % kStages], (qg / kStages) & 1, abort);
+        tc_fence_after();
+      };
+      auto q_done = [&]() {  // after the last S product of the tile
+        mma_commit(&k_empty[qg % kStages]);
+        if (qt == qp.t1 - 1) mma_commit(&q_empty[qpc % C::kQBuf]);
+        ++qg;
+      };
+      qt = -1;
+      q_next();
+      if (ok && more) {
+        for (int m = 0; m < NM; ++m)
+          if (qp.rows > 128 * m) qk(m, qpc % C::kQBuf, qg);
+        q_done();
+      }
+      int g = 0;  // tile of the P V products
+      while (ok && more) {
+        cp = qp;
+        const int ctile = qt;
+        q_next();
+        if (!ok) break;
+        if (NM == 1 && more) {
+          qk(0, qpc % C::kQBuf, qg);
+          q_done();
+        }
+        ok = wait_bar(&v_full[g % kStages], (g / kStages) & 1, abort);
+        if (!ok) break;
+        for (int m = 0; m < NM; ++m) {
+          if (cp.rows > 128 * m) pv(m, g, ctile == cp.t0);
+          if (!ok) break;
+          // the next S of this row tile overwrites the P just read: the products run in order
+          if (NM > 1 && more && qp.rows > 128 * m) qk(m, qpc % C::kQBuf, qg);
+        }
+        if (!ok) break;
+        mma_commit(&v_empty[g % kStages]);
+        if (NM > 1 && more) q_done();
+        ++g;
+      }
+      if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
+      // every product has completed before the tensor memory is released
+      mma_commit(drain);
+      if (!mbar_wait(drain, 0)) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols)
+                 : "memory");
+  }
+}
+
+// ---------------------------------------------------------------- joining the pieces
+// One warp per output row (b, u, h), 4 channels per lane: the pieces' common maximum, then
+// their weighted sums.  STREAM: the blocks that hold tiles T0 .. T1 - 1 of a unit are
+// T0 / per .. (T1 - 1) / per, and their pieces have consecutive slots.
+template <int MT, bool STREAM>
+__global__ void __launch_bounds__(256) combine_kernel(const Params p, int rows, int units, int grid_x) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int Hq = p.Hkv * p.nrep;
+  const int h = row % Hq, u = (row / Hq) % units, b = row / (Hq * units);
+  const int kvh = h / p.nrep, hr = h - kvh * p.nrep;
+  const float* src[2];
+  int n[2] = {0, 0};
+  int64_t stride[2] = {0, 0};
+  if constexpr (STREAM) {
+    const int ne = p.seg[0].nb + (p.nseg > 1 ? p.seg[1].nb : 0);
+    const int per = max(p.min_tiles, (p.cum[ne] + grid_x - 1) / grid_x);
+    for (int si = 0; si < p.nseg; ++si) {
+      const Seg& s = p.seg[si];
+      // with two segments, the first is shared by the s.units sequences of a group
+      const int eb = p.nseg > 1 && si == 0 ? b / s.units : b;
+      const int r_all = (p.nseg > 1 && si == 0 ? (b % s.units) : u) * p.nrep + hr;
+      const int e = eb + (si ? p.seg[0].nb : 0);
+      const int rt = r_all / MT, n_rt = row_tiles(s.units * p.nrep, MT);
+      const int idx = rt * p.Hkv + kvh;
+      const int nt = (p.cum[e + 1] - p.cum[e]) / (p.Hkv * n_rt);
+      if (nt == 0) continue;
+      const int T0 = p.cum[e] + idx * nt, c0 = T0 / per, c1 = (T0 + nt - 1) / per;
+      if (!p.merge_all && c0 == c1) return;  // written by the block that held all of it
+      src[si] = part_row(p, si, eb * p.Hkv * n_rt + idx + c0, r_all - rt * MT);
+      n[si] = c1 - c0 + 1;
+      stride[si] = static_cast<int64_t>(p.rows_cap[si]) * kPartRow;
+    }
+  } else {
+    const Seg& s = p.seg[0];
+    const int nq = p.q_lens ? min(max(p.q_lens[b], 0), s.units) : s.units;
+    if (u >= nq) return;
+    const int r = u * p.nrep + hr, rt = r / MT;
+    src[0] = part_row(p, 0, ((b * p.Hkv + kvh) * p.n_rt + rt) * p.n_split, r - rt * MT);
+    n[0] = p.n_split;
+    stride[0] = static_cast<int64_t>(p.rows_cap[0]) * kPartRow;
+  }
+  float M = -INFINITY;
+  for (int k = 0; k < 2; ++k)
+    for (int i = lane; i < n[k]; i += 32) M = fmaxf(M, src[k][i * stride[k]]);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float L = 0.0f;
+  if (M != -INFINITY) {
+    for (int k = 0; k < 2; ++k)
+#pragma unroll 4
+      for (int i = 0; i < n[k]; ++i) {
+        const float* x = src[k] + i * stride[k];
+        const float2 ml = *reinterpret_cast<const float2*>(x);
+        const float4 o = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
+        const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+        L += f * ml.y;
+        acc.x += f * o.x;
+        acc.y += f * o.y;
+        acc.z += f * o.z;
+        acc.w += f * o.w;
+      }
+  }
+  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  store4(out_row(p, b, u, h), p.q_dt, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+}
+
+// ---------------------------------------------------------------- host side
+inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+inline bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Row tiles per block: two for more than 128 rows; float16 models (q' in two parts, whose
+// second tile takes the shared memory of a second row tile) always one.
+inline int tiles_of(int q_dt, int rows) { return q_dt == HQ_DTYPE_F16 || rows <= 128 ? 1 : 2; }
+
+struct Plan {
+  int nm, n_rt, n_split, grid;
+  int rows_cap[2];
+  int64_t part_floats[2];
+  size_t cum_bytes;
+  int64_t units[2];
+  size_t bytes() const {
+    return cum_bytes + align256(sizeof(float) * static_cast<size_t>(part_floats[0] + part_floats[1]));
+  }
+};
+
+// STREAM plan: rows0 / rows1 rows per entry of the two segments (nb1 == 0: one segment).
+inline bool plan_stream(Plan& pl, int q_dt, int Hkv, int nb0, int64_t rows0, int cap0, int nb1,
+                        int64_t rows1, int cap1) {
+  const int64_t rmax = std::max(rows0, rows1);
+  pl = Plan{};
+  pl.nm = tiles_of(q_dt, static_cast<int>(std::min<int64_t>(rmax, 1 << 20)));
+  const int MT = 128 * pl.nm;
+  const int64_t u0 = int64_t(nb0) * Hkv * ((rows0 + MT - 1) / MT);
+  const int64_t u1 = int64_t(nb1) * Hkv * ((rows1 + MT - 1) / MT);
+  const int64_t tiles = u0 * std::max(1, cap0 / kBN + 1) + u1 * std::max(1, cap1 / kBN + 1);
+  if (tiles > (int64_t(1) << 30) || nb0 + nb1 > kMaxEntries) return false;
+  pl.units[0] = u0;
+  pl.units[1] = u1;
+  pl.grid = static_cast<int>(std::min<int64_t>(current_sm_count(), std::max<int64_t>(tiles, 1)));
+  pl.rows_cap[0] = static_cast<int>(std::min<int64_t>(rows0, MT));
+  pl.rows_cap[1] = static_cast<int>(std::min<int64_t>(rows1, MT));
+  pl.part_floats[0] = (u0 + pl.grid) * pl.rows_cap[0] * kPartRow;
+  pl.part_floats[1] = nb1 ? (u1 + pl.grid) * pl.rows_cap[1] * kPartRow : 0;
+  pl.cum_bytes = align256(sizeof(int) * (nb0 + nb1 + 1));
+  return true;
+}
+
+// Prefill plan: one block per row tile; with fewer blocks than SMs the keys of each row
+// tile are split, down to two key tiles per block.
+inline bool plan_prefill(Plan& pl, int q_dt, int B, int Hkv, int nrep, int Sq, int cap, int window,
+                         int sinks) {
+  pl = Plan{};
+  const int64_t rows = int64_t(Sq) * nrep;
+  if (rows > (1 << 30)) return false;
+  pl.nm = tiles_of(q_dt, static_cast<int>(std::min<int64_t>(rows, 1 << 20)));
+  // small grids keep one row tile per block
+  if (pl.nm == 2 && int64_t(B) * Hkv * ((rows + 255) / 256) < current_sm_count()) pl.nm = 1;
+  const int MT = 128 * pl.nm;
+  pl.n_rt = static_cast<int>((rows + MT - 1) / MT);
+  const int64_t units = int64_t(B) * Hkv * pl.n_rt;
+  if (units * 64 > (int64_t(1) << 31) - 1 || int64_t(Hkv) * pl.n_rt > 65535) return false;
+  const int64_t seen = std::min<int64_t>(cap, int64_t(window) + sinks + MT / nrep + 1);
+  const int64_t nt = std::max<int64_t>(1, (seen + kBN - 1) / kBN);
+  const int sms = current_sm_count();
+  pl.n_split = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, sms / std::max<int64_t>(units, 1)),
+                                                   std::max<int64_t>(1, nt / 2), 16}));
+  pl.rows_cap[0] = static_cast<int>(std::min<int64_t>(rows, MT));
+  pl.part_floats[0] = pl.n_split > 1 ? units * pl.n_split * pl.rows_cap[0] * kPartRow : 0;
+  return true;
+}
+
+template <typename K>
+int set_smem(K kern, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = (dev >= 0 && dev < 64) ? (uint64_t(1) << dev) : 0;
+  if (!bit || !(ready.load(std::memory_order_acquire) & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    ready.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  return HQ_OK;
+}
+
+template <int NM, bool LO, bool STREAM>
+int launch(const Params& p, dim3 grid, int entries, int out_rows, int units, bool combine,
+           cudaStream_t st) {
+  using C = Cfg<NM, LO>;
+  static std::atomic<uint64_t> ready{0};
+  auto kern = ragged_kernel<NM, LO, STREAM>;
+  const int rc = set_smem(kern, C::smem(STREAM ? kMaxEntries : 0), ready);
+  if (rc != HQ_OK) return rc;
+  kern<<<grid, C::kThreads, C::smem(STREAM ? entries : 0), st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (!combine) return HQ_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((out_rows + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, combine_kernel<128 * NM, STREAM>, p, out_rows, units,
+                         static_cast<int>(grid.x));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return static_cast<int>(e);
+  }
+  return HQ_OK;
+}
+
+template <bool STREAM>
+int dispatch(const Params& p, int nm, dim3 grid, int entries, int out_rows, int units, bool combine,
+             cudaStream_t st) {
+  if (p.q_dt == HQ_DTYPE_F16) return launch<1, true, STREAM>(p, grid, entries, out_rows, units, combine, st);
+  if (nm == 1) return launch<1, false, STREAM>(p, grid, entries, out_rows, units, combine, st);
+  return launch<2, false, STREAM>(p, grid, entries, out_rows, units, combine, st);
+}
+
+inline int fill_seg(Seg& s, const int8_t* k, const int8_t* v, const int64_t* kvs, const void* ksc,
+                    const void* vsc, const int64_t* kss, const int64_t* vss, const int* lens,
+                    int cap, int nb, int units, int window, int sinks) {
+  if (cap > 0 && (!k || !v || !ksc || !vsc)) return HQ_ERR_INVALID_ARGUMENT;
+  if (!kvs || !kss || !vss || cap < 0 || nb < 0 || units < 0 || window < 0 || sinks < 0)
+    return HQ_ERR_INVALID_ARGUMENT;
+  if (!aligned(k, 16) || !aligned(v, 16) || kvs[0] % 16 || kvs[1] % 16 || kvs[2] % 16)
+    return HQ_ERR_INVALID_ARGUMENT;
+  s.k = k;
+  s.v = v;
+  s.sb = kvs[0];
+  s.sh = kvs[1];
+  s.ss = kvs[2];
+  s.ksc = ksc;
+  s.vsc = vsc;
+  s.kscb = kss[0];
+  s.ksch = kss[1];
+  s.kscd = kss[2];
+  s.vscb = vss[0];
+  s.vsch = vss[1];
+  s.vscs = vss[2];
+  s.lens = lens;
+  s.cap = cap;
+  s.nb = nb;
+  s.units = units;
+  s.window = window > 0 ? window : 1 << 30;
+  s.sinks = sinks;
+  return HQ_OK;
+}
+
+inline int check_common(const void* q, int q_dtype, const int64_t* qs, int nqs, const void* out,
+                        const int64_t* os, int scale_dtype, int Hq, int Hkv, int D) {
+  if (!q || !out || !qs || !os || Hq <= 0 || Hkv <= 0) return HQ_ERR_INVALID_ARGUMENT;
+  if (D != kD || Hq % Hkv || Hq / Hkv > 128 || Hq > 65535 ||
+      (q_dtype != HQ_DTYPE_BF16 && q_dtype != HQ_DTYPE_F16) ||
+      (scale_dtype != HQ_DTYPE_F32 && scale_dtype != HQ_DTYPE_F16))
+    return HQ_ERR_UNSUPPORTED;
+  if (qs[nqs - 1] != 1 || os[nqs - 1] != 1 || !aligned(q, 16) || !aligned(out, 8))
+    return HQ_ERR_INVALID_ARGUMENT;
+  for (int i = 0; i + 1 < nqs; ++i)
+    if (qs[i] % 8 || os[i] % 4) return HQ_ERR_INVALID_ARGUMENT;
+  return HQ_OK;
+}
+
+inline int attach(Params& p, const Plan& pl, void* ws, size_t ws_bytes) {
+  if (pl.bytes() > 0 && (!ws || ws_bytes < pl.bytes() || !aligned(ws, 256))) return HQ_ERR_WORKSPACE;
+  p.cum = static_cast<int*>(ws);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.cum_bytes);
+  p.part1 = pl.part_floats[0];
+  p.rows_cap[0] = pl.rows_cap[0];
+  p.rows_cap[1] = pl.rows_cap[1];
+  p.n_split = pl.n_split;
+  p.n_rt = pl.n_rt;
+  return HQ_OK;
+}
+
+}  // namespace rag
+}  // namespace hq
+
+using namespace hq;
+
+extern "C" size_t hq_window_workspace_bytes(int q_dtype, int B, int Hq, int Hkv, int Sq, int S_max,
+                                            int D, int window, int sinks) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq < 0 || S_max < 0 || window < 0 || sinks < 0 ||
+      D != rag::kD || Hq % Hkv)
+    return 0;
+  rag::Plan pl;
+  const bool ok = Sq == 0 ? rag::plan_stream(pl, q_dtype, Hkv, B, Hq / Hkv, S_max, 0, 0, 0)
+                          : rag::plan_prefill(pl, q_dtype, B, Hkv, Hq / Hkv, Sq, S_max,
+                                              window > 0 ? window : 1 << 30, sinks);
+  return ok ? std::max<size_t>(pl.bytes(), 256) : 0;
+}
+
+extern "C" int hq_window_decode_int8(const void* q, int q_dtype, const int64_t q_strides[3],
+                                     const int8_t* k, const int8_t* v, const int64_t kv_strides[3],
+                                     const void* k_scale, const void* v_scale, int scale_dtype,
+                                     const int64_t ksc_strides[3], const int64_t vsc_strides[3],
+                                     const int* lens, int B, int Hq, int Hkv, int S_max, int D,
+                                     int window, int sinks, float sm_scale, int q_quant, void* out,
+                                     const int64_t out_strides[3], void* workspace,
+                                     size_t workspace_bytes, int* status, hq_stream_t stream) {
+  int rc = rag::check_common(q, q_dtype, q_strides, 3, out, out_strides, scale_dtype, Hq, Hkv, D);
+  if (rc != HQ_OK) return rc;
+  if (B < 0) return HQ_ERR_INVALID_ARGUMENT;
+  rag::Params p{};
+  rc = rag::fill_seg(p.seg[0], k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
+                     S_max, B, 1, window, sinks);
+  if (rc != HQ_OK) return rc;
+  if (B == 0) return HQ_OK;
+  rag::Plan pl;
+  if (!rag::plan_stream(pl, q_dtype, Hkv, B, Hq / Hkv, S_max, 0, 0, 0)) return HQ_ERR_UNSUPPORTED;
+  rc = rag::attach(p, pl, workspace, workspace_bytes);
+  if (rc != HQ_OK) return rc;
+  p.nseg = 1;
+  p.seg[0].qsb = q_strides[0];
+  p.q = q;
+  p.qsh = q_strides[1];
+  p.q_dt = q_dtype;
+  p.s_dt = scale_dtype;
+  p.Hkv = Hkv;
+  p.nrep = Hq / Hkv;
+  p.qk_scale = sm_scale * rag::kLog2e;
+  p.q_quant = q_quant;
+  p.out = out;
+  p.osb = out_strides[0];
+  p.osh = out_strides[1];
+  p.status = status;
+  p.min_tiles = 1;
+  return rag::dispatch<true>(p, pl.nm, dim3(pl.grid), B, B * Hq, 1, true,
+                             reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int hq_window_prefill_int8(const void* q, int q_dtype, const int64_t q_strides[4],
+                                      const int8_t* k, const int8_t* v, const int64_t kv_strides[3],
+                                      const void* k_scale, const void* v_scale, int scale_dtype,
+                                      const int64_t ksc_strides[3], const int64_t vsc_strides[3],
+                                      const int* lens, const int* q_lens, int B, int Hq, int Hkv,
+                                      int Sq, int S_max, int D, int window, int sinks,
+                                      float sm_scale, int q_quant, void* out,
+                                      const int64_t out_strides[4], void* workspace,
+                                      size_t workspace_bytes, int* status, hq_stream_t stream) {
+  int rc = rag::check_common(q, q_dtype, q_strides, 4, out, out_strides, scale_dtype, Hq, Hkv, D);
+  if (rc != HQ_OK) return rc;
+  if (B < 0 || Sq < 0) return HQ_ERR_INVALID_ARGUMENT;
+  if (B > 65535) return HQ_ERR_UNSUPPORTED;
+  rag::Params p{};
+  rc = rag::fill_seg(p.seg[0], k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
+                     S_max, B, Sq, window, sinks);
+  if (rc != HQ_OK) return rc;
+  if (B == 0 || Sq == 0) return HQ_OK;
+  rag::Plan pl;
+  if (!rag::plan_prefill(pl, q_dtype, B, Hkv, Hq / Hkv, Sq, S_max, p.seg[0].window, sinks))
+    return HQ_ERR_UNSUPPORTED;
+  rc = rag::attach(p, pl, workspace, workspace_bytes);
+  if (rc != HQ_OK) return rc;
+  p.nseg = 1;
+  p.seg[0].step = 1;
+  p.seg[0].qsb = q_strides[0];
+  p.seg[0].qsu = q_strides[2];
+  p.q = q;
+  p.qsh = q_strides[1];
+  p.q_dt = q_dtype;
+  p.s_dt = scale_dtype;
+  p.Hkv = Hkv;
+  p.nrep = Hq / Hkv;
+  p.qk_scale = sm_scale * rag::kLog2e;
+  p.q_quant = q_quant;
+  p.q_lens = q_lens;
+  p.out = out;
+  p.osb = out_strides[0];
+  p.osh = out_strides[1];
+  p.osu = out_strides[2];
+  p.status = status;
+  return rag::dispatch<false>(p, pl.nm, dim3(pl.n_split, Hkv * pl.n_rt, B), 0, B * Sq * Hq, Sq,
+                              pl.n_split > 1, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t hq_prefix_decode_workspace_bytes(int q_dtype, int G, int B, int Hq, int Hkv,
+                                                   int P_max, int S_max, int D) {
+  if (G <= 0 || B <= 0 || B % G || Hq <= 0 || Hkv <= 0 || Hq % Hkv || P_max < 0 || S_max < 0 ||
+      D != rag::kD)
+    return 0;
+  rag::Plan pl;
+  const int nrep = Hq / Hkv;
+  if (!rag::plan_stream(pl, q_dtype, Hkv, G, int64_t(B / G) * nrep, P_max, B, nrep, S_max)) return 0;
+  return std::max<size_t>(pl.bytes(), 256);
+}
+
+extern "C" int hq_prefix_decode_int8(
+    const void* q, int q_dtype, const int64_t q_strides[3], const int8_t* pk, const int8_t* pv,
+    const int64_t pkv_strides[3], const void* pk_scale, const void* pv_scale,
+    const int64_t pksc_strides[3], const int64_t pvsc_strides[3], const int* prefix_lens, int G,
+    int P_max, const int8_t* k, const int8_t* v, const int64_t kv_strides[3], const void* k_scale,
+    const void* v_scale, const int64_t ksc_strides[3], const int64_t vsc_strides[3],
+    const int* lens, int S_max, int scale_dtype, int B, int Hq, int Hkv, int D, float sm_scale,
+    int q_quant, void* out, const int64_t out_strides[3], void* workspace, size_t workspace_bytes,
+    int* status, hq_stream_t stream) {
+  int rc = rag::check_common(q, q_dtype, q_strides, 3, out, out_strides, scale_dtype, Hq, Hkv, D);
+  if (rc != HQ_OK) return rc;
+  if (B < 0 || G <= 0 || B % G) return HQ_ERR_INVALID_ARGUMENT;
+  rag::Params p{};
+  rc = rag::fill_seg(p.seg[0], pk, pv, pkv_strides, pk_scale, pv_scale, pksc_strides, pvsc_strides,
+                     prefix_lens, P_max, G, B / G, 0, 0);
+  if (rc == HQ_OK)
+    rc = rag::fill_seg(p.seg[1], k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
+                       S_max, B, 1, 0, 0);
+  if (rc != HQ_OK) return rc;
+  if (B == 0) return HQ_OK;
+  const int nrep = Hq / Hkv;
+  rag::Plan pl;
+  if (!rag::plan_stream(pl, q_dtype, Hkv, G, int64_t(B / G) * nrep, P_max, B, nrep, S_max))
+    return HQ_ERR_UNSUPPORTED;
+  rc = rag::attach(p, pl, workspace, workspace_bytes);
+  if (rc != HQ_OK) return rc;
+  p.nseg = 2;
+  p.seg[0].qsb = q_strides[0] * (B / G);
+  p.seg[0].qsu = q_strides[0];
+  p.seg[1].qsb = q_strides[0];
+  p.q = q;
+  p.qsh = q_strides[1];
+  p.q_dt = q_dtype;
+  p.s_dt = scale_dtype;
+  p.Hkv = Hkv;
+  p.nrep = nrep;
+  p.qk_scale = sm_scale * rag::kLog2e;
+  p.q_quant = q_quant;
+  p.out = out;
+  p.osb = out_strides[0];
+  p.osh = out_strides[1];
+  p.status = status;
+  p.min_tiles = 1;
+  p.merge_all = 1;
+  return rag::dispatch<true>(p, pl.nm, dim3(pl.grid), G + B, B * Hq, 1, true,
+                             reinterpret_cast<cudaStream_t>(stream));
+}

@@ -16,6 +16,7 @@ stream of the input's device and raises on bad input; there is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 import threading
 
@@ -737,6 +738,7 @@ def set_plan_sms(sms: int, device=None) -> None:
     dev = torch.cuda.current_device() if device is None else torch.device(device).index
     check(_lib.lib().hq_set_plan_sms(int(dev), int(sms)), "hq_set_plan_sms")
     _decode_ws_bytes.clear()
+    _ragged_ws_bytes.clear()
 
 
 # ---------------------------------------------------------------- block-wise per-channel K
@@ -910,3 +912,382 @@ def kblock_dequant(cache: dict, S: int, dtype: torch.dtype = torch.float32) -> t
         _stream(kc.device))
     check(rc, "hq_kblock_dequant")
     return out
+
+
+# ---------------------------------------------------------------- ragged batches
+_ragged_status: dict = {}   # device index -> int32 [1] (first error sticks)
+_ragged_ws_bytes: dict = {}
+
+
+def _status_word(dev: torch.device) -> torch.Tensor:
+    """The status word the ragged-batch kernels of ``dev`` report into."""
+    t = _ragged_status.get(dev.index)
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first ragged-batch call on a device must run outside a CUDA "
+                               "graph capture: run the same call once before capturing it")
+        t = _ragged_status[dev.index] = torch.zeros(1, dtype=torch.int32, device=dev)
+    return t
+
+
+def ragged_status(device=None) -> int:
+    """Status of the ragged-batch kernels (``int8_window_decode_attn``,
+    ``int8_window_prefill_attn``, ``int8_prefix_decode_attn``, ``rope_append_kv``) on a device
+    since it was last reset: 0, or the first error found on the device (a wait that gave up, a
+    sequence whose new tokens did not fit).  Synchronises."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    t = _ragged_status.get(dev.index if dev.index is not None else torch.cuda.current_device())
+    return int(t.item()) if t is not None else 0
+
+
+def reset_ragged_status(device=None) -> None:
+    """Clears the word ``ragged_status`` reads (on the current stream)."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    t = _ragged_status.get(dev.index if dev.index is not None else torch.cuda.current_device())
+    if t is not None:
+        t.zero_()
+
+
+def _on_device(dev: torch.device):
+    """Makes ``dev`` the current device for a launch, where it is not already."""
+    if torch.cuda.current_device() == dev.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _lens_ptr(what: str, name: str, t: torch.Tensor | None, n: int, dev: torch.device):
+    if t is None:
+        return None
+    _cuda(t, f"{what} {name}")
+    if t.dtype != torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{what}: {name} must be a contiguous int32 tensor of {n} elements on q's "
+                         f"device, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _int8_cache(what: str, B: int, D: int, dev, k, k_sc, v, v_sc, scale_dtype=None):
+    """Checks an int8 cache (``[B,Hkv,S,D]`` codes sharing strides, K scales ``[B,Hkv,1,D]``, V
+    scales ``[B,Hkv,S,1]``) and returns the C arguments that describe it."""
+    for t, n in ((k, "k"), (k_sc, "k_sc"), (v, "v"), (v_sc, "v_sc")):
+        _cuda(t, f"{what} {n}")
+        if t.device != dev:
+            raise ValueError(f"{what}: {n} is on {t.device}, q on {dev}")
+    if k.dim() != 4 or v.dim() != 4 or k_sc.dim() != 4 or v_sc.dim() != 4:
+        raise ValueError(f"{what}: the cache must be 4-d: codes [B,Hkv,S,D], scales [B,Hkv,1,D] and "
+                         "[B,Hkv,S,1]")
+    if k.dtype != torch.int8 or v.dtype != torch.int8:
+        raise TypeError(f"{what}: K/V must be int8")
+    if k_sc.dtype != v_sc.dtype or k_sc.dtype not in (torch.float16, torch.float32):
+        raise TypeError(f"{what}: scales must both be float16 or float32")
+    if scale_dtype is not None and k_sc.dtype != scale_dtype:
+        raise TypeError(f"{what}: the scales of both caches must have one dtype")
+    _check_cache_shapes(what, B, D, k, v, k_sc, v_sc)
+    kst, vst = k.stride(), v.stride()
+    if kst != vst:
+        raise ValueError(f"{what}: K and V must share strides")
+    if k.numel() and (kst[3] != 1 or any(s % 16 for s in kst[:3])
+                      or k.data_ptr() % 16 or v.data_ptr() % 16):
+        raise ValueError(f"{what}: K/V rows must be contiguous and 16-byte aligned")
+    ks, vs = k_sc.stride(), v_sc.stride()
+    return (k.data_ptr(), v.data_ptr(), _lib.strides(kst[:3], 3), k_sc.data_ptr(), v_sc.data_ptr(),
+            _DT[k_sc.dtype], _lib.strides((ks[0], ks[1], ks[3]), 3),
+            _lib.strides((vs[0], vs[1], vs[2]), 3))
+
+
+def _q16(what: str, q: torch.Tensor) -> None:
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: q must be bfloat16 or float16")
+
+
+def _out_like(what: str, out, shape, q: torch.Tensor) -> None:
+    if tuple(out.shape) != tuple(shape) or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError(f"{what}: out must be {tuple(shape)} of q's dtype and device")
+    if out.stride(-1) != 1 or out.data_ptr() % 8 or any(s % 4 for s in out.stride()[:-1]):
+        raise ValueError(f"{what}: out rows must be contiguous and 8-byte aligned")
+
+
+def _window_args(what: str, window, sinks) -> tuple:
+    w = 0 if window is None else int(window)
+    if window is not None and w < 1 or w >= 1 << 30:
+        raise ValueError(f"{what}: window must be None or 1 .. 2^30 - 1")
+    if not 0 <= int(sinks) < 1 << 30:
+        raise ValueError(f"{what}: sinks must be 0 .. 2^30 - 1")
+    return w, int(sinks)
+
+
+def _scratch(key, query, dev) -> torch.Tensor:
+    """Scratch of one call: nothing lives in it from call to call, so each call takes its own
+    from the allocator (calls on other streams and captured graphs never share it)."""
+    nb = _ragged_ws_bytes.get(key)
+    if nb is None:
+        nb = query(*key[2:])
+        if nb == 0:
+            raise ValueError(f"{key[0]}: unsupported shape")
+        _ragged_ws_bytes[key] = nb
+    return torch.empty(nb, dtype=torch.uint8, device=dev)
+
+
+def int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sinks=0,
+                            sm_scale=None, q_quant=False, out=None):
+    """One decode step of a ragged batch over an int8 cache, under a sliding window with sink
+    tokens (``hq_window_decode_int8``).
+
+    q ``[B,Hq,1,D]`` or ``[B,Hq,D]`` (bf16/f16, D = 128); k_i8 / v_i8 capacity buffers
+    ``[B,Hkv,cap,D]``, k_sc ``[B,Hkv,1,D]``, v_sc ``[B,Hkv,cap,1]`` (f16/f32); ``lens`` int32
+    ``[B]`` on the device: the tokens each sequence holds, its newest being the query's own.
+    Sequence b sees token j < lens[b] when ``j >= lens[b] - window`` or ``j < sinks``
+    (``window=None``: every token).  Rows past ``lens[b]`` are never read; an empty sequence
+    gives zeros.  Returns the output in q's layout and dtype (or writes ``out [B,Hq,D]``).
+    ``q_quant``: the per-token fake quantization of ``int8_decode_attn``.  Nothing depends on
+    ``lens`` on the host, so the call replays in a CUDA graph while sequences grow.
+    """
+    what = "int8_window_decode_attn"
+    _cuda(q, f"{what} q")
+    qb, restore = _as_bhd(q)
+    _q16(what, qb)
+    qb = qb if _rows_ok(qb) else qb.contiguous()
+    B, Hq, D = qb.shape
+    dev = qb.device
+    cache = _int8_cache(what, B, D, dev, k_i8, k_sc, v_i8, v_sc)
+    Hkv, cap = k_i8.shape[1], k_i8.shape[2]
+    w, sinks = _window_args(what, window, sinks)
+    if lens is None:
+        raise ValueError(f"{what}: lens is needed")
+    lp = _lens_ptr(what, "lens", lens, B, dev)
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"{what}: {Hq} query heads over {Hkv} kv heads")
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(D)
+    if out is not None:
+        _out_like(what, out, (B, Hq, D), qb)
+    with _on_device(dev):
+        res = out if out is not None else torch.empty((B, Hq, D), dtype=qb.dtype, device=dev)
+        if B == 0:
+            return restore(res) if out is None else res
+        dt = _DT[qb.dtype]
+        ws = _scratch((what, dev.index, dt, B, Hq, Hkv, 0, cap, D, w, sinks),
+                      _lib.lib().hq_window_workspace_bytes, dev)
+        rc = _lib.lib().hq_window_decode_int8(
+            qb.data_ptr(), dt, _lib.strides(qb.stride(), 3), *cache, lp, B, Hq, Hkv, cap, D, w,
+            sinks, float(sm_scale), int(bool(q_quant)), res.data_ptr(),
+            _lib.strides(res.stride(), 3), ws.data_ptr(), ws.numel(), _status_word(dev).data_ptr(),
+            _stream(dev))
+    check(rc, "hq_window_decode_int8")
+    return restore(res) if out is None else res
+
+
+def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sinks=0,
+                             q_lens=None, sm_scale=None, q_quant=False, out=None):
+    """Causal attention of a chunk of new tokens per sequence over an int8 cache, under a
+    sliding window with sink tokens, for a ragged (right-padded) batch
+    (``hq_window_prefill_int8``).
+
+    q ``[B,Hq,Sq,D]`` (bf16/f16, D = 128), the cache as in ``int8_window_decode_attn``;
+    ``lens`` int32 ``[B]``: cached tokens, the chunk's own included; ``q_lens`` int32 ``[B]``
+    (default: Sq each): how many rows of q are queries of sequence b - query i stands at
+    position ``p = lens[b] - q_lens[b] + i`` and sees ``j <= p`` with ``j > p - window`` or
+    ``j < sinks``.  Returns ``[B,Sq,Hq,D]``; rows past ``q_lens[b]`` are zeros, or are left as
+    they were in ``out``.  Queries at a position below 0 give zeros.
+    """
+    what = "int8_window_prefill_attn"
+    _cuda(q, f"{what} q")
+    if q.dim() != 4:
+        raise ValueError(f"{what}: q must be [B,Hq,Sq,D]")
+    _q16(what, q)
+    q = q if _rows_ok(q) else q.contiguous()
+    B, Hq, Sq, D = q.shape
+    dev = q.device
+    cache = _int8_cache(what, B, D, dev, k_i8, k_sc, v_i8, v_sc)
+    Hkv, cap = k_i8.shape[1], k_i8.shape[2]
+    w, sinks = _window_args(what, window, sinks)
+    if lens is None:
+        raise ValueError(f"{what}: lens is needed")
+    lp, qlp = _lens_ptr(what, "lens", lens, B, dev), _lens_ptr(what, "q_lens", q_lens, B, dev)
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"{what}: {Hq} query heads over {Hkv} kv heads")
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(D)
+    if out is not None:
+        _out_like(what, out, (B, Sq, Hq, D), q)
+    with _on_device(dev):
+        if out is None:
+            make = torch.empty if q_lens is None else torch.zeros
+            out = make((B, Sq, Hq, D), dtype=q.dtype, device=dev)
+        if B == 0 or Sq == 0:
+            return out
+        dt = _DT[q.dtype]
+        ws = _scratch((what, dev.index, dt, B, Hq, Hkv, Sq, cap, D, w, sinks),
+                      _lib.lib().hq_window_workspace_bytes, dev)
+        os_ = out.stride()
+        rc = _lib.lib().hq_window_prefill_int8(
+            q.data_ptr(), dt, _lib.strides(q.stride(), 4), *cache, lp, qlp, B, Hq, Hkv, Sq, cap, D,
+            w, sinks, float(sm_scale), int(bool(q_quant)), out.data_ptr(),
+            _lib.strides((os_[0], os_[2], os_[1], os_[3]), 4), ws.data_ptr(), ws.numel(),
+            _status_word(dev).data_ptr(), _stream(dev))
+    check(rc, "hq_window_prefill_int8")
+    return out
+
+
+def int8_prefix_decode_attn(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_sc, lens, *,
+                            prefix_lens=None, sm_scale=None, q_quant=False, out=None):
+    """One decode step of sequences that share a prefix, the prefix read once for all of them
+    (``hq_prefix_decode_int8``).
+
+    q ``[B,Hq,1,D]`` or ``[B,Hq,D]`` (bf16/f16, D = 128).  The prefix is an int8 cache of G
+    groups (codes ``[G,Hkv,P,D]``, scales ``[G,Hkv,1,D]`` and ``[G,Hkv,P,1]``); B is a multiple
+    of G, and sequences ``g * B/G .. (g + 1) * B/G - 1`` share prefix g.  Each sequence's own
+    tokens are in ``k_i8 / k_sc / v_i8 / v_sc`` (``[B,Hkv,cap,D]`` and so on).  ``lens`` int32
+    ``[B]`` and ``prefix_lens`` int32 ``[G]`` (default: P), on the device, say how many tokens
+    are held; the output is the attention over both, and zeros where there is none.
+    """
+    what = "int8_prefix_decode_attn"
+    _cuda(q, f"{what} q")
+    qb, restore = _as_bhd(q)
+    _q16(what, qb)
+    qb = qb if _rows_ok(qb) else qb.contiguous()
+    B, Hq, D = qb.shape
+    dev = qb.device
+    _cuda(pk_i8, f"{what} pk")
+    G = pk_i8.shape[0]
+    if G < 1 or B % G:
+        raise ValueError(f"{what}: {B} sequences over {G} prefixes")
+    pre = _int8_cache(f"{what} prefix", G, D, dev, pk_i8, pk_sc, pv_i8, pv_sc)
+    own = _int8_cache(what, B, D, dev, k_i8, k_sc, v_i8, v_sc, pk_sc.dtype)
+    Hkv, cap, P = k_i8.shape[1], k_i8.shape[2], pk_i8.shape[2]
+    if pk_i8.shape[1] != Hkv or Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"{what}: {Hq} query heads over {Hkv} kv heads, {pk_i8.shape[1]} in the prefix")
+    if lens is None:
+        raise ValueError(f"{what}: lens is needed")
+    lp = _lens_ptr(what, "lens", lens, B, dev)
+    plp = _lens_ptr(what, "prefix_lens", prefix_lens, G, dev)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(D)
+    if out is not None:
+        _out_like(what, out, (B, Hq, D), qb)
+    with _on_device(dev):
+        res = out if out is not None else torch.empty((B, Hq, D), dtype=qb.dtype, device=dev)
+        if B == 0:
+            return restore(res) if out is None else res
+        dt = _DT[qb.dtype]
+        ws = _scratch((what, dev.index, dt, G, B, Hq, Hkv, P, cap, D),
+                      _lib.lib().hq_prefix_decode_workspace_bytes, dev)
+        rc = _lib.lib().hq_prefix_decode_int8(
+            qb.data_ptr(), dt, _lib.strides(qb.stride(), 3), *pre[:5], *pre[6:], plp, G, P,
+            *own[:5], *own[6:], lp, cap, own[5], B, Hq, Hkv, D, float(sm_scale),
+            int(bool(q_quant)), res.data_ptr(), _lib.strides(res.stride(), 3), ws.data_ptr(),
+            ws.numel(), _status_word(dev).data_ptr(), _stream(dev))
+    check(rc, "hq_prefix_decode_int8")
+    return restore(res) if out is None else res
+
+
+def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, *, scaling: str | None = None,
+                  factor: float = 1.0, original_len: int | None = None, beta_fast: float = 32.0,
+                  beta_slow: float = 1.0, device=None) -> tuple:
+    """Inverse frequencies for ``rope_append_kv`` and the factor its cos and sin take:
+    ``(float32 [rotary_dim / 2], factor)``.  ``theta ** (-2 j / rotary_dim)``, scaled for
+    contexts ``factor`` times longer than the model's: ``None``; ``"linear"`` (positions
+    divided by ``factor``); ``"ntk"`` (a larger base, the fastest pair unchanged, the slowest
+    divided by ``factor``); ``"yarn"`` (pairs that turn more than ``beta_fast`` times over
+    ``original_len`` unchanged, those under ``beta_slow`` divided, a linear ramp between; cos
+    and sin times ``0.1 ln(factor) + 1``; Peng et al., 2023)."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rope_inv_freq: rotary_dim must be even and positive")
+    if not theta > 0 or not factor >= 1:
+        raise ValueError("rope_inv_freq: theta > 0 and factor >= 1 expected")
+    j = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    f, mult = theta ** -j, 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("rope_inv_freq: ntk scaling needs rotary_dim >= 4")
+        f = (theta * factor ** (rotary_dim / (rotary_dim - 2))) ** -j
+    elif scaling == "yarn":
+        if not original_len or original_len < 1:
+            raise ValueError("rope_inv_freq: yarn scaling needs original_len")
+        turns = original_len * f / (2 * math.pi)
+        # in terms of the pair index, as the ramp is defined
+        index = lambda n: rotary_dim * math.log(original_len / (n * 2 * math.pi)) / (  # noqa: E731
+            2 * math.log(theta))
+        lo = max(math.floor(index(beta_fast)), 0)
+        hi = min(math.ceil(index(beta_slow)), rotary_dim - 1)
+        ramp = ((torch.arange(len(turns), dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        f = f * (1 - ramp) + f / factor * ramp
+        mult = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling is not None:
+        raise ValueError(f"rope_inv_freq: unknown scaling {scaling!r}")
+    return f.to(dtype=torch.float32, device=device if device is not None else "cuda"), mult
+
+
+def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache, lens, *,
+                   n_new=None, pos_offset=None, interleaved=False, factor=1.0, q_out=None):
+    """Rotary positions and the write of new tokens into an int8 cache, in one launch, for a
+    ragged (right-padded) batch (``hq_rope_append_kv``).
+
+    q ``[B,Hq,S,D]``, k_new / v_new ``[B,Hkv,S,D]`` (bf16/f16/f32; D 64, 128 or 256) before
+    rotation; ``inv_freq`` float32 ``[rotary_dim / 2]`` (``rope_inv_freq``); the cache's
+    capacity buffers ``[B,Hkv,cap,D]`` int8, its stored K scales ``k_sc [1|B,Hkv,1,D]`` and V
+    scales ``[B,Hkv,cap,1]`` (both f16 or f32).  Token i < n_new[b] (default S) of sequence b
+    stands at position ``lens[b] + i + pos_offset[b]`` (``pos_offset``: the length of a shared
+    prefix, for one) and goes to row ``lens[b] + i``; ``lens`` (int32 ``[B]``, device) is not
+    advanced.  K is coded with the stored scale, as ``quant_k_static`` codes it, from the
+    rotated and unrounded values; V per token, its scales written.  Returns the rotated q
+    (``q_out``, which may be q; rows past ``n_new[b]`` are q's).  A sequence whose tokens do not
+    fit its capacity writes nothing and sets ``ragged_status()``.
+    """
+    what = "rope_append_kv"
+    for t, n in ((q, "q"), (k_new, "k_new"), (v_new, "v_new"), (inv_freq, "inv_freq"),
+                 (k_cache, "k_cache"), (v_cache, "v_cache"), (k_sc, "k_sc"),
+                 (v_sc_cache, "v_sc_cache")):
+        _cuda(t, f"{what} {n}")
+        if t.device != q.device:
+            raise ValueError(f"{what}: {n} is on {t.device}, q on {q.device}")
+    if q.dim() != 4 or k_new.dim() != 4 or k_new.shape != v_new.shape:
+        raise ValueError(f"{what}: q [B,Hq,S,D] and k_new, v_new [B,Hkv,S,D] expected")
+    B, Hq, S, D = q.shape
+    Hkv, cap = k_new.shape[1], k_cache.shape[2] if k_cache.dim() == 4 else -1
+    dt = _dtype_code(q, what)
+    if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
+        raise TypeError(f"{what}: q, k_new and v_new must have one dtype")
+    if (k_new.shape[0], k_new.shape[2], k_new.shape[3]) != (B, S, D):
+        raise ValueError(f"{what}: k_new {tuple(k_new.shape)} does not fit q {tuple(q.shape)}")
+    for t in (k_cache, v_cache):
+        if tuple(t.shape) != (B, Hkv, cap, D) or t.dtype != torch.int8:
+            raise ValueError(f"{what}: caches must be int8 [B,Hkv,cap,D]")
+    if k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1 or any(
+            s % 16 for s in k_cache.stride()[:3]) or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise ValueError(f"{what}: K/V caches must share strides, with contiguous, 16-byte aligned rows")
+    if tuple(v_sc_cache.shape) != (B, Hkv, cap, 1):
+        raise ValueError(f"{what}: v_sc_cache must be [B,Hkv,cap,1]")
+    if k_sc.dtype != v_sc_cache.dtype or k_sc.dtype not in (torch.float16, torch.float32):
+        raise TypeError(f"{what}: scales must both be float16 or float32")
+    _, kst = _static_scale(k_sc, B, Hkv, D, what)
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or (
+            2 * inv_freq.numel() > D):
+        raise ValueError(f"{what}: inv_freq must be contiguous float32 of at most D / 2 elements")
+    dev = q.device
+    if lens is None:
+        raise ValueError(f"{what}: lens is needed")
+    lp = _lens_ptr(what, "lens", lens, B, dev)
+    nnp = _lens_ptr(what, "n_new", n_new, B, dev)
+    pop = _lens_ptr(what, "pos_offset", pos_offset, B, dev)
+    if q_out is None:
+        q, k_new, v_new = _rowmajor(q), _rowmajor(k_new), _rowmajor(v_new)
+    else:
+        k_new, v_new = _rowmajor(k_new), _rowmajor(v_new)
+        if q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != dev or not _rows_ok(q_out):
+            raise ValueError(f"{what}: q_out must have q's shape, dtype and device, with 16-byte "
+                             "aligned rows")
+        q = _rowmajor(q)
+    with _on_device(dev):
+        res = q_out if q_out is not None else torch.empty((B, Hq, S, D), dtype=q.dtype, device=dev)
+        rc = _lib.lib().hq_rope_append_kv(
+            q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), dt, _lib.strides(q.stride(), 4),
+            _lib.strides(k_new.stride(), 4), _lib.strides(v_new.stride(), 4), B, Hq, Hkv, S, D,
+            inv_freq.data_ptr(), 2 * inv_freq.numel(), int(bool(interleaved)), float(factor), lp,
+            nnp, pop, k_sc.data_ptr(), _DT[k_sc.dtype], kst, k_cache.data_ptr(),
+            v_cache.data_ptr(), _lib.strides(k_cache.stride()[:3], 3), v_sc_cache.data_ptr(),
+            _lib.strides(v_sc_cache.stride()[:3], 3), cap, res.data_ptr(),
+            _lib.strides(res.stride(), 4), _status_word(dev).data_ptr(), _stream(dev))
+    check(rc, "hq_rope_append_kv")
+    return res

@@ -9,7 +9,10 @@
  *      online softmax, plus a same-design dense (bf16/f16) twin, the
  *      log-sum-exp combine of partial results, a device-resident-length
  *      variant (graph replay) and a sequence-sharded variant over peer memory;
- *   3. causal prefill attention over the int8 cache.
+ *   3. causal prefill attention over the int8 cache;
+ *   4. batches whose sequences have lengths of their own: rotary positions
+ *      with the write to the cache, attention under a sliding window with sink
+ *      tokens, decode over a prefix shared by a group of sequences.
  *
  * Conventions (every entry point):
  *   - Pointers are device pointers; sizes and strides are in ELEMENTS of the
@@ -549,6 +552,95 @@ HQ_API int hq_kblock_dequant(const int8_t* k_cache, const int64_t kq_strides[3],
                              const float* k_scale, const int64_t ks_strides[3], int B, int H,
                              int S, int D, int block_tokens, void* out, int out_dtype,
                              const int64_t out_strides[4], hq_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Batches whose sequences have lengths of their own (no counterpart in the
+ * reference, whose batch has one length and whose attention sees all of it).
+ * lens int32[B] in device memory holds the cached tokens of each sequence
+ * (clamped to [0, S_max]); rows past it are never read.  K and V may have any
+ * (b, h, s) strides that are multiples of 16 bytes, shared by both, with
+ * 16-byte aligned bases.  V scales are zero or positive, finite float32 or
+ * float16; a token whose V scale is below 2^-60 counts as zeros.  q is bf16 or
+ * f16 with 16-byte aligned rows, out has q's type with 8-byte aligned rows; D =
+ * 128, Hq / Hkv whole and at most 128.  Scratch lies in `workspace` (256-byte
+ * aligned, contents undefined before and after: nothing carries over from call
+ * to call).  `status` (optional) receives HQ_ERR_DEVICE_TIMEOUT if a bounded
+ * wait inside a block gave up (first error sticks).
+ *
+ * hq_window_decode_int8: one query per sequence, the token at position
+ *   lens[b] - 1, over keys j with j >= lens[b] - window or j < sinks (window 0:
+ *   all keys).  lens[b] = 0 gives zeros.  q / out [B, Hq, D].
+ * hq_window_prefill_int8: q [B, Hq, Sq, D], out logical [B, Hq, Sq, D]; the
+ *   first q_lens[b] rows of sequence b are queries (q_lens NULL: all Sq), query
+ *   i at position p = lens[b] - q_lens[b] + i, over keys j <= p with j > p -
+ *   window or j < sinks.  The queries' own tokens are the last q_lens[b] cached
+ *   ones.  Output rows past q_lens[b] are left as they were; a query with p < 0
+ *   gives zeros.
+ * hq_window_workspace_bytes: of hq_window_prefill_int8, or with Sq = 0 of
+ *   hq_window_decode_int8; 0: unsupported.
+ * hq_prefix_decode_int8: one query per sequence; sequences g * B / G .. (g + 1)
+ *   * B / G - 1 share prefix g of pk / pv [G, Hkv, P_max, D] (prefix_lens
+ *   int32[G] tokens of it, NULL: P_max) and each has its own tokens in k / v
+ *   [B, Hkv, S_max, D] (lens int32[B], NULL: S_max).  A query sees all of both;
+ *   the prefix is read once for the whole group.  Scales as hq_decode_int8, of
+ *   one scale_dtype.  B + G <= 2048.
+ */
+HQ_API size_t hq_window_workspace_bytes(int q_dtype, int B, int Hq, int Hkv, int Sq, int S_max,
+                                        int D, int window, int sinks);
+HQ_API int hq_window_decode_int8(const void* q, int q_dtype, const int64_t q_strides[3],
+                                 const int8_t* k, const int8_t* v, const int64_t kv_strides[3],
+                                 const void* k_scale, const void* v_scale, int scale_dtype,
+                                 const int64_t ksc_strides[3], const int64_t vsc_strides[3],
+                                 const int* lens, int B, int Hq, int Hkv, int S_max, int D,
+                                 int window, int sinks, float sm_scale, int q_quant, void* out,
+                                 const int64_t out_strides[3], void* workspace,
+                                 size_t workspace_bytes, int* status, hq_stream_t stream);
+HQ_API int hq_window_prefill_int8(const void* q, int q_dtype, const int64_t q_strides[4],
+                                  const int8_t* k, const int8_t* v, const int64_t kv_strides[3],
+                                  const void* k_scale, const void* v_scale, int scale_dtype,
+                                  const int64_t ksc_strides[3], const int64_t vsc_strides[3],
+                                  const int* lens, const int* q_lens, int B, int Hq, int Hkv,
+                                  int Sq, int S_max, int D, int window, int sinks, float sm_scale,
+                                  int q_quant, void* out, const int64_t out_strides[4],
+                                  void* workspace, size_t workspace_bytes, int* status,
+                                  hq_stream_t stream);
+HQ_API size_t hq_prefix_decode_workspace_bytes(int q_dtype, int G, int B, int Hq, int Hkv,
+                                               int P_max, int S_max, int D);
+HQ_API int hq_prefix_decode_int8(
+    const void* q, int q_dtype, const int64_t q_strides[3], const int8_t* pk, const int8_t* pv,
+    const int64_t pkv_strides[3], const void* pk_scale, const void* pv_scale,
+    const int64_t pksc_strides[3], const int64_t pvsc_strides[3], const int* prefix_lens, int G,
+    int P_max, const int8_t* k, const int8_t* v, const int64_t kv_strides[3], const void* k_scale,
+    const void* v_scale, const int64_t ksc_strides[3], const int64_t vsc_strides[3],
+    const int* lens, int S_max, int scale_dtype, int B, int Hq, int Hkv, int D, float sm_scale,
+    int q_quant, void* out, const int64_t out_strides[3], void* workspace, size_t workspace_bytes,
+    int* status, hq_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * hq_rope_append_kv: rotary positions and the write of new tokens, one launch.
+ *   q [B, Hq, S_new, D], k_new / v_new [B, Hkv, S_new, D] of x_dtype (F32, BF16,
+ *   F16; D in {64, 128, 256}; 16-byte aligned rows).  Token i < n_new[b] (NULL:
+ *   S_new) of sequence b stands at position lens[b] + i + pos_offset[b] (NULL:
+ *   0) and goes to cache row lens[b] + i; lens is not advanced.  The first
+ *   rotary_dim channels (even) of q and k are turned by position * inv_freq[j]
+ *   (float32 [rotary_dim / 2]), pairs (j, j + rotary_dim / 2) or, interleaved,
+ *   (2j, 2j + 1), cos and sin times `factor`.  q_out receives the rotated q
+ *   (may be q itself; rows past n_new[b] are copied unturned).  K codes are
+ *   clamp(rint(k / k_scale), -127, 127) of the rotated, unrounded k with the
+ *   cache's per-channel scale [B, Hkv, D] (ksc_strides, a stride of 0
+ *   broadcasts); V codes and scales as hq_quant_v_pertoken.  k_cache / v_cache
+ *   are capacity buffers with strides kv_strides[3], v_scale [B, Hkv, capacity]
+ *   of scale_dtype (as k_scale).  A sequence whose tokens do not fit writes
+ *   nothing to the cache and sets HQ_ERR_INVALID_ARGUMENT in `status`.
+ */
+HQ_API int hq_rope_append_kv(
+    const void* q, const void* k_new, const void* v_new, int x_dtype, const int64_t q_strides[4],
+    const int64_t k_strides[4], const int64_t v_strides[4], int B, int Hq, int Hkv, int S_new,
+    int D, const float* inv_freq, int rotary_dim, int interleaved, float factor, const int* lens,
+    const int* n_new, const int* pos_offset, const void* k_scale, int scale_dtype,
+    const int64_t ksc_strides[3], int8_t* k_cache, int8_t* v_cache, const int64_t kv_strides[3],
+    void* v_scale, const int64_t vsc_strides[3], int capacity, void* q_out,
+    const int64_t qo_strides[4], int* status, hq_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Reads (and synchronises `stream` for) the device status word at the start

@@ -9,16 +9,20 @@
 // over a shared prefix sees all of it and all of its own sequence's tokens.
 //
 // Mathematics.  One pass over the keys with the running maximum and sum of a softmax, in
-// base 2.  Neither cache side is dequantized: the K scales, the softmax scale and log2(e)
-// are folded into q once per row (q' = q k_scale sm_scale log2 e, times a power of two
-// that brings the row's largest |q'| to [2^13, 2^14), rounded to float16; for float16
-// models a second float16 holds what the first leaves over), and the V scale of key j
-// joins the exponent: with t_j = s_j + log2 v_scale_j and m a running maximum of t,
-//   P_j = 2^(t_j - m) (float16),  O += P_j code_j,  l += P_j / v_scale_j (float32),
-// so o = O / l holds for V scales of any size, and P needs no scaling of its own.  The
-// int8 codes are exact in float16.  m moves only when t grows by more than 8 (P <= 256,
-// far inside float16), so O in tensor memory is rarely rescaled.  P rounded to float16 is
-// off by 2^-11 of itself at most, half a step of the coarsest output type below bf16.
+// base 2.  The K scales, the softmax scale and log2(e) are folded into q once per row (q' =
+// q k_scale sm_scale log2 e, times a power of two that brings the row's largest |q'| to
+// [2^13, 2^14), rounded to float16; for float16 models a second float16 holds what the first
+// leaves over); the int8 K codes are exact in float16.  V's scale is split in two: v_scale_j
+// = g_j 2^(E + e_j), where E belongs to the piece of work.  g_j goes into V's float16 tile
+// (code g_j), e_j joins the exponent: with t_j = s_j + e_j and m a running maximum of t,
+//   P_j = 2^(t_j - m) (float16),  O += P_j (code_j g_j),  l += P_j 2^-e_j (float32),
+// and o = 2^E O / l for V scales of any size.  A tile whose V scales lie within 2^-4 .. 2^6
+// of 2^E (nearly every one) has all e_j = 0, and costs nothing for them; the others look
+// e_j up.  Float16 models always put the whole scale into e_j (not a whole number then), so
+// that V stays exact.  m moves only when t grows by more than 8 (P <= 256, far inside
+// float16), so O in tensor memory is rarely rescaled.  Roundings to float16, each off by
+// 2^-11 of itself at most: q' (bf16 models), P, and for bf16 models g_j and code g_j, an
+// eighth of the output's own half step.
 //
 // Work.  Row r of a unit (kv head, sequence or group) is q head kvh * n_rep + r % n_rep of
 // query r / n_rep; 128 rows sit on the 128 lanes of tensor memory, one or two such tiles
@@ -29,12 +33,14 @@
 // block border leaves partial states (m, l, O) that combine_kernel joins.  Prefill blocks
 // take one row tile each (split over a few blocks when there are few).
 //
-// Roles of a block (one per SM): softmax warps (4 per row tile, one thread per row), 8
-// warps that read codes from global memory into registers two tiles ahead, turn them into
-// float16 with byte permutes and store them in the 128-byte-swizzled layouts the MMA reads
-// (they also form q'), and one warp whose first lane issues the tcgen05.mma products:
-// S = Q K^T into tensor memory, O += P V with P read from tensor memory, where it
-// overwrites the S it came from.  mbarriers order the roles; every wait is bounded.
+// Roles of a block (one per SM): softmax warps (4 per row tile, one thread per row; they also
+// form q'), 4 warps that turn staged codes into float16 with byte permutes and store them in
+// the 128-byte-swizzled layouts the MMA reads, one warp that fills the staging ring with bulk
+// copies (64 keys of K or V per slot) and reads the V scales, and one whose first lane issues
+// the tcgen05.mma products: S = Q K^T into tensor memory, O += P V with P read from tensor
+// memory, where it overwrites the S it came from.  mbarriers order the roles; every wait is
+// bounded.  (Codes loaded into registers and converted from there took 4000 cycles a tile:
+// the proxy fence before each hand-over waited for the loads of the next tile.)
 #include <algorithm>
 #include <atomic>
 
@@ -49,11 +55,13 @@ using namespace tc;
 
 constexpr int kD = 128;
 constexpr int kBN = 128;                  // keys per tile
-constexpr int kConvThreads = 256;
+constexpr int kConvThreads = 128;
 constexpr int kTileB = kBN * kD * 2;      // a float16 K, V or Q tile: 32 KB
 constexpr int kStages = 2;                // K and V tiles in shared memory
-constexpr int kLvSlots = 4;               // ring of the keys' log2 V scales and reciprocals
-constexpr int kMaxEntries = 2048;         // sequences plus groups of one call
+constexpr int kSlotKeys = 64;             // keys of a staging slot (K or V codes)
+constexpr int kSlotB = kSlotKeys * kD;
+constexpr int kLvSlots = 2;               // ring of what the tiles' V scales lead to
+constexpr int kMaxEntries = 1536;         // sequences plus groups of one call
 constexpr int kPartRow = kD + 4;          // partial rows: m, l, two pad words, o
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kWaitNs = 2000000000ull;
@@ -102,30 +110,25 @@ struct Params {
 template <int NM, bool LO>
 struct Cfg {
   static constexpr int kSoft = 128 * NM;
-  static constexpr int kThreads = kSoft + kConvThreads + 32;
+  static constexpr int kThreads = kSoft + kConvThreads + 64;
   static constexpr int kParts = LO ? 2 : 1;
-  static constexpr int kQBuf = NM * kParts == 1 ? 2 : 1;
-  static constexpr int kQB = kQBuf * NM * kParts * kTileB;
-  static constexpr int kOffK = kQB;
+  static constexpr int kSlots = NM * kParts == 1 ? 7 : 3;          // staging: 8 KB each
+  static constexpr int kOffK = NM * kParts * kTileB;
   static constexpr int kOffV = kOffK + kStages * kTileB;
-  static constexpr int kOffLv = kOffV + kStages * kTileB;          // [slot][log2, 1/x][128]
-  static constexpr int kOffFac = kOffLv + kLvSlots * 2 * kBN * 4;  // [qbuf][128 NM]
-  static constexpr int kOffBar = kOffFac + kQBuf * 128 * NM * 4;
-  static constexpr int kBars = 2 * kQBuf + 4 * kStages + kLvSlots + 2 + 2 + 2 * NM + 1;
+  static constexpr int kOffSlot = kOffV + kStages * kTileB;
+  static constexpr int kOffE = kOffSlot + kSlots * kSlotB;         // [slot][e_j, 2^-e_j][128]
+  static constexpr int kOffG = kOffE + kLvSlots * 2 * kBN * 4;     // [slot][128] float16 g_j
+  static constexpr int kOffInfo = kOffG + kLvSlots * kBN * 2;      // [slot]{any e_j, 2^E}
+  static constexpr int kOffBar = kOffInfo + kLvSlots * 8;
+  static constexpr int kBars = 1 + 4 * kStages + 2 * kSlots + kLvSlots + 2 + 2 + 2 * NM + 1;
   static constexpr int kOffMisc = kOffBar + ((kBars * 8 + 15) & ~15);
   static constexpr int kOffCum = kOffMisc + 16;
   static constexpr int smem(int entries) { return 1024 + kOffCum + 4 * (entries + 1); }
   static_assert(1024 + kOffCum + 4 * (kMaxEntries + 1) <= 232448, "one block per SM");
+  static_assert(kLvSlots == kStages, "a slot is free with its V stage");
 };
 
 // ---------------------------------------------------------------- small helpers
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 __device__ __forceinline__ float load_scale(const void* p, int64_t i, int dt) {
   return dt == HQ_DTYPE_F16 ? __half2float(static_cast<const __half*>(p)[i])
                             : static_cast<const float*>(p)[i];
@@ -133,6 +136,10 @@ __device__ __forceinline__ float load_scale(const void* p, int64_t i, int dt) {
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+constexpr float kTinyScale = 8.6736174e-19f;  // 2^-60: V scales below count as zero
+__device__ __forceinline__ float pow2i(int e) {  // 2^e, -126 <= e <= 127
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 // four int8 codes -> two float16 pairs, exact: the biased byte under the exponent of 1024
 __device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t& a, uint32_t& b) {
@@ -157,17 +164,47 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-// Bounded wait (2 s, or as soon as another role of the block has given up).
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_ns();
+// 32 columns of this thread's lane, loaded by tmem_get and valid after tmem_got (which
+// awaits every load issued before it; the registers pass through it, so no use moves up)
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+      "%28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_got(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31]));
+}
+// Bounded wait (2 s, or as soon as another role of the block has given up).  The loop is a
+// call: the roles' code together has to stay within the instruction cache.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  uint64_t t0 = 0;
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63) == 0 && (*abort || global_ns() - t0 > kWaitNs)) {
-      *abort = 1;
-      return false;
+    if ((i & 255) == 0) {
+      const uint64_t t = global_ns();
+      if (t0 == 0) t0 = t;
+      if (*abort || t - t0 > kWaitNs) {
+        *abort = 1;
+        return false;
+      }
     }
   }
+}
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return mbar_try_wait(bar, parity) || wait_long(bar, parity, abort);
 }
 
 // ---------------------------------------------------------------- pieces of work
@@ -272,8 +309,9 @@ struct Walk {
       if (w.rows <= 0) return false;
       w.key = make_keys(s, seg_len(s, b), nq, w.row0 / p.nrep, (w.row0 + w.rows - 1) / p.nrep);
       const int nt = max(w.key.nt, 1);
-      w.t0 = static_cast<int>(static_cast<int64_t>(nt) * split / p.n_split);
-      w.t1 = static_cast<int>(static_cast<int64_t>(nt) * (split + 1) / p.n_split);
+      const uint32_t ns = p.n_split;  // (nt < 2^24, n_split <= 16)
+      w.t0 = static_cast<int>(static_cast<uint32_t>(nt) * split / ns);
+      w.t1 = static_cast<int>(static_cast<uint32_t>(nt) * (split + 1) / ns);
       w.slot = p.n_split == 1 ? -1
                               : ((b * p.Hkv + w.kvh) * p.n_rt + rt) * p.n_split + split;
     }
@@ -301,46 +339,43 @@ __device__ __forceinline__ char* out_row(const Params& p, int b, int u, int h) {
   return static_cast<char*>(p.out) + 2 * (b * p.osb + u * p.osu + h * p.osh);
 }
 
+// Per-token int8 fake quantization of a q row held by 16 lanes, 8 channels each, rounded
+// back to the model dtype.
+struct Eight {
+  float x[8];
+};
+__device__ __noinline__ Eight fake_quant8(Eight f, int dt) {
+  float am = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(f.x[e]));
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+  const Quantizer qz = Quantizer::from_amax(am);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float y = static_cast<float>(qz.code(f.x[e])) * qz.scale;
+    f.x[e] = dt == HQ_DTYPE_BF16 ? __bfloat162float(__float2bfloat16_rn(y))
+                                 : __half2float(__float2half_rn(y));
+  }
+  return f;
+}
+
 // ---------------------------------------------------------------- softmax of one row tile
 struct RowLim {
   int hi, lo, vsk;  // key v is seen when v <= hi and (v >= lo or v < vsk)
+  // bit e: key v0 + e is seen
+  __device__ __forceinline__ uint32_t bits(int v0) const {
+    const uint32_t upto = below(hi + 1 - v0);
+    return upto & (~below(lo - v0) | below(vsk - v0));
+  }
+  __device__ __forceinline__ static uint32_t below(int n) {  // bits 0 .. n - 1
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+  }
 };
-// t = s * fac + log2(v_scale) of 32 keys, masked; returns into f (pairs)
-template <bool MASK>
-__device__ __forceinline__ void row_t(const float (&s)[32], const float* lv, float fac, int v0,
-                                      const RowLim& lim, float (&t)[32]) {
-  const F2 f2 = f2_make(fac, fac);
-#pragma unroll
-  for (int e = 0; e < 32; e += 4) {
-    const float4 l4 = *reinterpret_cast<const float4*>(lv + e);
-    const F2 a = f2_fma(f2_make(s[e], s[e + 1]), f2, f2_make(l4.x, l4.y));
-    const F2 b = f2_fma(f2_make(s[e + 2], s[e + 3]), f2, f2_make(l4.z, l4.w));
-    f2_split(a, t[e], t[e + 1]);
-    f2_split(b, t[e + 2], t[e + 3]);
-  }
-  if constexpr (MASK) {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      const int v = v0 + e;
-      if (!(v <= lim.hi && (v >= lim.lo || v < lim.vsk))) t[e] = -INFINITY;
-    }
-  }
-}
-
-template <bool MASK>
-__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, const float* lv,
-                                             float fac, int v0, const RowLim& lim, bool first,
-                                             uint64_t* pv_bar, int cnt, volatile int* abort,
-                                             float& m, float& l, bool& ok) {
-  float mx = -INFINITY;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    float s[32], t[32];
-    tmem_ld32(s_addr + 32 * c, s);
-    row_t<MASK>(s, lv + 32 * c, fac, v0 + 32 * c, lim, t);
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(t[e], t[e + 1]));
-  }
+// The running maximum takes this tile's largest t in, O and l are rescaled where it moves;
+// waits for the previous P V on the way.
+__device__ __forceinline__ void move_max(float mx, uint32_t o_addr, bool first, uint64_t* pv_bar,
+                                         int cnt, volatile int* abort, float& m, float& l, bool& ok) {
   float a = 1.0f;
   if (mx > m + 8.0f || (m == -INFINITY && mx != -INFINITY)) {
     a = ex2_ftz(m - mx);
@@ -365,36 +400,128 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, c
       tmem_st32(o_addr + 32 * c, o);
     }
   }
-  const float nb = m == -INFINITY ? 0.0f : -m;
-  const F2 nb2 = f2_make(nb, nb);
-  F2 ls0 = f2_make(0.0f, 0.0f), ls1 = ls0;
+}
+
+// One tile of one row, all of it seen and with all e_j = 0: the running maximum, then
+// P = 2^(s fac - m) over S and l.
+__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, float fac,
+                                             bool first, uint64_t* pv_bar, int cnt,
+                                             volatile int* abort, float& m, float& l, bool& ok) {
+  uint32_t sa[32], sb[32];
+  float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  auto fold = [&](const uint32_t (&s)[32]) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    float s[32], t[32];
-    tmem_ld32(s_addr + 32 * c, s);
-    row_t<MASK>(s, lv + 32 * c, fac, v0 + 32 * c, lim, t);
+    for (int e = 0; e < 32; e += 8)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[i] = fmaxf(x[i], fmaxf(__uint_as_float(s[e + 2 * i]), __uint_as_float(s[e + 2 * i + 1])));
+  };
+  tmem_get(s_addr, sa);
+  tmem_got(sa);
+  tmem_get(s_addr + 32, sb);
+  fold(sa);
+  tmem_got(sb);
+  tmem_get(s_addr + 64, sa);
+  fold(sb);
+  tmem_got(sa);
+  tmem_get(s_addr + 96, sb);
+  fold(sa);
+  tmem_got(sb);
+  fold(sb);
+  move_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * fac, o_addr, first, pv_bar, cnt, abort, m,
+           l, ok);
+  if (!ok) return;
+  const F2 nb2 = f2_make(-m, -m), fac2 = f2_make(fac, fac);
+  F2 ls0 = f2_make(0.0f, 0.0f), ls1 = ls0;
+  // P of keys 32 c .. goes over S columns 16 c .., which have been read by then
+  auto emit = [&](const uint32_t (&s)[32], int c) {
     uint32_t w[16];
 #pragma unroll
     for (int e = 0; e < 32; e += 4) {
-      const float4 r4 = *reinterpret_cast<const float4*>(lv + kBN + 32 * c + e);
-      float x0, x1, x2, x3;
-      f2_split(f2_add(f2_make(t[e], t[e + 1]), nb2), x0, x1);
-      f2_split(f2_add(f2_make(t[e + 2], t[e + 3]), nb2), x2, x3);
-      x0 = ex2_ftz(x0);
-      x1 = ex2_ftz(x1);
-      x2 = ex2_ftz(x2);
-      x3 = ex2_ftz(x3);
-      ls0 = f2_fma(f2_make(x0, x1), f2_make(r4.x, r4.y), ls0);
-      ls1 = f2_fma(f2_make(x2, x3), f2_make(r4.z, r4.w), ls1);
-      w[e / 2] = pack_h2(x0, x1);
-      w[e / 2 + 1] = pack_h2(x2, x3);
+      float t[4];
+      f2_split(f2_fma(f2_make(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), fac2, nb2), t[0], t[1]);
+      f2_split(f2_fma(f2_make(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), fac2, nb2), t[2], t[3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = ex2_ftz(t[i]);
+      ls0 = f2_add(ls0, f2_make(t[0], t[1]));
+      ls1 = f2_add(ls1, f2_make(t[2], t[3]));
+      w[e / 2] = pack_h2(t[0], t[1]);
+      w[e / 2 + 1] = pack_h2(t[2], t[3]);
     }
-    // P of keys 32 c .. over S columns 16 c .., which are read
     tmem_st16(s_addr + 16 * c, w);
-  }
+  };
+  tmem_get(s_addr, sa);
+  tmem_got(sa);
+  tmem_get(s_addr + 32, sb);
+  emit(sa, 0);
+  tmem_got(sb);
+  tmem_get(s_addr + 64, sa);
+  emit(sb, 1);
+  tmem_got(sa);
+  tmem_get(s_addr + 96, sb);
+  emit(sa, 2);
+  tmem_got(sb);
+  emit(sb, 3);
   float x0, x1;
   f2_split(f2_add(ls0, ls1), x0, x1);
   l += x0 + x1;
+  tmem_wait_st();
+}
+
+// The same for any tile: e_j from ev[j], 2^-e_j from ev[128 + j], and keys some rows do not
+// see.  Rolled over the four runs of 32 keys, to keep the code small.
+__device__ __forceinline__ void softmax_tile_any(uint32_t s_addr, uint32_t o_addr, const float* ev,
+                                                 float fac, int v0, const RowLim& lim, bool first,
+                                                 uint64_t* pv_bar, int cnt, volatile int* abort,
+                                                 float& m, float& l, bool& ok) {
+  uint32_t s[32];
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t seen = lim.bits(v0 + 32 * c);
+    tmem_get(s_addr + 32 * c, s);
+    tmem_got(s);
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      const float4 e4 = *reinterpret_cast<const float4*>(ev + 32 * c + e);
+      const float t0 = __fmaf_rn(__uint_as_float(s[e]), fac, e4.x);
+      const float t1 = __fmaf_rn(__uint_as_float(s[e + 1]), fac, e4.y);
+      const float t2 = __fmaf_rn(__uint_as_float(s[e + 2]), fac, e4.z);
+      const float t3 = __fmaf_rn(__uint_as_float(s[e + 3]), fac, e4.w);
+      mx = fmaxf(mx, fmaxf(seen >> e & 1 ? t0 : -INFINITY, seen >> (e + 1) & 1 ? t1 : -INFINITY));
+      mx = fmaxf(mx, fmaxf(seen >> (e + 2) & 1 ? t2 : -INFINITY, seen >> (e + 3) & 1 ? t3 : -INFINITY));
+    }
+  }
+  move_max(mx, o_addr, first, pv_bar, cnt, abort, m, l, ok);
+  if (!ok) return;
+  const float nb = m == -INFINITY ? 0.0f : -m;
+  float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t seen = lim.bits(v0 + 32 * c);
+    tmem_get(s_addr + 32 * c, s);
+    tmem_got(s);
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      const float4 e4 = *reinterpret_cast<const float4*>(ev + 32 * c + e);
+      const float4 r4 = *reinterpret_cast<const float4*>(ev + kBN + 32 * c + e);
+      float t[4] = {__fmaf_rn(__uint_as_float(s[e]), fac, e4.x + nb),
+                    __fmaf_rn(__uint_as_float(s[e + 1]), fac, e4.y + nb),
+                    __fmaf_rn(__uint_as_float(s[e + 2]), fac, e4.z + nb),
+                    __fmaf_rn(__uint_as_float(s[e + 3]), fac, e4.w + nb)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = seen >> (e + i) & 1 ? ex2_ftz(t[i]) : 0.0f;
+      ls[0] = __fmaf_rn(t[0], r4.x, ls[0]);
+      ls[1] = __fmaf_rn(t[1], r4.y, ls[1]);
+      ls[2] = __fmaf_rn(t[2], r4.z, ls[2]);
+      ls[3] = __fmaf_rn(t[3], r4.w, ls[3]);
+      w[e / 2] = pack_h2(t[0], t[1]);
+      w[e / 2 + 1] = pack_h2(t[2], t[3]);
+    }
+    tmem_st16(s_addr + 16 * c, w);  // over S columns that have been read
+  }
+  l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
   tmem_wait_st();
 }
 
@@ -406,16 +533,18 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* lvb = reinterpret_cast<float*>(smem + C::kOffLv);
-  float* facb = reinterpret_cast<float*>(smem + C::kOffFac);
+  float* eb = reinterpret_cast<float*>(smem + C::kOffE);
+  __half* gb = reinterpret_cast<__half*>(smem + C::kOffG);
+  float2* info = reinterpret_cast<float2*>(smem + C::kOffInfo);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* q_full = bars;
-  uint64_t* q_empty = q_full + C::kQBuf;
-  uint64_t* k_full = q_empty + C::kQBuf;
+  uint64_t* k_full = q_full + 1;
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
-  uint64_t* lv_full = v_empty + kStages;
+  uint64_t* st_full = v_empty + kStages;
+  uint64_t* st_empty = st_full + C::kSlots;
+  uint64_t* lv_full = st_empty + C::kSlots;
   uint64_t* s_full = lv_full + kLvSlots;  // per S buffer
   uint64_t* p_ready = s_full + 2;
   uint64_t* pv_done = p_ready + 2;        // per row tile
@@ -426,7 +555,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
   int* cum = reinterpret_cast<int*>(smem + C::kOffCum);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kMmaWarp = (C::kSoft + kConvThreads) / 32;
+  constexpr int kMmaWarp = (C::kSoft + kConvThreads) / 32, kCopyWarp = kMmaWarp + 1;
   // combine_kernel's blocks may be scheduled; they wait for this grid
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == kMmaWarp) {
@@ -437,17 +566,18 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     if (lane == 0) {
       *abort = 0;
-      for (int i = 0; i < C::kQBuf; ++i) {
-        mbar_init(&q_full[i], kConvThreads / 32);
-        mbar_init(&q_empty[i], 1 + C::kSoft / 32);  // the products' commit, each softmax warp
-      }
+      mbar_init(q_full, C::kSoft / 32);
       for (int i = 0; i < kStages; ++i) {
         mbar_init(&k_full[i], kConvThreads / 32);
         mbar_init(&k_empty[i], 1);
         mbar_init(&v_full[i], kConvThreads / 32);
         mbar_init(&v_empty[i], 1);
       }
-      for (int i = 0; i < kLvSlots; ++i) mbar_init(&lv_full[i], kConvThreads / 32);
+      for (int i = 0; i < C::kSlots; ++i) {
+        mbar_init(&st_full[i], 1);
+        mbar_init(&st_empty[i], kConvThreads / 32);
+      }
+      for (int i = 0; i < kLvSlots; ++i) mbar_init(&lv_full[i], 1);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
         mbar_init(&p_ready[i], 4);
@@ -493,7 +623,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
                  v_base = smem_u32(smem + C::kOffV);
   Walk<MT, STREAM> walk;
   walk.start(p, cum);
-  Piece w;
+  Piece w{};
 
   if (warp < C::kSoft / 32) {
     // ================= softmax: one thread per row
@@ -502,17 +632,91 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
     const uint32_t o_addr = tmem + kColO + 128 * mt + lane_base;
     int pc = 0, gt = 0, cnt = 0;        // pieces, tiles of the block, tiles of this row tile
     bool ok = true;
+    // q' of this warp's 32 rows into the Q tile (16 lanes per row, two rows at a time, the
+    // loads of 8 rows in flight); returns 2^-ex of this lane's row.  The Q tile is free: this
+    // warp has seen the last S of the piece before.
+    auto make_q = [&]() -> float {
+      const Seg& s = p.seg[w.seg];
+      const int l16 = lane & 15, half = lane >> 4, r0 = 32 * warp;
+      float ks[8];
+      const int64_t k0 = w.b * s.kscb + w.kvh * s.ksch;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        ks[e] = load_scale(s.ksc, k0 + (8 * l16 + e) * s.kscd, p.s_dt) * p.qk_scale;
+      unsigned char* tile = smem + mt * C::kParts * kTileB;
+      float mine = 0.0f;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32 && r0 + i0 < w.rows; i0 += 8) {
+        uint4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rr = r0 + i0 + 2 * i + half;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (rr < w.rows) {
+            const int u = (w.row0 + rr) / p.nrep, h = w.kvh * p.nrep + (w.row0 + rr) % p.nrep;
+            x[i] = *reinterpret_cast<const uint4*>(
+                static_cast<const char*>(p.q) +
+                2 * (w.b * s.qsb + u * s.qsu + h * p.qsh + 8 * l16));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rr = r0 + i0 + 2 * i + half;
+          float f[8];
+          if (p.q_dt == HQ_DTYPE_BF16) Vec16<HQ_DTYPE_BF16>::unpack(x[i], f);
+          else Vec16<HQ_DTYPE_F16>::unpack(x[i], f);
+          if (p.q_quant) {
+            const Eight g = fake_quant8(*reinterpret_cast<const Eight*>(f), p.q_dt);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = g.x[e];
+          }
+          float am = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f[e] *= ks[e];
+            am = fmaxf(am, fabsf(f[e]));
+          }
+#pragma unroll
+          for (int o = 8; o >= 1; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+          // 2^ex brings am to [2^13, 2^14)
+          const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am) >> 23) - 127), -100), 100);
+          const float mul = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
+          const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+          const float a = __shfl_sync(0xffffffffu, inv, 0), b = __shfl_sync(0xffffffffu, inv, 16);
+          if (lane == i0 + 2 * i) mine = a;
+          if (lane == i0 + 2 * i + 1) mine = b;
+          if (rr >= w.rows) continue;
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y0 = f[2 * e] * mul, y1 = f[2 * e + 1] * mul;
+            hi[e] = pack_h2(y0, y1);
+            if constexpr (LO) {
+              const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+              lo[e] = pack_h2(y0 - g.x, y1 - g.y);
+            }
+          }
+          const uint32_t at = static_cast<uint32_t>(l16 >> 3) * (kBN * 128) + sw128(rr & 127, l16 & 7);
+          *reinterpret_cast<uint4*>(tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if constexpr (LO)
+            *reinterpret_cast<uint4*>(tile + kTileB + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      return mine;
+    };
     for (; ok && walk.next(p, cum, w); ++pc) {
       const int n_tiles = w.t1 - w.t0;
-      const int qb = pc % C::kQBuf;
-      float m = -INFINITY, l = 0.0f, fac = 0.0f;
+      float m = -INFINITY, l = 0.0f, fac = 0.0f, vscale = 1.0f;
       if (n_tiles > 0) {
-        ok = wait_bar(&q_full[qb], (pc / C::kQBuf) & 1, abort);
+        if (w.rows > 128 * mt) fac = make_q();
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+        // two row tiles keep step from piece to piece: a tile without rows must not arrive for
+        // the next piece in this one's phase, nor look at a tile two ahead of the other's
+        if (NM > 1) ok = wait_bar(q_full, pc & 1, abort);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (r < w.rows) fac = facb[qb * MT + r];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_empty[qb]);
       }
       if (w.rows <= 128 * mt) {         // nothing for this row tile
         gt += n_tiles;
@@ -536,16 +740,18 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          const float* lv = lvb + slot * 2 * kBN;
+          const float* ev = eb + slot * 2 * kBN;
           const uint32_t s_addr = tmem + 128 * buf + lane_base;
           const int v0 = t * kBN;
+          const float2 ti = info[slot];
+          if (t == w.t0) vscale = ti.y;
           const bool need = v0 + kBN - 1 > lim.hi || (v0 < lim.lo && v0 + kBN > lim.vsk && lim.lo > lim.vsk);
-          if (__any_sync(0xffffffffu, need))
-            softmax_tile<true>(s_addr, o_addr, lv, fac, v0, lim, t == w.t0, &pv_done[mt], cnt,
-                               abort, m, l, ok);
+          const bool mask = __any_sync(0xffffffffu, need);
+          if (!LO && ti.x == 0.0f && !mask)
+            softmax_tile(s_addr, o_addr, fac, t == w.t0, &pv_done[mt], cnt, abort, m, l, ok);
           else
-            softmax_tile<false>(s_addr, o_addr, lv, fac, v0, lim, t == w.t0, &pv_done[mt], cnt,
-                                abort, m, l, ok);
+            softmax_tile_any(s_addr, o_addr, ev, fac, v0, lim, t == w.t0, &pv_done[mt], cnt, abort,
+                             m, l, ok);
         } else if (cnt > 0) {
           ok = wait_bar(&pv_done[mt], (cnt - 1) & 1, abort);
           ok = __all_sync(0xffffffffu, ok);
@@ -568,10 +774,10 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         const int h = w.kvh * p.nrep + (w.row0 + r) % p.nrep;
         char* dst = nullptr;
         float* prt = nullptr;
-        float scale = 1.0f;
+        float scale = vscale;           // 2^E
         if (w.slot < 0) {
           dst = out_row(p, w.b, u, h);
-          scale = have ? 1.0f / l : 0.0f;
+          scale = have ? vscale / l : 0.0f;
         } else {
           prt = part_row(p, w.seg, w.slot, r);
           if (live) {
@@ -598,7 +804,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               *reinterpret_cast<float4*>(prt + 4 + 32 * c + e) =
-                  have ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3])
+                  have ? make_float4(o[e] * scale, o[e + 1] * scale, o[e + 2] * scale, o[e + 3] * scale)
                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           }
         }
@@ -611,216 +817,182 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
     }
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
   } else if (warp < kMmaWarp) {
-    // ================= codes -> float16 tiles, q -> q'
+    // ================= staged codes -> float16 tiles
     const int ct = tid - C::kSoft;
-    const int c16 = ct & 7, row = ct >> 3;  // 16 codes of rows row + 32 i
+    const int c16 = ct & 7, row = ct >> 3;  // 16 codes of rows row + 16 i of a slot
     // where this thread's two 16-byte chunks go; the upper half of each 8 lanes stores its
     // second chunk first, so that 8 lanes write 8 different chunk columns
     const int first = c16 >> 2;
     const uint32_t blk = static_cast<uint32_t>(c16 >> 2) * (kBN * 128);
-    const int ch = (2 * c16) & 7;
-    struct Buf {
-      uint4 k[4], v[4];
-      float vs[4];
-    } bufs[2];
-    // cursor of the loads
-    Walk<MT, STREAM> lw = walk;
-    Piece lp;
-    lp.t0 = lp.t1 = 0;
-    int lt = 0;
-    const int8_t *kp = nullptr, *vp = nullptr;
-    int64_t vs0 = 0;
-    auto advance = [&]() -> bool {  // to the next tile to load
-      if (++lt < lp.t1) return true;
-      do {
-        if (!lw.next(p, cum, lp)) return false;
-      } while (lp.t0 >= lp.t1);
-      lt = lp.t0;
-      const Seg& s = p.seg[lp.seg];
-      const int64_t o = lp.b * s.sb + lp.kvh * s.sh + 16 * c16;
-      kp = s.k + o;
-      vp = s.v + o;
-      vs0 = lp.b * s.vscb + lp.kvh * s.vsch;
-      return true;
-    };
-    auto key_of = [&](int i, bool& in) -> int64_t {
-      const int v = lt * kBN + row + 32 * i;
-      in = v < lp.key.nv;
-      return v < lp.key.ns ? v : v + lp.key.sh;
-    };
-    auto load_k = [&](Buf& b) {
-      const Seg& s = p.seg[lp.seg];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        bool in;
-        const int64_t key = key_of(i, in);
-        b.k[i] = in ? ldg_stream(kp + key * s.ss) : make_uint4(0, 0, 0, 0);
-        b.vs[i] = in ? load_scale(s.vsc, vs0 + key * s.vscs, p.s_dt) : 0.0f;
-      }
-    };
-    auto load_v = [&](Buf& b) {
-      const Seg& s = p.seg[lp.seg];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        bool in;
-        const int64_t key = key_of(i, in);
-        b.v[i] = in ? ldg_stream(vp + key * s.ss) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    auto put = [&](unsigned char* tile, int rr, const uint4& x) {
-      uint4 a, b;
-      codes_to_h2(x.x, a.x, a.y);
-      codes_to_h2(x.y, a.z, a.w);
-      codes_to_h2(x.z, b.x, b.y);
-      codes_to_h2(x.w, b.z, b.w);
-      *reinterpret_cast<uint4*>(tile + blk + sw128(rr, ch + first)) = first ? b : a;
-      *reinterpret_cast<uint4*>(tile + blk + sw128(rr, ch + 1 - first)) = first ? a : b;
-    };
-    int pc = 0, gt = 0, ct0 = 0, ct1 = 0;  // pieces, tiles; tiles of the piece at hand
+    const uint32_t at0 = blk + sw128(row, ((2 * c16) & 7) + first);
+    const uint32_t at1 = blk + sw128(row, ((2 * c16) & 7) + 1 - first);
+    constexpr int NI = kSlotKeys / 16;
+    int sc = 0, gt = 0;  // slots, tiles
     bool ok = true;
-    // q' of the rows of piece w into buffer pc % kQBuf
-    auto make_q = [&]() {
-      const int qb = pc % C::kQBuf;
-      if (pc >= C::kQBuf) ok = wait_bar(&q_empty[qb], ((pc / C::kQBuf) - 1) & 1, abort);
-      if (!ok) return;
-      const Seg& s = p.seg[w.seg];
-      const int l16 = ct & 15, rg = ct >> 4;
-      float ks[8];
-      const int64_t k0 = w.b * s.kscb + w.kvh * s.ksch;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        ks[e] = load_scale(s.ksc, k0 + (8 * l16 + e) * s.kscd, p.s_dt) * p.qk_scale;
-#pragma unroll 2
-      for (int r0 = 0; r0 < w.rows; r0 += kConvThreads / 16) {
-        const int r = r0 + rg;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < w.rows) {
-          const int u = (w.row0 + r) / p.nrep, h = w.kvh * p.nrep + (w.row0 + r) % p.nrep;
-          x = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) +
-                                              2 * (w.b * s.qsb + u * s.qsu + h * p.qsh + 8 * l16));
-        }
-        float f[8];
-        if (p.q_dt == HQ_DTYPE_BF16) Vec16<HQ_DTYPE_BF16>::unpack(x, f);
-        else Vec16<HQ_DTYPE_F16>::unpack(x, f);
-        if (p.q_quant) {  // per-token int8 fake quantization, rounded back to the model dtype
-          float am = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(f[e]));
-#pragma unroll
-          for (int o = 8; o >= 1; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
-          const Quantizer qz = Quantizer::from_amax(am);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float y = static_cast<float>(qz.code(f[e])) * qz.scale;
-            f[e] = p.q_dt == HQ_DTYPE_BF16 ? __bfloat162float(__float2bfloat16_rn(y))
-                                           : __half2float(__float2half_rn(y));
-          }
-        }
-        float am = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f[e] *= ks[e];
-          am = fmaxf(am, fabsf(f[e]));
-        }
-#pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
-        // 2^ex brings am to [2^13, 2^14)
-        const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am) >> 23) - 127), -100), 100);
-        const float mul = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
-        if (r >= w.rows) continue;
-        if (l16 == 0)
-          facb[qb * MT + r] = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = f[2 * e] * mul, b = f[2 * e + 1] * mul;
-          hi[e] = pack_h2(a, b);
-          if constexpr (LO) {
-            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-            lo[e] = pack_h2(a - g.x, b - g.y);
-          }
-        }
-        unsigned char* tile = smem + (qb * NM + (r >> 7)) * C::kParts * kTileB;
-        const uint32_t at = static_cast<uint32_t>(l16 >> 3) * (kBN * 128) + sw128(r & 127, l16 & 7);
-        *reinterpret_cast<uint4*>(tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (LO)
-          *reinterpret_cast<uint4*>(tile + kTileB + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[qb]);
-      ++pc;
+    auto put = [&](unsigned char* tile, int i, const uint32_t (&x)[8]) {  // row + 16 i
+      const uint4 a = make_uint4(x[0], x[1], x[2], x[3]), b = make_uint4(x[4], x[5], x[6], x[7]);
+      *reinterpret_cast<uint4*>(tile + at0 + i * 2048) = first ? b : a;
+      *reinterpret_cast<uint4*>(tile + at1 + i * 2048) = first ? a : b;
     };
-    // tile gt from b into shared memory; b then takes the next tile to load
-    auto step = [&](Buf& b, bool& have) {
-      if (ct0 >= ct1) {  // a new piece (pieces without tiles have no q)
-        do {
-          if (!walk.next(p, cum, w)) {
-            ok = false;
-            return;
-          }
-          if (w.t0 >= w.t1) ++pc;
-        } while (w.t0 >= w.t1);
-        ct0 = w.t0;
-        ct1 = w.t1;
-        make_q();
-        if (!ok) return;
-      }
-      ++ct0;
-      const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
-      if (use > 0) ok = wait_bar(&k_empty[st], (use - 1) & 1, abort);
+    // the next staging slot into rows 64 half .. of a tile; V rows times their g
+    auto convert = [&](unsigned char* tile, int half, const __half* g) {
+      const int sl = sc % C::kSlots;
+      ok = wait_bar(&st_full[sl], (sc / C::kSlots) & 1, abort);
       if (!ok) return;
-      unsigned char* kt = smem + C::kOffK + st * kTileB;
-      unsigned char* vt = smem + C::kOffV + st * kTileB;
-      bool zero[4];
+      const unsigned char* src = smem + C::kOffSlot + sl * kSlotB + row * kD + 16 * c16;
+      uint4 x[NI];
+      uint32_t g2[NI];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        put(kt, row + 32 * i, b.k[i]);
-        zero[i] = b.vs[i] < 8.6736174e-19f;  // 2^-60: such a token's values are zeros
-        if (c16 == 0) {
-          const float x = zero[i] ? 8.6736174e-19f : b.vs[i];
-          lvb[slot * 2 * kBN + row + 32 * i] = __log2f(x);
-          lvb[slot * 2 * kBN + kBN + row + 32 * i] = 1.0f / x;
+      for (int i = 0; i < NI; ++i) {
+        x[i] = *reinterpret_cast<const uint4*>(src + i * 16 * kD);
+        if (g) {
+          const uint32_t h = *reinterpret_cast<const uint16_t*>(g + 64 * half + row + 16 * i);
+          g2[i] = h | h << 16;
         }
       }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&k_full[st]);
-        mbar_arrive(&lv_full[slot]);
-      }
-      have = advance();
-      if (have) load_k(b);
-      if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1, abort);
-      if (!ok) return;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        put(vt, row + 32 * i, zero[i] ? make_uint4(0, 0, 0, 0) : b.v[i]);
-      fence_async_smem();
+      for (int i = 0; i < NI; ++i) {
+        uint32_t y[8];
+        codes_to_h2(x[i].x, y[0], y[1]);
+        codes_to_h2(x[i].y, y[2], y[3]);
+        codes_to_h2(x[i].z, y[4], y[5]);
+        codes_to_h2(x[i].w, y[6], y[7]);
+        if (g) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y[e]) : "r"(y[e]), "r"(g2[i]));
+        }
+        put(tile, 4 * half + i, y);
+      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[st]);
-      if (have) load_v(b);
-      ++gt;
+      if (lane == 0) mbar_arrive(&st_empty[sl]);
+      ++sc;
     };
-    lt = -1;
-    bool have[2];
-    have[0] = advance();
-    if (have[0]) {
-      load_k(bufs[0]);
-      load_v(bufs[0]);
-    }
-    have[1] = have[0] && advance();
-    if (have[1]) {
-      load_k(bufs[1]);
-      load_v(bufs[1]);
-    }
-    while (ok && have[0]) {
-      step(bufs[0], have[0]);
-      if (!ok || !have[1]) break;
-      step(bufs[1], have[1]);
+    for (; ok && walk.next(p, cum, w);) {
+      for (int t = w.t0; t < w.t1; ++t, ++gt) {
+        const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
+        if (use > 0) ok = wait_bar(&k_empty[st], (use - 1) & 1, abort);
+        if (!ok) break;
+#pragma unroll 1
+        for (int half = 0; half < 2 && ok; ++half)
+          convert(smem + C::kOffK + st * kTileB, half, nullptr);
+        if (!ok) break;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_full[st]);
+        if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1, abort);
+        ok = ok && wait_bar(&lv_full[slot], (gt / kLvSlots) & 1, abort);
+        if (!ok) break;
+#pragma unroll 1
+        for (int half = 0; half < 2 && ok; ++half)
+          convert(smem + C::kOffV + st * kTileB, half, gb + slot * kBN);
+        if (!ok) break;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[st]);
+      }
     }
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
-  } else {
+  } else if (warp == kCopyWarp) {
+    // ================= codes into the staging ring, V scales into g_j and e_j
+    int sc = 0, gt = 0;
+    bool ok = true;
+    for (; ok && walk.next(p, cum, w);) {
+      const Seg& s = p.seg[w.seg];
+      const int8_t* base[2] = {s.k + w.b * s.sb + w.kvh * s.sh, s.v + w.b * s.sb + w.kvh * s.sh};
+      const int64_t vs0 = w.b * s.vscb + w.kvh * s.vsch;
+      int E = 0;
+      for (int t = w.t0; ok && t < w.t1; ++t, ++gt) {
+        float vs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int v = t * kBN + 32 * i + lane;
+          const int64_t key = v < w.key.ns ? v : v + w.key.sh;
+          vs[i] = v < w.key.nv ? load_scale(s.vsc, vs0 + key * s.vscs, p.s_dt) : -1.0f;
+        }
+#pragma unroll 1
+        for (int c = 0; ok && c < 4; ++c, ++sc) {  // K 0 .. 63, K 64 .., V 0 .., V 64 ..
+          const int sl = sc % C::kSlots, use = sc / C::kSlots;
+          if (use > 0) ok = wait_bar(&st_empty[sl], (use - 1) & 1, abort);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int v0 = t * kBN + (c & 1) * kSlotKeys;
+          const int n = min(max(w.key.nv - v0, 0), kSlotKeys);
+          unsigned char* dst = smem + C::kOffSlot + sl * kSlotB;
+          const int8_t* src = base[c >> 1];
+          if (lane == 0) mbar_arrive_expect_tx(&st_full[sl], n * kD);
+          __syncwarp();
+          if (s.ss == kD) {  // rows back to back: the sinks' run and the window's
+            const int n0 = min(max(w.key.ns - v0, 0), n);
+            if (lane == 0 && n0 > 0) bulk_g2s(dst, src + static_cast<int64_t>(v0) * kD, n0 * kD, &st_full[sl]);
+            if (lane == 0 && n > n0)
+              bulk_g2s(dst + n0 * kD, src + static_cast<int64_t>(v0 + n0 + w.key.sh) * kD,
+                       (n - n0) * kD, &st_full[sl]);
+          } else {
+            for (int i = lane; i < n; i += 32) {
+              const int v = v0 + i;
+              const int64_t key = v < w.key.ns ? v : v + w.key.sh;
+              bulk_g2s(dst + i * kD, src + key * s.ss, kD, &st_full[sl]);
+            }
+          }
+        }
+        if (!ok) break;
+        // slot gt % kLvSlots is free once P V of the tile two before is done
+        const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
+        if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float* ev = eb + slot * 2 * kBN;
+        bool any = LO;
+        if constexpr (LO) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool zero = vs[i] < kTinyScale;
+            const float x = zero ? kTinyScale : vs[i];
+            ev[32 * i + lane] = __log2f(x);
+            ev[kBN + 32 * i + lane] = __frcp_rn(x);
+            gb[slot * kBN + 32 * i + lane] = __float2half_rn(zero ? 0.0f : 1.0f);
+          }
+        } else {
+          int ex[4];
+          bool odd = false;
+          int top = -1000;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ex[i] = vs[i] < kTinyScale ? -60 : static_cast<int>(__float_as_uint(vs[i]) >> 23 & 255) - 127;
+            top = max(top, vs[i] < kTinyScale ? -1000 : ex[i]);
+          }
+          if (t == w.t0) {
+            top = __reduce_max_sync(0xffffffffu, top);
+            E = top == -1000 ? 0 : min(max(top, -100), 100);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ex[i] -= E;
+            odd = odd || (vs[i] >= 0.0f && (ex[i] < -4 || ex[i] > 6 || vs[i] < kTinyScale));
+          }
+          any = __any_sync(0xffffffffu, odd);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = any ? min(max(ex[i], -100), 100) : 0;
+            ev[32 * i + lane] = static_cast<float>(e);
+            ev[kBN + 32 * i + lane] = pow2i(-e);
+            // (two factors: the exponent of their product may leave float32's)
+            gb[slot * kBN + 32 * i + lane] =
+                __float2half_rn(vs[i] < kTinyScale ? 0.0f : vs[i] * pow2i(-E) * pow2i(-e));
+          }
+        }
+        if (lane == 0) info[slot] = make_float2(any ? 1.0f : 0.0f, pow2i(E));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&lv_full[slot]);
+      }
+    }
+    if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
+    // no copy is in flight when the block ends
+    for (int k = max(0, sc - C::kSlots); k < sc; ++k)
+      if (!mbar_wait(&st_full[k % C::kSlots], (k / C::kSlots) & 1))
+        report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
+  } else if (warp == kMmaWarp) {
     // ================= tensor-core products, issued by one thread
     if (lane == 0) {
       constexpr uint32_t id_s = idesc<HQ_DTYPE_F16>(128, 128, false);
@@ -829,17 +1001,18 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       int cntq[NM], cntp[NM], pieces[NM];  // S products, P V products, pieces of each row tile
       for (int i = 0; i < NM; ++i) cntq[i] = cntp[i] = pieces[i] = 0;
       // S = Q K^T of tile g for row tile m
-      auto qk = [&](int m, int qb, int g) {
+      auto qk = [&](int m, int g) {
         const uint32_t buf = NM == 1 ? (cntq[m] & 1) : m;
-        const uint32_t ka = k_base + (g % kStages) * kTileB;
-        const uint32_t qa = q_base + (qb * NM + m) * C::kParts * kTileB;
-#pragma unroll
+        const uint64_t dk = sdesc(k_base + (g % kStages) * kTileB, 16, 1024);
+        const uint64_t dq = sdesc(q_base + m * C::kParts * kTileB, 16, 1024);
+#pragma unroll 1
         for (int part = 0; part < C::kParts; ++part)
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk) {
-            const uint32_t off = (kk >> 2) * (kBN * 128) + (kk & 3) * 32;
-            mma_f16(tmem + 128 * buf, sdesc(qa + part * kTileB + off, 16, 1024),
-                    sdesc(ka + off, 16, 1024), id_s, part + kk > 0);
+            // (the address field counts 16 bytes; no sum leaves its 14 bits)
+            const uint32_t off = ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) >> 4;
+            mma_f16(tmem + 128 * buf, dq + (part * (kTileB >> 4) + off), dk + off, id_s,
+                    part + kk > 0);
           }
         mma_commit(&s_full[buf]);
         ++cntq[m];
@@ -851,11 +1024,11 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         if (first && pieces[m] > 0) ok = ok && wait_bar(&o_empty[m], (pieces[m] - 1) & 1, abort);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t va = v_base + (g % kStages) * kTileB;
+        const uint64_t dv = sdesc(v_base + (g % kStages) * kTileB, kBN * 128, 1024);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          mma_f16_ts(tmem + kColO + 128 * m, tmem + 128 * buf + 8 * kk,
-                     sdesc(va + kk * 16 * 128, kBN * 128, 1024), id_o, !first || kk > 0);
+          mma_f16_ts(tmem + kColO + 128 * m, tmem + 128 * buf + 8 * kk, dv + (kk * 16 * 128 >> 4),
+                     id_o, !first || kk > 0);
         mma_commit(&pv_done[m]);
         ++cntp[m];
         if (first) ++pieces[m];
@@ -865,55 +1038,64 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       Piece qp, cp;
       int qpc = -1, qt = 0, qg = 0;
       qp.t0 = qp.t1 = 0;
-      bool more = true;
-      auto q_next = [&]() {  // qp, qt: the next tile's piece and index; waits for its q and K
-        if (++qt >= qp.t1) {
-          do {
-            if (!qw.next(p, cum, qp)) {
-              more = false;
-              return;
-            }
-            ++qpc;
-          } while (qp.t0 >= qp.t1);
-          qt = qp.t0;
-          ok = ok && wait_bar(&q_full[qpc % C::kQBuf], (qpc / C::kQBuf) & 1, abort);
-        }
+      bool more = true, fresh = false;
+      auto q_next = [&]() {  // qp, qt: the next tile's piece and index
+        fresh = false;
+        if (++qt < qp.t1) return;
+        do {
+          if (!qw.next(p, cum, qp)) {
+            more = false;
+            return;
+          }
+        } while (qp.t0 >= qp.t1);
+        ++qpc;
+        qt = qp.t0;
+        fresh = true;
+      };
+      auto q_wait = [&]() {  // its q (of a piece's first tile) and K
+        if (fresh) ok = ok && wait_bar(q_full, qpc & 1, abort);
         ok = ok && wait_bar(&k_full[qg % kStages], (qg / kStages) & 1, abort);
         tc_fence_after();
       };
       auto q_done = [&]() {  // after the last S product of the tile
         mma_commit(&k_empty[qg % kStages]);
-        if (qt == qp.t1 - 1) mma_commit(&q_empty[qpc % C::kQBuf]);
         ++qg;
+      };
+      auto q_all = [&]() {
+        q_wait();
+        if (!ok) return;
+        for (int m = 0; m < NM; ++m)
+          if (qp.rows > 128 * m) qk(m, qg);
+        q_done();
       };
       qt = -1;
       q_next();
-      if (ok && more) {
-        for (int m = 0; m < NM; ++m)
-          if (qp.rows > 128 * m) qk(m, qpc % C::kQBuf, qg);
-        q_done();
-      }
+      if (more) q_all();
       int g = 0;  // tile of the P V products
       while (ok && more) {
         cp = qp;
         const int ctile = qt;
         q_next();
-        if (!ok) break;
-        if (NM == 1 && more) {
-          qk(0, qpc % C::kQBuf, qg);
-          q_done();
-        }
-        ok = wait_bar(&v_full[g % kStages], (g / kStages) & 1, abort);
+        // within a piece the next S goes out ahead of (one row tile) or between (two) the P V
+        // products; a piece's first S comes after them, since its q is made by the warps that
+        // wait for the last P V of the piece before
+        const bool ahead = more && !fresh;
+        if (ahead && NM == 1) q_all();
+        if (ahead && NM > 1) q_wait();
+        ok = ok && wait_bar(&v_full[g % kStages], (g / kStages) & 1, abort);
         if (!ok) break;
         for (int m = 0; m < NM; ++m) {
-          if (cp.rows > 128 * m) pv(m, g, ctile == cp.t0);
-          if (!ok) break;
-          // the next S of this row tile overwrites the P just read: the products run in order
-          if (NM > 1 && more && qp.rows > 128 * m) qk(m, qpc % C::kQBuf, qg);
+          if (cp.rows > 128 * m) {
+            pv(m, g, ctile == cp.t0);
+            if (!ok) break;
+            // the next S of this row tile overwrites the P just read: the products run in order
+            if (NM > 1 && ahead) qk(m, qg);
+          }
         }
         if (!ok) break;
         mma_commit(&v_empty[g % kStages]);
-        if (NM > 1 && more) q_done();
+        if (NM > 1 && ahead) q_done();
+        if (more && fresh) q_all();
         ++g;
       }
       if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);

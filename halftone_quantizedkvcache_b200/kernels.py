@@ -738,7 +738,7 @@ def set_plan_sms(sms: int, device=None) -> None:
     dev = torch.cuda.current_device() if device is None else torch.device(device).index
     check(_lib.lib().hq_set_plan_sms(int(dev), int(sms)), "hq_set_plan_sms")
     _decode_ws_bytes.clear()
-    _ragged_ws_bytes.clear()
+    _plans.clear()
 
 
 # ---------------------------------------------------------------- block-wise per-channel K
@@ -916,7 +916,6 @@ def kblock_dequant(cache: dict, S: int, dtype: torch.dtype = torch.float32) -> t
 
 # ---------------------------------------------------------------- ragged batches
 _ragged_status: dict = {}   # device index -> int32 [1] (first error sticks)
-_ragged_ws_bytes: dict = {}
 
 
 def _status_word(dev: torch.device) -> torch.Tensor:
@@ -955,19 +954,18 @@ def _on_device(dev: torch.device):
     return torch.cuda.device(dev)
 
 
-def _lens_ptr(what: str, name: str, t: torch.Tensor | None, n: int, dev: torch.device):
+def _lens_ok(what: str, name: str, t: torch.Tensor | None, n: int, dev: torch.device) -> None:
     if t is None:
-        return None
+        return
     _cuda(t, f"{what} {name}")
     if t.dtype != torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous() or t.device != dev:
         raise ValueError(f"{what}: {name} must be a contiguous int32 tensor of {n} elements on q's "
                          f"device, got {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr()
 
 
 def _int8_cache(what: str, B: int, D: int, dev, k, k_sc, v, v_sc, scale_dtype=None):
     """Checks an int8 cache (``[B,Hkv,S,D]`` codes sharing strides, K scales ``[B,Hkv,1,D]``, V
-    scales ``[B,Hkv,S,1]``) and returns the C arguments that describe it."""
+    scales ``[B,Hkv,S,1]``) and returns the C strides (codes, K scales, V scales)."""
     for t, n in ((k, "k"), (k_sc, "k_sc"), (v, "v"), (v_sc, "v_sc")):
         _cuda(t, f"{what} {n}")
         if t.device != dev:
@@ -989,14 +987,8 @@ def _int8_cache(what: str, B: int, D: int, dev, k, k_sc, v, v_sc, scale_dtype=No
                       or k.data_ptr() % 16 or v.data_ptr() % 16):
         raise ValueError(f"{what}: K/V rows must be contiguous and 16-byte aligned")
     ks, vs = k_sc.stride(), v_sc.stride()
-    return (k.data_ptr(), v.data_ptr(), _lib.strides(kst[:3], 3), k_sc.data_ptr(), v_sc.data_ptr(),
-            _DT[k_sc.dtype], _lib.strides((ks[0], ks[1], ks[3]), 3),
+    return (_lib.strides(kst[:3], 3), _lib.strides((ks[0], ks[1], ks[3]), 3),
             _lib.strides((vs[0], vs[1], vs[2]), 3))
-
-
-def _q16(what: str, q: torch.Tensor) -> None:
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"{what}: q must be bfloat16 or float16")
 
 
 def _out_like(what: str, out, shape, q: torch.Tensor) -> None:
@@ -1015,16 +1007,47 @@ def _window_args(what: str, window, sinks) -> tuple:
     return w, int(sinks)
 
 
-def _scratch(key, query, dev) -> torch.Tensor:
-    """Scratch of one call: nothing lives in it from call to call, so each call takes its own
-    from the allocator (calls on other streams and captured graphs never share it)."""
-    nb = _ragged_ws_bytes.get(key)
-    if nb is None:
-        nb = query(*key[2:])
-        if nb == 0:
-            raise ValueError(f"{key[0]}: unsupported shape")
-        _ragged_ws_bytes[key] = nb
-    return torch.empty(nb, dtype=torch.uint8, device=dev)
+# What a call's shapes, strides, types and devices lead to (checked arguments, C stride arrays,
+# scratch sizes), kept per combination: a decode step makes the same call for every layer and
+# token.  Nothing is kept by the tensors themselves.
+_plans: dict = {}
+_PLANS_MAX = 4096
+
+
+def _sig(*tensors) -> tuple:
+    return tuple([(t.shape, t.stride(), t.dtype, t.get_device()) if t is not None else None
+                  for t in tensors])
+
+
+def _keep(key, plan):
+    if len(_plans) >= _PLANS_MAX:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _tensors(what: str, **named) -> None:
+    for n, t in named.items():
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what}: {n} must be a tensor, got {type(t).__name__}")
+
+
+def _aligned_q(q: torch.Tensor) -> torch.Tensor:
+    """q with contiguous, 16-byte aligned rows (a copy where it has none)."""
+    return q if _rows_ok(q) else q.clone(memory_format=torch.contiguous_format)
+
+
+def _attn_common(what, q, Hq, Hkv) -> None:
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: q must be bfloat16 or float16")
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"{what}: {Hq} query heads over {Hkv} kv heads")
+
+
+def _ws_size(what: str, dev, nbytes: int) -> int:
+    if nbytes == 0:
+        raise ValueError(f"{what}: unsupported shape")
+    return nbytes
 
 
 def int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sinks=0,
@@ -1036,44 +1059,55 @@ def int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sin
     ``[B,Hkv,cap,D]``, k_sc ``[B,Hkv,1,D]``, v_sc ``[B,Hkv,cap,1]`` (f16/f32); ``lens`` int32
     ``[B]`` on the device: the tokens each sequence holds, its newest being the query's own.
     Sequence b sees token j < lens[b] when ``j >= lens[b] - window`` or ``j < sinks``
-    (``window=None``: every token).  Rows past ``lens[b]`` are never read; an empty sequence
-    gives zeros.  Returns the output in q's layout and dtype (or writes ``out [B,Hq,D]``).
-    ``q_quant``: the per-token fake quantization of ``int8_decode_attn``.  Nothing depends on
-    ``lens`` on the host, so the call replays in a CUDA graph while sequences grow.
+    (``window=None``: every token).  What rows past ``lens[b]`` hold does not matter; an empty
+    sequence gives zeros.  Returns the output in q's layout and dtype (or writes
+    ``out [B,Hq,D]``).  ``q_quant``: the per-token fake quantization of ``int8_decode_attn``.
+    Nothing depends on ``lens`` on the host, so the call replays in a CUDA graph while
+    sequences grow.
     """
     what = "int8_window_decode_attn"
-    _cuda(q, f"{what} q")
-    qb, restore = _as_bhd(q)
-    _q16(what, qb)
-    qb = qb if _rows_ok(qb) else qb.contiguous()
-    B, Hq, D = qb.shape
-    dev = qb.device
-    cache = _int8_cache(what, B, D, dev, k_i8, k_sc, v_i8, v_sc)
-    Hkv, cap = k_i8.shape[1], k_i8.shape[2]
-    w, sinks = _window_args(what, window, sinks)
-    if lens is None:
-        raise ValueError(f"{what}: lens is needed")
-    lp = _lens_ptr(what, "lens", lens, B, dev)
-    if Hkv == 0 or Hq % Hkv:
-        raise ValueError(f"{what}: {Hq} query heads over {Hkv} kv heads")
+    _tensors(what, q=q, k_i8=k_i8, k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens)
+    key = (what, window, sinks, _sig(q, k_i8, k_sc, v_i8, v_sc, lens))
+    plan = _plans.get(key)
+    if plan is None:
+        _cuda(q, f"{what} q")
+        qb, _ = _as_bhd(q)
+        B, Hq, D = qb.shape
+        dev = qb.device
+        st = _int8_cache(what, B, D, dev, k_i8, k_sc, v_i8, v_sc)
+        Hkv, cap = k_i8.shape[1], k_i8.shape[2]
+        _attn_common(what, q, Hq, Hkv)
+        w, sk = _window_args(what, window, sinks)
+        _lens_ok(what, "lens", lens, B, dev)
+        qb = _aligned_q(qb)
+        dt = _DT[qb.dtype]
+        with _on_device(dev):
+            nb = _ws_size(what, dev, _lib.lib().hq_window_workspace_bytes(
+                dt, max(B, 1), Hq, Hkv, 0, cap, D, w, sk))
+        plan = _keep(key, (dev, (B, Hq, D), q.shape, dt, _lib.strides(qb.stride(), 3), st,
+                           _DT[k_sc.dtype], Hkv, cap, w, sk, nb, _lib.strides((Hq * D, D, 1), 3)))
+    dev, (B, Hq, D), shape, dt, qst, st, sdt, Hkv, cap, w, sk, nb, ost = plan
+    if q.data_ptr() % 16 or q.stride(-1) != 1 or any(s % 8 for s in q.stride()[:-1]):
+        q = _aligned_q(q)  # the strides of the copy are those of the plan's copy
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    if out is not None:
-        _out_like(what, out, (B, Hq, D), qb)
     with _on_device(dev):
-        res = out if out is not None else torch.empty((B, Hq, D), dtype=qb.dtype, device=dev)
+        if out is None:
+            res = torch.empty(shape, dtype=q.dtype, device=dev)
+        else:
+            _out_like(what, out, (B, Hq, D), q)
+            res, ost = out, _lib.strides(out.stride(), 3)
         if B == 0:
-            return restore(res) if out is None else res
-        dt = _DT[qb.dtype]
-        ws = _scratch((what, dev.index, dt, B, Hq, Hkv, 0, cap, D, w, sinks),
-                      _lib.lib().hq_window_workspace_bytes, dev)
+            return res
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         rc = _lib.lib().hq_window_decode_int8(
-            qb.data_ptr(), dt, _lib.strides(qb.stride(), 3), *cache, lp, B, Hq, Hkv, cap, D, w,
-            sinks, float(sm_scale), int(bool(q_quant)), res.data_ptr(),
-            _lib.strides(res.stride(), 3), ws.data_ptr(), ws.numel(), _status_word(dev).data_ptr(),
-            _stream(dev))
-    check(rc, "hq_window_decode_int8")
-    return restore(res) if out is None else res
+            q.data_ptr(), dt, qst, k_i8.data_ptr(), v_i8.data_ptr(), st[0], k_sc.data_ptr(),
+            v_sc.data_ptr(), sdt, st[1], st[2], lens.data_ptr(), B, Hq, Hkv, cap, D, w, sk, sm_scale,
+            1 if q_quant else 0, res.data_ptr(), ost, ws.data_ptr(), nb,
+            _status_word(dev).data_ptr(), _stream(dev))
+    if rc:
+        check(rc, "hq_window_decode_int8")
+    return res
 
 
 def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sinks=0,
@@ -1090,41 +1124,50 @@ def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, si
     they were in ``out``.  Queries at a position below 0 give zeros.
     """
     what = "int8_window_prefill_attn"
-    _cuda(q, f"{what} q")
-    if q.dim() != 4:
-        raise ValueError(f"{what}: q must be [B,Hq,Sq,D]")
-    _q16(what, q)
-    q = q if _rows_ok(q) else q.contiguous()
-    B, Hq, Sq, D = q.shape
-    dev = q.device
-    cache = _int8_cache(what, B, D, dev, k_i8, k_sc, v_i8, v_sc)
-    Hkv, cap = k_i8.shape[1], k_i8.shape[2]
-    w, sinks = _window_args(what, window, sinks)
-    if lens is None:
-        raise ValueError(f"{what}: lens is needed")
-    lp, qlp = _lens_ptr(what, "lens", lens, B, dev), _lens_ptr(what, "q_lens", q_lens, B, dev)
-    if Hkv == 0 or Hq % Hkv:
-        raise ValueError(f"{what}: {Hq} query heads over {Hkv} kv heads")
+    _tensors(what, q=q, k_i8=k_i8, k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens)
+    key = (what, window, sinks, _sig(q, k_i8, k_sc, v_i8, v_sc, lens, q_lens))
+    plan = _plans.get(key)
+    if plan is None:
+        _cuda(q, f"{what} q")
+        if q.dim() != 4:
+            raise ValueError(f"{what}: q must be [B,Hq,Sq,D]")
+        B, Hq, Sq, D = q.shape
+        dev = q.device
+        st = _int8_cache(what, B, D, dev, k_i8, k_sc, v_i8, v_sc)
+        Hkv, cap = k_i8.shape[1], k_i8.shape[2]
+        _attn_common(what, q, Hq, Hkv)
+        w, sk = _window_args(what, window, sinks)
+        _lens_ok(what, "lens", lens, B, dev)
+        _lens_ok(what, "q_lens", q_lens, B, dev)
+        dt = _DT[q.dtype]
+        with _on_device(dev):
+            nb = _ws_size(what, dev, _lib.lib().hq_window_workspace_bytes(
+                dt, max(B, 1), Hq, Hkv, max(Sq, 1), cap, D, w, sk))
+        plan = _keep(key, (dev, (B, Sq, Hq, D), dt, st, _DT[k_sc.dtype], Hkv, cap, w, sk, nb))
+    dev, shape, dt, st, sdt, Hkv, cap, w, sk, nb = plan
+    B, Sq, Hq, D = shape
+    q = _aligned_q(q)
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    if out is not None:
-        _out_like(what, out, (B, Sq, Hq, D), q)
     with _on_device(dev):
         if out is None:
             make = torch.empty if q_lens is None else torch.zeros
-            out = make((B, Sq, Hq, D), dtype=q.dtype, device=dev)
+            out = make(shape, dtype=q.dtype, device=dev)
+        else:
+            _out_like(what, out, shape, q)
         if B == 0 or Sq == 0:
             return out
-        dt = _DT[q.dtype]
-        ws = _scratch((what, dev.index, dt, B, Hq, Hkv, Sq, cap, D, w, sinks),
-                      _lib.lib().hq_window_workspace_bytes, dev)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         os_ = out.stride()
         rc = _lib.lib().hq_window_prefill_int8(
-            q.data_ptr(), dt, _lib.strides(q.stride(), 4), *cache, lp, qlp, B, Hq, Hkv, Sq, cap, D,
-            w, sinks, float(sm_scale), int(bool(q_quant)), out.data_ptr(),
-            _lib.strides((os_[0], os_[2], os_[1], os_[3]), 4), ws.data_ptr(), ws.numel(),
+            q.data_ptr(), dt, _lib.strides(q.stride(), 4), k_i8.data_ptr(), v_i8.data_ptr(), st[0],
+            k_sc.data_ptr(), v_sc.data_ptr(), sdt, st[1], st[2], lens.data_ptr(),
+            q_lens.data_ptr() if q_lens is not None else None, B, Hq, Hkv, Sq, cap, D, w, sk,
+            sm_scale, 1 if q_quant else 0, out.data_ptr(),
+            _lib.strides((os_[0], os_[2], os_[1], os_[3]), 4), ws.data_ptr(), nb,
             _status_word(dev).data_ptr(), _stream(dev))
-    check(rc, "hq_window_prefill_int8")
+    if rc:
+        check(rc, "hq_window_prefill_int8")
     return out
 
 
@@ -1141,43 +1184,58 @@ def int8_prefix_decode_attn(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_s
     are held; the output is the attention over both, and zeros where there is none.
     """
     what = "int8_prefix_decode_attn"
-    _cuda(q, f"{what} q")
-    qb, restore = _as_bhd(q)
-    _q16(what, qb)
-    qb = qb if _rows_ok(qb) else qb.contiguous()
-    B, Hq, D = qb.shape
-    dev = qb.device
-    _cuda(pk_i8, f"{what} pk")
-    G = pk_i8.shape[0]
-    if G < 1 or B % G:
-        raise ValueError(f"{what}: {B} sequences over {G} prefixes")
-    pre = _int8_cache(f"{what} prefix", G, D, dev, pk_i8, pk_sc, pv_i8, pv_sc)
-    own = _int8_cache(what, B, D, dev, k_i8, k_sc, v_i8, v_sc, pk_sc.dtype)
-    Hkv, cap, P = k_i8.shape[1], k_i8.shape[2], pk_i8.shape[2]
-    if pk_i8.shape[1] != Hkv or Hkv == 0 or Hq % Hkv:
-        raise ValueError(f"{what}: {Hq} query heads over {Hkv} kv heads, {pk_i8.shape[1]} in the prefix")
-    if lens is None:
-        raise ValueError(f"{what}: lens is needed")
-    lp = _lens_ptr(what, "lens", lens, B, dev)
-    plp = _lens_ptr(what, "prefix_lens", prefix_lens, G, dev)
+    _tensors(what, q=q, pk_i8=pk_i8, pk_sc=pk_sc, pv_i8=pv_i8, pv_sc=pv_sc, k_i8=k_i8, k_sc=k_sc,
+             v_i8=v_i8, v_sc=v_sc, lens=lens)
+    key = (what, _sig(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_sc, lens, prefix_lens))
+    plan = _plans.get(key)
+    if plan is None:
+        _cuda(q, f"{what} q")
+        qb, _ = _as_bhd(q)
+        B, Hq, D = qb.shape
+        dev = qb.device
+        _cuda(pk_i8, f"{what} pk")
+        G = pk_i8.shape[0] if pk_i8.dim() == 4 else 0
+        if G < 1 or B % G:
+            raise ValueError(f"{what}: {B} sequences over {G} prefixes")
+        pst = _int8_cache(f"{what} prefix", G, D, dev, pk_i8, pk_sc, pv_i8, pv_sc)
+        st = _int8_cache(what, B, D, dev, k_i8, k_sc, v_i8, v_sc, pk_sc.dtype)
+        Hkv, cap, P = k_i8.shape[1], k_i8.shape[2], pk_i8.shape[2]
+        _attn_common(what, q, Hq, Hkv)
+        if pk_i8.shape[1] != Hkv:
+            raise ValueError(f"{what}: {Hkv} kv heads, {pk_i8.shape[1]} in the prefix")
+        _lens_ok(what, "lens", lens, B, dev)
+        _lens_ok(what, "prefix_lens", prefix_lens, G, dev)
+        qb = _aligned_q(qb)
+        dt = _DT[qb.dtype]
+        with _on_device(dev):
+            nb = _ws_size(what, dev, _lib.lib().hq_prefix_decode_workspace_bytes(
+                dt, G, max(B, G), Hq, Hkv, P, cap, D))
+        plan = _keep(key, (dev, (B, Hq, D), q.shape, dt, _lib.strides(qb.stride(), 3), pst, st, G,
+                           P, _DT[k_sc.dtype], Hkv, cap, nb, _lib.strides((Hq * D, D, 1), 3)))
+    dev, (B, Hq, D), shape, dt, qst, pst, st, G, P, sdt, Hkv, cap, nb, ost = plan
+    if q.data_ptr() % 16 or q.stride(-1) != 1 or any(s % 8 for s in q.stride()[:-1]):
+        q = _aligned_q(q)  # the strides of the copy are those of the plan's copy
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    if out is not None:
-        _out_like(what, out, (B, Hq, D), qb)
     with _on_device(dev):
-        res = out if out is not None else torch.empty((B, Hq, D), dtype=qb.dtype, device=dev)
+        if out is None:
+            res = torch.empty(shape, dtype=q.dtype, device=dev)
+        else:
+            _out_like(what, out, (B, Hq, D), q)
+            res, ost = out, _lib.strides(out.stride(), 3)
         if B == 0:
-            return restore(res) if out is None else res
-        dt = _DT[qb.dtype]
-        ws = _scratch((what, dev.index, dt, G, B, Hq, Hkv, P, cap, D),
-                      _lib.lib().hq_prefix_decode_workspace_bytes, dev)
+            return res
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         rc = _lib.lib().hq_prefix_decode_int8(
-            qb.data_ptr(), dt, _lib.strides(qb.stride(), 3), *pre[:5], *pre[6:], plp, G, P,
-            *own[:5], *own[6:], lp, cap, own[5], B, Hq, Hkv, D, float(sm_scale),
-            int(bool(q_quant)), res.data_ptr(), _lib.strides(res.stride(), 3), ws.data_ptr(),
-            ws.numel(), _status_word(dev).data_ptr(), _stream(dev))
-    check(rc, "hq_prefix_decode_int8")
-    return restore(res) if out is None else res
+            q.data_ptr(), dt, qst, pk_i8.data_ptr(), pv_i8.data_ptr(), pst[0], pk_sc.data_ptr(),
+            pv_sc.data_ptr(), pst[1], pst[2],
+            prefix_lens.data_ptr() if prefix_lens is not None else None, G, P, k_i8.data_ptr(),
+            v_i8.data_ptr(), st[0], k_sc.data_ptr(), v_sc.data_ptr(), st[1], st[2],
+            lens.data_ptr(), cap, sdt, B, Hq, Hkv, D, sm_scale, 1 if q_quant else 0,
+            res.data_ptr(), ost, ws.data_ptr(), nb, _status_word(dev).data_ptr(), _stream(dev))
+    if rc:
+        check(rc, "hq_prefix_decode_int8")
+    return res
 
 
 def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, *, scaling: str | None = None,
@@ -1236,58 +1294,69 @@ def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache
     fit its capacity writes nothing and sets ``ragged_status()``.
     """
     what = "rope_append_kv"
-    for t, n in ((q, "q"), (k_new, "k_new"), (v_new, "v_new"), (inv_freq, "inv_freq"),
-                 (k_cache, "k_cache"), (v_cache, "v_cache"), (k_sc, "k_sc"),
-                 (v_sc_cache, "v_sc_cache")):
-        _cuda(t, f"{what} {n}")
-        if t.device != q.device:
-            raise ValueError(f"{what}: {n} is on {t.device}, q on {q.device}")
-    if q.dim() != 4 or k_new.dim() != 4 or k_new.shape != v_new.shape:
-        raise ValueError(f"{what}: q [B,Hq,S,D] and k_new, v_new [B,Hkv,S,D] expected")
-    B, Hq, S, D = q.shape
-    Hkv, cap = k_new.shape[1], k_cache.shape[2] if k_cache.dim() == 4 else -1
-    dt = _dtype_code(q, what)
-    if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
-        raise TypeError(f"{what}: q, k_new and v_new must have one dtype")
-    if (k_new.shape[0], k_new.shape[2], k_new.shape[3]) != (B, S, D):
-        raise ValueError(f"{what}: k_new {tuple(k_new.shape)} does not fit q {tuple(q.shape)}")
-    for t in (k_cache, v_cache):
-        if tuple(t.shape) != (B, Hkv, cap, D) or t.dtype != torch.int8:
-            raise ValueError(f"{what}: caches must be int8 [B,Hkv,cap,D]")
-    if k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1 or any(
-            s % 16 for s in k_cache.stride()[:3]) or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
-        raise ValueError(f"{what}: K/V caches must share strides, with contiguous, 16-byte aligned rows")
-    if tuple(v_sc_cache.shape) != (B, Hkv, cap, 1):
-        raise ValueError(f"{what}: v_sc_cache must be [B,Hkv,cap,1]")
-    if k_sc.dtype != v_sc_cache.dtype or k_sc.dtype not in (torch.float16, torch.float32):
-        raise TypeError(f"{what}: scales must both be float16 or float32")
-    _, kst = _static_scale(k_sc, B, Hkv, D, what)
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or (
-            2 * inv_freq.numel() > D):
-        raise ValueError(f"{what}: inv_freq must be contiguous float32 of at most D / 2 elements")
-    dev = q.device
-    if lens is None:
-        raise ValueError(f"{what}: lens is needed")
-    lp = _lens_ptr(what, "lens", lens, B, dev)
-    nnp = _lens_ptr(what, "n_new", n_new, B, dev)
-    pop = _lens_ptr(what, "pos_offset", pos_offset, B, dev)
-    if q_out is None:
-        q, k_new, v_new = _rowmajor(q), _rowmajor(k_new), _rowmajor(v_new)
-    else:
-        k_new, v_new = _rowmajor(k_new), _rowmajor(v_new)
-        if q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != dev or not _rows_ok(q_out):
-            raise ValueError(f"{what}: q_out must have q's shape, dtype and device, with 16-byte "
+    _tensors(what, q=q, k_new=k_new, v_new=v_new, inv_freq=inv_freq, k_cache=k_cache,
+             v_cache=v_cache, k_sc=k_sc, v_sc_cache=v_sc_cache, lens=lens)
+    key = (what, _sig(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache, lens, n_new,
+                      pos_offset))
+    plan = _plans.get(key)
+    if plan is None:
+        for t, n in ((q, "q"), (k_new, "k_new"), (v_new, "v_new"), (inv_freq, "inv_freq"),
+                     (k_cache, "k_cache"), (v_cache, "v_cache"), (k_sc, "k_sc"),
+                     (v_sc_cache, "v_sc_cache")):
+            _cuda(t, f"{what} {n}")
+            if t.device != q.device:
+                raise ValueError(f"{what}: {n} is on {t.device}, q on {q.device}")
+        if q.dim() != 4 or k_new.dim() != 4 or k_new.shape != v_new.shape or k_cache.dim() != 4:
+            raise ValueError(f"{what}: q [B,Hq,S,D], k_new and v_new [B,Hkv,S,D] and caches "
+                             "[B,Hkv,cap,D] expected")
+        B, Hq, S, D = q.shape
+        Hkv, cap = k_new.shape[1], k_cache.shape[2]
+        dt = _dtype_code(q, what)
+        if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
+            raise TypeError(f"{what}: q, k_new and v_new must have one dtype")
+        if (k_new.shape[0], k_new.shape[2], k_new.shape[3]) != (B, S, D):
+            raise ValueError(f"{what}: k_new {tuple(k_new.shape)} does not fit q {tuple(q.shape)}")
+        if Hkv < 1:
+            raise ValueError(f"{what}: no kv heads")
+        for t in (k_cache, v_cache):
+            if tuple(t.shape) != (B, Hkv, cap, D) or t.dtype != torch.int8:
+                raise ValueError(f"{what}: caches must be int8 [B,Hkv,cap,D]")
+        cst = k_cache.stride()
+        if cst != v_cache.stride() or cst[3] != 1 or any(s % 16 for s in cst[:3]):
+            raise ValueError(f"{what}: K/V caches must share strides, with contiguous, 16-byte "
                              "aligned rows")
-        q = _rowmajor(q)
+        if tuple(v_sc_cache.shape) != (B, Hkv, cap, 1):
+            raise ValueError(f"{what}: v_sc_cache must be [B,Hkv,cap,1]")
+        if k_sc.dtype != v_sc_cache.dtype or k_sc.dtype not in (torch.float16, torch.float32):
+            raise TypeError(f"{what}: scales must both be float16 or float32")
+        _, kst = _static_scale(k_sc, B, Hkv, D, what)
+        if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or (
+                not inv_freq.is_contiguous() or 2 * inv_freq.numel() > D):
+            raise ValueError(f"{what}: inv_freq must be contiguous float32 of at most D / 2 elements")
+        dev = q.device
+        _lens_ok(what, "lens", lens, B, dev)
+        _lens_ok(what, "n_new", n_new, B, dev)
+        _lens_ok(what, "pos_offset", pos_offset, B, dev)
+        plan = _keep(key, (dev, (B, Hq, S, D), dt, Hkv, 2 * inv_freq.numel(), _DT[k_sc.dtype], kst,
+                           _lib.strides(cst[:3], 3), _lib.strides(v_sc_cache.stride()[:3], 3), cap))
+    dev, shape, dt, Hkv, rot, sdt, kst, cst, vst, cap = plan
+    B, Hq, S, D = shape
+    if q_out is not None and (q_out.shape != shape or q_out.dtype != q.dtype or
+                              q_out.device != dev or not _rows_ok(q_out)):
+        raise ValueError(f"{what}: q_out must have q's shape, dtype and device, with 16-byte "
+                         "aligned rows")
+    q, k_new, v_new = _aligned_q(q), _aligned_q(k_new), _aligned_q(v_new)
     with _on_device(dev):
-        res = q_out if q_out is not None else torch.empty((B, Hq, S, D), dtype=q.dtype, device=dev)
+        res = q_out if q_out is not None else torch.empty(shape, dtype=q.dtype, device=dev)
         rc = _lib.lib().hq_rope_append_kv(
             q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), dt, _lib.strides(q.stride(), 4),
             _lib.strides(k_new.stride(), 4), _lib.strides(v_new.stride(), 4), B, Hq, Hkv, S, D,
-            inv_freq.data_ptr(), 2 * inv_freq.numel(), int(bool(interleaved)), float(factor), lp,
-            nnp, pop, k_sc.data_ptr(), _DT[k_sc.dtype], kst, k_cache.data_ptr(),
-            v_cache.data_ptr(), _lib.strides(k_cache.stride()[:3], 3), v_sc_cache.data_ptr(),
-            _lib.strides(v_sc_cache.stride()[:3], 3), cap, res.data_ptr(),
-            _lib.strides(res.stride(), 4), _status_word(dev).data_ptr(), _stream(dev))
-    check(rc, "hq_rope_append_kv")
+            inv_freq.data_ptr(), rot, 1 if interleaved else 0, factor, lens.data_ptr(),
+            n_new.data_ptr() if n_new is not None else None,
+            pos_offset.data_ptr() if pos_offset is not None else None, k_sc.data_ptr(), sdt, kst,
+            k_cache.data_ptr(), v_cache.data_ptr(), cst, v_sc_cache.data_ptr(), vst, cap,
+            res.data_ptr(), _lib.strides(res.stride(), 4), _status_word(dev).data_ptr(),
+            _stream(dev))
+    if rc:
+        check(rc, "hq_rope_append_kv")
     return res

@@ -2,12 +2,15 @@
 and shared-prefix decode, against the definitions in float64.
 
 Tolerance, derived from the arithmetic.  Write z_j for the scores, p_j for the softmax, v_j for
-the dequantized values, u = 2^-11 (half a step of float16).  The kernel rounds q' once to
-float16 (bf16 models: |dz_j| <= u sum_d |q_d k_jd| sm_scale; float16 models keep a second part,
-u^2) and P once (u P).  Weights off by a relative dz change a normalised sum by 2 dz at most, so
-    |out - ref| <= eps_out / 2 |ref| + A (u + 2 Z dq + 2^-16 (1 + Z)),
-A = sum_j p_j |v_j|, Z = max_j sum_d |q_d k_jd| sm_scale, dq = u or u^2; the last term covers
-float32 accumulation (128 products, up to 2^13 keys) and the approximate exp2 (2^-22 each).
+the dequantized values, u = 2^-11 (half a step of float16).  The kernel rounds P to float16
+once (u P); float16 models keep q' in two float16 parts (|dz_j| <= u^2 sum_d |q_d k_jd|
+sm_scale) and V exact, bf16 models q' in one (u in place of u^2) and V as a float16 product of
+the code and a float16 scale (2 u).  Weights off by a relative dz change a normalised sum by
+2 dz at most, so
+    |out - ref| <= eps_out / 2 |ref| + A (r u + 2 Z dq + 2^-16 (1 + Z)),
+A = sum_j p_j |v_j|, Z = max_j sum_d |q_d k_jd| sm_scale, r = 1 or 3, dq = u^2 or u; the last
+term covers float32 accumulation (128 products, up to 2^13 keys) and the approximate exp2
+(2^-22 each).
 """
 import math
 
@@ -53,8 +56,8 @@ def ref_rows(q, k, v, seen, dt):
     out = p @ v
     a = p @ v.abs()
     zabs = torch.where(seen, (q.abs() @ k.abs().T) * sm, torch.zeros_like(z)).amax(-1, keepdim=True)
-    dq = U if dt == "bf16" else U * U
-    tol = torch.finfo(TDT[dt]).eps / 2 * out.abs() + a * (U + 2 * zabs * dq + 2.0 ** -16 * (1 + zabs))
+    dq, r = (U, 3) if dt == "bf16" else (U * U, 1)
+    tol = torch.finfo(TDT[dt]).eps / 2 * out.abs() + a * (r * U + 2 * zabs * dq + 2.0 ** -16 * (1 + zabs))
     return out, tol + 1e-30
 
 

@@ -36,8 +36,8 @@
 // Roles of a block (one per SM): softmax warps (4 per row tile, one thread per row; they also
 // form q'), 4 warps that turn staged codes into float16 with byte permutes and store them in
 // the 128-byte-swizzled layouts the MMA reads, one warp that fills the staging ring with bulk
-// copies (64 keys of K or V per slot) and reads the V scales, and one whose first lane issues
-// the tcgen05.mma products: S = Q K^T into tensor memory, O += P V with P read from tensor
+// copies (64 keys of K or V per slot), one that reads the V scales, and one that issues the
+// tcgen05.mma products: S = Q K^T into tensor memory, O += P V with P read from tensor
 // memory, where it overwrites the S it came from.  mbarriers order the roles; every wait is
 // bounded.  (Codes loaded into registers and converted from there took 4000 cycles a tile:
 // the proxy fence before each hand-over waited for the loads of the next tile.)
@@ -110,7 +110,7 @@ struct Params {
 template <int NM, bool LO>
 struct Cfg {
   static constexpr int kSoft = 128 * NM;
-  static constexpr int kThreads = kSoft + kConvThreads + 64;
+  static constexpr int kThreads = kSoft + kConvThreads + 96;
   static constexpr int kParts = LO ? 2 : 1;
   static constexpr int kSlots = NM * kParts == 1 ? 7 : 3;          // staging: 8 KB each
   static constexpr int kOffK = NM * kParts * kTileB;
@@ -119,7 +119,8 @@ struct Cfg {
   static constexpr int kOffE = kOffSlot + kSlots * kSlotB;         // [slot][e_j, 2^-e_j][128]
   static constexpr int kOffG = kOffE + kLvSlots * 2 * kBN * 4;     // [slot][128] float16 g_j
   static constexpr int kOffInfo = kOffG + kLvSlots * kBN * 2;      // [slot]{any e_j, 2^E}
-  static constexpr int kOffBar = kOffInfo + kLvSlots * 8;
+  static constexpr int kOffKs = kOffInfo + kLvSlots * 8;           // [128] k_scale sm_scale log2 e
+  static constexpr int kOffBar = kOffKs + kD * 4;
   static constexpr int kBars = 1 + 4 * kStages + 2 * kSlots + kLvSlots + 2 + 2 + 2 * NM + 1;
   static constexpr int kOffMisc = kOffBar + ((kBars * 8 + 15) & ~15);
   static constexpr int kOffCum = kOffMisc + 16;
@@ -137,6 +138,21 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+      : "memory");
+}
 constexpr float kTinyScale = 8.6736174e-19f;  // 2^-60: V scales below count as zero
 __device__ __forceinline__ float pow2i(int e) {  // 2^e, -126 <= e <= 127
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
@@ -148,6 +164,11 @@ __device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t& a, uint32_t& b
   const uint32_t x = prmt(u, 0x64646464u, 0x4140u), y = prmt(u, 0x64646464u, 0x4342u);
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(a) : "r"(x), "r"(k1152));
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(b) : "r"(y), "r"(k1152));
+}
+__device__ __forceinline__ bool elect_one() {  // one lane of a converged warp
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
 }
 __device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db,
                                            uint32_t id, uint32_t accumulate) {
@@ -252,72 +273,74 @@ __device__ __forceinline__ int entry_tiles(const Params& p, int e) {
 }
 __device__ __host__ __forceinline__ int row_tiles(int rows, int mt) { return (rows + mt - 1) / mt; }
 
-// The pieces of one block, in order.
-template <int MT, bool STREAM>
+// The pieces of one block, in order.  (A call: every role walks them.)
 struct Walk {
   int cur, end, e;
-  __device__ __forceinline__ void start(const Params& p, const int* cum) {
-    if constexpr (STREAM) {
-      const int ne = p.seg[0].nb + (p.nseg > 1 ? p.seg[1].nb : 0);
-      const int total = cum[ne];
-      const int per = max(p.min_tiles, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-      cur = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total)));
-      end = static_cast<int>(min(static_cast<int64_t>(cur) + per, static_cast<int64_t>(total)));
-      // the entry that holds tile cur: cum[e] <= cur < cum[e + 1]
-      int lo = 0, hi = ne - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (cum[mid] <= cur) lo = mid; else hi = mid - 1;
-      }
-      e = lo;
-    } else {
-      cur = 0;
-      end = 1;
-    }
-  }
-  __device__ __forceinline__ bool next(const Params& p, const int* cum, Piece& w) {
-    if (cur >= end) return false;
-    if constexpr (STREAM) {
-      while (cum[e + 1] <= cur) ++e;
-      w.seg = e < p.seg[0].nb ? 0 : 1;
-      const Seg& s = p.seg[w.seg];
-      w.b = e - (w.seg ? p.seg[0].nb : 0);
-      const int rows = s.units * p.nrep, n_rt = row_tiles(rows, MT), per_e = p.Hkv * n_rt;
-      const int nt = (cum[e + 1] - cum[e]) / per_e;
-      const int idx = (cur - cum[e]) / nt, first = cum[e] + idx * nt;
-      const int rt = idx / p.Hkv;
-      w.kvh = idx - rt * p.Hkv;
-      w.row0 = rt * MT;
-      w.rows = min(MT, rows - w.row0);
-      w.key = make_keys(s, seg_len(s, w.b), s.units, 0, 0);
-      w.t0 = cur - first;
-      w.t1 = min(nt, w.t0 + end - cur);
-      cur = first + w.t1;
-      w.slot = !p.merge_all && w.t0 == 0 && w.t1 == nt ? -1 : w.b * per_e + idx + static_cast<int>(blockIdx.x);
-    } else {
-      cur = 1;
-      // longest row tiles (the last ones of a causal chunk) first
-      const int rt = p.n_rt - 1 - static_cast<int>(blockIdx.y) / p.Hkv;
-      const int b = blockIdx.z, split = blockIdx.x;
-      const Seg& s = p.seg[0];
-      const int nq = p.q_lens ? min(max(p.q_lens[b], 0), s.units) : s.units;
-      w.seg = 0;
-      w.b = b;
-      w.kvh = static_cast<int>(blockIdx.y) % p.Hkv;
-      w.row0 = rt * MT;
-      w.rows = min(MT, nq * p.nrep - w.row0);
-      if (w.rows <= 0) return false;
-      w.key = make_keys(s, seg_len(s, b), nq, w.row0 / p.nrep, (w.row0 + w.rows - 1) / p.nrep);
-      const int nt = max(w.key.nt, 1);
-      const uint32_t ns = p.n_split;  // (nt < 2^24, n_split <= 16)
-      w.t0 = static_cast<int>(static_cast<uint32_t>(nt) * split / ns);
-      w.t1 = static_cast<int>(static_cast<uint32_t>(nt) * (split + 1) / ns);
-      w.slot = p.n_split == 1 ? -1
-                              : ((b * p.Hkv + w.kvh) * p.n_rt + rt) * p.n_split + split;
-    }
-    return true;
-  }
 };
+template <int MT, bool STREAM>
+__device__ __forceinline__ Walk walk_start(const Params& p, const int* cum) {
+  Walk k{0, 1, 0};
+  if constexpr (STREAM) {
+    const int ne = p.seg[0].nb + (p.nseg > 1 ? p.seg[1].nb : 0);
+    const int total = cum[ne];
+    const int per = max(p.min_tiles, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    k.cur = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total)));
+    k.end = static_cast<int>(min(static_cast<int64_t>(k.cur) + per, static_cast<int64_t>(total)));
+    // the entry that holds tile cur: cum[e] <= cur < cum[e + 1]
+    int lo = 0, hi = ne - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cum[mid] <= k.cur) lo = mid; else hi = mid - 1;
+    }
+    k.e = lo;
+  }
+  return k;
+}
+template <int MT, bool STREAM>
+__device__ __noinline__ bool walk_next(Walk& k, const Params& p, const int* cum, Piece& w) {
+  if (k.cur >= k.end) return false;
+  if constexpr (STREAM) {
+    while (cum[k.e + 1] <= k.cur) ++k.e;
+    w.seg = k.e < p.seg[0].nb ? 0 : 1;
+    const Seg& s = p.seg[w.seg];
+    w.b = k.e - (w.seg ? p.seg[0].nb : 0);
+    const int rows = s.units * p.nrep, n_rt = row_tiles(rows, MT), per_e = p.Hkv * n_rt;
+    const uint32_t nt = static_cast<uint32_t>(cum[k.e + 1] - cum[k.e]) / static_cast<uint32_t>(per_e);
+    const int idx = static_cast<uint32_t>(k.cur - cum[k.e]) / nt, first = cum[k.e] + idx * nt;
+    const int rt = static_cast<uint32_t>(idx) / static_cast<uint32_t>(p.Hkv);
+    w.kvh = idx - rt * p.Hkv;
+    w.row0 = rt * MT;
+    w.rows = min(MT, rows - w.row0);
+    w.key = make_keys(s, seg_len(s, w.b), s.units, 0, 0);
+    w.t0 = k.cur - first;
+    w.t1 = min(static_cast<int>(nt), w.t0 + k.end - k.cur);
+    k.cur = first + w.t1;
+    w.slot = !p.merge_all && w.t0 == 0 && w.t1 == static_cast<int>(nt)
+                 ? -1
+                 : w.b * per_e + idx + static_cast<int>(blockIdx.x);
+  } else {
+    k.cur = 1;
+    // longest row tiles (the last ones of a causal chunk) first
+    const int rq = static_cast<uint32_t>(blockIdx.y) / static_cast<uint32_t>(p.Hkv);
+    const int rt = p.n_rt - 1 - rq;
+    const int b = blockIdx.z;
+    const Seg& s = p.seg[0];
+    const int nq = p.q_lens ? min(max(p.q_lens[b], 0), s.units) : s.units;
+    w.seg = 0;
+    w.b = b;
+    w.kvh = static_cast<int>(blockIdx.y) - rq * p.Hkv;
+    w.row0 = rt * MT;
+    w.rows = min(MT, nq * p.nrep - w.row0);
+    if (w.rows <= 0) return false;
+    w.key = make_keys(s, seg_len(s, b), nq, static_cast<uint32_t>(w.row0) / static_cast<uint32_t>(p.nrep),
+                      static_cast<uint32_t>(w.row0 + w.rows - 1) / static_cast<uint32_t>(p.nrep));
+    const uint32_t nt = max(w.key.nt, 1), ns = p.n_split, split = blockIdx.x;  // nt < 2^24, ns <= 16
+    w.t0 = static_cast<int>(nt * split / ns);
+    w.t1 = static_cast<int>(nt * (split + 1) / ns);
+    w.slot = ns == 1 ? -1 : ((b * p.Hkv + w.kvh) * p.n_rt + rt) * static_cast<int>(ns) + static_cast<int>(split);
+  }
+  return true;
+}
 
 __device__ __forceinline__ float* part_row(const Params& p, int seg, int slot, int r) {
   return p.part + (seg ? p.part1 : 0) +
@@ -335,29 +358,50 @@ __device__ __forceinline__ void store4(void* row, int dt, int d, float a, float 
   }
   *reinterpret_cast<uint2*>(static_cast<char*>(row) + 2 * d) = w;
 }
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, int dt) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+  return dt == HQ_DTYPE_BF16 ? *reinterpret_cast<const uint32_t*>(&x) : pack_h2(a, b);
+}
 __device__ __forceinline__ char* out_row(const Params& p, int b, int u, int h) {
   return static_cast<char*>(p.out) + 2 * (b * p.osb + u * p.osu + h * p.osh);
 }
 
-// Per-token int8 fake quantization of a q row held by 16 lanes, 8 channels each, rounded
-// back to the model dtype.
-struct Eight {
-  float x[8];
-};
-__device__ __noinline__ Eight fake_quant8(Eight f, int dt) {
+__device__ __forceinline__ void unpack8(const uint4& x, int dt, float (&f)[8]) {
+  if (dt == HQ_DTYPE_BF16) Vec16<HQ_DTYPE_BF16>::unpack(x, f);
+  else Vec16<HQ_DTYPE_F16>::unpack(x, f);
+}
+// Per-token int8 fake quantization of row r of a Q tile, rounded back to the model dtype.
+__device__ __noinline__ void fake_quant_row(unsigned char* tile, int r, int dt) {
+  auto chunk = [&](int c) {
+    return reinterpret_cast<uint4*>(tile + (c >> 3) * (kBN * 128) + sw128(r, c & 7));
+  };
   float am = 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < 16; ++c) {
+    float f[8];
+    unpack8(*chunk(c), dt, f);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(f.x[e]));
-#pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
-  const Quantizer qz = Quantizer::from_amax(am);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float y = static_cast<float>(qz.code(f.x[e])) * qz.scale;
-    f.x[e] = dt == HQ_DTYPE_BF16 ? __bfloat162float(__float2bfloat16_rn(y))
-                                 : __half2float(__float2half_rn(y));
+    for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(f[e]));
   }
-  return f;
+  const Quantizer qz = Quantizer::from_amax(am);
+#pragma unroll 1
+  for (int c = 0; c < 16; ++c) {
+    float f[8];
+    unpack8(*chunk(c), dt, f);
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = static_cast<float>(qz.code(f[2 * e])) * qz.scale;
+      const float b = static_cast<float>(qz.code(f[2 * e + 1])) * qz.scale;
+      if (dt == HQ_DTYPE_BF16) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+        w[e] = *reinterpret_cast<const uint32_t*>(&x);
+      } else {
+        w[e] = pack_h2(a, b);
+      }
+    }
+    *chunk(c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // ---------------------------------------------------------------- softmax of one row tile
@@ -372,6 +416,21 @@ struct RowLim {
     return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
   }
 };
+// Code size decides here: a straight run of instructions that is not in the instruction cache
+// costs about 10 cycles each, and the SM's schedulers hold some 12 KB each.  So the loops below
+// stay rolled as far as registers allow, and what is rare is a call.
+
+// O *= a
+__device__ __noinline__ void rescale(uint32_t o_addr, float a) {
+#pragma unroll 1
+  for (int c = 0; c < 8; ++c) {
+    uint32_t o[16];
+    tmem_ld16(o_addr + 16 * c, o);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+    tmem_st16(o_addr + 16 * c, o);
+  }
+}
 // The running maximum takes this tile's largest t in, O and l are rescaled where it moves;
 // waits for the previous P V on the way.
 __device__ __forceinline__ void move_max(float mx, uint32_t o_addr, bool first, uint64_t* pv_bar,
@@ -390,128 +449,139 @@ __device__ __forceinline__ void move_max(float mx, uint32_t o_addr, bool first, 
     if (!ok) return;
     tc_fence_after();
   }
-  if (!first && __any_sync(0xffffffffu, a != 1.0f)) {
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-      float o[32];
-      tmem_ld32(o_addr + 32 * c, o);
-#pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] *= a;
-      tmem_st32(o_addr + 32 * c, o);
-    }
-  }
+  if (!first && __any_sync(0xffffffffu, a != 1.0f)) rescale(o_addr, a);
 }
 
-// One tile of one row, all of it seen and with all e_j = 0: the running maximum, then
-// P = 2^(s fac - m) over S and l.
-__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, float fac,
-                                             bool first, uint64_t* pv_bar, int cnt,
+// One tile of one row that sees all of it: the running maximum, then P = 2^(t - m) over S, and
+// l.  EXP: t = s fac + e_j with e_j from ev[j] and 2^-e_j from ev[128 + j], else t = s fac.
+template <bool EXP>
+__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, const float* ev,
+                                             float fac, bool first, uint64_t* pv_bar, int cnt,
                                              volatile int* abort, float& m, float& l, bool& ok) {
   uint32_t sa[32], sb[32];
   float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  auto fold = [&](const uint32_t (&s)[32]) {
+  auto fold = [&](const uint32_t (&s)[32], const float* e_run) {
 #pragma unroll
-    for (int e = 0; e < 32; e += 8)
+    for (int e = 0; e < 32; e += 4) {
+      float t[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[i] = fmaxf(x[i], fmaxf(__uint_as_float(s[e + 2 * i]), __uint_as_float(s[e + 2 * i + 1])));
+      for (int i = 0; i < 4; ++i) t[i] = __uint_as_float(s[e + i]);
+      if constexpr (EXP) {
+        const float4 e4 = *reinterpret_cast<const float4*>(e_run + e);
+        t[0] = __fmaf_rn(t[0], fac, e4.x);
+        t[1] = __fmaf_rn(t[1], fac, e4.y);
+        t[2] = __fmaf_rn(t[2], fac, e4.z);
+        t[3] = __fmaf_rn(t[3], fac, e4.w);
+      }
+      const int k = (e >> 2) & 1;
+      x[2 * k] = fmaxf(x[2 * k], fmaxf(t[0], t[1]));
+      x[2 * k + 1] = fmaxf(x[2 * k + 1], fmaxf(t[2], t[3]));
+    }
   };
   tmem_get(s_addr, sa);
-  tmem_got(sa);
-  tmem_get(s_addr + 32, sb);
-  fold(sa);
-  tmem_got(sb);
-  tmem_get(s_addr + 64, sa);
-  fold(sb);
-  tmem_got(sa);
-  tmem_get(s_addr + 96, sb);
-  fold(sa);
-  tmem_got(sb);
-  fold(sb);
-  move_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * fac, o_addr, first, pv_bar, cnt, abort, m,
-           l, ok);
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 64) {
+    tmem_got(sa);
+    tmem_get(s_addr + c + 32, sb);
+    fold(sa, ev + c);
+    tmem_got(sb);
+    if (c == 0) tmem_get(s_addr + 64, sa);
+    fold(sb, ev + c + 32);
+  }
+  float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  if constexpr (!EXP) mx *= fac;
+  move_max(mx, o_addr, first, pv_bar, cnt, abort, m, l, ok);
   if (!ok) return;
-  const F2 nb2 = f2_make(-m, -m), fac2 = f2_make(fac, fac);
+  const float nb = m == -INFINITY ? 0.0f : -m;
+  const F2 nb2 = f2_make(nb, nb), fac2 = f2_make(fac, fac);
   F2 ls0 = f2_make(0.0f, 0.0f), ls1 = ls0;
-  // P of keys 32 c .. goes over S columns 16 c .., which have been read by then
+  // P of keys c .. goes over S columns c / 2 .., which have been read by then
   auto emit = [&](const uint32_t (&s)[32], int c) {
     uint32_t w[16];
 #pragma unroll
     for (int e = 0; e < 32; e += 4) {
       float t[4];
-      f2_split(f2_fma(f2_make(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), fac2, nb2), t[0], t[1]);
-      f2_split(f2_fma(f2_make(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), fac2, nb2), t[2], t[3]);
+      F2 n0 = nb2, n1 = nb2;
+      if constexpr (EXP) {
+        const float4 e4 = *reinterpret_cast<const float4*>(ev + c + e);
+        n0 = f2_add(f2_make(e4.x, e4.y), nb2);
+        n1 = f2_add(f2_make(e4.z, e4.w), nb2);
+      }
+      f2_split(f2_fma(f2_make(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), fac2, n0), t[0], t[1]);
+      f2_split(f2_fma(f2_make(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), fac2, n1), t[2], t[3]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) t[i] = ex2_ftz(t[i]);
-      ls0 = f2_add(ls0, f2_make(t[0], t[1]));
-      ls1 = f2_add(ls1, f2_make(t[2], t[3]));
+      if constexpr (EXP) {
+        const float4 r4 = *reinterpret_cast<const float4*>(ev + kBN + c + e);
+        ls0 = f2_fma(f2_make(t[0], t[1]), f2_make(r4.x, r4.y), ls0);
+        ls1 = f2_fma(f2_make(t[2], t[3]), f2_make(r4.z, r4.w), ls1);
+      } else {
+        ls0 = f2_add(ls0, f2_make(t[0], t[1]));
+        ls1 = f2_add(ls1, f2_make(t[2], t[3]));
+      }
       w[e / 2] = pack_h2(t[0], t[1]);
       w[e / 2 + 1] = pack_h2(t[2], t[3]);
     }
-    tmem_st16(s_addr + 16 * c, w);
+    tmem_st16(s_addr + c / 2, w);
   };
   tmem_get(s_addr, sa);
-  tmem_got(sa);
-  tmem_get(s_addr + 32, sb);
-  emit(sa, 0);
-  tmem_got(sb);
-  tmem_get(s_addr + 64, sa);
-  emit(sb, 1);
-  tmem_got(sa);
-  tmem_get(s_addr + 96, sb);
-  emit(sa, 2);
-  tmem_got(sb);
-  emit(sb, 3);
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 64) {
+    tmem_got(sa);
+    tmem_get(s_addr + c + 32, sb);
+    emit(sa, c);
+    tmem_got(sb);
+    if (c == 0) tmem_get(s_addr + 64, sa);
+    emit(sb, c + 32);
+  }
   float x0, x1;
   f2_split(f2_add(ls0, ls1), x0, x1);
   l += x0 + x1;
   tmem_wait_st();
 }
 
-// The same for any tile: e_j from ev[j], 2^-e_j from ev[128 + j], and keys some rows do not
-// see.  Rolled over the four runs of 32 keys, to keep the code small.
+// The same for a tile with e_j that some row of the warp does not see all of (bf16 models: for
+// any tile that softmax_tile<false> does not take).
 __device__ __forceinline__ void softmax_tile_any(uint32_t s_addr, uint32_t o_addr, const float* ev,
                                                  float fac, int v0, const RowLim& lim, bool first,
                                                  uint64_t* pv_bar, int cnt, volatile int* abort,
                                                  float& m, float& l, bool& ok) {
-  uint32_t s[32];
-  float mx = -INFINITY;
+  float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    const uint32_t seen = lim.bits(v0 + 32 * c);
-    tmem_get(s_addr + 32 * c, s);
-    tmem_got(s);
+  for (int c = 0; c < 128; c += 16) {
+    const uint32_t seen = lim.bits(v0 + c);
+    uint32_t s[16];
+    tmem_ld16(s_addr + c, s);
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {
-      const float4 e4 = *reinterpret_cast<const float4*>(ev + 32 * c + e);
+    for (int e = 0; e < 16; e += 4) {
+      const float4 e4 = *reinterpret_cast<const float4*>(ev + c + e);
       const float t0 = __fmaf_rn(__uint_as_float(s[e]), fac, e4.x);
       const float t1 = __fmaf_rn(__uint_as_float(s[e + 1]), fac, e4.y);
       const float t2 = __fmaf_rn(__uint_as_float(s[e + 2]), fac, e4.z);
       const float t3 = __fmaf_rn(__uint_as_float(s[e + 3]), fac, e4.w);
-      mx = fmaxf(mx, fmaxf(seen >> e & 1 ? t0 : -INFINITY, seen >> (e + 1) & 1 ? t1 : -INFINITY));
-      mx = fmaxf(mx, fmaxf(seen >> (e + 2) & 1 ? t2 : -INFINITY, seen >> (e + 3) & 1 ? t3 : -INFINITY));
+      x0 = fmaxf(x0, fmaxf(seen & (1u << e) ? t0 : -INFINITY, seen & (2u << e) ? t1 : -INFINITY));
+      x1 = fmaxf(x1, fmaxf(seen & (4u << e) ? t2 : -INFINITY, seen & (8u << e) ? t3 : -INFINITY));
     }
   }
-  move_max(mx, o_addr, first, pv_bar, cnt, abort, m, l, ok);
+  move_max(fmaxf(x0, x1), o_addr, first, pv_bar, cnt, abort, m, l, ok);
   if (!ok) return;
   const float nb = m == -INFINITY ? 0.0f : -m;
   float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    const uint32_t seen = lim.bits(v0 + 32 * c);
-    tmem_get(s_addr + 32 * c, s);
-    tmem_got(s);
-    uint32_t w[16];
+  for (int c = 0; c < 128; c += 16) {
+    const uint32_t seen = lim.bits(v0 + c);
+    uint32_t s[16], w[8];
+    tmem_ld16(s_addr + c, s);
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {
-      const float4 e4 = *reinterpret_cast<const float4*>(ev + 32 * c + e);
-      const float4 r4 = *reinterpret_cast<const float4*>(ev + kBN + 32 * c + e);
+    for (int e = 0; e < 16; e += 4) {
+      const float4 e4 = *reinterpret_cast<const float4*>(ev + c + e);
+      const float4 r4 = *reinterpret_cast<const float4*>(ev + kBN + c + e);
       float t[4] = {__fmaf_rn(__uint_as_float(s[e]), fac, e4.x + nb),
                     __fmaf_rn(__uint_as_float(s[e + 1]), fac, e4.y + nb),
                     __fmaf_rn(__uint_as_float(s[e + 2]), fac, e4.z + nb),
                     __fmaf_rn(__uint_as_float(s[e + 3]), fac, e4.w + nb)};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = seen >> (e + i) & 1 ? ex2_ftz(t[i]) : 0.0f;
+      for (int i = 0; i < 4; ++i) t[i] = seen & (1u << (e + i)) ? ex2_ftz(t[i]) : 0.0f;
       ls[0] = __fmaf_rn(t[0], r4.x, ls[0]);
       ls[1] = __fmaf_rn(t[1], r4.y, ls[1]);
       ls[2] = __fmaf_rn(t[2], r4.z, ls[2]);
@@ -519,7 +589,7 @@ __device__ __forceinline__ void softmax_tile_any(uint32_t s_addr, uint32_t o_add
       w[e / 2] = pack_h2(t[0], t[1]);
       w[e / 2 + 1] = pack_h2(t[2], t[3]);
     }
-    tmem_st16(s_addr + 16 * c, w);  // over S columns that have been read
+    tmem_st8(s_addr + c / 2, w);  // over S columns that have been read
   }
   l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
   tmem_wait_st();
@@ -527,7 +597,7 @@ __device__ __forceinline__ void softmax_tile_any(uint32_t s_addr, uint32_t o_add
 
 // ---------------------------------------------------------------- the kernel
 template <int NM, bool LO, bool STREAM>
-__global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const Params p) {
+__global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const __grid_constant__ Params p) {
   using C = Cfg<NM, LO>;
   constexpr int MT = 128 * NM;
   extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -536,6 +606,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
   float* eb = reinterpret_cast<float*>(smem + C::kOffE);
   __half* gb = reinterpret_cast<__half*>(smem + C::kOffG);
   float2* info = reinterpret_cast<float2*>(smem + C::kOffInfo);
+  float* ksm = reinterpret_cast<float*>(smem + C::kOffKs);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* q_full = bars;
   uint64_t* k_full = q_full + 1;
@@ -555,7 +626,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
   int* cum = reinterpret_cast<int*>(smem + C::kOffCum);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kMmaWarp = (C::kSoft + kConvThreads) / 32, kCopyWarp = kMmaWarp + 1;
+  constexpr int kMmaWarp = (C::kSoft + kConvThreads) / 32, kCopyWarp = kMmaWarp + 1;  // + 2: V scales
   // combine_kernel's blocks may be scheduled; they wait for this grid
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == kMmaWarp) {
@@ -621,8 +692,8 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
   const uint32_t tmem = *tmem_slot;
   const uint32_t q_base = smem_u32(smem), k_base = smem_u32(smem + C::kOffK),
                  v_base = smem_u32(smem + C::kOffV);
-  Walk<MT, STREAM> walk;
-  walk.start(p, cum);
+  Walk walk = walk_start<MT, STREAM>(p, cum);
+  auto next_piece = [&](Walk& k, Piece& to) { return walk_next<MT, STREAM>(k, p, cum, to); };
   Piece w{};
 
   if (warp < C::kSoft / 32) {
@@ -631,84 +702,72 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + kColO + 128 * mt + lane_base;
     int pc = 0, gt = 0, cnt = 0;        // pieces, tiles of the block, tiles of this row tile
+    int64_t q_off = 0;                  // byte offset of this thread's q row
     bool ok = true;
-    // q' of this warp's 32 rows into the Q tile (16 lanes per row, two rows at a time, the
-    // loads of 8 rows in flight); returns 2^-ex of this lane's row.  The Q tile is free: this
-    // warp has seen the last S of the piece before.
-    auto make_q = [&]() -> float {
-      const Seg& s = p.seg[w.seg];
-      const int l16 = lane & 15, half = lane >> 4, r0 = 32 * warp;
-      float ks[8];
-      const int64_t k0 = w.b * s.kscb + w.kvh * s.ksch;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        ks[e] = load_scale(s.ksc, k0 + (8 * l16 + e) * s.kscd, p.s_dt) * p.qk_scale;
-      unsigned char* tile = smem + mt * C::kParts * kTileB;
-      float mine = 0.0f;
-#pragma unroll 1
-      for (int i0 = 0; i0 < 32 && r0 + i0 < w.rows; i0 += 8) {
-        uint4 x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int rr = r0 + i0 + 2 * i + half;
-          x[i] = make_uint4(0, 0, 0, 0);
-          if (rr < w.rows) {
-            const int u = (w.row0 + rr) / p.nrep, h = w.kvh * p.nrep + (w.row0 + rr) % p.nrep;
-            x[i] = *reinterpret_cast<const uint4*>(
-                static_cast<const char*>(p.q) +
-                2 * (w.b * s.qsb + u * s.qsu + h * p.qsh + 8 * l16));
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int rr = r0 + i0 + 2 * i + half;
-          float f[8];
-          if (p.q_dt == HQ_DTYPE_BF16) Vec16<HQ_DTYPE_BF16>::unpack(x[i], f);
-          else Vec16<HQ_DTYPE_F16>::unpack(x[i], f);
-          if (p.q_quant) {
-            const Eight g = fake_quant8(*reinterpret_cast<const Eight*>(f), p.q_dt);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = g.x[e];
-          }
-          float am = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f[e] *= ks[e];
-            am = fmaxf(am, fabsf(f[e]));
-          }
-#pragma unroll
-          for (int o = 8; o >= 1; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
-          // 2^ex brings am to [2^13, 2^14)
-          const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am) >> 23) - 127), -100), 100);
-          const float mul = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
-          const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-          const float a = __shfl_sync(0xffffffffu, inv, 0), b = __shfl_sync(0xffffffffu, inv, 16);
-          if (lane == i0 + 2 * i) mine = a;
-          if (lane == i0 + 2 * i + 1) mine = b;
-          if (rr >= w.rows) continue;
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y0 = f[2 * e] * mul, y1 = f[2 * e + 1] * mul;
-            hi[e] = pack_h2(y0, y1);
-            if constexpr (LO) {
-              const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-              lo[e] = pack_h2(y0 - g.x, y1 - g.y);
-            }
-          }
-          const uint32_t at = static_cast<uint32_t>(l16 >> 3) * (kBN * 128) + sw128(rr & 127, l16 & 7);
-          *reinterpret_cast<uint4*>(tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if constexpr (LO)
-            *reinterpret_cast<uint4*>(tile + kTileB + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-      }
-      return mine;
+    // q' of this thread's row, formed in place in the Q tile: the raw row, its fake
+    // quantization, its largest |q'|, q'.  Returns 2^-ex.  The tile is free: this warp has
+    // seen the last S of the piece before.  Compact loops: this runs once per piece.
+    unsigned char* q_tile = smem + mt * C::kParts * kTileB;
+    auto chunk = [&](int c) {  // 8 channels of the row
+      return reinterpret_cast<uint4*>(q_tile + (c >> 3) * (kBN * 128) + sw128(r & 127, c & 7));
     };
-    for (; ok && walk.next(p, cum, w); ++pc) {
+    auto make_q = [&]() -> float {
+      {
+        const char* src = static_cast<const char*>(p.q) + q_off;
+        uint4 x[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) x[c] = reinterpret_cast<const uint4*>(src)[c];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) *chunk(c) = x[c];
+      }
+      if (p.q_quant) fake_quant_row(q_tile, r & 127, p.q_dt);
+      float am = 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < 16; ++c) {
+        float f[8];
+        unpack8(*chunk(c), p.q_dt, f);
+        const float4 a = reinterpret_cast<const float4*>(ksm)[2 * c], b = reinterpret_cast<const float4*>(ksm)[2 * c + 1];
+        am = fmaxf(am, fmaxf(fmaxf(fabsf(f[0] * a.x), fabsf(f[1] * a.y)), fmaxf(fabsf(f[2] * a.z), fabsf(f[3] * a.w))));
+        am = fmaxf(am, fmaxf(fmaxf(fabsf(f[4] * b.x), fabsf(f[5] * b.y)), fmaxf(fabsf(f[6] * b.z), fabsf(f[7] * b.w))));
+      }
+      // 2^ex brings am to [2^13, 2^14)
+      const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am) >> 23) - 127), -100), 100);
+      const float mul = pow2i(ex);
+#pragma unroll 1
+      for (int c = 0; c < 16; ++c) {
+        float f[8];
+        unpack8(*chunk(c), p.q_dt, f);
+        const float4 a = reinterpret_cast<const float4*>(ksm)[2 * c], b = reinterpret_cast<const float4*>(ksm)[2 * c + 1];
+        const float k8[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y0 = f[2 * e] * k8[2 * e] * mul, y1 = f[2 * e + 1] * k8[2 * e + 1] * mul;
+          hi[e] = pack_h2(y0, y1);
+          if constexpr (LO) {
+            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+            lo[e] = pack_h2(y0 - g.x, y1 - g.y);
+          }
+        }
+        *chunk(c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (LO) *(chunk(c) + kTileB / 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      return pow2i(-ex);
+    };
+    for (; ok && next_piece(walk, w); ++pc) {
       const int n_tiles = w.t1 - w.t0;
       float m = -INFINITY, l = 0.0f, fac = 0.0f, vscale = 1.0f;
+      const Seg& s = p.seg[w.seg];
+      const bool live = r < w.rows;
+      const int u = (w.row0 + r) / p.nrep, h = w.kvh * p.nrep + (w.row0 + r) - u * p.nrep;
       if (n_tiles > 0) {
-        if (w.rows > 128 * mt) fac = make_q();
+        // the piece's K scales (every softmax thread takes part in both barriers)
+        asm volatile("bar.sync 1, %0;" ::"n"(C::kSoft) : "memory");
+        if (tid < kD)
+          ksm[tid] = load_scale(s.ksc, w.b * s.kscb + w.kvh * s.ksch + tid * s.kscd, p.s_dt) * p.qk_scale;
+        asm volatile("bar.sync 1, %0;" ::"n"(C::kSoft) : "memory");
+        q_off = 2 * (w.b * s.qsb + u * s.qsu + h * p.qsh);
+        if (live) fac = make_q();
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
@@ -722,10 +781,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         gt += n_tiles;
         continue;
       }
-      const Seg& s = p.seg[w.seg];
-      const bool live = r < w.rows;
       const bool warp_live = 32 * warp < w.rows;
-      const int u = (w.row0 + r) / p.nrep;
       const int pos = w.key.pos0 + (s.step ? u : 0);
       const RowLim lim = {live ? pos - w.key.sh : 1 << 30,
                           live ? pos - s.window + 1 - w.key.sh : 0,
@@ -747,8 +803,8 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
           if (t == w.t0) vscale = ti.y;
           const bool need = v0 + kBN - 1 > lim.hi || (v0 < lim.lo && v0 + kBN > lim.vsk && lim.lo > lim.vsk);
           const bool mask = __any_sync(0xffffffffu, need);
-          if (!LO && ti.x == 0.0f && !mask)
-            softmax_tile(s_addr, o_addr, fac, t == w.t0, &pv_done[mt], cnt, abort, m, l, ok);
+          if (!mask && (LO || ti.x == 0.0f))
+            softmax_tile<LO>(s_addr, o_addr, ev, fac, t == w.t0, &pv_done[mt], cnt, abort, m, l, ok);
           else
             softmax_tile_any(s_addr, o_addr, ev, fac, v0, lim, t == w.t0, &pv_done[mt], cnt, abort,
                              m, l, ok);
@@ -770,41 +826,48 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         tc_fence_after();
       }
       if (warp_live) {
-        const bool have = live && l > 0.0f;
-        const int h = w.kvh * p.nrep + (w.row0 + r) % p.nrep;
-        char* dst = nullptr;
-        float* prt = nullptr;
-        float scale = vscale;           // 2^E
+        // (rows that saw nothing have l = 0 and give zeros, whatever their O holds; a NaN stays)
+        const bool have = live && !(l <= 0.0f) && n_tiles > 0;
         if (w.slot < 0) {
-          dst = out_row(p, w.b, u, h);
-          scale = have ? vscale / l : 0.0f;
-        } else {
-          prt = part_row(p, w.seg, w.slot, r);
-          if (live) {
-            prt[0] = have ? m : -INFINITY;
-            prt[1] = have ? l : 0.0f;
-          }
-        }
+          // the row into the Q tile, then the warp's rows out, 256 bytes at a time
+          const float scale = have ? vscale / l : 0.0f;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float o[32];
-          if (n_tiles > 0) {
-            tmem_ld32(o_addr + 32 * c, o);
-          } else {
+          for (int c = 0; c < 16; c += 2) {
+            uint32_t o[16], y[8];
+            tmem_ld16(o_addr + 8 * c, o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+            for (int e = 0; e < 8; ++e) {
+              const float a = __uint_as_float(o[2 * e]) * scale, b2 = __uint_as_float(o[2 * e + 1]) * scale;
+              y[e] = have ? pack_pair(a, b2, p.q_dt) : 0u;
+            }
+            *chunk(c) = make_uint4(y[0], y[1], y[2], y[3]);
+            *chunk(c + 1) = make_uint4(y[4], y[5], y[6], y[7]);
           }
-          if (!live) continue;
-          if (dst) {
+          __syncwarp();
+          const uint64_t dst = reinterpret_cast<uint64_t>(out_row(p, w.b, u, h));
+          const int n_rows = min(32, w.rows - 32 * warp);
+#pragma unroll 1
+          for (int i = 0; i < n_rows; ++i) {
+            char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, dst, i));
+            const int c = lane >> 1;
+            const unsigned char* from = q_tile + (c >> 3) * (kBN * 128) +
+                                        sw128((32 * warp + i) & 127, c & 7) + 8 * (lane & 1);
+            *reinterpret_cast<uint2*>(to + 8 * lane) = *reinterpret_cast<const uint2*>(from);
+          }
+          __syncwarp();
+        } else {
+          float* prt = part_row(p, w.seg, w.slot, r);
+          if (live) *reinterpret_cast<float2*>(prt) = make_float2(have ? m : -INFINITY, have ? l : 0.0f);
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + c, o);
+            if (!live) continue;
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              store4(dst, p.q_dt, 32 * c + e, have ? o[e] * scale : 0.0f, have ? o[e + 1] * scale : 0.0f,
-                     have ? o[e + 2] * scale : 0.0f, have ? o[e + 3] * scale : 0.0f);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(prt + 4 + 32 * c + e) =
-                  have ? make_float4(o[e] * scale, o[e + 1] * scale, o[e + 2] * scale, o[e + 3] * scale)
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<float4*>(prt + 4 + c + e) =
+                  have ? make_float4(__uint_as_float(o[e]) * vscale, __uint_as_float(o[e + 1]) * vscale,
+                                     __uint_as_float(o[e + 2]) * vscale, __uint_as_float(o[e + 3]) * vscale)
                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           }
         }
@@ -840,35 +903,29 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       ok = wait_bar(&st_full[sl], (sc / C::kSlots) & 1, abort);
       if (!ok) return;
       const unsigned char* src = smem + C::kOffSlot + sl * kSlotB + row * kD + 16 * c16;
-      uint4 x[NI];
-      uint32_t g2[NI];
-#pragma unroll
+      tile += half * 64 * 128;
+#pragma unroll 2
       for (int i = 0; i < NI; ++i) {
-        x[i] = *reinterpret_cast<const uint4*>(src + i * 16 * kD);
+        const uint4 x = *reinterpret_cast<const uint4*>(src + i * 16 * kD);
+        uint32_t y[8];
+        codes_to_h2(x.x, y[0], y[1]);
+        codes_to_h2(x.y, y[2], y[3]);
+        codes_to_h2(x.z, y[4], y[5]);
+        codes_to_h2(x.w, y[6], y[7]);
         if (g) {
           const uint32_t h = *reinterpret_cast<const uint16_t*>(g + 64 * half + row + 16 * i);
-          g2[i] = h | h << 16;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        uint32_t y[8];
-        codes_to_h2(x[i].x, y[0], y[1]);
-        codes_to_h2(x[i].y, y[2], y[3]);
-        codes_to_h2(x[i].z, y[4], y[5]);
-        codes_to_h2(x[i].w, y[6], y[7]);
-        if (g) {
+          const uint32_t g2 = h | h << 16;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y[e]) : "r"(y[e]), "r"(g2[i]));
+            asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y[e]) : "r"(y[e]), "r"(g2));
         }
-        put(tile, 4 * half + i, y);
+        put(tile, i, y);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&st_empty[sl]);
       ++sc;
     };
-    for (; ok && walk.next(p, cum, w);) {
+    for (; ok && next_piece(walk, w);) {
       for (int t = w.t0; t < w.t1; ++t, ++gt) {
         const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
         if (use > 0) ok = wait_bar(&k_empty[st], (use - 1) & 1, abort);
@@ -894,97 +951,37 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
     }
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
   } else if (warp == kCopyWarp) {
-    // ================= codes into the staging ring, V scales into g_j and e_j
-    int sc = 0, gt = 0;
+    // ================= codes into the staging ring
+    int sc = 0;
     bool ok = true;
-    for (; ok && walk.next(p, cum, w);) {
+    for (; ok && next_piece(walk, w);) {
       const Seg& s = p.seg[w.seg];
-      const int8_t* base[2] = {s.k + w.b * s.sb + w.kvh * s.sh, s.v + w.b * s.sb + w.kvh * s.sh};
-      const int64_t vs0 = w.b * s.vscb + w.kvh * s.vsch;
-      int E = 0;
-      for (int t = w.t0; ok && t < w.t1; ++t, ++gt) {
-        float vs[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int v = t * kBN + 32 * i + lane;
-          const int64_t key = v < w.key.ns ? v : v + w.key.sh;
-          vs[i] = v < w.key.nv ? load_scale(s.vsc, vs0 + key * s.vscs, p.s_dt) : -1.0f;
-        }
+      const int64_t o = w.b * s.sb + w.kvh * s.sh;
 #pragma unroll 1
-        for (int c = 0; ok && c < 4; ++c, ++sc) {  // K 0 .. 63, K 64 .., V 0 .., V 64 ..
-          const int sl = sc % C::kSlots, use = sc / C::kSlots;
-          if (use > 0) ok = wait_bar(&st_empty[sl], (use - 1) & 1, abort);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int v0 = t * kBN + (c & 1) * kSlotKeys;
-          const int n = min(max(w.key.nv - v0, 0), kSlotKeys);
-          unsigned char* dst = smem + C::kOffSlot + sl * kSlotB;
-          const int8_t* src = base[c >> 1];
-          if (lane == 0) mbar_arrive_expect_tx(&st_full[sl], n * kD);
-          __syncwarp();
-          if (s.ss == kD) {  // rows back to back: the sinks' run and the window's
-            const int n0 = min(max(w.key.ns - v0, 0), n);
-            if (lane == 0 && n0 > 0) bulk_g2s(dst, src + static_cast<int64_t>(v0) * kD, n0 * kD, &st_full[sl]);
-            if (lane == 0 && n > n0)
-              bulk_g2s(dst + n0 * kD, src + static_cast<int64_t>(v0 + n0 + w.key.sh) * kD,
-                       (n - n0) * kD, &st_full[sl]);
-          } else {
-            for (int i = lane; i < n; i += 32) {
-              const int v = v0 + i;
-              const int64_t key = v < w.key.ns ? v : v + w.key.sh;
-              bulk_g2s(dst + i * kD, src + key * s.ss, kD, &st_full[sl]);
-            }
-          }
-        }
-        if (!ok) break;
-        // slot gt % kLvSlots is free once P V of the tile two before is done
-        const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
-        if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1, abort);
+      for (int t2 = 4 * w.t0; ok && t2 < 4 * w.t1; ++t2, ++sc) {  // K 0 .., K 64 .., V 0 .., V 64 ..
+        const int sl = sc % C::kSlots, use = sc / C::kSlots;
+        if (use > 0) ok = wait_bar(&st_empty[sl], (use - 1) & 1, abort);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        float* ev = eb + slot * 2 * kBN;
-        bool any = LO;
-        if constexpr (LO) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool zero = vs[i] < kTinyScale;
-            const float x = zero ? kTinyScale : vs[i];
-            ev[32 * i + lane] = __log2f(x);
-            ev[kBN + 32 * i + lane] = __frcp_rn(x);
-            gb[slot * kBN + 32 * i + lane] = __float2half_rn(zero ? 0.0f : 1.0f);
-          }
+        const int v0 = (t2 >> 2) * kBN + (t2 & 1) * kSlotKeys;
+        const int n = min(max(w.key.nv - v0, 0), kSlotKeys);
+        unsigned char* dst = smem + C::kOffSlot + sl * kSlotB;
+        const int8_t* src = (t2 & 2 ? s.v : s.k) + o;
+        if (lane == 0) mbar_arrive_expect_tx(&st_full[sl], n * kD);
+        __syncwarp();
+        if (s.ss == kD) {  // rows back to back: the sinks' run and the window's
+          const int n0 = min(max(w.key.ns - v0, 0), n);
+          if (lane == 0 && n0 > 0) bulk_g2s(dst, src + static_cast<int64_t>(v0) * kD, n0 * kD, &st_full[sl]);
+          if (lane == 0 && n > n0)
+            bulk_g2s(dst + n0 * kD, src + static_cast<int64_t>(v0 + n0 + w.key.sh) * kD,
+                     (n - n0) * kD, &st_full[sl]);
         } else {
-          int ex[4];
-          bool odd = false;
-          int top = -1000;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ex[i] = vs[i] < kTinyScale ? -60 : static_cast<int>(__float_as_uint(vs[i]) >> 23 & 255) - 127;
-            top = max(top, vs[i] < kTinyScale ? -1000 : ex[i]);
-          }
-          if (t == w.t0) {
-            top = __reduce_max_sync(0xffffffffu, top);
-            E = top == -1000 ? 0 : min(max(top, -100), 100);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ex[i] -= E;
-            odd = odd || (vs[i] >= 0.0f && (ex[i] < -4 || ex[i] > 6 || vs[i] < kTinyScale));
-          }
-          any = __any_sync(0xffffffffu, odd);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int e = any ? min(max(ex[i], -100), 100) : 0;
-            ev[32 * i + lane] = static_cast<float>(e);
-            ev[kBN + 32 * i + lane] = pow2i(-e);
-            // (two factors: the exponent of their product may leave float32's)
-            gb[slot * kBN + 32 * i + lane] =
-                __float2half_rn(vs[i] < kTinyScale ? 0.0f : vs[i] * pow2i(-E) * pow2i(-e));
+          for (int i = lane; i < n; i += 32) {
+            const int v = v0 + i;
+            const int64_t key = v < w.key.ns ? v : v + w.key.sh;
+            bulk_g2s(dst + i * kD, src + key * s.ss, kD, &st_full[sl]);
           }
         }
-        if (lane == 0) info[slot] = make_float2(any ? 1.0f : 0.0f, pow2i(E));
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&lv_full[slot]);
       }
     }
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
@@ -992,9 +989,95 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
     for (int k = max(0, sc - C::kSlots); k < sc; ++k)
       if (!mbar_wait(&st_full[k % C::kSlots], (k / C::kSlots) & 1))
         report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
+  } else if (warp == kCopyWarp + 1) {
+    // ================= V scales into g_j and e_j, loaded a tile ahead
+    int gt = 0;
+    bool ok = true;
+    // cursor of the loads
+    Piece lp{};
+    int lt = -1;
+    float next[4];
+    auto load_next = [&]() -> bool {
+      if (++lt >= lp.t1) {
+        do {
+          if (!next_piece(walk, lp)) return false;
+        } while (lp.t0 >= lp.t1);
+        lt = lp.t0;
+      }
+      const Seg& s = p.seg[lp.seg];
+      const int64_t vs0 = lp.b * s.vscb + lp.kvh * s.vsch;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int v = lt * kBN + 32 * i + lane;
+        const int64_t key = v < lp.key.ns ? v : v + lp.key.sh;
+        next[i] = v < lp.key.nv ? load_scale(s.vsc, vs0 + key * s.vscs, p.s_dt) : -1.0f;
+      }
+      return true;
+    };
+    bool have = load_next();
+    int E = 0;
+    while (have) {
+      float vs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vs[i] = next[i];
+      const bool first = lt == lp.t0;
+      have = load_next();
+      // slot gt % kLvSlots is free once P V of the tile two before is done
+      const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
+      if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1, abort);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      float* ev = eb + slot * 2 * kBN;
+      bool any = LO;
+      if constexpr (LO) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool zero = vs[i] < kTinyScale;
+          const float x = zero ? kTinyScale : vs[i];
+          ev[32 * i + lane] = __log2f(x);
+          ev[kBN + 32 * i + lane] = __frcp_rn(x);
+          gb[slot * kBN + 32 * i + lane] = __float2half_rn(zero ? 0.0f : 1.0f);
+        }
+      } else {
+        int ex[4];
+        bool odd = false;
+        int top = -1000;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ex[i] = vs[i] < kTinyScale ? -60 : static_cast<int>(__float_as_uint(vs[i]) >> 23 & 255) - 127;
+          top = max(top, vs[i] < kTinyScale ? -1000 : ex[i]);
+        }
+        if (first) {
+          top = __reduce_max_sync(0xffffffffu, top);
+          E = top == -1000 ? 0 : min(max(top, -100), 100);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ex[i] -= E;
+          odd = odd || (vs[i] >= 0.0f && (ex[i] < -4 || ex[i] > 6 || vs[i] < kTinyScale));
+        }
+        any = __any_sync(0xffffffffu, odd);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = any ? min(max(ex[i], -100), 100) : 0;
+          ev[32 * i + lane] = static_cast<float>(e);
+          ev[kBN + 32 * i + lane] = pow2i(-e);
+          // (two factors: the exponent of their product may leave float32's)
+          gb[slot * kBN + 32 * i + lane] =
+              __float2half_rn(vs[i] < kTinyScale ? 0.0f : vs[i] * pow2i(-E) * pow2i(-e));
+        }
+      }
+      if (lane == 0) info[slot] = make_float2(any ? 1.0f : 0.0f, pow2i(E));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&lv_full[slot]);
+      ++gt;
+    }
+    if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
   } else if (warp == kMmaWarp) {
-    // ================= tensor-core products, issued by one thread
-    if (lane == 0) {
+    // ================= tensor-core products, issued by one thread; the warp stays together,
+    // so that descriptors and addresses live in uniform registers
+    {
+      const bool lead = elect_one();
       constexpr uint32_t id_s = idesc<HQ_DTYPE_F16>(128, 128, false);
       constexpr uint32_t id_o = idesc<HQ_DTYPE_F16>(128, 128, true);
       bool ok = true;
@@ -1005,16 +1088,19 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         const uint32_t buf = NM == 1 ? (cntq[m] & 1) : m;
         const uint64_t dk = sdesc(k_base + (g % kStages) * kTileB, 16, 1024);
         const uint64_t dq = sdesc(q_base + m * C::kParts * kTileB, 16, 1024);
-#pragma unroll 1
-        for (int part = 0; part < C::kParts; ++part)
+        if (lead) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            // (the address field counts 16 bytes; no sum leaves its 14 bits)
-            const uint32_t off = ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) >> 4;
-            mma_f16(tmem + 128 * buf, dq + (part * (kTileB >> 4) + off), dk + off, id_s,
-                    part + kk > 0);
-          }
-        mma_commit(&s_full[buf]);
+          for (int part = 0; part < C::kParts; ++part)
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              // (the address field counts 16 bytes; no sum leaves its 14 bits)
+              const uint32_t off = ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) >> 4;
+              mma_f16(tmem + 128 * buf, dq + (part * (kTileB >> 4) + off), dk + off, id_s,
+                      part + kk > 0);
+            }
+          mma_commit(&s_full[buf]);
+        }
+        __syncwarp();
         ++cntq[m];
       };
       auto pv = [&](int m, int g, bool first) {
@@ -1022,19 +1108,23 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         const uint32_t par = NM == 1 ? ((cntp[m] >> 1) & 1) : (cntp[m] & 1);
         ok = ok && wait_bar(&p_ready[buf], par, abort);
         if (first && pieces[m] > 0) ok = ok && wait_bar(&o_empty[m], (pieces[m] - 1) & 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
         tc_fence_after();
         const uint64_t dv = sdesc(v_base + (g % kStages) * kTileB, kBN * 128, 1024);
+        if (lead) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          mma_f16_ts(tmem + kColO + 128 * m, tmem + 128 * buf + 8 * kk, dv + (kk * 16 * 128 >> 4),
-                     id_o, !first || kk > 0);
-        mma_commit(&pv_done[m]);
+          for (int kk = 0; kk < 8; ++kk)
+            mma_f16_ts(tmem + kColO + 128 * m, tmem + 128 * buf + 8 * kk, dv + (kk * 16 * 128 >> 4),
+                       id_o, !first || kk > 0);
+          mma_commit(&pv_done[m]);
+        }
+        __syncwarp();
         ++cntp[m];
         if (first) ++pieces[m];
       };
       // cursor of the S products, one tile ahead of the P V products
-      Walk<MT, STREAM> qw = walk;
+      Walk qw = walk;
       Piece qp, cp;
       int qpc = -1, qt = 0, qg = 0;
       qp.t0 = qp.t1 = 0;
@@ -1043,7 +1133,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         fresh = false;
         if (++qt < qp.t1) return;
         do {
-          if (!qw.next(p, cum, qp)) {
+          if (!next_piece(qw, qp)) {
             more = false;
             return;
           }
@@ -1055,10 +1145,11 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       auto q_wait = [&]() {  // its q (of a piece's first tile) and K
         if (fresh) ok = ok && wait_bar(q_full, qpc & 1, abort);
         ok = ok && wait_bar(&k_full[qg % kStages], (qg / kStages) & 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       };
       auto q_done = [&]() {  // after the last S product of the tile
-        mma_commit(&k_empty[qg % kStages]);
+        if (lead) mma_commit(&k_empty[qg % kStages]);
         ++qg;
       };
       auto q_all = [&]() {
@@ -1083,6 +1174,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         if (ahead && NM == 1) q_all();
         if (ahead && NM > 1) q_wait();
         ok = ok && wait_bar(&v_full[g % kStages], (g / kStages) & 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         for (int m = 0; m < NM; ++m) {
           if (cp.rows > 128 * m) {
@@ -1093,14 +1185,14 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
           }
         }
         if (!ok) break;
-        mma_commit(&v_empty[g % kStages]);
+        if (lead) mma_commit(&v_empty[g % kStages]);
         if (NM > 1 && ahead) q_done();
         if (more && fresh) q_all();
         ++g;
       }
       if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
       // every product has completed before the tensor memory is released
-      mma_commit(drain);
+      if (lead) mma_commit(drain);
       if (!mbar_wait(drain, 0)) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
     }
     __syncwarp();
@@ -1180,7 +1272,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const Params p, int rows, 
         acc.w += f * o.w;
       }
   }
-  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  const float inv = L <= 0.0f ? 0.0f : 1.0f / L;  // (a NaN stays)
   store4(out_row(p, b, u, h), p.q_dt, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 

@@ -11,8 +11,17 @@
 // Exactness.  P * inv_freq has at most 31 + 24 significant bits and is formed in float64;
 // angles near 10^6 rad would be off by 0.06 rad in float32.  k is never rounded to the
 // model's type between rotation and coding, and a code is the nearest integer of the
-// float64 quotient: one rounding of the exact value.
+// float64 quotient: one rounding of the exact value.  The 16-bit kernel gets there mostly in
+// float32: the angle's fraction of a turn is taken in float64 and kept as a float32 pair, the
+// turned values are off by 2^-22 of the pair's size at most, and a quotient closer to a
+// rounding border than that (about one in 10^4) is formed again in float64.
+//
+// Bound by memory: a q element is read and written (4 bytes), a k or v element read and coded
+// (3 bytes).  A lane holds 8 channels (16 bytes), D / 8 lanes a row, and keeps the cos and sin
+// of its channels for all rows of its token.  8 sequences x 4096 tokens, 16 + 8 + 8 heads, bf16:
+// 141 us, 3.3 TB/s of the 470 MB it cannot do without (0.51 of measured).
 #include <algorithm>
+#include <cmath>
 
 #include "hq_common.cuh"
 
@@ -49,6 +58,9 @@ struct Params {
   int64_t qos[3];
   int* status;
   int rows_per_block;
+  int64_t tokens;                // 16-bit kernel
+  int groups, ks_vec;
+  float slack;                   // 2^-21 max(1, |factor|)
 };
 
 // CPL consecutive channels of a row
@@ -177,6 +189,249 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const Params p) {
   }
 }
 
+// ---------------------------------------------------------------- 16-bit types
+// Code of one k channel in float64: x turned with its partner o by the angle (lead: x is the
+// first of the pair; turned: the channel is rotated at all).
+__device__ __noinline__ int exact_code(float x, float o, bool lead, bool turned, double angle,
+                                       double factor, float scale) {
+  double y = x;
+  if (turned) {
+    double s, c;
+    sincos(angle, &s, &c);
+    c *= factor;
+    s *= factor;
+    y = lead ? x * c - o * s : x * c + o * s;
+  }
+  return static_cast<int>(fmin(fmax(rint(y / scale), -127.0), 127.0));
+}
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (DT == HQ_DTYPE_BF16) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&x);
+  } else {
+    const __half2 x = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&x);
+  }
+}
+
+// D / 8 lanes per token; a warp takes 32 / (D / 8) neighbouring tokens and `rows_per_block`
+// rows of each (the same ones, so that its branches agree).  Needs rot % 16 == 0: the partner
+// of a lane's 8 channels is another lane's 8 (or, interleaved, the lane's own).
+constexpr int kThreads16 = 128;
+// resident blocks per SM that the registers are held to: 8 x 4096 tokens took 189 us with none
+// (110 registers, 4 blocks), 151 / 141 / 149 / 167 us for 5 / 6 / 8 / 10
+constexpr int kBlocks16 = 6;
+template <int DT, int D>
+__global__ void __launch_bounds__(kThreads16, kBlocks16) rope_append16_kernel(const __grid_constant__ Params p) {
+  constexpr int LPR = D / 8, TPW = 32 / LPR;
+  using E = Elem<DT>;
+  const int lane = threadIdx.x & 31, sub = lane / LPR, l = lane % LPR, d0 = 8 * l;
+  const int64_t wg = static_cast<int64_t>(blockIdx.x) * (kThreads16 / 32) + (threadIdx.x >> 5);
+  const int rows = p.Hq + 2 * p.Hkv;
+  const int64_t first = wg / p.groups * TPW;
+  if (first >= p.tokens) return;  // the whole warp
+  const bool here = first + sub < p.tokens;
+  const int64_t token = here ? first + sub : first;
+  const int r0 = static_cast<int>(wg % p.groups) * p.rows_per_block, r1 = min(rows, r0 + p.rows_per_block);
+  const int b = static_cast<int>(token / p.S), i = static_cast<int>(token - static_cast<int64_t>(b) * p.S);
+  const int len = p.lens[b];
+  const int n = p.n_new ? min(max(p.n_new[b], 0), p.S) : p.S;
+  const bool live = here && i < n;
+  const int64_t row = static_cast<int64_t>(len) + i;
+  const bool fits = len >= 0 && static_cast<int64_t>(len) + n <= p.cap;
+  if (live && !fits && l == 0) report_error(p.status, HQ_ERR_INVALID_ARGUMENT);
+  const bool write = live && fits;
+  const double pos = static_cast<double>(row + (p.pos_offset ? p.pos_offset[b] : 0));
+  const int half = p.rot / 2;
+  const bool turned = d0 < p.rot;
+  const bool lead = d0 < half;                 // half layout: this lane's side of its pairs
+  const int j0 = p.inter ? d0 / 2 : lead ? d0 : d0 - half;
+  // y = x cs + o sg, o the partner
+  float cs[8], sg[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    cs[e] = 1.0f;
+    sg[e] = 0.0f;
+  }
+  if (turned && r0 < p.Hq + p.Hkv) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (p.inter && (e & 1)) {
+        cs[e] = cs[e - 1];
+        sg[e] = -sg[e - 1];
+        continue;
+      }
+      const int j = j0 + (p.inter ? e / 2 : e);
+      const double turns = pos * static_cast<double>(p.inv_freq[j]) * 0.15915494309189535;
+      const double f = 2.0 * (turns - rint(turns));  // angle / pi
+      const float h = static_cast<float>(f), r = static_cast<float>(f - h) * 3.14159265f;
+      float s, c;
+      sincospif(h, &s, &c);
+      const float c1 = __fmaf_rn(-s, r, c), s1 = __fmaf_rn(c, r, s);
+      cs[e] = c1 * p.factor;
+      sg[e] = (p.inter || lead ? -s1 : s1) * p.factor;
+    }
+  }
+  // the lane that holds this lane's partners
+  const int partner = sub * LPR + (p.inter || !turned ? l : lead ? l + half / 8 : l - half / 8);
+
+  // One loop per kind of row, a row per turn with the next two in flight: short loops, since
+  // the three kinds unrolled side by side ran at a quarter of this speed (the code of a turn
+  // left the schedulers' instruction caches).
+  auto each = [&](const void* src, const int64_t (&st)[3], int h0, int h1, auto&& row_of) {
+    const char* base = static_cast<const char*>(src) + 2 * (b * st[0] + i * st[2] + d0);
+    const int64_t step = 2 * st[1];
+    uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
+    if (h0 < h1) x0 = ld_stream(base + h0 * step);
+    if (h0 + 1 < h1) x1 = ld_stream(base + (h0 + 1) * step);
+#pragma unroll 1
+    for (int h = h0; h < h1; ++h) {
+      const uint4 x = x0;
+      x0 = x1;
+      if (h + 2 < h1) x1 = ld_stream(base + (h + 2) * step);
+      row_of(h, x);
+    }
+  };
+  auto partners = [&](const uint4& x, const float (&f)[8], float (&o)[8]) {
+    if (p.inter) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = f[e ^ 1];
+    } else {
+      uint4 w;
+      w.x = __shfl_sync(0xffffffffu, x.x, partner);
+      w.y = __shfl_sync(0xffffffffu, x.y, partner);
+      w.z = __shfl_sync(0xffffffffu, x.z, partner);
+      w.w = __shfl_sync(0xffffffffu, x.w, partner);
+      Vec16<DT>::unpack(w, o);
+    }
+  };
+  each(p.q, p.qs, r0, min(r1, p.Hq), [&](int h, const uint4& x) {
+    float f[8], o[8], y[8];
+    Vec16<DT>::unpack(x, f);
+    partners(x, f, o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = __fmaf_rn(f[e], cs[e], o[e] * sg[e]);
+    uint4 w = x;
+    if (live) w = make_uint4(pack16<DT>(y[0], y[1]), pack16<DT>(y[2], y[3]), pack16<DT>(y[4], y[5]),
+                             pack16<DT>(y[6], y[7]));
+    if (here)
+      *reinterpret_cast<uint4*>(static_cast<char*>(p.q_out) +
+                                2 * (b * p.qos[0] + h * p.qos[1] + i * p.qos[2] + d0)) = w;
+  });
+  each(p.k, p.ks, max(r0 - p.Hq, 0), min(r1 - p.Hq, p.Hkv), [&](int h, const uint4& x) {
+    float f[8], o[8], sc[8];
+    Vec16<DT>::unpack(x, f);
+    partners(x, f, o);
+    const int64_t si = b * p.kss[0] + h * p.kss[1] + d0 * p.kss[2];
+    if (p.ks_vec && p.s_dt == HQ_DTYPE_F16) {
+      Vec16<HQ_DTYPE_F16>::unpack(*reinterpret_cast<const uint4*>(static_cast<const __half*>(p.ksc) + si), sc);
+    } else if (p.ks_vec) {
+      Vec16<HQ_DTYPE_F32>::unpack(*reinterpret_cast<const uint4*>(static_cast<const float*>(p.ksc) + si), sc);
+      Vec16<HQ_DTYPE_F32>::unpack(*reinterpret_cast<const uint4*>(static_cast<const float*>(p.ksc) + si + 4), sc + 4);
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) {
+        const float v = p.s_dt == HQ_DTYPE_F16 ? __half2float(static_cast<const __half*>(p.ksc)[si + e * p.kss[2]])
+                                               : static_cast<const float*>(p.ksc)[si + e * p.kss[2]];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) sc[g] = g == e ? v : sc[g];
+      }
+    }
+    // |error of t| <= (|x| + |o|) / scale 2^-21 + 2^-15 for |t| < 128
+    float t[8];
+    uint32_t near = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float rs;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rs) : "f"(sc[e]));
+      t[e] = __fmaf_rn(f[e], cs[e], o[e] * sg[e]) * rs;
+      const float k0 = rintf(t[e]);
+      const float slack = __fmaf_rn((fabsf(f[e]) + fabsf(o[e])) * rs, p.slack, 3.0517578e-5f);
+      if (!(fabsf(t[e] - k0) + slack < 0.5f) && !(fabsf(t[e]) > 128.0f)) near |= 1u << e;
+      t[e] = fminf(fmaxf(k0, -127.0f), 127.0f) + 12582912.0f;  // the code in the low byte
+    }
+    if (write) {
+      uint32_t lo = pack_low_bytes(f2_make(t[0], t[1]), f2_make(t[2], t[3]));
+      uint32_t hi = pack_low_bytes(f2_make(t[4], t[5]), f2_make(t[6], t[7]));
+      while (near) {
+        const int e = __ffs(near) - 1;
+        near &= near - 1;
+        float fe = 0.0f, oe = 0.0f, se = 1.0f;
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+          if (g == e) {
+            fe = f[g];
+            oe = o[g];
+            se = sc[g];
+          }
+        const int j = j0 + (p.inter ? e / 2 : e);
+        const uint32_t c = exact_code(fe, oe, p.inter ? !(e & 1) : lead, turned,
+                                      turned ? pos * static_cast<double>(p.inv_freq[j]) : 0.0,
+                                      p.factor, se) & 0xff;
+        const int at = 8 * (e & 3);
+        if (e < 4) lo = (lo & ~(0xffu << at)) | c << at;
+        else hi = (hi & ~(0xffu << at)) | c << at;
+      }
+      *reinterpret_cast<uint2*>(p.kc + b * p.cs[0] + h * p.cs[1] + row * p.cs[2] + d0) = make_uint2(lo, hi);
+    }
+  });
+  each(p.v, p.vs, max(r0 - p.Hq - p.Hkv, 0), r1 - p.Hq - p.Hkv, [&](int h, const uint4& x) {
+    float f[8];
+    Vec16<DT>::unpack(x, f);
+    uint32_t a = absmax_x2<DT>(absmax_x2<DT>(x.x, x.y), absmax_x2<DT>(x.z, x.w));
+    float m = absmax_of_x2<DT>(a);
+#pragma unroll
+    for (int o = LPR / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (write) {
+      const Quantizer qz = Quantizer::from_amax16(m);
+      // the branch-free exact quotient of 16-bit inputs
+      const F2 ns = f2_make(-qz.scale, -qz.scale), rc = f2_make(qz.rcp, qz.rcp);
+      F2 y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = round_magic(quot_pair(f2_make(f[2 * e], f[2 * e + 1]), ns, rc));
+      *reinterpret_cast<uint2*>(p.vc + b * p.cs[0] + h * p.cs[1] + row * p.cs[2] + d0) =
+          make_uint2(pack_low_bytes(y[0], y[1]), pack_low_bytes(y[2], y[3]));
+      if (l == 0) {
+        const int64_t so = b * p.vss[0] + h * p.vss[1] + row * p.vss[2];
+        if (p.s_dt == HQ_DTYPE_F16) static_cast<__half*>(p.vsc)[so] = __float2half_rn(qz.scale);
+        else static_cast<float*>(p.vsc)[so] = qz.scale;
+      }
+    }
+  });
+}
+
+template <int DT, int D>
+int launch16(Params p, int B, cudaStream_t st) {
+  constexpr int TPW = 32 / (D / 8);
+  p.tokens = static_cast<int64_t>(B) * p.S;
+  const int rows = p.Hq + 2 * p.Hkv;
+  const int64_t warps = (p.tokens + TPW - 1) / TPW;
+  // a token's rows stay with one warp (its cos and sin made once) as long as that leaves 16
+  // warps per SM; below, they are split, down to one row per warp
+  const int64_t want = std::max<int64_t>(1, 16LL * current_sm_count() / warps);
+  const int groups = static_cast<int>(std::min<int64_t>(rows, want));
+  p.rows_per_block = (rows + groups - 1) / groups;
+  p.groups = (rows + p.rows_per_block - 1) / p.rows_per_block;
+  const size_t es = p.s_dt == HQ_DTYPE_F16 ? 2 : 4;
+  p.ks_vec = p.kss[2] == 1 && reinterpret_cast<uintptr_t>(p.ksc) % 16 == 0 &&
+             p.kss[0] * es % 16 == 0 && p.kss[1] * es % 16 == 0;
+  p.slack = fmaxf(1.0f, fabsf(p.factor)) * 4.76837158e-7f;  // 2^-21
+  const int64_t blocks = (warps * p.groups + kThreads16 / 32 - 1) / (kThreads16 / 32);
+  if (blocks > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
+  rope_append16_kernel<DT, D><<<static_cast<unsigned>(blocks), kThreads16, 0, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? HQ_OK : static_cast<int>(e);
+}
+
+// ---------------------------------------------------------------- any type and rotary size
 template <int DT, int D>
 int launch(Params p, int B, cudaStream_t st) {
   const int64_t tokens = static_cast<int64_t>(B) * p.S;
@@ -193,6 +448,13 @@ int launch(Params p, int B, cudaStream_t st) {
 
 template <int DT>
 int dispatch(const Params& p, int B, cudaStream_t st) {
+  if constexpr (DT != HQ_DTYPE_F32) {
+    if (p.rot % 16 == 0) {
+      if (p.D == 64) return launch16<DT, 64>(p, B, st);
+      if (p.D == 128) return launch16<DT, 128>(p, B, st);
+      return launch16<DT, 256>(p, B, st);
+    }
+  }
   if (p.D == 64) return launch<DT, 64>(p, B, st);
   if (p.D == 128) return launch<DT, 128>(p, B, st);
   return launch<DT, 256>(p, B, st);

@@ -1,0 +1,406 @@
+// Plans, joining of partial states and entry points of the attention over int8 caches whose
+// sequences have lengths of their own: sliding window with sinks (decode, prefill) and decode
+// over a shared prefix.  The kernels are in ragged_attn.cu and ragged_rows.cu.
+#include <algorithm>
+
+#include "ragged_common.cuh"
+
+namespace hq {
+namespace rag {
+
+// ---------------------------------------------------------------- joining the pieces
+struct Source {
+  Params p;
+  int grid, mt;    // blocks that shared the line of tiles; rows per row tile
+  int per_entry;   // sequences per entry (a prefix: those of its group)
+};
+
+// The partial rows of one output row in one source: first row, count, distance.
+struct Run {
+  const float* at;
+  int n;
+  int64_t step;
+};
+// STREAM: the blocks that hold tiles T0 .. T1 - 1 of a unit are T0 / per .. (T1 - 1) / per, and
+// their pieces have consecutive slots.  n < 0: the row was written by the one block that held
+// all of its tiles.
+__device__ __forceinline__ Run stream_run(const Source& s, int b, int kvh, int hr) {
+  const Params& p = s.p;
+  const int e = b / s.per_entry, r = (b - e * s.per_entry) * p.nrep + hr;
+  const int rt = r / s.mt, n_rt = row_tiles(p.seg.units * p.nrep, s.mt), idx = rt * p.Hkv + kvh;
+  const int per = tiles_per_block(p, p.cum[p.seg.nb], s.grid);
+  const int nt = (p.cum[e + 1] - p.cum[e]) / (p.Hkv * n_rt);
+  if (nt == 0) return {nullptr, 0, 0};
+  const int T0 = p.cum[e] + idx * nt, c0 = T0 / per, c1 = (T0 + nt - 1) / per;
+  if (!p.merge_all && c0 == c1) return {nullptr, -1, 0};
+  return {part_row(p, e * p.Hkv * n_rt + idx + c0, r - rt * s.mt), c1 - c0 + 1,
+          static_cast<int64_t>(p.rows_cap) * kPartRow};
+}
+// Prefill: the n_split pieces of query u's row tile.
+__device__ __forceinline__ Run split_run(const Source& s, int b, int u, int kvh, int hr) {
+  const Params& p = s.p;
+  const int r = u * p.nrep + hr, rt = r / s.mt;
+  return {part_row(p, ((b * p.Hkv + kvh) * p.n_rt + rt) * p.n_split, r - rt * s.mt), p.n_split,
+          static_cast<int64_t>(p.rows_cap) * kPartRow};
+}
+
+// One warp per output row (b, u, h), 4 channels per lane: the pieces' common maximum, then
+// their weighted sums.
+template <int NSRC, bool STREAM>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Source s0,
+                                                      const __grid_constant__ Source s1, int rows,
+                                                      int units) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const Params& p = s0.p;
+  const int Hq = p.Hkv * p.nrep;
+  const int h = row % Hq, bu = row / Hq, b = bu / units, u = bu - b * units;
+  const int kvh = h / p.nrep, hr = h - kvh * p.nrep;
+  Run run[NSRC];
+  if constexpr (STREAM) {
+    run[0] = stream_run(s0, b, kvh, hr);
+    if (run[0].n < 0) return;
+    if constexpr (NSRC > 1) run[1] = stream_run(s1, b, kvh, hr);
+  } else {
+    const int nq = p.q_lens ? min(max(p.q_lens[b], 0), p.seg.units) : p.seg.units;
+    if (u >= nq) return;
+    run[0] = split_run(s0, b, u, kvh, hr);
+  }
+  float M = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < NSRC; ++k)
+    for (int i = lane; i < run[k].n; i += 32) M = fmaxf(M, run[k].at[i * run[k].step]);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float L = 0.0f;
+  if (M != -INFINITY) {
+#pragma unroll
+    for (int k = 0; k < NSRC; ++k)
+#pragma unroll 4
+      for (int i = 0; i < run[k].n; ++i) {
+        const float* x = run[k].at + i * run[k].step;
+        const float2 ml = *reinterpret_cast<const float2*>(x);
+        const float4 o = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
+        const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+        L += f * ml.y;
+        acc.x += f * o.x;
+        acc.y += f * o.y;
+        acc.z += f * o.z;
+        acc.w += f * o.w;
+      }
+  }
+  const float inv = L <= 0.0f ? 0.0f : 1.0f / L;  // (a NaN stays)
+  store4(out_row(p, b, u, h), p.q_dt, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+}
+
+template <int NSRC, bool STREAM>
+int combine(const Source& s0, const Source& s1, int rows, int units, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((rows + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, combine_kernel<NSRC, STREAM>, s0, s1, rows, units);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return static_cast<int>(e);
+  }
+  return HQ_OK;
+}
+
+// ---------------------------------------------------------------- plans
+inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+inline bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Row tiles per block: two for more than 128 rows; float16 models (q' in two parts, whose
+// second tile takes the shared memory of a second row tile) always one.
+inline int tiles_of(int q_dt, int64_t rows) { return q_dt == HQ_DTYPE_F16 || rows <= 128 ? 1 : 2; }
+
+// One line of tiles: `entries` sequences or groups with `rows` rows per kv head each.
+struct Stream {
+  bool few;          // ragged_rows.cu (two blocks per SM, no tensor memory)
+  int nm, mt, grid, rows_cap;
+  int64_t part_floats;
+  size_t cum_bytes;
+  size_t bytes() const { return cum_bytes + align256(sizeof(float) * static_cast<size_t>(part_floats)); }
+};
+inline bool plan_stream(Stream& pl, int q_dt, int Hkv, int entries, int64_t rows, int cap) {
+  pl = Stream{};
+  // up to 4 rows: the int8 tensor-core kernel, whose work per key grows with the rows and which
+  // needs no conversion of the codes; more: 128 rows at a time
+  pl.few = rows <= kMaxRows;
+  pl.nm = pl.few ? 1 : tiles_of(q_dt, rows);
+  pl.mt = 128 * pl.nm;
+  const int64_t units = int64_t(entries) * Hkv * ((rows + pl.mt - 1) / pl.mt);
+  const int64_t tiles = units * (cap / kBN + 1);
+  if (tiles > (int64_t(1) << 30) || entries > kMaxEntries || rows > (1 << 24)) return false;
+  pl.grid = static_cast<int>(std::min<int64_t>((pl.few ? 2 : 1) * int64_t(current_sm_count()),
+                                               std::max<int64_t>(tiles, 1)));
+  pl.rows_cap = static_cast<int>(std::min<int64_t>(rows, pl.mt));
+  pl.part_floats = (units + pl.grid) * pl.rows_cap * kPartRow;
+  pl.cum_bytes = align256(sizeof(int) * (entries + 1));
+  return true;
+}
+inline void attach(Params& p, const Stream& pl, char* ws) {
+  p.cum = reinterpret_cast<int*>(ws);
+  p.part = reinterpret_cast<float*>(ws + pl.cum_bytes);
+  p.rows_cap = pl.rows_cap;
+  p.min_tiles = 1;
+}
+inline int run_stream(const Params& p, const Stream& pl, cudaStream_t st) {
+  return pl.few ? rows_stream(p, pl.grid, st) : tiles_stream(p, pl.nm, pl.grid, st);
+}
+
+// Prefill plan: one block per row tile; with fewer blocks than SMs the keys of each row
+// tile are split, down to two key tiles per block.
+struct Prefill {
+  int nm, n_rt, n_split, rows_cap;
+  int64_t part_floats;
+  size_t bytes() const { return align256(sizeof(float) * static_cast<size_t>(part_floats)); }
+};
+inline bool plan_prefill(Prefill& pl, int q_dt, int B, int Hkv, int nrep, int Sq, int cap, int window,
+                         int sinks) {
+  pl = Prefill{};
+  const int64_t rows = int64_t(Sq) * nrep;
+  if (rows > (1 << 30)) return false;
+  pl.nm = tiles_of(q_dt, rows);
+  // small grids keep one row tile per block
+  if (pl.nm == 2 && int64_t(B) * Hkv * ((rows + 255) / 256) < current_sm_count()) pl.nm = 1;
+  const int MT = 128 * pl.nm;
+  pl.n_rt = static_cast<int>((rows + MT - 1) / MT);
+  const int64_t units = int64_t(B) * Hkv * pl.n_rt;
+  if (units * 64 > (int64_t(1) << 31) - 1 || int64_t(Hkv) * pl.n_rt > 65535) return false;
+  const int64_t seen = std::min<int64_t>(cap, int64_t(window) + sinks + MT / nrep + 1);
+  const int64_t nt = std::max<int64_t>(1, (seen + kBN - 1) / kBN);
+  const int sms = current_sm_count();
+  pl.n_split = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, sms / std::max<int64_t>(units, 1)),
+                                                   std::max<int64_t>(1, nt / 2), 16}));
+  pl.rows_cap = static_cast<int>(std::min<int64_t>(rows, MT));
+  pl.part_floats = pl.n_split > 1 ? units * pl.n_split * pl.rows_cap * kPartRow : 0;
+  return true;
+}
+
+// ---------------------------------------------------------------- arguments
+inline int fill_seg(Seg& s, const int8_t* k, const int8_t* v, const int64_t* kvs, const void* ksc,
+                    const void* vsc, const int64_t* kss, const int64_t* vss, const int* lens,
+                    int cap, int nb, int units, int window, int sinks) {
+  if (cap > 0 && (!k || !v || !ksc || !vsc)) return HQ_ERR_INVALID_ARGUMENT;
+  if (!kvs || !kss || !vss || cap < 0 || nb < 0 || units < 0 || window < 0 || sinks < 0)
+    return HQ_ERR_INVALID_ARGUMENT;
+  if (!aligned(k, 16) || !aligned(v, 16) || kvs[0] % 16 || kvs[1] % 16 || kvs[2] % 16)
+    return HQ_ERR_INVALID_ARGUMENT;
+  s.k = k;
+  s.v = v;
+  s.sb = kvs[0];
+  s.sh = kvs[1];
+  s.ss = kvs[2];
+  s.ksc = ksc;
+  s.vsc = vsc;
+  s.kscb = kss[0];
+  s.ksch = kss[1];
+  s.kscd = kss[2];
+  s.vscb = vss[0];
+  s.vsch = vss[1];
+  s.vscs = vss[2];
+  s.lens = lens;
+  s.cap = cap;
+  s.nb = nb;
+  s.units = units;
+  s.window = window > 0 ? window : 1 << 30;
+  s.sinks = sinks;
+  return HQ_OK;
+}
+
+inline int check_common(const void* q, int q_dtype, const int64_t* qs, int nqs, const void* out,
+                        const int64_t* os, int scale_dtype, int Hq, int Hkv, int D) {
+  if (!q || !out || !qs || !os || Hq <= 0 || Hkv <= 0) return HQ_ERR_INVALID_ARGUMENT;
+  if (D != kD || Hq % Hkv || Hq / Hkv > 128 || Hq > 65535 ||
+      (q_dtype != HQ_DTYPE_BF16 && q_dtype != HQ_DTYPE_F16) ||
+      (scale_dtype != HQ_DTYPE_F32 && scale_dtype != HQ_DTYPE_F16))
+    return HQ_ERR_UNSUPPORTED;
+  if (qs[nqs - 1] != 1 || os[nqs - 1] != 1 || !aligned(q, 16) || !aligned(out, 8))
+    return HQ_ERR_INVALID_ARGUMENT;
+  for (int i = 0; i + 1 < nqs; ++i)
+    if (qs[i] % 8 || os[i] % 4) return HQ_ERR_INVALID_ARGUMENT;
+  return HQ_OK;
+}
+
+
+inline Params make_params(const void* q, int q_dtype, int64_t qsh, int scale_dtype, int Hq, int Hkv,
+                          float sm_scale, int q_quant, void* out, int64_t osb, int64_t osh,
+                          int* status) {
+  Params p{};
+  p.q = q;
+  p.qsh = qsh;
+  p.q_dt = q_dtype;
+  p.s_dt = scale_dtype;
+  p.Hkv = Hkv;
+  p.nrep = Hq / Hkv;
+  p.qk_scale = sm_scale * kLog2e;
+  p.q_quant = q_quant;
+  p.out = out;
+  p.osb = osb;
+  p.osh = osh;
+  p.status = status;
+  return p;
+}
+
+}  // namespace rag
+}  // namespace hq
+
+using namespace hq;
+
+extern "C" size_t hq_window_workspace_bytes(int q_dtype, int B, int Hq, int Hkv, int Sq, int S_max,
+                                            int D, int window, int sinks) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq < 0 || S_max < 0 || window < 0 || sinks < 0 ||
+      D != rag::kD || Hq % Hkv || Hq / Hkv > 128)
+    return 0;
+  if (Sq == 0) {
+    rag::Stream pl;
+    return rag::plan_stream(pl, q_dtype, Hkv, B, Hq / Hkv, S_max) ? std::max<size_t>(pl.bytes(), 256) : 0;
+  }
+  rag::Prefill pl;
+  return rag::plan_prefill(pl, q_dtype, B, Hkv, Hq / Hkv, Sq, S_max, window > 0 ? window : 1 << 30, sinks)
+             ? std::max<size_t>(pl.bytes(), 256)
+             : 0;
+}
+
+extern "C" int hq_window_decode_int8(const void* q, int q_dtype, const int64_t q_strides[3],
+                                     const int8_t* k, const int8_t* v, const int64_t kv_strides[3],
+                                     const void* k_scale, const void* v_scale, int scale_dtype,
+                                     const int64_t ksc_strides[3], const int64_t vsc_strides[3],
+                                     const int* lens, int B, int Hq, int Hkv, int S_max, int D,
+                                     int window, int sinks, float sm_scale, int q_quant, void* out,
+                                     const int64_t out_strides[3], void* workspace,
+                                     size_t workspace_bytes, int* status, hq_stream_t stream) {
+  int rc = rag::check_common(q, q_dtype, q_strides, 3, out, out_strides, scale_dtype, Hq, Hkv, D);
+  if (rc != HQ_OK) return rc;
+  if (B < 0) return HQ_ERR_INVALID_ARGUMENT;
+  rag::Source s{};
+  s.p = rag::make_params(q, q_dtype, q_strides[1], scale_dtype, Hq, Hkv, sm_scale, q_quant, out,
+                         out_strides[0], out_strides[1], status);
+  rc = rag::fill_seg(s.p.seg, k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
+                     S_max, B, 1, window, sinks);
+  if (rc != HQ_OK) return rc;
+  if (B == 0) return HQ_OK;
+  s.p.seg.qsb = q_strides[0];
+  rag::Stream pl;
+  if (!rag::plan_stream(pl, q_dtype, Hkv, B, Hq / Hkv, S_max)) return HQ_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < pl.bytes() || !rag::aligned(workspace, 256)) return HQ_ERR_WORKSPACE;
+  rag::attach(s.p, pl, static_cast<char*>(workspace));
+  s.grid = pl.grid;
+  s.mt = pl.mt;
+  s.per_entry = 1;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  rc = rag::run_stream(s.p, pl, st);
+  return rc != HQ_OK ? rc : rag::combine<1, true>(s, s, B * Hq, 1, st);
+}
+
+extern "C" int hq_window_prefill_int8(const void* q, int q_dtype, const int64_t q_strides[4],
+                                      const int8_t* k, const int8_t* v, const int64_t kv_strides[3],
+                                      const void* k_scale, const void* v_scale, int scale_dtype,
+                                      const int64_t ksc_strides[3], const int64_t vsc_strides[3],
+                                      const int* lens, const int* q_lens, int B, int Hq, int Hkv,
+                                      int Sq, int S_max, int D, int window, int sinks,
+                                      float sm_scale, int q_quant, void* out,
+                                      const int64_t out_strides[4], void* workspace,
+                                      size_t workspace_bytes, int* status, hq_stream_t stream) {
+  int rc = rag::check_common(q, q_dtype, q_strides, 4, out, out_strides, scale_dtype, Hq, Hkv, D);
+  if (rc != HQ_OK) return rc;
+  if (B < 0 || Sq < 0) return HQ_ERR_INVALID_ARGUMENT;
+  if (B > 65535 || int64_t(B) * Sq * Hq > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
+  rag::Source s{};
+  s.p = rag::make_params(q, q_dtype, q_strides[1], scale_dtype, Hq, Hkv, sm_scale, q_quant, out,
+                         out_strides[0], out_strides[1], status);
+  rc = rag::fill_seg(s.p.seg, k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
+                     S_max, B, Sq, window, sinks);
+  if (rc != HQ_OK) return rc;
+  if (B == 0 || Sq == 0) return HQ_OK;
+  s.p.seg.step = 1;
+  s.p.seg.qsb = q_strides[0];
+  s.p.seg.qsu = q_strides[2];
+  s.p.osu = out_strides[2];
+  s.p.q_lens = q_lens;
+  rag::Prefill pl;
+  if (!rag::plan_prefill(pl, q_dtype, B, Hkv, Hq / Hkv, Sq, S_max, s.p.seg.window, sinks))
+    return HQ_ERR_UNSUPPORTED;
+  if (pl.bytes() && (!workspace || workspace_bytes < pl.bytes() || !rag::aligned(workspace, 256)))
+    return HQ_ERR_WORKSPACE;
+  s.p.part = static_cast<float*>(workspace);
+  s.p.rows_cap = pl.rows_cap;
+  s.p.n_split = pl.n_split;
+  s.p.n_rt = pl.n_rt;
+  s.mt = 128 * pl.nm;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  rc = rag::tiles_prefill(s.p, pl.nm, B, st);
+  if (rc != HQ_OK || pl.n_split == 1) return rc;
+  return rag::combine<1, false>(s, s, B * Sq * Hq, Sq, st);
+}
+
+extern "C" size_t hq_prefix_decode_workspace_bytes(int q_dtype, int G, int B, int Hq, int Hkv,
+                                                   int P_max, int S_max, int D) {
+  if (G <= 0 || B <= 0 || B % G || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 128 || P_max < 0 ||
+      S_max < 0 || D != rag::kD)
+    return 0;
+  const int nrep = Hq / Hkv;
+  rag::Stream a, b;
+  if (!rag::plan_stream(a, q_dtype, Hkv, G, int64_t(B / G) * nrep, P_max) ||
+      !rag::plan_stream(b, q_dtype, Hkv, B, nrep, S_max))
+    return 0;
+  return a.bytes() + b.bytes();
+}
+
+extern "C" int hq_prefix_decode_int8(
+    const void* q, int q_dtype, const int64_t q_strides[3], const int8_t* pk, const int8_t* pv,
+    const int64_t pkv_strides[3], const void* pk_scale, const void* pv_scale,
+    const int64_t pksc_strides[3], const int64_t pvsc_strides[3], const int* prefix_lens, int G,
+    int P_max, const int8_t* k, const int8_t* v, const int64_t kv_strides[3], const void* k_scale,
+    const void* v_scale, const int64_t ksc_strides[3], const int64_t vsc_strides[3],
+    const int* lens, int S_max, int scale_dtype, int B, int Hq, int Hkv, int D, float sm_scale,
+    int q_quant, void* out, const int64_t out_strides[3], void* workspace, size_t workspace_bytes,
+    int* status, hq_stream_t stream) {
+  int rc = rag::check_common(q, q_dtype, q_strides, 3, out, out_strides, scale_dtype, Hq, Hkv, D);
+  if (rc != HQ_OK) return rc;
+  if (B < 0 || G <= 0 || B % G) return HQ_ERR_INVALID_ARGUMENT;
+  rag::Source own{}, pre{};
+  own.p = rag::make_params(q, q_dtype, q_strides[1], scale_dtype, Hq, Hkv, sm_scale, q_quant, out,
+                           out_strides[0], out_strides[1], status);
+  own.p.merge_all = 1;
+  pre.p = own.p;
+  rc = rag::fill_seg(pre.p.seg, pk, pv, pkv_strides, pk_scale, pv_scale, pksc_strides, pvsc_strides,
+                     prefix_lens, P_max, G, B / G, 0, 0);
+  if (rc == HQ_OK)
+    rc = rag::fill_seg(own.p.seg, k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
+                       S_max, B, 1, 0, 0);
+  if (rc != HQ_OK) return rc;
+  if (B == 0) return HQ_OK;
+  const int nrep = Hq / Hkv;
+  rag::Stream a, b;
+  if (!rag::plan_stream(a, q_dtype, Hkv, G, int64_t(B / G) * nrep, P_max) ||
+      !rag::plan_stream(b, q_dtype, Hkv, B, nrep, S_max))
+    return HQ_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < a.bytes() + b.bytes() || !rag::aligned(workspace, 256))
+    return HQ_ERR_WORKSPACE;
+  rag::attach(pre.p, a, static_cast<char*>(workspace));
+  rag::attach(own.p, b, static_cast<char*>(workspace) + a.bytes());
+  pre.p.seg.qsb = q_strides[0] * (B / G);
+  pre.p.seg.qsu = q_strides[0];
+  own.p.seg.qsb = q_strides[0];
+  pre.grid = a.grid;
+  pre.mt = a.mt;
+  pre.per_entry = B / G;
+  own.grid = b.grid;
+  own.mt = b.mt;
+  own.per_entry = 1;
+  own.p.after = 1;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  rc = rag::run_stream(pre.p, a, st);
+  if (rc == HQ_OK) rc = rag::run_stream(own.p, b, st);
+  return rc != HQ_OK ? rc : rag::combine<2, true>(own, pre, B * Hq, 1, st);
+}

@@ -41,71 +41,22 @@
 // memory, where it overwrites the S it came from.  mbarriers order the roles; every wait is
 // bounded.  (Codes loaded into registers and converted from there took 4000 cycles a tile:
 // the proxy fence before each hand-over waited for the loads of the next tile.)
-#include <algorithm>
-#include <atomic>
-
-#include "hq_common.cuh"
+#include "ragged_common.cuh"
 #include "umma.cuh"
 
 namespace hq {
-int current_sm_count();
-
 namespace rag {
 using namespace tc;
 
-constexpr int kD = 128;
-constexpr int kBN = 128;                  // keys per tile
 constexpr int kConvThreads = 128;
 constexpr int kTileB = kBN * kD * 2;      // a float16 K, V or Q tile: 32 KB
 constexpr int kStages = 2;                // K and V tiles in shared memory
 constexpr int kSlotKeys = 64;             // keys of a staging slot (K or V codes)
 constexpr int kSlotB = kSlotKeys * kD;
 constexpr int kLvSlots = 2;               // ring of what the tiles' V scales lead to
-constexpr int kMaxEntries = 1536;         // sequences plus groups of one call
-constexpr int kPartRow = kD + 4;          // partial rows: m, l, two pad words, o
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 256;           // S buffers at columns 0 and 128
-
-// One set of keys and the rows that read it.
-struct Seg {
-  const int8_t* k;
-  const int8_t* v;
-  int64_t sb, sh, ss;                     // strides of both (b, h, token)
-  const void* ksc;
-  const void* vsc;
-  int64_t kscb, ksch, kscd, vscb, vsch, vscs;
-  const int* lens;                        // tokens held, per entry; null: cap
-  int cap;
-  int nb;                                 // entries (sequences, or groups)
-  int units;                              // queries per entry
-  int step;                               // 1: query u stands u positions after query 0
-  int64_t qsb, qsu;
-  int window, sinks;
-};
-
-struct Params {
-  Seg seg[2];
-  int nseg;
-  const void* q;
-  int64_t qsh;
-  int q_dt, s_dt;
-  int Hkv, nrep;
-  float qk_scale;                         // sm_scale * log2(e)
-  int q_quant;
-  const int* q_lens;                      // prefill: queries per sequence; null: all
-  void* out;                              // rows [b][u][h]
-  int64_t osb, osu, osh;
-  float* part;                            // partial states
-  int* cum;                               // STREAM: first tile of each entry, for combine_kernel
-  int* status;
-  int n_split, n_rt;                      // prefill grid: splits, row tiles
-  int merge_all;                          // every piece goes through combine_kernel
-  int rows_cap[2];                        // partial rows per piece of each segment
-  int64_t part1;                          // float offset of the second segment's pieces
-  int min_tiles;                          // STREAM: least tiles per block
-};
 
 template <int NM, bool LO>
 struct Cfg {
@@ -130,14 +81,6 @@ struct Cfg {
 };
 
 // ---------------------------------------------------------------- small helpers
-__device__ __forceinline__ float load_scale(const void* p, int64_t i, int dt) {
-  return dt == HQ_DTYPE_F16 ? __half2float(static_cast<const __half*>(p)[i])
-                            : static_cast<const float*>(p)[i];
-}
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
@@ -226,144 +169,6 @@ __device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, volatile 
 }
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return mbar_try_wait(bar, parity) || wait_long(bar, parity, abort);
-}
-
-// ---------------------------------------------------------------- pieces of work
-// The keys of one row tile, numbered v = 0 .. nv - 1: key = v < ns ? v : v + sh.
-struct Keys {
-  int pos0;        // position of the entry's query 0
-  int ns, sh, nv, nt;
-};
-__device__ __forceinline__ int seg_len(const Seg& s, int b) {
-  return s.lens ? min(max(s.lens[b], 0), s.cap) : s.cap;
-}
-// n tokens held, nq queries of which rows u_lo .. u_hi are in the tile
-__device__ __forceinline__ Keys make_keys(const Seg& s, int n, int nq, int u_lo, int u_hi) {
-  Keys k;
-  k.pos0 = s.step ? n - nq : n - 1;
-  const int p_lo = k.pos0 + (s.step ? u_lo : 0), p_hi = k.pos0 + (s.step ? u_hi : 0);
-  const int w0 = max(0, p_lo - s.window + 1);
-  if (w0 <= s.sinks) {
-    k.ns = 0;
-    k.sh = 0;
-    k.nv = p_hi + 1;
-  } else {
-    k.ns = s.sinks;
-    k.sh = w0 - s.sinks;
-    k.nv = p_hi + 1 - k.sh;
-  }
-  k.nv = max(k.nv, 0);
-  k.nt = (k.nv + kBN - 1) / kBN;
-  return k;
-}
-struct Piece {
-  int seg, b, kvh, row0, rows;
-  Keys key;
-  int t0, t1;
-  int slot;        // -1: final output
-};
-
-// STREAM: tiles of entry e, one row tile (0: the call is answered by combine_kernel)
-__device__ __forceinline__ int entry_tiles(const Params& p, int e) {
-  const int si = e < p.seg[0].nb ? 0 : 1;
-  const Seg& s = p.seg[si];
-  const int n = seg_len(s, e - (si ? p.seg[0].nb : 0));
-  const int nt = make_keys(s, n, s.units, 0, 0).nt;
-  return p.merge_all ? nt : max(nt, 1);
-}
-__device__ __host__ __forceinline__ int row_tiles(int rows, int mt) { return (rows + mt - 1) / mt; }
-
-// The pieces of one block, in order.  (A call: every role walks them.)
-struct Walk {
-  int cur, end, e;
-};
-template <int MT, bool STREAM>
-__device__ __forceinline__ Walk walk_start(const Params& p, const int* cum) {
-  Walk k{0, 1, 0};
-  if constexpr (STREAM) {
-    const int ne = p.seg[0].nb + (p.nseg > 1 ? p.seg[1].nb : 0);
-    const int total = cum[ne];
-    const int per = max(p.min_tiles, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-    k.cur = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total)));
-    k.end = static_cast<int>(min(static_cast<int64_t>(k.cur) + per, static_cast<int64_t>(total)));
-    // the entry that holds tile cur: cum[e] <= cur < cum[e + 1]
-    int lo = 0, hi = ne - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (cum[mid] <= k.cur) lo = mid; else hi = mid - 1;
-    }
-    k.e = lo;
-  }
-  return k;
-}
-template <int MT, bool STREAM>
-__device__ __noinline__ bool walk_next(Walk& k, const Params& p, const int* cum, Piece& w) {
-  if (k.cur >= k.end) return false;
-  if constexpr (STREAM) {
-    while (cum[k.e + 1] <= k.cur) ++k.e;
-    w.seg = k.e < p.seg[0].nb ? 0 : 1;
-    const Seg& s = p.seg[w.seg];
-    w.b = k.e - (w.seg ? p.seg[0].nb : 0);
-    const int rows = s.units * p.nrep, n_rt = row_tiles(rows, MT), per_e = p.Hkv * n_rt;
-    const uint32_t nt = static_cast<uint32_t>(cum[k.e + 1] - cum[k.e]) / static_cast<uint32_t>(per_e);
-    const int idx = static_cast<uint32_t>(k.cur - cum[k.e]) / nt, first = cum[k.e] + idx * nt;
-    const int rt = static_cast<uint32_t>(idx) / static_cast<uint32_t>(p.Hkv);
-    w.kvh = idx - rt * p.Hkv;
-    w.row0 = rt * MT;
-    w.rows = min(MT, rows - w.row0);
-    w.key = make_keys(s, seg_len(s, w.b), s.units, 0, 0);
-    w.t0 = k.cur - first;
-    w.t1 = min(static_cast<int>(nt), w.t0 + k.end - k.cur);
-    k.cur = first + w.t1;
-    w.slot = !p.merge_all && w.t0 == 0 && w.t1 == static_cast<int>(nt)
-                 ? -1
-                 : w.b * per_e + idx + static_cast<int>(blockIdx.x);
-  } else {
-    k.cur = 1;
-    // longest row tiles (the last ones of a causal chunk) first
-    const int rq = static_cast<uint32_t>(blockIdx.y) / static_cast<uint32_t>(p.Hkv);
-    const int rt = p.n_rt - 1 - rq;
-    const int b = blockIdx.z;
-    const Seg& s = p.seg[0];
-    const int nq = p.q_lens ? min(max(p.q_lens[b], 0), s.units) : s.units;
-    w.seg = 0;
-    w.b = b;
-    w.kvh = static_cast<int>(blockIdx.y) - rq * p.Hkv;
-    w.row0 = rt * MT;
-    w.rows = min(MT, nq * p.nrep - w.row0);
-    if (w.rows <= 0) return false;
-    w.key = make_keys(s, seg_len(s, b), nq, static_cast<uint32_t>(w.row0) / static_cast<uint32_t>(p.nrep),
-                      static_cast<uint32_t>(w.row0 + w.rows - 1) / static_cast<uint32_t>(p.nrep));
-    const uint32_t nt = max(w.key.nt, 1), ns = p.n_split, split = blockIdx.x;  // nt < 2^24, ns <= 16
-    w.t0 = static_cast<int>(nt * split / ns);
-    w.t1 = static_cast<int>(nt * (split + 1) / ns);
-    w.slot = ns == 1 ? -1 : ((b * p.Hkv + w.kvh) * p.n_rt + rt) * static_cast<int>(ns) + static_cast<int>(split);
-  }
-  return true;
-}
-
-__device__ __forceinline__ float* part_row(const Params& p, int seg, int slot, int r) {
-  return p.part + (seg ? p.part1 : 0) +
-         (static_cast<int64_t>(slot) * p.rows_cap[seg] + r) * kPartRow;
-}
-
-// Stores 4 consecutive values of an output row.
-__device__ __forceinline__ void store4(void* row, int dt, int d, float a, float b, float c, float e) {
-  uint2 w;
-  if (dt == HQ_DTYPE_BF16) {
-    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, e);
-    w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-  } else {
-    w = make_uint2(pack_h2(a, b), pack_h2(c, e));
-  }
-  *reinterpret_cast<uint2*>(static_cast<char*>(row) + 2 * d) = w;
-}
-__device__ __forceinline__ uint32_t pack_pair(float a, float b, int dt) {
-  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
-  return dt == HQ_DTYPE_BF16 ? *reinterpret_cast<const uint32_t*>(&x) : pack_h2(a, b);
-}
-__device__ __forceinline__ char* out_row(const Params& p, int b, int u, int h) {
-  return static_cast<char*>(p.out) + 2 * (b * p.osb + u * p.osu + h * p.osh);
 }
 
 __device__ __forceinline__ void unpack8(const uint4& x, int dt, float (&f)[8]) {
@@ -661,31 +466,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       fence_mbar_init();
     }
   }
-  if constexpr (STREAM) {  // cum[e]: first tile of entry e in the line of all tiles
-    const int ne = p.seg[0].nb + (p.nseg > 1 ? p.seg[1].nb : 0);
-    for (int e = tid; e < ne; e += C::kThreads) {
-      const int si = e < p.seg[0].nb ? 0 : 1;
-      cum[e + 1] = entry_tiles(p, e) * p.Hkv * row_tiles(p.seg[si].units * p.nrep, MT);
-    }
-    __syncthreads();
-    if (warp == 0) {
-      int run = 0;
-      if (lane == 0) cum[0] = 0;
-      for (int e0 = 0; e0 < ne; e0 += 32) {
-        int x = e0 + lane < ne ? cum[e0 + lane + 1] : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, x, o);
-          if (lane >= o) x += y;
-        }
-        if (e0 + lane < ne) cum[e0 + lane + 1] = run + x;
-        run += __shfl_sync(0xffffffffu, x, 31);
-      }
-      __syncwarp();
-      if (blockIdx.x == 0)
-        for (int e = lane; e <= ne; e += 32) p.cum[e] = cum[e];
-    }
-  }
+  if constexpr (STREAM) build_cum<MT>(p, cum, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -757,7 +538,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
     for (; ok && next_piece(walk, w); ++pc) {
       const int n_tiles = w.t1 - w.t0;
       float m = -INFINITY, l = 0.0f, fac = 0.0f, vscale = 1.0f;
-      const Seg& s = p.seg[w.seg];
+      const Seg& s = p.seg;
       const bool live = r < w.rows;
       const int u = (w.row0 + r) / p.nrep, h = w.kvh * p.nrep + (w.row0 + r) - u * p.nrep;
       if (n_tiles > 0) {
@@ -856,7 +637,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
           }
           __syncwarp();
         } else {
-          float* prt = part_row(p, w.seg, w.slot, r);
+          float* prt = part_row(p, w.slot, r);
           if (live) *reinterpret_cast<float2*>(prt) = make_float2(have ? m : -INFINITY, have ? l : 0.0f);
 #pragma unroll 1
           for (int c = 0; c < 128; c += 16) {
@@ -955,7 +736,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
     int sc = 0;
     bool ok = true;
     for (; ok && next_piece(walk, w);) {
-      const Seg& s = p.seg[w.seg];
+      const Seg& s = p.seg;
       const int64_t o = w.b * s.sb + w.kvh * s.sh;
 #pragma unroll 1
       for (int t2 = 4 * w.t0; ok && t2 < 4 * w.t1; ++t2, ++sc) {  // K 0 .., K 64 .., V 0 .., V 64 ..
@@ -1004,7 +785,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         } while (lp.t0 >= lp.t1);
         lt = lp.t0;
       }
-      const Seg& s = p.seg[lp.seg];
+      const Seg& s = p.seg;
       const int64_t vs0 = lp.b * s.vscb + lp.kvh * s.vsch;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -1205,405 +986,34 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
                  "r"(kTmemCols)
                  : "memory");
   }
-}
-
-// ---------------------------------------------------------------- joining the pieces
-// One warp per output row (b, u, h), 4 channels per lane: the pieces' common maximum, then
-// their weighted sums.  STREAM: the blocks that hold tiles T0 .. T1 - 1 of a unit are
-// T0 / per .. (T1 - 1) / per, and their pieces have consecutive slots.
-template <int MT, bool STREAM>
-__global__ void __launch_bounds__(256) combine_kernel(const Params p, int rows, int units, int grid_x) {
+  // launched beside the kernel before it: complete only after it
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  const int Hq = p.Hkv * p.nrep;
-  const int h = row % Hq, u = (row / Hq) % units, b = row / (Hq * units);
-  const int kvh = h / p.nrep, hr = h - kvh * p.nrep;
-  const float* src[2];
-  int n[2] = {0, 0};
-  int64_t stride[2] = {0, 0};
-  if constexpr (STREAM) {
-    const int ne = p.seg[0].nb + (p.nseg > 1 ? p.seg[1].nb : 0);
-    const int per = max(p.min_tiles, (p.cum[ne] + grid_x - 1) / grid_x);
-    for (int si = 0; si < p.nseg; ++si) {
-      const Seg& s = p.seg[si];
-      // with two segments, the first is shared by the s.units sequences of a group
-      const int eb = p.nseg > 1 && si == 0 ? b / s.units : b;
-      const int r_all = (p.nseg > 1 && si == 0 ? (b % s.units) : u) * p.nrep + hr;
-      const int e = eb + (si ? p.seg[0].nb : 0);
-      const int rt = r_all / MT, n_rt = row_tiles(s.units * p.nrep, MT);
-      const int idx = rt * p.Hkv + kvh;
-      const int nt = (p.cum[e + 1] - p.cum[e]) / (p.Hkv * n_rt);
-      if (nt == 0) continue;
-      const int T0 = p.cum[e] + idx * nt, c0 = T0 / per, c1 = (T0 + nt - 1) / per;
-      if (!p.merge_all && c0 == c1) return;  // written by the block that held all of it
-      src[si] = part_row(p, si, eb * p.Hkv * n_rt + idx + c0, r_all - rt * MT);
-      n[si] = c1 - c0 + 1;
-      stride[si] = static_cast<int64_t>(p.rows_cap[si]) * kPartRow;
-    }
-  } else {
-    const Seg& s = p.seg[0];
-    const int nq = p.q_lens ? min(max(p.q_lens[b], 0), s.units) : s.units;
-    if (u >= nq) return;
-    const int r = u * p.nrep + hr, rt = r / MT;
-    src[0] = part_row(p, 0, ((b * p.Hkv + kvh) * p.n_rt + rt) * p.n_split, r - rt * MT);
-    n[0] = p.n_split;
-    stride[0] = static_cast<int64_t>(p.rows_cap[0]) * kPartRow;
-  }
-  float M = -INFINITY;
-  for (int k = 0; k < 2; ++k)
-    for (int i = lane; i < n[k]; i += 32) M = fmaxf(M, src[k][i * stride[k]]);
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float L = 0.0f;
-  if (M != -INFINITY) {
-    for (int k = 0; k < 2; ++k)
-#pragma unroll 4
-      for (int i = 0; i < n[k]; ++i) {
-        const float* x = src[k] + i * stride[k];
-        const float2 ml = *reinterpret_cast<const float2*>(x);
-        const float4 o = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
-        const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
-        L += f * ml.y;
-        acc.x += f * o.x;
-        acc.y += f * o.y;
-        acc.z += f * o.z;
-        acc.w += f * o.w;
-      }
-  }
-  const float inv = L <= 0.0f ? 0.0f : 1.0f / L;  // (a NaN stays)
-  store4(out_row(p, b, u, h), p.q_dt, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
-// ---------------------------------------------------------------- host side
-inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
-inline bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
-
-// Row tiles per block: two for more than 128 rows; float16 models (q' in two parts, whose
-// second tile takes the shared memory of a second row tile) always one.
-inline int tiles_of(int q_dt, int rows) { return q_dt == HQ_DTYPE_F16 || rows <= 128 ? 1 : 2; }
-
-struct Plan {
-  int nm, n_rt, n_split, grid;
-  int rows_cap[2];
-  int64_t part_floats[2];
-  size_t cum_bytes;
-  int64_t units[2];
-  size_t bytes() const {
-    return cum_bytes + align256(sizeof(float) * static_cast<size_t>(part_floats[0] + part_floats[1]));
-  }
-};
-
-// STREAM plan: rows0 / rows1 rows per entry of the two segments (nb1 == 0: one segment).
-inline bool plan_stream(Plan& pl, int q_dt, int Hkv, int nb0, int64_t rows0, int cap0, int nb1,
-                        int64_t rows1, int cap1) {
-  const int64_t rmax = std::max(rows0, rows1);
-  pl = Plan{};
-  pl.nm = tiles_of(q_dt, static_cast<int>(std::min<int64_t>(rmax, 1 << 20)));
-  const int MT = 128 * pl.nm;
-  const int64_t u0 = int64_t(nb0) * Hkv * ((rows0 + MT - 1) / MT);
-  const int64_t u1 = int64_t(nb1) * Hkv * ((rows1 + MT - 1) / MT);
-  const int64_t tiles = u0 * std::max(1, cap0 / kBN + 1) + u1 * std::max(1, cap1 / kBN + 1);
-  if (tiles > (int64_t(1) << 30) || nb0 + nb1 > kMaxEntries) return false;
-  pl.units[0] = u0;
-  pl.units[1] = u1;
-  pl.grid = static_cast<int>(std::min<int64_t>(current_sm_count(), std::max<int64_t>(tiles, 1)));
-  pl.rows_cap[0] = static_cast<int>(std::min<int64_t>(rows0, MT));
-  pl.rows_cap[1] = static_cast<int>(std::min<int64_t>(rows1, MT));
-  pl.part_floats[0] = (u0 + pl.grid) * pl.rows_cap[0] * kPartRow;
-  pl.part_floats[1] = nb1 ? (u1 + pl.grid) * pl.rows_cap[1] * kPartRow : 0;
-  pl.cum_bytes = align256(sizeof(int) * (nb0 + nb1 + 1));
-  return true;
-}
-
-// Prefill plan: one block per row tile; with fewer blocks than SMs the keys of each row
-// tile are split, down to two key tiles per block.
-inline bool plan_prefill(Plan& pl, int q_dt, int B, int Hkv, int nrep, int Sq, int cap, int window,
-                         int sinks) {
-  pl = Plan{};
-  const int64_t rows = int64_t(Sq) * nrep;
-  if (rows > (1 << 30)) return false;
-  pl.nm = tiles_of(q_dt, static_cast<int>(std::min<int64_t>(rows, 1 << 20)));
-  // small grids keep one row tile per block
-  if (pl.nm == 2 && int64_t(B) * Hkv * ((rows + 255) / 256) < current_sm_count()) pl.nm = 1;
-  const int MT = 128 * pl.nm;
-  pl.n_rt = static_cast<int>((rows + MT - 1) / MT);
-  const int64_t units = int64_t(B) * Hkv * pl.n_rt;
-  if (units * 64 > (int64_t(1) << 31) - 1 || int64_t(Hkv) * pl.n_rt > 65535) return false;
-  const int64_t seen = std::min<int64_t>(cap, int64_t(window) + sinks + MT / nrep + 1);
-  const int64_t nt = std::max<int64_t>(1, (seen + kBN - 1) / kBN);
-  const int sms = current_sm_count();
-  pl.n_split = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, sms / std::max<int64_t>(units, 1)),
-                                                   std::max<int64_t>(1, nt / 2), 16}));
-  pl.rows_cap[0] = static_cast<int>(std::min<int64_t>(rows, MT));
-  pl.part_floats[0] = pl.n_split > 1 ? units * pl.n_split * pl.rows_cap[0] * kPartRow : 0;
-  return true;
-}
-
-template <typename K>
-int set_smem(K kern, int bytes, std::atomic<uint64_t>& ready) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = (dev >= 0 && dev < 64) ? (uint64_t(1) << dev) : 0;
-  if (!bit || !(ready.load(std::memory_order_acquire) & bit)) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    ready.fetch_or(bit, std::memory_order_acq_rel);
-  }
-  return HQ_OK;
-}
-
+// ---------------------------------------------------------------- launches
 template <int NM, bool LO, bool STREAM>
-int launch(const Params& p, dim3 grid, int entries, int out_rows, int units, bool combine,
-           cudaStream_t st) {
+int launch(const Params& p, dim3 grid, cudaStream_t st) {
   using C = Cfg<NM, LO>;
   static std::atomic<uint64_t> ready{0};
   auto kern = ragged_kernel<NM, LO, STREAM>;
   const int rc = set_smem(kern, C::smem(STREAM ? kMaxEntries : 0), ready);
   if (rc != HQ_OK) return rc;
-  kern<<<grid, C::kThreads, C::smem(STREAM ? entries : 0), st>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (!combine) return HQ_OK;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((out_rows + 7) / 8);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, combine_kernel<128 * NM, STREAM>, p, out_rows, units,
-                         static_cast<int>(grid.x));
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return static_cast<int>(e);
-  }
-  return HQ_OK;
+  return launch_after(kern, p, grid, C::kThreads, C::smem(STREAM ? p.seg.nb : 0), st);
 }
 
 template <bool STREAM>
-int dispatch(const Params& p, int nm, dim3 grid, int entries, int out_rows, int units, bool combine,
-             cudaStream_t st) {
-  if (p.q_dt == HQ_DTYPE_F16) return launch<1, true, STREAM>(p, grid, entries, out_rows, units, combine, st);
-  if (nm == 1) return launch<1, false, STREAM>(p, grid, entries, out_rows, units, combine, st);
-  return launch<2, false, STREAM>(p, grid, entries, out_rows, units, combine, st);
+int dispatch(const Params& p, int nm, dim3 grid, cudaStream_t st) {
+  if (p.q_dt == HQ_DTYPE_F16) return launch<1, true, STREAM>(p, grid, st);
+  if (nm == 1) return launch<1, false, STREAM>(p, grid, st);
+  return launch<2, false, STREAM>(p, grid, st);
 }
 
-inline int fill_seg(Seg& s, const int8_t* k, const int8_t* v, const int64_t* kvs, const void* ksc,
-                    const void* vsc, const int64_t* kss, const int64_t* vss, const int* lens,
-                    int cap, int nb, int units, int window, int sinks) {
-  if (cap > 0 && (!k || !v || !ksc || !vsc)) return HQ_ERR_INVALID_ARGUMENT;
-  if (!kvs || !kss || !vss || cap < 0 || nb < 0 || units < 0 || window < 0 || sinks < 0)
-    return HQ_ERR_INVALID_ARGUMENT;
-  if (!aligned(k, 16) || !aligned(v, 16) || kvs[0] % 16 || kvs[1] % 16 || kvs[2] % 16)
-    return HQ_ERR_INVALID_ARGUMENT;
-  s.k = k;
-  s.v = v;
-  s.sb = kvs[0];
-  s.sh = kvs[1];
-  s.ss = kvs[2];
-  s.ksc = ksc;
-  s.vsc = vsc;
-  s.kscb = kss[0];
-  s.ksch = kss[1];
-  s.kscd = kss[2];
-  s.vscb = vss[0];
-  s.vsch = vss[1];
-  s.vscs = vss[2];
-  s.lens = lens;
-  s.cap = cap;
-  s.nb = nb;
-  s.units = units;
-  s.window = window > 0 ? window : 1 << 30;
-  s.sinks = sinks;
-  return HQ_OK;
+int tiles_stream(const Params& p, int nm, int grid, cudaStream_t st) {
+  return dispatch<true>(p, nm, dim3(grid), st);
 }
-
-inline int check_common(const void* q, int q_dtype, const int64_t* qs, int nqs, const void* out,
-                        const int64_t* os, int scale_dtype, int Hq, int Hkv, int D) {
-  if (!q || !out || !qs || !os || Hq <= 0 || Hkv <= 0) return HQ_ERR_INVALID_ARGUMENT;
-  if (D != kD || Hq % Hkv || Hq / Hkv > 128 || Hq > 65535 ||
-      (q_dtype != HQ_DTYPE_BF16 && q_dtype != HQ_DTYPE_F16) ||
-      (scale_dtype != HQ_DTYPE_F32 && scale_dtype != HQ_DTYPE_F16))
-    return HQ_ERR_UNSUPPORTED;
-  if (qs[nqs - 1] != 1 || os[nqs - 1] != 1 || !aligned(q, 16) || !aligned(out, 8))
-    return HQ_ERR_INVALID_ARGUMENT;
-  for (int i = 0; i + 1 < nqs; ++i)
-    if (qs[i] % 8 || os[i] % 4) return HQ_ERR_INVALID_ARGUMENT;
-  return HQ_OK;
-}
-
-inline int attach(Params& p, const Plan& pl, void* ws, size_t ws_bytes) {
-  if (pl.bytes() > 0 && (!ws || ws_bytes < pl.bytes() || !aligned(ws, 256))) return HQ_ERR_WORKSPACE;
-  p.cum = static_cast<int*>(ws);
-  p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.cum_bytes);
-  p.part1 = pl.part_floats[0];
-  p.rows_cap[0] = pl.rows_cap[0];
-  p.rows_cap[1] = pl.rows_cap[1];
-  p.n_split = pl.n_split;
-  p.n_rt = pl.n_rt;
-  return HQ_OK;
+int tiles_prefill(const Params& p, int nm, int B, cudaStream_t st) {
+  return dispatch<false>(p, nm, dim3(p.n_split, p.Hkv * p.n_rt, B), st);
 }
 
 }  // namespace rag
 }  // namespace hq
-
-using namespace hq;
-
-extern "C" size_t hq_window_workspace_bytes(int q_dtype, int B, int Hq, int Hkv, int Sq, int S_max,
-                                            int D, int window, int sinks) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq < 0 || S_max < 0 || window < 0 || sinks < 0 ||
-      D != rag::kD || Hq % Hkv)
-    return 0;
-  rag::Plan pl;
-  const bool ok = Sq == 0 ? rag::plan_stream(pl, q_dtype, Hkv, B, Hq / Hkv, S_max, 0, 0, 0)
-                          : rag::plan_prefill(pl, q_dtype, B, Hkv, Hq / Hkv, Sq, S_max,
-                                              window > 0 ? window : 1 << 30, sinks);
-  return ok ? std::max<size_t>(pl.bytes(), 256) : 0;
-}
-
-extern "C" int hq_window_decode_int8(const void* q, int q_dtype, const int64_t q_strides[3],
-                                     const int8_t* k, const int8_t* v, const int64_t kv_strides[3],
-                                     const void* k_scale, const void* v_scale, int scale_dtype,
-                                     const int64_t ksc_strides[3], const int64_t vsc_strides[3],
-                                     const int* lens, int B, int Hq, int Hkv, int S_max, int D,
-                                     int window, int sinks, float sm_scale, int q_quant, void* out,
-                                     const int64_t out_strides[3], void* workspace,
-                                     size_t workspace_bytes, int* status, hq_stream_t stream) {
-  int rc = rag::check_common(q, q_dtype, q_strides, 3, out, out_strides, scale_dtype, Hq, Hkv, D);
-  if (rc != HQ_OK) return rc;
-  if (B < 0) return HQ_ERR_INVALID_ARGUMENT;
-  rag::Params p{};
-  rc = rag::fill_seg(p.seg[0], k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
-                     S_max, B, 1, window, sinks);
-  if (rc != HQ_OK) return rc;
-  if (B == 0) return HQ_OK;
-  rag::Plan pl;
-  if (!rag::plan_stream(pl, q_dtype, Hkv, B, Hq / Hkv, S_max, 0, 0, 0)) return HQ_ERR_UNSUPPORTED;
-  rc = rag::attach(p, pl, workspace, workspace_bytes);
-  if (rc != HQ_OK) return rc;
-  p.nseg = 1;
-  p.seg[0].qsb = q_strides[0];
-  p.q = q;
-  p.qsh = q_strides[1];
-  p.q_dt = q_dtype;
-  p.s_dt = scale_dtype;
-  p.Hkv = Hkv;
-  p.nrep = Hq / Hkv;
-  p.qk_scale = sm_scale * rag::kLog2e;
-  p.q_quant = q_quant;
-  p.out = out;
-  p.osb = out_strides[0];
-  p.osh = out_strides[1];
-  p.status = status;
-  p.min_tiles = 1;
-  return rag::dispatch<true>(p, pl.nm, dim3(pl.grid), B, B * Hq, 1, true,
-                             reinterpret_cast<cudaStream_t>(stream));
-}
-
-extern "C" int hq_window_prefill_int8(const void* q, int q_dtype, const int64_t q_strides[4],
-                                      const int8_t* k, const int8_t* v, const int64_t kv_strides[3],
-                                      const void* k_scale, const void* v_scale, int scale_dtype,
-                                      const int64_t ksc_strides[3], const int64_t vsc_strides[3],
-                                      const int* lens, const int* q_lens, int B, int Hq, int Hkv,
-                                      int Sq, int S_max, int D, int window, int sinks,
-                                      float sm_scale, int q_quant, void* out,
-                                      const int64_t out_strides[4], void* workspace,
-                                      size_t workspace_bytes, int* status, hq_stream_t stream) {
-  int rc = rag::check_common(q, q_dtype, q_strides, 4, out, out_strides, scale_dtype, Hq, Hkv, D);
-  if (rc != HQ_OK) return rc;
-  if (B < 0 || Sq < 0) return HQ_ERR_INVALID_ARGUMENT;
-  if (B > 65535) return HQ_ERR_UNSUPPORTED;
-  rag::Params p{};
-  rc = rag::fill_seg(p.seg[0], k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
-                     S_max, B, Sq, window, sinks);
-  if (rc != HQ_OK) return rc;
-  if (B == 0 || Sq == 0) return HQ_OK;
-  rag::Plan pl;
-  if (!rag::plan_prefill(pl, q_dtype, B, Hkv, Hq / Hkv, Sq, S_max, p.seg[0].window, sinks))
-    return HQ_ERR_UNSUPPORTED;
-  rc = rag::attach(p, pl, workspace, workspace_bytes);
-  if (rc != HQ_OK) return rc;
-  p.nseg = 1;
-  p.seg[0].step = 1;
-  p.seg[0].qsb = q_strides[0];
-  p.seg[0].qsu = q_strides[2];
-  p.q = q;
-  p.qsh = q_strides[1];
-  p.q_dt = q_dtype;
-  p.s_dt = scale_dtype;
-  p.Hkv = Hkv;
-  p.nrep = Hq / Hkv;
-  p.qk_scale = sm_scale * rag::kLog2e;
-  p.q_quant = q_quant;
-  p.q_lens = q_lens;
-  p.out = out;
-  p.osb = out_strides[0];
-  p.osh = out_strides[1];
-  p.osu = out_strides[2];
-  p.status = status;
-  return rag::dispatch<false>(p, pl.nm, dim3(pl.n_split, Hkv * pl.n_rt, B), 0, B * Sq * Hq, Sq,
-                              pl.n_split > 1, reinterpret_cast<cudaStream_t>(stream));
-}
-
-extern "C" size_t hq_prefix_decode_workspace_bytes(int q_dtype, int G, int B, int Hq, int Hkv,
-                                                   int P_max, int S_max, int D) {
-  if (G <= 0 || B <= 0 || B % G || Hq <= 0 || Hkv <= 0 || Hq % Hkv || P_max < 0 || S_max < 0 ||
-      D != rag::kD)
-    return 0;
-  rag::Plan pl;
-  const int nrep = Hq / Hkv;
-  if (!rag::plan_stream(pl, q_dtype, Hkv, G, int64_t(B / G) * nrep, P_max, B, nrep, S_max)) return 0;
-  return std::max<size_t>(pl.bytes(), 256);
-}
-
-extern "C" int hq_prefix_decode_int8(
-    const void* q, int q_dtype, const int64_t q_strides[3], const int8_t* pk, const int8_t* pv,
-    const int64_t pkv_strides[3], const void* pk_scale, const void* pv_scale,
-    const int64_t pksc_strides[3], const int64_t pvsc_strides[3], const int* prefix_lens, int G,
-    int P_max, const int8_t* k, const int8_t* v, const int64_t kv_strides[3], const void* k_scale,
-    const void* v_scale, const int64_t ksc_strides[3], const int64_t vsc_strides[3],
-    const int* lens, int S_max, int scale_dtype, int B, int Hq, int Hkv, int D, float sm_scale,
-    int q_quant, void* out, const int64_t out_strides[3], void* workspace, size_t workspace_bytes,
-    int* status, hq_stream_t stream) {
-  int rc = rag::check_common(q, q_dtype, q_strides, 3, out, out_strides, scale_dtype, Hq, Hkv, D);
-  if (rc != HQ_OK) return rc;
-  if (B < 0 || G <= 0 || B % G) return HQ_ERR_INVALID_ARGUMENT;
-  rag::Params p{};
-  rc = rag::fill_seg(p.seg[0], pk, pv, pkv_strides, pk_scale, pv_scale, pksc_strides, pvsc_strides,
-                     prefix_lens, P_max, G, B / G, 0, 0);
-  if (rc == HQ_OK)
-    rc = rag::fill_seg(p.seg[1], k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
-                       S_max, B, 1, 0, 0);
-  if (rc != HQ_OK) return rc;
-  if (B == 0) return HQ_OK;
-  const int nrep = Hq / Hkv;
-  rag::Plan pl;
-  if (!rag::plan_stream(pl, q_dtype, Hkv, G, int64_t(B / G) * nrep, P_max, B, nrep, S_max))
-    return HQ_ERR_UNSUPPORTED;
-  rc = rag::attach(p, pl, workspace, workspace_bytes);
-  if (rc != HQ_OK) return rc;
-  p.nseg = 2;
-  p.seg[0].qsb = q_strides[0] * (B / G);
-  p.seg[0].qsu = q_strides[0];
-  p.seg[1].qsb = q_strides[0];
-  p.q = q;
-  p.qsh = q_strides[1];
-  p.q_dt = q_dtype;
-  p.s_dt = scale_dtype;
-  p.Hkv = Hkv;
-  p.nrep = nrep;
-  p.qk_scale = sm_scale * rag::kLog2e;
-  p.q_quant = q_quant;
-  p.out = out;
-  p.osb = out_strides[0];
-  p.osh = out_strides[1];
-  p.status = status;
-  p.min_tiles = 1;
-  p.merge_all = 1;
-  return rag::dispatch<true>(p, pl.nm, dim3(pl.grid), G + B, B * Hq, 1, true,
-                             reinterpret_cast<cudaStream_t>(stream));
-}

@@ -567,7 +567,7 @@ HQ_API int hq_kblock_dequant(const int8_t* k_cache, const int64_t kq_strides[3],
  * to call).  `status` (optional) receives HQ_ERR_DEVICE_TIMEOUT if a bounded
  * wait inside a block gave up (first error sticks).
  *
- * hq_window_decode_int8 (B <= 1536): one query per sequence, the token at position
+ * hq_window_decode_int8 (B <= 1024): one query per sequence, the token at position
  *   lens[b] - 1, over keys j with j >= lens[b] - window or j < sinks (window 0:
  *   all keys).  lens[b] = 0 gives zeros.  q / out [B, Hq, D].
  * hq_window_prefill_int8: q [B, Hq, Sq, D], out logical [B, Hq, Sq, D]; the
@@ -583,7 +583,7 @@ HQ_API int hq_kblock_dequant(const int8_t* k_cache, const int64_t kq_strides[3],
  *   int32[G] tokens of it, NULL: P_max) and each has its own tokens in k / v
  *   [B, Hkv, S_max, D] (lens int32[B], NULL: S_max).  A query sees all of both;
  *   the prefix is read once for the whole group.  Scales as hq_decode_int8, of
- *   one scale_dtype.  B + G <= 1536.
+ *   one scale_dtype.  B <= 1024.
  */
 HQ_API size_t hq_window_workspace_bytes(int q_dtype, int B, int Hq, int Hkv, int Sq, int S_max,
                                         int D, int window, int sinks);

@@ -44,18 +44,18 @@ __device__ __forceinline__ Run split_run(const Source& s, int b, int u, int kvh,
           static_cast<int64_t>(p.rows_cap) * kPartRow};
 }
 
-// One warp per output row (b, u, h), 4 channels per lane: the pieces' common maximum, then
-// their weighted sums.
+// One block per output row (b, u, h): the pieces' common maximum (every warp finds it), then
+// their weighted sums, warp w taking pieces w, w + 4, .., a lane 4 channels.
+constexpr int kJoinWarps = 4;
 template <int NSRC, bool STREAM>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Source s0,
-                                                      const __grid_constant__ Source s1, int rows,
-                                                      int units) {
+__global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_constant__ Source s0,
+                                                                  const __grid_constant__ Source s1,
+                                                                  int units) {
+  __shared__ float4 sum[kJoinWarps][33];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= rows) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Params& p = s0.p;
-  const int Hq = p.Hkv * p.nrep;
-  const int h = row % Hq, bu = row / Hq, b = bu / units, u = bu - b * units;
+  const int h = blockIdx.y, b = STREAM ? blockIdx.x : blockIdx.x / units, u = blockIdx.x - b * units;
   const int kvh = h / p.nrep, hr = h - kvh * p.nrep;
   Run run[NSRC];
   if constexpr (STREAM) {
@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ So
   float M = -INFINITY;
 #pragma unroll
   for (int k = 0; k < NSRC; ++k)
+#pragma unroll 1
     for (int i = lane; i < run[k].n; i += 32) M = fmaxf(M, run[k].at[i * run[k].step]);
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
@@ -79,7 +80,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ So
 #pragma unroll
     for (int k = 0; k < NSRC; ++k)
 #pragma unroll 4
-      for (int i = 0; i < run[k].n; ++i) {
+      for (int i = warp; i < run[k].n; i += kJoinWarps) {
         const float* x = run[k].at + i * run[k].step;
         const float2 ml = *reinterpret_cast<const float2*>(x);
         const float4 o = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
@@ -91,22 +92,37 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ So
         acc.w += f * o.w;
       }
   }
+  sum[warp][lane] = acc;
+  if (lane == 0) sum[warp][32].x = L;
+  __syncthreads();
+  if (warp) return;
+  L = 0.0f;
+  acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) {
+    const float4 o = sum[i][lane];
+    L += sum[i][32].x;
+    acc.x += o.x;
+    acc.y += o.y;
+    acc.z += o.z;
+    acc.w += o.w;
+  }
   const float inv = L <= 0.0f ? 0.0f : 1.0f / L;  // (a NaN stays)
   store4(out_row(p, b, u, h), p.q_dt, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
 template <int NSRC, bool STREAM>
-int combine(const Source& s0, const Source& s1, int rows, int units, cudaStream_t st) {
+int combine(const Source& s0, const Source& s1, int B, int units, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((rows + 7) / 8);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(B * units, s0.p.Hkv * s0.p.nrep);
+  cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, combine_kernel<NSRC, STREAM>, s0, s1, rows, units);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, combine_kernel<NSRC, STREAM>, s0, s1, units);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return static_cast<int>(e);
@@ -299,7 +315,7 @@ extern "C" int hq_window_decode_int8(const void* q, int q_dtype, const int64_t q
   s.per_entry = 1;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   rc = rag::run_stream(s.p, pl, st);
-  return rc != HQ_OK ? rc : rag::combine<1, true>(s, s, B * Hq, 1, st);
+  return rc != HQ_OK ? rc : rag::combine<1, true>(s, s, B, 1, st);
 }
 
 extern "C" int hq_window_prefill_int8(const void* q, int q_dtype, const int64_t q_strides[4],
@@ -314,7 +330,7 @@ extern "C" int hq_window_prefill_int8(const void* q, int q_dtype, const int64_t 
   int rc = rag::check_common(q, q_dtype, q_strides, 4, out, out_strides, scale_dtype, Hq, Hkv, D);
   if (rc != HQ_OK) return rc;
   if (B < 0 || Sq < 0) return HQ_ERR_INVALID_ARGUMENT;
-  if (B > 65535 || int64_t(B) * Sq * Hq > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
+  if (B > 65535 || int64_t(B) * Sq > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
   rag::Source s{};
   s.p = rag::make_params(q, q_dtype, q_strides[1], scale_dtype, Hq, Hkv, sm_scale, q_quant, out,
                          out_strides[0], out_strides[1], status);
@@ -340,7 +356,7 @@ extern "C" int hq_window_prefill_int8(const void* q, int q_dtype, const int64_t 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   rc = rag::tiles_prefill(s.p, pl.nm, B, st);
   if (rc != HQ_OK || pl.n_split == 1) return rc;
-  return rag::combine<1, false>(s, s, B * Sq * Hq, Sq, st);
+  return rag::combine<1, false>(s, s, B, Sq, st);
 }
 
 extern "C" size_t hq_prefix_decode_workspace_bytes(int q_dtype, int G, int B, int Hq, int Hkv,
@@ -402,5 +418,5 @@ extern "C" int hq_prefix_decode_int8(
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   rc = rag::run_stream(pre.p, a, st);
   if (rc == HQ_OK) rc = rag::run_stream(own.p, b, st);
-  return rc != HQ_OK ? rc : rag::combine<2, true>(own, pre, B * Hq, 1, st);
+  return rc != HQ_OK ? rc : rag::combine<2, true>(own, pre, B, 1, st);
 }

@@ -466,15 +466,15 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       fence_mbar_init();
     }
   }
-  if constexpr (STREAM) build_cum<MT>(p, cum, C::kThreads);
+  if constexpr (STREAM) build_cum<MT, 1>(p, cum, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t q_base = smem_u32(smem), k_base = smem_u32(smem + C::kOffK),
                  v_base = smem_u32(smem + C::kOffV);
-  Walk walk = walk_start<MT, STREAM>(p, cum);
-  auto next_piece = [&](Walk& k, Piece& to) { return walk_next<MT, STREAM>(k, p, cum, to); };
+  Walk walk = walk_start<MT, STREAM, 1>(p, cum);
+  auto next_piece = [&](Walk& k, Piece& to) { return walk_next<MT, STREAM, 1>(k, p, cum, to); };
   Piece w{};
 
   if (warp < C::kSoft / 32) {
@@ -998,7 +998,7 @@ int launch(const Params& p, dim3 grid, cudaStream_t st) {
   auto kern = ragged_kernel<NM, LO, STREAM>;
   const int rc = set_smem(kern, C::smem(STREAM ? kMaxEntries : 0), ready);
   if (rc != HQ_OK) return rc;
-  return launch_after(kern, p, grid, C::kThreads, C::smem(STREAM ? p.seg.nb : 0), st);
+  return launch_after(kern, grid, C::kThreads, C::smem(STREAM ? p.seg.nb : 0), st, p);
 }
 
 template <bool STREAM>

@@ -66,30 +66,31 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 // ---------------------------------------------------------------- pieces of work
-// The keys of one row tile, numbered v = 0 .. nv - 1: key = v < ns ? v : v + sh.
+// The keys of one row tile, numbered v = 0 .. nv - 1: the sinks 0 .. ns - 1, then numbers up to
+// nsp that nobody sees (where the copies want the next run to start at a multiple of 8), then
+// key v + sh.
 struct Keys {
   int pos0;        // position of the entry's query 0
-  int ns, sh, nv, nt;
+  int ns, nsp, sh, nv, nt;
+  __device__ __forceinline__ int key(int v) const { return v < nsp ? v : v + sh; }
+  __device__ __forceinline__ bool padding(int v) const { return v >= ns && v < nsp; }
 };
 __device__ __forceinline__ int seg_len(const Seg& s, int b) {
   return s.lens ? min(max(s.lens[b], 0), s.cap) : s.cap;
 }
 // n tokens held, nq queries of which rows u_lo .. u_hi are in the tile
+template <int AL>
 __device__ __forceinline__ Keys make_keys(const Seg& s, int n, int nq, int u_lo, int u_hi) {
   Keys k;
   k.pos0 = s.step ? n - nq : n - 1;
   const int p_lo = k.pos0 + (s.step ? u_lo : 0), p_hi = k.pos0 + (s.step ? u_hi : 0);
-  const int w0 = max(0, p_lo - s.window + 1);
-  if (w0 <= s.sinks) {
-    k.ns = 0;
-    k.sh = 0;
-    k.nv = p_hi + 1;
-  } else {
-    k.ns = s.sinks;
-    k.sh = w0 - s.sinks;
-    k.nv = p_hi + 1 - k.sh;
-  }
-  k.nv = max(k.nv, 0);
+  const int w0 = max(0, p_lo - s.window + 1), nsp = (s.sinks + AL - 1) / AL * AL;
+  // apart: two runs; else one run of keys (of which sinks .. w0 - 1 may be unseen)
+  const bool apart = w0 > nsp, gap = w0 > s.sinks;
+  k.ns = gap ? s.sinks : 0;
+  k.nsp = apart ? nsp : gap ? w0 : 0;
+  k.sh = apart ? w0 - nsp : 0;
+  k.nv = max(p_hi + 1 - k.sh, 0);
   k.nt = (k.nv + kBN - 1) / kBN;
   return k;
 }
@@ -99,57 +100,76 @@ struct Piece {
   int t0, t1;
   int slot;        // -1: final output
 };
-
-// STREAM: tiles of entry e, one row tile (0: the call is answered by combine_kernel)
-__device__ __forceinline__ int entry_tiles(const Params& p, int e) {
-  const int nt = make_keys(p.seg, seg_len(p.seg, e), p.seg.units, 0, 0).nt;
-  return p.merge_all ? nt : max(nt, 1);
-}
 __device__ __host__ __forceinline__ int row_tiles(int rows, int mt) { return (rows + mt - 1) / mt; }
 
+// STREAM: keys of entry e; tiles of one row tile (0: the call is answered by combine_kernel)
+template <int AL>
+__device__ __forceinline__ Keys entry_keys(const Params& p, int e) {
+  Keys k = make_keys<AL>(p.seg, seg_len(p.seg, e), p.seg.units, 0, 0);
+  if (!p.merge_all) k.nt = max(k.nt, 1);
+  return k;
+}
 // cum[e]: first tile of entry e in the line of all tiles (shared memory, nb + 1 words; ends
 // with a block barrier).  Block 0 leaves a copy for combine_kernel.
-template <int MT>
+template <int MT, int AL>
 __device__ __forceinline__ void build_cum(const Params& p, int* cum, int n_threads) {
   const int ne = p.seg.nb, per = p.Hkv * row_tiles(p.seg.units * p.nrep, MT);
-  for (int e = threadIdx.x; e < ne; e += n_threads) cum[e + 1] = entry_tiles(p, e) * per;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    int run = 0;
-    if (lane == 0) cum[0] = 0;
-    for (int e0 = 0; e0 < ne; e0 += 32) {
-      int x = e0 + lane < ne ? cum[e0 + lane + 1] : 0;
+  if (ne <= 32) {  // one warp does it alone
+    if (threadIdx.x < 32) {
+      int x = threadIdx.x < ne ? entry_keys<AL>(p, threadIdx.x).nt * per : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        if (threadIdx.x >= o) x += y;
       }
-      if (e0 + lane < ne) cum[e0 + lane + 1] = run + x;
-      run += __shfl_sync(0xffffffffu, x, 31);
+      if (threadIdx.x == 0) cum[0] = 0;
+      if (threadIdx.x < ne) cum[threadIdx.x + 1] = x;
     }
-    __syncwarp();
-    if (blockIdx.x == 0)
-      for (int e = lane; e <= ne; e += 32) p.cum[e] = cum[e];
+  } else {
+    for (int e = threadIdx.x; e < ne; e += n_threads) cum[e + 1] = entry_keys<AL>(p, e).nt * per;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const int lane = threadIdx.x;
+      int run = 0;
+      if (lane == 0) cum[0] = 0;
+#pragma unroll 1
+      for (int e0 = 0; e0 < ne; e0 += 32) {
+        int x = e0 + lane < ne ? cum[e0 + lane + 1] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        if (e0 + lane < ne) cum[e0 + lane + 1] = run + x;
+        run += __shfl_sync(0xffffffffu, x, 31);
+      }
+    }
   }
   __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= ne; e += n_threads) p.cum[e] = cum[e];
 }
 __device__ __forceinline__ int tiles_per_block(const Params& p, int total, int grid) {
   return max(p.min_tiles, (total + grid - 1) / grid);
 }
 
-// The pieces of one block, in order.  (A call: every role walks them.)
+// The pieces of one block, in order.  STREAM: an equal run of the line of tiles, cut where the
+// units (entry, row tile, kv head) end; the state is the unit at hand, stepped from one to the
+// next (a divide and two modulos per piece cost 2400 cycles of a cold call).
 struct Walk {
-  int cur, end, e;
+  int cur, end;                  // tiles of the line
+  int e, rt, kvh, first;         // the unit, its first tile
+  Keys key;
 };
-template <int MT, bool STREAM>
+template <int MT, bool STREAM, int AL>
 __device__ __forceinline__ Walk walk_start(const Params& p, const int* cum) {
-  Walk k{0, 1, 0};
+  Walk k{};
   if constexpr (STREAM) {
     const int ne = p.seg.nb, total = cum[ne];
     const int per = tiles_per_block(p, total, static_cast<int>(gridDim.x));
     k.cur = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total)));
     k.end = static_cast<int>(min(static_cast<int64_t>(k.cur) + per, static_cast<int64_t>(total)));
+    if (k.cur >= k.end) return k;
     // the entry that holds tile cur: cum[e] <= cur < cum[e + 1]
     int lo = 0, hi = ne - 1;
     while (lo < hi) {
@@ -157,45 +177,58 @@ __device__ __forceinline__ Walk walk_start(const Params& p, const int* cum) {
       if (cum[mid] <= k.cur) lo = mid; else hi = mid - 1;
     }
     k.e = lo;
+    k.key = entry_keys<AL>(p, lo);
+    const uint32_t idx = static_cast<uint32_t>(k.cur - cum[lo]) / static_cast<uint32_t>(k.key.nt);
+    k.rt = idx / static_cast<uint32_t>(p.Hkv);
+    k.kvh = idx - k.rt * p.Hkv;
+    k.first = cum[lo] + idx * k.key.nt;
+  } else {
+    k.end = 1;
   }
   return k;
 }
-template <int MT, bool STREAM>
-__device__ __noinline__ bool walk_next(Walk& k, const Params& p, const int* cum, Piece& w) {
+template <int MT, bool STREAM, int AL>
+__device__ __forceinline__ bool walk_next(Walk& k, const Params& p, const int* cum, Piece& w) {
   if (k.cur >= k.end) return false;
+  const Seg& s = p.seg;
   if constexpr (STREAM) {
-    while (cum[k.e + 1] <= k.cur) ++k.e;
-    const Seg& s = p.seg;
+    const int rows = s.units * p.nrep, n_rt = MT == 128 && rows <= 128 ? 1 : row_tiles(rows, MT);
     w.b = k.e;
-    const int rows = s.units * p.nrep, n_rt = row_tiles(rows, MT), per_e = p.Hkv * n_rt;
-    const uint32_t nt = static_cast<uint32_t>(cum[k.e + 1] - cum[k.e]) / static_cast<uint32_t>(per_e);
-    const int idx = static_cast<uint32_t>(k.cur - cum[k.e]) / nt, first = cum[k.e] + idx * nt;
-    const int rt = static_cast<uint32_t>(idx) / static_cast<uint32_t>(p.Hkv);
-    w.kvh = idx - rt * p.Hkv;
-    w.row0 = rt * MT;
+    w.kvh = k.kvh;
+    w.row0 = k.rt * MT;
     w.rows = min(MT, rows - w.row0);
-    w.key = make_keys(s, seg_len(s, w.b), s.units, 0, 0);
-    w.t0 = k.cur - first;
-    w.t1 = min(static_cast<int>(nt), w.t0 + k.end - k.cur);
-    k.cur = first + w.t1;
-    w.slot = !p.merge_all && w.t0 == 0 && w.t1 == static_cast<int>(nt)
+    w.key = k.key;
+    w.t0 = k.cur - k.first;
+    w.t1 = min(k.key.nt, w.t0 + k.end - k.cur);
+    w.slot = !p.merge_all && w.t0 == 0 && w.t1 == k.key.nt
                  ? -1
-                 : w.b * per_e + idx + static_cast<int>(blockIdx.x);
+                 : (k.e * n_rt + k.rt) * p.Hkv + k.kvh + static_cast<int>(blockIdx.x);
+    k.cur = k.first + w.t1;
+    if (w.t1 == k.key.nt && k.cur < k.end) {  // on to the next unit
+      k.first = k.cur;
+      if (++k.kvh == p.Hkv) {
+        k.kvh = 0;
+        if (++k.rt == n_rt) {
+          k.rt = 0;
+          do ++k.e; while (cum[k.e + 1] == k.cur);
+          k.key = entry_keys<AL>(p, k.e);
+        }
+      }
+    }
   } else {
     k.cur = 1;
     // longest row tiles (the last ones of a causal chunk) first
     const int rq = static_cast<uint32_t>(blockIdx.y) / static_cast<uint32_t>(p.Hkv);
     const int rt = p.n_rt - 1 - rq;
     const int b = blockIdx.z;
-    const Seg& s = p.seg;
     const int nq = p.q_lens ? min(max(p.q_lens[b], 0), s.units) : s.units;
     w.b = b;
     w.kvh = static_cast<int>(blockIdx.y) - rq * p.Hkv;
     w.row0 = rt * MT;
     w.rows = min(MT, nq * p.nrep - w.row0);
     if (w.rows <= 0) return false;
-    w.key = make_keys(s, seg_len(s, b), nq, static_cast<uint32_t>(w.row0) / static_cast<uint32_t>(p.nrep),
-                      static_cast<uint32_t>(w.row0 + w.rows - 1) / static_cast<uint32_t>(p.nrep));
+    w.key = make_keys<AL>(s, seg_len(s, b), nq, static_cast<uint32_t>(w.row0) / static_cast<uint32_t>(p.nrep),
+                          static_cast<uint32_t>(w.row0 + w.rows - 1) / static_cast<uint32_t>(p.nrep));
     const uint32_t nt = max(w.key.nt, 1), ns = p.n_split, split = blockIdx.x;  // nt < 2^24, ns <= 16
     w.t0 = static_cast<int>(nt * split / ns);
     w.t1 = static_cast<int>(nt * (split + 1) / ns);
@@ -241,10 +274,10 @@ int set_smem(K kern, int bytes, std::atomic<uint64_t>& ready) {
   return HQ_OK;
 }
 
-// Launches a kernel of one Params; with p.after it may start beside the kernel before it on the
+// Launches a kernel of Params (and more); with p.after it may start beside the kernel before it on the
 // stream (which it does not read from), and completes after it.
-template <typename K>
-int launch_after(K kern, const Params& p, dim3 grid, int threads, int smem, cudaStream_t st) {
+template <typename K, typename... A>
+int launch_after(K kern, dim3 grid, int threads, int smem, cudaStream_t st, const Params& p, const A&... more) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -255,7 +288,7 @@ int launch_after(K kern, const Params& p, dim3 grid, int threads, int smem, cuda
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.after ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, more...);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return static_cast<int>(e);

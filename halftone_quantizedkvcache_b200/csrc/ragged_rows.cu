@@ -9,9 +9,11 @@
 // scale, and P v_scale likewise goes in as three digits; O is float32.
 //
 // A block is 4 warps, 32 keys of a tile each with their own online softmax; two blocks per SM.
-// Tiles arrive by cp.async into a ring of 3 stages, 128-byte swizzled: 16 bytes per copy, each
-// with an address of its own, so sinks and window share a tile and rows may have any stride.
-// Two tiles are in flight while one is worked on, across the borders of sequences.
+// Tiles arrive by TMA into a ring of 3 stages, 128-byte swizzled; two are in flight while one
+// is worked on, across the borders of sequences.  A tile inside one run of keys is one box per
+// side; the tile in which the sinks end and the window begins is put together from boxes of 8
+// keys.  (cp.async of 16 bytes a thread did both with one rule, but under load its issue held
+// the warps up for 2400 cycles a tile: 138 us against NEW_US at 64 sequences x 4096 keys.)
 #include "decode_common.cuh"
 #include "ragged_common.cuh"
 
@@ -25,30 +27,38 @@ constexpr int kWarps = 4;
 template <int NR>
 struct RCfg {
   static constexpr int NT = (NR + 1) / 2;                  // n8 tiles, 2 rows each
-  // q' and its digit table, dead once the fragments are in registers; the warps' sums later
-  static constexpr int kOffQs = kStagesM * 2 * kTileB;     // [NR][kD]
-  static constexpr int kOffQtab = kOffQs + NR * kD * 4;    // NT x 1 KB
-  static constexpr int kOffWo = kOffQs;                    // [kWarps][NR][kD]
+  // the digit table of q', dead once the fragments are in registers; the warps' sums later
+  static constexpr int kOffQtab = kStagesM * 2 * kTileB;   // NT x 1 KB
+  static constexpr int kOffWo = kOffQtab;                  // [kWarps][NR][kD]
   static constexpr int kOffLimb = kOffWo + kWarps * NR * kD * 4;  // p' digits, per warp
-  static_assert(kOffQtab + NT * 1024 <= kOffLimb, "q' lies inside the sums");
+  static_assert(kOffQtab + NT * 1024 <= kOffLimb, "the table lies inside the sums");
   static constexpr int kOffWm = kOffLimb + kWarps * NT * 256;     // [kWarps][NR] (m, l)
-  static constexpr int kOffCum = kOffWm + kWarps * NR * 8;
+  static constexpr int kOffBar = kOffWm + kWarps * NR * 8;        // [kStagesM] tile arrived
+  static constexpr int kOffCum = kOffBar + 32;
   static constexpr int smem(int entries) { return 1024 + kOffCum + 4 * (entries + 1); }
   static_assert(2 * (smem(kMaxEntries) + 1024) <= 233472, "two blocks per SM");
 };
 
+struct Maps {
+  CUtensorMap k, v;      // boxes of 128 keys
+  CUtensorMap k8, v8;    // boxes of 8 keys
+  int bm, hm;            // batch and head coordinates' factors (0: one copy for all)
+  int inner;             // dimensions (channel, head, key, batch): heads closer than keys
+};
+
 template <int NR>
-__global__ void __launch_bounds__(kThreads, 2) rows_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2)
+    rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps) {
   using C = RCfg<NR>;
   constexpr int NT = C::NT;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* qs = reinterpret_cast<float*>(ring + C::kOffQs);
   unsigned char* plimb = ring + C::kOffLimb;
   uint32_t* qtab = reinterpret_cast<uint32_t*>(ring + C::kOffQtab);
   float* wo = reinterpret_cast<float*>(ring + C::kOffWo);
   float2* wm = reinterpret_cast<float2*>(ring + C::kOffWm);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::kOffBar);
   int* cum = reinterpret_cast<int*>(ring + C::kOffCum);
   __shared__ float red[kWarps][NR];
   __shared__ float qmax_s[NR];
@@ -57,60 +67,74 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const __grid_constant
   const int g = lane >> 2, t4 = lane & 3;
   // dependents may be scheduled; they wait for this grid
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    for (int i = 0; i < kStagesM; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
   // zero the p' staging (columns 3 and 7 stay zero)
   for (int i = tid; i < kWarps * NT * 64; i += kThreads) reinterpret_cast<uint32_t*>(plimb)[i] = 0;
-  build_cum<128>(p, cum, kThreads);
-  Walk walk = walk_start<128, true>(p, cum);
+  build_cum<128, 8>(p, cum, kThreads);
+  Walk walk = walk_start<128, true, 8>(p, cum);
   const Seg& s = p.seg;
   const uint64_t pol = l2_evict_first();
 
   // ---- the loads' cursor, two tiles ahead
   Walk lw = walk;
   Piece lp{};
-  int lt = -1;
+  int lt = -1, issued = 0;
   bool more = true;
-  const int crow = tid >> 3, cch = tid & 7;
-  const int8_t *kp = nullptr, *vp = nullptr;
   int64_t vs0 = 0;
-  float vs_n[3][2];  // V scales of this lane's own keys: this tile, the next two
-  // the next tile into stage `st` (nothing past the last), its V scales into v
-  auto issue = [&](int st, float (&v)[2]) {
-    v[0] = v[1] = 0.0f;
+  float vs_n[3][2] = {};  // V scales of this lane's own keys: this tile, the next two
+  // the next tile into stage `st` (nothing past the last), its V scales into the queue's end
+  auto issue = [&](int st) {
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+      vs_n[0][rb] = vs_n[1][rb];
+      vs_n[1][rb] = vs_n[2][rb];
+      vs_n[2][rb] = 0.0f;
+    }
     if (more && ++lt >= lp.t1) {
-      more = walk_next<128, true>(lw, p, cum, lp);
+      more = walk_next<128, true, 8>(lw, p, cum, lp);
       lt = lp.t0;
-      const int64_t o = lp.b * s.sb + lp.kvh * s.sh + 16 * cch;
-      kp = s.k + o;
-      vp = s.v + o;
       vs0 = lp.b * s.vscb + lp.kvh * s.vsch;
     }
-    if (more) {
-      unsigned char* kd = ring + st * 2 * kTileB + swz(crow, cch);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {  // row crow + 16 i: the same swizzle
-        const int vk = lt * kBN + crow + 16 * i;
-        const int64_t key = vk < lp.key.ns ? vk : vk + lp.key.sh;
-        const int nb = vk < lp.key.nv ? 16 : 0;
-        const int64_t off = nb ? key * s.ss : 0;
-        cp_async16(kd + i * 2048, kp + off, nb, pol);
-        cp_async16(kd + kTileB + i * 2048, vp + off, nb, pol);
-      }
-#pragma unroll
-      for (int rb = 0; rb < 2; ++rb) {
-        const int vk = lt * kBN + warp * 32 + rb * 16 + g + 8 * (t4 & 1);
-        const int64_t key = vk < lp.key.ns ? vk : vk + lp.key.sh;
-        if (vk < lp.key.nv) v[rb] = load_scale(s.vsc, vs0 + key * s.vscs, p.s_dt);
+    if (!more) return;
+    ++issued;
+    const int v0 = lt * kBN;
+    if (tid == 0) {
+      unsigned char* kd = ring + st * 2 * kTileB;
+      const int head = lp.kvh * maps.hm, z = lp.b * maps.bm;
+      const bool one = lp.key.sh == 0 || v0 >= lp.key.nsp || v0 + kBN <= lp.key.nsp;
+      const CUtensorMap* mk = one ? &maps.k : &maps.k8;
+      const CUtensorMap* mv = one ? &maps.v : &maps.v8;
+      if (v0 >= lp.key.nv) {  // an empty sequence: nothing to read, and nothing of it is seen
+        mbar_arrive(&full[st]);
+      } else {
+        mbar_arrive_expect_tx(&full[st], 2 * kTileB);  // (boxes past the cache's end: zeros)
+#pragma unroll 1
+        for (int i = 0; i < (one ? 1 : kBN); i += 8) {
+          const int key = lp.key.key(v0 + i);
+          const int x1 = maps.inner ? head : key, x2 = maps.inner ? key : head;
+          tma_load_4d(kd + i * kD, mk, 0, x1, x2, z, &full[st], pol);
+          tma_load_4d(kd + kTileB + i * kD, mv, 0, x1, x2, z, &full[st], pol);
+        }
       }
     }
-    cp_async_commit();
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+      const int v = v0 + warp * 32 + rb * 16 + g + 8 * (t4 & 1);
+      if (v < lp.key.nv && !lp.key.padding(v))
+        vs_n[2][rb] = load_scale(s.vsc, vs0 + static_cast<int64_t>(lp.key.key(v)) * s.vscs, p.s_dt);
+    }
   };
-  issue(0, vs_n[0]);
-  issue(1, vs_n[1]);
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) issue(i);
 
   unsigned char* my_limb = plimb + warp * NT * 256;
-  int stage = 0;
+  int done = 0;  // tiles worked on
+  bool ok = true;
   Piece w{};
-  while (walk_next<128, true>(walk, p, cum, w)) {
+  while (ok && walk_next<128, true, 8>(walk, p, cum, w)) {
     // ---- q' and its digits; thread owns channel d
     const int d = tid, rows = w.rows;
     {
@@ -145,36 +169,32 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const __grid_constant
       }
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        const float v = qv[r] * ks * p.qk_scale;
-        qs[r * kD + d] = v;
-        const float m = dec::warp_max(fabsf(v), 1);
+        qv[r] *= ks * p.qk_scale;
+        const float m = dec::warp_max(fabsf(qv[r]), 1);
         if (lane == 0) red[warp][r] = m;
       }
       __syncthreads();
-      if (tid < NR) qmax_s[tid] = fmaxf(fmaxf(red[0][tid], red[1][tid]), fmaxf(red[2][tid], red[3][tid]));
+      // B fragments: word (nt, j, hh, lane g * 4 + t4) packs digit g % 4 of row 2 nt + g / 4 at
+      // the channels 32 j + 16 hh + 4 t4 + e (what digit 3 and rows past NR hold is multiplied
+      // by zero)
+      unsigned char* at = reinterpret_cast<unsigned char*>(qtab) +
+                          4 * ((d >> 5) * 64 + ((d >> 4) & 1) * 32 + ((d >> 2) & 3)) + (d & 3);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float qm = fmaxf(fmaxf(red[0][r], red[1][r]), fmaxf(red[2][r], red[3][r]));
+        if (tid == 0) qmax_s[r] = qm;
+        const float inv = qm > 0.0f ? kLimbMax / qm : 0.0f;
+        const int x = max(-static_cast<int>(kLimbMax),
+                          min(static_cast<int>(kLimbMax), __float2int_rn(qv[r] * inv)));
+        int la, lb, lc;
+        limbs24(x, la, lb, lc);
+        unsigned char* row = at + 4 * ((r >> 1) * 256 + 4 * (4 * (r & 1)));
+        row[0] = static_cast<unsigned char>(la);
+        row[16] = static_cast<unsigned char>(lb);
+        row[32] = static_cast<unsigned char>(lc);
+      }
       __syncthreads();
     }
-    // B fragments: word (nt, j, hh, lane g * 4 + t4) packs digit g % 4 of row 2 nt + g / 4 at
-    // the channels 32 j + 16 hh + 4 t4 + e
-#pragma unroll 1
-    for (int i = tid; i < NT * 256; i += kThreads) {
-      const int nt = i >> 8, j = (i >> 6) & 3, hh = (i >> 5) & 1, gg = (i >> 2) & 7, tt = i & 3;
-      const int r = 2 * nt + (gg >> 2), limb = gg & 3;
-      uint32_t wd = 0;
-      if (r < NR && limb < 3) {
-        const float qm = qmax_s[r];
-        const float inv = qm > 0.0f ? kLimbMax / qm : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int dd = 32 * j + 16 * hh + 4 * tt + e;
-          const int x = max(-static_cast<int>(kLimbMax),
-                            min(static_cast<int>(kLimbMax), __float2int_rn(qs[r * kD + dd] * inv)));
-          wd |= limb_byte(x, limb) << (8 * e);
-        }
-      }
-      qtab[i] = wd;
-    }
-    __syncthreads();
     uint32_t bq[NT][4][2];
     float f0[NT], f1[NT];
 #pragma unroll
@@ -233,18 +253,16 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const __grid_constant
     int since = 0;
 #pragma unroll 1
     for (int t = w.t0; t < w.t1; ++t) {
-      cp_async_wait<1>();
-      __syncthreads();  // this tile has arrived for every thread; the one before is done with
-      const int st = stage;
-      stage = stage == kStagesM - 1 ? 0 : stage + 1;
-      const int st2 = stage == kStagesM - 1 ? 0 : stage + 1;  // tile + 2
-      issue(st2, vs_n[2]);
-      const float vsf[2] = {vs_n[0][0], vs_n[0][1]};
-#pragma unroll
-      for (int rb = 0; rb < 2; ++rb) {
-        vs_n[0][rb] = vs_n[1][rb];
-        vs_n[1][rb] = vs_n[2][rb];
+      const int st = done % kStagesM;
+      ok = mbar_wait(&full[st], (done / kStagesM) & 1);
+      // (all threads: the stage of the tile before is free for the tile two on)
+      if (__syncthreads_or(!ok)) {
+        ok = false;
+        break;
       }
+      ++done;
+      issue((st + 2) % kStagesM);
+      const float vsf[2] = {vs_n[0][0], vs_n[0][1]};
       const int base = t * kBN + warp * 32, lim = w.key.nv;
       const uint32_t kt = smem_u32(ring + st * 2 * kTileB);
       const uint32_t vt = kt + kTileB;
@@ -274,8 +292,8 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const __grid_constant
           lo += __shfl_xor_sync(0xffffffffu, lo, 1);
           hi += __shfl_xor_sync(0xffffffffu, hi, 1);
           const int key = base + rb * 16 + g;
-          sc[nt][rb][0] = key < lim ? lo : -INFINITY;
-          sc[nt][rb][1] = key + 8 < lim ? hi : -INFINITY;
+          sc[nt][rb][0] = key < lim && !w.key.padding(key) ? lo : -INFINITY;
+          sc[nt][rb][1] = key + 8 < lim && !w.key.padding(key + 8) ? hi : -INFINITY;
         }
       }
       // ---- online softmax per row; p' digits of this lane's own two keys
@@ -292,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const __grid_constant
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
           const float sown = (t4 & 1) ? sc[nt][rb][1] : sc[nt][rb][0];
-          pr[rb] = base + rb * 16 + g + 8 * (t4 & 1) < lim ? exp2f(sown - m_new) : 0.0f;
+          pr[rb] = sown == -INFINITY ? 0.0f : exp2f(sown - m_new);
           pv[rb] = pr[rb] * vsf[rb];
           pm = fmaxf(pm, pv[rb]);
         }
@@ -370,6 +388,8 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const __grid_constant
       }
     }
 
+    if (!ok) break;
+
     // ---- the 4 warps' states into one, per row
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -418,26 +438,65 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const __grid_constant
     }
     __syncthreads();  // q' of the next piece goes where the sums lie
   }
-  cp_async_wait<0>();
+  if (!ok) {
+    report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
+    if (tid == 0)  // no copy is in flight when the block ends
+      for (int i = done; i < issued; ++i) mbar_wait(&full[i % kStagesM], (i / kStagesM) & 1);
+  }
   // launched beside the kernel before it: complete only after it
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// Codes [B, Hkv, cap, 128] in boxes of `keys` keys, 128-byte swizzle, zeros past cap.
+inline int encode_map(CUtensorMap* m, const int8_t* base, const Seg& s, int Hkv, int keys,
+                      const Maps& maps) {
+  auto enc = dec::encode_fn();
+  if (!enc) return HQ_ERR_UNSUPPORTED;
+  const int in = maps.inner;
+  const cuuint64_t cap = s.cap, heads = maps.hm ? Hkv : 1, ss = s.ss, sh = maps.hm ? s.sh : s.ss;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(kD), in ? heads : cap, in ? cap : heads,
+                              static_cast<cuuint64_t>(maps.bm ? s.nb : 1)};
+  const cuuint64_t strides[3] = {in ? sh : ss, in ? ss : sh, static_cast<cuuint64_t>(maps.bm ? s.sb : s.ss)};
+  const cuuint32_t n = keys;
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(kD), in ? 1u : n, in ? n : 1u, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(base), dims, strides, box,
+                         es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? HQ_OK : HQ_ERR_INVALID_ARGUMENT;
+}
+
 template <int NR>
-int launch_rows(const Params& p, int grid, cudaStream_t st) {
+int launch_rows(const Params& p, const Maps& maps, int grid, cudaStream_t st) {
   using C = RCfg<NR>;
   static std::atomic<uint64_t> ready{0};
   auto kern = rows_kernel<NR>;
   const int rc = set_smem(kern, C::smem(kMaxEntries), ready);
   if (rc != HQ_OK) return rc;
-  return launch_after(kern, p, dim3(grid), kThreads, C::smem(p.seg.nb), st);
+  return launch_after(kern, dim3(grid), kThreads, C::smem(p.seg.nb), st, p, maps);
 }
 
 int rows_stream(const Params& p, int grid, cudaStream_t st) {
-  const int rows = p.seg.units * p.nrep;
-  if (rows == 1) return launch_rows<1>(p, grid, st);
-  if (rows == 2) return launch_rows<2>(p, grid, st);
-  return launch_rows<4>(p, grid, st);
+  Maps maps{};
+  const Seg& s = p.seg;
+  // (an extent of 1, or a stride of 0, is one copy for all)
+  maps.hm = p.Hkv > 1 && s.sh != 0;
+  maps.bm = s.nb > 1 && s.sb != 0;
+  maps.inner = maps.hm && s.sh < s.ss;
+  int rc = HQ_OK;
+  if (s.cap > 0) {  // (an empty cache is never read)
+    rc = encode_map(&maps.k, s.k, s, p.Hkv, kBN, maps);
+    if (rc == HQ_OK) rc = encode_map(&maps.v, s.v, s, p.Hkv, kBN, maps);
+    if (s.sinks > 0 && s.window < s.cap) {  // (else the keys are one run)
+      if (rc == HQ_OK) rc = encode_map(&maps.k8, s.k, s, p.Hkv, 8, maps);
+      if (rc == HQ_OK) rc = encode_map(&maps.v8, s.v, s, p.Hkv, 8, maps);
+    }
+  }
+  if (rc != HQ_OK) return rc;
+  const int rows = s.units * p.nrep;
+  if (rows == 1) return launch_rows<1>(p, maps, grid, st);
+  if (rows == 2) return launch_rows<2>(p, maps, grid, st);
+  return launch_rows<4>(p, maps, grid, st);
 }
 
 }  // namespace rag

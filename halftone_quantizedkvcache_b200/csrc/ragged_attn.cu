@@ -41,6 +41,8 @@
 // memory, where it overwrites the S it came from.  mbarriers order the roles; every wait is
 // bounded.  (Codes loaded into registers and converted from there took 4000 cycles a tile:
 // the proxy fence before each hand-over waited for the loads of the next tile.)
+#include <type_traits>
+
 #include "ragged_common.cuh"
 #include "umma.cuh"
 
@@ -68,8 +70,8 @@ struct Cfg {
   static constexpr int kOffV = kOffK + kStages * kTileB;
   static constexpr int kOffSlot = kOffV + kStages * kTileB;
   static constexpr int kOffE = kOffSlot + kSlots * kSlotB;         // [slot][e_j, 2^-e_j][128]
-  static constexpr int kOffG = kOffE + kLvSlots * 2 * kBN * 4;     // [slot][128] float16 g_j
-  static constexpr int kOffInfo = kOffG + kLvSlots * kBN * 2;      // [slot]{any e_j, 2^E}
+  static constexpr int kOffG = kOffE + kLvSlots * 2 * kBN * 4;     // [slot][128] g_j, float16 twice
+  static constexpr int kOffInfo = kOffG + kLvSlots * kBN * 4;      // [slot]{any e_j, 2^E}
   static constexpr int kOffKs = kOffInfo + kLvSlots * 8;           // [128] k_scale sm_scale log2 e
   static constexpr int kOffBar = kOffKs + kD * 4;
   static constexpr int kBars = 1 + 4 * kStages + 2 * kSlots + kLvSlots + 2 + 2 + 2 * NM + 1;
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* eb = reinterpret_cast<float*>(smem + C::kOffE);
-  __half* gb = reinterpret_cast<__half*>(smem + C::kOffG);
+  uint32_t* gb = reinterpret_cast<uint32_t*>(smem + C::kOffG);
   float2* info = reinterpret_cast<float2*>(smem + C::kOffInfo);
   float* ksm = reinterpret_cast<float*>(smem + C::kOffKs);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
@@ -663,44 +665,37 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
   } else if (warp < kMmaWarp) {
     // ================= staged codes -> float16 tiles
     const int ct = tid - C::kSoft;
-    const int c16 = ct & 7, row = ct >> 3;  // 16 codes of rows row + 16 i of a slot
-    // where this thread's two 16-byte chunks go; the upper half of each 8 lanes stores its
-    // second chunk first, so that 8 lanes write 8 different chunk columns
-    const int first = c16 >> 2;
-    const uint32_t blk = static_cast<uint32_t>(c16 >> 2) * (kBN * 128);
-    const uint32_t at0 = blk + sw128(row, ((2 * c16) & 7) + first);
-    const uint32_t at1 = blk + sw128(row, ((2 * c16) & 7) + 1 - first);
-    constexpr int NI = kSlotKeys / 16;
+    // 8 codes (one 16-byte chunk) of rows row + 8 i of a slot: 8 lanes store 8 different chunk
+    // columns, and rows 8 apart have the same swizzle
+    const int c8 = ct & 15, row = ct >> 4;
+    const uint32_t at = static_cast<uint32_t>(c8 >> 3) * (kBN * 128) + sw128(row, c8 & 7);
     int sc = 0, gt = 0;  // slots, tiles
     bool ok = true;
-    auto put = [&](unsigned char* tile, int i, const uint32_t (&x)[8]) {  // row + 16 i
-      const uint4 a = make_uint4(x[0], x[1], x[2], x[3]), b = make_uint4(x[4], x[5], x[6], x[7]);
-      *reinterpret_cast<uint4*>(tile + at0 + i * 2048) = first ? b : a;
-      *reinterpret_cast<uint4*>(tile + at1 + i * 2048) = first ? a : b;
-    };
     // the next staging slot into rows 64 half .. of a tile; V rows times their g
-    auto convert = [&](unsigned char* tile, int half, const __half* g) {
+    auto convert = [&](unsigned char* tile, auto is_v, const uint32_t* g) {
       const int sl = sc % C::kSlots;
       ok = wait_bar(&st_full[sl], (sc / C::kSlots) & 1, abort);
       if (!ok) return;
-      const unsigned char* src = smem + C::kOffSlot + sl * kSlotB + row * kD + 16 * c16;
-      tile += half * 64 * 128;
-#pragma unroll 2
-      for (int i = 0; i < NI; ++i) {
-        const uint4 x = *reinterpret_cast<const uint4*>(src + i * 16 * kD);
-        uint32_t y[8];
-        codes_to_h2(x.x, y[0], y[1]);
-        codes_to_h2(x.y, y[2], y[3]);
-        codes_to_h2(x.z, y[4], y[5]);
-        codes_to_h2(x.w, y[6], y[7]);
-        if (g) {
-          const uint32_t h = *reinterpret_cast<const uint16_t*>(g + 64 * half + row + 16 * i);
-          const uint32_t g2 = h | h << 16;
+      const unsigned char* src = smem + C::kOffSlot + sl * kSlotB + row * kD + 8 * c8;
+      uint2 x[8];
+      uint32_t g2[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y[e]) : "r"(y[e]), "r"(g2));
+      for (int i = 0; i < 8; ++i) {
+        x[i] = *reinterpret_cast<const uint2*>(src + i * 8 * kD);
+        if constexpr (is_v.value) g2[i] = g[row + 8 * i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint4 y;
+        codes_to_h2(x[i].x, y.x, y.y);
+        codes_to_h2(x[i].y, y.z, y.w);
+        if constexpr (is_v.value) {
+          asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.x) : "r"(y.x), "r"(g2[i]));
+          asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.y) : "r"(y.y), "r"(g2[i]));
+          asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.z) : "r"(y.z), "r"(g2[i]));
+          asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.w) : "r"(y.w), "r"(g2[i]));
         }
-        put(tile, i, y);
+        *reinterpret_cast<uint4*>(tile + at + i * 1024) = y;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&st_empty[sl]);
@@ -713,7 +708,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         if (!ok) break;
 #pragma unroll 1
         for (int half = 0; half < 2 && ok; ++half)
-          convert(smem + C::kOffK + st * kTileB, half, nullptr);
+          convert(smem + C::kOffK + st * kTileB + half * 8192, std::false_type{}, nullptr);
         if (!ok) break;
         fence_async_smem();
         __syncwarp();
@@ -723,7 +718,8 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         if (!ok) break;
 #pragma unroll 1
         for (int half = 0; half < 2 && ok; ++half)
-          convert(smem + C::kOffV + st * kTileB, half, gb + slot * kBN);
+          convert(smem + C::kOffV + st * kTileB + half * 8192, std::true_type{},
+                  gb + slot * kBN + half * kSlotKeys);
         if (!ok) break;
         fence_async_smem();
         __syncwarp();
@@ -817,7 +813,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
           const float x = zero ? kTinyScale : vs[i];
           ev[32 * i + lane] = __log2f(x);
           ev[kBN + 32 * i + lane] = __frcp_rn(x);
-          gb[slot * kBN + 32 * i + lane] = __float2half_rn(zero ? 0.0f : 1.0f);
+          gb[slot * kBN + 32 * i + lane] = zero ? 0u : 0x3c003c00u;
         }
       } else {
         int ex[4];
@@ -844,8 +840,8 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
           ev[32 * i + lane] = static_cast<float>(e);
           ev[kBN + 32 * i + lane] = pow2i(-e);
           // (two factors: the exponent of their product may leave float32's)
-          gb[slot * kBN + 32 * i + lane] =
-              __float2half_rn(vs[i] < kTinyScale ? 0.0f : vs[i] * pow2i(-E) * pow2i(-e));
+          const float gj = vs[i] < kTinyScale ? 0.0f : vs[i] * pow2i(-E) * pow2i(-e);
+          gb[slot * kBN + 32 * i + lane] = pack_h2(gj, gj);
         }
       }
       if (lane == 0) info[slot] = make_float2(any ? 1.0f : 0.0f, pow2i(E));

@@ -25,16 +25,18 @@
 // eighth of the output's own half step.
 //
 // Work.  Row r of a unit (kv head, sequence or group) is q head kvh * n_rep + r % n_rep of
-// query r / n_rep; 128 rows sit on the 128 lanes of tensor memory, one or two such tiles
-// per block share every key tile (NM).  Keys that no row of the block can see are never
-// read: a block's keys are numbered v = 0 .. nv - 1, the sinks first, then the window's
+// query r / n_rep; 128 rows sit on the 128 lanes of tensor memory.  A block has two groups of
+// softmax warps, S buffers and O accumulators: for more than 128 rows the groups hold two row
+// tiles that share every key tile, else (ALT) one row tile whose key tiles they take in turn,
+// each with a softmax state of its own, joined at the end.  Keys that no row of the block can
+// see are never read: a block's keys are numbered v = 0 .. nv - 1, the sinks first, then the window's
 // run, and cut into tiles of 128.  Decode kernels (STREAM) lay the tiles of all units in
 // one line and give each block an equal run of it, whatever the lengths; a unit cut by a
 // block border leaves partial states (m, l, O) that combine_kernel joins.  Prefill blocks
 // take one row tile each (split over a few blocks when there are few).
 //
-// Roles of a block (one per SM): softmax warps (4 per row tile, one thread per row; they also
-// form q'), 4 warps that turn staged codes into float16 with byte permutes and store them in
+// Roles of a block (one per SM): softmax warps (2 x 4, one thread per row; they also form q'),
+// 8 warps that turn staged codes into float16 with byte permutes and store them in
 // the 128-byte-swizzled layouts the MMA reads, one warp that fills the staging ring with bulk
 // copies (64 keys of K or V per slot), one that reads the V scales, and one that issues the
 // tcgen05.mma products: S = Q K^T into tensor memory, O += P V with P read from tensor
@@ -50,31 +52,33 @@ namespace hq {
 namespace rag {
 using namespace tc;
 
-constexpr int kConvThreads = 128;
+constexpr int kSoft = 256;                // softmax threads: two groups of 128
+constexpr int kConvThreads = 256;
 constexpr int kTileB = kBN * kD * 2;      // a float16 K, V or Q tile: 32 KB
 constexpr int kStages = 2;                // K and V tiles in shared memory
 constexpr int kSlotKeys = 64;             // keys of a staging slot (K or V codes)
 constexpr int kSlotB = kSlotKeys * kD;
 constexpr int kLvSlots = 2;               // ring of what the tiles' V scales lead to
-constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 256;           // S buffers at columns 0 and 128
 
-template <int NM, bool LO>
+template <bool ALT, bool LO>
 struct Cfg {
-  static constexpr int kSoft = 128 * NM;
   static constexpr int kThreads = kSoft + kConvThreads + 96;
+  static constexpr int kRowTiles = ALT ? 1 : 2;
   static constexpr int kParts = LO ? 2 : 1;
-  static constexpr int kSlots = NM * kParts == 1 ? 7 : 3;          // staging: 8 KB each
-  static constexpr int kOffK = NM * kParts * kTileB;
+  static constexpr int kSlots = kRowTiles * kParts == 1 ? 7 : 3;   // staging: 8 KB each
+  static constexpr int kOffK = kRowTiles * kParts * kTileB;
   static constexpr int kOffV = kOffK + kStages * kTileB;
   static constexpr int kOffSlot = kOffV + kStages * kTileB;
   static constexpr int kOffE = kOffSlot + kSlots * kSlotB;         // [slot][e_j, 2^-e_j][128]
   static constexpr int kOffG = kOffE + kLvSlots * 2 * kBN * 4;     // [slot][128] g_j, float16 twice
   static constexpr int kOffInfo = kOffG + kLvSlots * kBN * 4;      // [slot]{any e_j, 2^E}
   static constexpr int kOffKs = kOffInfo + kLvSlots * 8;           // [128] k_scale sm_scale log2 e
-  static constexpr int kOffBar = kOffKs + kD * 4;
-  static constexpr int kBars = 1 + 4 * kStages + 2 * kSlots + kLvSlots + 2 + 2 + 2 * NM + 1;
+  // [2][128] float2: a row's halves' largest |q|; later the groups' (m, l)
+  static constexpr int kOffRow = kOffKs + kD * 4;
+  static constexpr int kOffBar = kOffRow + (ALT ? 2 * kBN * 8 : 0);
+  static constexpr int kBars = 1 + 4 * kStages + 2 * kSlots + kLvSlots + 2 + 2 + 2 + 1 + 1 + 1;
   static constexpr int kOffMisc = kOffBar + ((kBars * 8 + 15) & ~15);
   static constexpr int kOffCum = kOffMisc + 16;
   static constexpr int smem(int entries) { return 1024 + kOffCum + 4 * (entries + 1); }
@@ -130,47 +134,37 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-// 32 columns of this thread's lane, loaded by tmem_get and valid after tmem_got (which
+// 16 columns of this thread's lane, loaded by tmem_get and valid after tmem_got (which
 // awaits every load issued before it; the registers pass through it, so no use moves up)
-__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-      "%28, %29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_got(uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_got(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
                  "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
-                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                 "+r"(r[30]), "+r"(r[31]));
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
-// Bounded wait (2 s, or as soon as another role of the block has given up).  The loop is a
-// call: the roles' code together has to stay within the instruction cache.
-__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255) == 0) {
-      const uint64_t t = global_ns();
-      if (t0 == 0) t0 = t;
-      if (*abort || t - t0 > kWaitNs) {
-        *abort = 1;
-        return false;
-      }
-    }
-  }
-}
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return mbar_try_wait(bar, parity) || wait_long(bar, parity, abort);
+// Bounded wait: some seconds, then false.  One opaque loop: as C++ with its convergence
+// instructions the waits took a third of all issue slots.
+constexpr uint32_t kPolls = 1u << 22;
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
+      "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n"
+      " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
+      "there:\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "n"(kPolls)
+      : "memory");
+  return ok != 0;
 }
 
 __device__ __forceinline__ void unpack8(const uint4& x, int dt, float (&f)[8]) {
@@ -241,7 +235,7 @@ __device__ __noinline__ void rescale(uint32_t o_addr, float a) {
 // The running maximum takes this tile's largest t in, O and l are rescaled where it moves;
 // waits for the previous P V on the way.
 __device__ __forceinline__ void move_max(float mx, uint32_t o_addr, bool first, uint64_t* pv_bar,
-                                         int cnt, volatile int* abort, float& m, float& l, bool& ok) {
+                                         int cnt, float& m, float& l, bool& ok) {
   float a = 1.0f;
   if (mx > m + 8.0f || (m == -INFINITY && mx != -INFINITY)) {
     a = ex2_ftz(m - mx);
@@ -251,7 +245,7 @@ __device__ __forceinline__ void move_max(float mx, uint32_t o_addr, bool first, 
   // The previous P V is in O.  Every tile waits here, whether it rescales or not: a wait by
   // parity tells neighbouring completions apart, so none may be skipped.
   if (cnt > 0) {
-    ok = wait_bar(pv_bar, (cnt - 1) & 1, abort);
+    ok = wait_bar(pv_bar, (cnt - 1) & 1);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) return;
     tc_fence_after();
@@ -259,26 +253,33 @@ __device__ __forceinline__ void move_max(float mx, uint32_t o_addr, bool first, 
   if (!first && __any_sync(0xffffffffu, a != 1.0f)) rescale(o_addr, a);
 }
 
-// One tile of one row that sees all of it: the running maximum, then P = 2^(t - m) over S, and
-// l.  EXP: t = s fac + e_j with e_j from ev[j] and 2^-e_j from ev[128 + j], else t = s fac.
-template <bool EXP>
+// One tile of one row: the running maximum, then P = 2^(t - m) over S, and l.  EXP: t = s fac +
+// e_j with e_j from ev[j] and 2^-e_j from ev[128 + j], else t = s fac.  MASK: some row of the
+// warp does not see all of the tile.
+template <bool EXP, bool MASK>
 __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, const float* ev,
-                                             float fac, bool first, uint64_t* pv_bar, int cnt,
-                                             volatile int* abort, float& m, float& l, bool& ok) {
-  uint32_t sa[32], sb[32];
+                                             float fac, int v0, const RowLim& lim, bool first,
+                                             uint64_t* pv_bar, int cnt,
+                                             float& m, float& l, bool& ok) {
+  uint32_t sa[16], sb[16];
   float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  auto fold = [&](const uint32_t (&s)[32], const float* e_run) {
+  auto fold = [&](const uint32_t (&s)[16], int c) {
+    const uint32_t seen = MASK ? lim.bits(v0 + c) : 0xffffu;
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {
+    for (int e = 0; e < 16; e += 4) {
       float t[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) t[i] = __uint_as_float(s[e + i]);
       if constexpr (EXP) {
-        const float4 e4 = *reinterpret_cast<const float4*>(e_run + e);
+        const float4 e4 = *reinterpret_cast<const float4*>(ev + c + e);
         t[0] = __fmaf_rn(t[0], fac, e4.x);
         t[1] = __fmaf_rn(t[1], fac, e4.y);
         t[2] = __fmaf_rn(t[2], fac, e4.z);
         t[3] = __fmaf_rn(t[3], fac, e4.w);
+      }
+      if constexpr (MASK) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = seen & (1u << (e + i)) ? t[i] : -INFINITY;
       }
       const int k = (e >> 2) & 1;
       x[2 * k] = fmaxf(x[2 * k], fmaxf(t[0], t[1]));
@@ -287,71 +288,75 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, c
   };
   tmem_get(s_addr, sa);
 #pragma unroll 1
-  for (int c = 0; c < 128; c += 64) {
+  for (int c = 0; c < 128; c += 32) {
     tmem_got(sa);
-    tmem_get(s_addr + c + 32, sb);
-    fold(sa, ev + c);
+    tmem_get(s_addr + c + 16, sb);
+    fold(sa, c);
     tmem_got(sb);
-    if (c == 0) tmem_get(s_addr + 64, sa);
-    fold(sb, ev + c + 32);
+    if (c < 96) tmem_get(s_addr + c + 32, sa);
+    fold(sb, c + 16);
   }
   float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
   if constexpr (!EXP) mx *= fac;
-  move_max(mx, o_addr, first, pv_bar, cnt, abort, m, l, ok);
+  tmem_get(s_addr, sa);
+  move_max(mx, o_addr, first, pv_bar, cnt, m, l, ok);
   if (!ok) return;
   const float nb = m == -INFINITY ? 0.0f : -m;
-  const F2 nb2 = f2_make(nb, nb), fac2 = f2_make(fac, fac);
-  F2 ls0 = f2_make(0.0f, 0.0f), ls1 = ls0;
+  // (scalar: packed pairs cost more moves than they save)
+  float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   // P of keys c .. goes over S columns c / 2 .., which have been read by then
-  auto emit = [&](const uint32_t (&s)[32], int c) {
-    uint32_t w[16];
+  auto emit = [&](const uint32_t (&s)[16], int c) {
+    const uint32_t seen = MASK ? lim.bits(v0 + c) : 0xffffu;
+    uint32_t w[8];
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {
+    for (int e = 0; e < 16; e += 4) {
       float t[4];
-      F2 n0 = nb2, n1 = nb2;
+      float en[4] = {nb, nb, nb, nb};
       if constexpr (EXP) {
         const float4 e4 = *reinterpret_cast<const float4*>(ev + c + e);
-        n0 = f2_add(f2_make(e4.x, e4.y), nb2);
-        n1 = f2_add(f2_make(e4.z, e4.w), nb2);
+        en[0] += e4.x;
+        en[1] += e4.y;
+        en[2] += e4.z;
+        en[3] += e4.w;
       }
-      f2_split(f2_fma(f2_make(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), fac2, n0), t[0], t[1]);
-      f2_split(f2_fma(f2_make(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), fac2, n1), t[2], t[3]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = ex2_ftz(t[i]);
+      for (int i = 0; i < 4; ++i) {
+        t[i] = ex2_ftz(__fmaf_rn(__uint_as_float(s[e + i]), fac, en[i]));
+        if constexpr (MASK) t[i] = seen & (1u << (e + i)) ? t[i] : 0.0f;
+      }
       if constexpr (EXP) {
         const float4 r4 = *reinterpret_cast<const float4*>(ev + kBN + c + e);
-        ls0 = f2_fma(f2_make(t[0], t[1]), f2_make(r4.x, r4.y), ls0);
-        ls1 = f2_fma(f2_make(t[2], t[3]), f2_make(r4.z, r4.w), ls1);
+        ls[0] = __fmaf_rn(t[0], r4.x, ls[0]);
+        ls[1] = __fmaf_rn(t[1], r4.y, ls[1]);
+        ls[2] = __fmaf_rn(t[2], r4.z, ls[2]);
+        ls[3] = __fmaf_rn(t[3], r4.w, ls[3]);
       } else {
-        ls0 = f2_add(ls0, f2_make(t[0], t[1]));
-        ls1 = f2_add(ls1, f2_make(t[2], t[3]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ls[i] += t[i];
       }
       w[e / 2] = pack_h2(t[0], t[1]);
       w[e / 2 + 1] = pack_h2(t[2], t[3]);
     }
-    tmem_st16(s_addr + c / 2, w);
+    tmem_st8(s_addr + c / 2, w);
   };
-  tmem_get(s_addr, sa);
 #pragma unroll 1
-  for (int c = 0; c < 128; c += 64) {
+  for (int c = 0; c < 128; c += 32) {
     tmem_got(sa);
-    tmem_get(s_addr + c + 32, sb);
+    tmem_get(s_addr + c + 16, sb);
     emit(sa, c);
     tmem_got(sb);
-    if (c == 0) tmem_get(s_addr + 64, sa);
-    emit(sb, c + 32);
+    if (c < 96) tmem_get(s_addr + c + 32, sa);
+    emit(sb, c + 16);
   }
-  float x0, x1;
-  f2_split(f2_add(ls0, ls1), x0, x1);
-  l += x0 + x1;
+  l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
   tmem_wait_st();
 }
 
-// The same for a tile with e_j that some row of the warp does not see all of (bf16 models: for
-// any tile that softmax_tile<false> does not take).
+// softmax_tile<true, true> with less code: for a tile with e_j that some row does not see all
+// of, and any tile with e_j of a bf16 model (rare).
 __device__ __forceinline__ void softmax_tile_any(uint32_t s_addr, uint32_t o_addr, const float* ev,
                                                  float fac, int v0, const RowLim& lim, bool first,
-                                                 uint64_t* pv_bar, int cnt, volatile int* abort,
+                                                 uint64_t* pv_bar, int cnt,
                                                  float& m, float& l, bool& ok) {
   float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll 1
@@ -370,7 +375,7 @@ __device__ __forceinline__ void softmax_tile_any(uint32_t s_addr, uint32_t o_add
       x1 = fmaxf(x1, fmaxf(seen & (4u << e) ? t2 : -INFINITY, seen & (8u << e) ? t3 : -INFINITY));
     }
   }
-  move_max(fmaxf(x0, x1), o_addr, first, pv_bar, cnt, abort, m, l, ok);
+  move_max(fmaxf(x0, x1), o_addr, first, pv_bar, cnt, m, l, ok);
   if (!ok) return;
   const float nb = m == -INFINITY ? 0.0f : -m;
   float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -403,17 +408,18 @@ __device__ __forceinline__ void softmax_tile_any(uint32_t s_addr, uint32_t o_add
 }
 
 // ---------------------------------------------------------------- the kernel
-template <int NM, bool LO, bool STREAM>
-__global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<NM, LO>;
-  constexpr int MT = 128 * NM;
-  extern __shared__ __align__(128) unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+template <bool ALT, bool LO, bool STREAM>
+__global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<ALT, LO>;
+  constexpr int MT = 128 * C::kRowTiles;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  // (an offset, not a rounded address: the compiler keeps knowing that this is shared memory)
+  unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   float* eb = reinterpret_cast<float*>(smem + C::kOffE);
   uint32_t* gb = reinterpret_cast<uint32_t*>(smem + C::kOffG);
   float2* info = reinterpret_cast<float2*>(smem + C::kOffInfo);
   float* ksm = reinterpret_cast<float*>(smem + C::kOffKs);
+  float2* rowb = reinterpret_cast<float2*>(smem + C::kOffRow);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* q_full = bars;
   uint64_t* k_full = q_full + 1;
@@ -423,17 +429,18 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
   uint64_t* st_full = v_empty + kStages;
   uint64_t* st_empty = st_full + C::kSlots;
   uint64_t* lv_full = st_empty + C::kSlots;
-  uint64_t* s_full = lv_full + kLvSlots;  // per S buffer
+  uint64_t* s_full = lv_full + kLvSlots;  // per group
   uint64_t* p_ready = s_full + 2;
-  uint64_t* pv_done = p_ready + 2;        // per row tile
-  uint64_t* o_empty = pv_done + NM;
-  uint64_t* drain = o_empty + NM;
+  uint64_t* pv_done = p_ready + 2;
+  uint64_t* o_empty = pv_done + 2;
+  uint64_t* drain = o_empty + 1;
+  uint64_t* soft_bar = drain + 1;         // the softmax warps among themselves
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
-  volatile int* abort = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+  float* two_e = reinterpret_cast<float*>(smem + C::kOffMisc + 8);  // ALT: 2^E of the piece
   int* cum = reinterpret_cast<int*>(smem + C::kOffCum);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kMmaWarp = (C::kSoft + kConvThreads) / 32, kCopyWarp = kMmaWarp + 1;  // + 2: V scales
+  constexpr int kMmaWarp = (kSoft + kConvThreads) / 32, kCopyWarp = kMmaWarp + 1;  // + 2: V scales
   // combine_kernel's blocks may be scheduled; they wait for this grid
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == kMmaWarp) {
@@ -443,8 +450,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     if (lane == 0) {
-      *abort = 0;
-      mbar_init(q_full, C::kSoft / 32);
+      mbar_init(q_full, kSoft / 32);
       for (int i = 0; i < kStages; ++i) {
         mbar_init(&k_full[i], kConvThreads / 32);
         mbar_init(&k_empty[i], 1);
@@ -459,12 +465,11 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
         mbar_init(&p_ready[i], 4);
-      }
-      for (int i = 0; i < NM; ++i) {
         mbar_init(&pv_done[i], 1);
-        mbar_init(&o_empty[i], 4);
       }
+      mbar_init(o_empty, kSoft / 32);
       mbar_init(drain, 1);
+      mbar_init(soft_bar, kSoft / 32);
       fence_mbar_init();
     }
   }
@@ -479,63 +484,28 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
   auto next_piece = [&](Walk& k, Piece& to) { return walk_next<MT, STREAM, 1>(k, p, cum, to); };
   Piece w{};
 
-  if (warp < C::kSoft / 32) {
-    // ================= softmax: one thread per row
-    const int mt = warp >> 2, r = tid;  // row of the piece
+  if (warp < kSoft / 32) {
+    // ================= softmax: one thread per row (ALT: and group)
+    const int grp = warp >> 2, lr = tid & 127, r = ALT ? lr : tid;  // row of its tile, of the piece
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t o_addr = tmem + kColO + 128 * mt + lane_base;
-    int pc = 0, gt = 0, cnt = 0;        // pieces, tiles of the block, tiles of this row tile
-    int64_t q_off = 0;                  // byte offset of this thread's q row
+    const uint32_t s_addr = tmem + 128 * grp + lane_base;
+    const uint32_t o_addr = tmem + kColO + 128 * grp + lane_base;
+    int pc = 0, gt0 = 0, cnt = 0;       // pieces, tiles of the block before this piece, own tiles
     bool ok = true;
-    // q' of this thread's row, formed in place in the Q tile: the raw row, its fake
-    // quantization, its largest |q'|, q'.  Returns 2^-ex.  The tile is free: this warp has
-    // seen the last S of the piece before.  Compact loops: this runs once per piece.
-    unsigned char* q_tile = smem + mt * C::kParts * kTileB;
+    unsigned char* q_tile = smem + (ALT ? 0 : grp) * C::kParts * kTileB;
     auto chunk = [&](int c) {  // 8 channels of the row
-      return reinterpret_cast<uint4*>(q_tile + (c >> 3) * (kBN * 128) + sw128(r & 127, c & 7));
+      return reinterpret_cast<uint4*>(q_tile + (c >> 3) * (kBN * 128) + sw128(lr, c & 7));
     };
-    auto make_q = [&]() -> float {
-      {
-        const char* src = static_cast<const char*>(p.q) + q_off;
-        uint4 x[16];
-#pragma unroll
-        for (int c = 0; c < 16; ++c) x[c] = reinterpret_cast<const uint4*>(src)[c];
-#pragma unroll
-        for (int c = 0; c < 16; ++c) *chunk(c) = x[c];
-      }
-      if (p.q_quant) fake_quant_row(q_tile, r & 127, p.q_dt);
-      float am = 0.0f;
-#pragma unroll 1
-      for (int c = 0; c < 16; ++c) {
-        float f[8];
-        unpack8(*chunk(c), p.q_dt, f);
-        const float4 a = reinterpret_cast<const float4*>(ksm)[2 * c], b = reinterpret_cast<const float4*>(ksm)[2 * c + 1];
-        am = fmaxf(am, fmaxf(fmaxf(fabsf(f[0] * a.x), fabsf(f[1] * a.y)), fmaxf(fabsf(f[2] * a.z), fabsf(f[3] * a.w))));
-        am = fmaxf(am, fmaxf(fmaxf(fabsf(f[4] * b.x), fabsf(f[5] * b.y)), fmaxf(fabsf(f[6] * b.z), fabsf(f[7] * b.w))));
-      }
-      // 2^ex brings am to [2^13, 2^14)
-      const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am) >> 23) - 127), -100), 100);
-      const float mul = pow2i(ex);
-#pragma unroll 1
-      for (int c = 0; c < 16; ++c) {
-        float f[8];
-        unpack8(*chunk(c), p.q_dt, f);
-        const float4 a = reinterpret_cast<const float4*>(ksm)[2 * c], b = reinterpret_cast<const float4*>(ksm)[2 * c + 1];
-        const float k8[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y0 = f[2 * e] * k8[2 * e] * mul, y1 = f[2 * e + 1] * k8[2 * e + 1] * mul;
-          hi[e] = pack_h2(y0, y1);
-          if constexpr (LO) {
-            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-            lo[e] = pack_h2(y0 - g.x, y1 - g.y);
-          }
-        }
-        *chunk(c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (LO) *(chunk(c) + kTileB / 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-      return pow2i(-ex);
+    // the chunks this thread forms of q' and of the output: ALT: half a row each
+    constexpr int kCh = ALT ? 8 : 16;
+    const int ch0 = ALT ? 8 * grp : 0;
+    // a barrier of the softmax warps whose wait is bounded, as all waits here are
+    uint32_t syncs = 0;
+    auto soft_sync = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(soft_bar);
+      ok = wait_bar(soft_bar, syncs++ & 1) && ok;
+      __syncwarp();
     };
     for (; ok && next_piece(walk, w); ++pc) {
       const int n_tiles = w.t1 - w.t0;
@@ -544,148 +514,225 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       const bool live = r < w.rows;
       const int u = (w.row0 + r) / p.nrep, h = w.kvh * p.nrep + (w.row0 + r) - u * p.nrep;
       if (n_tiles > 0) {
-        // the piece's K scales (every softmax thread takes part in both barriers)
-        asm volatile("bar.sync 1, %0;" ::"n"(C::kSoft) : "memory");
-        if (tid < kD)
-          ksm[tid] = load_scale(s.ksc, w.b * s.kscb + w.kvh * s.ksch + tid * s.kscd, p.s_dt) * p.qk_scale;
-        asm volatile("bar.sync 1, %0;" ::"n"(C::kSoft) : "memory");
-        q_off = 2 * (w.b * s.qsb + u * s.qsu + h * p.qsh);
-        if (live) fac = make_q();
+        // ---- q' of the row, in place in the Q tile.  (The tile is free: every S of the piece
+        // before has been seen; the barrier ends its use for the output.)
+        float am = 0.0f;
+        {
+          const uint4* src = reinterpret_cast<const uint4*>(
+              static_cast<const char*>(p.q) + 2 * (w.b * s.qsb + u * s.qsu + h * p.qsh)) + ch0;
+          uint4 x[kCh];
+#pragma unroll
+          for (int c = 0; c < kCh; ++c) x[c] = live ? src[c] : make_uint4(0, 0, 0, 0);
+          float ks = 0.0f;
+          if (tid < kD)
+            ks = load_scale(s.ksc, w.b * s.kscb + w.kvh * s.ksch + tid * s.kscd, p.s_dt) * p.qk_scale;
+          uint32_t a = 0;
+#pragma unroll
+          for (int c = 0; c < kCh; ++c)
+            a = p.q_dt == HQ_DTYPE_BF16
+                    ? absmax_x2<HQ_DTYPE_BF16>(a, absmax_x2<HQ_DTYPE_BF16>(absmax_x2<HQ_DTYPE_BF16>(x[c].x, x[c].y),
+                                                                           absmax_x2<HQ_DTYPE_BF16>(x[c].z, x[c].w)))
+                    : absmax_x2<HQ_DTYPE_F16>(a, absmax_x2<HQ_DTYPE_F16>(absmax_x2<HQ_DTYPE_F16>(x[c].x, x[c].y),
+                                                                         absmax_x2<HQ_DTYPE_F16>(x[c].z, x[c].w)));
+          am = p.q_dt == HQ_DTYPE_BF16 ? absmax_of_x2<HQ_DTYPE_BF16>(a) : absmax_of_x2<HQ_DTYPE_F16>(a);
+          soft_sync();
+#pragma unroll
+          for (int c = 0; c < kCh; ++c) *chunk(ch0 + c) = x[c];
+          if (tid < kD) ksm[tid] = ks;
+          if (ALT) rowb[tid].x = am;
+        }
+        soft_sync();
+        if (ALT) am = fmaxf(rowb[lr].x, rowb[kBN + lr].x);
+        if (p.q_quant) {
+          if (live && (!ALT || grp == 0)) fake_quant_row(q_tile, lr, p.q_dt);
+          soft_sync();
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        // 2^ex brings the bound max |q| max k_scale to [2^13, 2^14): the row's largest |q'| may
+        // lie some powers of two below, of which float16 has 14 to spare
+        const float4 k4 = reinterpret_cast<const float4*>(ksm)[lane];
+        float km = fmaxf(fmaxf(fabsf(k4.x), fabsf(k4.y)), fmaxf(fabsf(k4.z), fabsf(k4.w)));
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
+        const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am * km) >> 23) - 127), -100), 100);
+        const float mul = pow2i(ex);
+        fac = pow2i(-ex);
+        if (live) {
+#pragma unroll 1
+          for (int c = ch0; c < ch0 + kCh; ++c) {
+            float f[8];
+            unpack8(*chunk(c), p.q_dt, f);
+            const float4 a = reinterpret_cast<const float4*>(ksm)[2 * c], b = reinterpret_cast<const float4*>(ksm)[2 * c + 1];
+            const float k8[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y0 = f[2 * e] * k8[2 * e] * mul, y1 = f[2 * e + 1] * k8[2 * e + 1] * mul;
+              hi[e] = pack_h2(y0, y1);
+              if constexpr (LO) {
+                const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+                lo[e] = pack_h2(y0 - g.x, y1 - g.y);
+              }
+            }
+            *chunk(c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (LO) *(chunk(c) + kTileB / 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+        }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
-        // two row tiles keep step from piece to piece: a tile without rows must not arrive for
-        // the next piece in this one's phase, nor look at a tile two ahead of the other's
-        if (NM > 1) ok = wait_bar(q_full, pc & 1, abort);
+        // the groups keep step from piece to piece: one without tiles must not arrive for the
+        // next piece in this one's phase, nor look at a tile two ahead of the other's
+        ok = wait_bar(q_full, pc & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
-      if (w.rows <= 128 * mt) {         // nothing for this row tile
-        gt += n_tiles;
-        continue;
-      }
-      const bool warp_live = 32 * warp < w.rows;
+      const int wr0 = 32 * (ALT ? warp & 3 : warp);        // the warp's first row
+      const bool warp_live = wr0 < w.rows;
+      const bool mine = ALT || w.rows > 128 * grp;          // this group has rows
       const int pos = w.key.pos0 + (s.step ? u : 0);
       const RowLim lim = {live ? pos - w.key.sh : 1 << 30,
                           live ? pos - s.window + 1 - w.key.sh : 0,
                           w.key.sh > 0 ? w.key.ns : s.sinks};
-      for (int t = w.t0; ok && t < w.t1; ++t, ++gt, ++cnt) {
-        const int buf = NM == 1 ? (cnt & 1) : mt;
-        const uint32_t par = NM == 1 ? ((cnt >> 1) & 1) : (cnt & 1);
-        const int slot = gt % kLvSlots;
-        ok = wait_bar(&lv_full[slot], (gt / kLvSlots) & 1, abort) &&
-             wait_bar(&s_full[buf], par, abort);
+      const int tf = w.t0 + (ALT ? grp : 0);                // this group's first tile
+      for (int t = tf; ok && mine && t < w.t1; t += ALT ? 2 : 1, ++cnt) {
+        const int gt = gt0 + t - w.t0, slot = gt % kLvSlots;
+        ok = wait_bar(&lv_full[slot], (gt / kLvSlots) & 1) &&
+             wait_bar(&s_full[grp], cnt & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
           const float* ev = eb + slot * 2 * kBN;
-          const uint32_t s_addr = tmem + 128 * buf + lane_base;
           const int v0 = t * kBN;
           const float2 ti = info[slot];
-          if (t == w.t0) vscale = ti.y;
+          vscale = ti.y;
           const bool need = v0 + kBN - 1 > lim.hi || (v0 < lim.lo && v0 + kBN > lim.vsk && lim.lo > lim.vsk);
           const bool mask = __any_sync(0xffffffffu, need);
-          if (!mask && (LO || ti.x == 0.0f))
-            softmax_tile<LO>(s_addr, o_addr, ev, fac, t == w.t0, &pv_done[mt], cnt, abort, m, l, ok);
+          if ((!LO && ti.x != 0.0f) || (LO && mask))
+            softmax_tile_any(s_addr, o_addr, ev, fac, v0, lim, t == tf, &pv_done[grp], cnt, m, l, ok);
+          else if (LO || !mask)
+            softmax_tile<LO, false>(s_addr, o_addr, ev, fac, v0, lim, t == tf, &pv_done[grp], cnt, m, l, ok);
           else
-            softmax_tile_any(s_addr, o_addr, ev, fac, v0, lim, t == w.t0, &pv_done[mt], cnt, abort,
-                             m, l, ok);
+            softmax_tile<false, true>(s_addr, o_addr, ev, fac, v0, lim, t == tf, &pv_done[grp], cnt, m, l, ok);
         } else if (cnt > 0) {
-          ok = wait_bar(&pv_done[mt], (cnt - 1) & 1, abort);
+          ok = wait_bar(&pv_done[grp], (cnt - 1) & 1);
           ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok) break;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[buf]);
+        if (lane == 0) mbar_arrive(&p_ready[grp]);
       }
       if (!ok) break;
+      gt0 += n_tiles;
       // ---- the rows' results
-      if (n_tiles > 0) {
-        ok = wait_bar(&pv_done[mt], (cnt - 1) & 1, abort);
+      const int my_tiles = !mine ? 0 : ALT ? (n_tiles + 1 - grp) / 2 : n_tiles;
+      if (my_tiles > 0) {
+        ok = wait_bar(&pv_done[grp], (cnt - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         tc_fence_after();
       }
-      if (warp_live) {
-        // (rows that saw nothing have l = 0 and give zeros, whatever their O holds; a NaN stays)
-        const bool have = live && !(l <= 0.0f) && n_tiles > 0;
-        if (w.slot < 0) {
-          // the row into the Q tile, then the warp's rows out, 256 bytes at a time
-          const float scale = have ? vscale / l : 0.0f;
+      // (rows that saw nothing have l = 0 and give zeros, whatever their O holds; a NaN stays)
+      bool has0 = my_tiles > 0 && !(l <= 0.0f), has1 = false;
+      float f0 = 1.0f, f1 = 0.0f;
+      if constexpr (ALT) {  // both groups' states; each thread then takes half of the columns
+        rowb[tid] = make_float2(m, l);
+        if (tid == 0) *two_e = vscale;
+        tc_fence_before();
+        soft_sync();
+        tc_fence_after();
+        const float2 a = rowb[lr], b = rowb[kBN + lr];
+        has0 = n_tiles > 0 && !(a.y <= 0.0f);
+        has1 = n_tiles > 1 && !(b.y <= 0.0f);
+        m = fmaxf(a.x, b.x);
+        f0 = a.x == -INFINITY ? 0.0f : ex2_ftz(a.x - m);
+        f1 = b.x == -INFINITY ? 0.0f : ex2_ftz(b.x - m);
+        l = a.y * f0 + b.y * f1;
+        vscale = *two_e;
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const bool have = live && (has0 || has1);
+      const uint32_t o0 = ALT ? tmem + kColO + lane_base : o_addr, o1 = tmem + kColO + 128 + lane_base;
+      if (warp_live && mine) {
+        const float scale = w.slot < 0 ? (have ? vscale / l : 0.0f) : vscale;
+        f0 = has0 ? f0 * scale : 0.0f;
+        f1 = has1 ? f1 * scale : 0.0f;
+        float* prt = part_row(p, w.slot < 0 ? 0 : w.slot, r);
+        if (w.slot >= 0 && live && (!ALT || grp == 0))
+          *reinterpret_cast<float2*>(prt) = make_float2(have ? m : -INFINITY, have ? l : 0.0f);
 #pragma unroll 1
-          for (int c = 0; c < 16; c += 2) {
-            uint32_t o[16], y[8];
-            tmem_ld16(o_addr + 8 * c, o);
+        for (int c = ch0; c < ch0 + kCh; c += 2) {
+          uint32_t o[16];
+          float y[16];
+          tmem_ld16(o0 + 8 * c, o);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float a = __uint_as_float(o[2 * e]) * scale, b2 = __uint_as_float(o[2 * e + 1]) * scale;
-              y[e] = have ? pack_pair(a, b2, p.q_dt) : 0u;
-            }
-            *chunk(c) = make_uint4(y[0], y[1], y[2], y[3]);
-            *chunk(c + 1) = make_uint4(y[4], y[5], y[6], y[7]);
+          for (int e = 0; e < 16; ++e) y[e] = has0 ? __uint_as_float(o[e]) * f0 : 0.0f;
+          if constexpr (ALT) {
+            tmem_ld16(o1 + 8 * c, o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] += has1 ? __uint_as_float(o[e]) * f1 : 0.0f;
           }
-          __syncwarp();
-          const uint64_t dst = reinterpret_cast<uint64_t>(out_row(p, w.b, u, h));
-          const int n_rows = min(32, w.rows - 32 * warp);
-#pragma unroll 1
-          for (int i = 0; i < n_rows; ++i) {
-            char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, dst, i));
-            const int c = lane >> 1;
-            const unsigned char* from = q_tile + (c >> 3) * (kBN * 128) +
-                                        sw128((32 * warp + i) & 127, c & 7) + 8 * (lane & 1);
-            *reinterpret_cast<uint2*>(to + 8 * lane) = *reinterpret_cast<const uint2*>(from);
-          }
-          __syncwarp();
-        } else {
-          float* prt = part_row(p, w.slot, r);
-          if (live) *reinterpret_cast<float2*>(prt) = make_float2(have ? m : -INFINITY, have ? l : 0.0f);
-#pragma unroll 1
-          for (int c = 0; c < 128; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(o_addr + c, o);
-            if (!live) continue;
+          if (w.slot < 0) {  // into the Q tile
+            uint32_t z[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = pack_pair(y[2 * e], y[2 * e + 1], p.q_dt);
+            *chunk(c) = make_uint4(z[0], z[1], z[2], z[3]);
+            *chunk(c + 1) = make_uint4(z[4], z[5], z[6], z[7]);
+          } else if (live) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(prt + 4 + c + e) =
-                  have ? make_float4(__uint_as_float(o[e]) * vscale, __uint_as_float(o[e + 1]) * vscale,
-                                     __uint_as_float(o[e + 2]) * vscale, __uint_as_float(o[e + 3]) * vscale)
-                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              *reinterpret_cast<float4*>(prt + 4 + 8 * c + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
           }
         }
       }
       if (n_tiles > 0) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&o_empty[mt]);
+        if (lane == 0) mbar_arrive(o_empty);
+      }
+      if (w.slot < 0) {  // the warp's rows out, 256 bytes at a time
+        if (ALT) soft_sync(); else __syncwarp();
+        const uint64_t dst = reinterpret_cast<uint64_t>(out_row(p, w.b, u, h));
+        const int i0 = ALT ? 16 * grp : 0, i1 = min(ALT ? i0 + 16 : 32, w.rows - wr0);
+#pragma unroll 2
+        for (int i = i0; i < i1; ++i) {
+          char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, dst, i));
+          const int c = lane >> 1;
+          const unsigned char* from = q_tile + (c >> 3) * (kBN * 128) +
+                                      sw128((wr0 + i) & 127, c & 7) + 8 * (lane & 1);
+          *reinterpret_cast<uint2*>(to + 8 * lane) = *reinterpret_cast<const uint2*>(from);
+        }
       }
     }
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
   } else if (warp < kMmaWarp) {
     // ================= staged codes -> float16 tiles
-    const int ct = tid - C::kSoft;
-    // 8 codes (one 16-byte chunk) of rows row + 8 i of a slot: 8 lanes store 8 different chunk
-    // columns, and rows 8 apart have the same swizzle
+    const int ct = tid - kSoft;
+    // 8 codes (one 16-byte chunk) of rows row + 16 i of a slot: 8 lanes store 8 different chunk
+    // columns, and rows 16 apart have the same swizzle
     const int c8 = ct & 15, row = ct >> 4;
     const uint32_t at = static_cast<uint32_t>(c8 >> 3) * (kBN * 128) + sw128(row, c8 & 7);
-    int sc = 0, gt = 0;  // slots, tiles
+    int sl = 0, gt = 0;  // slot, tiles
+    uint32_t sl_par = 0;
     bool ok = true;
     // the next staging slot into rows 64 half .. of a tile; V rows times their g
     auto convert = [&](unsigned char* tile, auto is_v, const uint32_t* g) {
-      const int sl = sc % C::kSlots;
-      ok = wait_bar(&st_full[sl], (sc / C::kSlots) & 1, abort);
+      ok = wait_bar(&st_full[sl], sl_par);
       if (!ok) return;
       const unsigned char* src = smem + C::kOffSlot + sl * kSlotB + row * kD + 8 * c8;
-      uint2 x[8];
-      uint32_t g2[8];
+      constexpr int NI = kSlotKeys / (kConvThreads / 16);
+      uint2 x[NI];
+      uint32_t g2[NI];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = *reinterpret_cast<const uint2*>(src + i * 8 * kD);
-        if constexpr (is_v.value) g2[i] = g[row + 8 * i];
+      for (int i = 0; i < NI; ++i) {
+        x[i] = *reinterpret_cast<const uint2*>(src + i * 16 * kD);
+        if constexpr (is_v.value) g2[i] = g[row + 16 * i];
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < NI; ++i) {
         uint4 y;
         codes_to_h2(x[i].x, y.x, y.y);
         codes_to_h2(x[i].y, y.z, y.w);
@@ -695,16 +742,19 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
           asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.z) : "r"(y.z), "r"(g2[i]));
           asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.w) : "r"(y.w), "r"(g2[i]));
         }
-        *reinterpret_cast<uint4*>(tile + at + i * 1024) = y;
+        *reinterpret_cast<uint4*>(tile + at + i * 2048) = y;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&st_empty[sl]);
-      ++sc;
+      if (++sl == C::kSlots) {
+        sl = 0;
+        sl_par ^= 1;
+      }
     };
     for (; ok && next_piece(walk, w);) {
       for (int t = w.t0; t < w.t1; ++t, ++gt) {
         const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
-        if (use > 0) ok = wait_bar(&k_empty[st], (use - 1) & 1, abort);
+        if (use > 0) ok = wait_bar(&k_empty[st], (use - 1) & 1);
         if (!ok) break;
 #pragma unroll 1
         for (int half = 0; half < 2 && ok; ++half)
@@ -713,8 +763,8 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[st]);
-        if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1, abort);
-        ok = ok && wait_bar(&lv_full[slot], (gt / kLvSlots) & 1, abort);
+        if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1);
+        ok = ok && wait_bar(&lv_full[slot], (gt / kLvSlots) & 1);
         if (!ok) break;
 #pragma unroll 1
         for (int half = 0; half < 2 && ok; ++half)
@@ -737,7 +787,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
 #pragma unroll 1
       for (int t2 = 4 * w.t0; ok && t2 < 4 * w.t1; ++t2, ++sc) {  // K 0 .., K 64 .., V 0 .., V 64 ..
         const int sl = sc % C::kSlots, use = sc / C::kSlots;
-        if (use > 0) ok = wait_bar(&st_empty[sl], (use - 1) & 1, abort);
+        if (use > 0) ok = wait_bar(&st_empty[sl], (use - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const int v0 = (t2 >> 2) * kBN + (t2 & 1) * kSlotKeys;
@@ -801,7 +851,7 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       have = load_next();
       // slot gt % kLvSlots is free once P V of the tile two before is done
       const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
-      if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1, abort);
+      if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       float* ev = eb + slot * 2 * kBN;
@@ -858,13 +908,11 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       constexpr uint32_t id_s = idesc<HQ_DTYPE_F16>(128, 128, false);
       constexpr uint32_t id_o = idesc<HQ_DTYPE_F16>(128, 128, true);
       bool ok = true;
-      int cntq[NM], cntp[NM], pieces[NM];  // S products, P V products, pieces of each row tile
-      for (int i = 0; i < NM; ++i) cntq[i] = cntp[i] = pieces[i] = 0;
-      // S = Q K^T of tile g for row tile m
+      int cntp[2] = {0, 0}, pieces = 0;  // P V products of each group, pieces
+      // S = Q K^T of tile g for group m
       auto qk = [&](int m, int g) {
-        const uint32_t buf = NM == 1 ? (cntq[m] & 1) : m;
         const uint64_t dk = sdesc(k_base + (g % kStages) * kTileB, 16, 1024);
-        const uint64_t dq = sdesc(q_base + m * C::kParts * kTileB, 16, 1024);
+        const uint64_t dq = sdesc(q_base + (ALT ? 0 : m) * C::kParts * kTileB, 16, 1024);
         if (lead) {
 #pragma unroll
           for (int part = 0; part < C::kParts; ++part)
@@ -872,19 +920,14 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
             for (int kk = 0; kk < 8; ++kk) {
               // (the address field counts 16 bytes; no sum leaves its 14 bits)
               const uint32_t off = ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) >> 4;
-              mma_f16(tmem + 128 * buf, dq + (part * (kTileB >> 4) + off), dk + off, id_s,
-                      part + kk > 0);
+              mma_f16(tmem + 128 * m, dq + (part * (kTileB >> 4) + off), dk + off, id_s, part + kk > 0);
             }
-          mma_commit(&s_full[buf]);
+          mma_commit(&s_full[m]);
         }
         __syncwarp();
-        ++cntq[m];
       };
       auto pv = [&](int m, int g, bool first) {
-        const uint32_t buf = NM == 1 ? (cntp[m] & 1) : m;
-        const uint32_t par = NM == 1 ? ((cntp[m] >> 1) & 1) : (cntp[m] & 1);
-        ok = ok && wait_bar(&p_ready[buf], par, abort);
-        if (first && pieces[m] > 0) ok = ok && wait_bar(&o_empty[m], (pieces[m] - 1) & 1, abort);
+        ok = ok && wait_bar(&p_ready[m], (m ? cntp[1] : cntp[0]) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
         tc_fence_after();
@@ -892,13 +935,12 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         if (lead) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            mma_f16_ts(tmem + kColO + 128 * m, tmem + 128 * buf + 8 * kk, dv + (kk * 16 * 128 >> 4),
+            mma_f16_ts(tmem + kColO + 128 * m, tmem + 128 * m + 8 * kk, dv + (kk * 16 * 128 >> 4),
                        id_o, !first || kk > 0);
           mma_commit(&pv_done[m]);
         }
         __syncwarp();
-        ++cntp[m];
-        if (first) ++pieces[m];
+        if (m) ++cntp[1]; else ++cntp[0];
       };
       // cursor of the S products, one tile ahead of the P V products
       Walk qw = walk;
@@ -920,8 +962,8 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         fresh = true;
       };
       auto q_wait = [&]() {  // its q (of a piece's first tile) and K
-        if (fresh) ok = ok && wait_bar(q_full, qpc & 1, abort);
-        ok = ok && wait_bar(&k_full[qg % kStages], (qg / kStages) & 1, abort);
+        if (fresh) ok = ok && wait_bar(q_full, qpc & 1);
+        ok = ok && wait_bar(&k_full[qg % kStages], (qg / kStages) & 1);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       };
@@ -932,8 +974,13 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
       auto q_all = [&]() {
         q_wait();
         if (!ok) return;
-        for (int m = 0; m < NM; ++m)
-          if (qp.rows > 128 * m) qk(m, qg);
+        if constexpr (ALT) {
+          qk((qt - qp.t0) & 1, qg);
+        } else {
+#pragma unroll 1
+          for (int m = 0; m < 2; ++m)
+            if (qp.rows > 128 * m) qk(m, qg);
+        }
         q_done();
       };
       qt = -1;
@@ -944,26 +991,33 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
         cp = qp;
         const int ctile = qt;
         q_next();
-        // within a piece the next S goes out ahead of (one row tile) or between (two) the P V
-        // products; a piece's first S comes after them, since its q is made by the warps that
-        // wait for the last P V of the piece before
+        // within a piece the next S goes out ahead of (ALT: it is the other group's) or between
+        // (two row tiles) the P V products; a piece's first S comes after them, since its q is
+        // made by the warps that wait for the last P V of the piece before
         const bool ahead = more && !fresh;
-        if (ahead && NM == 1) q_all();
-        if (ahead && NM > 1) q_wait();
-        ok = ok && wait_bar(&v_full[g % kStages], (g / kStages) & 1, abort);
+        if (ahead && ALT) q_all();
+        if (ahead && !ALT) q_wait();
+        ok = ok && wait_bar(&v_full[g % kStages], (g / kStages) & 1);
+        if (ctile == cp.t0) {
+          if (pieces > 0) ok = ok && wait_bar(o_empty, (pieces - 1) & 1);
+          ++pieces;
+        }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        for (int m = 0; m < NM; ++m) {
-          if (cp.rows > 128 * m) {
-            pv(m, g, ctile == cp.t0);
-            if (!ok) break;
-            // the next S of this row tile overwrites the P just read: the products run in order
-            if (NM > 1 && ahead) qk(m, qg);
-          }
+        if constexpr (ALT) {
+          pv((ctile - cp.t0) & 1, g, ctile - cp.t0 < 2);
+        } else {
+#pragma unroll 1
+          for (int m = 0; m < 2 && ok; ++m)
+            if (cp.rows > 128 * m) {
+              pv(m, g, ctile == cp.t0);
+              // the next S of this row tile overwrites the P just read: the products run in order
+              if (ok && ahead) qk(m, qg);
+            }
         }
         if (!ok) break;
         if (lead) mma_commit(&v_empty[g % kStages]);
-        if (NM > 1 && ahead) q_done();
+        if (!ALT && ahead) q_done();
         if (more && fresh) q_all();
         ++g;
       }
@@ -987,11 +1041,11 @@ __global__ void __launch_bounds__(Cfg<NM, LO>::kThreads, 1) ragged_kernel(const 
 }
 
 // ---------------------------------------------------------------- launches
-template <int NM, bool LO, bool STREAM>
+template <bool ALT, bool LO, bool STREAM>
 int launch(const Params& p, dim3 grid, cudaStream_t st) {
-  using C = Cfg<NM, LO>;
+  using C = Cfg<ALT, LO>;
   static std::atomic<uint64_t> ready{0};
-  auto kern = ragged_kernel<NM, LO, STREAM>;
+  auto kern = ragged_kernel<ALT, LO, STREAM>;
   const int rc = set_smem(kern, C::smem(STREAM ? kMaxEntries : 0), ready);
   if (rc != HQ_OK) return rc;
   return launch_after(kern, grid, C::kThreads, C::smem(STREAM ? p.seg.nb : 0), st, p);
@@ -999,9 +1053,9 @@ int launch(const Params& p, dim3 grid, cudaStream_t st) {
 
 template <bool STREAM>
 int dispatch(const Params& p, int nm, dim3 grid, cudaStream_t st) {
-  if (p.q_dt == HQ_DTYPE_F16) return launch<1, true, STREAM>(p, grid, st);
-  if (nm == 1) return launch<1, false, STREAM>(p, grid, st);
-  return launch<2, false, STREAM>(p, grid, st);
+  if (p.q_dt == HQ_DTYPE_F16) return launch<true, true, STREAM>(p, grid, st);
+  if (nm == 1) return launch<true, false, STREAM>(p, grid, st);
+  return launch<false, false, STREAM>(p, grid, st);
 }
 
 int tiles_stream(const Params& p, int nm, int grid, cudaStream_t st) {

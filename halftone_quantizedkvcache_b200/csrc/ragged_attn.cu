@@ -19,8 +19,7 @@
 // and o = 2^E O / l for V scales of any size.  A tile whose V scales lie within 2^-4 .. 2^6
 // of 2^E (nearly every one) has all e_j = 0, and costs nothing for them; the others look
 // e_j up.  Float16 models always put the whole scale into e_j (not a whole number then), so
-// that V stays exact.  m moves only when t grows by more than 8 (P <= 256, far inside
-// float16), so O in tensor memory is rarely rescaled.  Roundings to float16, each off by
+// that V stays exact.  m moves only when t grows by more than 14 (P <= 2^14), so O in tensor memory is rarely rescaled.  Roundings to float16, each off by
 // 2^-11 of itself at most: q' (bf16 models), P, and for bf16 models g_j and code g_j, an
 // eighth of the output's own half step.
 //
@@ -54,36 +53,36 @@ using namespace tc;
 
 constexpr int kSoft = 256;                // softmax threads: two groups of 128
 constexpr int kConvThreads = 256;
+constexpr int kBS = 64;                   // keys of a softmax step: half a tile
 constexpr int kTileB = kBN * kD * 2;      // a float16 K, V or Q tile: 32 KB
 constexpr int kStages = 2;                // K and V tiles in shared memory
 constexpr int kSlotKeys = 64;             // keys of a staging slot (K or V codes)
 constexpr int kSlotB = kSlotKeys * kD;
-constexpr int kLvSlots = 2;               // ring of what the tiles' V scales lead to
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 256;           // S buffers at columns 0 and 128
 
 template <bool ALT, bool LO>
 struct Cfg {
-  static constexpr int kThreads = kSoft + kConvThreads + 96;
+  static constexpr int kThreads = kSoft + kConvThreads + 128;
   static constexpr int kRowTiles = ALT ? 1 : 2;
   static constexpr int kParts = LO ? 2 : 1;
-  static constexpr int kSlots = kRowTiles * kParts == 1 ? 7 : 3;   // staging: 8 KB each
+  static constexpr int kSlots = kRowTiles * kParts == 1 ? 6 : 3;   // staging: 8 KB each
+  static constexpr int kLvSlots = LO ? 2 : 3;  // ring of what the tiles' V scales lead to
   static constexpr int kOffK = kRowTiles * kParts * kTileB;
   static constexpr int kOffV = kOffK + kStages * kTileB;
   static constexpr int kOffSlot = kOffV + kStages * kTileB;
   static constexpr int kOffE = kOffSlot + kSlots * kSlotB;         // [slot][e_j, 2^-e_j][128]
   static constexpr int kOffG = kOffE + kLvSlots * 2 * kBN * 4;     // [slot][128] g_j, float16 twice
   static constexpr int kOffInfo = kOffG + kLvSlots * kBN * 4;      // [slot]{any e_j, 2^E}
-  static constexpr int kOffKs = kOffInfo + kLvSlots * 8;           // [128] k_scale sm_scale log2 e
-  // [2][128] float2: a row's halves' largest |q|; later the groups' (m, l)
-  static constexpr int kOffRow = kOffKs + kD * 4;
+  static constexpr int kOffFac = kOffInfo + 16 * ((kLvSlots + 1) / 2);  // [row] what q' was divided by
+  static constexpr int kOffRow = kOffFac + kRowTiles * 128 * 4;     // ALT: [2][128] the groups' (m, l)
   static constexpr int kOffBar = kOffRow + (ALT ? 2 * kBN * 8 : 0);
-  static constexpr int kBars = 1 + 4 * kStages + 2 * kSlots + kLvSlots + 2 + 2 + 2 + 1 + 1 + 1;
+  static constexpr int kBars = 1 + 4 * kStages + 2 * kSlots + 2 * kLvSlots + 4 + 4 + 4 + 1 + 1 + 1;
   static constexpr int kOffMisc = kOffBar + ((kBars * 8 + 15) & ~15);
   static constexpr int kOffCum = kOffMisc + 16;
+  static_assert(kOffFac % 16 == 0 && kOffRow % 16 == 0 && kOffBar % 8 == 0, "vector accesses");
   static constexpr int smem(int entries) { return 1024 + kOffCum + 4 * (entries + 1); }
   static_assert(1024 + kOffCum + 4 * (kMaxEntries + 1) <= 232448, "one block per SM");
-  static_assert(kLvSlots == kStages, "a slot is free with its V stage");
 };
 
 // ---------------------------------------------------------------- small helpers
@@ -119,12 +118,31 @@ __device__ __forceinline__ bool elect_one() {  // one lane of a converged warp
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
   return e != 0;
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db,
-                                           uint32_t id, uint32_t accumulate) {
+// tcgen05.mma by the lane whose `lead` is set.  The whole warp runs the code around it, and a
+// descriptor comes as its low word and a constant high word: so all operands stay in uniform
+// registers (under a branch each product took six moves into them, 80 cycles).
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint32_t a_lo, uint32_t a_hi,
+                                       uint32_t b_lo, uint32_t b_hi, uint32_t id, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(db), "r"(id), "r"(accumulate));
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %7, 0;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %6, p;\n\t}\n" ::"r"(lead),
+      "r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b_lo,
+                                       uint32_t b_hi, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], b, %5, p;\n\t}\n" ::"r"(lead),
+      "r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}\n" ::"r"(lead),
+      "r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
@@ -134,22 +152,28 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-// 16 columns of this thread's lane, loaded by tmem_get and valid after tmem_got (which
-// awaits every load issued before it; the registers pass through it, so no use moves up)
-__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[16]) {
+// 32 columns of this thread's lane, valid after tmem_got (which awaits every load issued before
+// it; the registers pass through it, so no use moves up)
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15}, [%16];"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+      "%29, %30, %31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_got(uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_got(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
                  "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]));
+  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
 }
 // Bounded wait: some seconds, then false.  One opaque loop: as C++ with its convergence
 // instructions the waits took a third of all issue slots.
@@ -167,42 +191,21 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-__device__ __forceinline__ void unpack8(const uint4& x, int dt, float (&f)[8]) {
-  if (dt == HQ_DTYPE_BF16) Vec16<HQ_DTYPE_BF16>::unpack(x, f);
-  else Vec16<HQ_DTYPE_F16>::unpack(x, f);
-}
-// Per-token int8 fake quantization of row r of a Q tile, rounded back to the model dtype.
-__device__ __noinline__ void fake_quant_row(unsigned char* tile, int r, int dt) {
-  auto chunk = [&](int c) {
-    return reinterpret_cast<uint4*>(tile + (c >> 3) * (kBN * 128) + sw128(r, c & 7));
-  };
-  float am = 0.0f;
-#pragma unroll 1
-  for (int c = 0; c < 16; ++c) {
-    float f[8];
-    unpack8(*chunk(c), dt, f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(f[e]));
-  }
+// Per-token int8 fake quantization of 8 values of a row with the largest |value| am, rounded back
+// to the model dtype.
+template <int DT>
+__device__ __noinline__ uint4 fake_quant(uint4 x, float am) {
   const Quantizer qz = Quantizer::from_amax(am);
-#pragma unroll 1
-  for (int c = 0; c < 16; ++c) {
-    float f[8];
-    unpack8(*chunk(c), dt, f);
-    uint32_t w[4];
+  float f[8];
+  Vec16<DT>::unpack(x, f);
+  uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float a = static_cast<float>(qz.code(f[2 * e])) * qz.scale;
-      const float b = static_cast<float>(qz.code(f[2 * e + 1])) * qz.scale;
-      if (dt == HQ_DTYPE_BF16) {
-        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
-        w[e] = *reinterpret_cast<const uint32_t*>(&x);
-      } else {
-        w[e] = pack_h2(a, b);
-      }
-    }
-    *chunk(c) = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int e = 0; e < 4; ++e) {
+    const float a = static_cast<float>(qz.code(f[2 * e])) * qz.scale;
+    const float b = static_cast<float>(qz.code(f[2 * e + 1])) * qz.scale;
+    w[e] = pack_pair(a, b, DT);
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---------------------------------------------------------------- softmax of one row tile
@@ -221,6 +224,9 @@ struct RowLim {
 // costs about 10 cycles each, and the SM's schedulers hold some 12 KB each.  So the loops below
 // stay rolled as far as registers allow, and what is rare is a call.
 
+// t may exceed the running maximum by this: P <= 2^14, 2^16 is float16's end, and what float16
+// rounds away of the smallest P (2^-25) is nothing beside the row's largest, 1 at least
+constexpr float kSlack = 14.0f;
 // O *= a
 __device__ __noinline__ void rescale(uint32_t o_addr, float a) {
 #pragma unroll 1
@@ -232,100 +238,81 @@ __device__ __noinline__ void rescale(uint32_t o_addr, float a) {
     tmem_st16(o_addr + 16 * c, o);
   }
 }
-// The running maximum takes this tile's largest t in, O and l are rescaled where it moves;
-// waits for the previous P V on the way.
+// The running maximum takes this step's largest t in, O and l are rescaled where it moves.
+// pv_bar: the barrier of the step before, whose P V must be in O by then.  (Two barriers in turn:
+// S of this step follows P V of the step before that one, so no wait that is skipped here can
+// leave a parity behind.)
 __device__ __forceinline__ void move_max(float mx, uint32_t o_addr, bool first, uint64_t* pv_bar,
-                                         int cnt, float& m, float& l, bool& ok) {
+                                         uint32_t pv_par, float& m, float& l, bool& ok) {
+  const bool move = mx > m + kSlack || (m == -INFINITY && mx != -INFINITY);
+  if (!__any_sync(0xffffffffu, move)) return;
   float a = 1.0f;
-  if (mx > m + 8.0f || (m == -INFINITY && mx != -INFINITY)) {
+  if (move) {
     a = ex2_ftz(m - mx);
     m = mx;
     l *= a;
   }
-  // The previous P V is in O.  Every tile waits here, whether it rescales or not: a wait by
-  // parity tells neighbouring completions apart, so none may be skipped.
-  if (cnt > 0) {
-    ok = wait_bar(pv_bar, (cnt - 1) & 1);
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) return;
-    tc_fence_after();
-  }
-  if (!first && __any_sync(0xffffffffu, a != 1.0f)) rescale(o_addr, a);
+  if (first) return;
+  ok = wait_bar(pv_bar, pv_par);
+  ok = __all_sync(0xffffffffu, ok);
+  if (!ok) return;
+  tc_fence_after();
+  rescale(o_addr, a);
 }
 
-// One tile of one row: the running maximum, then P = 2^(t - m) over S, and l.  EXP: t = s fac +
-// e_j with e_j from ev[j] and 2^-e_j from ev[128 + j], else t = s fac.  MASK: some row of the
-// warp does not see all of the tile.
-template <bool EXP, bool MASK>
-__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, const float* ev,
-                                             float fac, int v0, const RowLim& lim, bool first,
-                                             uint64_t* pv_bar, int cnt,
+// One step of one row, 64 keys held in registers: the running maximum, then P = 2^(t - m) over S,
+// and l.  EXP: t = s fac + e_j with e_j from ev[j] and 2^-e_j from ev[128 + j], else t = s fac.
+// mask: some row of the warp does not see all of the keys.
+template <bool EXP>
+__device__ __forceinline__ void softmax_step(uint32_t s_addr, uint32_t o_addr, const float* ev,
+                                             float fac, int v0, const RowLim& lim, bool mask,
+                                             bool first, uint64_t* pv_bar, uint32_t pv_par,
                                              float& m, float& l, bool& ok) {
-  uint32_t sa[16], sb[16];
-  float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  auto fold = [&](const uint32_t (&s)[16], int c) {
-    const uint32_t seen = MASK ? lim.bits(v0 + c) : 0xffffu;
+  uint32_t s[kBS];
+  tmem_get(s_addr, s);
+  tmem_get(s_addr + 32, s + 32);
+  tmem_got(s);
+  tmem_got(s + 32);
+  if constexpr (EXP) {
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      float t[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = __uint_as_float(s[e + i]);
-      if constexpr (EXP) {
-        const float4 e4 = *reinterpret_cast<const float4*>(ev + c + e);
-        t[0] = __fmaf_rn(t[0], fac, e4.x);
-        t[1] = __fmaf_rn(t[1], fac, e4.y);
-        t[2] = __fmaf_rn(t[2], fac, e4.z);
-        t[3] = __fmaf_rn(t[3], fac, e4.w);
-      }
-      if constexpr (MASK) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = seen & (1u << (e + i)) ? t[i] : -INFINITY;
-      }
-      const int k = (e >> 2) & 1;
-      x[2 * k] = fmaxf(x[2 * k], fmaxf(t[0], t[1]));
-      x[2 * k + 1] = fmaxf(x[2 * k + 1], fmaxf(t[2], t[3]));
+    for (int e = 0; e < kBS; e += 4) {
+      const float4 e4 = *reinterpret_cast<const float4*>(ev + e);
+      s[e] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e]), fac, e4.x));
+      s[e + 1] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e + 1]), fac, e4.y));
+      s[e + 2] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e + 2]), fac, e4.z));
+      s[e + 3] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e + 3]), fac, e4.w));
     }
-  };
-  tmem_get(s_addr, sa);
-#pragma unroll 1
-  for (int c = 0; c < 128; c += 32) {
-    tmem_got(sa);
-    tmem_get(s_addr + c + 16, sb);
-    fold(sa, c);
-    tmem_got(sb);
-    if (c < 96) tmem_get(s_addr + c + 32, sa);
-    fold(sb, c + 16);
   }
+  if (mask) {
+    const uint32_t seen0 = lim.bits(v0), seen1 = lim.bits(v0 + 32);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      s[e] = seen0 & (1u << e) ? s[e] : 0xff800000u;
+      s[e + 32] = seen1 & (1u << e) ? s[e + 32] : 0xff800000u;
+    }
+  }
+  float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int e = 0; e < kBS; e += 2)
+    x[(e >> 1) & 3] = fmaxf(x[(e >> 1) & 3], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
   float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
   if constexpr (!EXP) mx *= fac;
-  tmem_get(s_addr, sa);
-  move_max(mx, o_addr, first, pv_bar, cnt, m, l, ok);
+  move_max(mx, o_addr, first, pv_bar, pv_par, m, l, ok);
   if (!ok) return;
   const float nb = m == -INFINITY ? 0.0f : -m;
   // (scalar: packed pairs cost more moves than they save)
   float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  // P of keys c .. goes over S columns c / 2 .., which have been read by then
-  auto emit = [&](const uint32_t (&s)[16], int c) {
-    const uint32_t seen = MASK ? lim.bits(v0 + c) : 0xffffu;
+#pragma unroll
+  for (int c = 0; c < kBS; c += 16) {
     uint32_t w[8];
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
+    for (int e = c; e < c + 16; e += 4) {
       float t[4];
-      float en[4] = {nb, nb, nb, nb};
-      if constexpr (EXP) {
-        const float4 e4 = *reinterpret_cast<const float4*>(ev + c + e);
-        en[0] += e4.x;
-        en[1] += e4.y;
-        en[2] += e4.z;
-        en[3] += e4.w;
-      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        t[i] = ex2_ftz(__fmaf_rn(__uint_as_float(s[e + i]), fac, en[i]));
-        if constexpr (MASK) t[i] = seen & (1u << (e + i)) ? t[i] : 0.0f;
-      }
+      for (int i = 0; i < 4; ++i)
+        t[i] = ex2_ftz(EXP ? __uint_as_float(s[e + i]) + nb : __fmaf_rn(__uint_as_float(s[e + i]), fac, nb));
       if constexpr (EXP) {
-        const float4 r4 = *reinterpret_cast<const float4*>(ev + kBN + c + e);
+        const float4 r4 = *reinterpret_cast<const float4*>(ev + kBN + e);
         ls[0] = __fmaf_rn(t[0], r4.x, ls[0]);
         ls[1] = __fmaf_rn(t[1], r4.y, ls[1]);
         ls[2] = __fmaf_rn(t[2], r4.z, ls[2]);
@@ -334,33 +321,23 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, c
 #pragma unroll
         for (int i = 0; i < 4; ++i) ls[i] += t[i];
       }
-      w[e / 2] = pack_h2(t[0], t[1]);
-      w[e / 2 + 1] = pack_h2(t[2], t[3]);
+      w[(e - c) / 2] = pack_h2(t[0], t[1]);
+      w[(e - c) / 2 + 1] = pack_h2(t[2], t[3]);
     }
     tmem_st8(s_addr + c / 2, w);
-  };
-#pragma unroll 1
-  for (int c = 0; c < 128; c += 32) {
-    tmem_got(sa);
-    tmem_get(s_addr + c + 16, sb);
-    emit(sa, c);
-    tmem_got(sb);
-    if (c < 96) tmem_get(s_addr + c + 32, sa);
-    emit(sb, c + 16);
   }
   l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
   tmem_wait_st();
 }
 
-// softmax_tile<true, true> with less code: for a tile with e_j that some row does not see all
-// of, and any tile with e_j of a bf16 model (rare).
-__device__ __forceinline__ void softmax_tile_any(uint32_t s_addr, uint32_t o_addr, const float* ev,
+// softmax_step<true> with less code, for the rare tiles of bf16 models with e_j.
+__device__ __forceinline__ void softmax_step_any(uint32_t s_addr, uint32_t o_addr, const float* ev,
                                                  float fac, int v0, const RowLim& lim, bool first,
-                                                 uint64_t* pv_bar, int cnt,
+                                                 uint64_t* pv_bar, uint32_t pv_par,
                                                  float& m, float& l, bool& ok) {
   float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll 1
-  for (int c = 0; c < 128; c += 16) {
+  for (int c = 0; c < kBS; c += 16) {
     const uint32_t seen = lim.bits(v0 + c);
     uint32_t s[16];
     tmem_ld16(s_addr + c, s);
@@ -375,12 +352,12 @@ __device__ __forceinline__ void softmax_tile_any(uint32_t s_addr, uint32_t o_add
       x1 = fmaxf(x1, fmaxf(seen & (4u << e) ? t2 : -INFINITY, seen & (8u << e) ? t3 : -INFINITY));
     }
   }
-  move_max(fmaxf(x0, x1), o_addr, first, pv_bar, cnt, m, l, ok);
+  move_max(fmaxf(x0, x1), o_addr, first, pv_bar, pv_par, m, l, ok);
   if (!ok) return;
   const float nb = m == -INFINITY ? 0.0f : -m;
   float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-  for (int c = 0; c < 128; c += 16) {
+  for (int c = 0; c < kBS; c += 16) {
     const uint32_t seen = lim.bits(v0 + c);
     uint32_t s[16], w[8];
     tmem_ld16(s_addr + c, s);
@@ -418,7 +395,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
   float* eb = reinterpret_cast<float*>(smem + C::kOffE);
   uint32_t* gb = reinterpret_cast<uint32_t*>(smem + C::kOffG);
   float2* info = reinterpret_cast<float2*>(smem + C::kOffInfo);
-  float* ksm = reinterpret_cast<float*>(smem + C::kOffKs);
+  float* facs = reinterpret_cast<float*>(smem + C::kOffFac);
   float2* rowb = reinterpret_cast<float2*>(smem + C::kOffRow);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* q_full = bars;
@@ -429,10 +406,11 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
   uint64_t* st_full = v_empty + kStages;
   uint64_t* st_empty = st_full + C::kSlots;
   uint64_t* lv_full = st_empty + C::kSlots;
-  uint64_t* s_full = lv_full + kLvSlots;  // per group
-  uint64_t* p_ready = s_full + 2;
-  uint64_t* pv_done = p_ready + 2;
-  uint64_t* o_empty = pv_done + 2;
+  uint64_t* lv_empty = lv_full + C::kLvSlots;
+  uint64_t* s_full = lv_empty + C::kLvSlots;  // [group][S buffer]
+  uint64_t* p_ready = s_full + 4;
+  uint64_t* pv_done = p_ready + 4;             // (of P V)
+  uint64_t* o_empty = pv_done + 4;
   uint64_t* drain = o_empty + 1;
   uint64_t* soft_bar = drain + 1;         // the softmax warps among themselves
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
@@ -461,8 +439,11 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
         mbar_init(&st_full[i], 1);
         mbar_init(&st_empty[i], kConvThreads / 32);
       }
-      for (int i = 0; i < kLvSlots; ++i) mbar_init(&lv_full[i], 1);
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < C::kLvSlots; ++i) {
+        mbar_init(&lv_full[i], 1);
+        mbar_init(&lv_empty[i], 1);
+      }
+      for (int i = 0; i < 4; ++i) {
         mbar_init(&s_full[i], 1);
         mbar_init(&p_ready[i], 4);
         mbar_init(&pv_done[i], 1);
@@ -477,20 +458,37 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = *tmem_slot;  // 0: a block allocates all columns
   const uint32_t q_base = smem_u32(smem), k_base = smem_u32(smem + C::kOffK),
                  v_base = smem_u32(smem + C::kOffV);
   Walk walk = walk_start<MT, STREAM, 1>(p, cum);
   auto next_piece = [&](Walk& k, Piece& to) { return walk_next<MT, STREAM, 1>(k, p, cum, to); };
   Piece w{};
+  // the block's tiles one after the other, whatever the piece
+  struct Cursor {
+    Walk k;
+    Piece w;
+    int t;
+  };
+  auto next_tile = [&](Cursor& c) -> bool {
+    if (++c.t < c.w.t1) return true;
+    do {
+      if (!next_piece(c.k, c.w)) return false;
+    } while (c.w.t0 >= c.w.t1);
+    c.t = c.w.t0;
+    return true;
+  };
 
+  // registers: 640 threads x 96 at launch = 61,440 = 256 x 120 + 384 x 80
+  if (warp >= kSoft / 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
   if (warp < kSoft / 32) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
     // ================= softmax: one thread per row (ALT: and group)
     const int grp = warp >> 2, lr = tid & 127, r = ALT ? lr : tid;  // row of its tile, of the piece
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + 128 * grp + lane_base;
-    const uint32_t o_addr = tmem + kColO + 128 * grp + lane_base;
-    int pc = 0, gt0 = 0, cnt = 0;       // pieces, tiles of the block before this piece, own tiles
+    const uint32_t s_addr = 128 * grp + lane_base;
+    const uint32_t o_addr = kColO + 128 * grp + lane_base;
+    int pc = 0, gt0 = 0, cnt = 0;       // pieces, tiles of the block before this piece, own steps
     bool ok = true;
     unsigned char* q_tile = smem + (ALT ? 0 : grp) * C::kParts * kTileB;
     auto chunk = [&](int c) {  // 8 channels of the row
@@ -513,129 +511,131 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
       const Seg& s = p.seg;
       const bool live = r < w.rows;
       const int u = (w.row0 + r) / p.nrep, h = w.kvh * p.nrep + (w.row0 + r) - u * p.nrep;
+      const int wr0 = 32 * (ALT ? warp & 3 : warp);        // the warp's first row
       if (n_tiles > 0) {
-        // ---- q' of the row, in place in the Q tile.  (The tile is free: every S of the piece
-        // before has been seen; the barrier ends its use for the output.)
-        float am = 0.0f;
+        // ---- q' of kForm rows (those the warp stores in the end), 16 lanes a row.  The Q tile is
+        // free: every S of the piece before has been seen.
+        constexpr int DT = LO ? HQ_DTYPE_F16 : HQ_DTYPE_BF16, kForm = ALT ? 16 : 32;
+        const int fr0 = ALT ? wr0 + 16 * grp : wr0, c = lane & 15, odd = lane >> 4;
+        uint64_t from;  // of row fr0 + lane
         {
-          const uint4* src = reinterpret_cast<const uint4*>(
-              static_cast<const char*>(p.q) + 2 * (w.b * s.qsb + u * s.qsu + h * p.qsh)) + ch0;
-          uint4 x[kCh];
-#pragma unroll
-          for (int c = 0; c < kCh; ++c) x[c] = live ? src[c] : make_uint4(0, 0, 0, 0);
-          float ks = 0.0f;
-          if (tid < kD)
-            ks = load_scale(s.ksc, w.b * s.kscb + w.kvh * s.ksch + tid * s.kscd, p.s_dt) * p.qk_scale;
-          uint32_t a = 0;
-#pragma unroll
-          for (int c = 0; c < kCh; ++c)
-            a = p.q_dt == HQ_DTYPE_BF16
-                    ? absmax_x2<HQ_DTYPE_BF16>(a, absmax_x2<HQ_DTYPE_BF16>(absmax_x2<HQ_DTYPE_BF16>(x[c].x, x[c].y),
-                                                                           absmax_x2<HQ_DTYPE_BF16>(x[c].z, x[c].w)))
-                    : absmax_x2<HQ_DTYPE_F16>(a, absmax_x2<HQ_DTYPE_F16>(absmax_x2<HQ_DTYPE_F16>(x[c].x, x[c].y),
-                                                                         absmax_x2<HQ_DTYPE_F16>(x[c].z, x[c].w)));
-          am = p.q_dt == HQ_DTYPE_BF16 ? absmax_of_x2<HQ_DTYPE_BF16>(a) : absmax_of_x2<HQ_DTYPE_F16>(a);
-          soft_sync();
-#pragma unroll
-          for (int c = 0; c < kCh; ++c) *chunk(ch0 + c) = x[c];
-          if (tid < kD) ksm[tid] = ks;
-          if (ALT) rowb[tid].x = am;
+          const int rr = w.row0 + min(fr0 + (lane & (kForm - 1)), w.rows - 1), uu = rr / p.nrep;
+          from = reinterpret_cast<uint64_t>(p.q) +
+                 2 * (w.b * s.qsb + uu * s.qsu + (w.kvh * p.nrep + rr - uu * p.nrep) * p.qsh);
         }
-        soft_sync();
-        if (ALT) am = fmaxf(rowb[lr].x, rowb[kBN + lr].x);
-        if (p.q_quant) {
-          if (live && (!ALT || grp == 0)) fake_quant_row(q_tile, lr, p.q_dt);
-          soft_sync();
+        float k8[8], km = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float k = load_scale(s.ksc, w.b * s.kscb + w.kvh * s.ksch + (4 * lane + e) * s.kscd, p.s_dt) * p.qk_scale;
+          k8[e] = __shfl_sync(0xffffffffu, k, 2 * c);
+          k8[4 + e] = __shfl_sync(0xffffffffu, k, 2 * c + 1);
+          km = fmaxf(km, fabsf(k));
         }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        // 2^ex brings the bound max |q| max k_scale to [2^13, 2^14): the row's largest |q'| may
-        // lie some powers of two below, of which float16 has 14 to spare
-        const float4 k4 = reinterpret_cast<const float4*>(ksm)[lane];
-        float km = fmaxf(fmaxf(fabsf(k4.x), fabsf(k4.y)), fmaxf(fabsf(k4.z), fabsf(k4.w)));
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
-        const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am * km) >> 23) - 127), -100), 100);
-        const float mul = pow2i(ex);
-        fac = pow2i(-ex);
-        if (live) {
-#pragma unroll 1
-          for (int c = ch0; c < ch0 + kCh; ++c) {
-            float f[8];
-            unpack8(*chunk(c), p.q_dt, f);
-            const float4 a = reinterpret_cast<const float4*>(ksm)[2 * c], b = reinterpret_cast<const float4*>(ksm)[2 * c + 1];
-            const float k8[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            uint32_t hi[4], lo[4];
+        {
+          constexpr int NX = kForm / 2;
+          uint4 x[NX];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y0 = f[2 * e] * k8[2 * e] * mul, y1 = f[2 * e + 1] * k8[2 * e + 1] * mul;
-              hi[e] = pack_h2(y0, y1);
-              if constexpr (LO) {
-                const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-                lo[e] = pack_h2(y0 - g.x, y1 - g.y);
+          for (int i = 0; i < NX; ++i) {
+            const int k = 2 * i + odd;
+            const uint64_t src = __shfl_sync(0xffffffffu, from, k);
+            x[i] = fr0 + k < w.rows ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll 1
+          for (int i0 = 0; i0 < NX; i0 += 2) {  // (rolled, the rows move up: straight code would run cold)
+            uint4 y[2] = {x[0], x[1]};
+            float am[2];
+#pragma unroll
+            for (int k = 0; k < NX - 2; ++k) x[k] = x[k + 2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              am[i] = absmax_of_x2<DT>(absmax_x2<DT>(absmax_x2<DT>(y[i].x, y[i].y), absmax_x2<DT>(y[i].z, y[i].w)));
+#pragma unroll
+            for (int o = 8; o >= 1; o >>= 1)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) am[i] = fmaxf(am[i], __shfl_xor_sync(0xffffffffu, am[i], o));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (p.q_quant) y[i] = fake_quant<DT>(y[i], am[i]);
+              // 2^ex brings the bound max |q| max k_scale to [2^13, 2^14): the row's largest |q'|
+              // may lie some powers of two below, of which float16 has 14 to spare
+              const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am[i] * km) >> 23) - 127), -100), 100);
+              const float mul = pow2i(ex);
+              float f[8];
+              Vec16<DT>::unpack(y[i], f);
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float y0 = f[2 * e] * k8[2 * e] * mul, y1 = f[2 * e + 1] * k8[2 * e + 1] * mul;
+                hi[e] = pack_h2(y0, y1);
+                if constexpr (LO) {
+                  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+                  lo[e] = pack_h2(y0 - g.x, y1 - g.y);
+                }
               }
+              const int row = fr0 + 2 * (i0 + i) + odd;
+              unsigned char* to = smem + (row >> 7) * C::kParts * kTileB + (c >> 3) * (kBN * 128) + sw128(row & 127, c & 7);
+              *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              if constexpr (LO) *reinterpret_cast<uint4*>(to + kTileB) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              if (c == 0) facs[row] = pow2i(-ex);
             }
-            *chunk(c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if constexpr (LO) *(chunk(c) + kTileB / 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
-        // the groups keep step from piece to piece: one without tiles must not arrive for the
+        // the groups keep step from piece to piece: one without rows must not arrive for the
         // next piece in this one's phase, nor look at a tile two ahead of the other's
         ok = wait_bar(q_full, pc & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        fac = facs[r];
       }
-      const int wr0 = 32 * (ALT ? warp & 3 : warp);        // the warp's first row
       const bool warp_live = wr0 < w.rows;
       const bool mine = ALT || w.rows > 128 * grp;          // this group has rows
       const int pos = w.key.pos0 + (s.step ? u : 0);
       const RowLim lim = {live ? pos - w.key.sh : 1 << 30,
                           live ? pos - s.window + 1 - w.key.sh : 0,
                           w.key.sh > 0 ? w.key.ns : s.sinks};
-      const int tf = w.t0 + (ALT ? grp : 0);                // this group's first tile
-      for (int t = tf; ok && mine && t < w.t1; t += ALT ? 2 : 1, ++cnt) {
-        const int gt = gt0 + t - w.t0, slot = gt % kLvSlots;
-        ok = wait_bar(&lv_full[slot], (gt / kLvSlots) & 1) &&
-             wait_bar(&s_full[grp], cnt & 1);
+      const int steps = !mine ? 0 : ALT ? n_tiles : 2 * n_tiles;
+      for (int i = 0; ok && i < steps; ++i, ++cnt) {
+        const int t = ALT ? i : i >> 1, half = ALT ? grp : i & 1;
+        const int slot = (gt0 + t) % C::kLvSlots, buf = cnt & 1;
+        ok = wait_bar(&lv_full[slot], ((gt0 + t) / C::kLvSlots) & 1) &&
+             wait_bar(&s_full[2 * grp + buf], (cnt >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          const float* ev = eb + slot * 2 * kBN;
-          const int v0 = t * kBN;
+          const float* ev = eb + slot * 2 * kBN + kBS * half;
+          const int v0 = (w.t0 + t) * kBN + kBS * half;
           const float2 ti = info[slot];
           vscale = ti.y;
-          const bool need = v0 + kBN - 1 > lim.hi || (v0 < lim.lo && v0 + kBN > lim.vsk && lim.lo > lim.vsk);
+          const bool need = v0 + kBS - 1 > lim.hi || (v0 < lim.lo && v0 + kBS > lim.vsk && lim.lo > lim.vsk);
           const bool mask = __any_sync(0xffffffffu, need);
-          if ((!LO && ti.x != 0.0f) || (LO && mask))
-            softmax_tile_any(s_addr, o_addr, ev, fac, v0, lim, t == tf, &pv_done[grp], cnt, m, l, ok);
-          else if (LO || !mask)
-            softmax_tile<LO, false>(s_addr, o_addr, ev, fac, v0, lim, t == tf, &pv_done[grp], cnt, m, l, ok);
+          uint64_t* pvb = &pv_done[2 * grp + (buf ^ 1)];
+          const uint32_t pvp = ((cnt - 1) >> 1) & 1;
+          if (!LO && ti.x != 0.0f)
+            softmax_step_any(s_addr + kBS * buf, o_addr, ev, fac, v0, lim, i == 0, pvb, pvp, m, l, ok);
           else
-            softmax_tile<false, true>(s_addr, o_addr, ev, fac, v0, lim, t == tf, &pv_done[grp], cnt, m, l, ok);
-        } else if (cnt > 0) {
-          ok = wait_bar(&pv_done[grp], (cnt - 1) & 1);
-          ok = __all_sync(0xffffffffu, ok);
+            softmax_step<LO>(s_addr + kBS * buf, o_addr, ev, fac, v0, lim, mask, i == 0, pvb, pvp, m, l, ok);
         }
         if (!ok) break;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[grp]);
+        if (lane == 0) mbar_arrive(&p_ready[2 * grp + buf]);
       }
       if (!ok) break;
       gt0 += n_tiles;
       // ---- the rows' results
-      const int my_tiles = !mine ? 0 : ALT ? (n_tiles + 1 - grp) / 2 : n_tiles;
-      if (my_tiles > 0) {
-        ok = wait_bar(&pv_done[grp], (cnt - 1) & 1);
+      if (steps > 0) {
+        ok = wait_bar(&pv_done[2 * grp + ((cnt - 1) & 1)], ((cnt - 1) >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
       // (rows that saw nothing have l = 0 and give zeros, whatever their O holds; a NaN stays)
-      bool has0 = my_tiles > 0 && !(l <= 0.0f), has1 = false;
+      bool has0 = steps > 0 && !(l <= 0.0f), has1 = false;
       float f0 = 1.0f, f1 = 0.0f;
       if constexpr (ALT) {  // both groups' states; each thread then takes half of the columns
         rowb[tid] = make_float2(m, l);
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
         tc_fence_after();
         const float2 a = rowb[lr], b = rowb[kBN + lr];
         has0 = n_tiles > 0 && !(a.y <= 0.0f);
-        has1 = n_tiles > 1 && !(b.y <= 0.0f);
+        has1 = n_tiles > 0 && !(b.y <= 0.0f);
         m = fmaxf(a.x, b.x);
         f0 = a.x == -INFINITY ? 0.0f : ex2_ftz(a.x - m);
         f1 = b.x == -INFINITY ? 0.0f : ex2_ftz(b.x - m);
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const bool have = live && (has0 || has1);
-      const uint32_t o0 = ALT ? tmem + kColO + lane_base : o_addr, o1 = tmem + kColO + 128 + lane_base;
+      const uint32_t o0 = ALT ? kColO + lane_base : o_addr, o1 = kColO + 128 + lane_base;
       if (warp_live && mine) {
         const float scale = w.slot < 0 ? (have ? vscale / l : 0.0f) : vscale;
         f0 = has0 ? f0 * scale : 0.0f;
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     // columns, and rows 16 apart have the same swizzle
     const int c8 = ct & 15, row = ct >> 4;
     const uint32_t at = static_cast<uint32_t>(c8 >> 3) * (kBN * 128) + sw128(row, c8 & 7);
-    int sl = 0, gt = 0;  // slot, tiles
+    int sl = 0;  // slot
     uint32_t sl_par = 0;
     bool ok = true;
     // the next staging slot into rows 64 half .. of a tile; V rows times their g
@@ -751,49 +751,57 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
         sl_par ^= 1;
       }
     };
-    for (; ok && next_piece(walk, w);) {
-      for (int t = w.t0; t < w.t1; ++t, ++gt) {
-        const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
-        if (use > 0) ok = wait_bar(&k_empty[st], (use - 1) & 1);
-        if (!ok) break;
+    // K of the next tile goes before V of this one: V waits for the P V of two tiles before, and
+    // S of the next tile must not wait with it
+    Cursor kc{walk, w, -1};
+    int gk = 0;  // K tiles done
+    auto next_k = [&] {
+      if (!next_tile(kc)) return;
+      const int st = gk % kStages, use = gk / kStages;
+      if (use > 0) ok = wait_bar(&k_empty[st], (use - 1) & 1);
 #pragma unroll 1
-        for (int half = 0; half < 2 && ok; ++half)
-          convert(smem + C::kOffK + st * kTileB + half * 8192, std::false_type{}, nullptr);
-        if (!ok) break;
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&k_full[st]);
-        if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1);
-        ok = ok && wait_bar(&lv_full[slot], (gt / kLvSlots) & 1);
-        if (!ok) break;
+      for (int half = 0; half < 2 && ok; ++half)
+        convert(smem + C::kOffK + st * kTileB + half * 8192, std::false_type{}, nullptr);
+      if (!ok) return;
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[st]);
+      ++gk;
+    };
 #pragma unroll 1
-        for (int half = 0; half < 2 && ok; ++half)
-          convert(smem + C::kOffV + st * kTileB + half * 8192, std::true_type{},
-                  gb + slot * kBN + half * kSlotKeys);
-        if (!ok) break;
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[st]);
-      }
+    for (int gt = -1; ok && gt < gk; ++gt) {
+      next_k();
+      if (!ok || gt < 0 || gt >= gk) continue;
+      const int st = gt % kStages, use = gt / kStages, slot = gt % C::kLvSlots;
+      if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1);
+      ok = ok && wait_bar(&lv_full[slot], (gt / C::kLvSlots) & 1);
+#pragma unroll 1
+      for (int half = 0; half < 2 && ok; ++half)
+        convert(smem + C::kOffV + st * kTileB + half * 8192, std::true_type{},
+                gb + slot * kBN + half * kSlotKeys);
+      if (!ok) break;
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[st]);
     }
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
   } else if (warp == kCopyWarp) {
     // ================= codes into the staging ring
     int sc = 0;
     bool ok = true;
-    for (; ok && next_piece(walk, w);) {
-      const Seg& s = p.seg;
-      const int64_t o = w.b * s.sb + w.kvh * s.sh;
+    const Seg& s = p.seg;
+    auto copy_tile = [&](const Cursor& c, const int8_t* base) {
+      const Piece& w = c.w;
 #pragma unroll 1
-      for (int t2 = 4 * w.t0; ok && t2 < 4 * w.t1; ++t2, ++sc) {  // K 0 .., K 64 .., V 0 .., V 64 ..
+      for (int half = 0; ok && half < 2; ++half, ++sc) {
         const int sl = sc % C::kSlots, use = sc / C::kSlots;
         if (use > 0) ok = wait_bar(&st_empty[sl], (use - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const int v0 = (t2 >> 2) * kBN + (t2 & 1) * kSlotKeys;
+        const int v0 = c.t * kBN + half * kSlotKeys;
         const int n = min(max(w.key.nv - v0, 0), kSlotKeys);
         unsigned char* dst = smem + C::kOffSlot + sl * kSlotB;
-        const int8_t* src = (t2 & 2 ? s.v : s.k) + o;
+        const int8_t* src = base + w.b * s.sb + w.kvh * s.sh;
         if (lane == 0) mbar_arrive_expect_tx(&st_full[sl], n * kD);
         __syncwarp();
         if (s.ss == kD) {  // rows back to back: the sinks' run and the window's
@@ -810,6 +818,14 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
           }
         }
       }
+    };
+    Cursor kc{walk, w, -1}, vc{walk, w, -1};
+    bool more = next_tile(kc);
+    if (more) copy_tile(kc, s.k);
+    while (ok && next_tile(vc)) {  // K 1, V 0, K 2, V 1, ..
+      more = more && next_tile(kc);
+      if (more) copy_tile(kc, s.k);
+      if (ok) copy_tile(vc, s.v);
     }
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
     // no copy is in flight when the block ends
@@ -820,24 +836,17 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     // ================= V scales into g_j and e_j, loaded a tile ahead
     int gt = 0;
     bool ok = true;
-    // cursor of the loads
-    Piece lp{};
-    int lt = -1;
+    Cursor c{walk, w, -1};  // of the loads
     float next[4];
     auto load_next = [&]() -> bool {
-      if (++lt >= lp.t1) {
-        do {
-          if (!next_piece(walk, lp)) return false;
-        } while (lp.t0 >= lp.t1);
-        lt = lp.t0;
-      }
+      if (!next_tile(c)) return false;
       const Seg& s = p.seg;
-      const int64_t vs0 = lp.b * s.vscb + lp.kvh * s.vsch;
+      const int64_t vs0 = c.w.b * s.vscb + c.w.kvh * s.vsch;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int v = lt * kBN + 32 * i + lane;
-        const int64_t key = v < lp.key.ns ? v : v + lp.key.sh;
-        next[i] = v < lp.key.nv ? load_scale(s.vsc, vs0 + key * s.vscs, p.s_dt) : -1.0f;
+        const int v = c.t * kBN + 32 * i + lane;
+        const int64_t key = v < c.w.key.ns ? v : v + c.w.key.sh;
+        next[i] = v < c.w.key.nv ? load_scale(s.vsc, vs0 + key * s.vscs, p.s_dt) : -1.0f;
       }
       return true;
     };
@@ -847,11 +856,10 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
       float vs[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) vs[i] = next[i];
-      const bool first = lt == lp.t0;
+      const bool first = c.t == c.w.t0;
       have = load_next();
-      // slot gt % kLvSlots is free once P V of the tile two before is done
-      const int st = gt % kStages, use = gt / kStages, slot = gt % kLvSlots;
-      if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1);
+      const int use = gt / C::kLvSlots, slot = gt % C::kLvSlots;
+      if (use > 0) ok = wait_bar(&lv_empty[slot], (use - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       float* ev = eb + slot * 2 * kBN;
@@ -904,126 +912,112 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     // ================= tensor-core products, issued by one thread; the warp stays together,
     // so that descriptors and addresses live in uniform registers
     {
-      const bool lead = elect_one();
-      constexpr uint32_t id_s = idesc<HQ_DTYPE_F16>(128, 128, false);
+      const uint32_t lead = elect_one();
+      constexpr uint32_t id_s = idesc<HQ_DTYPE_F16>(128, kBS, false);
       constexpr uint32_t id_o = idesc<HQ_DTYPE_F16>(128, 128, true);
+      // descriptors: the high word does not depend on the address, whose low word counts 16 bytes
+      // (no sum leaves its 14 bits)
+      constexpr uint32_t k_hi = sdesc(0, 16, 1024) >> 32, v_hi = sdesc(0, kBN * 128, 1024) >> 32;
+      const uint32_t q_lo = static_cast<uint32_t>(sdesc(q_base, 16, 1024));
+      const uint32_t k_lo = static_cast<uint32_t>(sdesc(k_base, 16, 1024));
+      const uint32_t v_lo = static_cast<uint32_t>(sdesc(v_base, kBN * 128, 1024));
       bool ok = true;
-      int cntp[2] = {0, 0}, pieces = 0;  // P V products of each group, pieces
-      // S = Q K^T of tile g for group m
-      auto qk = [&](int m, int g) {
-        const uint64_t dk = sdesc(k_base + (g % kStages) * kTileB, 16, 1024);
-        const uint64_t dq = sdesc(q_base + (ALT ? 0 : m) * C::kParts * kTileB, 16, 1024);
-        if (lead) {
-#pragma unroll
-          for (int part = 0; part < C::kParts; ++part)
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {
-              // (the address field counts 16 bytes; no sum leaves its 14 bits)
-              const uint32_t off = ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) >> 4;
-              mma_f16(tmem + 128 * m, dq + (part * (kTileB >> 4) + off), dk + off, id_s, part + kk > 0);
-            }
-          mma_commit(&s_full[m]);
-        }
-        __syncwarp();
-      };
-      auto pv = [&](int m, int g, bool first) {
-        ok = ok && wait_bar(&p_ready[m], (m ? cntp[1] : cntp[0]) & 1);
+      int g0 = 0, pieces = 0;   // tiles of the block before this piece, pieces
+      int n0 = 0, n1 = 0;       // steps before this piece of each group
+      // Step i of a piece, for group m: tile i and half m (ALT), or half i & 1 of tile i / 2
+      auto tile_of = [&](int i) { return g0 + (ALT ? i : i >> 1); };
+      auto k_wait = [&](int i) {
+        const int g = tile_of(i);
+        if (ALT || !(i & 1)) ok = ok && wait_bar(&k_full[g % kStages], (g / kStages) & 1);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
         tc_fence_after();
-        const uint64_t dv = sdesc(v_base + (g % kStages) * kTileB, kBN * 128, 1024);
-        if (lead) {
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            mma_f16_ts(tmem + kColO + 128 * m, tmem + 128 * m + 8 * kk, dv + (kk * 16 * 128 >> 4),
-                       id_o, !first || kk > 0);
-          mma_commit(&pv_done[m]);
-        }
-        __syncwarp();
-        if (m) ++cntp[1]; else ++cntp[0];
       };
-      // cursor of the S products, one tile ahead of the P V products
-      Walk qw = walk;
-      Piece qp, cp;
-      int qpc = -1, qt = 0, qg = 0;
-      qp.t0 = qp.t1 = 0;
-      bool more = true, fresh = false;
-      auto q_next = [&]() {  // qp, qt: the next tile's piece and index
-        fresh = false;
-        if (++qt < qp.t1) return;
-        do {
-          if (!next_piece(qw, qp)) {
-            more = false;
-            return;
+      auto k_done = [&](int i) {  // after the last S product that reads the tile
+        if (ALT || (i & 1)) commit(lead, &k_empty[tile_of(i) % kStages]);
+      };
+      auto qk = [&](auto group, int i) {  // S = Q K^T
+        constexpr int m = decltype(group)::value;
+        const int buf = ((m ? n1 : n0) + i) & 1, half = ALT ? m : i & 1;
+        const uint32_t b = k_lo + ((tile_of(i) % kStages * kTileB + half * kBS * 128) >> 4);
+        const uint32_t a = q_lo + ((ALT ? 0 : m) * C::kParts * kTileB >> 4);
+#pragma unroll
+        for (int part = 0; part < C::kParts; ++part)
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t off = ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) >> 4;
+            mma_ss(lead, 128 * m + kBS * buf, a + (part * (kTileB >> 4) + off), k_hi, b + off, k_hi,
+                   id_s, part + kk > 0);
           }
-        } while (qp.t0 >= qp.t1);
-        ++qpc;
-        qt = qp.t0;
-        fresh = true;
+        commit(lead, &s_full[2 * m + buf]);
       };
-      auto q_wait = [&]() {  // its q (of a piece's first tile) and K
-        if (fresh) ok = ok && wait_bar(q_full, qpc & 1);
-        ok = ok && wait_bar(&k_full[qg % kStages], (qg / kStages) & 1);
+      auto pv = [&](auto group, int i) {  // O += P V
+        constexpr int m = decltype(group)::value;
+        const int n = (m ? n1 : n0) + i, buf = n & 1, half = ALT ? m : i & 1;
+        ok = wait_bar(&p_ready[2 * m + buf], (n >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
-        tc_fence_after();
-      };
-      auto q_done = [&]() {  // after the last S product of the tile
-        if (lead) mma_commit(&k_empty[qg % kStages]);
-        ++qg;
-      };
-      auto q_all = [&]() {
-        q_wait();
         if (!ok) return;
-        if constexpr (ALT) {
-          qk((qt - qp.t0) & 1, qg);
-        } else {
-#pragma unroll 1
-          for (int m = 0; m < 2; ++m)
-            if (qp.rows > 128 * m) qk(m, qg);
-        }
-        q_done();
+        tc_fence_after();
+        const uint32_t b = v_lo + ((tile_of(i) % kStages * kTileB + half * kBS * 128) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kBS / 16; ++kk)
+          mma_ts(lead, kColO + 128 * m, 128 * m + kBS * buf + 8 * kk, b + (kk * 16 * 128 >> 4), v_hi,
+                 id_o, kk > 0 ? 1 : i > 0);
+        commit(lead, &pv_done[2 * m + buf]);
       };
-      qt = -1;
-      q_next();
-      if (more) q_all();
-      int g = 0;  // tile of the P V products
-      while (ok && more) {
-        cp = qp;
-        const int ctile = qt;
-        q_next();
-        // within a piece the next S goes out ahead of (ALT: it is the other group's) or between
-        // (two row tiles) the P V products; a piece's first S comes after them, since its q is
-        // made by the warps that wait for the last P V of the piece before
-        const bool ahead = more && !fresh;
-        if (ahead && ALT) q_all();
-        if (ahead && !ALT) q_wait();
-        ok = ok && wait_bar(&v_full[g % kStages], (g / kStages) & 1);
-        if (ctile == cp.t0) {
-          if (pieces > 0) ok = ok && wait_bar(o_empty, (pieces - 1) & 1);
-          ++pieces;
-        }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if constexpr (ALT) {
-          pv((ctile - cp.t0) & 1, g, ctile - cp.t0 < 2);
-        } else {
+      using G0 = std::integral_constant<int, 0>;
+      using G1 = std::integral_constant<int, 1>;
+      // (all of the tensor memory is this block's: its columns count from 0)
+      if (tmem != 0) ok = false;
+      for (; ok && next_piece(walk, w);) {
+        const int n_tiles = w.t1 - w.t0, steps = ALT ? n_tiles : 2 * n_tiles;
+        if (n_tiles <= 0) continue;
+        const bool two = ALT || w.rows > 128;
+        // (a piece's q is made by the warps that wait for the last P V of the piece before)
+        ok = wait_bar(q_full, pieces & 1);
+        // S of the first two steps; from then on S of step i + 2 follows P V of step i, whose P
+        // lies in the same columns: the products run in order
 #pragma unroll 1
-          for (int m = 0; m < 2 && ok; ++m)
-            if (cp.rows > 128 * m) {
-              pv(m, g, ctile == cp.t0);
-              // the next S of this row tile overwrites the P just read: the products run in order
-              if (ok && ahead) qk(m, qg);
-            }
+        for (int i = 0; ok && i < min(steps, 2); ++i) {
+          k_wait(i);
+          if (!ok) break;
+          qk(G0{}, i);
+          if (two) qk(G1{}, i);
+          k_done(i);
         }
-        if (!ok) break;
-        if (lead) mma_commit(&v_empty[g % kStages]);
-        if (!ALT && ahead) q_done();
-        if (more && fresh) q_all();
-        ++g;
+        if (pieces > 0) ok = ok && wait_bar(o_empty, (pieces - 1) & 1);
+        ++pieces;
+#pragma unroll 1
+        for (int i = 0; ok && i < steps; ++i) {
+          const int g = tile_of(i);
+          if (ALT || !(i & 1)) ok = wait_bar(&v_full[g % kStages], (g / kStages) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          pv(G0{}, i);
+          if (!ok) break;
+          const bool more = i + 2 < steps;
+          if (more) {
+            k_wait(i + 2);
+            if (!ok) break;
+            qk(G0{}, i + 2);
+          }
+          if (two) {
+            pv(G1{}, i);
+            if (!ok) break;
+            if (more) qk(G1{}, i + 2);
+          }
+          if (ALT || (i & 1)) {
+            commit(lead, &v_empty[g % kStages]);
+            commit(lead, &lv_empty[g % C::kLvSlots]);  // (its readers are done with the tile, too)
+          }
+          if (more) k_done(i + 2);
+        }
+        g0 += n_tiles;
+        n0 += steps;
+        n1 += two ? steps : 0;
       }
       if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
       // every product has completed before the tensor memory is released
-      if (lead) mma_commit(drain);
+      commit(lead, drain);
       if (!mbar_wait(drain, 0)) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
     }
     __syncwarp();

@@ -56,8 +56,6 @@ constexpr int kConvThreads = 256;
 constexpr int kBS = 64;                   // keys of a softmax step: half a tile
 constexpr int kTileB = kBN * kD * 2;      // a float16 K, V or Q tile: 32 KB
 constexpr int kStages = 2;                // K and V tiles in shared memory
-constexpr int kSlotKeys = 64;             // keys of a staging slot (K or V codes)
-constexpr int kSlotB = kSlotKeys * kD;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 256;           // S buffers at columns 0 and 128
 
@@ -66,18 +64,21 @@ struct Cfg {
   static constexpr int kThreads = kSoft + kConvThreads + 128;
   static constexpr int kRowTiles = ALT ? 1 : 2;
   static constexpr int kParts = LO ? 2 : 1;
-  static constexpr int kSlots = kRowTiles * kParts == 1 ? 6 : 3;   // staging: 8 KB each
+  // staging rings, one for K codes and one for V codes
+  static constexpr int kSlots = 3;
+  static constexpr int kSlotKeys = kRowTiles * kParts == 1 ? 64 : 32;
+  static constexpr int kSlotB = kSlotKeys * kD;
   static constexpr int kLvSlots = LO ? 2 : 3;  // ring of what the tiles' V scales lead to
   static constexpr int kOffK = kRowTiles * kParts * kTileB;
   static constexpr int kOffV = kOffK + kStages * kTileB;
   static constexpr int kOffSlot = kOffV + kStages * kTileB;
-  static constexpr int kOffE = kOffSlot + kSlots * kSlotB;         // [slot][e_j, 2^-e_j][128]
+  static constexpr int kOffE = kOffSlot + 2 * kSlots * kSlotB;     // [slot][e_j, 2^-e_j][128]
   static constexpr int kOffG = kOffE + kLvSlots * 2 * kBN * 4;     // [slot][128] g_j, float16 twice
   static constexpr int kOffInfo = kOffG + kLvSlots * kBN * 4;      // [slot]{any e_j, 2^E}
   static constexpr int kOffFac = kOffInfo + 16 * ((kLvSlots + 1) / 2);  // [row] what q' was divided by
   static constexpr int kOffRow = kOffFac + kRowTiles * 128 * 4;     // ALT: [2][128] the groups' (m, l)
   static constexpr int kOffBar = kOffRow + (ALT ? 2 * kBN * 8 : 0);
-  static constexpr int kBars = 1 + 4 * kStages + 2 * kSlots + 2 * kLvSlots + 4 + 4 + 4 + 1 + 1 + 1;
+  static constexpr int kBars = 1 + 4 * kStages + 4 * kSlots + 2 * kLvSlots + 4 + 4 + 4 + 1 + 1 + 1;
   static constexpr int kOffMisc = kOffBar + ((kBars * 8 + 15) & ~15);
   static constexpr int kOffCum = kOffMisc + 16;
   static_assert(kOffFac % 16 == 0 && kOffRow % 16 == 0 && kOffBar % 8 == 0, "vector accesses");
@@ -152,28 +153,26 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-// 32 columns of this thread's lane, valid after tmem_got (which awaits every load issued before
-// it; the registers pass through it, so no use moves up)
-__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t* r) {
+// 64 columns of this thread's lane
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
-      "%29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, "
+      "%36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, "
+      "%53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63"
+      "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]),
+        "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]),
+        "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]),
+        "=r"(r[63])
       : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_got(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
-                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
-                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]));
-  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
 }
 // Bounded wait: some seconds, then false.  One opaque loop: as C++ with its convergence
 // instructions the waits took a third of all issue slots.
@@ -269,10 +268,7 @@ __device__ __forceinline__ void softmax_step(uint32_t s_addr, uint32_t o_addr, c
                                              bool first, uint64_t* pv_bar, uint32_t pv_par,
                                              float& m, float& l, bool& ok) {
   uint32_t s[kBS];
-  tmem_get(s_addr, s);
-  tmem_get(s_addr + 32, s + 32);
-  tmem_got(s);
-  tmem_got(s + 32);
+  tmem_ld64(s_addr, s);
   if constexpr (EXP) {
 #pragma unroll
     for (int e = 0; e < kBS; e += 4) {
@@ -404,8 +400,8 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
   uint64_t* st_full = v_empty + kStages;
-  uint64_t* st_empty = st_full + C::kSlots;
-  uint64_t* lv_full = st_empty + C::kSlots;
+  uint64_t* st_empty = st_full + 2 * C::kSlots;  // [K, V][slot]
+  uint64_t* lv_full = st_empty + 2 * C::kSlots;
   uint64_t* lv_empty = lv_full + C::kLvSlots;
   uint64_t* s_full = lv_empty + C::kLvSlots;  // [group][S buffer]
   uint64_t* p_ready = s_full + 4;
@@ -418,7 +414,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
   int* cum = reinterpret_cast<int*>(smem + C::kOffCum);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kMmaWarp = (kSoft + kConvThreads) / 32, kCopyWarp = kMmaWarp + 1;  // + 2: V scales
+  constexpr int kMmaWarp = (kSoft + kConvThreads) / 32, kCopyWarp = kMmaWarp + 1;  // K; V scales; V
   // combine_kernel's blocks may be scheduled; they wait for this grid
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == kMmaWarp) {
@@ -430,14 +426,14 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     if (lane == 0) {
       mbar_init(q_full, kSoft / 32);
       for (int i = 0; i < kStages; ++i) {
-        mbar_init(&k_full[i], kConvThreads / 32);
+        mbar_init(&k_full[i], kConvThreads / 64);
         mbar_init(&k_empty[i], 1);
-        mbar_init(&v_full[i], kConvThreads / 32);
+        mbar_init(&v_full[i], kConvThreads / 64);
         mbar_init(&v_empty[i], 1);
       }
-      for (int i = 0; i < C::kSlots; ++i) {
+      for (int i = 0; i < 2 * C::kSlots; ++i) {
         mbar_init(&st_full[i], 1);
-        mbar_init(&st_empty[i], kConvThreads / 32);
+        mbar_init(&st_empty[i], kConvThreads / 64);
       }
       for (int i = 0; i < C::kLvSlots; ++i) {
         mbar_init(&lv_full[i], 1);
@@ -710,127 +706,113 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
   } else if (warp < kMmaWarp) {
     // ================= staged codes -> float16 tiles
-    const int ct = tid - kSoft;
-    // 8 codes (one 16-byte chunk) of rows row + 16 i of a slot: 8 lanes store 8 different chunk
-    // columns, and rows 16 apart have the same swizzle
+    // 4 warps turn K, 4 V: fewer waits for each, and V, which waits for the P V of two tiles
+    // before, holds up no K
+    const bool is_v = warp >= (kSoft + kConvThreads / 2) / 32;
+    const int ct = (tid - kSoft) % (kConvThreads / 2);
+    // 8 codes (one 16-byte chunk) of rows row + 8 i of a slot: 8 lanes store 8 different chunk
+    // columns, and rows 8 apart have the same swizzle
     const int c8 = ct & 15, row = ct >> 4;
     const uint32_t at = static_cast<uint32_t>(c8 >> 3) * (kBN * 128) + sw128(row, c8 & 7);
-    int sl = 0;  // slot
-    uint32_t sl_par = 0;
     bool ok = true;
-    // the next staging slot into rows 64 half .. of a tile; V rows times their g
-    auto convert = [&](unsigned char* tile, auto is_v, const uint32_t* g) {
-      ok = wait_bar(&st_full[sl], sl_par);
-      if (!ok) return;
-      const unsigned char* src = smem + C::kOffSlot + sl * kSlotB + row * kD + 8 * c8;
-      constexpr int NI = kSlotKeys / (kConvThreads / 16);
-      uint2 x[NI];
-      uint32_t g2[NI];
+    auto turn = [&](auto v, uint64_t* full, uint64_t* empty, uint64_t* sfull, uint64_t* sempty,
+                    unsigned char* tiles, const unsigned char* slots) {
+      constexpr bool V = decltype(v)::value;
+      constexpr int NI = C::kSlotKeys / 8;
+      int sl = 0, gt = 0;
+      uint32_t sl_par = 0;
+      Cursor c{walk, w, -1};
+      for (; ok && next_tile(c); ++gt) {
+        const int st = gt % kStages, use = gt / kStages;
+        if (use > 0) ok = wait_bar(&empty[st], (use - 1) & 1);
+        if constexpr (V) ok = ok && wait_bar(&lv_full[gt % C::kLvSlots], (gt / C::kLvSlots) & 1);
+        const uint32_t* g = gb + gt % C::kLvSlots * kBN;
+        unsigned char* to = tiles + st * kTileB + at;
+#pragma unroll 1
+        for (int k0 = 0; ok && k0 < kBN; k0 += C::kSlotKeys) {
+          ok = wait_bar(&sfull[sl], sl_par);
+          if (!ok) break;
+          const unsigned char* src = slots + sl * C::kSlotB + row * kD + 8 * c8;
+          uint2 x[NI];
+          uint32_t g2[NI];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        x[i] = *reinterpret_cast<const uint2*>(src + i * 16 * kD);
-        if constexpr (is_v.value) g2[i] = g[row + 16 * i];
-      }
+          for (int i = 0; i < NI; ++i) {
+            x[i] = *reinterpret_cast<const uint2*>(src + i * 8 * kD);
+            if constexpr (V) g2[i] = g[k0 + row + 8 * i];  // V rows times their g
+          }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        uint4 y;
-        codes_to_h2(x[i].x, y.x, y.y);
-        codes_to_h2(x[i].y, y.z, y.w);
-        if constexpr (is_v.value) {
-          asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.x) : "r"(y.x), "r"(g2[i]));
-          asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.y) : "r"(y.y), "r"(g2[i]));
-          asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.z) : "r"(y.z), "r"(g2[i]));
-          asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.w) : "r"(y.w), "r"(g2[i]));
+          for (int i = 0; i < NI; ++i) {
+            uint4 y;
+            codes_to_h2(x[i].x, y.x, y.y);
+            codes_to_h2(x[i].y, y.z, y.w);
+            if constexpr (V) {
+              asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.x) : "r"(y.x), "r"(g2[i]));
+              asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.y) : "r"(y.y), "r"(g2[i]));
+              asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.z) : "r"(y.z), "r"(g2[i]));
+              asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.w) : "r"(y.w), "r"(g2[i]));
+            }
+            *reinterpret_cast<uint4*>(to + (k0 + 8 * i) * 128) = y;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sempty[sl]);
+          if (++sl == C::kSlots) {
+            sl = 0;
+            sl_par ^= 1;
+          }
         }
-        *reinterpret_cast<uint4*>(tile + at + i * 2048) = y;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st_empty[sl]);
-      if (++sl == C::kSlots) {
-        sl = 0;
-        sl_par ^= 1;
+        if (!ok) break;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);
       }
     };
-    // K of the next tile goes before V of this one: V waits for the P V of two tiles before, and
-    // S of the next tile must not wait with it
-    Cursor kc{walk, w, -1};
-    int gk = 0;  // K tiles done
-    auto next_k = [&] {
-      if (!next_tile(kc)) return;
-      const int st = gk % kStages, use = gk / kStages;
-      if (use > 0) ok = wait_bar(&k_empty[st], (use - 1) & 1);
-#pragma unroll 1
-      for (int half = 0; half < 2 && ok; ++half)
-        convert(smem + C::kOffK + st * kTileB + half * 8192, std::false_type{}, nullptr);
-      if (!ok) return;
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[st]);
-      ++gk;
-    };
-#pragma unroll 1
-    for (int gt = -1; ok && gt < gk; ++gt) {
-      next_k();
-      if (!ok || gt < 0 || gt >= gk) continue;
-      const int st = gt % kStages, use = gt / kStages, slot = gt % C::kLvSlots;
-      if (use > 0) ok = wait_bar(&v_empty[st], (use - 1) & 1);
-      ok = ok && wait_bar(&lv_full[slot], (gt / C::kLvSlots) & 1);
-#pragma unroll 1
-      for (int half = 0; half < 2 && ok; ++half)
-        convert(smem + C::kOffV + st * kTileB + half * 8192, std::true_type{},
-                gb + slot * kBN + half * kSlotKeys);
-      if (!ok) break;
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[st]);
-    }
+    if (is_v)
+      turn(std::true_type{}, v_full, v_empty, st_full + C::kSlots, st_empty + C::kSlots,
+           smem + C::kOffV, smem + C::kOffSlot + C::kSlots * C::kSlotB);
+    else
+      turn(std::false_type{}, k_full, k_empty, st_full, st_empty, smem + C::kOffK, smem + C::kOffSlot);
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
-  } else if (warp == kCopyWarp) {
+  } else if (warp == kCopyWarp || warp == kCopyWarp + 2) {
     // ================= codes into the staging ring
+    const int is_v = warp == kCopyWarp + 2;
+    uint64_t* full = st_full + is_v * C::kSlots;
+    uint64_t* empty = st_empty + is_v * C::kSlots;
+    unsigned char* slots = smem + C::kOffSlot + is_v * C::kSlots * C::kSlotB;
     int sc = 0;
     bool ok = true;
-    const Seg& s = p.seg;
-    auto copy_tile = [&](const Cursor& c, const int8_t* base) {
-      const Piece& w = c.w;
+    Cursor c{walk, w, -1};
+    while (ok && next_tile(c)) {
+      const Seg& s = p.seg;
+      const int8_t* src = (is_v ? s.v : s.k) + c.w.b * s.sb + c.w.kvh * s.sh;
 #pragma unroll 1
-      for (int half = 0; ok && half < 2; ++half, ++sc) {
+      for (int v0 = c.t * kBN; v0 < (c.t + 1) * kBN; v0 += C::kSlotKeys, ++sc) {
         const int sl = sc % C::kSlots, use = sc / C::kSlots;
-        if (use > 0) ok = wait_bar(&st_empty[sl], (use - 1) & 1);
+        if (use > 0) ok = wait_bar(&empty[sl], (use - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const int v0 = c.t * kBN + half * kSlotKeys;
-        const int n = min(max(w.key.nv - v0, 0), kSlotKeys);
-        unsigned char* dst = smem + C::kOffSlot + sl * kSlotB;
-        const int8_t* src = base + w.b * s.sb + w.kvh * s.sh;
-        if (lane == 0) mbar_arrive_expect_tx(&st_full[sl], n * kD);
+        const int n = min(max(c.w.key.nv - v0, 0), C::kSlotKeys);
+        unsigned char* dst = slots + sl * C::kSlotB;
+        if (lane == 0) mbar_arrive_expect_tx(&full[sl], n * kD);
         __syncwarp();
         if (s.ss == kD) {  // rows back to back: the sinks' run and the window's
-          const int n0 = min(max(w.key.ns - v0, 0), n);
-          if (lane == 0 && n0 > 0) bulk_g2s(dst, src + static_cast<int64_t>(v0) * kD, n0 * kD, &st_full[sl]);
+          const int n0 = min(max(c.w.key.ns - v0, 0), n);
+          if (lane == 0 && n0 > 0) bulk_g2s(dst, src + static_cast<int64_t>(v0) * kD, n0 * kD, &full[sl]);
           if (lane == 0 && n > n0)
-            bulk_g2s(dst + n0 * kD, src + static_cast<int64_t>(v0 + n0 + w.key.sh) * kD,
-                     (n - n0) * kD, &st_full[sl]);
+            bulk_g2s(dst + n0 * kD, src + static_cast<int64_t>(v0 + n0 + c.w.key.sh) * kD,
+                     (n - n0) * kD, &full[sl]);
         } else {
           for (int i = lane; i < n; i += 32) {
             const int v = v0 + i;
-            const int64_t key = v < w.key.ns ? v : v + w.key.sh;
-            bulk_g2s(dst + i * kD, src + key * s.ss, kD, &st_full[sl]);
+            const int64_t key = v < c.w.key.ns ? v : v + c.w.key.sh;
+            bulk_g2s(dst + i * kD, src + key * s.ss, kD, &full[sl]);
           }
         }
       }
-    };
-    Cursor kc{walk, w, -1}, vc{walk, w, -1};
-    bool more = next_tile(kc);
-    if (more) copy_tile(kc, s.k);
-    while (ok && next_tile(vc)) {  // K 1, V 0, K 2, V 1, ..
-      more = more && next_tile(kc);
-      if (more) copy_tile(kc, s.k);
-      if (ok) copy_tile(vc, s.v);
     }
     if (!ok) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
     // no copy is in flight when the block ends
     for (int k = max(0, sc - C::kSlots); k < sc; ++k)
-      if (!mbar_wait(&st_full[k % C::kSlots], (k / C::kSlots) & 1))
+      if (!mbar_wait(&full[k % C::kSlots], (k / C::kSlots) & 1))
         report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
   } else if (warp == kCopyWarp + 1) {
     // ================= V scales into g_j and e_j, loaded a tile ahead

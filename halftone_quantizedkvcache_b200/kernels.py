@@ -947,10 +947,18 @@ def reset_ragged_status(device=None) -> None:
         t.zero_()
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
+    """A call's workspace, fresh from the allocator (the device's status word lends its type)."""
+    return _status_word(dev).new_empty((nbytes + 3) // 4)
+
+
 def _on_device(dev: torch.device):
     """Makes ``dev`` the current device for a launch, where it is not already."""
     if torch.cuda.current_device() == dev.index:
-        return contextlib.nullcontext()
+        return _NO_GUARD
     return torch.cuda.device(dev)
 
 
@@ -1015,8 +1023,14 @@ _PLANS_MAX = 4096
 
 
 def _sig(*tensors) -> tuple:
-    return tuple([(t.shape, t.stride(), t.dtype, t.get_device()) if t is not None else None
-                  for t in tensors])
+    sig = []
+    for t in tensors:
+        sig += (t.shape, t.stride(), t.dtype, t.get_device())
+    return tuple(sig)
+
+
+def _sig_opt(t) -> tuple:
+    return (None,) if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
 def _keep(key, plan):
@@ -1026,9 +1040,12 @@ def _keep(key, plan):
     return plan
 
 
+_OPTIONAL = ('q_lens', 'prefix_lens', 'n_new', 'pos_offset')
+
+
 def _tensors(what: str, **named) -> None:
     for n, t in named.items():
-        if not isinstance(t, torch.Tensor):
+        if not isinstance(t, torch.Tensor) and (t is not None or n not in _OPTIONAL):
             raise ValueError(f"{what}: {n} must be a tensor, got {type(t).__name__}")
 
 
@@ -1066,8 +1083,11 @@ def int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sin
     sequences grow.
     """
     what = "int8_window_decode_attn"
-    _tensors(what, q=q, k_i8=k_i8, k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens)
-    key = (what, window, sinks, _sig(q, k_i8, k_sc, v_i8, v_sc, lens))
+    try:
+        key = (what, window, sinks, _sig(q, k_i8, k_sc, v_i8, v_sc, lens))
+    except AttributeError:
+        _tensors(what, q=q, k_i8=k_i8, k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens)
+        raise
     plan = _plans.get(key)
     if plan is None:
         _cuda(q, f"{what} q")
@@ -1079,27 +1099,29 @@ def int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sin
         _attn_common(what, q, Hq, Hkv)
         w, sk = _window_args(what, window, sinks)
         _lens_ok(what, "lens", lens, B, dev)
-        qb = _aligned_q(qb)
         dt = _DT[qb.dtype]
+        ost = _lib.strides((Hq * D, D, 1), 3)
+        in_place = qb.stride(2) == 1 and all(s % 8 == 0 for s in qb.stride()[:2])
+        qst = _lib.strides(qb.stride(), 3) if in_place else ost
         with _on_device(dev):
             nb = _ws_size(what, dev, _lib.lib().hq_window_workspace_bytes(
                 dt, max(B, 1), Hq, Hkv, 0, cap, D, w, sk))
-        plan = _keep(key, (dev, (B, Hq, D), q.shape, dt, _lib.strides(qb.stride(), 3), st,
-                           _DT[k_sc.dtype], Hkv, cap, w, sk, nb, _lib.strides((Hq * D, D, 1), 3)))
-    dev, (B, Hq, D), shape, dt, qst, st, sdt, Hkv, cap, w, sk, nb, ost = plan
-    if q.data_ptr() % 16 or q.stride(-1) != 1 or any(s % 8 for s in q.stride()[:-1]):
-        q = _aligned_q(q)  # the strides of the copy are those of the plan's copy
+        plan = _keep(key, (dev, (B, Hq, D), q.shape, dt, qst, in_place,
+                           st, _DT[k_sc.dtype], Hkv, cap, w, sk, nb, ost))
+    dev, (B, Hq, D), shape, dt, qst, in_place, st, sdt, Hkv, cap, w, sk, nb, ost = plan
+    if not in_place or q.data_ptr() % 16:  # rows that the kernels cannot read in place
+        q, qst = q.clone(memory_format=torch.contiguous_format), ost
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
     with _on_device(dev):
         if out is None:
-            res = torch.empty(shape, dtype=q.dtype, device=dev)
+            res = q.new_empty(shape)
         else:
             _out_like(what, out, (B, Hq, D), q)
             res, ost = out, _lib.strides(out.stride(), 3)
         if B == 0:
             return res
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        ws = _scratch(dev, nb)
         rc = _lib.lib().hq_window_decode_int8(
             q.data_ptr(), dt, qst, k_i8.data_ptr(), v_i8.data_ptr(), st[0], k_sc.data_ptr(),
             v_sc.data_ptr(), sdt, st[1], st[2], lens.data_ptr(), B, Hq, Hkv, cap, D, w, sk, sm_scale,
@@ -1124,8 +1146,11 @@ def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, si
     they were in ``out``.  Queries at a position below 0 give zeros.
     """
     what = "int8_window_prefill_attn"
-    _tensors(what, q=q, k_i8=k_i8, k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens)
-    key = (what, window, sinks, _sig(q, k_i8, k_sc, v_i8, v_sc, lens, q_lens))
+    try:
+        key = (what, window, sinks, _sig(q, k_i8, k_sc, v_i8, v_sc, lens) + _sig_opt(q_lens))
+    except AttributeError:
+        _tensors(what, q=q, k_i8=k_i8, k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens, q_lens=q_lens)
+        raise
     plan = _plans.get(key)
     if plan is None:
         _cuda(q, f"{what} q")
@@ -1151,13 +1176,12 @@ def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, si
         sm_scale = 1.0 / math.sqrt(D)
     with _on_device(dev):
         if out is None:
-            make = torch.empty if q_lens is None else torch.zeros
-            out = make(shape, dtype=q.dtype, device=dev)
+            out = q.new_empty(shape) if q_lens is None else q.new_zeros(shape)
         else:
             _out_like(what, out, shape, q)
         if B == 0 or Sq == 0:
             return out
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        ws = _scratch(dev, nb)
         os_ = out.stride()
         rc = _lib.lib().hq_window_prefill_int8(
             q.data_ptr(), dt, _lib.strides(q.stride(), 4), k_i8.data_ptr(), v_i8.data_ptr(), st[0],
@@ -1184,9 +1208,13 @@ def int8_prefix_decode_attn(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_s
     are held; the output is the attention over both, and zeros where there is none.
     """
     what = "int8_prefix_decode_attn"
-    _tensors(what, q=q, pk_i8=pk_i8, pk_sc=pk_sc, pv_i8=pv_i8, pv_sc=pv_sc, k_i8=k_i8, k_sc=k_sc,
-             v_i8=v_i8, v_sc=v_sc, lens=lens)
-    key = (what, _sig(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_sc, lens, prefix_lens))
+    try:
+        key = (what, _sig(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_sc, lens)
+               + _sig_opt(prefix_lens))
+    except AttributeError:
+        _tensors(what, q=q, pk_i8=pk_i8, pk_sc=pk_sc, pv_i8=pv_i8, pv_sc=pv_sc, k_i8=k_i8,
+                 k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens, prefix_lens=prefix_lens)
+        raise
     plan = _plans.get(key)
     if plan is None:
         _cuda(q, f"{what} q")
@@ -1205,27 +1233,29 @@ def int8_prefix_decode_attn(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_s
             raise ValueError(f"{what}: {Hkv} kv heads, {pk_i8.shape[1]} in the prefix")
         _lens_ok(what, "lens", lens, B, dev)
         _lens_ok(what, "prefix_lens", prefix_lens, G, dev)
-        qb = _aligned_q(qb)
         dt = _DT[qb.dtype]
+        ost = _lib.strides((Hq * D, D, 1), 3)
+        in_place = qb.stride(2) == 1 and all(s % 8 == 0 for s in qb.stride()[:2])
+        qst = _lib.strides(qb.stride(), 3) if in_place else ost
         with _on_device(dev):
             nb = _ws_size(what, dev, _lib.lib().hq_prefix_decode_workspace_bytes(
                 dt, G, max(B, G), Hq, Hkv, P, cap, D))
-        plan = _keep(key, (dev, (B, Hq, D), q.shape, dt, _lib.strides(qb.stride(), 3), pst, st, G,
-                           P, _DT[k_sc.dtype], Hkv, cap, nb, _lib.strides((Hq * D, D, 1), 3)))
-    dev, (B, Hq, D), shape, dt, qst, pst, st, G, P, sdt, Hkv, cap, nb, ost = plan
-    if q.data_ptr() % 16 or q.stride(-1) != 1 or any(s % 8 for s in q.stride()[:-1]):
-        q = _aligned_q(q)  # the strides of the copy are those of the plan's copy
+        plan = _keep(key, (dev, (B, Hq, D), q.shape, dt, qst, in_place, pst, st, G,
+                           P, _DT[k_sc.dtype], Hkv, cap, nb, ost))
+    dev, (B, Hq, D), shape, dt, qst, in_place, pst, st, G, P, sdt, Hkv, cap, nb, ost = plan
+    if not in_place or q.data_ptr() % 16:  # rows that the kernels cannot read in place
+        q, qst = q.clone(memory_format=torch.contiguous_format), ost
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
     with _on_device(dev):
         if out is None:
-            res = torch.empty(shape, dtype=q.dtype, device=dev)
+            res = q.new_empty(shape)
         else:
             _out_like(what, out, (B, Hq, D), q)
             res, ost = out, _lib.strides(out.stride(), 3)
         if B == 0:
             return res
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        ws = _scratch(dev, nb)
         rc = _lib.lib().hq_prefix_decode_int8(
             q.data_ptr(), dt, qst, pk_i8.data_ptr(), pv_i8.data_ptr(), pst[0], pk_sc.data_ptr(),
             pv_sc.data_ptr(), pst[1], pst[2],
@@ -1294,10 +1324,14 @@ def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache
     fit its capacity writes nothing and sets ``ragged_status()``.
     """
     what = "rope_append_kv"
-    _tensors(what, q=q, k_new=k_new, v_new=v_new, inv_freq=inv_freq, k_cache=k_cache,
-             v_cache=v_cache, k_sc=k_sc, v_sc_cache=v_sc_cache, lens=lens)
-    key = (what, _sig(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache, lens, n_new,
-                      pos_offset))
+    try:
+        key = (what, _sig(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache, lens)
+               + _sig_opt(n_new) + _sig_opt(pos_offset))
+    except AttributeError:
+        _tensors(what, q=q, k_new=k_new, v_new=v_new, inv_freq=inv_freq, k_cache=k_cache,
+                 v_cache=v_cache, k_sc=k_sc, v_sc_cache=v_sc_cache, lens=lens, n_new=n_new,
+                 pos_offset=pos_offset)
+        raise
     plan = _plans.get(key)
     if plan is None:
         for t, n in ((q, "q"), (k_new, "k_new"), (v_new, "v_new"), (inv_freq, "inv_freq"),
@@ -1347,7 +1381,7 @@ def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache
                          "aligned rows")
     q, k_new, v_new = _aligned_q(q), _aligned_q(k_new), _aligned_q(v_new)
     with _on_device(dev):
-        res = q_out if q_out is not None else torch.empty(shape, dtype=q.dtype, device=dev)
+        res = q_out if q_out is not None else q.new_empty(shape)
         rc = _lib.lib().hq_rope_append_kv(
             q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), dt, _lib.strides(q.stride(), 4),
             _lib.strides(k_new.stride(), 4), _lib.strides(v_new.stride(), 4), B, Hq, Hkv, S, D,

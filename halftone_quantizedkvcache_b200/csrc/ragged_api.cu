@@ -209,6 +209,7 @@ inline int fill_seg(Seg& s, const int8_t* k, const int8_t* v, const int64_t* kvs
   if (cap > 0 && (!k || !v || !ksc || !vsc)) return HQ_ERR_INVALID_ARGUMENT;
   if (!kvs || !kss || !vss || cap < 0 || nb < 0 || units < 0 || window < 0 || sinks < 0)
     return HQ_ERR_INVALID_ARGUMENT;
+  if (cap > 1 << 30) return HQ_ERR_UNSUPPORTED;  // key numbers and windows are ints
   if (!aligned(k, 16) || !aligned(v, 16) || kvs[0] % 16 || kvs[1] % 16 || kvs[2] % 16)
     return HQ_ERR_INVALID_ARGUMENT;
   s.k = k;

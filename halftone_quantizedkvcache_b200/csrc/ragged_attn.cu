@@ -815,7 +815,9 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
       if (!mbar_wait(&full[k % C::kSlots], (k / C::kSlots) & 1))
         report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
   } else if (warp == kCopyWarp + 1) {
-    // ================= V scales into g_j and e_j, loaded a tile ahead
+    // ================= V scales into g_j and e_j, loaded a tile ahead.  A scale that is no
+    // number goes into e_j alone, where the mask comes after it: V's tile stays finite, and rows
+    // that do not see the key keep their sums.
     int gt = 0;
     bool ok = true;
     Cursor c{walk, w, -1};  // of the loads
@@ -852,7 +854,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
           const bool zero = vs[i] < kTinyScale;
           const float x = zero ? kTinyScale : vs[i];
           ev[32 * i + lane] = __log2f(x);
-          ev[kBN + 32 * i + lane] = __frcp_rn(x);
+          ev[kBN + 32 * i + lane] = x == x ? __frcp_rn(x) : 1.0f;
           gb[slot * kBN + 32 * i + lane] = zero ? 0u : 0x3c003c00u;
         }
       } else {
@@ -862,7 +864,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           ex[i] = vs[i] < kTinyScale ? -60 : static_cast<int>(__float_as_uint(vs[i]) >> 23 & 255) - 127;
-          top = max(top, vs[i] < kTinyScale ? -1000 : ex[i]);
+          top = max(top, vs[i] < kTinyScale || !(vs[i] < INFINITY) ? -1000 : ex[i]);
         }
         if (first) {
           top = __reduce_max_sync(0xffffffffu, top);
@@ -871,16 +873,17 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           ex[i] -= E;
-          odd = odd || (vs[i] >= 0.0f && (ex[i] < -4 || ex[i] > 6 || vs[i] < kTinyScale));
+          odd = odd || !(vs[i] < INFINITY) || (vs[i] >= 0.0f && (ex[i] < -4 || ex[i] > 6 || vs[i] < kTinyScale));
         }
         any = __any_sync(0xffffffffu, odd);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int e = any ? min(max(ex[i], -100), 100) : 0;
-          ev[32 * i + lane] = static_cast<float>(e);
+          const bool zero = vs[i] < kTinyScale || !(vs[i] < INFINITY);
+          ev[32 * i + lane] = vs[i] < INFINITY ? static_cast<float>(e) : NAN;
           ev[kBN + 32 * i + lane] = pow2i(-e);
           // (two factors: the exponent of their product may leave float32's)
-          const float gj = vs[i] < kTinyScale ? 0.0f : vs[i] * pow2i(-E) * pow2i(-e);
+          const float gj = zero ? 0.0f : vs[i] * pow2i(-E) * pow2i(-e);
           gb[slot * kBN + 32 * i + lane] = pack_h2(gj, gj);
         }
       }

@@ -1382,6 +1382,8 @@ def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache
     q, k_new, v_new = _aligned_q(q), _aligned_q(k_new), _aligned_q(v_new)
     with _on_device(dev):
         res = q_out if q_out is not None else q.new_empty(shape)
+        if B == 0 or S == 0:
+            return res
         rc = _lib.lib().hq_rope_append_kv(
             q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), dt, _lib.strides(q.stride(), 4),
             _lib.strides(k_new.stride(), 4), _lib.strides(v_new.stride(), 4), B, Hq, Hkv, S, D,

@@ -25,23 +25,32 @@
 //
 // Work.  Row r of a unit (kv head, sequence or group) is q head kvh * n_rep + r % n_rep of
 // query r / n_rep; 128 rows sit on the 128 lanes of tensor memory.  A block has two groups of
-// softmax warps, S buffers and O accumulators: for more than 128 rows the groups hold two row
-// tiles that share every key tile, else (ALT) one row tile whose key tiles they take in turn,
-// each with a softmax state of its own, joined at the end.  Keys that no row of the block can
-// see are never read: a block's keys are numbered v = 0 .. nv - 1, the sinks first, then the window's
-// run, and cut into tiles of 128.  Decode kernels (STREAM) lay the tiles of all units in
-// one line and give each block an equal run of it, whatever the lengths; a unit cut by a
-// block border leaves partial states (m, l, O) that combine_kernel joins.  Prefill blocks
-// take one row tile each (split over a few blocks when there are few).
+// softmax warps, each with two S buffers of 64 keys and one O accumulator: for more than 128 rows
+// the groups hold two row tiles that share every key tile and step through its halves, else (ALT)
+// one row tile, and each group takes one half of every key tile with a softmax state of its own,
+// joined at the end.  Keys that no row of the block can see are never read: a block's keys are
+// numbered v = 0 .. nv - 1, the sinks first, then the window's run, and cut into tiles of 128.
+// Decode kernels (STREAM) lay the tiles of all units in one line and give each block an equal run
+// of it, whatever the lengths; a unit cut by a block border leaves partial states (m, l, O) that
+// combine_kernel joins.  Prefill blocks take one row tile each (split over a few blocks when there
+// are few).
 //
-// Roles of a block (one per SM): softmax warps (2 x 4, one thread per row; they also form q'),
-// 8 warps that turn staged codes into float16 with byte permutes and store them in
-// the 128-byte-swizzled layouts the MMA reads, one warp that fills the staging ring with bulk
-// copies (64 keys of K or V per slot), one that reads the V scales, and one that issues the
-// tcgen05.mma products: S = Q K^T into tensor memory, O += P V with P read from tensor
-// memory, where it overwrites the S it came from.  mbarriers order the roles; every wait is
-// bounded.  (Codes loaded into registers and converted from there took 4000 cycles a tile:
-// the proxy fence before each hand-over waited for the loads of the next tile.)
+// Roles of a block (one per SM, 20 warps): softmax warps (2 x 4, one thread per row; they also
+// form q', 16 lanes a row), 4 warps that turn staged K codes into float16 with byte permutes and
+// store them in the 128-byte-swizzled layout the MMA reads and 4 that do so for V, two that fill
+// the staging rings with bulk copies, one that reads the V scales, and one that issues the
+// tcgen05.mma products: S = Q K^T into tensor memory, O += P V with P read from tensor memory,
+// where it overwrites the S it came from.  mbarriers order the roles; every wait is bounded.
+//
+// Measured (bf16, 16 q heads over 8 kv heads unless noted): causal chunks of 2 x 8192 under a
+// window of 2048, 387 us = 625 TFLOP/s, 0.38 of the measured bf16 rate; 64 sequences over 32768
+// shared keys 55 us = 313 TFLOP/s, 1240 GB/s of codes.  What bounds it is the softmax warps'
+// instruction latency: a step of 64 keys takes some 2000 cycles a warp, of which the exponentials
+// alone need 512; tensor pipe 33 % busy, issue slots 55 %, exp2 unit 33 %.  What it replaced, same
+// sizes: one S buffer of 128 keys a group, so that the softmax waited for P V and the next S in
+// turn, 436 us; operands of the products moved into uniform registers one by one under a branch
+// (80 cycles a product), 487; codes loaded into registers and converted from there, 4000 cycles a
+// tile, since the proxy fence before each hand-over waited for the loads of the next tile.
 #include <type_traits>
 
 #include "ragged_common.cuh"

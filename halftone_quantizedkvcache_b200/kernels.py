@@ -950,11 +950,6 @@ def reset_ragged_status(device=None) -> None:
 _NO_GUARD = contextlib.nullcontext()
 
 
-def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
-    """A call's workspace, fresh from the allocator (the device's status word lends its type)."""
-    return _status_word(dev).new_empty((nbytes + 3) // 4)
-
-
 def _on_device(dev: torch.device):
     """Makes ``dev`` the current device for a launch, where it is not already."""
     if torch.cuda.current_device() == dev.index:
@@ -1018,19 +1013,17 @@ def _window_args(what: str, window, sinks) -> tuple:
 # What a call's shapes, strides, types and devices lead to (checked arguments, C stride arrays,
 # scratch sizes), kept per combination: a decode step makes the same call for every layer and
 # token.  Nothing is kept by the tensors themselves.
+# (Written out where a call has its tensors in hand: a decode step's kernels take a few
+# microseconds, and so does every avoidable line here.)
 _plans: dict = {}
 _PLANS_MAX = 4096
 
 
-def _sig(*tensors) -> tuple:
-    sig = []
-    for t in tensors:
-        sig += (t.shape, t.stride(), t.dtype, t.get_device())
-    return tuple(sig)
+_NONE = (None,)
 
 
 def _sig_opt(t) -> tuple:
-    return (None,) if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+    return _NONE if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
 def _keep(key, plan):
@@ -1049,9 +1042,16 @@ def _tensors(what: str, **named) -> None:
             raise ValueError(f"{what}: {n} must be a tensor, got {type(t).__name__}")
 
 
-def _aligned_q(q: torch.Tensor) -> torch.Tensor:
-    """q with contiguous, 16-byte aligned rows (a copy where it has none)."""
-    return q if _rows_ok(q) else q.clone(memory_format=torch.contiguous_format)
+def _rows_strided(t: torch.Tensor) -> bool:
+    """[..., D] whose strides keep rows contiguous and 16-byte aligned, given an aligned base."""
+    es = t.element_size()
+    st = t.stride()
+    return st[-1] == 1 and all((x * es) % 16 == 0 for x in st[:-1])
+
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous, 16-byte aligned rows (a copy where it has none)."""
+    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _attn_common(what, q, Hq, Hkv) -> None:
@@ -1084,7 +1084,11 @@ def int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sin
     """
     what = "int8_window_decode_attn"
     try:
-        key = (what, window, sinks, _sig(q, k_i8, k_sc, v_i8, v_sc, lens))
+        key = (what, window, sinks, q.shape, q.stride(), q.dtype, q.get_device(), k_i8.shape,
+               k_i8.stride(), k_i8.dtype, k_i8.get_device(), k_sc.shape, k_sc.stride(), k_sc.dtype,
+               k_sc.get_device(), v_i8.shape, v_i8.stride(), v_i8.dtype, v_i8.get_device(),
+               v_sc.shape, v_sc.stride(), v_sc.dtype, v_sc.get_device(), lens.shape, lens.stride(),
+               lens.dtype, lens.get_device())
     except AttributeError:
         _tensors(what, q=q, k_i8=k_i8, k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens)
         raise
@@ -1106,30 +1110,35 @@ def int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sin
         with _on_device(dev):
             nb = _ws_size(what, dev, _lib.lib().hq_window_workspace_bytes(
                 dt, max(B, 1), Hq, Hkv, 0, cap, D, w, sk))
-        plan = _keep(key, (dev, (B, Hq, D), q.shape, dt, qst, in_place,
-                           st, _DT[k_sc.dtype], Hkv, cap, w, sk, nb, ost))
-    dev, (B, Hq, D), shape, dt, qst, in_place, st, sdt, Hkv, cap, w, sk, nb, ost = plan
-    if not in_place or q.data_ptr() % 16:  # rows that the kernels cannot read in place
+        plan = _keep(key, (dev, (B, Hq, D), q.shape, in_place and q.is_contiguous(), dt, qst, in_place,
+                           st, _DT[k_sc.dtype], Hkv, cap, w, sk, nb, (nb + 3) // 4, ost,
+                           1.0 / math.sqrt(D), _lib.lib().hq_window_decode_int8))
+    (dev, (B, Hq, D), shape, dense, dt, qst, in_place, (kst, kss, vss), sdt, Hkv, cap, w, sk, nb,
+     nw, ost, default_scale, fn) = plan
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, window=window, sinks=sinks,
+                                           sm_scale=sm_scale, q_quant=q_quant, out=out)
+    qp = q.data_ptr()
+    if not in_place or qp % 16:  # rows that the kernels cannot read in place
         q, qst = q.clone(memory_format=torch.contiguous_format), ost
-    if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(D)
-    with _on_device(dev):
-        if out is None:
-            res = q.new_empty(shape)
-        else:
-            _out_like(what, out, (B, Hq, D), q)
-            res, ost = out, _lib.strides(out.stride(), 3)
-        if B == 0:
-            return res
-        ws = _scratch(dev, nb)
-        rc = _lib.lib().hq_window_decode_int8(
-            q.data_ptr(), dt, qst, k_i8.data_ptr(), v_i8.data_ptr(), st[0], k_sc.data_ptr(),
-            v_sc.data_ptr(), sdt, st[1], st[2], lens.data_ptr(), B, Hq, Hkv, cap, D, w, sk, sm_scale,
-            1 if q_quant else 0, res.data_ptr(), ost, ws.data_ptr(), nb,
-            _status_word(dev).data_ptr(), _stream(dev))
+        qp = q.data_ptr()
+    if out is None:
+        out = torch.empty_like(q) if dense else q.new_empty(shape)
+    else:
+        _out_like(what, out, (B, Hq, D), q)
+        ost = _lib.strides(out.stride(), 3)
+    if B == 0:
+        return out
+    status = _status_word(dev)
+    ws = status.new_empty(nw)
+    rc = fn(qp, dt, qst, k_i8.data_ptr(), v_i8.data_ptr(), kst, k_sc.data_ptr(), v_sc.data_ptr(), sdt,
+            kss, vss, lens.data_ptr(), B, Hq, Hkv, cap, D, w, sk,
+            default_scale if sm_scale is None else sm_scale, 1 if q_quant else 0, out.data_ptr(), ost,
+            ws.data_ptr(), nb, status.data_ptr(), _stream(dev))
     if rc:
         check(rc, "hq_window_decode_int8")
-    return res
+    return out
 
 
 def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sinks=0,
@@ -1147,7 +1156,12 @@ def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, si
     """
     what = "int8_window_prefill_attn"
     try:
-        key = (what, window, sinks, _sig(q, k_i8, k_sc, v_i8, v_sc, lens) + _sig_opt(q_lens))
+        key = (what, window, sinks, q.shape, q.stride(), q.dtype, q.get_device(), k_i8.shape,
+               k_i8.stride(), k_i8.dtype, k_i8.get_device(), k_sc.shape, k_sc.stride(), k_sc.dtype,
+               k_sc.get_device(), v_i8.shape, v_i8.stride(), v_i8.dtype, v_i8.get_device(),
+               v_sc.shape, v_sc.stride(), v_sc.dtype, v_sc.get_device(), lens.shape, lens.stride(),
+               lens.dtype, lens.get_device())
+        key += _sig_opt(q_lens)
     except AttributeError:
         _tensors(what, q=q, k_i8=k_i8, k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens, q_lens=q_lens)
         raise
@@ -1168,28 +1182,37 @@ def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, si
         with _on_device(dev):
             nb = _ws_size(what, dev, _lib.lib().hq_window_workspace_bytes(
                 dt, max(B, 1), Hq, Hkv, max(Sq, 1), cap, D, w, sk))
-        plan = _keep(key, (dev, (B, Sq, Hq, D), dt, st, _DT[k_sc.dtype], Hkv, cap, w, sk, nb))
-    dev, shape, dt, st, sdt, Hkv, cap, w, sk, nb = plan
+        in_place = _rows_strided(q)
+        cst = _lib.strides((Hq * Sq * D, Sq * D, D, 1), 4)
+        plan = _keep(key, (dev, (B, Sq, Hq, D), dt, _lib.strides(q.stride(), 4) if in_place else cst,
+                           in_place, cst, st, _DT[k_sc.dtype], Hkv, cap, w, sk, nb, (nb + 3) // 4,
+                           _lib.strides((Sq * Hq * D, D, Hq * D, 1), 4), 1.0 / math.sqrt(D),
+                           _lib.lib().hq_window_prefill_int8))
+    (dev, shape, dt, qst, in_place, cst, (kst, kss, vss), sdt, Hkv, cap, w, sk, nb, nw, ost,
+     default_scale, fn) = plan
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, window=window, sinks=sinks,
+                                            q_lens=q_lens, sm_scale=sm_scale, q_quant=q_quant, out=out)
     B, Sq, Hq, D = shape
-    q = _aligned_q(q)
-    if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(D)
-    with _on_device(dev):
-        if out is None:
-            out = q.new_empty(shape) if q_lens is None else q.new_zeros(shape)
-        else:
-            _out_like(what, out, shape, q)
-        if B == 0 or Sq == 0:
-            return out
-        ws = _scratch(dev, nb)
-        os_ = out.stride()
-        rc = _lib.lib().hq_window_prefill_int8(
-            q.data_ptr(), dt, _lib.strides(q.stride(), 4), k_i8.data_ptr(), v_i8.data_ptr(), st[0],
-            k_sc.data_ptr(), v_sc.data_ptr(), sdt, st[1], st[2], lens.data_ptr(),
-            q_lens.data_ptr() if q_lens is not None else None, B, Hq, Hkv, Sq, cap, D, w, sk,
-            sm_scale, 1 if q_quant else 0, out.data_ptr(),
-            _lib.strides((os_[0], os_[2], os_[1], os_[3]), 4), ws.data_ptr(), nb,
-            _status_word(dev).data_ptr(), _stream(dev))
+    qp = q.data_ptr()
+    if not in_place or qp % 16:  # rows that the kernels cannot read in place
+        q, qst = q.clone(memory_format=torch.contiguous_format), cst
+        qp = q.data_ptr()
+    if out is None:
+        out = q.new_empty(shape) if q_lens is None else q.new_zeros(shape)
+    else:
+        _out_like(what, out, shape, q)
+        o = out.stride()
+        ost = _lib.strides((o[0], o[2], o[1], o[3]), 4)
+    if B == 0 or Sq == 0:
+        return out
+    status = _status_word(dev)
+    ws = status.new_empty(nw)
+    rc = fn(qp, dt, qst, k_i8.data_ptr(), v_i8.data_ptr(), kst, k_sc.data_ptr(), v_sc.data_ptr(), sdt,
+            kss, vss, lens.data_ptr(), q_lens.data_ptr() if q_lens is not None else None, B, Hq, Hkv,
+            Sq, cap, D, w, sk, default_scale if sm_scale is None else sm_scale, 1 if q_quant else 0,
+            out.data_ptr(), ost, ws.data_ptr(), nb, status.data_ptr(), _stream(dev))
     if rc:
         check(rc, "hq_window_prefill_int8")
     return out
@@ -1209,8 +1232,15 @@ def int8_prefix_decode_attn(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_s
     """
     what = "int8_prefix_decode_attn"
     try:
-        key = (what, _sig(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_sc, lens)
-               + _sig_opt(prefix_lens))
+        key = (what, q.shape, q.stride(), q.dtype, q.get_device(), pk_i8.shape, pk_i8.stride(),
+               pk_i8.dtype, pk_i8.get_device(), pk_sc.shape, pk_sc.stride(), pk_sc.dtype,
+               pk_sc.get_device(), pv_i8.shape, pv_i8.stride(), pv_i8.dtype, pv_i8.get_device(),
+               pv_sc.shape, pv_sc.stride(), pv_sc.dtype, pv_sc.get_device(), k_i8.shape,
+               k_i8.stride(), k_i8.dtype, k_i8.get_device(), k_sc.shape, k_sc.stride(), k_sc.dtype,
+               k_sc.get_device(), v_i8.shape, v_i8.stride(), v_i8.dtype, v_i8.get_device(),
+               v_sc.shape, v_sc.stride(), v_sc.dtype, v_sc.get_device(), lens.shape, lens.stride(),
+               lens.dtype, lens.get_device())
+        key += _sig_opt(prefix_lens)
     except AttributeError:
         _tensors(what, q=q, pk_i8=pk_i8, pk_sc=pk_sc, pv_i8=pv_i8, pv_sc=pv_sc, k_i8=k_i8,
                  k_sc=k_sc, v_i8=v_i8, v_sc=v_sc, lens=lens, prefix_lens=prefix_lens)
@@ -1240,32 +1270,37 @@ def int8_prefix_decode_attn(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_s
         with _on_device(dev):
             nb = _ws_size(what, dev, _lib.lib().hq_prefix_decode_workspace_bytes(
                 dt, G, max(B, G), Hq, Hkv, P, cap, D))
-        plan = _keep(key, (dev, (B, Hq, D), q.shape, dt, qst, in_place, pst, st, G,
-                           P, _DT[k_sc.dtype], Hkv, cap, nb, ost))
-    dev, (B, Hq, D), shape, dt, qst, in_place, pst, st, G, P, sdt, Hkv, cap, nb, ost = plan
-    if not in_place or q.data_ptr() % 16:  # rows that the kernels cannot read in place
+        plan = _keep(key, (dev, (B, Hq, D), q.shape, in_place and q.is_contiguous(), dt, qst, in_place,
+                           pst, st, G, P, _DT[k_sc.dtype], Hkv, cap, nb, (nb + 3) // 4, ost,
+                           1.0 / math.sqrt(D), _lib.lib().hq_prefix_decode_int8))
+    (dev, (B, Hq, D), shape, dense, dt, qst, in_place, (pkst, pkss, pvss), (kst, kss, vss), G, P, sdt,
+     Hkv, cap, nb, nw, ost, default_scale, fn) = plan
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return int8_prefix_decode_attn(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_sc, lens,
+                                           prefix_lens=prefix_lens, sm_scale=sm_scale,
+                                           q_quant=q_quant, out=out)
+    qp = q.data_ptr()
+    if not in_place or qp % 16:  # rows that the kernels cannot read in place
         q, qst = q.clone(memory_format=torch.contiguous_format), ost
-    if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(D)
-    with _on_device(dev):
-        if out is None:
-            res = q.new_empty(shape)
-        else:
-            _out_like(what, out, (B, Hq, D), q)
-            res, ost = out, _lib.strides(out.stride(), 3)
-        if B == 0:
-            return res
-        ws = _scratch(dev, nb)
-        rc = _lib.lib().hq_prefix_decode_int8(
-            q.data_ptr(), dt, qst, pk_i8.data_ptr(), pv_i8.data_ptr(), pst[0], pk_sc.data_ptr(),
-            pv_sc.data_ptr(), pst[1], pst[2],
-            prefix_lens.data_ptr() if prefix_lens is not None else None, G, P, k_i8.data_ptr(),
-            v_i8.data_ptr(), st[0], k_sc.data_ptr(), v_sc.data_ptr(), st[1], st[2],
-            lens.data_ptr(), cap, sdt, B, Hq, Hkv, D, sm_scale, 1 if q_quant else 0,
-            res.data_ptr(), ost, ws.data_ptr(), nb, _status_word(dev).data_ptr(), _stream(dev))
+        qp = q.data_ptr()
+    if out is None:
+        out = torch.empty_like(q) if dense else q.new_empty(shape)
+    else:
+        _out_like(what, out, (B, Hq, D), q)
+        ost = _lib.strides(out.stride(), 3)
+    if B == 0:
+        return out
+    status = _status_word(dev)
+    ws = status.new_empty(nw)
+    rc = fn(qp, dt, qst, pk_i8.data_ptr(), pv_i8.data_ptr(), pkst, pk_sc.data_ptr(), pv_sc.data_ptr(),
+            pkss, pvss, prefix_lens.data_ptr() if prefix_lens is not None else None, G, P,
+            k_i8.data_ptr(), v_i8.data_ptr(), kst, k_sc.data_ptr(), v_sc.data_ptr(), kss, vss,
+            lens.data_ptr(), cap, sdt, B, Hq, Hkv, D, default_scale if sm_scale is None else sm_scale,
+            1 if q_quant else 0, out.data_ptr(), ost, ws.data_ptr(), nb, status.data_ptr(), _stream(dev))
     if rc:
         check(rc, "hq_prefix_decode_int8")
-    return res
+    return out
 
 
 def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, *, scaling: str | None = None,
@@ -1325,8 +1360,16 @@ def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache
     """
     what = "rope_append_kv"
     try:
-        key = (what, _sig(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache, lens)
-               + _sig_opt(n_new) + _sig_opt(pos_offset))
+        key = (what, q.shape, q.stride(), q.dtype, q.get_device(), k_new.shape, k_new.stride(),
+               k_new.dtype, k_new.get_device(), v_new.shape, v_new.stride(), v_new.dtype,
+               v_new.get_device(), inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
+               inv_freq.get_device(), k_cache.shape, k_cache.stride(), k_cache.dtype,
+               k_cache.get_device(), v_cache.shape, v_cache.stride(), v_cache.dtype,
+               v_cache.get_device(), k_sc.shape, k_sc.stride(), k_sc.dtype, k_sc.get_device(),
+               v_sc_cache.shape, v_sc_cache.stride(), v_sc_cache.dtype, v_sc_cache.get_device(),
+               lens.shape, lens.stride(), lens.dtype, lens.get_device())
+        key += _sig_opt(n_new)
+        key += _sig_opt(pos_offset)
     except AttributeError:
         _tensors(what, q=q, k_new=k_new, v_new=v_new, inv_freq=inv_freq, k_cache=k_cache,
                  v_cache=v_cache, k_sc=k_sc, v_sc_cache=v_sc_cache, lens=lens, n_new=n_new,
@@ -1371,28 +1414,40 @@ def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache
         _lens_ok(what, "lens", lens, B, dev)
         _lens_ok(what, "n_new", n_new, B, dev)
         _lens_ok(what, "pos_offset", pos_offset, B, dev)
-        plan = _keep(key, (dev, (B, Hq, S, D), dt, Hkv, 2 * inv_freq.numel(), _DT[k_sc.dtype], kst,
-                           _lib.strides(cst[:3], 3), _lib.strides(v_sc_cache.stride()[:3], 3), cap))
-    dev, shape, dt, Hkv, rot, sdt, kst, cst, vst, cap = plan
+        in_place = _rows_strided(q) and _rows_strided(k_new) and _rows_strided(v_new)
+        plan = _keep(key, (dev, (B, Hq, S, D), in_place and q.is_contiguous(), dt, in_place,
+                           *[_lib.strides(x.stride(), 4) for x in (q, k_new, v_new)], Hkv,
+                           2 * inv_freq.numel(), _DT[k_sc.dtype], kst, _lib.strides(cst[:3], 3),
+                           _lib.strides(v_sc_cache.stride()[:3], 3), cap,
+                           _lib.strides((Hq * S * D, S * D, D, 1), 4), _lib.lib().hq_rope_append_kv))
+    (dev, shape, dense, dt, in_place, qst, knst, vnst, Hkv, rot, sdt, kst, cst, vst, cap, ost,
+     fn) = plan
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache, lens,
+                                  n_new=n_new, pos_offset=pos_offset, interleaved=interleaved,
+                                  factor=factor, q_out=q_out)
     B, Hq, S, D = shape
-    if q_out is not None and (q_out.shape != shape or q_out.dtype != q.dtype or
-                              q_out.device != dev or not _rows_ok(q_out)):
-        raise ValueError(f"{what}: q_out must have q's shape, dtype and device, with 16-byte "
-                         "aligned rows")
-    q, k_new, v_new = _aligned_q(q), _aligned_q(k_new), _aligned_q(v_new)
-    with _on_device(dev):
-        res = q_out if q_out is not None else q.new_empty(shape)
-        if B == 0 or S == 0:
-            return res
-        rc = _lib.lib().hq_rope_append_kv(
-            q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), dt, _lib.strides(q.stride(), 4),
-            _lib.strides(k_new.stride(), 4), _lib.strides(v_new.stride(), 4), B, Hq, Hkv, S, D,
-            inv_freq.data_ptr(), rot, 1 if interleaved else 0, factor, lens.data_ptr(),
+    qp, kp, vp = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr()
+    if not in_place or (qp | kp | vp) % 16:  # rows that the kernel cannot read in place
+        q, k_new, v_new = _aligned_rows(q), _aligned_rows(k_new), _aligned_rows(v_new)
+        qst, knst, vnst = (_lib.strides(x.stride(), 4) for x in (q, k_new, v_new))
+        qp, kp, vp = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr()
+    if q_out is None:
+        q_out = torch.empty_like(q) if dense else q.new_empty(shape)
+    else:
+        if q_out.shape != shape or q_out.dtype != q.dtype or q_out.device != dev or not _rows_ok(q_out):
+            raise ValueError(f"{what}: q_out must have q's shape, dtype and device, with 16-byte "
+                             "aligned rows")
+        ost = _lib.strides(q_out.stride(), 4)
+    if B == 0 or S == 0:
+        return q_out
+    rc = fn(qp, kp, vp, dt, qst, knst, vnst, B, Hq, Hkv, S, D, inv_freq.data_ptr(), rot,
+            1 if interleaved else 0, factor, lens.data_ptr(),
             n_new.data_ptr() if n_new is not None else None,
             pos_offset.data_ptr() if pos_offset is not None else None, k_sc.data_ptr(), sdt, kst,
             k_cache.data_ptr(), v_cache.data_ptr(), cst, v_sc_cache.data_ptr(), vst, cap,
-            res.data_ptr(), _lib.strides(res.stride(), 4), _status_word(dev).data_ptr(),
-            _stream(dev))
+            q_out.data_ptr(), ost, _status_word(dev).data_ptr(), _stream(dev))
     if rc:
         check(rc, "hq_rope_append_kv")
-    return res
+    return q_out

@@ -529,15 +529,10 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
                  2 * (w.b * s.qsb + uu * s.qsu + (w.kvh * p.nrep + rr - uu * p.nrep) * p.qsh);
         }
         float k8[8], km = 0.0f;
+        uint32_t kb[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float k = load_scale(s.ksc, w.b * s.kscb + w.kvh * s.ksch + (4 * lane + e) * s.kscd, p.s_dt) * p.qk_scale;
-          k8[e] = __shfl_sync(0xffffffffu, k, 2 * c);
-          k8[4 + e] = __shfl_sync(0xffffffffu, k, 2 * c + 1);
-          km = fmaxf(km, fabsf(k));
-        }
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
+        for (int e = 0; e < 4; ++e)
+          kb[e] = load_bits(s.ksc, w.b * s.kscb + w.kvh * s.ksch + (4 * lane + e) * s.kscd, p.s_dt);
         {
           constexpr int NX = kForm / 2;
           uint4 x[NX];
@@ -547,6 +542,15 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
             const uint64_t src = __shfl_sync(0xffffffffu, from, k);
             x[i] = fr0 + k < w.rows ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float k = scale_of(kb[e], p.s_dt) * p.qk_scale;
+            k8[e] = __shfl_sync(0xffffffffu, k, 2 * c);
+            k8[4 + e] = __shfl_sync(0xffffffffu, k, 2 * c + 1);
+            km = fmaxf(km, fabsf(k));
+          }
+#pragma unroll
+          for (int o = 16; o >= 1; o >>= 1) km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
 #pragma unroll 1
           for (int i0 = 0; i0 < NX; i0 += 2) {  // (rolled, the rows move up: straight code would run cold)
             uint4 y[2] = {x[0], x[1]};
@@ -830,7 +834,8 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     int gt = 0;
     bool ok = true;
     Cursor c{walk, w, -1};  // of the loads
-    float next[4];
+    uint32_t next[4];
+    const uint32_t minus_one = p.s_dt == HQ_DTYPE_F32 ? __float_as_uint(-1.0f) : 0xbc00u;
     auto load_next = [&]() -> bool {
       if (!next_tile(c)) return false;
       const Seg& s = p.seg;
@@ -839,7 +844,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
       for (int i = 0; i < 4; ++i) {
         const int v = c.t * kBN + 32 * i + lane;
         const int64_t key = v < c.w.key.ns ? v : v + c.w.key.sh;
-        next[i] = v < c.w.key.nv ? load_scale(s.vsc, vs0 + key * s.vscs, p.s_dt) : -1.0f;
+        next[i] = v < c.w.key.nv ? load_bits(s.vsc, vs0 + key * s.vscs, p.s_dt) : minus_one;
       }
       return true;
     };
@@ -848,7 +853,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     while (have) {
       float vs[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vs[i] = next[i];
+      for (int i = 0; i < 4; ++i) vs[i] = scale_of(next[i], p.s_dt);
       const bool first = c.t == c.w.t0;
       have = load_next();
       const int use = gt / C::kLvSlots, slot = gt % C::kLvSlots;

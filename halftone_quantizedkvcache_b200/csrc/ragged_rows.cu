@@ -13,7 +13,7 @@
 // is worked on, across the borders of sequences.  A tile inside one run of keys is one box per
 // side; the tile in which the sinks end and the window begins is put together from boxes of 8
 // keys.  (cp.async of 16 bytes a thread did both with one rule, but under load its issue held
-// the warps up for 2400 cycles a tile: 138 us against 108 at 64 sequences x 4096 keys.)
+// the warps up for 2400 cycles a tile: 138 us against 108 then at 64 sequences x 4096 keys.)
 #include "decode_common.cuh"
 #include "ragged_common.cuh"
 
@@ -84,14 +84,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   int lt = -1, issued = 0;
   bool more = true;
   int64_t vs0 = 0;
-  float vs_n[3][2] = {};  // V scales of this lane's own keys: this tile, the next two
+  uint32_t vs_n[3][2] = {};  // V scales of this lane's own keys: this tile, the next two
   // the next tile into stage `st` (nothing past the last), its V scales into the queue's end
   auto issue = [&](int st) {
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
       vs_n[0][rb] = vs_n[1][rb];
       vs_n[1][rb] = vs_n[2][rb];
-      vs_n[2][rb] = 0.0f;
+      vs_n[2][rb] = 0u;
     }
     if (more && ++lt >= lp.t1) {
       more = walk_next<128, true, 8>(lw, p, cum, lp);
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int rb = 0; rb < 2; ++rb) {
       const int v = v0 + warp * 32 + rb * 16 + g + 8 * (t4 & 1);
       if (v < lp.key.nv && !lp.key.padding(v))
-        vs_n[2][rb] = load_scale(s.vsc, vs0 + static_cast<int64_t>(lp.key.key(v)) * s.vscs, p.s_dt);
+        vs_n[2][rb] = load_bits(s.vsc, vs0 + static_cast<int64_t>(lp.key.key(v)) * s.vscs, p.s_dt);
     }
   };
 #pragma unroll 1
@@ -138,18 +138,23 @@ __global__ void __launch_bounds__(kThreads, 2)
     // ---- q' and its digits; thread owns channel d
     const int d = tid, rows = w.rows;
     {
-      const float ks = load_scale(s.ksc, w.b * s.kscb + w.kvh * s.ksch + d * s.kscd, p.s_dt);
-      float qv[NR];
+      // (bits first, values after them: all loads are in flight together)
+      const uint32_t ksb = load_bits(s.ksc, w.b * s.kscb + w.kvh * s.ksch + d * s.kscd, p.s_dt);
+      unsigned short qb[NR];
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        qv[r] = 0.0f;
+        qb[r] = 0;
         if (r < rows) {
           const int u = r / p.nrep, h = w.kvh * p.nrep + r - u * p.nrep;
-          const int64_t at = w.b * s.qsb + u * s.qsu + h * p.qsh + d;
-          qv[r] = p.q_dt == HQ_DTYPE_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[at])
-                                          : __half2float(static_cast<const __half*>(p.q)[at]);
+          qb[r] = static_cast<const unsigned short*>(p.q)[w.b * s.qsb + u * s.qsu + h * p.qsh + d];
         }
       }
+      const float ks = scale_of(ksb, p.s_dt);
+      float qv[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        qv[r] = p.q_dt == HQ_DTYPE_BF16 ? __uint_as_float(static_cast<uint32_t>(qb[r]) << 16)
+                                        : __half2float(__ushort_as_half(qb[r]));
       if (p.q_quant) {  // per-token int8 fake quantization, rounded back to the model dtype
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       ++done;
       issue((st + 2) % kStagesM);
-      const float vsf[2] = {vs_n[0][0], vs_n[0][1]};
+      const float vsf[2] = {scale_of(vs_n[0][0], p.s_dt), scale_of(vs_n[0][1], p.s_dt)};
       const int base = t * kBN + warp * 32, lim = w.key.nv;
       const uint32_t kt = smem_u32(ring + st * 2 * kTileB);
       const uint32_t vt = kt + kTileB;

@@ -551,25 +551,30 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
           }
 #pragma unroll
           for (int o = 16; o >= 1; o >>= 1) km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
+          // the rows' largest |q|: straight code, whose shuffles overlap
+          float am[NX];
+#pragma unroll
+          for (int i = 0; i < NX; ++i)
+            am[i] = absmax_of_x2<DT>(absmax_x2<DT>(absmax_x2<DT>(x[i].x, x[i].y), absmax_x2<DT>(x[i].z, x[i].w)));
+#pragma unroll
+          for (int o = 8; o >= 1; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < NX; ++i) am[i] = fmaxf(am[i], __shfl_xor_sync(0xffffffffu, am[i], o));
 #pragma unroll 1
           for (int i0 = 0; i0 < NX; i0 += 2) {  // (rolled, the rows move up: straight code would run cold)
             uint4 y[2] = {x[0], x[1]};
-            float am[2];
+            const float a2[2] = {am[0], am[1]};
 #pragma unroll
-            for (int k = 0; k < NX - 2; ++k) x[k] = x[k + 2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              am[i] = absmax_of_x2<DT>(absmax_x2<DT>(absmax_x2<DT>(y[i].x, y[i].y), absmax_x2<DT>(y[i].z, y[i].w)));
-#pragma unroll
-            for (int o = 8; o >= 1; o >>= 1)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) am[i] = fmaxf(am[i], __shfl_xor_sync(0xffffffffu, am[i], o));
+            for (int k = 0; k < NX - 2; ++k) {
+              x[k] = x[k + 2];
+              am[k] = am[k + 2];
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              if (p.q_quant) y[i] = fake_quant<DT>(y[i], am[i]);
+              if (p.q_quant) y[i] = fake_quant<DT>(y[i], a2[i]);
               // 2^ex brings the bound max |q| max k_scale to [2^13, 2^14): the row's largest |q'|
               // may lie some powers of two below, of which float16 has 14 to spare
-              const int ex = min(max(13 - (static_cast<int>(__float_as_uint(am[i] * km) >> 23) - 127), -100), 100);
+              const int ex = min(max(13 - (static_cast<int>(__float_as_uint(a2[i] * km) >> 23) - 127), -100), 100);
               const float mul = pow2i(ex);
               float f[8];
               Vec16<DT>::unpack(y[i], f);
@@ -611,8 +616,8 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
       for (int i = 0; ok && i < steps; ++i, ++cnt) {
         const int t = ALT ? i : i >> 1, half = ALT ? grp : i & 1;
         const int slot = (gt0 + t) % C::kLvSlots, buf = cnt & 1;
-        ok = wait_bar(&lv_full[slot], ((gt0 + t) / C::kLvSlots) & 1) &&
-             wait_bar(&s_full[2 * grp + buf], (cnt >> 1) & 1);
+        if (ALT || half == 0) ok = wait_bar(&lv_full[slot], ((gt0 + t) / C::kLvSlots) & 1);
+        ok = ok && wait_bar(&s_full[2 * grp + buf], (cnt >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();

@@ -162,8 +162,20 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-// 64 columns of this thread's lane
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+// 32 or 64 columns of this thread's lane
+__device__ __forceinline__ void tmem_cols(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+      "%29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_cols(uint32_t taddr, uint32_t (&r)[64]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
@@ -268,38 +280,47 @@ __device__ __forceinline__ void move_max(float mx, uint32_t o_addr, bool first, 
   rescale(o_addr, a);
 }
 
-// One step of one row, 64 keys held in registers: the running maximum, then P = 2^(t - m) over S,
-// and l.  EXP: t = s fac + e_j with e_j from ev[j] and 2^-e_j from ev[128 + j], else t = s fac.
+// One step of one row, 64 keys: the running maximum, then P = 2^(t - m) over S, and l.  CH: the
+// scores held at a time.  All 64 in registers save the second read, 32 save half of the code, which
+// runs cold in short blocks: 2 x 8192 rows took 381 us with 64 and 407 with 32, one prompt of 512
+// 14.0 and 13.3, 33 sequences over three prefixes 43.9 and 40.3, so one row tile a block takes 32.
+// EXP: t = s fac + e_j with e_j from ev[j] and 2^-e_j from ev[128 + j], else t = s fac.
 // mask: some row of the warp does not see all of the keys.
-template <bool EXP>
+template <bool EXP, int CH>
 __device__ __forceinline__ void softmax_step(uint32_t s_addr, uint32_t o_addr, const float* ev,
                                              float fac, int v0, const RowLim& lim, bool mask,
                                              bool first, uint64_t* pv_bar, uint32_t pv_par,
                                              float& m, float& l, bool& ok) {
-  uint32_t s[kBS];
-  tmem_ld64(s_addr, s);
-  if constexpr (EXP) {
+  uint32_t s[CH];
+  auto scores = [&](int c) {  // t (EXP) or s, -inf where unseen
+    tmem_cols(s_addr + c, s);
+    if constexpr (EXP) {
 #pragma unroll
-    for (int e = 0; e < kBS; e += 4) {
-      const float4 e4 = *reinterpret_cast<const float4*>(ev + e);
-      s[e] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e]), fac, e4.x));
-      s[e + 1] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e + 1]), fac, e4.y));
-      s[e + 2] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e + 2]), fac, e4.z));
-      s[e + 3] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e + 3]), fac, e4.w));
+      for (int e = 0; e < CH; e += 4) {
+        const float4 e4 = *reinterpret_cast<const float4*>(ev + c + e);
+        s[e] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e]), fac, e4.x));
+        s[e + 1] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e + 1]), fac, e4.y));
+        s[e + 2] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e + 2]), fac, e4.z));
+        s[e + 3] = __float_as_uint(__fmaf_rn(__uint_as_float(s[e + 3]), fac, e4.w));
+      }
     }
-  }
-  if (mask) {
-    const uint32_t seen0 = lim.bits(v0), seen1 = lim.bits(v0 + 32);
+    if (mask) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      s[e] = seen0 & (1u << e) ? s[e] : 0xff800000u;
-      s[e + 32] = seen1 & (1u << e) ? s[e + 32] : 0xff800000u;
+      for (int h = 0; h < CH; h += 32) {
+        const uint32_t seen = lim.bits(v0 + c + h);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[h + e] = seen & (1u << e) ? s[h + e] : 0xff800000u;
+      }
     }
-  }
+  };
   float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int c = 0; c < kBS; c += CH) {
+    scores(c);
 #pragma unroll
-  for (int e = 0; e < kBS; e += 2)
-    x[(e >> 1) & 3] = fmaxf(x[(e >> 1) & 3], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+    for (int e = 0; e < CH; e += 2)
+      x[(e >> 1) & 3] = fmaxf(x[(e >> 1) & 3], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+  }
   float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
   if constexpr (!EXP) mx *= fac;
   move_max(mx, o_addr, first, pv_bar, pv_par, m, l, ok);
@@ -307,17 +328,18 @@ __device__ __forceinline__ void softmax_step(uint32_t s_addr, uint32_t o_addr, c
   const float nb = m == -INFINITY ? 0.0f : -m;
   // (scalar: packed pairs cost more moves than they save)
   float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int c = 0; c < kBS; c += 16) {
+#pragma unroll 1
+  for (int c = 0; c < kBS; c += CH) {
+    if (CH < kBS) scores(c);
     uint32_t w[8];
 #pragma unroll
-    for (int e = c; e < c + 16; e += 4) {
+    for (int e = 0; e < CH; e += 4) {
       float t[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         t[i] = ex2_ftz(EXP ? __uint_as_float(s[e + i]) + nb : __fmaf_rn(__uint_as_float(s[e + i]), fac, nb));
       if constexpr (EXP) {
-        const float4 r4 = *reinterpret_cast<const float4*>(ev + kBN + e);
+        const float4 r4 = *reinterpret_cast<const float4*>(ev + kBN + c + e);
         ls[0] = __fmaf_rn(t[0], r4.x, ls[0]);
         ls[1] = __fmaf_rn(t[1], r4.y, ls[1]);
         ls[2] = __fmaf_rn(t[2], r4.z, ls[2]);
@@ -326,10 +348,10 @@ __device__ __forceinline__ void softmax_step(uint32_t s_addr, uint32_t o_addr, c
 #pragma unroll
         for (int i = 0; i < 4; ++i) ls[i] += t[i];
       }
-      w[(e - c) / 2] = pack_h2(t[0], t[1]);
-      w[(e - c) / 2 + 1] = pack_h2(t[2], t[3]);
+      w[e / 2 % 8] = pack_h2(t[0], t[1]);
+      w[e / 2 % 8 + 1] = pack_h2(t[2], t[3]);
+      if (e % 16 == 12) tmem_st8(s_addr + (c + e - 12) / 2, w);  // over S columns that have been read
     }
-    tmem_st8(s_addr + c / 2, w);
   }
   l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
   tmem_wait_st();
@@ -633,7 +655,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
           if (!LO && ti.x != 0.0f)
             softmax_step_any(s_addr + kBS * buf, o_addr, ev, fac, v0, lim, i == 0, pvb, pvp, m, l, ok);
           else
-            softmax_step<LO>(s_addr + kBS * buf, o_addr, ev, fac, v0, lim, mask, i == 0, pvb, pvp, m, l, ok);
+            softmax_step<LO, ALT ? 32 : 64>(s_addr + kBS * buf, o_addr, ev, fac, v0, lim, mask, i == 0, pvb, pvp, m, l, ok);
         }
         if (!ok) break;
         tc_fence_before();

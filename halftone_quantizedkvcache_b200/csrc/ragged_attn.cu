@@ -490,7 +490,9 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
                  v_base = smem_u32(smem + C::kOffV);
   Walk walk = walk_start<MT, STREAM, 1>(p, cum);
   auto next_piece = [&](Walk& k, Piece& to) { return walk_next<MT, STREAM, 1>(k, p, cum, to); };
+  // the first piece, for all roles at once: a copy of this code in each would run cold in each
   Piece w{};
+  const bool any = next_piece(walk, w);
   // the block's tiles one after the other, whatever the piece
   struct Cursor {
     Walk k;
@@ -532,7 +534,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
       ok = wait_bar(soft_bar, syncs++ & 1) && ok;
       __syncwarp();
     };
-    for (; ok && next_piece(walk, w); ++pc) {
+    for (bool go = any; ok && go; go = next_piece(walk, w), ++pc) {
       const int n_tiles = w.t1 - w.t0;
       float m = -INFINITY, l = 0.0f, fac = 0.0f, vscale = 1.0f;
       const Seg& s = p.seg;
@@ -761,7 +763,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
       constexpr int NI = C::kSlotKeys / 8;
       int sl = 0, gt = 0;
       uint32_t sl_par = 0;
-      Cursor c{walk, w, -1};
+      Cursor c{walk, w, w.t0 - 1};
       for (; ok && next_tile(c); ++gt) {
         const int st = gt % kStages, use = gt / kStages;
         if (use > 0) ok = wait_bar(&empty[st], (use - 1) & 1);
@@ -820,7 +822,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     unsigned char* slots = smem + C::kOffSlot + is_v * C::kSlots * C::kSlotB;
     int sc = 0;
     bool ok = true;
-    Cursor c{walk, w, -1};
+    Cursor c{walk, w, w.t0 - 1};
     while (ok && next_tile(c)) {
       const Seg& s = p.seg;
       const int8_t* src = (is_v ? s.v : s.k) + c.w.b * s.sb + c.w.kvh * s.sh;
@@ -860,7 +862,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     // that do not see the key keep their sums.
     int gt = 0;
     bool ok = true;
-    Cursor c{walk, w, -1};  // of the loads
+    Cursor c{walk, w, w.t0 - 1};  // of the loads
     uint32_t next[4];
     const uint32_t minus_one = p.s_dt == HQ_DTYPE_F32 ? __float_as_uint(-1.0f) : 0xbc00u;
     auto load_next = [&]() -> bool {
@@ -994,7 +996,7 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
       using G1 = std::integral_constant<int, 1>;
       // (all of the tensor memory is this block's: its columns count from 0)
       if (tmem != 0) ok = false;
-      for (; ok && next_piece(walk, w);) {
+      for (bool go = any; ok && go; go = next_piece(walk, w)) {
         const int n_tiles = w.t1 - w.t0, steps = ALT ? n_tiles : 2 * n_tiles;
         if (n_tiles <= 0) continue;
         const bool two = ALT || w.rows > 128;

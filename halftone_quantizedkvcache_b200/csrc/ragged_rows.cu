@@ -79,11 +79,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint64_t pol = l2_evict_first();
 
   // ---- the loads' cursor, two tiles ahead
+  Piece w{};
+  const bool any = walk_next<128, true, 8>(walk, p, cum, w);
   Walk lw = walk;
-  Piece lp{};
-  int lt = -1, issued = 0;
-  bool more = true;
-  int64_t vs0 = 0;
+  Piece lp = w;
+  int lt = w.t0 - 1, issued = 0;
+  bool more = any;
+  int64_t vs0 = lp.b * s.vscb + lp.kvh * s.vsch;
   uint32_t vs_n[3][2] = {};  // V scales of this lane's own keys: this tile, the next two
   // the next tile into stage `st` (nothing past the last), its V scales into the queue's end
   auto issue = [&](int st) {
@@ -133,8 +135,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   unsigned char* my_limb = plimb + warp * NT * 256;
   int done = 0;  // tiles worked on
   bool ok = true;
-  Piece w{};
-  while (ok && walk_next<128, true, 8>(walk, p, cum, w)) {
+  for (bool go = any; ok && go; go = walk_next<128, true, 8>(walk, p, cum, w)) {
     // ---- q' and its digits; thread owns channel d
     const int d = tid, rows = w.rows;
     {

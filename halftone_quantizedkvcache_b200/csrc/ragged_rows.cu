@@ -176,7 +176,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         qv[r] *= ks * p.qk_scale;
-        const float m = dec::warp_max(fabsf(qv[r]), 1);
+        // (a NaN must not get lost in the maximum)
+        const float m = dec::warp_max(qv[r] == qv[r] ? fabsf(qv[r]) : INFINITY, 1);
         if (lane == 0) red[warp][r] = m;
       }
       __syncthreads();
@@ -342,7 +343,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (grow) pmax[nt] = 2.0f * pm;
         }
         m_run[nt] = m_new;
-        l_run[nt] += pr[0] + pr[1];
+        // (a seen key's V scale that is no number would get lost in the digits: the sum carries it)
+        l_run[nt] += __fmaf_rn(0.0f, vsf[0], pr[0]) + __fmaf_rn(0.0f, vsf[1], pr[1]);
         const float inv_ps = pmax[nt] > 0.0f ? kLimbMax / pmax[nt] : 0.0f;
         unsigned char* dst = my_limb + nt * 256;
 #pragma unroll

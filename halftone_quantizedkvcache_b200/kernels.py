@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import contextlib
 import math
+import operator
 import threading
 
 import torch
@@ -1001,13 +1002,20 @@ def _out_like(what: str, out, shape, q: torch.Tensor) -> None:
         raise ValueError(f"{what}: out rows must be contiguous and 8-byte aligned")
 
 
+def _whole(what: str, window, sinks) -> tuple:
+    try:
+        return None if window is None else operator.index(window), operator.index(sinks)
+    except TypeError:
+        raise TypeError(f"{what}: window (or None) and sinks must be whole numbers") from None
+
+
 def _window_args(what: str, window, sinks) -> tuple:
-    w = 0 if window is None else int(window)
+    w = 0 if window is None else window
     if window is not None and w < 1 or w >= 1 << 30:
         raise ValueError(f"{what}: window must be None or 1 .. 2^30 - 1")
-    if not 0 <= int(sinks) < 1 << 30:
+    if not 0 <= sinks < 1 << 30:
         raise ValueError(f"{what}: sinks must be 0 .. 2^30 - 1")
-    return w, int(sinks)
+    return w, sinks
 
 
 # What a call's shapes, strides, types and devices lead to (checked arguments, C stride arrays,
@@ -1083,6 +1091,8 @@ def int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sin
     sequences grow.
     """
     what = "int8_window_decode_attn"
+    if type(window) is not int or type(sinks) is not int:
+        window, sinks = _whole(what, window, sinks)
     try:
         key = (what, window, sinks, q.shape, q.stride(), q.dtype, q.get_device(), k_i8.shape,
                k_i8.stride(), k_i8.dtype, k_i8.get_device(), k_sc.shape, k_sc.stride(), k_sc.dtype,
@@ -1155,6 +1165,8 @@ def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, si
     they were in ``out``.  Queries at a position below 0 give zeros.
     """
     what = "int8_window_prefill_attn"
+    if type(window) is not int or type(sinks) is not int:
+        window, sinks = _whole(what, window, sinks)
     try:
         key = (what, window, sinks, q.shape, q.stride(), q.dtype, q.get_device(), k_i8.shape,
                k_i8.stride(), k_i8.dtype, k_i8.get_device(), k_sc.shape, k_sc.stride(), k_sc.dtype,

@@ -221,6 +221,30 @@ def test_nan_query_row_keeps_to_itself():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("rep", [1, 2, 4, 8])
+def test_broken_values_that_are_seen(rep, dt):
+    """A NaN in one head's query spoils that row alone; a V scale that is no number, in sight,
+    spoils its sequence's rows of that kv head alone."""
+    g = torch.Generator(device="cuda").manual_seed(13)
+    cache = make_cache(g, 2, 2, 400, "f32")
+    q = torch.randn((2, 2 * rep, 1, D), generator=g, device="cuda").to(TDT[dt])
+    n = i32([400, 150])
+    want = kernels.int8_window_decode_attn(q, *cache, n, window=100, sinks=2)
+    q2 = q.clone()
+    q2[1, rep - 1, 0, 7] = float("nan")
+    got = kernels.int8_window_decode_attn(q2, *cache, n, window=100, sinks=2)
+    assert torch.isnan(got[1, rep - 1]).all()
+    got[1, rep - 1] = want[1, rep - 1]
+    assert torch.equal(got, want)
+    for bad in (float("nan"), float("inf")):
+        cache[3][0, 1, 350] = bad
+        got = kernels.int8_window_decode_attn(q, *cache, n, window=100, sinks=2)
+        assert not torch.isfinite(got[0, rep:]).any()
+        got[0, rep:] = want[0, rep:]
+        assert torch.equal(got, want)
+
+
 def test_empty_caches():
     q = torch.randn((2, 4, 1, D), device="cuda").to(torch.bfloat16)
     g = torch.Generator(device="cuda").manual_seed(8)
@@ -295,7 +319,8 @@ def test_refusals():
     odd = torch.zeros(k.numel() + 8, dtype=torch.int8, device="cuda")[8:].view_as(k)
     for call in (
             lambda: dec(q, *cache, n, window=0), lambda: dec(q, *cache, n, window=-1),
-            lambda: dec(q, *cache, n, sinks=-1), lambda: dec(q, *cache, n, window=1 << 30),
+            lambda: dec(q, *cache, n, sinks=-1), lambda: dec(q, *cache, n, window=2.5),
+            lambda: dec(q, *cache, n, sinks="2"), lambda: pre(q, *cache, n, window=1.0), lambda: dec(q, *cache, n, window=1 << 30),
             lambda: dec(q, *cache, n.long()), lambda: dec(q, *cache, n.cpu()),
             lambda: dec(q, *cache, i32([1])), lambda: dec(q.float(), *cache, n),
             lambda: dec(q[..., :64].contiguous(), k[..., :64].contiguous(), ksc[..., :64].contiguous(),

@@ -44,8 +44,9 @@ __device__ __forceinline__ Run split_run(const Source& s, int b, int u, int kvh,
           static_cast<int64_t>(p.rows_cap) * kPartRow};
 }
 
-// One block per output row (b, u, h): the pieces' common maximum (every warp finds it), then
-// their weighted sums, warp w taking pieces w, w + 4, .., a lane 4 channels.
+// One block per output row (b, u, h): warp w joins pieces w, w + 4, .., a lane 4 channels, under a
+// maximum of its own, then warp 0 the warps' sums.  (One round of loads: finding the common maximum
+// first took another.  A piece whose sums are no number has a maximum of -inf and passes them on.)
 constexpr int kJoinWarps = 4;
 template <int NSRC, bool STREAM>
 __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_constant__ Source s0,
@@ -67,45 +68,34 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_c
     if (u >= nq) return;
     run[0] = split_run(s0, b, u, kvh, hr);
   }
-  float M = -INFINITY;
+  float M = -INFINITY, L = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto join = [&](float m, float l, const float4& o) {
+    const float top = fmaxf(M, m);
+    const float f0 = M == -INFINITY ? 0.0f : exp2f(M - top), f1 = m == -INFINITY ? 0.0f : exp2f(m - top);
+    M = top;
+    L = L * f0 + l * f1;
+    acc.x = acc.x * f0 + o.x * f1;
+    acc.y = acc.y * f0 + o.y * f1;
+    acc.z = acc.z * f0 + o.z * f1;
+    acc.w = acc.w * f0 + o.w * f1;
+  };
 #pragma unroll
   for (int k = 0; k < NSRC; ++k)
-#pragma unroll 1
-    for (int i = lane; i < run[k].n; i += 32) M = fmaxf(M, run[k].at[i * run[k].step]);
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float L = 0.0f;
-  if (M != -INFINITY) {
-#pragma unroll
-    for (int k = 0; k < NSRC; ++k)
 #pragma unroll 4
-      for (int i = warp; i < run[k].n; i += kJoinWarps) {
-        const float* x = run[k].at + i * run[k].step;
-        const float2 ml = *reinterpret_cast<const float2*>(x);
-        const float4 o = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
-        const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
-        L += f * ml.y;
-        acc.x += f * o.x;
-        acc.y += f * o.y;
-        acc.z += f * o.z;
-        acc.w += f * o.w;
-      }
-  }
+    for (int i = warp; i < run[k].n; i += kJoinWarps) {
+      const float* x = run[k].at + i * run[k].step;
+      const float2 ml = *reinterpret_cast<const float2*>(x);
+      join(ml.x, ml.y, *reinterpret_cast<const float4*>(x + 4 + 4 * lane));
+    }
   sum[warp][lane] = acc;
-  if (lane == 0) sum[warp][32].x = L;
+  if (lane == 0) sum[warp][32] = make_float4(M, L, 0.0f, 0.0f);
   __syncthreads();
   if (warp) return;
-  L = 0.0f;
-  acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) {
-    const float4 o = sum[i][lane];
-    L += sum[i][32].x;
-    acc.x += o.x;
-    acc.y += o.y;
-    acc.z += o.z;
-    acc.w += o.w;
+  for (int i = 1; i < kJoinWarps; ++i) {
+    const float4 ml = sum[i][32];
+    join(ml.x, ml.y, sum[i][lane]);
   }
   const float inv = L <= 0.0f ? 0.0f : 1.0f / L;  // (a NaN stays)
   store4(out_row(p, b, u, h), p.q_dt, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);

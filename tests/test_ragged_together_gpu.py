@@ -245,6 +245,25 @@ def test_broken_values_that_are_seen(rep, dt):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("rep", [2, 8])
+def test_nan_query_over_many_blocks(rep):
+    """The same where a row's keys are cut over many blocks and joined."""
+    g = torch.Generator(device="cuda").manual_seed(14)
+    cache = make_cache(g, 1, 1, 9000, "f16")
+    q = torch.randn((1, rep, 7, D), generator=g, device="cuda").to(torch.bfloat16)
+    n = i32([9000])
+    for call in (lambda x: kernels.int8_window_decode_attn(x[:, :, -1:], *cache, n)[:, :, 0][None],
+                 lambda x: kernels.int8_window_prefill_attn(x, *cache, n),
+                 lambda x: kernels.int8_prefix_decode_attn(x[:, :, -1:], *cache, *cache, n)[:, :, 0][None]):
+        want = call(q)
+        q2 = q.clone()
+        q2[0, 1, -1, 100] = float("nan")
+        got = call(q2)
+        assert torch.isnan(got[0, -1, 1]).all()
+        got[0, -1, 1] = want[0, -1, 1]
+        assert torch.equal(got, want)
+
+
 def test_empty_caches():
     q = torch.randn((2, 4, 1, D), device="cuda").to(torch.bfloat16)
     g = torch.Generator(device="cuda").manual_seed(8)

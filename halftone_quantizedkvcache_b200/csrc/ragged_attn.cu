@@ -42,15 +42,16 @@
 // tcgen05.mma products: S = Q K^T into tensor memory, O += P V with P read from tensor memory,
 // where it overwrites the S it came from.  mbarriers order the roles; every wait is bounded.
 //
-// Measured (bf16, 16 q heads over 8 kv heads unless noted): causal chunks of 2 x 8192 under a
-// window of 2048, 387 us = 625 TFLOP/s, 0.38 of the measured bf16 rate; 64 sequences over 32768
-// shared keys 55 us = 313 TFLOP/s, 1240 GB/s of codes.  What bounds it is the softmax warps'
-// instruction latency: a step of 64 keys takes some 2000 cycles a warp, of which the exponentials
-// alone need 512; tensor pipe 33 % busy, issue slots 55 %, exp2 unit 33 %.  What it replaced, same
-// sizes: one S buffer of 128 keys a group, so that the softmax waited for P V and the next S in
-// turn, 436 us; operands of the products moved into uniform registers one by one under a branch
-// (80 cycles a product), 487; codes loaded into registers and converted from there, 4000 cycles a
-// tile, since the proxy fence before each hand-over waited for the loads of the next tile.
+// Measured (bf16, 16 q heads over 8 kv heads): causal chunks of 2 x 8192 under a window of 2048,
+// 359 us = 675 TFLOP/s, 0.41 of the measured bf16 rate; 64 sequences over 32768 shared keys 51 us
+// = 337 TFLOP/s, 1340 GB/s of codes.  What bounds it is the softmax warps' instruction latency: a
+// step of 64 keys takes some 2000 cycles a warp, of which the exponentials alone need 512; tensor
+// pipe 36 % busy, issue slots 58 %, exp2 unit 36 %; and a fifth of a block is its start and end.
+// What it replaced, same sizes: one S buffer of 128 keys a group, so that the softmax waited for
+// P V and the next S in turn, 436 us; operands of the products moved into uniform registers one by
+// one under a branch (80 cycles a product), 487; a first-piece search in every role (cold code
+// each time), 380; codes loaded into registers and converted from there, 4000 cycles a tile, since
+// the proxy fence before each hand-over waited for the loads of the next tile.
 #include <type_traits>
 
 #include "ragged_common.cuh"

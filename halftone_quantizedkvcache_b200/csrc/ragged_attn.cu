@@ -43,8 +43,8 @@
 // where it overwrites the S it came from.  mbarriers order the roles; every wait is bounded.
 //
 // Measured (bf16, 16 q heads over 8 kv heads): causal chunks of 2 x 8192 under a window of 2048,
-// 359 us = 675 TFLOP/s, 0.41 of the measured bf16 rate; 64 sequences over 32768 shared keys 51 us
-// = 337 TFLOP/s, 1340 GB/s of codes.  What bounds it is the softmax warps' instruction latency: a
+// 359 us = 675 TFLOP/s, 0.41 of the measured bf16 rate; 64 sequences over 32768 shared keys 48 us
+// = 355 TFLOP/s, 1410 GB/s of codes.  What bounds it is the softmax warps' instruction latency: a
 // step of 64 keys takes some 2000 cycles a warp, of which the exponentials alone need 512; tensor
 // pipe 36 % busy, issue slots 58 %, exp2 unit 36 %; and a fifth of a block is its start and end.
 // What it replaced, same sizes: one S buffer of 128 keys a group, so that the softmax waited for
@@ -61,6 +61,8 @@ namespace hq {
 namespace rag {
 using namespace tc;
 
+// registers a thread after the split (softmax warps, the others)
+constexpr int kSoftRegs = 120, kOtherRegs = 80;
 constexpr int kSoft = 256;                // softmax threads: two groups of 128
 constexpr int kConvThreads = 256;
 constexpr int kBS = 64;                   // keys of a softmax step: half a tile
@@ -509,10 +511,10 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
     return true;
   };
 
-  // registers: 640 threads x 96 at launch = 61,440 = 256 x 120 + 384 x 80
-  if (warp >= kSoft / 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  // (the shares' sum is what the block was launched with, 640 x 96: launch() checks it)
+  if (warp >= kSoft / 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp < kSoft / 32) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     // ================= softmax: one thread per row (ALT: and group)
     const int grp = warp >> 2, lr = tid & 127, r = ALT ? lr : tid;  // row of its tile, of the piece
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -776,25 +778,28 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
           ok = wait_bar(&sfull[sl], sl_par);
           if (!ok) break;
           const unsigned char* src = slots + sl * C::kSlotB + row * kD + 8 * c8;
-          uint2 x[NI];
-          uint32_t g2[NI];
+#pragma unroll 1
+          for (int i0 = 0; i0 < NI; i0 += 4) {  // (all of a slot at once: 5 % slower, more code)
+            uint2 x[4];
+            uint32_t g2[4];
 #pragma unroll
-          for (int i = 0; i < NI; ++i) {
-            x[i] = *reinterpret_cast<const uint2*>(src + i * 8 * kD);
-            if constexpr (V) g2[i] = g[k0 + row + 8 * i];  // V rows times their g
-          }
-#pragma unroll
-          for (int i = 0; i < NI; ++i) {
-            uint4 y;
-            codes_to_h2(x[i].x, y.x, y.y);
-            codes_to_h2(x[i].y, y.z, y.w);
-            if constexpr (V) {
-              asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.x) : "r"(y.x), "r"(g2[i]));
-              asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.y) : "r"(y.y), "r"(g2[i]));
-              asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.z) : "r"(y.z), "r"(g2[i]));
-              asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.w) : "r"(y.w), "r"(g2[i]));
+            for (int i = 0; i < 4; ++i) {
+              x[i] = *reinterpret_cast<const uint2*>(src + (i0 + i) * 8 * kD);
+              if constexpr (V) g2[i] = g[k0 + row + 8 * (i0 + i)];  // V rows times their g
             }
-            *reinterpret_cast<uint4*>(to + (k0 + 8 * i) * 128) = y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4 y;
+              codes_to_h2(x[i].x, y.x, y.y);
+              codes_to_h2(x[i].y, y.z, y.w);
+              if constexpr (V) {
+                asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.x) : "r"(y.x), "r"(g2[i]));
+                asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.y) : "r"(y.y), "r"(g2[i]));
+                asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.z) : "r"(y.z), "r"(g2[i]));
+                asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y.w) : "r"(y.w), "r"(g2[i]));
+              }
+              *reinterpret_cast<uint4*>(to + (k0 + 8 * (i0 + i)) * 128) = y;
+            }
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sempty[sl]);
@@ -1069,6 +1074,13 @@ int launch(const Params& p, dim3 grid, cudaStream_t st) {
   using C = Cfg<ALT, LO>;
   static std::atomic<uint64_t> ready{0};
   auto kern = ragged_kernel<ALT, LO, STREAM>;
+  // an increase beyond the registers of the launch would wait for ever
+  static const bool fits = [&] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kern) == cudaSuccess &&
+           a.numRegs * C::kThreads >= kSoft * kSoftRegs + (C::kThreads - kSoft) * kOtherRegs;
+  }();
+  if (!fits) return HQ_ERR_UNSUPPORTED;
   const int rc = set_smem(kern, C::smem(STREAM ? kMaxEntries : 0), ready);
   if (rc != HQ_OK) return rc;
   return launch_after(kern, grid, C::kThreads, C::smem(STREAM ? p.seg.nb : 0), st, p);

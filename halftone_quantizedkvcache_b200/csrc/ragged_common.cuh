@@ -57,10 +57,6 @@ struct Params {
   int after;                              // launched beside the kernel before: ends after it
 };
 
-__device__ __forceinline__ float load_scale(const void* p, int64_t i, int dt) {
-  return dt == HQ_DTYPE_F16 ? __half2float(static_cast<const __half*>(p)[i])
-                            : static_cast<const float*>(p)[i];
-}
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);

@@ -129,33 +129,43 @@ __global__ void __launch_bounds__(kThreads, 2)
         vs_n[2][rb] = load_bits(s.vsc, vs0 + static_cast<int64_t>(lp.key.key(v)) * s.vscs, p.s_dt);
     }
   };
-#pragma unroll 1
-  for (int i = 0; i < 2; ++i) issue(i);
 
   unsigned char* my_limb = plimb + warp * NT * 256;
   int done = 0;  // tiles worked on
   bool ok = true;
-  for (bool go = any; ok && go; go = walk_next<128, true, 8>(walk, p, cum, w)) {
-    // ---- q' and its digits; thread owns channel d
-    const int d = tid, rows = w.rows;
-    {
-      // (bits first, values after them: all loads are in flight together)
-      const uint32_t ksb = load_bits(s.ksc, w.b * s.kscb + w.kvh * s.ksch + d * s.kscd, p.s_dt);
-      unsigned short qb[NR];
+  // a piece's q and K scale of this thread's channel, loaded a piece ahead (bits: a conversion
+  // would wait for them)
+  const int d = tid;
+  uint32_t ksb = 0;
+  unsigned short qb[NR] = {};
+  auto load_q = [&](const Piece& of) {
+    ksb = load_bits(s.ksc, of.b * s.kscb + of.kvh * s.ksch + d * s.kscd, p.s_dt);
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        qb[r] = 0;
-        if (r < rows) {
-          const int u = r / p.nrep, h = w.kvh * p.nrep + r - u * p.nrep;
-          qb[r] = static_cast<const unsigned short*>(p.q)[w.b * s.qsb + u * s.qsu + h * p.qsh + d];
-        }
+    for (int r = 0; r < NR; ++r) {
+      qb[r] = 0;
+      if (r < of.rows) {
+        const int u = r / p.nrep, h = of.kvh * p.nrep + r - u * p.nrep;
+        qb[r] = static_cast<const unsigned short*>(p.q)[of.b * s.qsb + u * s.qsu + h * p.qsh + d];
       }
+    }
+  };
+  if (any) load_q(w);
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) issue(i);
+  Piece next{};
+  bool go = any;
+  for (; ok && go; w = next) {
+    // ---- q' and its digits; thread owns channel d
+    const int rows = w.rows;
+    {
       const float ks = scale_of(ksb, p.s_dt);
       float qv[NR];
 #pragma unroll
       for (int r = 0; r < NR; ++r)
         qv[r] = p.q_dt == HQ_DTYPE_BF16 ? __uint_as_float(static_cast<uint32_t>(qb[r]) << 16)
                                         : __half2float(__ushort_as_half(qb[r]));
+      go = walk_next<128, true, 8>(walk, p, cum, next);
+      if (go) load_q(next);
       if (p.q_quant) {  // per-token int8 fake quantization, rounded back to the model dtype
 #pragma unroll
         for (int r = 0; r < NR; ++r) {

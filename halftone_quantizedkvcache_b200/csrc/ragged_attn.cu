@@ -87,7 +87,7 @@ struct Cfg {
   static constexpr int kOffE = kOffSlot + 2 * kSlots * kSlotB;     // [slot][e_j, 2^-e_j][128]
   static constexpr int kOffG = kOffE + kLvSlots * 2 * kBN * 4;     // [slot][128] g_j, float16 twice
   static constexpr int kOffInfo = kOffG + kLvSlots * kBN * 4;      // [slot]{any e_j, 2^E}
-  static constexpr int kOffFac = kOffInfo + 16 * ((kLvSlots + 1) / 2);  // [row] what q' was divided by
+  static constexpr int kOffFac = kOffInfo + 16 * ((kLvSlots + 1) / 2);  // [row] undoes q's power of two
   static constexpr int kOffRow = kOffFac + kRowTiles * 128 * 4;     // ALT: [2][128] the groups' (m, l)
   static constexpr int kOffBar = kOffRow + (ALT ? 2 * kBN * 8 : 0);
   static constexpr int kBars = 1 + 4 * kStages + 4 * kSlots + 2 * kLvSlots + 4 + 4 + 4 + 1 + 1 + 1;

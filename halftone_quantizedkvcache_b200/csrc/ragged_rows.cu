@@ -14,6 +14,11 @@
 // side; the tile in which the sinks end and the window begins is put together from boxes of 8
 // keys.  (cp.async of 16 bytes a thread did both with one rule, but under load its issue held
 // the warps up for 2400 cycles a tile: 138 us against 108 then at 64 sequences x 4096 keys.)
+//
+// Measured at 64 sequences x 4096 keys (bf16, 16 q heads over 8 kv heads): 96 us = 5.6 TB/s, 0.86
+// of the measured rate.  Short runs pay for their starts: 64 sequences of 64 to 1024 tokens, 34 us =
+// 2.1 TB/s, of which a block's start, the joins of its three pieces and their joining kernel take
+// two thirds.
 #include "decode_common.cuh"
 #include "ragged_common.cuh"
 

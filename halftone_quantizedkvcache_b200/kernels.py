@@ -926,7 +926,9 @@ def _status_word(dev: torch.device) -> torch.Tensor:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first ragged-batch call on a device must run outside a CUDA "
                                "graph capture: run the same call once before capturing it")
-        t = _ragged_status[dev.index] = torch.zeros(1, dtype=torch.int32, device=dev)
+        t = torch.zeros(1, dtype=torch.int32, device=dev)
+        torch.cuda.current_stream(dev).synchronize()  # it is zero before any other stream's call
+        _ragged_status[dev.index] = t
     return t
 
 
@@ -934,10 +936,13 @@ def ragged_status(device=None) -> int:
     """Status of the ragged-batch kernels (``int8_window_decode_attn``,
     ``int8_window_prefill_attn``, ``int8_prefix_decode_attn``, ``rope_append_kv``) on a device
     since it was last reset: 0, or the first error found on the device (a wait that gave up, a
-    sequence whose new tokens did not fit).  Synchronises."""
+    sequence whose new tokens did not fit).  Synchronises the device."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     t = _ragged_status.get(dev.index if dev.index is not None else torch.cuda.current_device())
-    return int(t.item()) if t is not None else 0
+    if t is None:
+        return 0
+    torch.cuda.synchronize(t.device)
+    return int(t.item())
 
 
 def reset_ragged_status(device=None) -> None:
@@ -1020,13 +1025,10 @@ def _window_args(what: str, window, sinks) -> tuple:
 
 # What a call's shapes, strides, types and devices lead to (checked arguments, C stride arrays,
 # scratch sizes), kept per combination: a decode step makes the same call for every layer and
-# token.  Nothing is kept by the tensors themselves.
-# (Written out where a call has its tensors in hand: a decode step's kernels take a few
-# microseconds, and so does every avoidable line here.)
+# token.  Nothing is kept by the tensors themselves.  (The keys are written out in each call: a
+# decode step's kernels take ten microseconds, and a helper over lists would take three of them.)
 _plans: dict = {}
 _PLANS_MAX = 4096
-
-
 _NONE = (None,)
 
 

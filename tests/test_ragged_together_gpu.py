@@ -383,3 +383,12 @@ def test_no_room_is_reported_and_reset():
     assert (cache[2][0] == 0).all() and (cache[3][1, :, 12:] > 0).all()
     kernels.reset_ragged_status()
     assert kernels.ragged_status() == 0
+    # an error found on another stream is seen, too
+    side = torch.cuda.Stream()
+    full = i32([14, 14])
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kernels.rope_append_kv(q, kn, vn, inv, cache[0], cache[2], cache[1], cache[3], full)
+    assert kernels.ragged_status() == _lib.ERR_INVALID_ARGUMENT
+    kernels.reset_ragged_status()
+    assert kernels.ragged_status() == 0

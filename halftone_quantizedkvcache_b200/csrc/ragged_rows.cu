@@ -355,7 +355,10 @@ __global__ void __launch_bounds__(kThreads, 2)
                 o_acc[nt][j][pi][1] *= alpha;
               }
           }
-          if (grow) pmax[nt] = 2.0f * pm;
+          // The digits' scale is chosen afresh where the maximum moves as well: what the earlier
+          // keys needed is 2^(m - m_new) of itself now, and a scale left at it would round the
+          // new leader away where its V scale is much smaller.
+          if (rescale || grow) pmax[nt] = 2.0f * pm;
         }
         m_run[nt] = m_new;
         // (a seen key's V scale that is no number would get lost in the digits: the sum carries it)

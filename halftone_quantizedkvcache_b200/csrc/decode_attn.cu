@@ -864,7 +864,10 @@ __global__ void __launch_bounds__(kThreads, 2) decode_mma_kernel(
               o_acc[nt][j][pi][1] *= alpha;
             }
         }
-        if (grow) pmax[nt] = 2.0f * pm;
+        // The scale of the p' limbs is chosen afresh, too, where the maximum has moved and this
+        // tile's largest is far below it: what the earlier tokens needed has shrunk with the
+        // maximum, and would round a leader with a much smaller V scale away.
+        if (grow || (rescale && pm < 0.0625f * pmax[nt])) pmax[nt] = 2.0f * pm;
       }
       m_run[nt] = m_new;
       l_run[nt] += pr[0] + pr[1];

@@ -347,7 +347,8 @@ __global__ void __launch_bounds__(kThreads, 2) kblock_mma_kernel(
               o_acc[nt][j][pi][1] *= alpha;
             }
         }
-        if (grow) pmax[nt] = 2.0f * pm;
+        // (chosen afresh, too, where the maximum has moved and little of the scale is still needed)
+        if (grow || (rescale && pm < 0.0625f * pmax[nt])) pmax[nt] = 2.0f * pm;
       }
       m_run[nt] = m_new;
       l_run[nt] += pr[0] + pr[1];

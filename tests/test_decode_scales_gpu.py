@@ -65,3 +65,20 @@ def test_a_late_key_with_small_values_takes_the_lead(rep, dt, at, rise):
     check(kernels.int8_decode_attn(q, *cache, dynamic_tiles=True), cache, rep, dt, rise)
     n = torch.tensor([S], dtype=torch.int32, device="cuda")
     check(kernels.int8_decode_attn(q, *cache, seq_len=n), cache, rep, dt, rise)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("rep", [1, 2, 4])
+@pytest.mark.parametrize("at,rise", [(130, 40.0), (300, 40.0), (261, 60.0), (259, 30.0)])
+def test_the_same_in_the_block_wise_layout(rep, dt, at, rise):
+    cache = late_leader(at, rise)
+    k, ksc, v, vsc = cache
+    blocks = kernels.kblock_alloc(B, HKV, S, D, dtype=TDT[dt], v_scale_dtype=torch.float32)
+    blocks["k"].copy_(k)
+    blocks["k_scale"].copy_(ksc.expand(B, HKV, S // 128, D))
+    blocks["v"].copy_(v)
+    blocks["v_scale"].copy_(vsc[..., 0])
+    q = torch.ones((B, HKV * rep, D), device="cuda").to(TDT[dt])
+    check(kernels.kblock_decode(q, blocks, S), cache, rep, dt, rise)
+    n = torch.tensor([S], dtype=torch.int32, device="cuda")
+    check(kernels.kblock_decode(q, blocks, S, seq_len=n), cache, rep, dt, rise)

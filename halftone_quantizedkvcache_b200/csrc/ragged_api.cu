@@ -219,8 +219,9 @@ inline int fill_seg(Seg& s, const int8_t* k, const int8_t* v, const int64_t* kvs
   s.cap = cap;
   s.nb = nb;
   s.units = units;
-  s.window = window > 0 ? window : 1 << 30;
-  s.sinks = sinks;
+  // (all of a cache holds is seen at either bound, and sums of positions stay ints)
+  s.window = window > 0 ? std::min(window, 1 << 30) : 1 << 30;
+  s.sinks = std::min(sinks, cap);
   return HQ_OK;
 }
 

@@ -570,7 +570,8 @@ HQ_API int hq_kblock_dequant(const int8_t* k_cache, const int64_t kq_strides[3],
  *
  * hq_window_decode_int8 (B <= 1024): one query per sequence, the token at position
  *   lens[b] - 1, over keys j with j >= lens[b] - window or j < sinks (window 0:
- *   all keys).  lens[b] = 0 gives zeros.  q / out [B, Hq, D].
+ *   all keys; any int from 0 on may be given for both).  lens[b] = 0 gives
+ *   zeros.  q / out [B, Hq, D].
  * hq_window_prefill_int8: q [B, Hq, Sq, D], out logical [B, Hq, Sq, D]; the
  *   first q_lens[b] rows of sequence b are queries (q_lens NULL: all Sq), query
  *   i at position p = lens[b] - q_lens[b] + i, over keys j <= p with j > p -

@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from halftone_quantizedkvcache_b200 import kernels
-from test_ragged_gpu import D, TDT, check, ref_rows
+from halftone_quantizedkvcache_b200 import _lib, kernels
+from test_ragged_gpu import D, TDT, check, make_cache, ref_rows, window_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,54 @@ def test_a_late_key_with_small_values_takes_the_lead(rep, dt, at, rise):
             check(got[b, h * rep:(h + 1) * rep, 0], ref.expand(rep, D), tol.expand(rep, D) + step,
                   f"b={b} h={h}")
     assert kernels.ragged_status() == 0
+
+
+INT_MAX = 2 ** 31 - 1
+
+
+def c_window(q, cache, lens, window, sinks):
+    """The C entries of the windowed attention, whose window and sinks are any int: decode for
+    q [B,Hq,D], prefill for q [B,Hq,Sq,D] (output [B,Sq,Hq,D])."""
+    k, ksc, v, vsc = cache
+    B, Hkv, cap = k.shape[:3]
+    Hq, Sq = q.shape[1], q.shape[2] if q.dim() == 4 else 0
+    dt, st = kernels._DT[q.dtype], lambda t, n=3: _lib.strides(t.stride()[:n], n)
+    nb = _lib.lib().hq_window_workspace_bytes(dt, B, Hq, Hkv, Sq, cap, D, window, sinks)
+    ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kss, vss = _lib.strides((ksc.stride(0), ksc.stride(1), ksc.stride(3)), 3), st(vsc)
+    common = (st(k), ksc.data_ptr(), vsc.data_ptr(), kernels._DT[ksc.dtype], kss, vss, lens.data_ptr())
+    tail = (D, window, sinks, 1 / math.sqrt(D), 0)
+    stream = torch.cuda.current_stream().cuda_stream
+    if Sq:
+        out = torch.empty((B, Sq, Hq, D), dtype=q.dtype, device="cuda")
+        rc = _lib.lib().hq_window_prefill_int8(
+            q.data_ptr(), dt, st(q, 4), k.data_ptr(), v.data_ptr(), *common, None, B, Hq, Hkv, Sq, cap,
+            *tail, out.data_ptr(), st(out.transpose(1, 2), 4), ws.data_ptr(), nb, status.data_ptr(), stream)
+    else:
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device="cuda")
+        rc = _lib.lib().hq_window_decode_int8(
+            q.data_ptr(), dt, st(q), k.data_ptr(), v.data_ptr(), *common, B, Hq, Hkv, cap,
+            *tail, out.data_ptr(), st(out), ws.data_ptr(), nb, status.data_ptr(), stream)
+    assert rc == 0 and status.item() == 0
+    return out
+
+
+@pytest.mark.parametrize("rep", [2, 8])
+@pytest.mark.parametrize("window,sinks", [
+    (0, INT_MAX), (100, INT_MAX), (INT_MAX, 0), (INT_MAX, INT_MAX), (100, INT_MAX - 7),
+    (1 << 30, 1 << 30), ((1 << 30) + 1, (1 << 30) + 1)])
+def test_windows_and_sinks_up_to_the_largest_int(rep, window, sinks):
+    """All of these let every query see every key before it."""
+    g = torch.Generator(device="cuda").manual_seed(rep)
+    lens = [300, 0, 17]
+    cache = make_cache(g, 3, 2, 300, "f16")
+    q = torch.randn((3, 2 * rep, D), generator=g, device="cuda").to(torch.bfloat16)
+    got = c_window(q, cache, i32(lens), window, sinks)
+    ref, tol = window_ref(q[:, :, None], cache, lens, [1] * 3, None, 0, "bf16")
+    check(got, ref[:, 0], tol[:, 0], "decode")
+    # 40 queries each: those of the last two sequences begin before position 0
+    q = torch.randn((3, 2 * rep, 40, D), generator=g, device="cuda").to(torch.bfloat16)
+    got = c_window(q, cache, i32(lens), window, sinks)
+    ref, tol = window_ref(q, cache, lens, [40] * 3, None, 0, "bf16")
+    check(got, ref, tol, "prefill")

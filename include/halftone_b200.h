@@ -558,7 +558,8 @@ HQ_API int hq_kblock_dequant(const int8_t* k_cache, const int64_t kq_strides[3],
  * reference, whose batch has one length and whose attention sees all of it).
  * lens int32[B] in device memory holds the cached tokens of each sequence
  * (clamped to [0, S_max], S_max <= 2^30); what rows past it hold does not matter.
- * K and V may have any
+ * A cache (or prefix) of S_max (P_max) = 0 is not read: its codes and scales may
+ * be NULL.  K and V may have any
  * (b, h, s) strides that are multiples of 16 bytes, shared by both, with
  * 16-byte aligned bases.  V scales are zero or positive, finite float32 or
  * float16; a token whose V scale is below 2^-60 counts as zeros.  q is bf16 or

@@ -101,3 +101,34 @@ def test_windows_and_sinks_up_to_the_largest_int(rep, window, sinks):
     got = c_window(q, cache, i32(lens), window, sinks)
     ref, tol = window_ref(q, cache, lens, [40] * 3, None, 0, "bf16")
     check(got, ref, tol, "prefill")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("rep", [1, 2, 4, 8])
+def test_an_empty_cache_needs_no_pointers(rep, dt):
+    """Capacity 0, codes and scales NULL: zeros from every entry, and no read."""
+    L, B, Hkv, one = _lib.lib(), 3, 2, _lib.strides((D, D, 1), 3)
+    Hq, t = Hkv * rep, kernels._DT[TDT[dt]]
+    lens = i32([0, 5, 1])
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    rows = _lib.strides((D, D, D), 3)
+    none = (None, None, rows, None, None, kernels._DT[torch.float16], one, one)
+    q = torch.randn((B, Hq, 9, D), device="cuda").to(TDT[dt])
+    end = (ws.data_ptr(), ws.numel(), status.data_ptr(), stream)
+    st3, st4 = _lib.strides((Hq * D, D, 1), 3), _lib.strides((Hq * 9 * D, 9 * D, D, 1), 4)
+    out = torch.ones((B, Hq, D), dtype=TDT[dt], device="cuda")
+    assert L.hq_window_decode_int8(q.data_ptr(), t, st3, *none, lens.data_ptr(), B, Hq, Hkv, 0, D, 7, 1,
+                                   0.1, 1, out.data_ptr(), st3, *end) == 0
+    assert (out == 0).all()
+    wide = torch.ones_like(q)
+    assert L.hq_window_prefill_int8(q.data_ptr(), t, st4, *none, lens.data_ptr(), None, B, Hq, Hkv, 9, 0, D,
+                                    7, 1, 0.1, 1, wide.data_ptr(), st4, *end) == 0
+    assert (wide == 0).all()
+    out.fill_(1)
+    empty = (None, None, rows, None, None, one, one)
+    assert L.hq_prefix_decode_int8(q.data_ptr(), t, st3, *empty, None, 1, 0, *empty, lens.data_ptr(), 0,
+                                   kernels._DT[torch.float16], B, Hq, Hkv, D, 0.1, 0, out.data_ptr(), st3,
+                                   *end) == 0
+    assert (out == 0).all() and status.item() == 0

@@ -195,7 +195,7 @@ inline bool plan_prefill(Prefill& pl, int q_dt, int B, int Hkv, int nrep, int Sq
 // ---------------------------------------------------------------- arguments
 inline int fill_seg(Seg& s, const int8_t* k, const int8_t* v, const int64_t* kvs, const void* ksc,
                     const void* vsc, const int64_t* kss, const int64_t* vss, const int* lens,
-                    int cap, int nb, int units, int window, int sinks) {
+                    int cap, int nb, int units, int window, int sinks, const void* q) {
   if (cap > 0 && (!k || !v || !ksc || !vsc)) return HQ_ERR_INVALID_ARGUMENT;
   if (!kvs || !kss || !vss || cap < 0 || nb < 0 || units < 0 || window < 0 || sinks < 0)
     return HQ_ERR_INVALID_ARGUMENT;
@@ -215,6 +215,13 @@ inline int fill_seg(Seg& s, const int8_t* k, const int8_t* v, const int64_t* kvs
   s.vscb = vss[0];
   s.vsch = vss[1];
   s.vscs = vss[2];
+  // An empty cache may come without scales.  The kernels read K's before they know of any key (a
+  // test there took 2 % of prefix decode over 200 x 4096), so they are given readable ones; no score
+  // made from them is seen.
+  if (cap == 0) {
+    s.ksc = q;
+    s.kscb = s.ksch = s.kscd = 0;
+  }
   s.lens = lens;
   s.cap = cap;
   s.nb = nb;
@@ -294,7 +301,7 @@ extern "C" int hq_window_decode_int8(const void* q, int q_dtype, const int64_t q
   s.p = rag::make_params(q, q_dtype, q_strides[1], scale_dtype, Hq, Hkv, sm_scale, q_quant, out,
                          out_strides[0], out_strides[1], status);
   rc = rag::fill_seg(s.p.seg, k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
-                     S_max, B, 1, window, sinks);
+                     S_max, B, 1, window, sinks, q);
   if (rc != HQ_OK) return rc;
   if (B == 0) return HQ_OK;
   s.p.seg.qsb = q_strides[0];
@@ -327,7 +334,7 @@ extern "C" int hq_window_prefill_int8(const void* q, int q_dtype, const int64_t 
   s.p = rag::make_params(q, q_dtype, q_strides[1], scale_dtype, Hq, Hkv, sm_scale, q_quant, out,
                          out_strides[0], out_strides[1], status);
   rc = rag::fill_seg(s.p.seg, k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
-                     S_max, B, Sq, window, sinks);
+                     S_max, B, Sq, window, sinks, q);
   if (rc != HQ_OK) return rc;
   if (B == 0 || Sq == 0) return HQ_OK;
   s.p.seg.step = 1;
@@ -382,10 +389,10 @@ extern "C" int hq_prefix_decode_int8(
   own.p.merge_all = 1;
   pre.p = own.p;
   rc = rag::fill_seg(pre.p.seg, pk, pv, pkv_strides, pk_scale, pv_scale, pksc_strides, pvsc_strides,
-                     prefix_lens, P_max, G, B / G, 0, 0);
+                     prefix_lens, P_max, G, B / G, 0, 0, q);
   if (rc == HQ_OK)
     rc = rag::fill_seg(own.p.seg, k, v, kv_strides, k_scale, v_scale, ksc_strides, vsc_strides, lens,
-                       S_max, B, 1, 0, 0);
+                       S_max, B, 1, 0, 0, q);
   if (rc != HQ_OK) return rc;
   if (B == 0) return HQ_OK;
   const int nrep = Hq / Hkv;

@@ -558,10 +558,8 @@ __global__ void __launch_bounds__(Cfg<ALT, LO>::kThreads, 1) ragged_kernel(const
         float k8[8], km = 0.0f;
         uint32_t kb[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)  // (an empty cache may come without scales)
-          kb[e] = w.key.nv > 0
-                      ? load_bits(s.ksc, w.b * s.kscb + w.kvh * s.ksch + (4 * lane + e) * s.kscd, p.s_dt)
-                      : 0u;
+        for (int e = 0; e < 4; ++e)
+          kb[e] = load_bits(s.ksc, w.b * s.kscb + w.kvh * s.ksch + (4 * lane + e) * s.kscd, p.s_dt);
         {
           constexpr int NX = kForm / 2;
           uint4 x[NX];

@@ -144,8 +144,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint32_t ksb = 0;
   unsigned short qb[NR] = {};
   auto load_q = [&](const Piece& of) {
-    // (an empty cache may come without scales)
-    ksb = of.key.nv > 0 ? load_bits(s.ksc, of.b * s.kscb + of.kvh * s.ksch + d * s.kscd, p.s_dt) : 0;
+    ksb = load_bits(s.ksc, of.b * s.kscb + of.kvh * s.ksch + d * s.kscd, p.s_dt);
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       qb[r] = 0;

@@ -198,22 +198,6 @@ __device__ __forceinline__ void tmem_cols(uint32_t taddr, uint32_t (&r)[64]) {
         "=r"(r[63])
       : "r"(taddr));
 }
-// Bounded wait: some seconds, then false.  One opaque loop: as C++ with its convergence
-// instructions the waits took a third of all issue slots.
-constexpr uint32_t kPolls = 1u << 22;
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
-      "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n"
-      " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
-      "there:\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "n"(kPolls)
-      : "memory");
-  return ok != 0;
-}
-
 // Per-token int8 fake quantization of 8 values of a row with the largest |value| am, rounded back
 // to the model dtype.
 template <int DT>

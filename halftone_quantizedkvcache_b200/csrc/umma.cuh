@@ -1,8 +1,8 @@
 // tcgen05 helpers shared by the tensor-memory kernels (sm_100a): the swizzled
 // shared-memory layout and its matrix descriptor, the kind::f16 instruction
-// descriptor, issue and commit of an MMA, the proxy and thread-sync fences, and
-// 32-column tensor-memory loads and stores.  Used by prefill_attn.cu and
-// ragged_attn.cu.
+// descriptor, issue and commit of an MMA, the proxy and thread-sync fences,
+// 32-column tensor-memory loads and stores, and a bounded wait.  Used by
+// prefill_attn.cu and ragged_attn.cu.
 #pragma once
 
 #include "hq_common.cuh"
@@ -94,6 +94,25 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) 
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Bounded wait: false after kPolls polls.  A poll that finds nothing returns after 4 us at most
+// (measured on an idle SM), so a wait ends after some 2 s.  (A limit by the clock, one look at it
+// after every poll, took 6 % of decode with 8 rows per kv head: 64 x 4096 229 to 243 us, all in code
+// size.)  One opaque loop: as C++ with its convergence instructions the waits took a third of all
+// issue slots of ragged_attn.cu.
+constexpr uint32_t kPolls = 1u << 19;
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
+      "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n"
+      " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
+      "there:\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "n"(kPolls)
+      : "memory");
+  return ok != 0;
 }
 
 }  // namespace tc

@@ -917,6 +917,7 @@ def kblock_dequant(cache: dict, S: int, dtype: torch.dtype = torch.float32) -> t
 
 # ---------------------------------------------------------------- ragged batches
 _ragged_status: dict = {}   # device index -> int32 [1] (first error sticks)
+_ragged_lock = threading.Lock()
 
 
 def _status_word(dev: torch.device) -> torch.Tensor:
@@ -926,9 +927,12 @@ def _status_word(dev: torch.device) -> torch.Tensor:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first ragged-batch call on a device must run outside a CUDA "
                                "graph capture: run the same call once before capturing it")
-        t = torch.zeros(1, dtype=torch.int32, device=dev)
-        torch.cuda.current_stream(dev).synchronize()  # it is zero before any other stream's call
-        _ragged_status[dev.index] = t
+        with _ragged_lock:  # (one word, whichever thread comes first: errors in another would be lost)
+            t = _ragged_status.get(dev.index)
+            if t is None:
+                t = torch.zeros(1, dtype=torch.int32, device=dev)
+                torch.cuda.current_stream(dev).synchronize()  # zero before any other stream's call
+                _ragged_status[dev.index] = t
     return t
 
 

@@ -232,6 +232,9 @@ inline int fill_seg(Seg& s, const int8_t* k, const int8_t* v, const int64_t* kvs
   return HQ_OK;
 }
 
+// (an extent above 1 with a stride of 0: blocks would write the same rows)
+inline bool shared_rows(int64_t n, int64_t stride) { return n > 1 && stride == 0; }
+
 inline int check_common(const void* q, int q_dtype, const int64_t* qs, int nqs, const void* out,
                         const int64_t* os, int scale_dtype, int Hq, int Hkv, int D) {
   if (!q || !out || !qs || !os || Hq <= 0 || Hkv <= 0) return HQ_ERR_INVALID_ARGUMENT;
@@ -296,7 +299,8 @@ extern "C" int hq_window_decode_int8(const void* q, int q_dtype, const int64_t q
                                      size_t workspace_bytes, int* status, hq_stream_t stream) {
   int rc = rag::check_common(q, q_dtype, q_strides, 3, out, out_strides, scale_dtype, Hq, Hkv, D);
   if (rc != HQ_OK) return rc;
-  if (B < 0) return HQ_ERR_INVALID_ARGUMENT;
+  if (B < 0 || rag::shared_rows(B, out_strides[0]) || rag::shared_rows(Hq, out_strides[1]))
+    return HQ_ERR_INVALID_ARGUMENT;
   rag::Source s{};
   s.p = rag::make_params(q, q_dtype, q_strides[1], scale_dtype, Hq, Hkv, sm_scale, q_quant, out,
                          out_strides[0], out_strides[1], status);
@@ -328,7 +332,9 @@ extern "C" int hq_window_prefill_int8(const void* q, int q_dtype, const int64_t 
                                       size_t workspace_bytes, int* status, hq_stream_t stream) {
   int rc = rag::check_common(q, q_dtype, q_strides, 4, out, out_strides, scale_dtype, Hq, Hkv, D);
   if (rc != HQ_OK) return rc;
-  if (B < 0 || Sq < 0) return HQ_ERR_INVALID_ARGUMENT;
+  if (B < 0 || Sq < 0 || rag::shared_rows(B, out_strides[0]) || rag::shared_rows(Hq, out_strides[1]) ||
+      rag::shared_rows(Sq, out_strides[2]))
+    return HQ_ERR_INVALID_ARGUMENT;
   if (B > 65535 || int64_t(B) * Sq > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
   rag::Source s{};
   s.p = rag::make_params(q, q_dtype, q_strides[1], scale_dtype, Hq, Hkv, sm_scale, q_quant, out,
@@ -382,7 +388,9 @@ extern "C" int hq_prefix_decode_int8(
     int* status, hq_stream_t stream) {
   int rc = rag::check_common(q, q_dtype, q_strides, 3, out, out_strides, scale_dtype, Hq, Hkv, D);
   if (rc != HQ_OK) return rc;
-  if (B < 0 || G <= 0 || B % G) return HQ_ERR_INVALID_ARGUMENT;
+  if (B < 0 || G <= 0 || B % G || rag::shared_rows(B, out_strides[0]) ||
+      rag::shared_rows(Hq, out_strides[1]))
+    return HQ_ERR_INVALID_ARGUMENT;
   rag::Source own{}, pre{};
   own.p = rag::make_params(q, q_dtype, q_strides[1], scale_dtype, Hq, Hkv, sm_scale, q_quant, out,
                            out_strides[0], out_strides[1], status);

@@ -490,6 +490,12 @@ extern "C" int hq_rope_append_kv(
   if (!al(q) || !al(k_new) || !al(v_new) || !al(q_out) || !al(k_cache) || !al(v_cache) ||
       kv_strides[0] % 16 || kv_strides[1] % 16 || kv_strides[2] % 16)
     return HQ_ERR_INVALID_ARGUMENT;
+  // what is written has rows of its own for every sequence, head and token
+  const int64_t* written[3] = {qo_strides, kv_strides, vsc_strides};
+  const int extent[3][3] = {{B, Hq, S_new}, {B, Hkv, capacity}, {B, Hkv, capacity}};
+  for (int t = 0; t < 3; ++t)
+    for (int i = 0; i < 3; ++i)
+      if (extent[t][i] > 1 && written[t][i] == 0) return HQ_ERR_INVALID_ARGUMENT;
   if (B == 0 || S_new == 0) return HQ_OK;
   if (static_cast<int64_t>(B) * S_new > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
   rope::Params p{};

@@ -559,15 +559,15 @@ HQ_API int hq_kblock_dequant(const int8_t* k_cache, const int64_t kq_strides[3],
  * lens int32[B] in device memory holds the cached tokens of each sequence
  * (clamped to [0, S_max], S_max <= 2^30); what rows past it hold does not matter.
  * A cache (or prefix) of S_max (P_max) = 0 is not read: its codes and scales may
- * be NULL.  K and V may have any
- * (b, h, s) strides that are multiples of 16 bytes, shared by both, with
- * 16-byte aligned bases.  V scales are zero or positive, finite float32 or
- * float16; a token whose V scale is below 2^-60 counts as zeros.  q is bf16 or
- * f16 with 16-byte aligned rows, out has q's type with 8-byte aligned rows; D =
- * 128, Hq / Hkv whole and at most 128.  Scratch lies in `workspace` (256-byte
- * aligned, contents undefined before and after: nothing carries over from call
- * to call).  `status` (optional) receives HQ_ERR_DEVICE_TIMEOUT if a bounded
- * wait inside a block gave up (first error sticks).
+ * be NULL.  K and V may have any (b, h, s) strides that are multiples of 16
+ * bytes, shared by both, with 16-byte aligned bases.  V scales are zero or
+ * positive, finite float32 or float16; a token whose V scale is below 2^-60
+ * counts as zeros.  q is bf16 or f16 with 16-byte aligned rows, out has q's type
+ * with 8-byte aligned rows, one for every query and head (strides of 0 are
+ * refused); D = 128, Hq / Hkv whole and at most 128.  Scratch lies in `workspace`
+ * (256-byte aligned, contents undefined before and after: nothing carries over
+ * from call to call).  `status` (optional) receives HQ_ERR_DEVICE_TIMEOUT if a
+ * bounded wait inside a block gave up (first error sticks).
  *
  * hq_window_decode_int8 (B <= 1024): one query per sequence, the token at position
  *   lens[b] - 1, over keys j with j >= lens[b] - window or j < sinks (window 0:
@@ -633,7 +633,8 @@ HQ_API int hq_prefix_decode_int8(
  *   cache's per-channel scale [B, Hkv, D] (ksc_strides, a stride of 0
  *   broadcasts); V codes and scales as hq_quant_v_pertoken.  k_cache / v_cache
  *   are capacity buffers with strides kv_strides[3], v_scale [B, Hkv, capacity]
- *   of scale_dtype (as k_scale).  A sequence whose tokens do not fit writes
+ *   of scale_dtype (as k_scale); no rows of what is written are shared (strides
+ *   of 0 are refused).  A sequence whose tokens do not fit writes
  *   nothing to the cache and sets HQ_ERR_INVALID_ARGUMENT in `status`.
  */
 HQ_API int hq_rope_append_kv(

@@ -1346,6 +1346,8 @@ def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, *, scaling: str | Non
     elif scaling == "yarn":
         if not original_len or original_len < 1:
             raise ValueError("rope_inv_freq: yarn scaling needs original_len")
+        if not (theta > 1 and beta_fast > 0 and beta_slow > 0):  # the ramp's ends are logarithms
+            raise ValueError("rope_inv_freq: yarn scaling needs theta > 1 and positive betas")
         turns = original_len * f / (2 * math.pi)
         # in terms of the pair index, as the ramp is defined
         index = lambda n: rotary_dim * math.log(original_len / (n * 2 * math.pi)) / (  # noqa: E731

@@ -1,6 +1,7 @@
 """Calls of the ragged-batch operators at the edges of what their documentation allows, on the
 GPU.  Bounds as in test_ragged_gpu."""
 import math
+import threading
 
 import pytest
 import torch
@@ -132,3 +133,61 @@ def test_an_empty_cache_needs_no_pointers(rep, dt):
                                    kernels._DT[torch.float16], B, Hq, Hkv, D, 0.1, 0, out.data_ptr(), st3,
                                    *end) == 0
     assert (out == 0).all() and status.item() == 0
+
+
+@pytest.mark.parametrize("dt,sdt,rep", [("bf16", "f16", 8), ("f16", "f32", 8), ("bf16", "f32", 5), ("bf16", "f16", 2)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (2500, 9)])
+def test_many_tiles_of_one_sequence_to_a_block(rep, dt, sdt, window, sinks):
+    """Batches of long caches: a block walks tens of tiles, whole sequences and parts of two."""
+    g = torch.Generator(device="cuda").manual_seed(rep)
+    B, Hkv, cap = 48, 4, 4000
+    cache = make_cache(g, B, Hkv, cap, sdt)
+    lens = [(977 * b * b + 13) % (cap + 1) for b in range(B)]
+    lens[5], lens[6], lens[40] = cap, 0, cap
+    q = torch.randn((B, Hkv * rep, 1, D), generator=g, device="cuda").to(TDT[dt])
+    got = kernels.int8_window_decode_attn(q, *cache, i32(lens), window=window, sinks=sinks)
+    some = [0, 1, 5, 6, 7, 23, 24, 40, 47]
+    ref, tol = window_ref(q[some], [x[some] for x in cache], [lens[b] for b in some], [1] * len(some), window,
+                          sinks, dt)
+    check(got[some][:, :, 0], ref[:, 0], tol[:, 0], "decode")
+    assert kernels.ragged_status() == 0
+
+
+def test_two_threads_at_once():
+    """Two threads on streams of their own make the same calls: each gets its own results."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    sets = []
+    for i in range(2):
+        cache = make_cache(g, 6, 2, 900, "f16")
+        n = i32([(331 * (b + 1 + i)) % 900 for b in range(6)])
+        q = torch.randn((6, 16, 20, D), generator=g, device="cuda").to(torch.bfloat16)
+        sets.append((cache, n, q))
+
+    def calls(cache, n, q):
+        few, one = q[:, :4, :1].contiguous(), q[:, :, :1].contiguous()
+        return [kernels.int8_window_decode_attn(few, *cache, n, window=500, sinks=4),
+                kernels.int8_window_decode_attn(one, *cache, n),
+                kernels.int8_window_prefill_attn(q, *cache, n, window=300, sinks=2),
+                kernels.int8_prefix_decode_attn(one, *[x[:1] for x in cache], *cache, n)]
+
+    want = [calls(*s) for s in sets]
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(2), []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(40):
+                    got = calls(*sets[i])
+                    torch.cuda.current_stream().synchronize()
+                    wrong.extend(k for k, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a, b))
+        except Exception as e:  # noqa: BLE001 - reported by the assertion below
+            wrong.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and kernels.ragged_status() == 0

@@ -10,8 +10,8 @@
 //
 // Mathematics.  One pass over the keys with the running maximum and sum of a softmax, in
 // base 2.  The K scales, the softmax scale and log2(e) are folded into q once per row (q' =
-// q k_scale sm_scale log2 e, times a power of two that brings the row's largest |q'| to
-// [2^13, 2^14), rounded to float16; for float16 models a second float16 holds what the first
+// q k_scale sm_scale log2 e, times a power of two that brings the bound max |q| max k_scale on it
+// to [2^13, 2^14), rounded to float16; for float16 models a second float16 holds what the first
 // leaves over); the int8 K codes are exact in float16.  V's scale is split in two: v_scale_j
 // = g_j 2^(E + e_j), where E belongs to the piece of work.  g_j goes into V's float16 tile
 // (code g_j), e_j joins the exponent: with t_j = s_j + e_j and m a running maximum of t,
@@ -19,9 +19,11 @@
 // and o = 2^E O / l for V scales of any size.  A tile whose V scales lie within 2^-4 .. 2^6
 // of 2^E (nearly every one) has all e_j = 0, and costs nothing for them; the others look
 // e_j up.  Float16 models always put the whole scale into e_j (not a whole number then), so
-// that V stays exact.  m moves only when t grows by more than 14 (P <= 2^14), so O in tensor memory is rarely rescaled.  Roundings to float16, each off by
-// 2^-11 of itself at most: q' (bf16 models), P, and for bf16 models g_j and code g_j, an
-// eighth of the output's own half step.
+// that V stays exact.  m moves only when t grows by more than 14 (P <= 2^14), so O in tensor memory
+// is rarely rescaled.  Roundings to float16, each off by 2^-11 of itself at most: q' (bf16 models),
+// P (one float16; prefill_attn.cu keeps two parts of it), and for bf16 models g_j and code g_j, an
+// eighth of the output's own half step.  Errors against float64 are 4 % (bf16) and 14 to 20 %
+// (float16) above those of a float32 form rounded once; V scales below 2^-60 count as zero.
 //
 // Work.  Row r of a unit (kv head, sequence or group) is q head kvh * n_rep + r % n_rep of
 // query r / n_rep; 128 rows sit on the 128 lanes of tensor memory.  A block has two groups of

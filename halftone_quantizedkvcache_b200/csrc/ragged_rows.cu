@@ -6,7 +6,8 @@
 // Both products run on the int8 tensor cores (mma.sync m16n8k32) straight from the codes, so
 // nothing is converted: with q' = q k_scale sm_scale log2(e) in 24-bit fixed point per row
 // (three balanced base-256 digits, one column each) the scores are exact integers times one
-// scale, and P v_scale likewise goes in as three digits; O is float32.
+// scale, and P v_scale likewise goes in as three digits; O is float32.  The digits' scale is twice
+// the largest p v_scale since a warp's maximum last moved.
 //
 // A block is 4 warps, 32 keys of a tile each with their own online softmax; two blocks per SM.
 // Tiles arrive by TMA into a ring of 3 stages, 128-byte swizzled; two are in flight while one

@@ -16,10 +16,13 @@
 // turned values are off by 2^-22 of the pair's size at most, and a quotient closer to a
 // rounding border than that (about one in 10^4) is formed again in float64.
 //
-// Bound by memory: a q element is read and written (4 bytes), a k or v element read and coded
-// (3 bytes).  A lane holds 8 channels (16 bytes), D / 8 lanes a row, and keeps the cos and sin
-// of its channels for all rows of its token.  8 sequences x 4096 tokens, 16 + 8 + 8 heads, bf16:
-// 141 us, 3.3 TB/s of the 470 MB it cannot do without (0.51 of measured).
+// A q element is read and written (4 bytes), a k or v element read and coded (3 bytes).  A lane
+// holds 8 channels (16 bytes), D / 8 lanes a row, and keeps the cos and sin of its channels for all
+// rows of its token.  8 sequences x 4096 tokens, 16 + 8 + 8 heads, bf16: 144 us, 3.3 TB/s of the
+// 470 MB it cannot do without (0.50 of measured).  Bound by latency: issue slots are 60 % full and
+// memory half, since no load is in flight while a warp forms its sines and two are in between.  The
+// kernel for float32 and for rotary sizes off the lanes' grid forms every channel in float64: 402 us
+// (2.2 TB/s of 873 MB) and, bf16 with 72 channels turned, 387 us at the same sizes.
 #include <algorithm>
 #include <cmath>
 

@@ -1095,6 +1095,9 @@ def int8_window_decode_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, sin
     ``out [B,Hq,D]``).  ``q_quant``: the per-token fake quantization of ``int8_decode_attn``.
     Nothing depends on ``lens`` on the host, so the call replays in a CUDA graph while
     sequences grow.
+
+    V scales are zero or positive and finite; one below 2^-60 may count as zero.  Up to 4 q heads
+    per kv head the weights are held in 24 bits, beyond that in float16 (2^-11 of each weight).
     """
     what = "int8_window_decode_attn"
     if type(window) is not int or type(sinks) is not int:
@@ -1169,6 +1172,10 @@ def int8_window_prefill_attn(q, k_i8, k_sc, v_i8, v_sc, lens, *, window=None, si
     position ``p = lens[b] - q_lens[b] + i`` and sees ``j <= p`` with ``j > p - window`` or
     ``j < sinks``.  Returns ``[B,Sq,Hq,D]``; rows past ``q_lens[b]`` are zeros, or are left as
     they were in ``out``.  Queries at a position below 0 give zeros.
+
+    V scales as in ``int8_window_decode_attn``.  The weights are held in one float16 (2^-11 of each,
+    an eighth of bf16's own rounding), where ``int8_prefill_attn``, for batches of one length without
+    a window, keeps some 16 bits.
     """
     what = "int8_window_prefill_attn"
     if type(window) is not int or type(sinks) is not int:
@@ -1246,7 +1253,8 @@ def int8_prefix_decode_attn(q, pk_i8, pk_sc, pv_i8, pv_sc, k_i8, k_sc, v_i8, v_s
     of G, and sequences ``g * B/G .. (g + 1) * B/G - 1`` share prefix g.  Each sequence's own
     tokens are in ``k_i8 / k_sc / v_i8 / v_sc`` (``[B,Hkv,cap,D]`` and so on).  ``lens`` int32
     ``[B]`` and ``prefix_lens`` int32 ``[G]`` (default: P), on the device, say how many tokens
-    are held; the output is the attention over both, and zeros where there is none.
+    are held; the output is the attention over both, and zeros where there is none.  V scales and
+    weights as in ``int8_window_decode_attn``, the prefix's rows being those of its whole group.
     """
     what = "int8_prefix_decode_attn"
     try:
@@ -1373,10 +1381,12 @@ def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache
     scales ``[B,Hkv,cap,1]`` (both f16 or f32).  Token i < n_new[b] (default S) of sequence b
     stands at position ``lens[b] + i + pos_offset[b]`` (``pos_offset``: the length of a shared
     prefix, for one) and goes to row ``lens[b] + i``; ``lens`` (int32 ``[B]``, device) is not
-    advanced.  K is coded with the stored scale, as ``quant_k_static`` codes it, from the
-    rotated and unrounded values; V per token, its scales written.  Returns the rotated q
-    (``q_out``, which may be q; rows past ``n_new[b]`` are q's).  A sequence whose tokens do not
-    fit its capacity writes nothing and sets ``ragged_status()``.
+    advanced.  K is coded with the stored scale from the rotated and unrounded values: the whole
+    number nearest the exact quotient, clamped to +-127 (``quant_k_static`` rounds the quotient to
+    float32 first, which moves a code next to a border now and then).  V is quantized per token,
+    its scales written.  K and V of real tokens are finite.  Returns the rotated q (``q_out``, which
+    may be q; rows past ``n_new[b]`` are q's).  A sequence whose tokens do not fit its capacity
+    writes nothing and sets ``ragged_status()``.
     """
     what = "rope_append_kv"
     try:

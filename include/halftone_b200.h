@@ -562,7 +562,7 @@ HQ_API int hq_kblock_dequant(const int8_t* k_cache, const int64_t kq_strides[3],
  * be NULL.  K and V may have any (b, h, s) strides that are multiples of 16
  * bytes, shared by both, with 16-byte aligned bases.  V scales are zero or
  * positive, finite float32 or float16; a token whose V scale is below 2^-60
- * counts as zeros.  q is bf16 or f16 with 16-byte aligned rows, out has q's type
+ * may count as zeros.  q is bf16 or f16 with 16-byte aligned rows, out has q's type
  * with 8-byte aligned rows, one for every query and head (strides of 0 are
  * refused); D = 128, Hq / Hkv whole and at most 128.  Scratch lies in `workspace`
  * (256-byte aligned, contents undefined before and after: nothing carries over
@@ -629,13 +629,14 @@ HQ_API int hq_prefix_decode_int8(
  *   (float32 [rotary_dim / 2]), pairs (j, j + rotary_dim / 2) or, interleaved,
  *   (2j, 2j + 1), cos and sin times `factor`.  q_out receives the rotated q
  *   (may be q itself; rows past n_new[b] are copied unturned).  K codes are
- *   clamp(rint(k / k_scale), -127, 127) of the rotated, unrounded k with the
- *   cache's per-channel scale [B, Hkv, D] (ksc_strides, a stride of 0
- *   broadcasts); V codes and scales as hq_quant_v_pertoken.  k_cache / v_cache
- *   are capacity buffers with strides kv_strides[3], v_scale [B, Hkv, capacity]
- *   of scale_dtype (as k_scale); no rows of what is written are shared (strides
- *   of 0 are refused).  A sequence whose tokens do not fit writes
- *   nothing to the cache and sets HQ_ERR_INVALID_ARGUMENT in `status`.
+ *   clamp(rint(k / k_scale), -127, 127) of the rotated, unrounded k and the exact
+ *   quotient, with the cache's per-channel scale [B, Hkv, D] (ksc_strides, a
+ *   stride of 0 broadcasts); V codes and scales as hq_quant_v_pertoken; k and v
+ *   of real tokens are finite.  k_cache / v_cache are capacity buffers with
+ *   strides kv_strides[3], v_scale [B, Hkv, capacity] of scale_dtype (as
+ *   k_scale); no rows of what is written are shared (strides of 0 are refused).
+ *   A sequence whose tokens do not fit writes nothing to the cache and sets
+ *   HQ_ERR_INVALID_ARGUMENT in `status`.
  */
 HQ_API int hq_rope_append_kv(
     const void* q, const void* k_new, const void* v_new, int x_dtype, const int64_t q_strides[4],

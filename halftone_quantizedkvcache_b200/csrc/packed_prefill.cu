@@ -1,0 +1,743 @@
+// Causal attention of packed sequences of different lengths, 16-bit Q, K and V, grouped heads
+// (sm_100a):  o_i = sum_j softmax_j(sm_scale q_i . k_j) v_j  over the keys j that query i sees.
+//
+// Sequence b has queries cu_q[b] .. cu_q[b + 1] - 1 and keys cu_k[b] .. cu_k[b + 1] - 1, the queries
+// standing at its last positions: query i of n sees keys j <= m - n + i (all m, without the mask).
+//
+// Work.  Row r of a unit (sequence, kv head) is q head kvh n_rep + r % n_rep of query r / n_rep; 128
+// rows are the lanes of a tile in tensor memory, and a block takes two tiles, 256 rows, that share
+// every K and V tile of 128 keys.  Where that leaves SMs idle the keys are split over several blocks,
+// whose states (m, l, O) join_kernel puts together.  Blocks with the most keys start first.
+//
+// Roles of a block (12 warps): two groups of 4 softmax warps, a thread per row; one warp that issues
+// the products; one that loads K and V by TMA; two that look over the V tiles of masked steps.
+// S = Q K^T goes to tensor memory; the softmax thread takes its row into registers, and writes P in
+// 16 bits over the S it came from; O += P V reads P from there.  While one tile is in its softmax the
+// other's products run.  The running maximum moves only when it grows by more than 8 (P <= 2^8), so O
+// is rarely rescaled; sums are float32.  P is rounded to the model's type (2^-9 of each weight in
+// bf16, 2^-12 in float16: what the output itself is rounded by).
+//
+// A V row holding an infinity or NaN spoils the rows that see it and no others: 0 x NaN is NaN in the
+// product, so on steps where some row does not see every key such rows are zeroed in shared memory
+// and rows that see them get a NaN sum.  (K needs none of this: unseen scores are replaced.)
+#include <algorithm>
+#include <atomic>
+
+#include "decode_common.cuh"
+#include "umma.cuh"
+
+namespace hq {
+int current_sm_count();
+
+namespace pk {
+using namespace tc;
+
+constexpr int kD = 128;
+constexpr int kBN = 128;                  // keys per tile
+constexpr int kRows = 256;                // rows per block: two tiles
+constexpr int kThreads = 384;
+constexpr int kSoft = 256;
+constexpr int kSoftRegs = 208, kOtherRegs = 88;
+constexpr int kStages = 4;                // K, V, K, V, ..
+constexpr int kTileB = kBN * kD * 2;
+constexpr int kOffKv = 2 * kTileB;        // behind the two Q tiles
+constexpr int kOffBar = kOffKv + kStages * kTileB;
+// barriers
+constexpr int kFull = 0, kEmpty = kFull + kStages, kSFull = kEmpty + kStages, kPFull = kSFull + 2,
+              kOFull = kPFull + 4, kClean = kOFull + 2, kDrain = kClean + 2, kBars = kDrain + 1;
+constexpr int kOffBad = kOffBar + kBars * 8;       // [2][4] words of spoiled V rows
+constexpr int kOffMisc = kOffBad + 32;
+constexpr int kSmem = 1024 + kOffMisc + 32;
+constexpr int kPartRow = kD + 4;
+constexpr uint32_t kColO = 256;           // tensor memory: S tiles at 0 and 128, O at 256 and 384
+constexpr int kCleanWarps = 2;
+constexpr int kMaxSplit = 16;
+
+struct Params {
+  const void* q;
+  void* out;
+  int64_t qs[2], os[2];
+  const int* cu_q;
+  const int* cu_k;
+  int T, Tk, B, Hkv, nrep;
+  int causal;
+  float c;                                // sm_scale log2(e)
+  int n_split, units;                     // units: an upper bound of (sequence, 256 rows, kv head)
+  int swap;                               // tensor maps: (channel, token, head) instead of (channel, head, token)
+  int zero_rest;
+  float* part;
+  int* status;
+};
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
+// Products by the lane whose `lead` is set, the warp converged (operands stay in uniform registers).
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                       uint32_t b_hi, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %7, 0;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %6, p;\n\t}\n" ::"r"(lead),
+      "r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
+                                       uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], b, %5, p;\n\t}\n" ::"r"(lead),
+      "r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}\n" ::"r"(lead),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, "
+      "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
+      "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
+      "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
+      "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127"
+      "}, [%128];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_stw32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+      "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32"
+      "};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == HQ_DTYPE_BF16) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&x);
+  } else {
+    const __half2 x = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&x);
+  }
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// ---------------------------------------------------------------- what a block works on
+struct Seq {
+  int q0, nq, k0, nk;
+};
+__device__ __forceinline__ Seq seq_of(const Params& p, int b) {
+  Seq s;
+  s.q0 = min(max(p.cu_q[b], 0), p.T);
+  s.nq = min(max(p.cu_q[b + 1], s.q0), p.T) - s.q0;
+  s.k0 = min(max(p.cu_k[b], 0), p.Tk);
+  s.nk = min(max(p.cu_k[b + 1], s.k0), p.Tk) - s.k0;
+  return s;
+}
+__device__ __forceinline__ int pairs_of(const Params& p, int b) {
+  const int q0 = min(max(p.cu_q[b], 0), p.T), q1 = min(max(p.cu_q[b + 1], q0), p.T);
+  return static_cast<int>((static_cast<int64_t>(q1 - q0) * p.nrep + kRows - 1) / kRows);
+}
+// All lanes of a warp: the sequence that holds pair u of the line of all pairs, and the pair's place in
+// it (b = B: behind the last).
+__device__ __forceinline__ void find_pair(const Params& p, int u, int& b, int& y) {
+  const int lane = threadIdx.x & 31;
+  int run = 0;
+  b = p.B;
+  y = 0;
+#pragma unroll 1
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int mine = b0 + lane < p.B ? pairs_of(p, b0 + lane) : 0;
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int z = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += z;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, run + x > u);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      b = b0 + l;
+      y = u - run - __shfl_sync(0xffffffffu, x - mine, l);
+      return;
+    }
+    run += __shfl_sync(0xffffffffu, x, 31);
+  }
+}
+// keys that row r of a unit sees: 0 .. lim - 1
+__device__ __forceinline__ int limit_of(const Params& p, const Seq& s, int r) {
+  const int i = static_cast<uint32_t>(r) / static_cast<uint32_t>(p.nrep);
+  return p.causal ? min(max(s.nk - s.nq + i + 1, 0), s.nk) : s.nk;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 1)
+    packed_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kOffBar);
+  uint32_t* bad = reinterpret_cast<uint32_t*>(smem + kOffBad);
+  int* misc = reinterpret_cast<int*>(smem + kOffMisc);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // rows behind the last sequence
+  if (p.zero_rest) {
+    const int rest = p.B > 0 ? min(max(p.cu_q[p.B], 0), p.T) : 0;
+    for (int64_t i = rest + static_cast<int64_t>(blockIdx.x); i < p.T; i += gridDim.x)
+      for (int x = tid; x < p.Hkv * p.nrep * (kD / 8); x += kThreads)
+        *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + 2 * (i * p.os[0] + x / (kD / 8) * p.os[1] + x % (kD / 8) * 8)) =
+            make_uint4(0, 0, 0, 0);
+  }
+  if (warp == 0) {
+    // heavy (last) pairs first
+    const int item = p.units - 1 - static_cast<int>(blockIdx.x) / p.n_split;
+    int b, y;
+    find_pair(p, item / p.Hkv, b, y);
+    if (lane == 0) {
+      misc[0] = b;
+      misc[1] = y;
+    }
+  }
+  __syncthreads();
+  const int b = misc[0];
+  if (b >= p.B) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  const int split = static_cast<int>(blockIdx.x) % p.n_split, item = p.units - 1 - static_cast<int>(blockIdx.x) / p.n_split;
+  const int kvh = item % p.Hkv;
+  const Seq s = seq_of(p, b);
+  const int row0 = misc[1] * kRows, rows = min(kRows, s.nq * p.nrep - row0);  // rows >= 1
+  // key tiles of the two row tiles, and the block's share of them
+  int nt[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int last = min(rows, 128 * (t + 1)) - 1;
+    nt[t] = last >= 128 * t ? (limit_of(p, s, row0 + last) + kBN - 1) / kBN : 0;
+  }
+  const int all = max(nt[0], nt[1]);
+  const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / p.n_split);
+  const int j1 = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.n_split);
+  // masked steps: those from jm on, past the keys that every row sees.  The two barriers that say that
+  // their V is looked over take turns: each V stage has its own, which cannot run a phase ahead.
+  const int jm = max(j0, limit_of(p, s, row0) / kBN);
+  auto clean_bar = [&](int j) { return &bar[kClean + (j & 1)]; };
+  auto clean_phase = [&](int j) { return static_cast<uint32_t>((j - jm) >> 1) & 1u; };
+  const uint32_t base = smem_u32(smem);
+
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&misc[4])), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bar[kFull + i], 1);
+      mbar_init(&bar[kEmpty + i], i & 1 ? 1 + kCleanWarps : 1);  // V stages: products, and the warps that look
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bar[kSFull + t], 1);
+      mbar_init(&bar[kPFull + 2 * t], 4);
+      mbar_init(&bar[kPFull + 2 * t + 1], 4);
+      mbar_init(&bar[kOFull + t], 1);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&bar[kClean + i], kCleanWarps);
+    mbar_init(&bar[kDrain], 1);
+    fence_mbar_init();
+  }
+  // Q, 16 lanes a row: K-major tiles of two 64-channel halves, 128-byte swizzle; rows past the last: zeros
+  for (int x = tid; x < kRows * 16; x += kThreads) {
+    const int r = x >> 4, c = x & 15;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const int i = static_cast<uint32_t>(row0 + r) / static_cast<uint32_t>(p.nrep), h = kvh * p.nrep + row0 + r - i * p.nrep;
+      v = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + 2 * ((s.q0 + static_cast<int64_t>(i)) * p.qs[0] + h * p.qs[1] + 8 * c));
+    }
+    *reinterpret_cast<uint4*>(smem + (r >> 7) * kTileB + (c >> 3) * (kBN * 128) + sw128(r & 127, c & 7)) = v;
+  }
+  fence_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = static_cast<uint32_t>(misc[4]);
+  bool ok = true;
+
+  if (warp >= kSoft / 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp < kSoft / 32) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    // ------------------------------------------------------------ softmax: a thread per row
+    const int t = warp >> 2, r = 128 * t + 32 * (warp & 3) + lane;
+    const int lim = limit_of(p, s, row0 + min(r, rows - 1));
+    const uint32_t s_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + 128 * t;
+    const uint32_t o_addr = s_addr - 128 * t + kColO + 128 * t;
+    float m = -INFINITY, l = 0.0f;        // m: of the raw scores
+    const int jt = min(j1, nt[t]);
+#pragma unroll 1
+    for (int j = j0; j < jt; ++j) {
+      ok = wait_bar(&bar[kSFull + t], (j - j0) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x[128];
+      tmem_ld128(s_addr, x);
+      const int left = lim - j * kBN;     // keys of the tile that this row sees
+      bool spoiled = false;
+      if (j >= jm) {
+        ok = wait_bar(clean_bar(j), clean_phase(j));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t* w = bad + 4 * (j & 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = min(max(left - 32 * i, 0), 32);
+          spoiled |= (w[i] & (n == 32 ? 0xffffffffu : (1u << n) - 1u)) != 0;
+        }
+        if (__any_sync(0xffffffffu, left < kBN)) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) x[i] = i < left ? x[i] : 0xff800000u;
+        }
+      }
+      float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[1]);
+#pragma unroll
+      for (int i = 2; i < 126; i += 4) {
+        m0 = max3(m0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        m1 = max3(m1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+      }
+      const float top = max3(fmaxf(m0, m1), __uint_as_float(x[126]), __uint_as_float(x[127]));
+      if (j == j0) {
+        m = top;
+      } else if (__any_sync(0xffffffffu, (top - m) * p.c > 8.0f || (m == -INFINITY && top > m))) {
+        // (lanes that need it and those that do not: the factor is 1 for a maximum that stays)
+        const float m_new = (top - m) * p.c > 8.0f || (m == -INFINITY && top > m) ? top : m;
+        const float f = m_new == m ? 1.0f : ex2_ftz((m - m_new) * p.c);
+        m = m_new;
+        l *= f;
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          float o[32];
+          tmem_ld32(o_addr + 32 * i, o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= f;
+          tmem_st32(o_addr + 32 * i, o);
+        }
+        tmem_wait_st();
+      }
+      const float mc = m == -INFINITY ? 0.0f : m * p.c;
+      const F2 c2 = f2_make(p.c, p.c), n2 = f2_make(-mc, -mc);
+      F2 sum = f2_make(0.0f, 0.0f), sum1 = sum;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          F2 z = f2_fma(f2_make(__uint_as_float(x[64 * h + 2 * i]), __uint_as_float(x[64 * h + 2 * i + 1])), c2, n2);
+          float a, e;
+          f2_split(z, a, e);
+          a = ex2_ftz(a);
+          e = ex2_ftz(e);
+          if (i & 1) sum = f2_add(sum, f2_make(a, e));
+          else sum1 = f2_add(sum1, f2_make(a, e));
+          w[i] = pack2<DT>(a, e);
+        }
+        tmem_stw32(s_addr + 32 * h, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar[kPFull + 2 * t + h]);
+      }
+      float a, e;
+      f2_split(f2_add(sum, sum1), a, e);
+      l += a + e;
+      if (spoiled) l = NAN;
+    }
+    // ---- the rows' results
+    if (ok && jt > j0) {
+      ok = wait_bar(&bar[kOFull + t], 0);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    if (ok && 128 * t + 32 * (warp & 3) < rows) {
+      const bool live = r < rows, has = jt > j0;
+      const int i = static_cast<uint32_t>(row0 + min(r, rows - 1)) / static_cast<uint32_t>(p.nrep);
+      const int h = kvh * p.nrep + row0 + min(r, rows - 1) - i * p.nrep;
+      const float inv = !has || l <= 0.0f ? 0.0f : 1.0f / l;  // (a NaN stays)
+      char* dst = static_cast<char*>(p.out) + 2 * ((s.q0 + static_cast<int64_t>(i)) * p.os[0] + h * p.os[1]);
+      float* prt = p.part + ((static_cast<int64_t>(item) * p.n_split + split) * kRows + r) * kPartRow;
+      if (p.n_split > 1 && live)
+        *reinterpret_cast<float2*>(prt) = make_float2(has && m != -INFINITY ? m * p.c : -INFINITY, has ? l : 0.0f);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float o[32];
+        tmem_ld32(o_addr + 32 * c, o);
+        if (p.n_split > 1) {
+          if (live)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(prt + 4 + 32 * c + 4 * e) =
+                  has ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_float4(0, 0, 0, 0);
+        } else if (live) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (has && !(l <= 0.0f))
+              w = make_uint4(pack2<DT>(o[8 * e] * inv, o[8 * e + 1] * inv), pack2<DT>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                             pack2<DT>(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2<DT>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+            *reinterpret_cast<uint4*>(dst + 64 * c + 16 * e) = w;
+          }
+        }
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ products
+    const uint32_t lead = elect_one();
+    constexpr uint32_t id_s = idesc<DT>(128, kBN, false), id_o = idesc<DT>(128, kD, true);
+    constexpr uint32_t k_hi = sdesc(0, 16, 1024) >> 32, v_hi = sdesc(0, kBN * 128, 1024) >> 32;
+    const uint32_t q_lo = static_cast<uint32_t>(sdesc(base, 16, 1024));
+    const uint32_t k_lo = static_cast<uint32_t>(sdesc(base + kOffKv, 16, 1024));
+    const uint32_t v_lo = static_cast<uint32_t>(sdesc(base + kOffKv, kBN * 128, 1024));
+    auto score = [&](int t, int stage) {
+      const uint32_t a = q_lo + (t * kTileB >> 4), k = k_lo + (stage * kTileB >> 4);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const uint32_t off = ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) >> 4;
+        mma_ss(lead, tmem + 128 * t, a + off, k_hi, k + off, k_hi, id_s, kk > 0);
+      }
+      commit(lead, &bar[kSFull + t]);
+    };
+    if (j0 < j1) {
+      ok = wait_bar(&bar[kFull], 0);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (j0 < nt[t]) score(t, 0);
+        commit(lead, &bar[kEmpty]);
+      }
+    }
+#pragma unroll 1
+    for (int j = j0; ok && j < j1; ++j) {
+      const int n = j - j0, vi = 2 * n + 1, ki = 2 * n + 2;  // copies: V of this tile, K of the next
+      const int vs = vi % kStages, ks = ki % kStages;
+      ok = wait_bar(&bar[kFull + vs], (vi / kStages) & 1);
+      if (j >= jm) ok = ok && wait_bar(clean_bar(j), clean_phase(j));
+      if (j + 1 < j1) ok = ok && wait_bar(&bar[kFull + ks], (ki / kStages) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (j >= nt[t]) continue;
+        const uint32_t v = v_lo + (vs * kTileB >> 4);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          ok = ok && wait_bar(&bar[kPFull + 2 * t + h], n & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+            mma_ts(lead, tmem + kColO + 128 * t, tmem + 128 * t + 8 * kk, v + (kk * 16 * 128 >> 4), v_hi, id_o, n > 0 || kk > 0);
+        }
+        if (!ok) break;
+        if (j + 1 < min(j1, nt[t])) score(t, ks);
+        else commit(lead, &bar[kOFull + t]);
+      }
+      if (!ok) break;
+      commit(lead, &bar[kEmpty + vs]);
+      if (j + 1 < j1) commit(lead, &bar[kEmpty + ks]);
+    }
+    // no product is in flight when the block ends
+    commit(lead, &bar[kDrain]);
+    if (!wait_bar(&bar[kDrain], 0)) ok = false;
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ copies
+    const int copies = 2 * (j1 - j0);
+    int n = 0;
+    if (lane == 0) {
+      for (; n < copies; ++n) {
+        const int st = n % kStages;
+        if (n >= kStages && !(ok = wait_bar(&bar[kEmpty + st], (n / kStages - 1) & 1))) break;
+        unsigned char* to = smem + kOffKv + st * kTileB;
+        const CUtensorMap* map = n & 1 ? &vm : &km;
+        const int key = s.k0 + (j0 + (n >> 1)) * kBN;
+        mbar_arrive_expect_tx(&bar[kFull + st], kTileB);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          asm volatile(
+              "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                  smem_u32(to + h * (kBN * 128))),
+              "l"(reinterpret_cast<uint64_t>(map)), "r"(64 * h), "r"(p.swap ? key : kvh), "r"(p.swap ? kvh : key),
+              "r"(smem_u32(&bar[kFull + st]))
+              : "memory");
+      }
+      if (!ok)  // no copy is in flight when the block ends
+        for (int i = max(0, n - kStages); i < n; ++i) wait_bar(&bar[kFull + i % kStages], (i / kStages) & 1);
+    }
+    ok = __all_sync(0xffffffffu, ok);
+  } else {
+    // ------------------------------------------------------------ V rows that hold no numbers, on masked steps
+    const int g = warp - 10;
+    constexpr uint32_t mask = DT == HQ_DTYPE_BF16 ? 0x7f807f80u : 0x7c007c00u, one = DT == HQ_DTYPE_BF16 ? 0x00800080u : 0x04000400u;
+#pragma unroll 1
+    for (int j = j0; j < j1; ++j) {
+      const int vi = 2 * (j - j0) + 1, vs = vi % kStages;
+      ok = wait_bar(&bar[kFull + vs], (vi / kStages) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (j < jm) {  // (every phase is waited for: a parity says nothing of phases further back)
+        if (lane == 0) mbar_arrive(&bar[kEmpty + vs]);
+        continue;
+      }
+      unsigned char* v = smem + kOffKv + vs * kTileB;
+#pragma unroll 1
+      for (int q = 0; q < 2; ++q) {
+        const int row = 64 * g + 32 * q + lane;
+        uint32_t seen = 0;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const uint4 x = *reinterpret_cast<const uint4*>(v + (c >> 3) * (kBN * 128) + row * 128 + (((c + lane) & 7) << 4));
+          seen |= ((x.x & mask) + one) | ((x.y & mask) + one) | ((x.z & mask) + one) | ((x.w & mask) + one);
+        }
+        const bool broken = seen & 0x80008000u;
+        if (broken)
+          for (int c = 0; c < 16; ++c)
+            *reinterpret_cast<uint4*>(v + (c >> 3) * (kBN * 128) + row * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        const uint32_t word = __ballot_sync(0xffffffffu, broken);
+        if (lane == 0) bad[4 * (j & 1) + 2 * g + q] = word;
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(clean_bar(j));
+        mbar_arrive(&bar[kEmpty + vs]);
+      }
+    }
+  }
+  if (!ok && lane == 0) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// A warp per output row (token, q head) joins the pieces of its pair, in order; a lane 4 channels.
+template <int DT>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, heads = p.Hkv * p.nrep;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (at >= static_cast<int64_t>(p.T) * heads) return;
+  const int tok = static_cast<int>(at / heads), h = static_cast<int>(at - static_cast<int64_t>(tok) * heads);
+  const int kvh = h / p.nrep;
+  // the token's sequence, and the pairs before it
+  int pairs = 0, b = -1;
+#pragma unroll 1
+  for (int b0 = 0; b < 0 && b0 < p.B; b0 += 32) {
+    const int e = b0 + lane;
+    const bool holds = e < p.B && seq_of(p, e).q0 <= tok && tok < seq_of(p, e).q0 + seq_of(p, e).nq;
+    const unsigned hit = __ballot_sync(0xffffffffu, holds);
+    const int l = hit ? __ffs(hit) - 1 : 32;
+    pairs += __reduce_add_sync(0xffffffffu, e < p.B && lane < l ? pairs_of(p, e) : 0);
+    if (hit) b = b0 + l;
+  }
+  if (b < 0) return;
+  const int r = (tok - seq_of(p, b).q0) * p.nrep + h - kvh * p.nrep;
+  const int64_t item = static_cast<int64_t>(pairs + r / kRows) * p.Hkv + kvh;
+  if (item >= p.units) return;
+  const float* x = p.part + (item * p.n_split * kRows + r % kRows) * kPartRow;
+  float M = -INFINITY, L = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = 0; i < p.n_split; ++i, x += kRows * kPartRow) {
+    const float2 ml = *reinterpret_cast<const float2*>(x);
+    const float4 o = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
+    // (a piece whose sums are no number has a maximum of -inf and passes them on)
+    const float top = fmaxf(M, ml.x), f0 = M == -INFINITY ? 0.0f : exp2f(M - top), f1 = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
+    M = top;
+    L = L * f0 + ml.y * f1;
+    acc.x = acc.x * f0 + o.x * f1;
+    acc.y = acc.y * f0 + o.y * f1;
+    acc.z = acc.z * f0 + o.z * f1;
+    acc.w = acc.w * f0 + o.w * f1;
+  }
+  const float inv = L <= 0.0f ? 0.0f : 1.0f / L;
+  *reinterpret_cast<uint2*>(static_cast<char*>(p.out) + 2 * (tok * p.os[0] + h * p.os[1] + 4 * lane)) =
+      make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
+}
+
+// ---------------------------------------------------------------- host
+struct Plan {
+  int units, n_split;
+  size_t bytes;
+};
+inline bool plan(Plan& pl, int64_t T, int64_t Tk, int B, int Hkv, int nrep) {
+  const int64_t units = ((T * nrep + kRows - 1) / kRows + B) * Hkv;
+  if (units * kMaxSplit > 0x7fffffff || T * nrep > 0x3fffffff || Tk > 0x3fffffff) return false;
+  // With fewer blocks than SMs each row pair's keys go to several, down to two key tiles a block.
+  const int64_t tiles = std::max<int64_t>(1, Tk / kBN);
+  pl.n_split = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, current_sm_count() / std::max<int64_t>(units, 1)),
+                                                   std::max<int64_t>(1, tiles / 2), kMaxSplit}));
+  pl.units = static_cast<int>(units);
+  pl.bytes = pl.n_split > 1 ? sizeof(float) * static_cast<size_t>(units) * pl.n_split * kRows * kPartRow : 0;
+  return true;
+}
+
+// [T, H, 128] in boxes of 128 tokens x 64 channels, 128-byte swizzle, zeros past the end
+inline int encode(CUtensorMap* m, const void* base, int dt, const int64_t st[2], int T, int H, int swap) {
+  auto enc = dec::encode_fn();
+  if (!enc) return HQ_ERR_UNSUPPORTED;
+  const cuuint64_t ts = 2 * st[0], hs = H > 1 ? 2 * st[1] : (swap ? 2 * st[0] : 2 * kD);
+  const cuuint64_t dims[3] = {kD, static_cast<cuuint64_t>(swap ? T : H), static_cast<cuuint64_t>(swap ? H : T)};
+  const cuuint64_t strides[2] = {swap ? ts : hs, swap ? hs : ts};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(swap ? kBN : 1), static_cast<cuuint32_t>(swap ? 1 : kBN)};
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = enc(m, dt == HQ_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? HQ_OK : HQ_ERR_INVALID_ARGUMENT;
+}
+
+template <int DT>
+int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
+  auto kern = packed_kernel<DT>;
+  // an increase beyond the registers of the launch would wait for ever
+  static const bool fits = [&] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kern) == cudaSuccess && a.numRegs * kThreads >= kSoft * kSoftRegs + (kThreads - kSoft) * kOtherRegs;
+  }();
+  if (!fits) return HQ_ERR_UNSUPPORTED;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
+  if (!bit || !(ready.load(std::memory_order_acquire) & bit)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    ready.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  kern<<<p.units * p.n_split, kThreads, kSmem, st>>>(p, km, vm);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || p.n_split == 1) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.T) * p.Hkv * p.nrep + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, join_kernel<DT>, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return static_cast<int>(e);
+  }
+  return HQ_OK;
+}
+
+}  // namespace pk
+}  // namespace hq
+
+using namespace hq;
+
+extern "C" size_t hq_packed_prefill_workspace_bytes(int T, int Tk, int B, int Hq, int Hkv, int D) {
+  if (T <= 0 || Tk < 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D != pk::kD) return 0;
+  pk::Plan pl{};
+  return pk::plan(pl, T, Tk, B, Hkv, Hq / Hkv) ? std::max<size_t>(pl.bytes, 256) : 0;
+}
+
+extern "C" int hq_packed_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t q_strides[2],
+                                 const int64_t k_strides[2], const int64_t v_strides[2], const int* cu_q,
+                                 const int* cu_k, int T, int Tk, int B, int Hq, int Hkv, int D, int causal,
+                                 float sm_scale, void* out, const int64_t out_strides[2], int zero_rest,
+                                 void* workspace, size_t workspace_bytes, int* status, hq_stream_t stream) {
+  if (T < 0 || Tk < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || !q_strides || !k_strides || !v_strides || !out_strides ||
+      !(sm_scale > 0.0f) || !(sm_scale < INFINITY))
+    return HQ_ERR_INVALID_ARGUMENT;
+  if (D != pk::kD || Hq % Hkv || (dtype != HQ_DTYPE_BF16 && dtype != HQ_DTYPE_F16)) return HQ_ERR_UNSUPPORTED;
+  if (T == 0 || (B == 0 && !zero_rest)) return HQ_OK;
+  auto al = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
+  if (!q || !out || !cu_q || !cu_k || (Tk > 0 && (!k || !v)) || !al(q) || !al(k) || !al(v) || !al(out))
+    return HQ_ERR_INVALID_ARGUMENT;
+  const int64_t* in[4] = {q_strides, k_strides, v_strides, out_strides};
+  for (const int64_t* s : in)
+    if (s[0] % 8 || s[1] % 8 || s[0] < 0 || s[1] < 0) return HQ_ERR_INVALID_ARGUMENT;
+  if ((T > 1 && out_strides[0] == 0) || (Hq > 1 && out_strides[1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
+  // TMA takes no stride of 0
+  for (int i = 1; i < 3 && Tk > 0; ++i)
+    if ((Tk > 1 && in[i][0] == 0) || (Hkv > 1 && in[i][1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
+  pk::Plan pl{};
+  if (!pk::plan(pl, T, Tk, std::max(B, 1), Hkv, Hq / Hkv)) return HQ_ERR_UNSUPPORTED;
+  if (pl.bytes && (!workspace || workspace_bytes < pl.bytes || !al(workspace))) return HQ_ERR_WORKSPACE;
+  pk::Params p{};
+  p.q = q;
+  p.out = out;
+  for (int i = 0; i < 2; ++i) {
+    p.qs[i] = q_strides[i];
+    p.os[i] = out_strides[i];
+  }
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.T = T;
+  p.Tk = Tk;
+  p.B = B;
+  p.Hkv = Hkv;
+  p.nrep = Hq / Hkv;
+  p.causal = causal;
+  p.c = sm_scale * 1.4426950408889634f;
+  p.n_split = pl.n_split;
+  p.units = pl.units;
+  p.zero_rest = zero_rest;
+  p.part = static_cast<float*>(workspace);
+  p.status = status;
+  CUtensorMap km{}, vm{};
+  if (Tk > 0) {
+    // strides in rising order, K's and V's alike
+    p.swap = Hkv > 1 && k_strides[1] > k_strides[0];
+    if (Hkv > 1 && (v_strides[1] > v_strides[0]) != (p.swap != 0)) return HQ_ERR_INVALID_ARGUMENT;
+    int64_t ks[2] = {Tk > 1 ? k_strides[0] : int64_t(Hkv) * pk::kD, k_strides[1]}, vs[2] = {Tk > 1 ? v_strides[0] : int64_t(Hkv) * pk::kD, v_strides[1]};
+    int rc = pk::encode(&km, k, dtype, ks, Tk, Hkv, p.swap);
+    if (rc == HQ_OK) rc = pk::encode(&vm, v, dtype, vs, Tk, Hkv, p.swap);
+    if (rc != HQ_OK) return rc;
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == HQ_DTYPE_BF16 ? pk::launch<HQ_DTYPE_BF16>(p, km, vm, st) : pk::launch<HQ_DTYPE_F16>(p, km, vm, st);
+}

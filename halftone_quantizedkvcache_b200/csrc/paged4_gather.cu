@@ -1,0 +1,149 @@
+// Tokens of a paged 4-bit cache as packed 16-bit rows (sm_100a): row cu[b] + i takes token
+// first[b] + i of sequence b, the value s * code rounded once to the row's type.
+//
+// Bound by memory: 144 bytes read and 512 written per token and kv head.  16 lanes hold a row (a
+// word of 8 codes each); a half-warp takes one row and all of its heads, K and V.
+#include <algorithm>
+
+#include "paged4.cuh"
+
+namespace hq {
+int current_sm_count();
+
+namespace p4 {
+
+struct GatherParams {
+  Pages pg;
+  int T, B, Hkv;
+  const int* cu;
+  const int* lens;
+  const int* first;                       // null: 0
+  void* k_out;
+  void* v_out;
+  int64_t ks[2], vs[2];
+  int zero_rest;                          // rows that no token goes to become zeros
+  int* status;
+  int heads_per_block, groups;
+};
+
+template <int DT>
+__device__ __forceinline__ uint4 values8(uint32_t w, float s) {
+  uint32_t out[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float a = s * static_cast<float>(static_cast<int>((w >> (8 * e)) & 15u) - 8);
+    const float b = s * static_cast<float>(static_cast<int>((w >> (8 * e + 4)) & 15u) - 8);
+    if constexpr (DT == HQ_DTYPE_BF16) {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+      out[e] = *reinterpret_cast<const uint32_t*>(&x);
+    } else {
+      const __half2 x = __floats2half2_rn(a, b);
+      out[e] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+  }
+  return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+constexpr int kGThreads = 256;
+constexpr int kGRows = kGThreads / 16;
+
+template <int DT>
+__global__ void __launch_bounds__(kGThreads) gather_kernel(const __grid_constant__ GatherParams p) {
+  const int tid = threadIdx.x, lane = tid & 31, sub = tid >> 4, l = lane & 15;
+  const int group = static_cast<int>(blockIdx.x % p.groups);
+  const int64_t row64 = static_cast<int64_t>(blockIdx.x / p.groups) * kGRows + sub;
+  const bool here = row64 < p.T;
+  const int row = static_cast<int>(here ? row64 : p.T - 1);
+  const int b = find_seq(p.cu, p.B, row);
+  bool held = here && b < p.B;
+  int pid = 0;
+  int64_t at = 0;
+  if (held) {
+    const int64_t cap = static_cast<int64_t>(p.pg.max_pages) << p.pg.page_log;
+    const int64_t i = row - static_cast<int64_t>(p.cu[b]);
+    at = i + (p.first ? max(p.first[b], 0) : 0);
+    held = i >= 0 && at < min(static_cast<int64_t>(max(p.lens[b], 0)), cap);
+    if (held) {
+      pid = p.pg.tables[b * p.pg.tstride + (at >> p.pg.page_log)];
+      if (pid < 0 || pid >= p.pg.n_pages) {
+        if (l == 0) report_error(p.status, HQ_ERR_INVALID_ARGUMENT);
+        held = false;
+      }
+    }
+  }
+  if (!held && !(here && p.zero_rest)) return;
+  const int place = static_cast<int>(at) & (p.pg.page - 1);
+  const int h0 = group * p.heads_per_block, h1 = min(p.Hkv, h0 + p.heads_per_block);
+  const int64_t cat = pid * p.pg.cp + place * kRowB + word_at(place, l >> 2, l & 3);
+  const int64_t sat = pid * p.pg.sp + place * 4 + (l >> 2);
+#pragma unroll 2
+  for (int h = h0; h < h1; ++h) {
+    uint4 k = make_uint4(0, 0, 0, 0), v = k;
+    if (held) {
+      const uint32_t kw = *reinterpret_cast<const uint32_t*>(p.pg.k + cat + h * p.pg.ch);
+      const uint32_t vw = *reinterpret_cast<const uint32_t*>(p.pg.v + cat + h * p.pg.ch);
+      const float ks = __half2float(p.pg.ksc[sat + h * p.pg.sh]), vs = __half2float(p.pg.vsc[sat + h * p.pg.sh]);
+      k = values8<DT>(kw, ks);
+      v = values8<DT>(vw, vs);
+    }
+    *reinterpret_cast<uint4*>(static_cast<char*>(p.k_out) + 2 * (row * p.ks[0] + h * p.ks[1] + 8 * l)) = k;
+    *reinterpret_cast<uint4*>(static_cast<char*>(p.v_out) + 2 * (row * p.vs[0] + h * p.vs[1] + 8 * l)) = v;
+  }
+}
+
+}  // namespace p4
+}  // namespace hq
+
+using namespace hq;
+
+extern "C" int hq_paged4_gather(const uint8_t* k_codes, const uint8_t* v_codes, const int64_t code_strides[2],
+                                const void* k_scale, const void* v_scale, const int64_t scale_strides[2],
+                                int n_pages, int page_size, const int* tables, int64_t table_stride,
+                                int max_pages, const int* lens, const int* first, const int* cu_seqlens,
+                                int T, int B, int Hkv, int D, void* k_out, void* v_out, int out_dtype,
+                                const int64_t k_strides[2], const int64_t v_strides[2], int zero_rest,
+                                int* status, hq_stream_t stream) {
+  if (T < 0 || B < 0 || Hkv <= 0 || !k_strides || !v_strides || !cu_seqlens) return HQ_ERR_INVALID_ARGUMENT;
+  if (D != p4::kD || (out_dtype != HQ_DTYPE_BF16 && out_dtype != HQ_DTYPE_F16) || Hkv > 65535) return HQ_ERR_UNSUPPORTED;
+  const int rc = p4::check_pages(k_codes, v_codes, k_scale, v_scale, code_strides, scale_strides, n_pages,
+                                 page_size, tables, table_stride, max_pages, B, Hkv);
+  if (rc != HQ_OK) return rc;
+  if (T == 0) return HQ_OK;
+  auto al = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
+  if (!k_out || !v_out || (B > 0 && !lens) || !al(k_out) || !al(v_out) || k_strides[0] % 8 || k_strides[1] % 8 ||
+      v_strides[0] % 8 || v_strides[1] % 8)
+    return HQ_ERR_INVALID_ARGUMENT;
+  const int64_t* w[2] = {k_strides, v_strides};
+  for (const int64_t* s : w)
+    if ((T > 1 && s[0] == 0) || (Hkv > 1 && s[1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
+  p4::GatherParams p{};
+  p.pg = p4::make_pages(k_codes, v_codes, k_scale, v_scale, code_strides, scale_strides, n_pages, page_size,
+                        tables, table_stride, max_pages);
+  p.T = T;
+  p.B = B;
+  p.Hkv = Hkv;
+  p.cu = cu_seqlens;
+  p.lens = lens;
+  p.first = first;
+  p.k_out = k_out;
+  p.v_out = v_out;
+  for (int i = 0; i < 2; ++i) {
+    p.ks[i] = k_strides[i];
+    p.vs[i] = v_strides[i];
+  }
+  p.zero_rest = zero_rest;
+  p.status = status;
+  const int64_t blocks = (static_cast<int64_t>(T) + p4::kGRows - 1) / p4::kGRows;
+  // a row's heads stay together as long as that leaves 4 blocks an SM
+  const int64_t want = std::max<int64_t>(1, 4LL * current_sm_count() / blocks);
+  const int groups = static_cast<int>(std::min<int64_t>(Hkv, want));
+  p.heads_per_block = (Hkv + groups - 1) / groups;
+  p.groups = (Hkv + p.heads_per_block - 1) / p.heads_per_block;
+  if (blocks * p.groups > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const unsigned grid = static_cast<unsigned>(blocks * p.groups);
+  if (out_dtype == HQ_DTYPE_BF16) p4::gather_kernel<HQ_DTYPE_BF16><<<grid, p4::kGThreads, 0, st>>>(p);
+  else p4::gather_kernel<HQ_DTYPE_F16><<<grid, p4::kGThreads, 0, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? HQ_OK : static_cast<int>(e);
+}

@@ -938,9 +938,10 @@ def _status_word(dev: torch.device) -> torch.Tensor:
 
 def ragged_status(device=None) -> int:
     """Status of the ragged-batch kernels (``int8_window_decode_attn``,
-    ``int8_window_prefill_attn``, ``int8_prefix_decode_attn``, ``rope_append_kv``) on a device
-    since it was last reset: 0, or the first error found on the device (a wait that gave up, a
-    sequence whose new tokens did not fit).  Synchronises the device."""
+    ``int8_window_prefill_attn``, ``int8_prefix_decode_attn``, ``rope_append_kv``, ``paged4_append``,
+    ``paged4_decode_attn``, ``paged4_gather``, ``packed_prefill_attn``) on a device since it was last
+    reset: 0, or the first error found on the device (a wait that gave up, a sequence whose new tokens
+    did not fit, a page number that is none).  Synchronises the device."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     t = _ragged_status.get(dev.index if dev.index is not None else torch.cuda.current_device())
     if t is None:
@@ -1481,3 +1482,441 @@ def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache
     if rc:
         check(rc, "hq_rope_append_kv")
     return q_out
+
+
+# ---------------------------------------------------------------- paged cache in 4 bits
+PAGED4_SIZES = (16, 32, 64, 128, 256)
+
+
+def paged4_alloc(n_pages: int, n_kv_heads: int, *, page_size: int = 64, head_dim: int = 128,
+                 device=None) -> dict:
+    """Pages of a cache held in 4 bits (``paged4_append`` / ``paged4_decode_attn`` /
+    ``paged4_gather``): codes ``k`` / ``v`` uint8 ``[n_pages,Hkv,page_size,64]`` and scales
+    ``k_scale`` / ``v_scale`` float16 ``[n_pages,Hkv,page_size,4]``, 144 bytes per token and kv head.
+    Per token 4 groups of 32 channels: ``s = f16(amax / 7.5)``, codes ``clamp(rint(x / s), -8, 7)``
+    (the byte order within a row is the kernels' own, include/halftone_b200.h; ``paged4_gather``
+    reads it).  Which pages a sequence has is the caller's block table."""
+    if page_size not in PAGED4_SIZES:
+        raise ValueError(f"paged4: page_size must be one of {PAGED4_SIZES}")
+    if head_dim != 128:
+        raise ValueError("paged4: head_dim must be 128")
+    if n_pages < 1 or n_kv_heads < 1:
+        raise ValueError("paged4: at least one page and one kv head")
+    dev = torch.device("cuda") if device is None else torch.device(device)
+    codes, scales = (n_pages, n_kv_heads, page_size, 64), (n_pages, n_kv_heads, page_size, 4)
+    return {"k": torch.zeros(codes, dtype=torch.uint8, device=dev),
+            "v": torch.zeros(codes, dtype=torch.uint8, device=dev),
+            "k_scale": torch.zeros(scales, dtype=torch.float16, device=dev),
+            "v_scale": torch.zeros(scales, dtype=torch.float16, device=dev)}
+
+
+def _paged4_cache(what: str, cache: dict, tables, B: int, dev):
+    """Checks a paged cache and its block tables; returns (Hkv, page size, C arguments after the
+    codes' and scales' pointers: strides, page count, page size; table stride, pages per table)."""
+    try:
+        k, v, ks, vs = cache["k"], cache["v"], cache["k_scale"], cache["v_scale"]
+    except (TypeError, KeyError):
+        raise ValueError(f"{what}: cache must be a dict of paged4_alloc's buffers") from None
+    _tensors(what, k=k, v=v, k_scale=ks, v_scale=vs, block_tables=tables)
+    for t, n in ((k, "k"), (v, "v"), (ks, "k_scale"), (vs, "v_scale"), (tables, "block_tables")):
+        _cuda(t, f"{what} {n}")
+        if t.device != dev:
+            raise ValueError(f"{what}: {n} is on {t.device}, q on {dev}")
+    if k.dtype != torch.uint8 or v.dtype != torch.uint8 or ks.dtype != torch.float16 or (
+            vs.dtype != torch.float16):
+        raise TypeError(f"{what}: codes must be uint8 and scales float16")
+    if k.dim() != 4 or k.shape[3] != 64 or k.shape[2] not in PAGED4_SIZES or k.shape[0] < 1 or (
+            k.shape[1] < 1):
+        raise ValueError(f"{what}: codes must be [n_pages,Hkv,page_size,64] with page_size one of "
+                         f"{PAGED4_SIZES}, got {tuple(k.shape)}")
+    P, Hkv, page = k.shape[:3]
+    if v.shape != k.shape or tuple(ks.shape) != (P, Hkv, page, 4) or vs.shape != ks.shape:
+        raise ValueError(f"{what}: cache buffers do not fit one another")
+    if k.stride() != v.stride() or ks.stride() != vs.stride():
+        raise ValueError(f"{what}: K and V must share strides")
+    cs, ss = k.stride(), ks.stride()
+    if cs[2:] != (64, 1) or ss[2:] != (4, 1) or cs[0] % 16 or cs[1] % 16 or ss[0] % 8 or ss[1] % 8 or (
+            (k.data_ptr() | v.data_ptr() | ks.data_ptr() | vs.data_ptr()) % 16):
+        raise ValueError(f"{what}: each page and head must be contiguous and 16-byte aligned")
+    for st, n in ((cs, 64 * page), (ss, 4 * page)):
+        if (P > 1 and st[0] < n) or (Hkv > 1 and st[1] < n):
+            raise ValueError(f"{what}: pages and heads must have memory of their own")
+    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != B or (
+            tables.shape[1] and tables.stride(1) != 1):
+        raise ValueError(f"{what}: block_tables must be int32 [{B}, pages], rows contiguous, got "
+                         f"{tables.dtype} {tuple(tables.shape)}")
+    if tables.shape[1] * page > 1 << 30:
+        raise ValueError(f"{what}: a table of more than 2^30 tokens")
+    return (Hkv, _lib.strides(cs[:2], 2), _lib.strides(ss[:2], 2), P, page, max(tables.stride(0), 0),
+            tables.shape[1])
+
+
+def _paged4_key(cache: dict, tables) -> tuple:
+    """What a plan needs of a cache and its tables; an address counts by its alignment alone."""
+    k, v, ks, vs = cache["k"], cache["v"], cache["k_scale"], cache["v_scale"]
+    return (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(),
+            ks.shape, ks.stride(), ks.dtype, ks.get_device(), vs.shape, vs.stride(), vs.dtype,
+            vs.get_device(), (k.data_ptr() | v.data_ptr() | ks.data_ptr() | vs.data_ptr()) % 16,
+            tables.shape, tables.stride(), tables.dtype, tables.get_device())
+
+
+def _packed(what: str, name: str, t, dev, dtype, rows=None, heads=None) -> None:
+    _cuda(t, f"{what} {name}")
+    if t.device != dev:
+        raise ValueError(f"{what}: {name} is on {t.device}, q on {dev}")
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 3 or t.shape[2] != 128 or (rows is not None and t.shape[0] != rows) or (
+            heads is not None and t.shape[1] != heads) or t.shape[1] < 1:
+        raise ValueError(f"{what}: {name} must be [{'T' if rows is None else rows},"
+                         f"{'H' if heads is None else heads},128], got {tuple(t.shape)}")
+
+
+def _packed_out(what: str, name: str, t, shape, q) -> None:
+    if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape) or t.dtype != q.dtype or (
+            t.device != q.device) or not _rows_ok(t):
+        raise ValueError(f"{what}: {name} must be {tuple(shape)} of q's dtype and device, with "
+                         "16-byte aligned rows")
+    if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+        raise ValueError(f"{what}: {name} must have rows of its own")
+
+
+def _need16(what: str, q) -> None:
+    _cuda(q, f"{what} q")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: q must be bfloat16 or float16")
+
+
+def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None, inv_freq=None,
+                  interleaved=False, factor=1.0, pos_offset=None, q_weight=None, k_weight=None,
+                  eps=1e-6, q_out=None, k_out=None):
+    """New tokens into a paged 4-bit cache, with the norms of q and k per head and the rotation by
+    position on the way, in one launch (``hq_paged4_append``).
+
+    q ``[T,Hq,128]``, k_new / v_new ``[T,Hkv,128]`` (bf16/f16; token and head strides may be those of
+    a fused projection's output), packed: rows ``cu_seqlens[b] .. cu_seqlens[b+1]-1`` (int32
+    ``[B+1]``) are sequence b's new tokens; without ``cu_seqlens`` T is B, one token each.  Token i
+    of them goes to place ``lens[b] + i`` of the pages ``block_tables`` (int32 ``[B,pages]``) names
+    and stands at position ``lens[b] + i + pos_offset[b]``; ``lens`` (int32 ``[B]``) is not advanced.
+    ``q_weight`` / ``k_weight`` ``[128]`` (q's dtype or float32): the row becomes ``w x /
+    sqrt(mean(x^2) + eps)``; ``inv_freq`` float32 ``[rotary_dim / 2]`` (``rope_inv_freq``;
+    rotary_dim a multiple of 16) turns its first channels, half-split or ``interleaved``, cos and sin
+    times ``factor``.  Both happen in float32 and are rounded once.  K is coded from the unrounded
+    rotated values, codes and scales those of exact arithmetic; V as it came.
+
+    Returns the new q (``q_out``, which may be q; rows behind the last sequence stay what they were
+    there, or are q's in a result made by this call); ``k_out [T,Hkv,128]`` takes the new k, for the
+    prompt's own attention.  K and V of real tokens are finite (others spoil their group).  A
+    sequence whose tokens do not fit its table, and a token whose page is no page of the cache, are
+    not written and set ``ragged_status()``; no two new tokens may go to the same place.
+    """
+    what = "paged4_append"
+    try:
+        key = (what, q.shape, q.stride(), q.dtype, q.get_device(), k_new.shape, k_new.stride(),
+               k_new.dtype, k_new.get_device(), v_new.shape, v_new.stride(), v_new.dtype,
+               v_new.get_device(), lens.shape, lens.stride(), lens.dtype, lens.get_device())
+        key += _paged4_key(cache, block_tables)
+        for t in (cu_seqlens, inv_freq, pos_offset, q_weight, k_weight):
+            key += _sig_opt(t)
+    except (AttributeError, TypeError, KeyError):
+        _tensors(what, q=q, k_new=k_new, v_new=v_new, lens=lens)
+        for t, n in ((cu_seqlens, "cu_seqlens"), (inv_freq, "inv_freq"), (pos_offset, "pos_offset"),
+                     (q_weight, "q_weight"), (k_weight, "k_weight")):
+            if t is not None and not isinstance(t, torch.Tensor):
+                raise ValueError(f"{what}: {n} must be a tensor, got {type(t).__name__}") from None
+        _paged4_cache(what, cache, block_tables, lens.numel(), q.device)
+        raise
+    plan = _plans.get(key)
+    if plan is None:
+        _need16(what, q)
+        dev = q.device
+        _packed(what, "q", q, dev, q.dtype)
+        T, Hq, D = q.shape
+        if lens.dim() != 1:
+            raise ValueError(f"{what}: lens must be int32 [B]")
+        B = lens.shape[0]
+        Hkv, *pages = _paged4_cache(what, cache, block_tables, B, dev)
+        _packed(what, "k_new", k_new, dev, q.dtype, T, Hkv)
+        _packed(what, "v_new", v_new, dev, q.dtype, T, Hkv)
+        _lens_ok(what, "lens", lens, B, dev)
+        _lens_ok(what, "cu_seqlens", cu_seqlens, B + 1, dev)
+        _lens_ok(what, "pos_offset", pos_offset, B, dev)
+        if cu_seqlens is None and T != B:
+            raise ValueError(f"{what}: {T} tokens for {B} sequences need cu_seqlens")
+        wdt = None
+        for t, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+            if t is None:
+                continue
+            _cuda(t, f"{what} {n}")
+            if tuple(t.shape) != (D,) or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"{what}: {n} must be a contiguous [{D}] tensor on q's device")
+            if t.dtype not in (q.dtype, torch.float32) or wdt not in (None, t.dtype):
+                raise TypeError(f"{what}: norm weights must both have q's dtype, or be float32")
+            wdt = t.dtype
+        rot = 0
+        if inv_freq is not None:
+            _cuda(inv_freq, f"{what} inv_freq")
+            rot = 2 * inv_freq.numel()
+            if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or inv_freq.device != dev or (
+                    not inv_freq.is_contiguous() or rot > D or rot % 16):
+                raise ValueError(f"{what}: inv_freq must be contiguous float32 on q's device, for a "
+                                 f"rotary_dim of 16, 32, .. {D}")
+        in_place = _rows_strided(q) and _rows_strided(k_new) and _rows_strided(v_new)
+        plan = _keep(key, (dev, T, B, Hq, Hkv, in_place, q.is_contiguous(), _DT[q.dtype],
+                           _DT[wdt or q.dtype], rot,
+                           *[_lib.strides(x.stride()[:2], 2) for x in (q, k_new, v_new)], *pages,
+                           _lib.strides((Hq * D, D), 2), _lib.lib().hq_paged4_append))
+    (dev, T, B, Hq, Hkv, in_place, dense, dt, wdt, rot, qst, kst, vst, cst, sst, n_pages, page, tst,
+     max_pages, ost, fn) = plan
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return paged4_append(q, k_new, v_new, cache, block_tables, lens, cu_seqlens=cu_seqlens,
+                                 inv_freq=inv_freq, interleaved=interleaved, factor=factor,
+                                 pos_offset=pos_offset, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                 q_out=q_out, k_out=k_out)
+    if not eps >= 0:
+        raise ValueError(f"{what}: eps must not be negative")
+    qp, kp, vp = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr()
+    if not in_place or (qp | kp | vp) % 16:  # rows that the kernel cannot read in place
+        q, k_new, v_new = _aligned_rows(q), _aligned_rows(k_new), _aligned_rows(v_new)
+        qst, kst, vst = (_lib.strides(x.stride()[:2], 2) for x in (q, k_new, v_new))
+        qp, kp, vp = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr()
+    rest = q_out is None
+    if rest:
+        q_out = torch.empty_like(q) if dense else q.new_empty(q.shape)
+    else:
+        _packed_out(what, "q_out", q_out, q.shape, q)
+        ost = _lib.strides(q_out.stride()[:2], 2)
+    kop, kost = None, None
+    if k_out is not None:
+        _packed_out(what, "k_out", k_out, (T, Hkv, 128), q)
+        kop, kost = k_out.data_ptr(), _lib.strides(k_out.stride()[:2], 2)
+    if T == 0:
+        return q_out
+    if B == 0:
+        return q_out.copy_(q) if rest else q_out
+    rc = fn(qp, kp, vp, dt, qst, kst, vst, T, B, Hq, Hkv, 128,
+            cu_seqlens.data_ptr() if cu_seqlens is not None else None, lens.data_ptr(),
+            pos_offset.data_ptr() if pos_offset is not None else None,
+            q_weight.data_ptr() if q_weight is not None else None,
+            k_weight.data_ptr() if k_weight is not None else None, wdt, eps,
+            inv_freq.data_ptr() if rot else None, rot, 1 if interleaved else 0, factor,
+            cache["k"].data_ptr(), cache["v"].data_ptr(), cst, cache["k_scale"].data_ptr(),
+            cache["v_scale"].data_ptr(), sst, n_pages, page, block_tables.data_ptr(), tst, max_pages,
+            q_out.data_ptr(), ost, kop, kost, 1 if rest else 0, _status_word(dev).data_ptr(),
+            _stream(dev))
+    if rc:
+        check(rc, "hq_paged4_append")
+    return q_out
+
+
+def paged4_decode_attn(q, cache, block_tables, lens, *, sm_scale=None, out=None):
+    """One decode step of a ragged batch over a paged 4-bit cache (``hq_paged4_decode``).
+
+    q ``[B,Hq,128]`` or ``[B,Hq,1,128]`` (bf16/f16); ``cache`` as ``paged4_alloc`` makes it,
+    ``block_tables`` int32 ``[B,pages]`` and ``lens`` int32 ``[B]`` on the device: sequence b attends
+    its first ``lens[b]`` tokens (at most those its table holds), and gives zeros where there are
+    none.  What pages hold past them does not matter.  Returns the output in q's layout and dtype (or
+    writes ``out [B,Hq,128]``).  Nothing depends on ``lens`` on the host: a captured call replays while
+    sequences grow.  Scores and sums are float32; q and the weights are split in two bf16 parts (2^-17
+    of each).  A page number outside the cache sets ``ragged_status()``, and that sequence's output
+    has no meaning.
+    """
+    what = "paged4_decode_attn"
+    try:
+        key = (what, q.shape, q.stride(), q.dtype, q.get_device(), lens.shape, lens.stride(), lens.dtype,
+               lens.get_device())
+        key += _paged4_key(cache, block_tables)
+    except (AttributeError, TypeError, KeyError):
+        _tensors(what, q=q, lens=lens)
+        _paged4_cache(what, cache, block_tables, q.shape[0] if q.dim() else 0, q.device)
+        raise
+    plan = _plans.get(key)
+    if plan is None:
+        _need16(what, q)
+        if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[2] != 1) or q.shape[-1] != 128 or (
+                q.shape[1] < 1):
+            raise ValueError(f"{what}: q must be [B,Hq,128] or [B,Hq,1,128], got {tuple(q.shape)}")
+        B, Hq, D = q.shape[0], q.shape[1], 128
+        dev = q.device
+        Hkv, *pages = _paged4_cache(what, cache, block_tables, B, dev)
+        _attn_common(what, q, Hq, Hkv)
+        _lens_ok(what, "lens", lens, B, dev)
+        qb = q if q.dim() == 3 else q[:, :, 0]
+        in_place = _rows_strided(qb)
+        ost = _lib.strides((Hq * D, D), 2)
+        with _on_device(dev):
+            nb = _ws_size(what, dev, _lib.lib().hq_paged4_decode_workspace_bytes(
+                max(B, 1), Hq, Hkv, pages[3], pages[5], D))
+        plan = _keep(key, (dev, (B, Hq, D), q.shape, in_place and q.is_contiguous(), _DT[q.dtype],
+                           _lib.strides(qb.stride()[:2], 2) if in_place else ost, in_place, Hkv, *pages,
+                           nb, (nb + 3) // 4, ost, 1.0 / math.sqrt(D), _lib.lib().hq_paged4_decode))
+    (dev, (B, Hq, D), shape, dense, dt, qst, in_place, Hkv, cst, sst, n_pages, page, tst, max_pages, nb,
+     nw, ost, default_scale, fn) = plan
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return paged4_decode_attn(q, cache, block_tables, lens, sm_scale=sm_scale, out=out)
+    qp = q.data_ptr()
+    if not in_place or qp % 16:  # rows that the kernel cannot read in place
+        q, qst = q.clone(memory_format=torch.contiguous_format), ost
+        qp = q.data_ptr()
+    if out is None:
+        out = torch.empty_like(q) if dense else q.new_empty(shape)
+        ost = _lib.strides((Hq * D, D), 2)
+    else:
+        _out_like(what, out, (B, Hq, D), q)
+        if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+            raise ValueError(f"{what}: out must have rows of its own")
+        ost = _lib.strides(out.stride()[:2], 2)
+    if B == 0:
+        return out
+    status = _status_word(dev)
+    ws = status.new_empty(nw)
+    rc = fn(qp, dt, qst, cache["k"].data_ptr(), cache["v"].data_ptr(), cst, cache["k_scale"].data_ptr(),
+            cache["v_scale"].data_ptr(), sst, n_pages, page, block_tables.data_ptr(), tst, max_pages,
+            lens.data_ptr(), B, Hq, Hkv, D, default_scale if sm_scale is None else sm_scale,
+            out.data_ptr(), ost, ws.data_ptr(), nb, status.data_ptr(), _stream(dev))
+    if rc:
+        check(rc, "hq_paged4_decode")
+    return out
+
+
+def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, dtype=torch.bfloat16,
+                  k_out=None, v_out=None):
+    """Tokens of a paged 4-bit cache as packed 16-bit rows (``hq_paged4_gather``): ``(k, v)``
+    ``[n_rows,Hkv,128]`` of ``dtype``, or ``k_out`` / ``v_out``.
+
+    Row ``cu_seqlens[b] + i`` takes token ``first[b] + i`` (``first`` int32 ``[B]``, default 0) of
+    sequence b, as long as that is below ``lens[b]`` and the row below ``cu_seqlens[b+1]``: what a
+    chunk over a cached past attends (``packed_prefill_attn``), or with ``first`` the new tokens as
+    later steps will see them.  Values are ``scale * code``, rounded once.  Rows that no token goes to
+    are zeros, or what they were in ``k_out`` / ``v_out``.  A page number outside the cache sets
+    ``ragged_status()``; that token's row counts as one that no token goes to.
+    """
+    what = "paged4_gather"
+    _tensors(what, lens=lens, cu_seqlens=cu_seqlens)
+    if first is not None:
+        _tensors(what, first=first)
+    n_rows = operator.index(n_rows)
+    if n_rows < 0 or n_rows > 0x7fffffff:
+        raise ValueError(f"{what}: n_rows must be 0 .. 2^31 - 1")
+    if (k_out is None) != (v_out is None):
+        raise ValueError(f"{what}: k_out and v_out come together")
+    if k_out is not None:
+        _tensors(what, k_out=k_out, v_out=v_out)
+        dtype = k_out.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: rows must be bfloat16 or float16")
+    _cuda(lens, f"{what} lens")
+    dev = lens.device
+    if lens.dim() != 1:
+        raise ValueError(f"{what}: lens must be int32 [B]")
+    B = lens.shape[0]
+    Hkv, cst, sst, n_pages, page, tst, max_pages = _paged4_cache(what, cache, block_tables, B, dev)
+    _lens_ok(what, "lens", lens, B, dev)
+    _lens_ok(what, "cu_seqlens", cu_seqlens, B + 1, dev)
+    _lens_ok(what, "first", first, B, dev)
+    made = k_out is None
+    if made:
+        k_out, v_out = (torch.empty((n_rows, Hkv, 128), dtype=dtype, device=dev) for _ in range(2))
+    else:
+        for t, n in ((k_out, "k_out"), (v_out, "v_out")):
+            if t.device != dev:
+                raise ValueError(f"{what}: {n} is on {t.device}, the cache on {dev}")
+            _packed_out(what, n, t, (n_rows, Hkv, 128), k_out)
+    if n_rows == 0:
+        return k_out, v_out
+    with _on_device(dev):
+        rc = _lib.lib().hq_paged4_gather(
+            cache["k"].data_ptr(), cache["v"].data_ptr(), cst, cache["k_scale"].data_ptr(),
+            cache["v_scale"].data_ptr(), sst, n_pages, page, block_tables.data_ptr(), tst, max_pages,
+            lens.data_ptr(), first.data_ptr() if first is not None else None, cu_seqlens.data_ptr(),
+            n_rows, B, Hkv, 128, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype],
+            _lib.strides(k_out.stride()[:2], 2), _lib.strides(v_out.stride()[:2], 2), 1 if made else 0,
+            _status_word(dev).data_ptr(), _stream(dev))
+    if rc:
+        check(rc, "hq_paged4_gather")
+    return k_out, v_out
+
+
+def packed_prefill_attn(q, k, v, cu_q, cu_k=None, *, causal=True, sm_scale=None, out=None):
+    """Attention of packed sequences of different lengths over 16-bit K and V, grouped heads, in one
+    launch (two where few rows have many keys; ``hq_packed_prefill``).
+
+    q ``[T,Hq,128]``, k / v ``[Tk,Hkv,128]`` (bf16/f16); sequence b has the queries
+    ``cu_q[b] .. cu_q[b+1]-1`` and the keys ``cu_k[b] .. cu_k[b+1]-1`` (int32 ``[B+1]`` on the device;
+    ``cu_k`` defaults to ``cu_q``: whole prompts).  The queries stand at the last positions: query i
+    of n sees keys ``j <= m - n + i`` of m (``causal=False``: all of them), and gives zeros where that
+    is none.  Returns ``[T,Hq,128]``; rows behind the last sequence are zeros, or are left as they were
+    in ``out``.  ``sm_scale`` (default 1/sqrt(128)) is positive.  Sums are float32, the weights rounded
+    to q's type.  A V row that holds an infinity or NaN spoils the rows that see it, and no others.
+    """
+    what = "packed_prefill_attn"
+    if cu_k is None:
+        cu_k = cu_q
+    try:
+        key = (what, causal, q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype,
+               k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), cu_q.shape, cu_q.stride(),
+               cu_q.dtype, cu_q.get_device(), cu_k.shape, cu_k.stride(), cu_k.dtype, cu_k.get_device())
+    except AttributeError:
+        _tensors(what, q=q, k=k, v=v, cu_q=cu_q, cu_k=cu_k)
+        raise
+    plan = _plans.get(key)
+    if plan is None:
+        _need16(what, q)
+        dev = q.device
+        _packed(what, "q", q, dev, q.dtype)
+        T, Hq, D = q.shape
+        _packed(what, "k", k, dev, q.dtype)
+        Tk, Hkv = k.shape[:2]
+        _packed(what, "v", v, dev, q.dtype, Tk, Hkv)
+        _attn_common(what, q, Hq, Hkv)
+        if cu_q.dim() != 1 or cu_q.shape[0] < 1:
+            raise ValueError(f"{what}: cu_q must be int32 [B+1]")
+        B = cu_q.shape[0] - 1
+        _lens_ok(what, "cu_q", cu_q, B + 1, dev)
+        _lens_ok(what, "cu_k", cu_k, B + 1, dev)
+
+        def tma(t):  # strides that a tensor map takes
+            return _rows_strided(t) and all(st > 0 or n <= 1 for n, st in zip(t.shape, t.stride()))
+        rising = [t.shape[1] > 1 and t.stride(1) > t.stride(0) for t in (k, v)]
+        with _on_device(dev):
+            nb = 0 if T == 0 or B == 0 else _ws_size(what, dev, _lib.lib().hq_packed_prefill_workspace_bytes(
+                T, Tk, B, Hq, Hkv, D))
+        plan = _keep(key, (dev, T, Tk, B, Hq, Hkv, _DT[q.dtype], 1 if causal else 0, _rows_strided(q),
+                           tma(k) and tma(v) and rising[0] == rising[1],
+                           *[_lib.strides(x.stride()[:2], 2) for x in (q, k, v)], nb, (nb + 3) // 4,
+                           _lib.strides((Hq * D, D), 2), 1.0 / math.sqrt(D), _lib.lib().hq_packed_prefill))
+    (dev, T, Tk, B, Hq, Hkv, dt, causal, q_ok, kv_ok, qst, kst, vst, nb, nw, ost, default_scale,
+     fn) = plan
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return packed_prefill_attn(q, k, v, cu_q, cu_k, causal=causal, sm_scale=sm_scale, out=out)
+    if sm_scale is None:
+        sm_scale = default_scale
+    elif not 0 < sm_scale < math.inf:
+        raise ValueError(f"{what}: sm_scale must be positive and finite")
+    if not q_ok or q.data_ptr() % 16:  # rows that the kernel cannot read in place
+        q = q.clone(memory_format=torch.contiguous_format)
+        qst = _lib.strides(q.stride()[:2], 2)
+    if not kv_ok or (k.data_ptr() | v.data_ptr()) % 16:
+        k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
+        kst, vst = (_lib.strides(t.stride()[:2], 2) for t in (k, v))
+    rest = out is None
+    if rest:
+        out = q.new_empty((T, Hq, 128))
+    else:
+        _packed_out(what, "out", out, (T, Hq, 128), q)
+        ost = _lib.strides(out.stride()[:2], 2)
+    if T == 0:
+        return out
+    if B == 0:
+        return out.zero_() if rest else out
+    status = _status_word(dev)
+    ws = status.new_empty(nw)
+    rc = fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, qst, kst, vst, cu_q.data_ptr(),
+            cu_k.data_ptr(), T, Tk, B, Hq, Hkv, 128, causal, sm_scale, out.data_ptr(), ost,
+            1 if rest else 0, ws.data_ptr(), nb, status.data_ptr(), _stream(dev))
+    if rc:
+        check(rc, "hq_packed_prefill")
+    return out

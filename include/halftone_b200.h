@@ -648,6 +648,90 @@ HQ_API int hq_rope_append_kv(
     const int64_t qo_strides[4], int* status, hq_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * A paged cache held in 4 bits.  Per token and kv head 128 channels in 4 groups
+ * of 32: scale s = f16(amax / 7.5), codes clamp(rint(x / s), -8, 7), values s *
+ * code.  k_codes / v_codes [n_pages, Hkv, page_size, 64] bytes and k_scale /
+ * v_scale [n_pages, Hkv, page_size, 4] float16, each page and head contiguous;
+ * code_strides (bytes, multiples of 16) and scale_strides (elements, multiples
+ * of 8) are {page, head}; page_size 16, 32, 64, 128 or 256.  A row's 64 bytes:
+ * the 16 bytes at position p hold chunk j = p ^ 2 ((t >> 1) & 1), t the token's
+ * place in its page; the chunk's 32-bit word g holds channels 32 g + 8 j + i, i
+ * = 0 .. 7, as code + 8 in bits 4 i .. 4 i + 3.  tables int32 [B, max_pages]
+ * (row stride table_stride): the pages of sequence b, in order; pages past a
+ * sequence's tokens are not read.  Packed arrays [T, H, 128] have strides
+ * {token, head} in elements (rows contiguous, 16-byte aligned).
+ *
+ * hq_paged4_append: new tokens, in one launch.  Packed rows cu_seqlens[b] ..
+ *   cu_seqlens[b + 1] - 1 (int32 [B + 1]; NULL: T == B, one row each) are new
+ *   tokens of sequence b, the i-th at cache place lens[b] + i (lens is not
+ *   advanced) and position lens[b] + i + pos_offset[b] (NULL: 0).  q and k rows
+ *   are normed where there are weights ([128], of x_dtype or F32): w x /
+ *   sqrt(mean(x^2) + eps); then their first rotary_dim channels (a multiple of
+ *   16; 0: none) are turned as in hq_rope_append_kv.  q_out takes q' (may be q),
+ *   k_out (or NULL) k', both rounded once; K is coded from the unrounded k', V as
+ *   it came.  Codes are those of exact arithmetic.  Rows behind the last sequence
+ *   are left as they were (q_out with copy_rest: q's).  A sequence whose tokens do
+ *   not fit its table, or a token whose page is none of the n_pages, is not
+ *   written to the cache and sets HQ_ERR_INVALID_ARGUMENT in `status`.
+ * hq_paged4_decode: one query per sequence (q, out [B, Hq, 128]) over its lens[b]
+ *   tokens (at most the table's); zeros where there are none.  B <= 1024, Hq /
+ *   Hkv <= 128.  The workspace (hq_paged4_decode_workspace_bytes, 256-byte
+ *   aligned, no initial contents) is not shared by launches that may overlap.  A
+ *   page that is none of the n_pages sets HQ_ERR_INVALID_ARGUMENT in `status`;
+ *   that sequence's output has no meaning then.
+ * hq_paged4_gather: rows cu_seqlens[b] + i of k_out / v_out [T, Hkv, 128] take
+ *   token first[b] + i (first NULL: 0) of sequence b, first[b] + i < lens[b], as
+ *   16-bit values rounded once; other rows are left as they were, or with
+ *   zero_rest become zeros.
+ * hq_packed_prefill: attention of packed sequences over 16-bit K and V, T query
+ *   rows and Tk key rows; sequence b has queries cu_q[b] .. and keys cu_k[b] ..,
+ *   query i of n seeing keys j <= m - n + i of m (causal = 0: all); a query that
+ *   sees none gives zeros.  sm_scale > 0.  K and V strides are positive, and both
+ *   have the larger stride at the same place.  A V row that holds an infinity or
+ *   NaN spoils the rows that see it.  Rows behind the last sequence are left as
+ *   they were, or with zero_rest become zeros.  The workspace
+ *   (hq_packed_prefill_workspace_bytes, 16-byte aligned) holds partial states
+ *   where keys are split over blocks.
+ */
+HQ_API int hq_paged4_append(const void* q, const void* k_new, const void* v_new, int x_dtype,
+                            const int64_t q_strides[2], const int64_t k_strides[2],
+                            const int64_t v_strides[2], int T, int B, int Hq, int Hkv, int D,
+                            const int* cu_seqlens, const int* lens, const int* pos_offset,
+                            const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                            const float* inv_freq, int rotary_dim, int interleaved, float factor,
+                            uint8_t* k_codes, uint8_t* v_codes, const int64_t code_strides[2],
+                            void* k_scale, void* v_scale, const int64_t scale_strides[2],
+                            int n_pages, int page_size, const int* tables, int64_t table_stride,
+                            int max_pages, void* q_out, const int64_t qo_strides[2], void* k_out,
+                            const int64_t ko_strides[2], int copy_rest, int* status,
+                            hq_stream_t stream);
+HQ_API size_t hq_paged4_decode_workspace_bytes(int B, int Hq, int Hkv, int page_size, int max_pages,
+                                               int D);
+HQ_API int hq_paged4_decode(const void* q, int q_dtype, const int64_t q_strides[2],
+                            const uint8_t* k_codes, const uint8_t* v_codes,
+                            const int64_t code_strides[2], const void* k_scale, const void* v_scale,
+                            const int64_t scale_strides[2], int n_pages, int page_size,
+                            const int* tables, int64_t table_stride, int max_pages, const int* lens,
+                            int B, int Hq, int Hkv, int D, float sm_scale, void* out,
+                            const int64_t out_strides[2], void* workspace, size_t workspace_bytes,
+                            int* status, hq_stream_t stream);
+HQ_API int hq_paged4_gather(const uint8_t* k_codes, const uint8_t* v_codes,
+                            const int64_t code_strides[2], const void* k_scale, const void* v_scale,
+                            const int64_t scale_strides[2], int n_pages, int page_size,
+                            const int* tables, int64_t table_stride, int max_pages, const int* lens,
+                            const int* first, const int* cu_seqlens, int T, int B, int Hkv, int D,
+                            void* k_out, void* v_out, int out_dtype, const int64_t k_strides[2],
+                            const int64_t v_strides[2], int zero_rest, int* status,
+                            hq_stream_t stream);
+HQ_API size_t hq_packed_prefill_workspace_bytes(int T, int Tk, int B, int Hq, int Hkv, int D);
+HQ_API int hq_packed_prefill(const void* q, const void* k, const void* v, int dtype,
+                             const int64_t q_strides[2], const int64_t k_strides[2],
+                             const int64_t v_strides[2], const int* cu_q, const int* cu_k, int T,
+                             int Tk, int B, int Hq, int Hkv, int D, int causal, float sm_scale,
+                             void* out, const int64_t out_strides[2], int zero_rest, void* workspace,
+                             size_t workspace_bytes, int* status, hq_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Reads (and synchronises `stream` for) the device status word at the start
  * of a quantize-K or decode workspace: HQ_OK, or HQ_ERR_DEVICE_TIMEOUT if a
  * bounded device wait gave up during an earlier call on that workspace.

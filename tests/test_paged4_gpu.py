@@ -1,0 +1,359 @@
+"""The paged 4-bit cache on a GPU against plain float64 forms: append (norms, rotation, codes), decode,
+gather."""
+import math
+
+import pytest
+import torch
+
+import paged4_plain as plain
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "f16": torch.float16}
+D = 128
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def cum(v):
+    return ints([0] + torch.tensor(v).cumsum(0).tolist())
+
+
+def near(got, ref, extra):
+    """Half a step of the output's type, and `extra` for the arithmetic before it."""
+    half = torch.finfo(got.dtype).eps / 2
+    err = (got.double() - ref).abs()
+    bad = ~(err <= half * ref.abs() * 1.01 + extra)
+    assert not bad.any(), (int(bad.sum()), float((err - half * ref.abs()).max()))
+
+
+# ---------------------------------------------------------------- append
+def append_case(new, past, Hkv, rep, dt, page, seed, fused=True):
+    g = gen(seed)
+    T, B = sum(new), len(new)
+    x = torch.randn((T, (rep + 2) * Hkv * D), generator=g, device="cuda").to(dt)
+    q, k, v = (y.unflatten(1, (-1, D)) for y in x.split([rep * Hkv * D, Hkv * D, Hkv * D], 1))
+    if not fused:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    from halftone_quantizedkvcache_b200 import kernels
+    per = max(1, -(-max(a + b for a, b in zip(new, past)) // page))
+    cache = plain.random_cache(kernels, B * per + 3, Hkv, page, g)
+    tables = plain.random_tables(B, per, B * per + 3, g)
+    return q, k, v, cache, tables
+
+
+def check_append(q, k, v, cache, tables, new, past, before, q_got, k_got, inv, weights, inter=False,
+                 factor=1.0, offset=None, eps=1e-6):
+    """Every byte of the cache and every row of q and k."""
+    dev, page = q.device, cache["k"].shape[2]
+    b = torch.repeat_interleave(torch.arange(len(new), device=dev), torch.tensor(new, device=dev))
+    i = torch.cat([torch.arange(n, device=dev) for n in new]) if sum(new) else torch.zeros(0, dtype=torch.long, device=dev)
+    at = torch.tensor(past, device=dev)[b] + i
+    pos = at + (offset.long()[b] if offset is not None else 0)
+    qw, kw = weights if weights is not None else (None, None)
+    n = len(at)
+    q64 = plain.turned(q[:n], qw, pos, inv, inter, factor, eps)
+    k64 = plain.turned(k[:n], kw, pos, inv, inter, factor, eps)
+    # the float32 route: 2^-20 of |x w| + |o w_o| (paged4_append.cu), normed rows below 12 x 2 x 2
+    size = 48.0 if weights is not None else 2.0 * float(k.abs().max()) + 2.0 * float(q.abs().max())
+    near(q_got[:n], q64, 1e-6 * size * abs(factor))
+    if k_got is not None:
+        near(k_got[:n], k64, 1e-6 * size * abs(factor))
+    pg, t = tables.long()[b, at // page], at % page
+    for name, x in (("k", k64), ("v", v[:n].double())):
+        codes, sc = plain.coded(x)
+        rows = before[name].clone()
+        scales = before[name + "_scale"].clone()
+        byte, sh = plain.byte_of(t, dev)
+        row = torch.zeros((n, x.shape[1], 64), dtype=torch.int64, device=dev)
+        row.scatter_add_(2, byte[:, None].expand(-1, x.shape[1], -1), (codes + 8) << sh)
+        rows[pg, :, t], scales[pg, :, t] = row.to(torch.uint8), sc
+        assert torch.equal(cache[name + "_scale"].view(torch.int16), scales.view(torch.int16)), name
+        assert torch.equal(cache[name], rows), (name, int((cache[name] != rows).sum()))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("new,past,Hkv,rep,page,rot,inter,norm", [
+    ([1], [0], 8, 2, 64, 128, False, True),
+    ([1], [4001], 1, 1, 16, 128, True, True),
+    ([1, 1, 1], [63, 64, 65], 2, 4, 64, 64, False, False),
+    ([5, 0, 17, 1], [0, 9, 31, 254], 4, 3, 32, 96, True, True),
+    ([300, 211], [7, 1000], 8, 2, 128, 128, False, True),
+    ([77, 33], [3, 0], 2, 6, 256, 32, False, False),
+    ([40, 9], [3, 0], 3, 1, 16, 0, False, True),
+    ([40, 9], [3, 0], 3, 1, 16, 0, False, False),
+    ([2000], [0], 4, 2, 64, 128, False, True),
+])
+def test_append(dtype, new, past, Hkv, rep, page, rot, inter, norm):
+    from halftone_quantizedkvcache_b200 import kernels
+    q, k, v, cache, tables = append_case(new, past, Hkv, rep, DT[dtype], page, 11)
+    before = {n: x.clone() for n, x in cache.items()}
+    inv = kernels.rope_inv_freq(rot, 1e6)[0] if rot else None
+    g = gen(5)
+    w = [torch.empty(D, device="cuda").uniform_(0.2, 2.0, generator=g).to(DT[dtype]) for _ in range(2)] if norm else None
+    k_out = torch.zeros_like(k, memory_format=torch.contiguous_format)
+    got = kernels.paged4_append(q, k, v, cache, tables, ints(past), cu_seqlens=cum(new), inv_freq=inv,
+                                interleaved=inter, q_weight=w and w[0], k_weight=w and w[1], k_out=k_out)
+    check_append(q, k, v, cache, tables, new, past, before, got, k_out, inv, w, inter)
+    assert kernels.ragged_status() == 0
+
+
+def test_append_without_starts_far_positions_and_float32_weights():
+    from halftone_quantizedkvcache_b200 import kernels
+    new, past = [1] * 7, [0, 5, 100, 3, 64, 63, 1]
+    q, k, v, cache, tables = append_case(new, past, 4, 2, torch.bfloat16, 16, 3, fused=False)
+    before = {n: x.clone() for n, x in cache.items()}
+    inv, factor = kernels.rope_inv_freq(128, 1e4, scaling="yarn", factor=4.0, original_len=4096)
+    off = ints([0, 1 << 20, 999_983, 131_072, 1, 2, 2_000_003])
+    w = [torch.rand(D, device="cuda", generator=gen(1)) + 0.5 for _ in range(2)]
+    q0 = q.clone()
+    got = kernels.paged4_append(q, k, v, cache, tables, ints(past), inv_freq=inv, factor=factor,
+                                pos_offset=off, q_weight=w[0], k_weight=w[1], eps=1e-5, q_out=q)
+    assert got is q
+    check_append(q0, k, v, cache, tables, new, past, before, got, None, inv, w, False, factor, off, 1e-5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_append_values_of_every_kind(dtype):
+    """Zeros, subnormals, the largest values, exact ties of x / s: all as the float64 form has them."""
+    from halftone_quantizedkvcache_b200 import kernels
+    dt = DT[dtype]
+    q, k, v, cache, tables = append_case([64], [0], 2, 1, dt, 64, 4, fused=False)
+    for x in (k, v):
+        x[0] = 0
+        x[1] *= torch.finfo(dt).tiny
+        x[2] = (x[2].sign() * 60000.0 * torch.rand_like(x[2].float())).to(dt)
+        x[3] *= 1e-6
+        # s = 2^-3 exactly, every quotient k / 2: ties at the odd ones
+        x[4] = (torch.arange(D, device="cuda") % 31 - 15).to(dt) / 16
+        x[4, :, ::32] = 7.5 / 8
+        x[5] = x[4] * 1024
+        x[6, :, 32:64] = 0
+        x[7, :, 3] *= 300
+    before = {n: x.clone() for n, x in cache.items()}
+    got = kernels.paged4_append(q, k, v, cache, tables, ints([0]), cu_seqlens=ints([0, 64]))
+    assert torch.equal(got, q)
+    check_append(q, k, v, cache, tables, [64], [0], before, got, None, None, None)
+
+
+def test_append_scale_beyond_float16_saturates():
+    from halftone_quantizedkvcache_b200 import kernels
+    q, k, v, cache, tables = append_case([2], [0], 1, 1, torch.bfloat16, 16, 4, fused=False)
+    v[0] = 1e6 * v[0].sign()
+    v[1, 0, 40] = math.inf
+    k[1, 0, 100] = math.nan
+    kernels.paged4_append(q, k, v, cache, tables, ints([0]), cu_seqlens=ints([0, 2]))
+    kv, vv = kernels.paged4_gather(cache, tables, ints([2]), ints([0, 2]), 2, dtype=torch.bfloat16)
+    assert torch.equal(vv[0], (torch.where(v[0] < 0, -8.0, 7.0) * 65504.0).to(torch.bfloat16))
+    # a group that holds no number says so, the others of its row do not care
+    assert vv[1, 0, 32:64].isnan().all() and vv[1, 0, :32].isfinite().all() and vv[1, 0, 64:].isfinite().all()
+    assert kv[1, 0, 96:].isnan().all() and kv[1, 0, :96].isfinite().all()
+
+
+def test_append_that_does_not_fit_writes_nothing():
+    from halftone_quantizedkvcache_b200 import kernels
+    new, past = [4, 3, 2], [13, 0, 5]
+    q, k, v, cache, tables = append_case(new, [0, 0, 0], 2, 2, torch.bfloat16, 16, 9)   # 16 places each
+    before = {n: x.clone() for n, x in cache.items()}
+    kernels.reset_ragged_status()
+    tables[2, 0] = cache["k"].shape[0]           # no page of the cache
+    got = kernels.paged4_append(q, k, v, cache, tables, ints(past), cu_seqlens=cum(new))
+    assert kernels.ragged_status() == -1
+    kernels.reset_ragged_status()
+    assert torch.equal(got, q)                   # q is served all the same
+    kept = dict(before)
+    page = int(tables[1, 0])
+    for n in cache:
+        other = torch.ones(cache[n].shape[0], dtype=torch.bool, device="cuda")
+        other[page] = False
+        assert torch.equal(cache[n][other], kept[n][other]), n
+        assert not torch.equal(cache[n][page, :, :3], kept[n][page, :, :3])
+
+
+def test_append_rows_behind_the_last_sequence():
+    from halftone_quantizedkvcache_b200 import kernels
+    q, k, v, cache, tables = append_case([6, 5], [0, 0], 2, 2, torch.float16, 16, 2)
+    inv = kernels.rope_inv_freq(128)[0]
+    k_out, q_out = torch.full((11, 2, D), 3.0, dtype=torch.float16, device="cuda"), torch.full((11, 4, D), 5.0, dtype=torch.float16, device="cuda")
+    before = {n: x.clone() for n, x in cache.items()}
+    kernels.paged4_append(q, k, v, cache, tables, ints([0, 0]), cu_seqlens=ints([0, 6, 9]), inv_freq=inv,
+                          q_out=q_out, k_out=k_out)
+    assert (q_out[9:] == 5).all() and (k_out[9:] == 3).all()
+    check_append(q, k, v, cache, tables, [6, 3], [0, 0], before, q_out, k_out, inv, None)
+    got = kernels.paged4_append(q, k, v, cache, tables, ints([0, 0]), cu_seqlens=ints([0, 6, 9]), inv_freq=inv)
+    assert torch.equal(got[9:], q[9:]) and torch.equal(got[:9], q_out[:9])
+    assert kernels.paged4_append(q[:0], k[:0], v[:0], cache, tables, ints([0, 0]), cu_seqlens=ints([0, 0, 0])).shape == (0, 4, D)
+
+
+# ---------------------------------------------------------------- decode
+def check_decode(out, q, cache, tables, lens, scale=None):
+    Hkv = cache["k"].shape[1]
+    for b, n in enumerate(lens):
+        k, v = (plain.values(cache, x, tables, b, n).transpose(0, 1) for x in ("k", "v"))
+        qq = q[b].view(Hkv, -1, D)
+        ref, mag = plain.attend(qq, k, v, torch.ones((1, n), dtype=torch.bool, device="cuda"), scale)
+        # Scores: q's split 2^-17 of sum |q k| (below 6.5 x the scale's 11), the biased sums 4 groups x 4
+        # roundings of 136 sum|q| s: 2^-13 together; the weights follow, twice, against sum p |v|.
+        near(out[b].view(ref.shape), ref, mag * 2.0 ** -11)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,Hkv,rep,page", [
+    ([1], 8, 2, 64), ([31], 1, 1, 16), ([32, 33, 0, 64], 2, 4, 16), ([512], 8, 2, 64),
+    ([5, 777, 1300, 2, 0, 129], 4, 3, 32), ([2501, 40, 1], 2, 8, 128), ([300, 301], 1, 5, 256),
+    ([100, 17], 2, 16, 64), ([90, 3], 1, 40, 16), ([0, 0], 2, 2, 16), ([9000], 1, 2, 64),
+])
+def test_decode(dtype, lens, Hkv, rep, page):
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(21)
+    per = max(1, -(-max(lens) // page))
+    cache = plain.random_cache(kernels, len(lens) * per + 2, Hkv, page, g)
+    tables = plain.random_tables(len(lens), per, len(lens) * per + 2, g)
+    q = torch.randn((len(lens), Hkv * rep, D), generator=g, device="cuda").to(DT[dtype])
+    out = kernels.paged4_decode_attn(q, cache, tables, ints(lens))
+    check_decode(out, q, cache, tables, lens)
+    assert kernels.ragged_status() == 0
+    # the same, bit by bit, on a second run, and as [B, H, 1, D]
+    again = kernels.paged4_decode_attn(q[:, :, None], cache, tables, ints(lens))
+    assert torch.equal(again[:, :, 0], out)
+
+
+def test_decode_many_short_sequences():
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(2)
+    lens = [(7 * i) % 130 for i in range(1000)]
+    cache = plain.random_cache(kernels, 9010, 2, 16, g)
+    tables = plain.random_tables(1000, 9, 9010, g)
+    q = torch.randn((1000, 4, D), generator=g, device="cuda").to(torch.bfloat16)
+    out = kernels.paged4_decode_attn(q, cache, tables, ints(lens))
+    check_decode(out[::37], q[::37], cache, tables[::37], lens[::37])
+    assert (out[0] == 0).all()
+
+
+def test_decode_ignores_what_no_token_wrote():
+    """Scales behind the last token NaN or infinite, table entries behind the last page no pages."""
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(8)
+    lens, page = [37, 70, 0], 32
+    cache = plain.random_cache(kernels, 14, 2, page, g)
+    tables = plain.random_tables(3, 4, 14, g)
+    q = torch.randn((3, 4, D), generator=g, device="cuda").to(torch.bfloat16)
+    ref = kernels.paged4_decode_attn(q, cache, tables, ints(lens))
+    for b, n in enumerate(lens):
+        pg, t = plain.slots(tables, page, b, 4 * page)
+        for name, x in (("k_scale", math.nan), ("v_scale", math.nan), ("k_scale", math.inf), ("v_scale", -math.inf)):
+            cache[name][pg[n:], :, t[n:]] = x
+            assert torch.equal(kernels.paged4_decode_attn(q, cache, tables, ints(lens)), ref)
+    tables[0, 2:], tables[1, 3:], tables[2] = -5, 1 << 30, 99
+    assert torch.equal(kernels.paged4_decode_attn(q, cache, tables, ints(lens)), ref)
+    assert kernels.ragged_status() == 0
+    # lengths past what the table holds end with it
+    long = kernels.paged4_decode_attn(q[:1], cache, tables[:1, :1], ints([10 ** 9]))
+    assert torch.equal(long, kernels.paged4_decode_attn(q[:1], cache, tables[:1, :1], ints([32])))
+    assert (kernels.paged4_decode_attn(q[:1], cache, tables[:1, :0], ints([5])) == 0).all()
+
+
+def test_decode_seen_scales_that_are_no_numbers_reach_the_output():
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(8)
+    cache = plain.random_cache(kernels, 8, 2, 64, g)
+    tables = plain.random_tables(2, 3, 8, g)
+    q = torch.randn((2, 4, D), generator=g, device="cuda").to(torch.bfloat16)
+    cache["k_scale"][int(tables[0, 1]), 0, 5, 2] = math.nan
+    cache["v_scale"][int(tables[1, 0]), 1, 9, 1] = math.nan
+    out = kernels.paged4_decode_attn(q, cache, tables, ints([150, 150]))
+    assert out[0, :2].isnan().all() and out[0, 2:].isfinite().all()
+    assert out[1, 2:, 32:64].isnan().all() and out[1, 2:, :32].isfinite().all() and out[1, :2].isfinite().all()
+
+
+def test_decode_extremes():
+    """Scores far apart (one key takes all), V scales from 2^-24 to 65504, a page that is none."""
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(13)
+    cache = plain.random_cache(kernels, 12, 1, 64, g)
+    tables = plain.random_tables(2, 4, 12, g)
+    q = (torch.randn((2, 2, D), generator=g, device="cuda") * 40).to(torch.float16)
+    cache["v_scale"].copy_(2.0 ** torch.randint(-24, 16, cache["v_scale"].shape, generator=g, device="cuda").float())
+    cache["v_scale"].clamp_(max=65504)
+    out = kernels.paged4_decode_attn(q, cache, tables, ints([256, 200])).float()
+    for b, n in enumerate([256, 200]):
+        k, v = (plain.values(cache, x, tables, b, n).transpose(0, 1) for x in ("k", "v"))
+        ref, mag = plain.attend(q[b].view(1, 2, D), k, v, torch.ones((1, n), dtype=torch.bool, device="cuda"))
+        # 40 times the scores: 2^-11 x 40 of the weights' errors.  Below 2^-14 float16's steps are 2^-24
+        # whatever the value, so its rounding is off by up to 2^-25 there.
+        err = (out[b].view(ref.shape).double() - ref.clamp(-65504, 65504)).abs()
+        bad = ~(err <= 2.0 ** -11 * ref.abs() + mag * 40 * 2.0 ** -11 + 2.0 ** -25) & (ref.abs() < 60000)
+        assert not bad.any(), (float(err[bad].max()), ref[bad][:4].tolist())
+    kernels.reset_ragged_status()
+    tables[1, 1] = -1
+    ok = kernels.paged4_decode_attn(q, cache, tables, ints([256, 200]))
+    assert kernels.ragged_status() == -1
+    kernels.reset_ragged_status()
+    assert torch.equal(ok[0].float(), out[0])
+
+
+def test_decode_strides_out_and_scale():
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(3)
+    big = plain.random_cache(kernels, 20, 4, 32, g)
+    cache = {n: x[4:, 1:3] for n, x in big.items()}      # a slice of a larger pool: other strides
+    tables = plain.random_tables(2, 8, 16, g).flip(0)[[0, 1, 0], :5]   # two sequences share their pages
+    tables = torch.cat([tables, tables], 1)[:, :5]
+    lens = [150, 31, 97]
+    q = torch.randn((3, 12, D), generator=g, device="cuda").to(torch.bfloat16)[:, ::2][:, :4]
+    out = torch.full((3, 4, 2 * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = kernels.paged4_decode_attn(q, cache, tables, ints(lens), out=out[..., :D], sm_scale=-0.05)
+    assert got.data_ptr() == out.data_ptr() and (out[..., D:] == 7).all()
+    check_decode(out[..., :D].contiguous(), q.contiguous(), cache, tables, lens, -0.05)
+    odd = torch.randn((3, 4 * D + 1), generator=g, device="cuda").to(torch.bfloat16)[:, 1:].unflatten(1, (4, D))
+    assert torch.equal(kernels.paged4_decode_attn(odd, cache, tables, ints(lens)),
+                       kernels.paged4_decode_attn(odd.contiguous(), cache, tables, ints(lens)))
+
+
+# ---------------------------------------------------------------- gather
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,Hkv,page", [([1], 1, 16), ([0, 33, 200], 2, 32), ([700, 5], 8, 64), ([300], 3, 256)])
+def test_gather(dtype, lens, Hkv, page):
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(6)
+    per = max(1, -(-max(lens) // page))
+    cache = plain.random_cache(kernels, len(lens) * per + 2, Hkv, page, g)
+    tables = plain.random_tables(len(lens), per, len(lens) * per + 2, g)
+    n = sum(lens)
+    k, v = kernels.paged4_gather(cache, tables, ints(lens), cum(lens), n + 3, dtype=DT[dtype])
+    for got, name in ((k, "k"), (v, "v")):
+        ref = torch.cat([plain.values(cache, name, tables, b, m) for b, m in enumerate(lens)])
+        # the product of a 4-bit and an 11-bit number is exact in float32, and rounded once
+        assert torch.equal(got[:n], ref.float().to(DT[dtype]))
+        assert (got[n:] == 0).all()
+    # from the second half on, into rows of a larger buffer
+    first = [m // 2 for m in lens]
+    rows = [m - f for m, f in zip(lens, first)]
+    out = [torch.full((n + 3, 2 * Hkv, D), 9.0, dtype=DT[dtype], device="cuda")[:, :Hkv] for _ in range(2)]
+    kernels.paged4_gather(cache, tables, ints(lens), cum(rows), n + 3, first=ints(first), k_out=out[0], v_out=out[1])
+    for got, name in ((out[0], "k"), (out[1], "v")):
+        ref = torch.cat([plain.values(cache, name, tables, b, m)[f:] for b, (m, f) in enumerate(zip(lens, first))])
+        assert torch.equal(got[:sum(rows)], ref.float().to(DT[dtype])) and (got[sum(rows):] == 9).all()
+    assert kernels.ragged_status() == 0
+
+
+def test_gather_bad_pages_and_short_rows():
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(6)
+    cache = plain.random_cache(kernels, 9, 2, 16, g)
+    tables = plain.random_tables(2, 4, 9, g)
+    ref = [plain.values(cache, "k", tables, b, 64).float().to(torch.bfloat16) for b in range(2)]
+    # fewer rows than tokens: the first ones; more rows than tokens: the others empty
+    k, _ = kernels.paged4_gather(cache, tables, ints([64, 10]), ints([0, 20, 50]), 50)
+    assert torch.equal(k[:20], ref[0][:20]) and torch.equal(k[20:30], ref[1][:10]) and (k[30:] == 0).all()
+    kernels.reset_ragged_status()
+    tables[0, 1] = 9
+    k, _ = kernels.paged4_gather(cache, tables, ints([40, 10]), ints([0, 40, 50]), 50)
+    assert kernels.ragged_status() == -1
+    kernels.reset_ragged_status()
+    assert torch.equal(k[:16], ref[0][:16]) and (k[16:32] == 0).all() and torch.equal(k[32:40], ref[0][32:40])

@@ -70,6 +70,7 @@ inline int check_pages(const void* k, const void* v, const void* ks, const void*
     auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     if (!al(k) || !al(v) || !al(ks) || !al(vs) || cs[0] % 16 || cs[1] % 16 || ss[0] % 8 || ss[1] % 8)
       return HQ_ERR_INVALID_ARGUMENT;
+    if (cs[0] >> 31 || ss[0] >> 30) return HQ_ERR_UNSUPPORTED;  // page strides below 2 GB
     // pages and heads have memory of their own
     if ((n_pages > 1 && cs[0] < static_cast<int64_t>(page) * kRowB) || (Hkv > 1 && cs[1] < static_cast<int64_t>(page) * kRowB) ||
         (n_pages > 1 && ss[0] < static_cast<int64_t>(page) * 4) || (Hkv > 1 && ss[1] < static_cast<int64_t>(page) * 4))

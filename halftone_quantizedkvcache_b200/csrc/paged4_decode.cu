@@ -2,25 +2,29 @@
 // device (sm_100a).
 //
 // All sequences, kv heads and tokens are one line of 32-token tiles; every warp takes an equal run of
-// it, with an online softmax of its own and no word to the other warps.  Units (sequence, kv head, up
-// to 4 NT query rows) that end inside one warp's run are written by it, the others leave partial
-// states (m, l, o) that join_kernel puts together in the order of the line.
+// it, with an online softmax of its own.  Units (sequence, kv head, up to 4 NT query rows) that end
+// inside one warp's run are written by it; the ends of the warps' runs are joined in the block, and
+// what crosses a block's border leaves partial states (m, l, o) that join_kernel puts together, always
+// in the order of the line.
 //
 // Bound by the cache's bytes and, close behind, by issue slots: 144 bytes a token and head are 256
-// codes to unpack.  Both products take the codes as the 16-row operand of mma.sync m16n8k16 (bf16),
-// query rows in pairs of columns (upper and lower part of a 16-bit split):
-//   * Q K^T: a code is 128 + c (its 4 bits under bf16's exponent), no subtraction: the accumulators
-//     start at -136 sum(q), formed per unit by the same instruction.  Per group of 32 channels the
-//     products are exact and the sum is float32; the group's scale multiplies it in float32.
-//   * P V: codes as 128 + c - 136 (exact), p times the token's group scale as a bf16 pair (16 bits,
-//     bf16's range: V scales of any size), transposed in registers by movmatrix.
-// Copies: every warp has its own ring of stages filled by bulk copies, one per page, side and kind.
-//
-// No sum is in fewer than 32 bits; q's and p's splits keep 16 bits (2^-17 of each).
+// codes to unpack.  Both products are whole-number products on bytes (mma.sync m16n8k32, exact), the
+// codes being the 16-row operand, since a word of 8 codes becomes bytes with two masks and a shift:
+//   * Q K^T: q is a 22-bit whole number per channel (of the row's largest |q|: 2^-22 of it is lost) in
+//     three base-256 digits, two columns and a third in a second product that starts at -8 sum(q) for
+//     the codes' offset; one product is one group of 32 channels, its scale joins in float32.
+//   * P V: p relative to the tile's maximum, times the token's group scale relative to the tile's
+//     largest, is a 16-bit whole number (2^-16 of the tile's largest weight is lost) in two digits,
+//     transposed in registers by movmatrix; four tokens' bytes are turned with permutes.  A tile's sums
+//     go into the float32 state with the tile's and the group's factor.
+// (As bf16 products, 7 to 12 instructions a word and twice the products, 64 x 8192 tokens took 138 us.)
+// Copies: every warp has its own ring of stages filled by bulk copies, one per page, side and kind,
+// issued by one lane each.
 #include <algorithm>
 #include <atomic>
 
 #include "paged4.cuh"
+#include "umma.cuh"
 
 namespace hq {
 int current_sm_count();
@@ -44,18 +48,19 @@ struct DecodeParams {
   int64_t os[2];
   float* part;
   int* cum;                               // for join_kernel: first tile of every sequence
-  int workers, min_tiles;
+  int grid;
   int* status;
 };
 
 template <int NT>
 struct Cfg {
-  // NT 1: 16 warps of 128 registers; NT 2 (twice the accumulators): 8 of 255
-  static constexpr int kWarps = NT == 1 ? 16 : 8;
-  static constexpr int kStages = NT == 1 ? 3 : 6;
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
+  static constexpr int kStages = NT == 1 ? 3 : 4;
   static constexpr int kRows = 4 * NT;
   static constexpr int kOffBar = kWarps * kStages * kStageB;
-  static constexpr int kOffCum = kOffBar + 8 * kWarps * kStages;
+  static constexpr int kOffState = kOffBar + 8 * kWarps * kStages;  // [2 warps' ends][rows][m, l, -, -, o]
+  static constexpr int kOffCum = kOffState + 2 * kWarps * kRows * kPartRow * 4;
+  static_assert(kOffState % 16 == 0, "vector accesses");
   static constexpr int smem(int B) { return kOffCum + 4 * (2 * B + 1); }
   static_assert(smem(kMaxSeqs) <= 232448, "one block per SM");
 };
@@ -65,32 +70,39 @@ __device__ __forceinline__ int seq_len(const DecodeParams& p, int b) {
 }
 __device__ __forceinline__ int tiles_of(int len) { return max(1, (len + kTile - 1) / kTile); }
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d = a b + c in whole numbers, bytes of a (16 x 32) and b (32 x 8) signed or not.  (c is a product's
+// result or zero: four other registers would be gathered for each product.)
+#define HQ_MMA_BYTES(NAME, A, B)                                                                          \
+  __device__ __forceinline__ void NAME(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,   \
+                                       uint32_t b0, uint32_t b1, const int (&c)[4]) {                     \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32." A "." B ".s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "      \
+        "{%8, %9}, {%10, %11, %12, %13};"                                                                 \
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                                  \
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3])); \
+  }
+HQ_MMA_BYTES(mma_u8s8, "u8", "s8")
+HQ_MMA_BYTES(mma_u8u8, "u8", "u8")
+HQ_MMA_BYTES(mma_s8s8, "s8", "s8")
+HQ_MMA_BYTES(mma_s8u8, "s8", "u8")
+#undef HQ_MMA_BYTES
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-// nibbles i and i + 4 of w under the exponent of 128
-template <int I>
-__device__ __forceinline__ uint32_t biased(uint32_t w) {
-  return ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u;
-}
-__device__ __forceinline__ uint32_t sub136(uint32_t x) {
-  uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x43084308u));
-  return d;
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&x);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -99,10 +111,10 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float2 half2_of(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// A place on the line of tiles.
+// A place on the line of tiles: unit `idx` of sequence e, whose first tile is `first`.
 struct Cursor {
   int line, end;
-  int e, idx, first;                      // sequence, unit within it, the unit's first tile
+  int e, idx, first;
   int len, nt;
 };
 __device__ __forceinline__ void enter(Cursor& c, const int* lens, int e) {
@@ -110,15 +122,41 @@ __device__ __forceinline__ void enter(Cursor& c, const int* lens, int e) {
   c.len = lens[e];
   c.nt = tiles_of(c.len);
 }
-// to the next tile; units per sequence `per`
-__device__ __forceinline__ void step(Cursor& c, const int* lens, int per) {
-  if (++c.line == c.first + c.nt && c.line < c.end) {
-    c.first = c.line;
-    if (++c.idx == per) {
-      c.idx = 0;
-      enter(c, lens, c.e + 1);
-    }
+// from the last tile of a unit to the next one's first; `per` units a sequence
+__device__ __forceinline__ void next_unit(Cursor& c, const int* lens, int per) {
+  c.first += c.nt;
+  if (++c.idx == per) {
+    c.idx = 0;
+    enter(c, lens, c.e + 1);
   }
+}
+// the whole number that a row's largest |q| becomes: below 2^21, and its upper digit below 32
+constexpr float kFixed = 2088960.0f;
+// and that a tile's largest weight becomes
+constexpr float kWeight = 32512.0f;
+__device__ constexpr int kZero[4] = {0, 0, 0, 0};
+
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, int dt) {
+  if (dt == HQ_DTYPE_BF16) return pack_bf16(a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// (m, l, o) into the state (M, L, acc).  A state whose sums are no number has a maximum of -inf and
+// passes them on.
+__device__ __forceinline__ void join_state(float& M, float& L, float4& acc, float m, float l, const float4& o) {
+  const float top = fmaxf(M, m);
+  const float f0 = M == -INFINITY ? 0.0f : exp2f(M - top), f1 = m == -INFINITY ? 0.0f : exp2f(m - top);
+  M = top;
+  L = L * f0 + l * f1;
+  acc.x = acc.x * f0 + o.x * f1;
+  acc.y = acc.y * f0 + o.y * f1;
+  acc.z = acc.z * f0 + o.z * f1;
+  acc.w = acc.w * f0 + o.w * f1;
+}
+__device__ __forceinline__ void store_row(const DecodeParams& p, int q_dt, int b, int h, int d, float L, const float4& o) {
+  const float inv = L <= 0.0f ? 0.0f : 1.0f / L;
+  *reinterpret_cast<uint2*>(static_cast<char*>(p.out) + 2 * (b * p.os[0] + h * p.os[1] + d)) =
+      make_uint2(pack_pair(o.x * inv, o.y * inv, q_dt), pack_pair(o.z * inv, o.w * inv, q_dt));
 }
 
 template <int NT>
@@ -129,11 +167,14 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
   const int n8 = lane >> 2, c4 = lane & 3;
   unsigned char* ring = smem + warp * C::kStages * kStageB;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar) + warp * C::kStages;
+  float* states = reinterpret_cast<float*>(smem + C::kOffState);
   int* cum = reinterpret_cast<int*>(smem + C::kOffCum);
+  __shared__ int ends[C::kWarps][2];      // units cut by the warps' runs: the one that began before, the one that goes on
   int* lens = cum + p.B + 1;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (lane == 0)
     for (int i = 0; i < C::kStages; ++i) mbar_init(&full[i], 1);
+  if (lane < 2) ends[warp][lane] = -1;
   fence_mbar_init();
   const int per = p.Hkv * p.n_rt;
   for (int b = tid; b < p.B; b += 32 * C::kWarps) lens[b] = seq_len(p, b);
@@ -157,17 +198,17 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
   if (blockIdx.x == 0)
     for (int b = tid; b <= p.B; b += 32 * C::kWarps) p.cum[b] = cum[b];
   const int total = cum[p.B];
-  const int chunk = max(p.min_tiles, (total + p.workers - 1) / p.workers);
-  // neighbouring runs on different SMs
-  const int worker = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
+  // an equal run of the line for each block, and of that for each warp
+  const int run = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const int chunk = (run + C::kWarps - 1) / C::kWarps;
   Cursor cur{};
-  cur.line = static_cast<int>(min(static_cast<int64_t>(worker) * chunk, static_cast<int64_t>(total)));
-  cur.end = static_cast<int>(min(static_cast<int64_t>(cur.line) + chunk, static_cast<int64_t>(total)));
-  if (cur.line >= cur.end) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
   {
+    const int64_t from = static_cast<int64_t>(blockIdx.x) * run, upto = min(from + run, static_cast<int64_t>(total));
+    cur.line = static_cast<int>(min(from + warp * chunk, upto));
+    cur.end = static_cast<int>(min(static_cast<int64_t>(cur.line) + chunk, upto));
+  }
+  const bool any = cur.line < cur.end;
+  if (any) {
     int lo = 0, hi = p.B - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -178,56 +219,61 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
     cur.first = cum[lo] + cur.idx * cur.nt;
   }
 
-  // ---- the copies' cursor, up to kStages tiles ahead
+  // ---- the copies' cursor, up to kStages tiles ahead.  Lane 4 i + kind copies codes (kind 0: K, 1: V)
+  // or scales (2: K, 3: V) of the tile's i-th page.
   Cursor ahead = cur;
-  int win_e = -1, win = 0, ids = 0;       // 32 page numbers of sequence win_e from entry `win` on
-  int issued = 0;
+  const int kind = lane & 3, half = lane >> 2 & 1;
+  const int here = min(p.pg.page, kTile);  // tokens of a page in a tile
+  const int row_log = kind < 2 ? 6 : 3;    // bytes of a row
+  static_assert(kRowB == 64 && kScaleB == 8, "row_log");
+  const char* lane_base = kind == 0 ? reinterpret_cast<const char*>(p.pg.k) : kind == 1 ? reinterpret_cast<const char*>(p.pg.v)
+                        : kind == 2 ? reinterpret_cast<const char*>(p.pg.ksc) : reinterpret_cast<const char*>(p.pg.vsc);
+  const uint32_t page_b = static_cast<uint32_t>(kind < 2 ? p.pg.cp : 2 * p.pg.sp);
+  const int64_t head_b = kind < 2 ? p.pg.ch : 2 * p.pg.sh;
+  const bool mine = lane < 8 && (half == 0 || here < kTile);
+  const uint32_t to0 = smem_u32(ring) + (kind == 0 ? 0 : kind == 1 ? kOffV : kind == 2 ? kOffKs : kOffVs) + (half * here << row_log);
+  const uint32_t bar0 = smem_u32(full);
+  const char* unit_base = nullptr;
+  const int* table = nullptr;
+  int tok = 0, win = 0, ids = 0;          // ids: 32 page numbers from table entry `win` on
+  int issued = 0, st_in = 0;
+  auto load_ids = [&](int at) {
+    win = at & ~31;
+    ids = (win + lane) << p.pg.page_log < ahead.len ? table[win + lane] : -1;
+  };
+  auto open_unit = [&](int t) {
+    const int kvh = p.n_rt == 1 ? ahead.idx : ahead.idx / p.n_rt;
+    unit_base = lane_base + kvh * head_b;
+    table = p.pg.tables + ahead.e * p.pg.tstride;
+    tok = t * kTile;
+    load_ids(tok >> p.pg.page_log);
+  };
+  if (any) open_unit(ahead.line - ahead.first);
   auto issue = [&]() {
     if (ahead.line >= ahead.end) return;
-    const int st = issued % C::kStages;
-    const int tok = (ahead.line - ahead.first) * kTile;
     const int pi = tok >> p.pg.page_log;
-    if (win_e != ahead.e || pi < win || pi >= win + 32) {
-      win_e = ahead.e;
-      win = pi & ~31;
-      const int at = win + lane;
-      ids = at << p.pg.page_log < ahead.len ? p.pg.tables[win_e * p.pg.tstride + at] : -1;
-    }
-    const int kvh = p.n_rt == 1 ? ahead.idx : ahead.idx / p.n_rt;
-    const int here = min(p.pg.page, kTile);  // tokens of a page in the tile
-    unsigned char* s = ring + st * kStageB;
-    uint32_t bytes = 0;
-    int page[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      page[i] = -1;
-      if (i * here < kTile && tok + i * here < ahead.len) {
-        page[i] = __shfl_sync(0xffffffffu, ids, (pi - win + i) & 31);
-        if (page[i] >= 0 && page[i] < p.pg.n_pages) {
-          bytes += 2 * here * (kRowB + kScaleB);
-        } else {
-          page[i] = -1;
-          if (lane == 0) report_error(p.status, HQ_ERR_INVALID_ARGUMENT);
-        }
-      }
-    }
-    if (lane == 0) {
-      if (bytes) mbar_arrive_expect_tx(&full[st], bytes);
-      else mbar_arrive(&full[st]);
-      const int off = tok & (p.pg.page - 1);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (page[i] < 0) continue;
-        const int64_t co = page[i] * p.pg.cp + kvh * p.pg.ch + off * kRowB;
-        const int64_t so = page[i] * p.pg.sp + kvh * p.pg.sh + off * 4;
-        bulk_g2s(s + i * here * kRowB, p.pg.k + co, here * kRowB, &full[st]);
-        bulk_g2s(s + kOffKs + i * here * kScaleB, p.pg.ksc + so, here * kScaleB, &full[st]);
-        bulk_g2s(s + kOffV + i * here * kRowB, p.pg.v + co, here * kRowB, &full[st]);
-        bulk_g2s(s + kOffVs + i * here * kScaleB, p.pg.vsc + so, here * kScaleB, &full[st]);
-      }
-    }
+    if (pi >= win + 32) load_ids(pi);
+    const int id = __shfl_sync(0xffffffffu, ids, pi - win + half);
+    const bool need = mine && tok + half * here < ahead.len;
+    const bool good = need && static_cast<uint32_t>(id) < static_cast<uint32_t>(p.pg.n_pages);
+    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, good)) * (here * (kRowB + kScaleB) / 2);  // 4 lanes a page
+    const uint32_t bar = bar0 + 8 * st_in;
+    if (lane == 0)
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+    if (good)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       to0 + st_in * kStageB),
+                   "l"(unit_base + static_cast<uint64_t>(static_cast<uint32_t>(id)) * page_b + ((tok & (p.pg.page - 1)) << row_log)),
+                   "r"(here << row_log), "r"(bar)
+                   : "memory");
+    if (need && !good) report_error(p.status, HQ_ERR_INVALID_ARGUMENT);
     ++issued;
-    step(ahead, lens, per);
+    st_in = st_in + 1 == C::kStages ? 0 : st_in + 1;
+    tok += kTile;
+    if (++ahead.line == ahead.first + ahead.nt && ahead.line < ahead.end) {
+      next_unit(ahead, lens, per);
+      open_unit(0);
+    }
   };
   __syncwarp();
 #pragma unroll 1
@@ -237,13 +283,14 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
   const int e1 = n8 & 1, slot_tok = 4 * e1 + ((n8 >> 1) ^ e1);
   // V: rows n8 (and n8 + 8) are channels of chunk vj, half vh
   const int vj = n8 & 3, vh = n8 >> 2;
-  const uint32_t vsel = vh ? 0x7632u : 0x5410u;
+  const uint32_t vsel = vh ? 0x7362u : 0x5140u;  // (a.b0, b.b0, a.b1, b.b1) of half vh
   // K rows of slots: byte offset of chunk c4 of token slot_tok; V: chunk vj of tokens c4, 4 + (c4 ^ 1)
   const int k_off = slot_tok * kRowB + 16 * (c4 ^ (slot_tok & 2));
   const int va = c4, vb = 4 + (c4 ^ 1);
   const int va_off = kOffV + va * kRowB + 16 * (vj ^ (va & 2)), vb_off = kOffV + vb * kRowB + 16 * (vj ^ (vb & 2));
 
-  int done = 0;
+  int done = 0, st = 0;
+  uint32_t phase = 0;
   bool ok = true;
 #pragma unroll 1
   while (ok && cur.line < cur.end) {
@@ -252,43 +299,59 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
     const int kvh = p.n_rt == 1 ? cur.idx : cur.idx / p.n_rt;
     const int row0 = (cur.idx - kvh * p.n_rt) * C::kRows;
     const int b = cur.e, len = cur.len;
-    const int slot = t0 == 0 && t1 == cur.nt ? -1 : cur.e * per + cur.idx + worker;
-    // B fragments of q: column n8 is the upper (n8 even) or lower part of row 4 nt + n8 / 2
+    const bool whole = t0 == 0 && t1 == cur.nt;
+    // B fragments of q: columns 2 r, 2 r + 1 are the upper two digits of row r (first product), 2 r the
+    // lowest (second); a lane's bytes are the channels 8 c4 + {0, 2, 4, 6} and + {1, 3, 5, 7} of a group
     uint32_t bq[NT][4][2][2];
-    float corr[NT][4][2];
+    int off[NT][4];                       // -8 sum(q) of row c4
+    float qk[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = row0 + 4 * nt + (n8 >> 1);
       const bool real = r < p.nrep;
       const char* row = static_cast<const char*>(p.q) + 2 * (b * p.qs[0] + (kvh * p.nrep + r) * p.qs[1] + 8 * c4);
       uint4 raw[4];
+      float big = 0.0f;
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < 4; ++g) {
         raw[g] = real ? *reinterpret_cast<const uint4*>(row + 64 * g) : make_uint4(0, 0, 0, 0);
+        float f[8];
+        if (q_dt == HQ_DTYPE_BF16) Vec16<HQ_DTYPE_BF16>::unpack(raw[g], f);
+        else Vec16<HQ_DTYPE_F16>::unpack(raw[g], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = max_nan(big, fabsf(f[e]));
+      }
+      big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // (not below 2^-100, so that the step stays finite; a row that is no number gives scores that are none)
+      const float fix = kFixed / fmaxf(big, 7.8886091e-31f);
+      const float unit = big < INFINITY ? 1.0f / fix : NAN;
+      qk[nt] = __shfl_sync(0xffffffffu, unit, 8 * c4) * p.qk_scale;  // of row c4: a lane that has its columns
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         float f[8];
         if (q_dt == HQ_DTYPE_BF16) Vec16<HQ_DTYPE_BF16>::unpack(raw[g], f);
         else Vec16<HQ_DTYPE_F16>::unpack(raw[g], f);
-        if (n8 & 1) {
+        uint32_t top[2] = {0, 0}, low[2] = {0, 0};
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] -= __bfloat162float(__float2bfloat16_rn(f[e]));
+        for (int e = 0; e < 8; ++e) {
+          const int x = __float2int_rn(f[e] * fix), y = (x + 128) >> 8, z = (y + 128) >> 8;
+          const uint32_t d = (n8 & 1 ? y - 256 * z : z) & 0xff, d0 = n8 & 1 ? 0 : (x - 256 * y) & 0xff;
+          top[e & 1] |= d << (8 * (e >> 1));
+          low[e & 1] |= d0 << (8 * (e >> 1));
         }
-        // channels 8 c4 + 2 m, + 4 and 8 c4 + 2 m + 1, + 5
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          bq[nt][g][m][0] = pack_bf16(f[2 * m], f[2 * m + 4]);
-          bq[nt][g][m][1] = pack_bf16(f[2 * m + 1], f[2 * m + 5]);
-        }
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        constexpr uint32_t kM136 = 0xc308c308u;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) mma_bf16(s, kM136, kM136, kM136, kM136, bq[nt][g][m][0], bq[nt][g][m][1]);
-        corr[nt][g][0] = s[0];
-        corr[nt][g][1] = s[1];
+        bq[nt][g][0][0] = top[0];
+        bq[nt][g][0][1] = top[1];
+        bq[nt][g][1][0] = low[0];
+        bq[nt][g][1][1] = low[1];
+        constexpr uint32_t k8 = 0x08080808u;
+        int u[4], w[4];
+        mma_u8s8(u, k8, k8, k8, k8, top[0], top[1], kZero);
+        mma_u8s8(w, k8, k8, k8, k8, low[0], low[1], kZero);
+        off[nt][g] = -((u[0] * 256 + u[1]) * 256 + w[0]);
       }
     }
-    float m_run[NT], l_run[NT], o[NT][4][2][4];
+    float m_run[NT], l_run[NT], o[NT][4][2][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m_run[nt] = -INFINITY;
@@ -297,22 +360,24 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
       for (int g = 0; g < 4; ++g)
 #pragma unroll
         for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][g][m][e] = 0.0f;
+          o[nt][g][m][0] = o[nt][g][m][1] = 0.0f;
     }
 
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
-      const int st = done % C::kStages;
-      ok = mbar_wait(&full[st], (done / C::kStages) & 1);
+      ok = tc::wait_bar(&full[st], phase);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       ++done;
       const unsigned char* s = ring + st * kStageB;
+      if (++st == C::kStages) {
+        st = 0;
+        phase ^= 1;
+      }
       const int left = len - t * kTile;   // tokens of the tile that exist
-      float sc[NT][2][2];
+      float sc[NT][4];                    // tokens 8 i + slot_tok
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
         const unsigned char* kr = s + blk * 16 * kRowB + k_off;
@@ -325,32 +390,33 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
         const float2 k00 = half2_of(u0.x), k01 = half2_of(u0.y), k10 = half2_of(u1.x), k11 = half2_of(u1.y);
         const float s0[4] = {k00.x, k00.y, k01.x, k01.y}, s1[4] = {k10.x, k10.y, k11.x, k11.y};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][blk][0] = sc[nt][blk][1] = 0.0f;
+        for (int nt = 0; nt < NT; ++nt) sc[nt][2 * blk] = sc[nt][2 * blk + 1] = 0.0f;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const uint32_t x0 = biased<0>(a0[g]), x1 = biased<1>(a0[g]), x2 = biased<2>(a0[g]), x3 = biased<3>(a0[g]);
-          const uint32_t y0 = biased<0>(a1[g]), y1 = biased<1>(a1[g]), y2 = biased<2>(a1[g]), y3 = biased<3>(a1[g]);
+          constexpr uint32_t kLow = 0x0f0f0f0fu;
+          const uint32_t x0 = a0[g] & kLow, x1 = (a0[g] >> 4) & kLow, y0 = a1[g] & kLow, y1 = (a1[g] >> 4) & kLow;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float c[4] = {corr[nt][g][0], corr[nt][g][1], corr[nt][g][0], corr[nt][g][1]};
-            mma_bf16(c, x0, y0, x1, y1, bq[nt][g][0][0], bq[nt][g][0][1]);
-            mma_bf16(c, x2, y2, x3, y3, bq[nt][g][1][0], bq[nt][g][1][1]);
-            sc[nt][blk][0] = __fmaf_rn(s0[g], c[0] + c[1], sc[nt][blk][0]);
-            sc[nt][blk][1] = __fmaf_rn(s1[g], c[2] + c[3], sc[nt][blk][1]);
+            int u[4], w[4];
+            mma_u8s8(u, x0, y0, x1, y1, bq[nt][g][0][0], bq[nt][g][0][1], kZero);
+            mma_u8s8(w, x0, y0, x1, y1, bq[nt][g][1][0], bq[nt][g][1][1], kZero);
+            // 32 x 8 x 2^21 is 2^29: whole numbers all the way
+            sc[nt][2 * blk] = __fmaf_rn(s0[g], static_cast<float>((u[0] * 256 + u[1]) * 256 + (w[0] + off[nt][g])), sc[nt][2 * blk]);
+            sc[nt][2 * blk + 1] = __fmaf_rn(s1[g], static_cast<float>((u[2] * 256 + u[3]) * 256 + (w[2] + off[nt][g])), sc[nt][2 * blk + 1]);
           }
         }
         const int tk = blk * 16 + slot_tok;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          sc[nt][blk][0] = tk < left ? sc[nt][blk][0] * p.qk_scale : -INFINITY;
-          sc[nt][blk][1] = tk + 8 < left ? sc[nt][blk][1] * p.qk_scale : -INFINITY;
+          sc[nt][2 * blk] = tk < left ? sc[nt][2 * blk] * qk[nt] : -INFINITY;
+          sc[nt][2 * blk + 1] = tk + 8 < left ? sc[nt][2 * blk + 1] * qk[nt] : -INFINITY;
         }
       }
-      // ---- online softmax
-      float pr[NT][2][2];
+      // ---- softmax of the tile, relative to its own maximum; f brings it to the running one
+      float pr[NT][4], f[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float mt = fmaxf(fmaxf(sc[nt][0][0], sc[nt][0][1]), fmaxf(sc[nt][1][0], sc[nt][1][1]));
+        float mt = fmaxf(fmaxf(sc[nt][0], sc[nt][1]), fmaxf(sc[nt][2], sc[nt][3]));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
@@ -362,99 +428,191 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
 #pragma unroll
           for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < 2; ++m) {
+              o[nt][g][m][0] *= alpha;
+              o[nt][g][m][1] *= alpha;
+            }
+        }
+        f[nt] = mt == -INFINITY ? 0.0f : ex2(mt - m_run[nt]);
+        float sum = 0.0f;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][g][m][e] *= alpha;
+        for (int i = 0; i < 4; ++i) {
+          pr[nt][i] = sc[nt][i] == -INFINITY ? 0.0f : ex2(sc[nt][i] - mt);
+          sum += pr[nt][i];
+        }
+        l_run[nt] = __fmaf_rn(f[nt], sum, l_run[nt]);
+      }
+      // ---- the tokens' V scales, relative to the tile's largest of each group
+      float vs[4][4], top[4];
+      {
+        uint2 u[4];
+        __half2 a = __float2half2_rn(0.0f), b2 = a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tk = 8 * i + slot_tok;
+          u[i] = *reinterpret_cast<const uint2*>(s + kOffVs + tk * kScaleB);
+          if (tk >= left) u[i] = make_uint2(0, 0);  // what no token wrote may be anything
+          a = __hmax2_nan(a, __habs2(*reinterpret_cast<const __half2*>(&u[i].x)));
+          b2 = __hmax2_nan(b2, __habs2(*reinterpret_cast<const __half2*>(&u[i].y)));
         }
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
+        for (int d = 4; d <= 16; d <<= 1) {
+          a = __hmax2_nan(a, __shfl_xor_sync(0xffffffffu, a, d));
+          b2 = __hmax2_nan(b2, __shfl_xor_sync(0xffffffffu, b2, d));
+        }
+        const float2 ta = __half22float2(a), tb = __half22float2(b2);
+        top[0] = ta.x;
+        top[1] = ta.y;
+        top[2] = tb.x;
+        top[3] = tb.y;
+        float inv[4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float x = sc[nt][blk][i];
-            pr[nt][blk][i] = x == -INFINITY ? 0.0f : ex2(x - m_run[nt]);
-            l_run[nt] += pr[nt][blk][i];
-          }
+        for (int g = 0; g < 4; ++g) inv[g] = top[g] == 0.0f ? 0.0f : kWeight * rcp(top[g]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = half2_of(u[i].x), y = half2_of(u[i].y);
+          vs[i][0] = x.x * inv[0];
+          vs[i][1] = x.y * inv[1];
+          vs[i][2] = y.x * inv[2];
+          vs[i][3] = y.y * inv[3];
+        }
       }
       // ---- P V
+      uint4 vw[8];                        // chunk vj of this lane's tokens: sets 0 .. 3, slots 2 c4 and 2 c4 + 1
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        const unsigned char* v0 = s + blk * 16 * kRowB;
-        const uint4 ta = *reinterpret_cast<const uint4*>(v0 + va_off), tb = *reinterpret_cast<const uint4*>(v0 + vb_off);
-        const uint4 tc = *reinterpret_cast<const uint4*>(v0 + va_off + 8 * kRowB);
-        const uint4 td = *reinterpret_cast<const uint4*>(v0 + vb_off + 8 * kRowB);
-        const uint32_t wa[4] = {ta.x, ta.y, ta.z, ta.w}, wb[4] = {tb.x, tb.y, tb.z, tb.w};
-        const uint32_t wc[4] = {tc.x, tc.y, tc.z, tc.w}, wd[4] = {td.x, td.y, td.z, td.w};
-        const int tk = blk * 16 + slot_tok;
-        const unsigned char* vs = s + kOffVs + tk * kScaleB;
-        uint2 u0 = *reinterpret_cast<const uint2*>(vs), u1 = *reinterpret_cast<const uint2*>(vs + 8 * kScaleB);
-        if (tk >= left) u0 = make_uint2(0, 0);      // what no token wrote may be anything
-        if (tk + 8 >= left) u1 = make_uint2(0, 0);
-        const float2 k00 = half2_of(u0.x), k01 = half2_of(u0.y), k10 = half2_of(u1.x), k11 = half2_of(u1.y);
-        const float s0[4] = {k00.x, k00.y, k01.x, k01.y}, s1[4] = {k10.x, k10.y, k11.x, k11.y};
+      for (int i = 0; i < 4; ++i) {
+        vw[2 * i] = *reinterpret_cast<const uint4*>(s + i * 8 * kRowB + va_off);
+        vw[2 * i + 1] = *reinterpret_cast<const uint4*>(s + i * 8 * kRowB + vb_off);
+      }
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const uint32_t x = prmt(wa[g], wb[g], vsel), y = prmt(wc[g], wd[g], vsel);
-          const uint32_t x0 = sub136(biased<0>(x)), x1 = sub136(biased<1>(x)), x2 = sub136(biased<2>(x)), x3 = sub136(biased<3>(x));
-          const uint32_t y0 = sub136(biased<0>(y)), y1 = sub136(biased<1>(y)), y2 = sub136(biased<2>(y)), y3 = sub136(biased<3>(y));
+      for (int gg = 0; gg < 2; ++gg) {    // groups 2 gg (columns 2 r) and 2 gg + 1 (2 r + 1)
+        uint32_t hi[NT][2], lo[NT][2];
+        int ch[NT][4], cl[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          constexpr float kRound = 12582912.0f;  // 1.5 x 2^23: the whole number in the low bits
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = transpose8(prmt(__float_as_uint(__fmaf_rn(pr[nt][i], vs[i][2 * gg], kRound)),
+                                   __float_as_uint(__fmaf_rn(pr[nt][i], vs[i][2 * gg + 1], kRound)), 0x5410u));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            lo[nt][i] = prmt(w[2 * i], w[2 * i + 1], 0x6420u);
+            hi[nt][i] = prmt(w[2 * i], w[2 * i + 1], 0x7531u);
+          }
+          constexpr uint32_t kM8 = 0xf8f8f8f8u;  // the codes' offset
+          mma_s8s8(ch[nt], kM8, kM8, kM8, kM8, hi[nt][0], hi[nt][1], kZero);
+          mma_s8u8(cl[nt], kM8, kM8, kM8, kM8, lo[nt][0], lo[nt][1], kZero);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int g = 2 * gg + e;
+          auto word = [&](int i) { return g == 0 ? vw[i].x : g == 1 ? vw[i].y : g == 2 ? vw[i].z : vw[i].w; };
+          uint32_t a[2][4];               // [channels 0, 1 / 2, 3][operand register]
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t x = prmt(word(4 * k), word(4 * k + 1), vsel), y = prmt(word(4 * k + 2), word(4 * k + 3), vsel);
+            const uint32_t b0 = prmt(x, y, 0x5410u), b1 = prmt(x, y, 0x7632u);
+            constexpr uint32_t kLow = 0x0f0f0f0fu;
+            a[0][2 * k] = b0 & kLow;
+            a[0][2 * k + 1] = (b0 >> 4) & kLow;
+            a[1][2 * k] = b1 & kLow;
+            a[1][2 * k + 1] = (b1 >> 4) & kLow;
+          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float p0 = pr[nt][blk][0] * s0[g], p1 = pr[nt][blk][1] * s1[g];
-            const uint32_t hi = pack_bf16(p0, p1);
-            const uint32_t lo = pack_bf16(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
-            const uint32_t b0 = transpose8(prmt(hi, lo, 0x5410u)), b1 = transpose8(prmt(hi, lo, 0x7632u));
-            mma_bf16(o[nt][g][0], x0, x1, y0, y1, b0, b1);
-            mma_bf16(o[nt][g][1], x2, x3, y2, y3, b0, b1);
+            const float w = f[nt] * (top[g] * (1.0f / kWeight));
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              int h[4], u[4];
+              mma_u8s8(h, a[m][0], a[m][1], a[m][2], a[m][3], hi[nt][0], hi[nt][1], ch[nt]);
+              mma_u8u8(u, a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][0], lo[nt][1], cl[nt]);
+              o[nt][g][m][0] = __fmaf_rn(w, static_cast<float>(h[e] * 256 + u[e]), o[nt][g][m][0]);
+              o[nt][g][m][1] = __fmaf_rn(w, static_cast<float>(h[2 + e] * 256 + u[2 + e]), o[nt][g][m][1]);
+            }
           }
         }
       }
       __syncwarp();
       issue();
-      step(cur, lens, per);
     }
     if (!ok) break;
 
     // ---- the piece's rows: lane (n8, c4) holds row 4 nt + c4, channels 32 g + 8 vj + 4 vh + 2 m, + 1
+    const int ch = 8 * vj + 4 * vh;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float l = l_run[nt];
-      l += __shfl_xor_sync(0xffffffffu, l, 4);
-      l += __shfl_xor_sync(0xffffffffu, l, 8);
-      l += __shfl_xor_sync(0xffffffffu, l, 16);
-      const int r = row0 + 4 * nt + c4;
-      if (r >= p.nrep) continue;
-      const int ch = 8 * vj + 4 * vh;
-      if (slot < 0) {
-        const float inv = l <= 0.0f ? 0.0f : 1.0f / l;  // (a NaN stays)
+      l_run[nt] += __shfl_xor_sync(0xffffffffu, l_run[nt], 4);
+      l_run[nt] += __shfl_xor_sync(0xffffffffu, l_run[nt], 8);
+      l_run[nt] += __shfl_xor_sync(0xffffffffu, l_run[nt], 16);
+    }
+    if (whole) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = row0 + 4 * nt + c4;
+        if (r >= p.nrep) continue;
+        const float inv = l_run[nt] <= 0.0f ? 0.0f : 1.0f / l_run[nt];  // (a NaN stays)
         char* dst = static_cast<char*>(p.out) + 2 * (b * p.os[0] + (kvh * p.nrep + r) * p.os[1] + ch);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          uint32_t w[2];
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint2*>(dst + 64 * g) =
+              make_uint2(pack_pair(o[nt][g][0][0] * inv, o[nt][g][0][1] * inv, q_dt),
+                         pack_pair(o[nt][g][1][0] * inv, o[nt][g][1][1] * inv, q_dt));
+      }
+    } else {
+      // the run's first or last unit (a third cannot be cut): to be joined with the other warps'
+      const int k = t0 == 0;              // 0: began in an earlier run, 1: begins here
+      if (lane == 0) ends[warp][k] = cur.e * per + cur.idx;
+      float* dst = states + (warp * 2 + k) * C::kRows * kPartRow;
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const float x = (o[nt][g][m][0] + o[nt][g][m][1]) * inv, y = (o[nt][g][m][2] + o[nt][g][m][3]) * inv;
-            if (q_dt == HQ_DTYPE_BF16) {
-              w[m] = pack_bf16(x, y);
-            } else {
-              const __half2 h = __floats2half2_rn(x, y);
-              w[m] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-          }
-          *reinterpret_cast<uint2*>(dst + 64 * g) = make_uint2(w[0], w[1]);
-        }
-      } else {
-        float* dst = p.part + (static_cast<int64_t>(slot) * C::kRows + 4 * nt + c4) * kPartRow;
-        if (n8 == 0) *reinterpret_cast<float2*>(dst) = make_float2(m_run[nt], l);
+      for (int nt = 0; nt < NT; ++nt) {
+        float* row = dst + (4 * nt + c4) * kPartRow;
+        if (n8 == 0) *reinterpret_cast<float2*>(row) = make_float2(m_run[nt], l_run[nt]);
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<float4*>(dst + 4 + 32 * g + ch) =
-              make_float4(o[nt][g][0][0] + o[nt][g][0][1], o[nt][g][0][2] + o[nt][g][0][3],
-                          o[nt][g][1][0] + o[nt][g][1][1], o[nt][g][1][2] + o[nt][g][1][3]);
+          *reinterpret_cast<float4*>(row + 4 + 32 * g + ch) =
+              make_float4(o[nt][g][0][0], o[nt][g][0][1], o[nt][g][1][0], o[nt][g][1][1]);
       }
     }
+    cur.line += t1 - t0;
+    if (t1 == cur.nt && cur.line < cur.end) next_unit(cur, lens, per);
   }
   if (!ok) {
     report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
-    for (int i = done; i < issued; ++i) mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1);
+    for (int i = done; i < issued; ++i) tc::wait_bar(&full[i % C::kStages], (i / C::kStages) & 1);
+  }
+  __syncthreads();
+
+  // ---- the ends of the warps' runs, in order: runs of one unit are joined, and written where they are
+  // all of it, else left for join_kernel
+  {
+    const int row = tid >> 5, d4 = 4 * lane;  // a warp per row
+    int i = 0;
+    while (i < 2 * C::kWarps) {
+      const int unit = ends[i >> 1][i & 1];
+      int n = i + 1;
+      while (n < 2 * C::kWarps && (ends[n >> 1][n & 1] == unit || ends[n >> 1][n & 1] < 0)) ++n;
+      if (unit >= 0 && row < C::kRows) {
+        float M = -INFINITY, L = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int x = i; x < n; ++x) {
+          if (ends[x >> 1][x & 1] != unit) continue;
+          const float* st = states + (x * C::kRows + row) * kPartRow;
+          join_state(M, L, acc, st[0], st[1], *reinterpret_cast<const float4*>(st + 4 + d4));
+        }
+        const int e = unit / per, idx = unit - e * per, kvh = idx / p.n_rt, r = (idx - kvh * p.n_rt) * C::kRows + row;
+        const int first = cum[e] + idx * tiles_of(lens[e]), w0 = first / run, w1 = (first + tiles_of(lens[e]) - 1) / run;
+        if (w0 != w1) {
+          float* dst = p.part + (static_cast<int64_t>(unit + static_cast<int>(blockIdx.x)) * C::kRows + row) * kPartRow;
+          if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(M, L);
+          *reinterpret_cast<float4*>(dst + 4 + d4) = acc;
+        } else if (r < p.nrep) {
+          store_row(p, q_dt, e, kvh * p.nrep + r, d4, L, acc);
+        }
+      }
+      i = n;
+    }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
@@ -469,29 +627,19 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
   const int h = blockIdx.x % (p.Hkv * p.nrep), b = blockIdx.x / (p.Hkv * p.nrep);
   const int kvh = h / p.nrep, hr = h - kvh * p.nrep, rt = hr / rows;
   const int per = p.Hkv * p.n_rt, idx = kvh * p.n_rt + rt;
-  const int total = p.cum[p.B], chunk = max(p.min_tiles, (total + p.workers - 1) / p.workers);
+  const int run = (p.cum[p.B] + p.grid - 1) / p.grid;
   const int nt = (p.cum[b + 1] - p.cum[b]) / per;
-  const int first = p.cum[b] + idx * nt, w0 = first / chunk, w1 = (first + nt - 1) / chunk;
-  if (w0 == w1) return;                   // written by its only worker
+  const int first = p.cum[b] + idx * nt, w0 = first / run, w1 = (first + nt - 1) / run;
+  if (w0 == w1) return;                   // written by its only block
   const float* at = p.part + (static_cast<int64_t>(b * per + idx + w0) * rows + hr - rt * rows) * kPartRow;
   const int64_t dist = static_cast<int64_t>(rows) * kPartRow;
   float M = -INFINITY, L = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto add = [&](float m, float l, const float4& x) {
-    const float top = fmaxf(M, m);
-    const float f0 = M == -INFINITY ? 0.0f : exp2f(M - top), f1 = m == -INFINITY ? 0.0f : exp2f(m - top);
-    M = top;
-    L = L * f0 + l * f1;
-    acc.x = acc.x * f0 + x.x * f1;
-    acc.y = acc.y * f0 + x.y * f1;
-    acc.z = acc.z * f0 + x.z * f1;
-    acc.w = acc.w * f0 + x.w * f1;
-  };
 #pragma unroll 4
   for (int i = warp; i <= w1 - w0; i += kJoinWarps) {
     const float* x = at + i * dist;
     const float2 ml = *reinterpret_cast<const float2*>(x);
-    add(ml.x, ml.y, *reinterpret_cast<const float4*>(x + 4 + 4 * lane));
+    join_state(M, L, acc, ml.x, ml.y, *reinterpret_cast<const float4*>(x + 4 + 4 * lane));
   }
   sum[warp][lane] = acc;
   if (lane == 0) sum[warp][32] = make_float4(M, L, 0.0f, 0.0f);
@@ -500,23 +648,14 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 #pragma unroll
   for (int i = 1; i < kJoinWarps; ++i) {
     const float4 ml = sum[i][32];
-    add(ml.x, ml.y, sum[i][lane]);
+    join_state(M, L, acc, ml.x, ml.y, sum[i][lane]);
   }
-  const float inv = L <= 0.0f ? 0.0f : 1.0f / L;
-  char* dst = static_cast<char*>(p.out) + 2 * (b * p.os[0] + h * p.os[1] + 4 * lane);
-  uint2 w;
-  if (q_dt == HQ_DTYPE_BF16) {
-    w = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-  } else {
-    const __half2 x = __floats2half2_rn(acc.x * inv, acc.y * inv), y = __floats2half2_rn(acc.z * inv, acc.w * inv);
-    w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-  }
-  *reinterpret_cast<uint2*>(dst) = w;
+  store_row(p, q_dt, b, h, 4 * lane, L, acc);
 }
 
 // ---------------------------------------------------------------- host
 struct DecodePlan {
-  int nt, n_rt, grid, workers;
+  int nt, n_rt, grid;
   size_t cum_bytes, bytes;
 };
 inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -528,12 +667,9 @@ inline bool plan_decode(DecodePlan& pl, int B, int Hkv, int nrep, int64_t cap) {
   pl.n_rt = (nrep + rows - 1) / rows;
   const int64_t units = int64_t(B) * Hkv * pl.n_rt, tiles = units * std::max<int64_t>(1, (cap + kTile - 1) / kTile);
   if (tiles > (int64_t(1) << 30)) return false;
-  const int warps = pl.nt == 1 ? Cfg<1>::kWarps : Cfg<2>::kWarps;
-  // a block per SM; with few tiles one tile a warp, spread over the SMs
-  pl.grid = static_cast<int>(std::min<int64_t>(current_sm_count(), std::max<int64_t>(tiles, 1)));
-  pl.workers = pl.grid * warps;
+  pl.grid = static_cast<int>(std::min<int64_t>(current_sm_count(), tiles));
   pl.cum_bytes = align256(sizeof(int) * (B + 1));
-  pl.bytes = pl.cum_bytes + align256(sizeof(float) * static_cast<size_t>(units + pl.workers) * rows * kPartRow);
+  pl.bytes = pl.cum_bytes + align256(sizeof(float) * static_cast<size_t>(units + pl.grid) * rows * kPartRow);
   return true;
 }
 
@@ -617,8 +753,7 @@ extern "C" int hq_paged4_decode(const void* q, int q_dtype, const int64_t q_stri
   p.qk_scale = sm_scale * 1.4426950408889634f;
   p.cum = static_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.cum_bytes);
-  p.workers = pl.workers;
-  p.min_tiles = 1;
+  p.grid = pl.grid;
   p.status = status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return pl.nt == 1 ? p4::launch_decode<1>(p, q_dtype, pl, st) : p4::launch_decode<2>(p, q_dtype, pl, st);

@@ -191,15 +191,30 @@ def test_append_rows_behind_the_last_sequence():
 
 
 # ---------------------------------------------------------------- decode
+def rounded_weights(q, cache, tables, b, n, scale=None):
+    """What rounding p x scale to a 16-bit whole number of its tile's largest can do to the output: per
+    tile of 32 tokens half a step, 1 / (2 x 32512), of the largest p times the group's largest scale,
+    times sum |code|.  q [Hkv, rep, D] -> [Hkv, rep, D]."""
+    Hkv, page = cache["k"].shape[1:3]
+    k = plain.values(cache, "k", tables, b, n).transpose(0, 1)
+    p = torch.softmax(q.double() @ k.transpose(1, 2) * (scale if scale is not None else 1 / math.sqrt(D)), -1)
+    codes, sc = plain.read_codes(cache, "v", *plain.slots(tables, page, b, n))
+    pad = -n % 32
+    p = torch.nn.functional.pad(p, (0, pad)).unflatten(-1, (-1, 32)).amax(-1)                 # [Hkv, rep, tiles]
+    sc = torch.nn.functional.pad(sc.abs().permute(1, 2, 0), (0, pad)).unflatten(-1, (-1, 32)).amax(-1)  # [Hkv, 4, tiles]
+    codes = torch.nn.functional.pad(codes.double().abs().permute(1, 2, 0), (0, pad)).unflatten(-1, (-1, 32)).sum(-1)
+    return torch.einsum("hrt,hdt,hdt->hrd", p, sc.repeat_interleave(32, 1), codes) / (2 * 32512)
+
+
 def check_decode(out, q, cache, tables, lens, scale=None):
     Hkv = cache["k"].shape[1]
     for b, n in enumerate(lens):
         k, v = (plain.values(cache, x, tables, b, n).transpose(0, 1) for x in ("k", "v"))
         qq = q[b].view(Hkv, -1, D)
         ref, mag = plain.attend(qq, k, v, torch.ones((1, n), dtype=torch.bool, device="cuda"), scale)
-        # Scores: q's split 2^-17 of sum |q k| (below 6.5 x the scale's 11), the biased sums 4 groups x 4
-        # roundings of 136 sum|q| s: 2^-13 together; the weights follow, twice, against sum p |v|.
-        near(out[b].view(ref.shape), ref, mag * 2.0 ** -11)
+        # Scores: q in steps of 2^-21 of the row's largest |q| (below 5), times sum |k| (below 128 x 1.6),
+        # and float32 roundings of sums below 16 x 11: 2^-14 of a weight at most, twice, against sum p |v|.
+        near(out[b].view(ref.shape), ref, mag * 2.0 ** -12 + 1.01 * rounded_weights(qq, cache, tables, b, n, scale) if n else mag)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -284,10 +299,11 @@ def test_decode_extremes():
     for b, n in enumerate([256, 200]):
         k, v = (plain.values(cache, x, tables, b, n).transpose(0, 1) for x in ("k", "v"))
         ref, mag = plain.attend(q[b].view(1, 2, D), k, v, torch.ones((1, n), dtype=torch.bool, device="cuda"))
-        # 40 times the scores: 2^-11 x 40 of the weights' errors.  Below 2^-14 float16's steps are 2^-24
-        # whatever the value, so its rounding is off by up to 2^-25 there.
+        # 40 times the scores: 40 times the weights' errors.  Below 2^-14 float16's steps are 2^-24 whatever
+        # the value, so its rounding is off by up to 2^-25 there.
         err = (out[b].view(ref.shape).double() - ref.clamp(-65504, 65504)).abs()
-        bad = ~(err <= 2.0 ** -11 * ref.abs() + mag * 40 * 2.0 ** -11 + 2.0 ** -25) & (ref.abs() < 60000)
+        extra = mag * 40 * 2.0 ** -12 + 1.01 * rounded_weights(q[b].view(1, 2, D), cache, tables, b, n)
+        bad = ~(err <= 2.0 ** -11 * ref.abs() + extra + 2.0 ** -25) & (ref.abs() < 60000)
         assert not bad.any(), (float(err[bad].max()), ref[bad][:4].tolist())
     kernels.reset_ragged_status()
     tables[1, 1] = -1

@@ -1,7 +1,7 @@
 // Decode attention over a paged 4-bit cache (paged4.cuh), one new token per sequence, lengths on the
 // device (sm_100a).
 //
-// All sequences, kv heads and tokens are one line of 32-token tiles; every warp takes an equal run of
+// All sequences, kv heads and tokens are one line of 64-token tiles; every warp takes an equal run of
 // it, with an online softmax of its own.  Units (sequence, kv head, up to 4 NT query rows) that end
 // inside one warp's run are written by it; the ends of the warps' runs are joined in the block, and
 // what crosses a block's border leaves partial states (m, l, o) that join_kernel puts together, always
@@ -31,7 +31,8 @@ int current_sm_count();
 
 namespace p4 {
 
-constexpr int kTile = 32;                 // tokens
+constexpr int kTile = 64;                 // tokens
+constexpr int kSets = kTile / 8;
 constexpr int kMaxSeqs = 1024;
 constexpr int kPartRow = kD + 4;          // m, l, two pad words, o
 constexpr int kStageB = 2 * kTile * (kRowB + kScaleB);
@@ -46,7 +47,8 @@ struct DecodeParams {
   float qk_scale;                         // sm_scale log2(e)
   void* out;
   int64_t os[2];
-  float* part;
+  float* part;                            // states of blocks' ends
+  float* ends;                            // and of warps'
   int* cum;                               // for join_kernel: first tile of every sequence
   int grid;
   int* status;
@@ -54,13 +56,13 @@ struct DecodeParams {
 
 template <int NT>
 struct Cfg {
-  static constexpr int kWarps = NT == 1 ? 12 : 8;
-  static constexpr int kStages = NT == 1 ? 3 : 4;
+  static constexpr int kWarps = 8;
+  static constexpr int kStages = 2;
   static constexpr int kRows = 4 * NT;
   static constexpr int kOffBar = kWarps * kStages * kStageB;
-  static constexpr int kOffState = kOffBar + 8 * kWarps * kStages;  // [2 warps' ends][rows][m, l, -, -, o]
-  static constexpr int kOffCum = kOffState + 2 * kWarps * kRows * kPartRow * 4;
-  static_assert(kOffState % 16 == 0, "vector accesses");
+  static constexpr int kOffCum = kOffBar + 8 * kWarps * kStages;
+  static constexpr int kState = kRows * kPartRow;
+  static_assert(2 * kWarps <= 32 && kStages * kStageB >= 4 * kState && kStageB % 16 == 0, "ends of the warps' runs");
   static constexpr int smem(int B) { return kOffCum + 4 * (2 * B + 1); }
   static_assert(smem(kMaxSeqs) <= 232448, "one block per SM");
 };
@@ -167,9 +169,14 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
   const int n8 = lane >> 2, c4 = lane & 3;
   unsigned char* ring = smem + warp * C::kStages * kStageB;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar) + warp * C::kStages;
-  float* states = reinterpret_cast<float*>(smem + C::kOffState);
   int* cum = reinterpret_cast<int*>(smem + C::kOffCum);
-  __shared__ int ends[C::kWarps][2];      // units cut by the warps' runs: the one that began before, the one that goes on
+  // units that the warps' runs cut: one that began before and ends here (its state in global memory),
+  // and the last (its state where the warp's ring was)
+  __shared__ int ends[C::kWarps][2];
+  auto end_state = [&](int x) {
+    return x & 1 ? reinterpret_cast<float*>(smem + (x >> 1) * C::kStages * kStageB)
+                 : p.ends + (static_cast<int64_t>(blockIdx.x) * C::kWarps + (x >> 1)) * C::kState;
+  };
   int* lens = cum + p.B + 1;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (lane == 0)
@@ -220,9 +227,9 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
   }
 
   // ---- the copies' cursor, up to kStages tiles ahead.  Lane 4 i + kind copies codes (kind 0: K, 1: V)
-  // or scales (2: K, 3: V) of the tile's i-th page.
+  // or scales (2: K, 3: V) of the tile's i-th page.  (Pages are no smaller than 16 tokens.)
   Cursor ahead = cur;
-  const int kind = lane & 3, half = lane >> 2 & 1;
+  const int kind = lane & 3, part = lane >> 2 & 3;
   const int here = min(p.pg.page, kTile);  // tokens of a page in a tile
   const int row_log = kind < 2 ? 6 : 3;    // bytes of a row
   static_assert(kRowB == 64 && kScaleB == 8, "row_log");
@@ -230,8 +237,8 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
                         : kind == 2 ? reinterpret_cast<const char*>(p.pg.ksc) : reinterpret_cast<const char*>(p.pg.vsc);
   const uint32_t page_b = static_cast<uint32_t>(kind < 2 ? p.pg.cp : 2 * p.pg.sp);
   const int64_t head_b = kind < 2 ? p.pg.ch : 2 * p.pg.sh;
-  const bool mine = lane < 8 && (half == 0 || here < kTile);
-  const uint32_t to0 = smem_u32(ring) + (kind == 0 ? 0 : kind == 1 ? kOffV : kind == 2 ? kOffKs : kOffVs) + (half * here << row_log);
+  const bool mine = lane < 16 && part * here < kTile;
+  const uint32_t to0 = smem_u32(ring) + (kind == 0 ? 0 : kind == 1 ? kOffV : kind == 2 ? kOffKs : kOffVs) + (part * here << row_log);
   const uint32_t bar0 = smem_u32(full);
   const char* unit_base = nullptr;
   const int* table = nullptr;
@@ -253,8 +260,8 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
     if (ahead.line >= ahead.end) return;
     const int pi = tok >> p.pg.page_log;
     if (pi >= win + 32) load_ids(pi);
-    const int id = __shfl_sync(0xffffffffu, ids, pi - win + half);
-    const bool need = mine && tok + half * here < ahead.len;
+    const int id = __shfl_sync(0xffffffffu, ids, pi - win + part);
+    const bool need = mine && tok + part * here < ahead.len;
     const bool good = need && static_cast<uint32_t>(id) < static_cast<uint32_t>(p.pg.n_pages);
     const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, good)) * (here * (kRowB + kScaleB) / 2);  // 4 lanes a page
     const uint32_t bar = bar0 + 8 * st_in;
@@ -377,9 +384,9 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
         phase ^= 1;
       }
       const int left = len - t * kTile;   // tokens of the tile that exist
-      float sc[NT][4];                    // tokens 8 i + slot_tok
+      float sc[NT][kSets];                // tokens 8 i + slot_tok
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
+      for (int blk = 0; blk < kSets / 2; ++blk) {
         const unsigned char* kr = s + blk * 16 * kRowB + k_off;
         const uint4 w0 = *reinterpret_cast<const uint4*>(kr);
         const uint4 w1 = *reinterpret_cast<const uint4*>(kr + 8 * kRowB);
@@ -413,10 +420,12 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
         }
       }
       // ---- softmax of the tile, relative to its own maximum; f brings it to the running one
-      float pr[NT][4], f[NT];
+      float f[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float mt = fmaxf(fmaxf(sc[nt][0], sc[nt][1]), fmaxf(sc[nt][2], sc[nt][3]));
+        float mt = sc[nt][0];
+#pragma unroll
+        for (int i = 1; i < kSets; ++i) mt = fmaxf(mt, sc[nt][i]);
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
@@ -436,100 +445,97 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
         f[nt] = mt == -INFINITY ? 0.0f : ex2(mt - m_run[nt]);
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pr[nt][i] = sc[nt][i] == -INFINITY ? 0.0f : ex2(sc[nt][i] - mt);
-          sum += pr[nt][i];
+        for (int i = 0; i < kSets; ++i) {
+          sc[nt][i] = sc[nt][i] == -INFINITY ? 0.0f : ex2(sc[nt][i] - mt);
+          sum += sc[nt][i];
         }
         l_run[nt] = __fmaf_rn(f[nt], sum, l_run[nt]);
       }
-      // ---- the tokens' V scales, relative to the tile's largest of each group
-      float vs[4][4], top[4];
-      {
-        uint2 u[4];
-        __half2 a = __float2half2_rn(0.0f), b2 = a;
+      // ---- P V, two groups at a time: 2 gg in columns 2 r, 2 gg + 1 in 2 r + 1
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+      for (int gg = 0; gg < 2; ++gg) {
+        // the tokens' V scales, and the largest
+        uint32_t u[kSets];
+        __half2 big = __float2half2_rn(0.0f);
+#pragma unroll
+        for (int i = 0; i < kSets; ++i) {
           const int tk = 8 * i + slot_tok;
-          u[i] = *reinterpret_cast<const uint2*>(s + kOffVs + tk * kScaleB);
-          if (tk >= left) u[i] = make_uint2(0, 0);  // what no token wrote may be anything
-          a = __hmax2_nan(a, __habs2(*reinterpret_cast<const __half2*>(&u[i].x)));
-          b2 = __hmax2_nan(b2, __habs2(*reinterpret_cast<const __half2*>(&u[i].y)));
+          u[i] = *reinterpret_cast<const uint32_t*>(s + kOffVs + tk * kScaleB + 4 * gg);
+          if (tk >= left) u[i] = 0;       // what no token wrote may be anything
+          big = __hmax2_nan(big, __habs2(*reinterpret_cast<const __half2*>(&u[i])));
         }
 #pragma unroll
-        for (int d = 4; d <= 16; d <<= 1) {
-          a = __hmax2_nan(a, __shfl_xor_sync(0xffffffffu, a, d));
-          b2 = __hmax2_nan(b2, __shfl_xor_sync(0xffffffffu, b2, d));
+        for (int d = 4; d <= 16; d <<= 1) big = __hmax2_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
+        const float2 top = __half22float2(big);
+        const float inv0 = top.x == 0.0f ? 0.0f : kWeight * rcp(top.x), inv1 = top.y == 0.0f ? 0.0f : kWeight * rcp(top.y);
+        // weights as whole numbers, then as operands: digits of 32 tokens each
+        uint32_t hi[NT][kSets / 2], lo[NT][kSets / 2];
+#pragma unroll
+        for (int i = 0; i < kSets / 2; ++i) {
+          const float2 x = half2_of(u[2 * i]), y = half2_of(u[2 * i + 1]);
+          const float x0 = x.x * inv0, x1 = x.y * inv1, y0 = y.x * inv0, y1 = y.y * inv1;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            constexpr float kRound = 12582912.0f;  // 1.5 x 2^23: the whole number in the low bits
+            const uint32_t a = transpose8(prmt(__float_as_uint(__fmaf_rn(sc[nt][2 * i], x0, kRound)),
+                                               __float_as_uint(__fmaf_rn(sc[nt][2 * i], x1, kRound)), 0x5410u));
+            const uint32_t b2 = transpose8(prmt(__float_as_uint(__fmaf_rn(sc[nt][2 * i + 1], y0, kRound)),
+                                                __float_as_uint(__fmaf_rn(sc[nt][2 * i + 1], y1, kRound)), 0x5410u));
+            lo[nt][i] = prmt(a, b2, 0x6420u);
+            hi[nt][i] = prmt(a, b2, 0x7531u);
+          }
         }
-        const float2 ta = __half22float2(a), tb = __half22float2(b2);
-        top[0] = ta.x;
-        top[1] = ta.y;
-        top[2] = tb.x;
-        top[3] = tb.y;
-        float inv[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) inv[g] = top[g] == 0.0f ? 0.0f : kWeight * rcp(top[g]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 x = half2_of(u[i].x), y = half2_of(u[i].y);
-          vs[i][0] = x.x * inv[0];
-          vs[i][1] = x.y * inv[1];
-          vs[i][2] = y.x * inv[2];
-          vs[i][3] = y.y * inv[3];
-        }
-      }
-      // ---- P V
-      uint4 vw[8];                        // chunk vj of this lane's tokens: sets 0 .. 3, slots 2 c4 and 2 c4 + 1
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        vw[2 * i] = *reinterpret_cast<const uint4*>(s + i * 8 * kRowB + va_off);
-        vw[2 * i + 1] = *reinterpret_cast<const uint4*>(s + i * 8 * kRowB + vb_off);
-      }
-#pragma unroll
-      for (int gg = 0; gg < 2; ++gg) {    // groups 2 gg (columns 2 r) and 2 gg + 1 (2 r + 1)
-        uint32_t hi[NT][2], lo[NT][2];
-        int ch[NT][4], cl[NT][4];
+        int ch[NT][4], cl[NT][4];         // the codes' offset
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          constexpr float kRound = 12582912.0f;  // 1.5 x 2^23: the whole number in the low bits
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = transpose8(prmt(__float_as_uint(__fmaf_rn(pr[nt][i], vs[i][2 * gg], kRound)),
-                                   __float_as_uint(__fmaf_rn(pr[nt][i], vs[i][2 * gg + 1], kRound)), 0x5410u));
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            lo[nt][i] = prmt(w[2 * i], w[2 * i + 1], 0x6420u);
-            hi[nt][i] = prmt(w[2 * i], w[2 * i + 1], 0x7531u);
-          }
-          constexpr uint32_t kM8 = 0xf8f8f8f8u;  // the codes' offset
+          constexpr uint32_t kM8 = 0xf8f8f8f8u;
           mma_s8s8(ch[nt], kM8, kM8, kM8, kM8, hi[nt][0], hi[nt][1], kZero);
           mma_s8u8(cl[nt], kM8, kM8, kM8, kM8, lo[nt][0], lo[nt][1], kZero);
+#pragma unroll
+          for (int k = 1; k < kSets / 4; ++k) {
+            mma_s8s8(ch[nt], kM8, kM8, kM8, kM8, hi[nt][2 * k], hi[nt][2 * k + 1], ch[nt]);
+            mma_s8u8(cl[nt], kM8, kM8, kM8, kM8, lo[nt][2 * k], lo[nt][2 * k + 1], cl[nt]);
+          }
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int g = 2 * gg + e;
-          auto word = [&](int i) { return g == 0 ? vw[i].x : g == 1 ? vw[i].y : g == 2 ? vw[i].z : vw[i].w; };
-          uint32_t a[2][4];               // [channels 0, 1 / 2, 3][operand register]
+          // the group's word of chunk vj of token slots 2 c4 and 2 c4 + 1, set by set (both groups' words in
+          // one load of 8 bytes hold 32 registers more)
+          auto word = [&](int i) {
+            return *reinterpret_cast<const uint32_t*>(s + (i >> 1) * 8 * kRowB + (i & 1 ? vb_off : va_off) + 4 * g);
+          };
+          int h[NT][2][4], q8[NT][2][4];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t x = prmt(word(4 * k), word(4 * k + 1), vsel), y = prmt(word(4 * k + 2), word(4 * k + 3), vsel);
-            const uint32_t b0 = prmt(x, y, 0x5410u), b1 = prmt(x, y, 0x7632u);
-            constexpr uint32_t kLow = 0x0f0f0f0fu;
-            a[0][2 * k] = b0 & kLow;
-            a[0][2 * k + 1] = (b0 >> 4) & kLow;
-            a[1][2 * k] = b1 & kLow;
-            a[1][2 * k + 1] = (b1 >> 4) & kLow;
+          for (int k = 0; k < kSets / 4; ++k) {
+            uint32_t a[2][4];             // [channels 0, 1 / 2, 3][operand register]
+#pragma unroll
+            for (int y8 = 0; y8 < 2; ++y8) {
+              const int w0 = 8 * k + 4 * y8;
+              const uint32_t x = prmt(word(w0), word(w0 + 1), vsel), y = prmt(word(w0 + 2), word(w0 + 3), vsel);
+              const uint32_t b0 = prmt(x, y, 0x5410u), b1 = prmt(x, y, 0x7632u);
+              constexpr uint32_t kLow = 0x0f0f0f0fu;
+              a[0][2 * y8] = b0 & kLow;
+              a[0][2 * y8 + 1] = (b0 >> 4) & kLow;
+              a[1][2 * y8] = b1 & kLow;
+              a[1][2 * y8 + 1] = (b1 >> 4) & kLow;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                mma_u8s8(h[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], hi[nt][2 * k], hi[nt][2 * k + 1], k ? h[nt][m] : ch[nt]);
+                mma_u8u8(q8[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][2 * k], lo[nt][2 * k + 1], k ? q8[nt][m] : cl[nt]);
+              }
           }
+          // 64 x 8 x 32512 is below 2^24: exact in float32
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float w = f[nt] * (top[g] * (1.0f / kWeight));
+            const float w = f[nt] * ((e ? top.y : top.x) * (1.0f / kWeight));
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-              int h[4], u[4];
-              mma_u8s8(h, a[m][0], a[m][1], a[m][2], a[m][3], hi[nt][0], hi[nt][1], ch[nt]);
-              mma_u8u8(u, a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][0], lo[nt][1], cl[nt]);
-              o[nt][g][m][0] = __fmaf_rn(w, static_cast<float>(h[e] * 256 + u[e]), o[nt][g][m][0]);
-              o[nt][g][m][1] = __fmaf_rn(w, static_cast<float>(h[2 + e] * 256 + u[2 + e]), o[nt][g][m][1]);
+              o[nt][g][m][0] = __fmaf_rn(w, static_cast<float>(h[nt][m][e] * 256 + q8[nt][m][e]), o[nt][g][m][0]);
+              o[nt][g][m][1] = __fmaf_rn(w, static_cast<float>(h[nt][m][2 + e] * 256 + q8[nt][m][2 + e]), o[nt][g][m][1]);
             }
           }
         }
@@ -562,9 +568,10 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
       }
     } else {
       // the run's first or last unit (a third cannot be cut): to be joined with the other warps'
-      const int k = t0 == 0;              // 0: began in an earlier run, 1: begins here
-      if (lane == 0) ends[warp][k] = cur.e * per + cur.idx;
-      float* dst = states + (warp * 2 + k) * C::kRows * kPartRow;
+      const int x = 2 * warp + (cur.line + t1 - t0 == cur.end);
+      if (lane == 0) ends[warp][x & 1] = cur.e * per + cur.idx;
+      float* dst = end_state(x);
+      __syncwarp();                       // (the last tile has been read by all lanes)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float* row = dst + (4 * nt + c4) * kPartRow;
@@ -584,34 +591,51 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
   }
   __syncthreads();
 
-  // ---- the ends of the warps' runs, in order: runs of one unit are joined, and written where they are
-  // all of it, else left for join_kernel
+  // ---- the ends of the warps' runs: those of one unit are joined, in order, and written where they are
+  // all of it, else left for join_kernel.  A warp per unit and row, a lane per end.
   {
-    const int row = tid >> 5, d4 = 4 * lane;  // a warp per row
-    int i = 0;
-    while (i < 2 * C::kWarps) {
-      const int unit = ends[i >> 1][i & 1];
-      int n = i + 1;
-      while (n < 2 * C::kWarps && (ends[n >> 1][n & 1] == unit || ends[n >> 1][n & 1] < 0)) ++n;
-      if (unit >= 0 && row < C::kRows) {
-        float M = -INFINITY, L = 0.0f;
+    const int mine = lane < 2 * C::kWarps ? ends[lane >> 1][lane & 1] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, mine);
+    uint32_t firsts = __ballot_sync(0xffffffffu, mine >= 0 && lane == __ffs(same) - 1);
+    for (int task = 0; firsts; firsts &= firsts - 1) {
+      const int at = __ffs(firsts) - 1;
+      const int unit = __shfl_sync(0xffffffffu, mine, at);
+      const uint32_t set = __shfl_sync(0xffffffffu, same, at);
+      for (int row = 0; row < C::kRows; ++row, ++task) {
+        if (task % C::kWarps != warp) continue;
+        float m = -INFINITY, l = 0.0f;
+        if (set >> lane & 1) {
+          const float2 ml = *reinterpret_cast<const float2*>(end_state(lane) + row * kPartRow);
+          m = ml.x;
+          l = ml.y;
+        }
+        float M = m;
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+        const float f = m == -INFINITY ? 0.0f : exp2f(m - M);
+        float L = l * f;                  // (a sum that is no number stays one)
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int x = i; x < n; ++x) {
-          if (ends[x >> 1][x & 1] != unit) continue;
-          const float* st = states + (x * C::kRows + row) * kPartRow;
-          join_state(M, L, acc, st[0], st[1], *reinterpret_cast<const float4*>(st + 4 + d4));
+        for (uint32_t left = set; left; left &= left - 1) {
+          const int x = __ffs(left) - 1;
+          const float g = __shfl_sync(0xffffffffu, f, x);
+          const float4 o = *reinterpret_cast<const float4*>(end_state(x) + row * kPartRow + 4 + 4 * lane);
+          acc.x = __fmaf_rn(o.x, g, acc.x);
+          acc.y = __fmaf_rn(o.y, g, acc.y);
+          acc.z = __fmaf_rn(o.z, g, acc.z);
+          acc.w = __fmaf_rn(o.w, g, acc.w);
         }
         const int e = unit / per, idx = unit - e * per, kvh = idx / p.n_rt, r = (idx - kvh * p.n_rt) * C::kRows + row;
-        const int first = cum[e] + idx * tiles_of(lens[e]), w0 = first / run, w1 = (first + tiles_of(lens[e]) - 1) / run;
-        if (w0 != w1) {
+        const int n = tiles_of(lens[e]), first = cum[e] + idx * n;
+        if (first / run != (first + n - 1) / run) {
           float* dst = p.part + (static_cast<int64_t>(unit + static_cast<int>(blockIdx.x)) * C::kRows + row) * kPartRow;
           if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(M, L);
-          *reinterpret_cast<float4*>(dst + 4 + d4) = acc;
+          *reinterpret_cast<float4*>(dst + 4 + 4 * lane) = acc;
         } else if (r < p.nrep) {
-          store_row(p, q_dt, e, kvh * p.nrep + r, d4, L, acc);
+          store_row(p, q_dt, e, kvh * p.nrep + r, 4 * lane, L, acc);
         }
       }
-      i = n;
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -656,7 +680,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 // ---------------------------------------------------------------- host
 struct DecodePlan {
   int nt, n_rt, grid;
-  size_t cum_bytes, bytes;
+  size_t cum_bytes, part_bytes, bytes;
 };
 inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 inline bool plan_decode(DecodePlan& pl, int B, int Hkv, int nrep, int64_t cap) {
@@ -669,7 +693,8 @@ inline bool plan_decode(DecodePlan& pl, int B, int Hkv, int nrep, int64_t cap) {
   if (tiles > (int64_t(1) << 30)) return false;
   pl.grid = static_cast<int>(std::min<int64_t>(current_sm_count(), tiles));
   pl.cum_bytes = align256(sizeof(int) * (B + 1));
-  pl.bytes = pl.cum_bytes + align256(sizeof(float) * static_cast<size_t>(units + pl.grid) * rows * kPartRow);
+  pl.part_bytes = align256(sizeof(float) * static_cast<size_t>(units + pl.grid) * rows * kPartRow);
+  pl.bytes = pl.cum_bytes + pl.part_bytes + sizeof(float) * static_cast<size_t>(pl.grid) * (pl.nt == 1 ? Cfg<1>::kWarps * Cfg<1>::kState : Cfg<2>::kWarps * Cfg<2>::kState);
   return true;
 }
 
@@ -753,6 +778,7 @@ extern "C" int hq_paged4_decode(const void* q, int q_dtype, const int64_t q_stri
   p.qk_scale = sm_scale * 1.4426950408889634f;
   p.cum = static_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.cum_bytes);
+  p.ends = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.cum_bytes + pl.part_bytes);
   p.grid = pl.grid;
   p.status = status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

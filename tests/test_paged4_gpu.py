@@ -193,16 +193,16 @@ def test_append_rows_behind_the_last_sequence():
 # ---------------------------------------------------------------- decode
 def rounded_weights(q, cache, tables, b, n, scale=None):
     """What rounding p x scale to a 16-bit whole number of its tile's largest can do to the output: per
-    tile of 32 tokens half a step, 1 / (2 x 32512), of the largest p times the group's largest scale,
+    tile of 64 tokens half a step, 1 / (2 x 32512), of the largest p times the group's largest scale,
     times sum |code|.  q [Hkv, rep, D] -> [Hkv, rep, D]."""
     Hkv, page = cache["k"].shape[1:3]
     k = plain.values(cache, "k", tables, b, n).transpose(0, 1)
     p = torch.softmax(q.double() @ k.transpose(1, 2) * (scale if scale is not None else 1 / math.sqrt(D)), -1)
     codes, sc = plain.read_codes(cache, "v", *plain.slots(tables, page, b, n))
-    pad = -n % 32
-    p = torch.nn.functional.pad(p, (0, pad)).unflatten(-1, (-1, 32)).amax(-1)                 # [Hkv, rep, tiles]
-    sc = torch.nn.functional.pad(sc.abs().permute(1, 2, 0), (0, pad)).unflatten(-1, (-1, 32)).amax(-1)  # [Hkv, 4, tiles]
-    codes = torch.nn.functional.pad(codes.double().abs().permute(1, 2, 0), (0, pad)).unflatten(-1, (-1, 32)).sum(-1)
+    pad = -n % 64
+    p = torch.nn.functional.pad(p, (0, pad)).unflatten(-1, (-1, 64)).amax(-1)                 # [Hkv, rep, tiles]
+    sc = torch.nn.functional.pad(sc.abs().permute(1, 2, 0), (0, pad)).unflatten(-1, (-1, 64)).amax(-1)  # [Hkv, 4, tiles]
+    codes = torch.nn.functional.pad(codes.double().abs().permute(1, 2, 0), (0, pad)).unflatten(-1, (-1, 64)).sum(-1)
     return torch.einsum("hrt,hdt,hdt->hrd", p, sc.repeat_interleave(32, 1), codes) / (2 * 32512)
 
 

@@ -7,15 +7,15 @@
 // by P * inv_freq[j] (pairs (j, j + rot / 2), or (2j, 2j + 1) interleaved).  q' and k' are rounded
 // once, to the model's type; K's codes are those of the unrounded k (paged4.cuh).
 //
-// Codes are those of exact arithmetic.  P * inv_freq is formed in float64 and taken as a fraction of
-// a turn; norms and turns are float32, off by at most kSlack of |x cos| + |o sin|.  A row with a
-// quotient or a scale closer to a rounding border than that (about 1 in 100) is formed again in
-// float64.  V's codes come from its 16-bit values: an 11-bit x over an 11-bit s is 2^-13 away from a
-// border unless it lies on it, and one corrected division finds both cases.
+// Codes are those of exact arithmetic.  P * inv_freq, its cos and its sin are formed in float64 (once a
+// token, kept as two float32 parts in shared memory); norms and turns are float32, off by at most kSlack
+// of |x w| + |o w_o|.  The k rows with a quotient or a scale closer to a rounding border than that (one in
+// 40) are listed, and formed again in float64 at the end of the block, its half-warps sharing them (on
+// the spot, one by one, they took a fifth of the time: 8 x 4096 tokens 149 us).  V's codes come from its 16-bit values: an 11-bit x over an 11-bit s
+// is 2^-13 away from a border unless it lies on it, and one corrected division finds both cases.
 //
-// Bound by memory: per token (Hq + 2 Hkv) rows read, Hq (+ Hkv) rows and Hkv 144 bytes written.  16
-// lanes hold a row (8 channels, 16 bytes, each); a half-warp takes one token and all of its rows, two
-// in flight.  cos and sin of a block's tokens are formed once, in shared memory.
+// Per token (Hq + 2 Hkv) rows are read, Hq (+ Hkv) rows and Hkv 144 bytes written.  16 lanes hold a row
+// (8 channels, 16 bytes, each); a half-warp takes one token and all of its rows, 7 of them in flight.
 #include <algorithm>
 
 #include "paged4.cuh"
@@ -27,6 +27,7 @@ namespace p4 {
 
 constexpr int kThreads = 128;
 constexpr int kTok = kThreads / 16;       // tokens per block
+constexpr int kRing = 8;                  // rows in flight for each, a power of two
 
 struct AppendParams {
   Pages pg;
@@ -50,13 +51,12 @@ struct AppendParams {
   int copy_rest;                          // q_out takes q's rows behind the last sequence
   int* status;
   int rows_per_block, groups;
-  float slack;
 };
 
-// Error of the float32 route, of |x w| + |o w_o|: half that of a sum of 128 squares (8 in a lane,
-// 4 rounds: 12 x 2^-24) 2^-21.4, rsqrt 2^-22, cos and sin 2^-22.5 and their product with a weight
-// 2^-24, the turn's roundings 2^-23.4 and r's product 2^-24: 2^-19.95 in all.
-constexpr float kSlack = 1.0e-6f;
+// Error of the float32 route, relative to |x w| + |o w_o| (times r and the factor), in units of 2^-24:
+// half that of a sum of 128 squares (4 in a lane's half, the halves, 4 rounds) 4, the mean 1 and r 1, cos
+// or sin 1, their weight 1 and factor 1, the turn's two products and sum 2, r's product 1: 12.
+constexpr float kSlack = 12.0f / 16777216.0f;
 
 template <int DT>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
@@ -73,28 +73,69 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 // The scale of a group from amax / 7.5: NaN where amax is no number, the largest float16 above it.
 __device__ __forceinline__ __half group_scale(float a75) {
   if (!(a75 < INFINITY)) return __ushort_as_half(0x7fff);
   return __float2half_rn(fminf(a75, 65504.0f));
 }
-// 8 rounded quotients as a word of nibbles
-__device__ __forceinline__ uint32_t pack_codes(const float (&t)[8]) {
-  float c[8];
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// a / 7.5 of a 16-bit a, correctly rounded: one correction of the product with 2 / 15
+__device__ __forceinline__ float over75(float a) {
+  const float q = a * 0.13333334f;
+  return a < 1e30f ? __fmaf_rn(__fmaf_rn(-q, 7.5f, a), 0.13333334f, q) : q;
+}
+// Channels in pairs (e, e + 4): 8 codes become a word of nibbles as one whole number per half.
+// k: whole numbers.
+__device__ __forceinline__ uint32_t pack_codes(const F2 (&k)[4]) {
+  F2 c[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) c[e] = fminf(fmaxf(rintf(t[e]), -8.0f), 7.0f);
-  // 4 codes as one whole number below 2^15 (c + 8 would cost an add each: 8 * 0x1111 at once)
-  const float lo = __fmaf_rn(4096.0f, c[3], __fmaf_rn(256.0f, c[2], __fmaf_rn(16.0f, c[1], c[0])));
-  const float hi = __fmaf_rn(4096.0f, c[7], __fmaf_rn(256.0f, c[6], __fmaf_rn(16.0f, c[5], c[4])));
-  return static_cast<uint32_t>(static_cast<int>(lo) + 0x8888) |
-         static_cast<uint32_t>(static_cast<int>(hi) + 0x8888) << 16;
+  for (int e = 0; e < 4; ++e) {
+    float a, b;
+    f2_split(k[e], a, b);
+    c[e] = f2_make(fminf(fmaxf(a, -8.0f), 7.0f), fminf(fmaxf(b, -8.0f), 7.0f));
+  }
+  auto same = [](float x) { return f2_make(x, x); };
+  // (8 x 0x1111 makes each code + 8; under 1.5 x 2^23 the low 16 bits hold the number)
+  const F2 v = f2_fma(c[3], same(4096.0f), f2_fma(c[2], same(256.0f), f2_fma(c[1], same(16.0f), c[0])));
+  const F2 w = f2_add(v, same(12582912.0f + 34952.0f));
+  return prmt(f2_lo_bits(w), f2_hi_bits(w), 0x5410u);
+}
+// rint(x / s) of 16-bit x, s, with rs ~ 1 / s: the quotient corrected once, exact where it is a tie
+__device__ __forceinline__ void quotients(const F2 (&x)[4], float s, float rs, F2 (&k)[4]) {
+  const F2 ns = f2_make(-s, -s), r2 = f2_make(rs, rs), big = f2_make(12582912.0f, 12582912.0f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const F2 q = f2_mul(x[e], r2);
+    k[e] = f2_sub(f2_add(f2_fma(f2_fma(q, ns, x[e]), r2, q), big), big);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void unpack_pairs(const uint4& w, F2 (&x)[4]) {
+  float f[8];
+  Vec16<DT>::unpack(w, f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = f2_make(f[e], f[e + 4]);
+}
+__device__ __forceinline__ float absmax(const F2 (&x)[4]) {  // NaN if any is
+  float m = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float a, b;
+    f2_split(x[e], a, b);
+    m = max_nan(m, max_nan(fabsf(a), fabsf(b)));
+  }
+  return m;
+}
+template <int DT>
+__device__ __forceinline__ uint4 pack_row(const F2 (&y)[4]) {
+  float a[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f2_split(y[e], a[e], a[e + 4]);
+  return make_uint4(pack16<DT>(a[0], a[1]), pack16<DT>(a[2], a[3]), pack16<DT>(a[4], a[5]), pack16<DT>(a[6], a[7]));
 }
 
 // One k row in float64 (all 16 lanes of the half-warp `mask`): this lane's word and group's scale.
@@ -104,58 +145,71 @@ struct Exact {
 };
 template <int DT>
 __device__ __noinline__ Exact exact_row(const AppendParams& p, const uint4& x, unsigned mask, int partner,
-                                        double pos, int l) {
+                                        const float4* turn, int l) {
   float f[8];
   Vec16<DT>::unpack(x, f);
   const int d0 = 8 * l, half = p.rot / 2;
-  double y[8], o[8], r = 1.0;
+  double y[8], r = 1.0;
   if (p.kw) {
     double s = 0.0;
-#pragma unroll 1
-    for (int e = 0; e < 8; ++e) s += static_cast<double>(f[e]) * f[e];
-#pragma unroll 1
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), s);
+#pragma unroll
     for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor_sync(mask, s, m);
-    r = 1.0 / sqrt(s / kD + static_cast<double>(p.eps));
+    s = s / kD + static_cast<double>(p.eps);
+    r = rsqrtf(static_cast<float>(s));
+    r = r * fma(-0.5 * s * r, r, 1.5);    // 2^-22 becomes 2^-43
   }
-#pragma unroll 1
+#pragma unroll
   for (int e = 0; e < 8; ++e) {
-    double w = 1.0;
+    float w = 1.0f;
     if (p.kw) w = p.w_f32 ? static_cast<const float*>(p.kw)[d0 + e]
                           : Elem<DT>::to_f32(static_cast<const typename Elem<DT>::T*>(p.kw)[d0 + e]);
-    y[e] = f[e] * r * w;
+    y[e] = f[e] * r * static_cast<double>(w);
   }
-#pragma unroll 1
-  for (int e = 0; e < 8; ++e) o[e] = p.inter ? y[e ^ 1] : __shfl_sync(mask, y[e], partner);
-  double amax = 0.0;
-#pragma unroll 1
+  double amax = 0.0, z[8];
+#pragma unroll
   for (int e = 0; e < 8; ++e) {
+    const double o = p.inter ? y[e ^ 1] : __shfl_sync(mask, y[e], partner);
     const int d = d0 + e;
+    z[e] = y[e];
     if (d < p.rot) {
-      const int j = p.inter ? d / 2 : d < half ? d : d - half;
-      const bool lead = p.inter ? !(d & 1) : d < half;
-      double s, c;
-      sincos(pos * static_cast<double>(p.inv_freq[j]), &s, &c);
-      y[e] = (lead ? y[e] * c - o[e] * s : y[e] * c + o[e] * s) * static_cast<double>(p.factor);
+      const float4 t = turn[p.inter ? d / 2 : d < half ? d : d - half];
+      const double c = static_cast<double>(t.x) + t.z, s = static_cast<double>(t.y) + t.w;
+      z[e] = ((p.inter ? !(d & 1) : d < half) ? y[e] * c - o * s : y[e] * c + o * s) * static_cast<double>(p.factor);
     }
+    amax = fmax(amax, fabs(z[e]));
   }
-#pragma unroll 1
-  for (int e = 0; e < 8; ++e) amax = fmax(amax, fabs(y[e]));
   amax = fmax(amax, __shfl_xor_sync(mask, amax, 1));
   amax = fmax(amax, __shfl_xor_sync(mask, amax, 2));
   Exact out;
-  out.scale = group_scale(static_cast<float>(amax / 7.5));
-  const double s = __half2float(out.scale);
-  float t[8];
-#pragma unroll 1
-  for (int e = 0; e < 8; ++e) t[e] = s > 0.0 ? static_cast<float>(fmin(fmax(rint(y[e] / s), -8.0), 7.0)) : 0.0f;
-  out.word = pack_codes(t);
+  out.scale = group_scale(static_cast<float>(amax * (2.0 / 15.0)));
+  const float s = __half2float(out.scale);
+  double rs = 0.0;
+  if (s > 0.0f) {
+    rs = rcp(s);
+    rs = rs * fma(-static_cast<double>(s), rs, 2.0);
+  }
+  F2 k[4];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {           // (channels that are not turned can lie on a border: corrected, exact there)
+    const double t = z[e] * rs;
+    z[e] = rint(fma(fma(-t, static_cast<double>(s), z[e]), rs, t));
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) k[e] = f2_make(static_cast<float>(z[e]), static_cast<float>(z[e + 4]));
+  out.word = pack_codes(k);
   return out;
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_constant__ AppendParams p) {
   using T16 = typename Elem<DT>::T;
-  __shared__ float2 turn[kTok][kD / 2];   // cos, sin
+  __shared__ uint4 ring[kTok][kRing * 16];
+  __shared__ float4 turn[kTok][kD / 2];   // cos and sin, and what is left of them
+  extern __shared__ uint32_t again[];     // k rows to form again: token of the block, head
+  __shared__ int n_again;
+  __shared__ int4 where[kTok];
   const int tid = threadIdx.x, lane = tid & 31, sub = tid >> 4, l = lane & 15, d0 = 8 * l;
   const unsigned mask = 0xffffu << (lane & 16);
   const int group = static_cast<int>(blockIdx.x % p.groups);
@@ -182,16 +236,44 @@ __global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_consta
   if (live && !fits && l == 0) report_error(p.status, HQ_ERR_INVALID_ARGUMENT);
   const int place = static_cast<int>(at) & (p.pg.page - 1);
   const double pos = static_cast<double>(at + (live && p.pos_offset ? p.pos_offset[b] : 0));
+  const bool plain_k = !p.kw && p.rot == 0;  // k is coded as it came: no rounding before the codes
+  if (l == 0) where[sub] = make_int4(tok, pid, place, 0);
+  if (tid == 0) n_again = 0;
+  __syncthreads();
   const int half = p.rot / 2;
   const int r0 = group * p.rows_per_block, r1 = min(p.Hq + 2 * p.Hkv, r0 + p.rows_per_block);
+  // rows r0 .. r1 - 1 (q heads, k heads, v heads) arrive in order through a ring of this half-warp's; a
+  // lane copies and reads its own 16 bytes
+  const uint4* slots = ring[sub] + l;
+  const uint32_t slots_at = smem_u32(slots);
+  int ahead = r0, turn_at = 0;            // the next row to fetch, the first of another tensor
+  const char* from = nullptr;
+  int64_t step = 0;
+  auto fetch = [&]() {
+    if (ahead >= turn_at && ahead < r1) {
+      const int h0 = ahead < p.Hq ? 0 : ahead < p.Hq + p.Hkv ? p.Hq : p.Hq + p.Hkv;  // the tensor's first row
+      const void* base = ahead < p.Hq ? p.q : ahead < p.Hq + p.Hkv ? p.k : p.v;
+      const int64_t* st = ahead < p.Hq ? p.qs : ahead < p.Hq + p.Hkv ? p.ks : p.vs;
+      from = static_cast<const char*>(base) + 2 * (tok * st[0] + (ahead - h0) * st[1] + d0);
+      step = 2 * st[1];
+      turn_at = ahead < p.Hq ? p.Hq : ahead < p.Hq + p.Hkv ? p.Hq + p.Hkv : 0x7fffffff;
+    }
+    if (ahead < r1)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots_at + 256 * (ahead & (kRing - 1))), "l"(from) : "memory");
+    cp_async_commit();                    // (a group a row, there or not)
+    from += step;
+    ++ahead;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kRing - 1; ++i) fetch();
   if (p.rot > 0 && r0 < p.Hq + p.Hkv && live) {
+#pragma unroll 2
     for (int j = l; j < half; j += 16) {
       const double turns = pos * static_cast<double>(p.inv_freq[j]) * 0.15915494309189535;
-      const double f = 2.0 * (turns - rint(turns));  // angle / pi
-      const float h = static_cast<float>(f), r = static_cast<float>(f - h) * 3.14159265f;
-      float s, c;
-      sincospif(h, &s, &c);
-      turn[sub][j] = make_float2(__fmaf_rn(-s, r, c) * p.factor, __fmaf_rn(c, r, s) * p.factor);
+      double s, c;
+      sincospi(2.0 * (turns - rint(turns)), &s, &c);
+      const float ch = static_cast<float>(c), sh = static_cast<float>(s);
+      turn[sub][j] = make_float4(ch, sh, static_cast<float>(c - ch), static_cast<float>(s - sh));
     }
   }
   __syncwarp();
@@ -199,11 +281,10 @@ __global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_consta
   const bool lead = d0 < half;
   const int partner = (lane & 16) + (p.inter || !turned ? l : lead ? l + half / 8 : l - half / 8);
 
-  // y_e = r (x_e cs_e + o_e sg_e), o the partner: weights and the angle's cos and sin in one factor
-  float cs[8], sg[8], wmax = 0.0f;
+  // y = r (x cs + o sg), o the partner: weights, factor and the angle's cos and sin in one
+  F2 cs[4], sg[4];
   auto factors = [&](const void* w) {
-    float wt[8];
-    wmax = 0.0f;
+    float wt[8], c[8], g[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       wt[e] = 1.0f;
@@ -212,166 +293,182 @@ __global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_consta
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float wo = p.inter ? wt[e ^ 1] : __shfl_sync(0xffffffffu, wt[e], partner);
-      wmax = fmaxf(wmax, fmaxf(fabsf(wt[e]), fabsf(wo)));
-      cs[e] = wt[e];
-      sg[e] = 0.0f;
+      c[e] = wt[e];
+      g[e] = 0.0f;
       if (turned && live) {
         const int j = p.inter ? (d0 + e) / 2 : lead ? d0 + e : d0 + e - half;
-        const float2 t = turn[sub][j];
-        cs[e] = t.x * wt[e];
-        sg[e] = ((p.inter ? !(e & 1) : lead) ? -t.y : t.y) * wo;
+        const float2 t = *reinterpret_cast<const float2*>(&turn[sub][j]);
+        c[e] = t.x * (wt[e] * p.factor);
+        g[e] = ((p.inter ? !(e & 1) : lead) ? -t.y : t.y) * (wo * p.factor);
       }
     }
-  };
-  auto each = [&](const void* src, const int64_t (&st)[2], int h0, int h1, auto&& row_of) {
-    const char* base = static_cast<const char*>(src) + 2 * (tok * st[0] + d0);
-    const int64_t step = 2 * st[1];
-    uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-    if (h0 < h1) x0 = ld_stream(base + h0 * step);
-    if (h0 + 1 < h1) x1 = ld_stream(base + (h0 + 1) * step);
-#pragma unroll 1
-    for (int h = h0; h < h1; ++h) {
-      const uint4 x = x0;
-      x0 = x1;
-      if (h + 2 < h1) x1 = ld_stream(base + (h + 2) * step);
-      row_of(h, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      cs[e] = f2_make(c[e], c[e + 4]);
+      sg[e] = f2_make(g[e], g[e + 4]);
     }
   };
-  auto norm_of = [&](const float (&f)[8]) {
-    float s = 0.0f;
+  auto each = [&](int from, int to, auto&& row_of) {
+#pragma unroll 1
+    for (int r = from; r < to; ++r) {
+      cp_async_wait<kRing - 2>();
+      const uint4 x = slots[16 * (r & (kRing - 1))];
+      fetch();                            // where the row before was
+      row_of(x);
+    }
+  };
+  auto norm_of = [&](const F2 (&f)[4]) {
+    F2 s2 = f2_mul(f[0], f[0]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = __fmaf_rn(f[e], f[e], s);
+    for (int e = 1; e < 4; ++e) s2 = f2_fma(f[e], f[e], s2);
+    float s, s1;
+    f2_split(s2, s, s1);
+    s += s1;
 #pragma unroll
     for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-    return rsqrtf(__fmaf_rn(s, 1.0f / kD, p.eps));
+    s = __fmaf_rn(s, 1.0f / kD, p.eps);
+    const float r = rsqrtf(s);
+    return r * __fmaf_rn(-0.5f * s * r, r, 1.5f);
   };
-  auto partners = [&](const uint4& x, const float (&f)[8], float (&o)[8]) {
-    if (p.inter) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = f[e ^ 1];
+  // normed and turned row
+  auto turned_row = [&](const uint4& x, bool norm, F2 (&y)[4]) {
+    F2 f[4], o[4];
+    unpack_pairs<DT>(x, f);
+    if (p.inter) {                        // partners e ^ 1: the halves of the words
+      unpack_pairs<DT>(make_uint4(prmt(x.x, 0, 0x1032u), prmt(x.y, 0, 0x1032u), prmt(x.z, 0, 0x1032u), prmt(x.w, 0, 0x1032u)), o);
     } else {
       uint4 w;
       w.x = __shfl_sync(0xffffffffu, x.x, partner);
       w.y = __shfl_sync(0xffffffffu, x.y, partner);
       w.z = __shfl_sync(0xffffffffu, x.z, partner);
       w.w = __shfl_sync(0xffffffffu, x.w, partner);
-      Vec16<DT>::unpack(w, o);
+      unpack_pairs<DT>(w, o);
     }
-  };
-  auto row_ptr = [&](void* base, const int64_t (&st)[2], int h) {
-    return reinterpret_cast<uint4*>(static_cast<char*>(base) + 2 * (tok * st[0] + h * st[1] + d0));
-  };
-  auto put = [&](uint8_t* codes, __half* scales, int h, uint32_t word, __half sc) {
-    if (!fits) return;
-    uint8_t* row = codes + pid * p.pg.cp + h * p.pg.ch + place * kRowB;
-    *reinterpret_cast<uint32_t*>(row + word_at(place, l >> 2, l & 3)) = word;
-    if ((l & 3) == 0) scales[pid * p.pg.sp + h * p.pg.sh + place * 4 + (l >> 2)] = sc;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = f2_fma(f[e], cs[e], f2_mul(o[e], sg[e]));
+    if (norm) {
+      const float r = norm_of(f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = f2_mul(y[e], f2_make(r, r));
+    }
   };
 
-  if (r0 < p.Hq) factors(p.qw);
-  each(p.q, p.qs, r0, min(r1, p.Hq), [&](int h, const uint4& x) {
-    float f[8], o[8];
-    Vec16<DT>::unpack(x, f);
-    partners(x, f, o);
-    const float r = p.qw ? norm_of(f) : 1.0f;
-    uint4 w = x;
-    if (live) {
-      float y[8];
+  if (r0 < p.Hq) {
+    factors(p.qw);
+    char* to = static_cast<char*>(p.q_out) + 2 * (tok * p.qos[0] + r0 * p.qos[1] + d0);
+    const bool store = live || (here && p.copy_rest);
+    each(r0, min(r1, p.Hq), [&](const uint4& x) {
+      F2 y[4];
+      turned_row(x, p.qw, y);
+      const uint4 w = live ? pack_row<DT>(y) : x;
+      if (store) *reinterpret_cast<uint4*>(to) = w;
+      to += 2 * p.qos[1];
+    });
+  }
+  // a lane's word and its group's scale in a head's page
+  const int64_t code_at = pid * p.pg.cp + place * kRowB + word_at(place, l >> 2, l & 3);
+  const int64_t scale_at = pid * p.pg.sp + place * 4 + (l >> 2);
+  if (r1 > p.Hq && r0 < p.Hq + p.Hkv) {
+    factors(p.kw);
+    const int h0 = max(r0 - p.Hq, 0);
+    uint8_t* codes = p.pg.k + code_at + h0 * p.pg.ch;
+    __half* scales = p.pg.ksc + scale_at + h0 * p.pg.sh;
+    char* to = static_cast<char*>(p.k_out) + 2 * (tok * p.kos[0] + h0 * p.kos[1] + d0);
+    int h = h0;
+    each(p.Hq + h0, min(r1, p.Hq + p.Hkv), [&](const uint4& x) {
+      F2 y[4], k[4];
+      turned_row(x, p.kw, y);
+      float a = absmax(y);
+      a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
+      a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+      const float a75 = over75(a);
+      const __half sc = group_scale(a75);
+      const float s = __half2float(sc), rs = s > 0.0f ? rcp(s) : 0.0f;
+      bool near = false;
+      if (!plain_k) {
+        // |x w| + |o w_o| is at most twice the larger of the pair's turned values
+        const float err = 2.0f * kSlack * fmaxf(a, p.inter ? a : __shfl_sync(0xffffffffu, a, partner));
+        const float e75 = __fmaf_rn(err, 0.13333334f, a75 * 1.2e-7f);
+        // the scale is the same for all a75 that this one may stand for
+        near = a75 < INFINITY && __half_as_ushort(group_scale(a75 + e75)) != __half_as_ushort(group_scale(fmaxf(a75 - e75, 0.0f)));
+        const F2 r2 = f2_make(rs, rs), big = f2_make(12582912.0f, 12582912.0f);  // 1.5 x 2^23
+        float far = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = r * __fmaf_rn(f[e], cs[e], o[e] * sg[e]);
-      w = make_uint4(pack16<DT>(y[0], y[1]), pack16<DT>(y[2], y[3]), pack16<DT>(y[4], y[5]), pack16<DT>(y[6], y[7]));
-    }
-    if (live || (here && p.copy_rest)) *row_ptr(p.q_out, p.qos, h) = w;
-  });
-  const bool plain_k = !p.kw && p.rot == 0;  // k is coded as it came: no rounding before the codes
-  if (r1 > p.Hq && r0 < p.Hq + p.Hkv) factors(p.kw);
-  each(p.k, p.ks, max(r0 - p.Hq, 0), min(r1 - p.Hq, p.Hkv), [&](int h, const uint4& x) {
-    float f[8], o[8], y[8], t[8];
-    Vec16<DT>::unpack(x, f);
-    partners(x, f, o);
-    const float r = p.kw ? norm_of(f) : 1.0f;
-    float a = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      y[e] = r * __fmaf_rn(f[e], cs[e], o[e] * sg[e]);
-      a = max_nan(a, fabsf(y[e]));
-    }
-    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
-    const float a75 = __fdiv_rn(a, 7.5f);
-    __half sc = group_scale(a75);
-    const float s = __half2float(sc);
-    const float rs = s > 0.0f ? __frcp_rn(s) : 0.0f;
-    bool near = false;
-    if (!plain_k) {
-      // the largest |x w| + |o w_o| of the group at most, for the errors of all its channels
-      float size = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) size = fmaxf(size, fabsf(f[e]) + fabsf(o[e]));
-      size *= wmax;
-      size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, 1));
-      size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, 2));
-      const float err = size * r * p.slack, e75 = err * 0.13333334f + a75 * 6.0e-8f;
-      // the scale's neighbours in float16 are the same for all a it may come from
-      near = a75 < INFINITY && __half_as_ushort(group_scale(a75 + e75)) != __half_as_ushort(group_scale(fmaxf(a75 - e75, 0.0f)));
-      const float et = __fmaf_rn(err, rs, 2.5e-6f);  // (8 * 2^-22 of the quotient's own roundings)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        t[e] = y[e] * rs;
-        const float d = fabsf(t[e] - rintf(t[e]));
-        near |= d + et > 0.5f && fabsf(t[e]) < 8.6f;
+        for (int e = 0; e < 4; ++e) {
+          const F2 t = f2_mul(y[e], r2);
+          k[e] = f2_sub(f2_add(t, big), big);
+          float d0, d1;
+          f2_split(f2_sub(t, k[e]), d0, d1);
+          far = fmaxf(far, fmaxf(fabsf(d0), fabsf(d1)));
+        }
+        near |= far + __fmaf_rn(err, rs, 4e-6f) > 0.5f;  // (8 x 2^-21 of the quotient's own roundings)
+      } else {
+        quotients(y, s, rs, k);
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float q0 = y[e] * rs;
-        t[e] = __fmaf_rn(__fmaf_rn(-q0, s, y[e]), rs, q0);
+      const uint32_t word = pack_codes(k);
+      if (live) {
+        if (__any_sync(mask, near && fits) && l == 0) again[atomicAdd(&n_again, 1)] = static_cast<uint32_t>(sub << 16 | h);
+        if (fits) {
+          *reinterpret_cast<uint32_t*>(codes) = word;
+          if ((l & 3) == 0) *scales = sc;
+        }
+        if (p.k_out) *reinterpret_cast<uint4*>(to) = pack_row<DT>(y);
       }
-    }
-    uint32_t word = pack_codes(t);
-    if (live) {
-      if (__any_sync(mask, near)) {
-        const Exact ex = exact_row<DT>(p, x, mask, partner, pos, l);
-        word = ex.word;
-        sc = ex.scale;
+      codes += p.pg.ch;
+      scales += p.pg.sh;
+      to += 2 * p.kos[1];
+      ++h;
+    });
+  }
+  if (r1 > p.Hq + p.Hkv) {
+    const int h0 = max(r0 - p.Hq - p.Hkv, 0);
+    uint8_t* codes = p.pg.v + code_at + h0 * p.pg.ch;
+    __half* scales = p.pg.vsc + scale_at + h0 * p.pg.sh;
+    each(p.Hq + p.Hkv + h0, r1, [&](const uint4& x) {
+      F2 f[4], k[4];
+      unpack_pairs<DT>(x, f);
+      float a = absmax(f);
+      a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
+      a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+      const __half sc = group_scale(over75(a));
+      const float s = __half2float(sc);
+      quotients(f, s, s > 0.0f ? rcp(s) : 0.0f, k);
+      const uint32_t word = pack_codes(k);
+      if (fits) {
+        *reinterpret_cast<uint32_t*>(codes) = word;
+        if ((l & 3) == 0) *scales = sc;
       }
-      put(p.pg.k, p.pg.ksc, h, word, sc);
-      if (p.k_out)
-        *row_ptr(p.k_out, p.kos, h) = make_uint4(pack16<DT>(y[0], y[1]), pack16<DT>(y[2], y[3]),
-                                                 pack16<DT>(y[4], y[5]), pack16<DT>(y[6], y[7]));
-    }
-  });
-  each(p.v, p.vs, max(r0 - p.Hq - p.Hkv, 0), r1 - p.Hq - p.Hkv, [&](int h, const uint4& x) {
-    float f[8], t[8];
-    Vec16<DT>::unpack(x, f);
-    float a = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) a = max_nan(a, fabsf(f[e]));
-    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
-    const __half sc = group_scale(__fdiv_rn(a, 7.5f));
-    const float s = __half2float(sc), rs = s > 0.0f ? __frcp_rn(s) : 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float q0 = f[e] * rs;
-      t[e] = __fmaf_rn(__fmaf_rn(-q0, s, f[e]), rs, q0);
-    }
-    put(p.pg.v, p.pg.vsc, h, pack_codes(t), sc);
-  });
+      codes += p.pg.ch;
+      scales += p.pg.sh;
+    });
+  }
+  // ---- rows whose codes float32 could not tell
+  if (plain_k || r1 <= p.Hq || r0 >= p.Hq + p.Hkv) return;
+  __syncthreads();
+  for (int i = sub; i < n_again; i += kTok) {
+    const int of = again[i] >> 16, h = again[i] & 0xffff;
+    const int4 w = where[of];             // token, page, place
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.k) + 2 * (w.x * p.ks[0] + h * p.ks[1] + d0));
+    const Exact ex = exact_row<DT>(p, x, mask, partner, turn[of], l);
+    *reinterpret_cast<uint32_t*>(p.pg.k + w.y * p.pg.cp + h * p.pg.ch + w.z * kRowB + word_at(w.z, l >> 2, l & 3)) = ex.word;
+    if ((l & 3) == 0) p.pg.ksc[w.y * p.pg.sp + h * p.pg.sh + w.z * 4 + (l >> 2)] = ex.scale;
+  }
 }
 
 template <int DT>
 int launch_append(AppendParams p, cudaStream_t st) {
   const int rows = p.Hq + 2 * p.Hkv;
   const int64_t blocks = (static_cast<int64_t>(p.T) + kTok - 1) / kTok;
-  // a token's rows stay together (its cos and sin made once) as long as that leaves 4 blocks of 4
+  // a token's rows stay together (its cos and sin made once) as long as that leaves 8 blocks of 4
   // warps an SM; below, they are split, down to one row each
-  const int64_t want = std::max<int64_t>(1, 4LL * current_sm_count() / blocks);
+  const int64_t want = std::max<int64_t>(1, 8LL * current_sm_count() / blocks);
   const int groups = static_cast<int>(std::min<int64_t>(rows, want));
   p.rows_per_block = (rows + groups - 1) / groups;
   p.groups = (rows + p.rows_per_block - 1) / p.rows_per_block;
   if (blocks * p.groups > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
-  append_kernel<DT><<<static_cast<unsigned>(blocks * p.groups), kThreads, 0, st>>>(p);
+  const int list = kTok * std::min(p.rows_per_block, p.Hkv) * 4;  // a block's k rows
+  if (list > 16384) return HQ_ERR_UNSUPPORTED;
+  append_kernel<DT><<<static_cast<unsigned>(blocks * p.groups), kThreads, list, st>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? HQ_OK : static_cast<int>(e);
 }
@@ -407,6 +504,7 @@ extern "C" int hq_paged4_append(const void* q, const void* k_new, const void* v_
   if (!q || !k_new || !v_new || !q_out || !lens) return HQ_ERR_INVALID_ARGUMENT;
   auto al = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
   if (!al(q) || !al(k_new) || !al(v_new) || !al(q_out) || !al(k_out)) return HQ_ERR_INVALID_ARGUMENT;
+  if (k_out == k_new) return HQ_ERR_INVALID_ARGUMENT;  // (rows of k are read a second time)
   const int64_t* all[5] = {q_strides, k_strides, v_strides, qo_strides, k_out ? ko_strides : qo_strides};
   for (const int64_t* s : all)
     if (s[0] % 8 || s[1] % 8) return HQ_ERR_INVALID_ARGUMENT;
@@ -446,7 +544,6 @@ extern "C" int hq_paged4_append(const void* q, const void* k_new, const void* v_
   p.k_out = k_out;
   p.copy_rest = copy_rest;
   p.status = status;
-  p.slack = p4::kSlack * fmaxf(1.0f, fabsf(factor));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return x_dtype == HQ_DTYPE_BF16 ? p4::launch_append<HQ_DTYPE_BF16>(p, st) : p4::launch_append<HQ_DTYPE_F16>(p, st);
 }

@@ -1605,8 +1605,8 @@ def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None
     rotated values, codes and scales those of exact arithmetic; V as it came.
 
     Returns the new q (``q_out``, which may be q; rows behind the last sequence stay what they were
-    there, or are q's in a result made by this call); ``k_out [T,Hkv,128]`` takes the new k, for the
-    prompt's own attention.  K and V of real tokens are finite (others spoil their group).  A
+    there, or are q's in a result made by this call); ``k_out [T,Hkv,128]`` (memory of its own) takes the
+    new k, for the prompt's own attention.  K and V of real tokens are finite (others spoil their group).  A
     sequence whose tokens do not fit its table, and a token whose page is no page of the cache, are
     not written and set ``ragged_status()``; no two new tokens may go to the same place.
     """
@@ -1691,6 +1691,8 @@ def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None
     if k_out is not None:
         _packed_out(what, "k_out", k_out, (T, Hkv, 128), q)
         kop, kost = k_out.data_ptr(), _lib.strides(k_out.stride()[:2], 2)
+        if T and kop == kp:
+            raise ValueError(f"{what}: k_out must not be k_new")
     if T == 0:
         return q_out
     if B == 0:

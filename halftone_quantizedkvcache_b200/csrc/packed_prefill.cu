@@ -34,24 +34,30 @@ using namespace tc;
 
 constexpr int kD = 128;
 constexpr int kBN = 128;                  // keys per tile
-constexpr int kRows = 256;                // rows per block: two tiles
-constexpr int kThreads = 384;
-constexpr int kSoft = 256;
-constexpr int kSoftRegs = 208, kOtherRegs = 88;
-constexpr int kStages = 4;                // K, V, K, V, ..
 constexpr int kTileB = kBN * kD * 2;
-constexpr int kOffKv = 2 * kTileB;        // behind the two Q tiles
-constexpr int kOffBar = kOffKv + kStages * kTileB;
-// barriers
-constexpr int kFull = 0, kEmpty = kFull + kStages, kSFull = kEmpty + kStages, kPFull = kSFull + 2,
-              kOFull = kPFull + 4, kClean = kOFull + 2, kDrain = kClean + 2, kBars = kDrain + 1;
-constexpr int kOffBad = kOffBar + kBars * 8;       // [2][4] words of spoiled V rows
-constexpr int kOffMisc = kOffBad + 32;
-constexpr int kSmem = 1024 + kOffMisc + 32;
 constexpr int kPartRow = kD + 4;
-constexpr uint32_t kColO = 256;           // tensor memory: S tiles at 0 and 128, O at 256 and 384
 constexpr int kCleanWarps = 2;
 constexpr int kMaxSplit = 16;
+
+// A block's row tiles: two, one block per SM; or one, two blocks per SM (short sequences and small
+// calls, where a block's start and end count).
+template <int NT>
+struct Cfg {
+  static constexpr int kRows = 128 * NT;
+  static constexpr int kSoft = 128 * NT, kThreads = kSoft + 128;
+  // registers a thread after the split (softmax warps, the others) of 168 or 128 at launch
+  static constexpr int kSoftRegs = NT == 2 ? 208 : 176, kOtherRegs = NT == 2 ? 88 : 80;
+  static constexpr int kStages = 2 * NT;                // K, V, ..
+  static constexpr int kOffKv = NT * kTileB;            // behind the Q tiles
+  static constexpr int kOffBar = kOffKv + kStages * kTileB;
+  static constexpr int kFull = 0, kEmpty = kFull + kStages, kSFull = kEmpty + kStages, kPFull = kSFull + NT,
+                       kOFull = kPFull + 2 * NT, kClean = kOFull + NT, kDrain = kClean + 2, kBars = kDrain + 1;
+  static constexpr int kOffBad = kOffBar + (kBars * 8 + 15) / 16 * 16;  // [2][4] words of spoiled V rows
+  static constexpr int kOffMisc = kOffBad + 32;
+  static constexpr int kSmem = 1024 + kOffMisc + 48;
+  static constexpr uint32_t kColO = 128 * NT;           // tensor memory: S tiles, then O tiles
+  static constexpr uint32_t kCols = 256 * NT;
+};
 
 struct Params {
   const void* q;
@@ -62,7 +68,7 @@ struct Params {
   int T, Tk, B, Hkv, nrep;
   int causal;
   float c;                                // sm_scale log2(e)
-  int n_split, units;                     // units: an upper bound of (sequence, 256 rows, kv head)
+  int n_split, units;                     // units: an upper bound of (sequence, piece of its rows, kv head)
   int swap;                               // tensor maps: (channel, token, head) instead of (channel, head, token)
   int zero_rest;
   float* part;
@@ -129,6 +135,28 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ldw32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31"
+      "}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_stw16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {"
+      "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16"
+      "};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_stw32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
@@ -170,21 +198,22 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   s.nk = min(max(p.cu_k[b + 1], s.k0), p.Tk) - s.k0;
   return s;
 }
-__device__ __forceinline__ int pairs_of(const Params& p, int b) {
-  const int q0 = min(max(p.cu_q[b], 0), p.T), q1 = min(max(p.cu_q[b + 1], q0), p.T);
-  return static_cast<int>((static_cast<int64_t>(q1 - q0) * p.nrep + kRows - 1) / kRows);
+__device__ __forceinline__ int blocks_of(const Params& p, int nq, int rows) {
+  return static_cast<int>((static_cast<int64_t>(nq) * p.nrep + rows - 1) / rows);
 }
-// All lanes of a warp: the sequence that holds pair u of the line of all pairs, and the pair's place in
-// it (b = B: behind the last).
-__device__ __forceinline__ void find_pair(const Params& p, int u, int& b, int& y) {
+// All lanes of a warp: the sequence that holds piece u of the line of all sequences' pieces of `rows`
+// rows (b = B: behind the last), and the piece's place in it.
+__device__ __forceinline__ void find_piece(const Params& p, int u, int rows, int& b, int& y, Seq& s) {
   const int lane = threadIdx.x & 31;
   int run = 0;
   b = p.B;
   y = 0;
 #pragma unroll 1
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int mine = b0 + lane < p.B ? pairs_of(p, b0 + lane) : 0;
-    int x = mine;
+    Seq mine{};
+    if (b0 + lane < p.B) mine = seq_of(p, b0 + lane);
+    const int n = blocks_of(p, mine.nq, rows);
+    int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int z = __shfl_up_sync(0xffffffffu, x, o);
@@ -194,7 +223,11 @@ __device__ __forceinline__ void find_pair(const Params& p, int u, int& b, int& y
     if (hit) {
       const int l = __ffs(hit) - 1;
       b = b0 + l;
-      y = u - run - __shfl_sync(0xffffffffu, x - mine, l);
+      y = u - run - __shfl_sync(0xffffffffu, x - n, l);
+      s.q0 = __shfl_sync(0xffffffffu, mine.q0, l);
+      s.nq = __shfl_sync(0xffffffffu, mine.nq, l);
+      s.k0 = __shfl_sync(0xffffffffu, mine.k0, l);
+      s.nk = __shfl_sync(0xffffffffu, mine.nk, l);
       return;
     }
     run += __shfl_sync(0xffffffffu, x, 31);
@@ -206,14 +239,16 @@ __device__ __forceinline__ int limit_of(const Params& p, const Seq& s, int r) {
   return p.causal ? min(max(s.nk - s.nq + i + 1, 0), s.nk) : s.nk;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int DT, int NT>
+__global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
     packed_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm) {
+  using C = Cfg<NT>;
+  constexpr int kRows = C::kRows, kThreads = C::kThreads, kStages = C::kStages, kSoftWarps = C::kSoft / 32;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kOffBar);
-  uint32_t* bad = reinterpret_cast<uint32_t*>(smem + kOffBad);
-  int* misc = reinterpret_cast<int*>(smem + kOffMisc);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint32_t* bad = reinterpret_cast<uint32_t*>(smem + C::kOffBad);
+  int* misc = reinterpret_cast<int*>(smem + C::kOffMisc);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -226,98 +261,128 @@ __global__ void __launch_bounds__(kThreads, 1)
             make_uint4(0, 0, 0, 0);
   }
   if (warp == 0) {
-    // heavy (last) pairs first
+    // heavy (last) pieces first
     const int item = p.units - 1 - static_cast<int>(blockIdx.x) / p.n_split;
     int b, y;
-    find_pair(p, item / p.Hkv, b, y);
+    Seq s{};
+    find_piece(p, item / p.Hkv, kRows, b, y, s);
     if (lane == 0) {
       misc[0] = b;
       misc[1] = y;
+      misc[2] = s.q0;
+      misc[3] = s.nq;
+      misc[4] = s.k0;
+      misc[5] = s.nk;
     }
   }
+  if (tid == 32) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bar[C::kFull + i], 1);
+      mbar_init(&bar[C::kEmpty + i], i & 1 ? 1 + kCleanWarps : 1);  // V stages: products, and the warps that look
+    }
+    for (int t = 0; t < NT; ++t) {
+      mbar_init(&bar[C::kSFull + t], 1);
+      mbar_init(&bar[C::kPFull + 2 * t], 4);
+      mbar_init(&bar[C::kPFull + 2 * t + 1], 4);
+      mbar_init(&bar[C::kOFull + t], 1);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&bar[C::kClean + i], kCleanWarps);
+    mbar_init(&bar[C::kDrain], 1);
+    fence_mbar_init();
+  }
   __syncthreads();
-  const int b = misc[0];
-  if (b >= p.B) {
+  if (misc[0] >= p.B) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
   const int split = static_cast<int>(blockIdx.x) % p.n_split, item = p.units - 1 - static_cast<int>(blockIdx.x) / p.n_split;
   const int kvh = item % p.Hkv;
-  const Seq s = seq_of(p, b);
+  const Seq s = {misc[2], misc[3], misc[4], misc[5]};
   const int row0 = misc[1] * kRows, rows = min(kRows, s.nq * p.nrep - row0);  // rows >= 1
   // key tiles of the two row tiles, and the block's share of them
-  int nt[2];
+  int nt[NT], all = 0;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < NT; ++t) {
     const int last = min(rows, 128 * (t + 1)) - 1;
     nt[t] = last >= 128 * t ? (limit_of(p, s, row0 + last) + kBN - 1) / kBN : 0;
+    all = max(all, nt[t]);
   }
-  const int all = max(nt[0], nt[1]);
   const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / p.n_split);
   const int j1 = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.n_split);
   // masked steps: those from jm on, past the keys that every row sees.  The two barriers that say that
   // their V is looked over take turns: each V stage has its own, which cannot run a phase ahead.
   const int jm = max(j0, limit_of(p, s, row0) / kBN);
-  auto clean_bar = [&](int j) { return &bar[kClean + (j & 1)]; };
+  auto clean_bar = [&](int j) { return &bar[C::kClean + (j & 1)]; };
   auto clean_phase = [&](int j) { return static_cast<uint32_t>((j - jm) >> 1) & 1u; };
   const uint32_t base = smem_u32(smem);
 
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&misc[4])), "r"(512));
+  if (warp == kSoftWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&misc[8])), "r"(C::kCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&bar[kFull + i], 1);
-      mbar_init(&bar[kEmpty + i], i & 1 ? 1 + kCleanWarps : 1);  // V stages: products, and the warps that look
-    }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&bar[kSFull + t], 1);
-      mbar_init(&bar[kPFull + 2 * t], 4);
-      mbar_init(&bar[kPFull + 2 * t + 1], 4);
-      mbar_init(&bar[kOFull + t], 1);
-    }
-    for (int i = 0; i < 2; ++i) mbar_init(&bar[kClean + i], kCleanWarps);
-    mbar_init(&bar[kDrain], 1);
-    fence_mbar_init();
-  }
+  // K and V tiles, in turn
+  const int copies = 2 * (j1 - j0);
+  auto copy = [&](int n) {
+    const int st = n % kStages;
+    unsigned char* to = smem + C::kOffKv + st * kTileB;
+    const CUtensorMap* map = n & 1 ? &vm : &km;
+    const int key = s.k0 + (j0 + (n >> 1)) * kBN;
+    mbar_arrive_expect_tx(&bar[C::kFull + st], kTileB);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      asm volatile(
+          "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+              smem_u32(to + h * (kBN * 128))),
+          "l"(reinterpret_cast<uint64_t>(map)), "r"(64 * h), "r"(p.swap ? key : kvh), "r"(p.swap ? kvh : key),
+          "r"(smem_u32(&bar[C::kFull + st]))
+          : "memory");
+  };
+  if (warp == kSoftWarps + 1 && lane == 0)
+    for (int n = 0; n < min(copies, kStages); ++n) copy(n);
   // Q, 16 lanes a row: K-major tiles of two 64-channel halves, 128-byte swizzle; rows past the last: zeros
-  for (int x = tid; x < kRows * 16; x += kThreads) {
-    const int r = x >> 4, c = x & 15;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < rows) {
-      const int i = static_cast<uint32_t>(row0 + r) / static_cast<uint32_t>(p.nrep), h = kvh * p.nrep + row0 + r - i * p.nrep;
-      v = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + 2 * ((s.q0 + static_cast<int64_t>(i)) * p.qs[0] + h * p.qs[1] + 8 * c));
+  {
+    constexpr int kEach = (kRows * 16 + kThreads - 1) / kThreads;
+    uint4 v[kEach];
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {     // (all loads in flight at once)
+      const int r = (tid + n * kThreads) >> 4, c = tid & 15;
+      v[n] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int i = static_cast<uint32_t>(row0 + r) / static_cast<uint32_t>(p.nrep), h = kvh * p.nrep + row0 + r - i * p.nrep;
+        v[n] = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + 2 * ((s.q0 + static_cast<int64_t>(i)) * p.qs[0] + h * p.qs[1] + 8 * c));
+      }
     }
-    *reinterpret_cast<uint4*>(smem + (r >> 7) * kTileB + (c >> 3) * (kBN * 128) + sw128(r & 127, c & 7)) = v;
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+      const int r = (tid + n * kThreads) >> 4, c = tid & 15;
+      if (r < kRows) *reinterpret_cast<uint4*>(smem + (r >> 7) * kTileB + (c >> 3) * (kBN * 128) + sw128(r & 127, c & 7)) = v[n];
+    }
   }
   fence_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = static_cast<uint32_t>(misc[4]);
+  const uint32_t tmem = static_cast<uint32_t>(misc[8]);
   bool ok = true;
 
-  if (warp >= kSoft / 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp < kSoft / 32) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+  if (warp >= kSoftWarps) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+  if (warp < kSoftWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
     // ------------------------------------------------------------ softmax: a thread per row
     const int t = warp >> 2, r = 128 * t + 32 * (warp & 3) + lane;
     const int lim = limit_of(p, s, row0 + min(r, rows - 1));
     const uint32_t s_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + 128 * t;
-    const uint32_t o_addr = s_addr - 128 * t + kColO + 128 * t;
+    const uint32_t o_addr = s_addr - 128 * t + C::kColO + 128 * t;
     float m = -INFINITY, l = 0.0f;        // m: of the raw scores
     const int jt = min(j1, nt[t]);
 #pragma unroll 1
     for (int j = j0; j < jt; ++j) {
-      ok = wait_bar(&bar[kSFull + t], (j - j0) & 1);
+      ok = wait_bar(&bar[C::kSFull + t], (j - j0) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      uint32_t x[128];
-      tmem_ld128(s_addr, x);
       const int left = lim - j * kBN;     // keys of the tile that this row sees
-      bool spoiled = false;
+      bool spoiled = false, masked = false;
       if (j >= jm) {
         ok = wait_bar(clean_bar(j), clean_phase(j));
         ok = __all_sync(0xffffffffu, ok);
@@ -328,18 +393,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int n = min(max(left - 32 * i, 0), 32);
           spoiled |= (w[i] & (n == 32 ? 0xffffffffu : (1u << n) - 1u)) != 0;
         }
-        if (__any_sync(0xffffffffu, left < kBN)) {
+        masked = __any_sync(0xffffffffu, left < kBN);
+      }
+      // the row: all of it in registers, or (half as many of those a thread) 32 scores at a time, twice
+      constexpr int kHold = NT == 2 ? 128 : 32;
+      uint32_t x[kHold];
+      auto load = [&](int c) {
+        if constexpr (kHold == 128) tmem_ld128(s_addr, x);
+        else tmem_ldw32(s_addr + 32 * c, x);
+        if (masked) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i) x[i] = i < left ? x[i] : 0xff800000u;
+          for (int i = 0; i < kHold; ++i) x[i] = kHold * c + i < left ? x[i] : 0xff800000u;
         }
-      }
-      float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[1]);
+      };
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 2; i < 126; i += 4) {
-        m0 = max3(m0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-        m1 = max3(m1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+      for (int c = 0; c < 128 / kHold; ++c) {
+        load(c);
+        float m0 = fmaxf(top, __uint_as_float(x[0])), m1 = __uint_as_float(x[1]);
+#pragma unroll
+        for (int i = 2; i < kHold - 2; i += 4) {
+          m0 = max3(m0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          m1 = max3(m1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+        }
+        top = max3(fmaxf(m0, m1), __uint_as_float(x[kHold - 2]), __uint_as_float(x[kHold - 1]));
       }
-      const float top = max3(fmaxf(m0, m1), __uint_as_float(x[126]), __uint_as_float(x[127]));
       if (j == j0) {
         m = top;
       } else if (__any_sync(0xffffffffu, (top - m) * p.c > 8.0f || (m == -INFINITY && top > m))) {
@@ -361,25 +439,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float mc = m == -INFINITY ? 0.0f : m * p.c;
       const F2 c2 = f2_make(p.c, p.c), n2 = f2_make(-mc, -mc);
       F2 sum = f2_make(0.0f, 0.0f), sum1 = sum;
+      // 2 n scores from x[at] on as weights of the model's type
+      auto weights = [&](int at, int n, uint32_t* w) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          F2 z = f2_fma(f2_make(__uint_as_float(x[64 * h + 2 * i]), __uint_as_float(x[64 * h + 2 * i + 1])), c2, n2);
+        for (int i = 0; i < n; ++i) {
           float a, e;
-          f2_split(z, a, e);
+          f2_split(f2_fma(f2_make(__uint_as_float(x[at + 2 * i]), __uint_as_float(x[at + 2 * i + 1])), c2, n2), a, e);
           a = ex2_ftz(a);
           e = ex2_ftz(e);
           if (i & 1) sum = f2_add(sum, f2_make(a, e));
           else sum1 = f2_add(sum1, f2_make(a, e));
           w[i] = pack2<DT>(a, e);
         }
-        tmem_stw32(s_addr + 32 * h, w);
+      };
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (kHold == 128) {
+          uint32_t w[32];
+          weights(64 * h, 32, w);
+          tmem_stw32(s_addr + 32 * h, w);
+        } else {
+#pragma unroll
+          for (int c = 2 * h; c < 2 * h + 2; ++c) {
+            load(c);
+            uint32_t w[16];
+            weights(0, 16, w);
+            tmem_stw16(s_addr + 16 * c, w);
+          }
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar[kPFull + 2 * t + h]);
+        if (lane == 0) mbar_arrive(&bar[C::kPFull + 2 * t + h]);
       }
       float a, e;
       f2_split(f2_add(sum, sum1), a, e);
@@ -388,19 +479,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // ---- the rows' results
     if (ok && jt > j0) {
-      ok = wait_bar(&bar[kOFull + t], 0);
+      ok = wait_bar(&bar[C::kOFull + t], 0);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
     if (ok && 128 * t + 32 * (warp & 3) < rows) {
-      const bool live = r < rows, has = jt > j0;
-      const int i = static_cast<uint32_t>(row0 + min(r, rows - 1)) / static_cast<uint32_t>(p.nrep);
-      const int h = kvh * p.nrep + row0 + min(r, rows - 1) - i * p.nrep;
-      const float inv = !has || l <= 0.0f ? 0.0f : 1.0f / l;  // (a NaN stays)
-      char* dst = static_cast<char*>(p.out) + 2 * ((s.q0 + static_cast<int64_t>(i)) * p.os[0] + h * p.os[1]);
-      float* prt = p.part + ((static_cast<int64_t>(item) * p.n_split + split) * kRows + r) * kPartRow;
-      if (p.n_split > 1 && live)
-        *reinterpret_cast<float2*>(prt) = make_float2(has && m != -INFINITY ? m * p.c : -INFINITY, has ? l : 0.0f);
+      const bool live = r < rows, has = jt > j0 && !(l <= 0.0f);
+      const float inv = has ? 1.0f / l : 0.0f;  // (a NaN stays)
+      // a partial row's 4 channels c lie beside those of the other rows
+      float4* prt = reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(item) * p.n_split + split) * kRows * kPartRow);
+      if (p.n_split > 1 && live) prt[r] = make_float4(has && m != -INFINITY ? m * p.c : -INFINITY, has ? l : 0.0f, 0.0f, 0.0f);
+      // this tile's Q is read no more (its last product has been awaited): its rows' place
+      unsigned char* q_tile = smem + t * kTileB;
+      const int lr = r & 127;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         float o[32];
@@ -409,28 +500,40 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (live)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<float4*>(prt + 4 + 32 * c + 4 * e) =
+              prt[(1 + 8 * c + e) * kRows + r] =
                   has ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_float4(0, 0, 0, 0);
-        } else if (live) {
+        } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (has && !(l <= 0.0f))
+            if (has)
               w = make_uint4(pack2<DT>(o[8 * e] * inv, o[8 * e + 1] * inv), pack2<DT>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
                              pack2<DT>(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2<DT>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
-            *reinterpret_cast<uint4*>(dst + 64 * c + 16 * e) = w;
+            *reinterpret_cast<uint4*>(q_tile + lr * 256 + (((4 * c + e) ^ (lr & 7)) << 4)) = w;
           }
         }
       }
+      __syncwarp();
+      if (p.n_split == 1) {               // 16 lanes a row
+        const int c = lane & 15;
+#pragma unroll 4
+        for (int k = 0; k < 16; ++k) {
+          const int r2 = 32 * (warp & 3) + 2 * k + (lane >> 4), row = 128 * t + r2;
+          if (row >= rows) break;
+          const int i = static_cast<uint32_t>(row0 + row) / static_cast<uint32_t>(p.nrep), h = kvh * p.nrep + row0 + row - i * p.nrep;
+          *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + 2 * ((s.q0 + static_cast<int64_t>(i)) * p.os[0] + h * p.os[1] + 8 * c)) =
+              *reinterpret_cast<const uint4*>(q_tile + r2 * 256 + ((c ^ (r2 & 7)) << 4));
+        }
+      }
     }
-  } else if (warp == 8) {
+  } else if (warp == kSoftWarps) {
     // ------------------------------------------------------------ products
     const uint32_t lead = elect_one();
     constexpr uint32_t id_s = idesc<DT>(128, kBN, false), id_o = idesc<DT>(128, kD, true);
     constexpr uint32_t k_hi = sdesc(0, 16, 1024) >> 32, v_hi = sdesc(0, kBN * 128, 1024) >> 32;
     const uint32_t q_lo = static_cast<uint32_t>(sdesc(base, 16, 1024));
-    const uint32_t k_lo = static_cast<uint32_t>(sdesc(base + kOffKv, 16, 1024));
-    const uint32_t v_lo = static_cast<uint32_t>(sdesc(base + kOffKv, kBN * 128, 1024));
+    const uint32_t k_lo = static_cast<uint32_t>(sdesc(base + C::kOffKv, 16, 1024));
+    const uint32_t v_lo = static_cast<uint32_t>(sdesc(base + C::kOffKv, kBN * 128, 1024));
     auto score = [&](int t, int stage) {
       const uint32_t a = q_lo + (t * kTileB >> 4), k = k_lo + (stage * kTileB >> 4);
 #pragma unroll
@@ -438,92 +541,80 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t off = ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) >> 4;
         mma_ss(lead, tmem + 128 * t, a + off, k_hi, k + off, k_hi, id_s, kk > 0);
       }
-      commit(lead, &bar[kSFull + t]);
+      commit(lead, &bar[C::kSFull + t]);
     };
     if (j0 < j1) {
-      ok = wait_bar(&bar[kFull], 0);
+      ok = wait_bar(&bar[C::kFull], 0);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
           if (j0 < nt[t]) score(t, 0);
-        commit(lead, &bar[kEmpty]);
+        commit(lead, &bar[C::kEmpty]);
       }
     }
 #pragma unroll 1
     for (int j = j0; ok && j < j1; ++j) {
       const int n = j - j0, vi = 2 * n + 1, ki = 2 * n + 2;  // copies: V of this tile, K of the next
       const int vs = vi % kStages, ks = ki % kStages;
-      ok = wait_bar(&bar[kFull + vs], (vi / kStages) & 1);
+      ok = wait_bar(&bar[C::kFull + vs], (vi / kStages) & 1);
       if (j >= jm) ok = ok && wait_bar(clean_bar(j), clean_phase(j));
-      if (j + 1 < j1) ok = ok && wait_bar(&bar[kFull + ks], (ki / kStages) & 1);
+      if (j + 1 < j1) ok = ok && wait_bar(&bar[C::kFull + ks], (ki / kStages) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < NT; ++t) {
         if (j >= nt[t]) continue;
         const uint32_t v = v_lo + (vs * kTileB >> 4);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          ok = ok && wait_bar(&bar[kPFull + 2 * t + h], n & 1);
+          ok = ok && wait_bar(&bar[C::kPFull + 2 * t + h], n & 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-            mma_ts(lead, tmem + kColO + 128 * t, tmem + 128 * t + 8 * kk, v + (kk * 16 * 128 >> 4), v_hi, id_o, n > 0 || kk > 0);
+            mma_ts(lead, tmem + C::kColO + 128 * t, tmem + 128 * t + 8 * kk, v + (kk * 16 * 128 >> 4), v_hi, id_o, n > 0 || kk > 0);
         }
         if (!ok) break;
         if (j + 1 < min(j1, nt[t])) score(t, ks);
-        else commit(lead, &bar[kOFull + t]);
+        else commit(lead, &bar[C::kOFull + t]);
       }
       if (!ok) break;
-      commit(lead, &bar[kEmpty + vs]);
-      if (j + 1 < j1) commit(lead, &bar[kEmpty + ks]);
+      commit(lead, &bar[C::kEmpty + vs]);
+      if (j + 1 < j1) commit(lead, &bar[C::kEmpty + ks]);
     }
     // no product is in flight when the block ends
-    commit(lead, &bar[kDrain]);
-    if (!wait_bar(&bar[kDrain], 0)) ok = false;
-  } else if (warp == 9) {
+    commit(lead, &bar[C::kDrain]);
+    if (!wait_bar(&bar[C::kDrain], 0)) ok = false;
+  } else if (warp == kSoftWarps + 1) {
     // ------------------------------------------------------------ copies
-    const int copies = 2 * (j1 - j0);
-    int n = 0;
+    int n = min(copies, kStages);
     if (lane == 0) {
       for (; n < copies; ++n) {
         const int st = n % kStages;
-        if (n >= kStages && !(ok = wait_bar(&bar[kEmpty + st], (n / kStages - 1) & 1))) break;
-        unsigned char* to = smem + kOffKv + st * kTileB;
-        const CUtensorMap* map = n & 1 ? &vm : &km;
-        const int key = s.k0 + (j0 + (n >> 1)) * kBN;
-        mbar_arrive_expect_tx(&bar[kFull + st], kTileB);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          asm volatile(
-              "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-                  smem_u32(to + h * (kBN * 128))),
-              "l"(reinterpret_cast<uint64_t>(map)), "r"(64 * h), "r"(p.swap ? key : kvh), "r"(p.swap ? kvh : key),
-              "r"(smem_u32(&bar[kFull + st]))
-              : "memory");
+        if (!(ok = wait_bar(&bar[C::kEmpty + st], (n / kStages - 1) & 1))) break;
+        copy(n);
       }
       if (!ok)  // no copy is in flight when the block ends
-        for (int i = max(0, n - kStages); i < n; ++i) wait_bar(&bar[kFull + i % kStages], (i / kStages) & 1);
+        for (int i = max(0, n - kStages); i < n; ++i) wait_bar(&bar[C::kFull + i % kStages], (i / kStages) & 1);
     }
     ok = __all_sync(0xffffffffu, ok);
   } else {
     // ------------------------------------------------------------ V rows that hold no numbers, on masked steps
-    const int g = warp - 10;
+    const int g = warp - kSoftWarps - 2;
     constexpr uint32_t mask = DT == HQ_DTYPE_BF16 ? 0x7f807f80u : 0x7c007c00u, one = DT == HQ_DTYPE_BF16 ? 0x00800080u : 0x04000400u;
 #pragma unroll 1
     for (int j = j0; j < j1; ++j) {
       const int vi = 2 * (j - j0) + 1, vs = vi % kStages;
-      ok = wait_bar(&bar[kFull + vs], (vi / kStages) & 1);
+      ok = wait_bar(&bar[C::kFull + vs], (vi / kStages) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (j < jm) {  // (every phase is waited for: a parity says nothing of phases further back)
-        if (lane == 0) mbar_arrive(&bar[kEmpty + vs]);
+        if (lane == 0) mbar_arrive(&bar[C::kEmpty + vs]);
         continue;
       }
-      unsigned char* v = smem + kOffKv + vs * kTileB;
+      unsigned char* v = smem + C::kOffKv + vs * kTileB;
 #pragma unroll 1
       for (int q = 0; q < 2; ++q) {
         const int row = 64 * g + 32 * q + lane;
@@ -544,79 +635,101 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(clean_bar(j));
-        mbar_arrive(&bar[kEmpty + vs]);
+        mbar_arrive(&bar[C::kEmpty + vs]);
       }
     }
   }
   if (!ok && lane == 0) report_error(p.status, HQ_ERR_DEVICE_TIMEOUT);
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kSoftWarps) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kCols));
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// A warp per output row (token, q head) joins the pieces of its pair, in order; a lane 4 channels.
-template <int DT>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p) {
+// Joins the pieces of a row tile, in order: block (piece of the line and kv head, 32 rows, 16 channels), a
+// warp 8 rows, 4 lanes a row, 4 channels each: one round of loads.
+template <int DT, int MOST>  // MOST: pieces at most (16 held the small calls up for 10 us)
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p, int rows) {
+  __shared__ int found[6];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, heads = p.Hkv * p.nrep;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (at >= static_cast<int64_t>(p.T) * heads) return;
-  const int tok = static_cast<int>(at / heads), h = static_cast<int>(at - static_cast<int64_t>(tok) * heads);
-  const int kvh = h / p.nrep;
-  // the token's sequence, and the pairs before it
-  int pairs = 0, b = -1;
-#pragma unroll 1
-  for (int b0 = 0; b < 0 && b0 < p.B; b0 += 32) {
-    const int e = b0 + lane;
-    const bool holds = e < p.B && seq_of(p, e).q0 <= tok && tok < seq_of(p, e).q0 + seq_of(p, e).nq;
-    const unsigned hit = __ballot_sync(0xffffffffu, holds);
-    const int l = hit ? __ffs(hit) - 1 : 32;
-    pairs += __reduce_add_sync(0xffffffffu, e < p.B && lane < l ? pairs_of(p, e) : 0);
-    if (hit) b = b0 + l;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int item = blockIdx.x, kvh = item % p.Hkv;
+  if (warp == 0) {
+    int b, y;
+    Seq s{};
+    find_piece(p, item / p.Hkv, rows, b, y, s);
+    if (lane == 0) {
+      found[0] = b;
+      found[1] = y;
+      found[2] = s.q0;
+      found[3] = s.nq;
+    }
   }
-  if (b < 0) return;
-  const int r = (tok - seq_of(p, b).q0) * p.nrep + h - kvh * p.nrep;
-  const int64_t item = static_cast<int64_t>(pairs + r / kRows) * p.Hkv + kvh;
-  if (item >= p.units) return;
-  const float* x = p.part + (item * p.n_split * kRows + r % kRows) * kPartRow;
-  float M = -INFINITY, L = 0.0f;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int i = 0; i < p.n_split; ++i, x += kRows * kPartRow) {
-    const float2 ml = *reinterpret_cast<const float2*>(x);
-    const float4 o = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
+  __syncthreads();
+  const int r = 32 * blockIdx.y + 8 * warp + (lane >> 2), row = found[1] * rows + r, cg = lane & 3;
+  if (found[0] >= p.B || row >= found[3] * p.nrep) return;
+  const float4* x = reinterpret_cast<const float4*>(p.part) + static_cast<int64_t>(item) * p.n_split * rows * (kPartRow / 4) + r;
+  const int64_t step = static_cast<int64_t>(rows) * (kPartRow / 4);
+  float f[MOST], l[MOST], M = -INFINITY, L = 0.0f;
+  float4 o[MOST];
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    const float4 ml = i < p.n_split ? x[i * step] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    f[i] = ml.x;
+    l[i] = ml.y;
+    if (i < p.n_split) o[i] = x[i * step + static_cast<int64_t>(1 + 4 * blockIdx.z + cg) * rows];
+  }
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) M = fmaxf(M, f[i]);
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    f[i] = f[i] == -INFINITY ? 0.0f : exp2f(f[i] - M);
     // (a piece whose sums are no number has a maximum of -inf and passes them on)
-    const float top = fmaxf(M, ml.x), f0 = M == -INFINITY ? 0.0f : exp2f(M - top), f1 = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
-    M = top;
-    L = L * f0 + ml.y * f1;
-    acc.x = acc.x * f0 + o.x * f1;
-    acc.y = acc.y * f0 + o.y * f1;
-    acc.z = acc.z * f0 + o.z * f1;
-    acc.w = acc.w * f0 + o.w * f1;
+    L = __fmaf_rn(l[i], f[i], L);
   }
   const float inv = L <= 0.0f ? 0.0f : 1.0f / L;
-  *reinterpret_cast<uint2*>(static_cast<char*>(p.out) + 2 * (tok * p.os[0] + h * p.os[1] + 4 * lane)) =
-      make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
+  const int i = static_cast<uint32_t>(row) / static_cast<uint32_t>(p.nrep), h = kvh * p.nrep + row - i * p.nrep;
+  char* dst = static_cast<char*>(p.out) + 2 * ((found[2] + static_cast<int64_t>(i)) * p.os[0] + h * p.os[1]);
+  const int c = 4 * blockIdx.z + cg;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int k = 0; k < MOST; ++k)
+    if (k < p.n_split) {
+      acc.x = __fmaf_rn(o[k].x, f[k], acc.x);
+      acc.y = __fmaf_rn(o[k].y, f[k], acc.y);
+      acc.z = __fmaf_rn(o[k].z, f[k], acc.z);
+      acc.w = __fmaf_rn(o[k].w, f[k], acc.w);
+    }
+  *reinterpret_cast<uint2*>(dst + 8 * c) = make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
 }
 
 // ---------------------------------------------------------------- host
 struct Plan {
-  int units, n_split;
+  int nt, units, n_split;
   size_t bytes;
 };
 inline bool plan(Plan& pl, int64_t T, int64_t Tk, int B, int Hkv, int nrep) {
-  const int64_t units = ((T * nrep + kRows - 1) / kRows + B) * Hkv;
-  if (units * kMaxSplit > 0x7fffffff || T * nrep > 0x3fffffff || Tk > 0x3fffffff) return false;
-  // With fewer blocks than SMs each row pair's keys go to several, down to two key tiles a block.
-  const int64_t tiles = std::max<int64_t>(1, Tk / kBN);
-  pl.n_split = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, current_sm_count() / std::max<int64_t>(units, 1)),
-                                                   std::max<int64_t>(1, tiles / 2), kMaxSplit}));
+  if (T * nrep > 0x3fffffff || Tk > 0x3fffffff) return false;
+  const int sms = current_sm_count();
+  // One row tile a block where sequences are short, in rows and in keys: 64 sequences of up to 200
+  // tokens 52 us against 60, one of 512 16.4 against 17.2; with more of either, K and V are better
+  // shared: one of 2048 39 us against 40, 2 x 8192 467 against 529, 3 x 77 queries over 4022 keys 22
+  // against 25.
+  pl.nt = T * nrep <= 1024LL * B && Tk <= 1024LL * B ? 1 : 2;
+  const int rows = 128 * pl.nt;
+  const int64_t units = ((T * nrep + rows - 1) / rows + B) * Hkv;
+  if (units * kMaxSplit > 0x7fffffff) return false;
+  // With fewer blocks than fit the GPU each piece's keys go to several, down to 4 key tiles of an average
+  // sequence a block (3 x 77 queries over 4022 keys: 57 us unsplit, 22 split; one of 512: 16.4 unsplit,
+  // 17.2 in two).
+  const int64_t room = (3 - pl.nt) * sms;
+  pl.n_split = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, room / std::max<int64_t>(units, 1)),
+                                                   std::max<int64_t>(1, Tk / (4 * kBN * std::max<int64_t>(B, 1))), kMaxSplit}));
   pl.units = static_cast<int>(units);
-  pl.bytes = pl.n_split > 1 ? sizeof(float) * static_cast<size_t>(units) * pl.n_split * kRows * kPartRow : 0;
+  pl.bytes = pl.n_split > 1 ? sizeof(float) * static_cast<size_t>(units) * pl.n_split * rows * kPartRow : 0;
   return true;
 }
 
@@ -635,29 +748,31 @@ inline int encode(CUtensorMap* m, const void* base, int dt, const int64_t st[2],
   return r == CUDA_SUCCESS ? HQ_OK : HQ_ERR_INVALID_ARGUMENT;
 }
 
-template <int DT>
+template <int DT, int NT>
 int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+  using C = Cfg<NT>;
   static std::atomic<uint64_t> ready{0};
-  auto kern = packed_kernel<DT>;
+  auto kern = packed_kernel<DT, NT>;
   // an increase beyond the registers of the launch would wait for ever
   static const bool fits = [&] {
     cudaFuncAttributes a;
-    return cudaFuncGetAttributes(&a, kern) == cudaSuccess && a.numRegs * kThreads >= kSoft * kSoftRegs + (kThreads - kSoft) * kOtherRegs;
+    return cudaFuncGetAttributes(&a, kern) == cudaSuccess &&
+           a.numRegs * C::kThreads >= C::kSoft * C::kSoftRegs + (C::kThreads - C::kSoft) * C::kOtherRegs;
   }();
   if (!fits) return HQ_ERR_UNSUPPORTED;
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
   if (!bit || !(ready.load(std::memory_order_acquire) & bit)) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     ready.fetch_or(bit, std::memory_order_acq_rel);
   }
-  kern<<<p.units * p.n_split, kThreads, kSmem, st>>>(p, km, vm);
+  kern<<<p.units * p.n_split, C::kThreads, C::kSmem, st>>>(p, km, vm);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.n_split == 1) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.T) * p.Hkv * p.nrep + 3) / 4));
+  cfg.gridDim = dim3(p.units, C::kRows / 32, kD / 16);
   cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -665,12 +780,17 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, cudaSt
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, join_kernel<DT>, p);
+  e = p.n_split <= 4 ? cudaLaunchKernelEx(&cfg, join_kernel<DT, 4>, p, C::kRows)
+                     : cudaLaunchKernelEx(&cfg, join_kernel<DT, kMaxSplit>, p, C::kRows);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return static_cast<int>(e);
   }
   return HQ_OK;
+}
+template <int DT>
+int launch(const Params& p, int nt, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+  return nt == 1 ? launch<DT, 1>(p, km, vm, st) : launch<DT, 2>(p, km, vm, st);
 }
 
 }  // namespace pk
@@ -739,5 +859,5 @@ extern "C" int hq_packed_prefill(const void* q, const void* k, const void* v, in
     if (rc != HQ_OK) return rc;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == HQ_DTYPE_BF16 ? pk::launch<HQ_DTYPE_BF16>(p, km, vm, st) : pk::launch<HQ_DTYPE_F16>(p, km, vm, st);
+  return dtype == HQ_DTYPE_BF16 ? pk::launch<HQ_DTYPE_BF16>(p, pl.nt, km, vm, st) : pk::launch<HQ_DTYPE_F16>(p, pl.nt, km, vm, st);
 }

@@ -252,13 +252,15 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // rows behind the last sequence
+  // rows before the first sequence and behind the last
   if (p.zero_rest) {
-    const int rest = p.B > 0 ? min(max(p.cu_q[p.B], 0), p.T) : 0;
-    for (int64_t i = rest + static_cast<int64_t>(blockIdx.x); i < p.T; i += gridDim.x)
+    const int first = min(max(p.cu_q[0], 0), p.T), end = min(max(p.cu_q[p.B], first), p.T);
+    for (int64_t i = blockIdx.x; i < p.T - (end - first); i += gridDim.x) {
+      const int64_t row = i < first ? i : i + (end - first);
       for (int x = tid; x < p.Hkv * p.nrep * (kD / 8); x += kThreads)
-        *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + 2 * (i * p.os[0] + x / (kD / 8) * p.os[1] + x % (kD / 8) * 8)) =
+        *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + 2 * (row * p.os[0] + x / (kD / 8) * p.os[1] + x % (kD / 8) * 8)) =
             make_uint4(0, 0, 0, 0);
+    }
   }
   if (warp == 0) {
     // heavy (last) pieces first

@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
     i = tok - first;
     n = b < p.B ? min(p.cu[b + 1], p.T) - first : 0;
   }
-  const bool live = here && i < n;
+  const bool live = here && i >= 0 && i < n;
   const int len = live ? p.lens[b] : 0;
   const int64_t at = static_cast<int64_t>(len) + i;
   bool fits = live && len >= 0 && static_cast<int64_t>(len) + n <= static_cast<int64_t>(p.pg.max_pages) << p.pg.page_log;

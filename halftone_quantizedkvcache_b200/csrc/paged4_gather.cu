@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kGThreads) gather_kernel(const __grid_constant
   const int h0 = group * p.heads_per_block, h1 = min(p.Hkv, h0 + p.heads_per_block);
   const int64_t cat = pid * p.pg.cp + place * kRowB + word_at(place, l >> 2, l & 3);
   const int64_t sat = pid * p.pg.sp + place * 4 + (l >> 2);
-#pragma unroll 2
+#pragma unroll 1  // (two heads at once: fewer warps fit, 8 x 8192 tokens 64 to 71 us)
   for (int h = h0; h < h1; ++h) {
     uint4 k = make_uint4(0, 0, 0, 0), v = k;
     if (held) {

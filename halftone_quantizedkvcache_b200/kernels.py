@@ -1796,46 +1796,66 @@ def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, 
     ``ragged_status()``; that token's row counts as one that no token goes to.
     """
     what = "paged4_gather"
-    _tensors(what, lens=lens, cu_seqlens=cu_seqlens)
-    if first is not None:
-        _tensors(what, first=first)
-    n_rows = operator.index(n_rows)
-    if n_rows < 0 or n_rows > 0x7fffffff:
-        raise ValueError(f"{what}: n_rows must be 0 .. 2^31 - 1")
-    if (k_out is None) != (v_out is None):
-        raise ValueError(f"{what}: k_out and v_out come together")
-    if k_out is not None:
+    try:
+        key = (what, n_rows, dtype, lens.shape, lens.stride(), lens.dtype, lens.get_device(),
+               cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.get_device())
+        key += _paged4_key(cache, block_tables)
+        key += _sig_opt(first)
+    except (AttributeError, TypeError, KeyError):
+        _tensors(what, lens=lens, cu_seqlens=cu_seqlens)
+        if first is not None:
+            _tensors(what, first=first)
+        _paged4_cache(what, cache, block_tables, lens.numel(), lens.device)
+        raise
+    plan = _plans.get(key)
+    if plan is None:
+        try:
+            rows = operator.index(n_rows)
+        except TypeError:
+            raise TypeError(f"{what}: n_rows must be a whole number") from None
+        if not 0 <= rows <= 0x7fffffff:
+            raise ValueError(f"{what}: n_rows must be 0 .. 2^31 - 1")
+        if k_out is None and v_out is None and dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"{what}: rows must be bfloat16 or float16")
+        _cuda(lens, f"{what} lens")
+        dev = lens.device
+        if lens.dim() != 1:
+            raise ValueError(f"{what}: lens must be int32 [B]")
+        B = lens.shape[0]
+        Hkv, *pages = _paged4_cache(what, cache, block_tables, B, dev)
+        _lens_ok(what, "lens", lens, B, dev)
+        _lens_ok(what, "cu_seqlens", cu_seqlens, B + 1, dev)
+        _lens_ok(what, "first", first, B, dev)
+        plan = _keep(key, (dev, rows, B, Hkv, *pages, _lib.strides((Hkv * 128, 128), 2),
+                           _lib.lib().hq_paged4_gather))
+    dev, rows, B, Hkv, cst, sst, n_pages, page, tst, max_pages, ost, fn = plan
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, first=first, dtype=dtype,
+                                 k_out=k_out, v_out=v_out)
+    kst = vst = ost
+    made = k_out is None and v_out is None
+    if made:
+        k_out, v_out = lens.new_empty((2, rows, Hkv, 128), dtype=dtype).unbind(0)
+    else:
+        if k_out is None or v_out is None:
+            raise ValueError(f"{what}: k_out and v_out come together")
         _tensors(what, k_out=k_out, v_out=v_out)
         dtype = k_out.dtype
-    if dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"{what}: rows must be bfloat16 or float16")
-    _cuda(lens, f"{what} lens")
-    dev = lens.device
-    if lens.dim() != 1:
-        raise ValueError(f"{what}: lens must be int32 [B]")
-    B = lens.shape[0]
-    Hkv, cst, sst, n_pages, page, tst, max_pages = _paged4_cache(what, cache, block_tables, B, dev)
-    _lens_ok(what, "lens", lens, B, dev)
-    _lens_ok(what, "cu_seqlens", cu_seqlens, B + 1, dev)
-    _lens_ok(what, "first", first, B, dev)
-    made = k_out is None
-    if made:
-        k_out, v_out = (torch.empty((n_rows, Hkv, 128), dtype=dtype, device=dev) for _ in range(2))
-    else:
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"{what}: rows must be bfloat16 or float16")
         for t, n in ((k_out, "k_out"), (v_out, "v_out")):
             if t.device != dev:
                 raise ValueError(f"{what}: {n} is on {t.device}, the cache on {dev}")
-            _packed_out(what, n, t, (n_rows, Hkv, 128), k_out)
-    if n_rows == 0:
+            _packed_out(what, n, t, (rows, Hkv, 128), k_out)
+        kst, vst = _lib.strides(k_out.stride()[:2], 2), _lib.strides(v_out.stride()[:2], 2)
+    if rows == 0:
         return k_out, v_out
-    with _on_device(dev):
-        rc = _lib.lib().hq_paged4_gather(
-            cache["k"].data_ptr(), cache["v"].data_ptr(), cst, cache["k_scale"].data_ptr(),
+    rc = fn(cache["k"].data_ptr(), cache["v"].data_ptr(), cst, cache["k_scale"].data_ptr(),
             cache["v_scale"].data_ptr(), sst, n_pages, page, block_tables.data_ptr(), tst, max_pages,
             lens.data_ptr(), first.data_ptr() if first is not None else None, cu_seqlens.data_ptr(),
-            n_rows, B, Hkv, 128, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype],
-            _lib.strides(k_out.stride()[:2], 2), _lib.strides(v_out.stride()[:2], 2), 1 if made else 0,
-            _status_word(dev).data_ptr(), _stream(dev))
+            rows, B, Hkv, 128, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype], kst, vst,
+            1 if made else 0, _status_word(dev).data_ptr(), _stream(dev))
     if rc:
         check(rc, "hq_paged4_gather")
     return k_out, v_out
@@ -1849,8 +1869,8 @@ def packed_prefill_attn(q, k, v, cu_q, cu_k=None, *, causal=True, sm_scale=None,
     ``cu_q[b] .. cu_q[b+1]-1`` and the keys ``cu_k[b] .. cu_k[b+1]-1`` (int32 ``[B+1]`` on the device;
     ``cu_k`` defaults to ``cu_q``: whole prompts).  The queries stand at the last positions: query i
     of n sees keys ``j <= m - n + i`` of m (``causal=False``: all of them), and gives zeros where that
-    is none.  Returns ``[T,Hq,128]``; rows behind the last sequence are zeros, or are left as they were
-    in ``out``.  ``sm_scale`` (default 1/sqrt(128)) is positive.  Sums are float32, the weights rounded
+    is none.  Returns ``[T,Hq,128]``; rows before the first sequence and behind the last are zeros, or are left
+    as they were in ``out``.  ``sm_scale`` (default 1/sqrt(128)) is positive.  Sums are float32, the weights rounded
     to q's type.  A V row that holds an infinity or NaN spoils the rows that see it, and no others.
     """
     what = "packed_prefill_attn"

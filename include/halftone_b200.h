@@ -688,8 +688,8 @@ HQ_API int hq_rope_append_kv(
  *   query i of n seeing keys j <= m - n + i of m (causal = 0: all); a query that
  *   sees none gives zeros.  sm_scale > 0.  K and V strides are positive, and both
  *   have the larger stride at the same place.  A V row that holds an infinity or
- *   NaN spoils the rows that see it.  Rows behind the last sequence are left as
- *   they were, or with zero_rest become zeros.  The workspace
+ *   NaN spoils the rows that see it.  Rows before the first sequence and behind
+ *   the last are left as they were, or with zero_rest become zeros.  The workspace
  *   (hq_packed_prefill_workspace_bytes, 16-byte aligned) holds partial states
  *   where keys are split over blocks.
  */

@@ -104,6 +104,9 @@ def test_rows_behind_the_last_sequence_and_out():
     kernels.packed_prefill_attn(q, k, v, cum(nq), out=buf[:, ::2])
     assert torch.equal(buf[:103, ::2], out[:103]) and (buf[103:] == 2.5).all() and (buf[:, 1::2] == 2.5).all()
     assert (kernels.packed_prefill_attn(q, k, v, ints([0])) == 0).all()
+    # rows before the first sequence
+    ahead = kernels.packed_prefill_attn(q, k, v, ints([70, 103]), ints([70, 103]))
+    assert (ahead[:70] == 0).all() and (ahead[103:] == 0).all() and torch.equal(ahead[70:103], out[70:103])
     assert kernels.packed_prefill_attn(q[:0], k, v, ints([0, 0]), ints([0, 5])).shape == (0, 4, D)
     assert (kernels.packed_prefill_attn(q, k[:0], v[:0], cum(nq), ints([0, 0, 0])) == 0).all()
 

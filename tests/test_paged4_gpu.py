@@ -187,6 +187,11 @@ def test_append_rows_behind_the_last_sequence():
     check_append(q, k, v, cache, tables, [6, 3], [0, 0], before, q_out, k_out, inv, None)
     got = kernels.paged4_append(q, k, v, cache, tables, ints([0, 0]), cu_seqlens=ints([0, 6, 9]), inv_freq=inv)
     assert torch.equal(got[9:], q[9:]) and torch.equal(got[:9], q_out[:9])
+    # and before the first
+    q_out.fill_(5)
+    kernels.paged4_append(q, k, v, cache, tables, ints([0, 0]), cu_seqlens=ints([4, 4, 9]), inv_freq=inv, q_out=q_out)
+    assert (q_out[:4] == 5).all() and (q_out[9:] == 5).all() and not (q_out[4:9] == 5).all()
+    assert kernels.ragged_status() == 0
     assert kernels.paged4_append(q[:0], k[:0], v[:0], cache, tables, ints([0, 0]), cu_seqlens=ints([0, 0, 0])).shape == (0, 4, D)
 
 

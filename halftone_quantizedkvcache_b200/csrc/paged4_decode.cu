@@ -33,6 +33,7 @@ namespace p4 {
 
 constexpr int kTile = 64;                 // tokens
 constexpr int kSets = kTile / 8;
+constexpr int kWhole = 1024;              // tokens that one block takes in one go
 constexpr int kMaxSeqs = 1024;
 constexpr int kPartRow = kD + 4;          // m, l, two pad words, o
 constexpr int kStageB = 2 * kTile * (kRowB + kScaleB);
@@ -51,6 +52,7 @@ struct DecodeParams {
   float* ends;                            // and of warps'
   int* cum;                               // for join_kernel: first tile of every sequence
   int grid;
+  int by_unit;                            // a block per unit, nothing to join across blocks
   int* status;
 };
 
@@ -184,47 +186,59 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
   if (lane < 2) ends[warp][lane] = -1;
   fence_mbar_init();
   const int per = p.Hkv * p.n_rt;
-  for (int b = tid; b < p.B; b += 32 * C::kWarps) lens[b] = seq_len(p, b);
-  __syncthreads();
-  if (warp == 0) {
-    int run = 0;
-    if (lane == 0) cum[0] = 0;
-#pragma unroll 1
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-      int x = b0 + lane < p.B ? tiles_of(lens[b0 + lane]) * per : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (b0 + lane < p.B) cum[b0 + lane + 1] = run + x;
-      run += __shfl_sync(0xffffffffu, x, 31);
-    }
-  }
-  __syncthreads();
-  if (blockIdx.x == 0)
-    for (int b = tid; b <= p.B; b += 32 * C::kWarps) p.cum[b] = cum[b];
-  const int total = cum[p.B];
-  // an equal run of the line for each block, and of that for each warp
-  const int run = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-  const int chunk = (run + C::kWarps - 1) / C::kWarps;
   Cursor cur{};
-  {
-    const int64_t from = static_cast<int64_t>(blockIdx.x) * run, upto = min(from + run, static_cast<int64_t>(total));
-    cur.line = static_cast<int>(min(from + warp * chunk, upto));
-    cur.end = static_cast<int>(min(static_cast<int64_t>(cur.line) + chunk, upto));
+  int run = 0;                            // tiles of a block
+  if (p.by_unit) {
+    cur.e = static_cast<int>(blockIdx.x / static_cast<uint32_t>(per));
+    cur.idx = static_cast<int>(blockIdx.x) - cur.e * per;
+    cur.len = seq_len(p, cur.e);
+    cur.nt = tiles_of(cur.len);
+    const int chunk = (cur.nt + C::kWarps - 1) / C::kWarps;
+    cur.line = min(warp * chunk, cur.nt);
+    cur.end = min(cur.line + chunk, cur.nt);
+    __syncwarp();
+  } else {
+    for (int b = tid; b < p.B; b += 32 * C::kWarps) lens[b] = seq_len(p, b);
+    __syncthreads();
+    if (warp == 0) {
+      int run = 0;
+      if (lane == 0) cum[0] = 0;
+#pragma unroll 1
+      for (int b0 = 0; b0 < p.B; b0 += 32) {
+        int x = b0 + lane < p.B ? tiles_of(lens[b0 + lane]) * per : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        if (b0 + lane < p.B) cum[b0 + lane + 1] = run + x;
+        run += __shfl_sync(0xffffffffu, x, 31);
+      }
+    }
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int b = tid; b <= p.B; b += 32 * C::kWarps) p.cum[b] = cum[b];
+    const int total = cum[p.B];
+    // an equal run of the line for each block, and of that for each warp
+    run = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+    const int chunk = (run + C::kWarps - 1) / C::kWarps;
+    {
+      const int64_t from = static_cast<int64_t>(blockIdx.x) * run, upto = min(from + run, static_cast<int64_t>(total));
+      cur.line = static_cast<int>(min(from + warp * chunk, upto));
+      cur.end = static_cast<int>(min(static_cast<int64_t>(cur.line) + chunk, upto));
+    }
+    if (cur.line < cur.end) {
+      int lo = 0, hi = p.B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cum[mid] <= cur.line) lo = mid; else hi = mid - 1;
+      }
+      enter(cur, lens, lo);
+      cur.idx = static_cast<uint32_t>(cur.line - cum[lo]) / static_cast<uint32_t>(cur.nt);
+      cur.first = cum[lo] + cur.idx * cur.nt;
+    }
   }
   const bool any = cur.line < cur.end;
-  if (any) {
-    int lo = 0, hi = p.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (cum[mid] <= cur.line) lo = mid; else hi = mid - 1;
-    }
-    enter(cur, lens, lo);
-    cur.idx = static_cast<uint32_t>(cur.line - cum[lo]) / static_cast<uint32_t>(cur.nt);
-    cur.first = cum[lo] + cur.idx * cur.nt;
-  }
 
   // ---- the copies' cursor, up to kStages tiles ahead.  Lane 4 i + kind copies codes (kind 0: K, 1: V)
   // or scales (2: K, 3: V) of the tile's i-th page.  (Pages are no smaller than 16 tokens.)
@@ -497,13 +511,22 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
             mma_s8u8(cl[nt], kM8, kM8, kM8, kM8, lo[nt][2 * k], lo[nt][2 * k + 1], cl[nt]);
           }
         }
+        // the groups' words of chunk vj of token slots 2 c4 and 2 c4 + 1, set by set: both groups' in one
+        // load, where there are registers for them (7 x 2501 tokens 10 us against 12; 64 x 8192 105 against 103)
+        uint2 vw[2 * kSets];
+        if constexpr (NT == 1) {
+#pragma unroll
+          for (int i = 0; i < kSets; ++i) {
+            vw[2 * i] = *reinterpret_cast<const uint2*>(s + i * 8 * kRowB + va_off + 8 * gg);
+            vw[2 * i + 1] = *reinterpret_cast<const uint2*>(s + i * 8 * kRowB + vb_off + 8 * gg);
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int g = 2 * gg + e;
-          // the group's word of chunk vj of token slots 2 c4 and 2 c4 + 1, set by set (both groups' words in
-          // one load of 8 bytes hold 32 registers more)
-          auto word = [&](int i) {
-            return *reinterpret_cast<const uint32_t*>(s + (i >> 1) * 8 * kRowB + (i & 1 ? vb_off : va_off) + 4 * g);
+          auto word = [&](int i) -> uint32_t {
+            if constexpr (NT == 1) return e == 0 ? vw[i].x : vw[i].y;
+            else return *reinterpret_cast<const uint32_t*>(s + (i >> 1) * 8 * kRowB + (i & 1 ? vb_off : va_off) + 4 * g);
           };
           int h[NT][2][4], q8[NT][2][4];
 #pragma unroll
@@ -627,8 +650,8 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
           acc.w = __fmaf_rn(o.w, g, acc.w);
         }
         const int e = unit / per, idx = unit - e * per, kvh = idx / p.n_rt, r = (idx - kvh * p.n_rt) * C::kRows + row;
-        const int n = tiles_of(lens[e]), first = cum[e] + idx * n;
-        if (first / run != (first + n - 1) / run) {
+        const int n = p.by_unit ? 1 : tiles_of(lens[e]), first = p.by_unit ? 0 : cum[e] + idx * n;
+        if (!p.by_unit && first / run != (first + n - 1) / run) {
           float* dst = p.part + (static_cast<int64_t>(unit + static_cast<int>(blockIdx.x)) * C::kRows + row) * kPartRow;
           if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(M, L);
           *reinterpret_cast<float4*>(dst + 4 + 4 * lane) = acc;
@@ -679,7 +702,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 
 // ---------------------------------------------------------------- host
 struct DecodePlan {
-  int nt, n_rt, grid;
+  int nt, n_rt, grid, by_unit;
   size_t cum_bytes, part_bytes, bytes;
 };
 inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -691,6 +714,15 @@ inline bool plan_decode(DecodePlan& pl, int B, int Hkv, int nrep, int64_t cap) {
   pl.n_rt = (nrep + rows - 1) / rows;
   const int64_t units = int64_t(B) * Hkv * pl.n_rt, tiles = units * std::max<int64_t>(1, (cap + kTile - 1) / kTile);
   if (tiles > (int64_t(1) << 30)) return false;
+  // Few units with tables of up to kWhole tokens: a block per unit, 2 tiles a warp at most, and no second
+  // launch (1 x 512 tokens 7.2 us against 8.9, 20 x 200 6.4 against 10.3; units for several rounds of
+  // blocks better share the line: 64 x 512 26 us against 20).
+  pl.by_unit = cap <= kWhole && units <= current_sm_count();
+  if (pl.by_unit) {
+    pl.grid = static_cast<int>(units);
+    pl.bytes = 1;
+    return true;
+  }
   pl.grid = static_cast<int>(std::min<int64_t>(current_sm_count(), tiles));
   pl.cum_bytes = align256(sizeof(int) * (B + 1));
   pl.part_bytes = align256(sizeof(float) * static_cast<size_t>(units + pl.grid) * rows * kPartRow);
@@ -710,9 +742,9 @@ int launch_decode(const DecodeParams& p, int q_dt, const DecodePlan& pl, cudaStr
     if (e != cudaSuccess) return static_cast<int>(e);
     ready.fetch_or(bit, std::memory_order_acq_rel);
   }
-  decode_kernel<NT><<<pl.grid, 32 * C::kWarps, C::smem(p.B), st>>>(p, q_dt);
+  decode_kernel<NT><<<pl.grid, 32 * C::kWarps, C::smem(p.by_unit ? 0 : p.B), st>>>(p, q_dt);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return static_cast<int>(e);
+  if (e != cudaSuccess || p.by_unit) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.B) * p.Hkv * p.nrep);
   cfg.blockDim = dim3(32 * kJoinWarps);
@@ -760,7 +792,7 @@ extern "C" int hq_paged4_decode(const void* q, int q_dtype, const int64_t q_stri
   p4::DecodePlan pl{};
   if (!p4::plan_decode(pl, B, Hkv, Hq / Hkv, int64_t(page_size) * max_pages) || int64_t(B) * Hq > 0x7fffffff)
     return HQ_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < pl.bytes || !al(workspace, 256)) return HQ_ERR_WORKSPACE;
+  if (!pl.by_unit && (!workspace || workspace_bytes < pl.bytes || !al(workspace, 256))) return HQ_ERR_WORKSPACE;
   p4::DecodeParams p{};
   p.pg = p4::make_pages(k_codes, v_codes, k_scale, v_scale, code_strides, scale_strides, n_pages, page_size,
                         tables, table_stride, max_pages);
@@ -776,10 +808,13 @@ extern "C" int hq_paged4_decode(const void* q, int q_dtype, const int64_t q_stri
   p.n_rt = pl.n_rt;
   p.lens = lens;
   p.qk_scale = sm_scale * 1.4426950408889634f;
-  p.cum = static_cast<int*>(workspace);
-  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.cum_bytes);
-  p.ends = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.cum_bytes + pl.part_bytes);
+  if (!pl.by_unit) {
+    p.cum = static_cast<int*>(workspace);
+    p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.cum_bytes);
+    p.ends = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.cum_bytes + pl.part_bytes);
+  }
   p.grid = pl.grid;
+  p.by_unit = pl.by_unit;
   p.status = status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return pl.nt == 1 ? p4::launch_decode<1>(p, q_dtype, pl, st) : p4::launch_decode<2>(p, q_dtype, pl, st);

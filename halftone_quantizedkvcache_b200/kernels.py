@@ -1773,11 +1773,11 @@ def paged4_decode_attn(q, cache, block_tables, lens, *, sm_scale=None, out=None)
     if B == 0:
         return out
     status = _status_word(dev)
-    ws = status.new_empty(nw)
+    ws = status.new_empty(nw) if nb > 1 else None  # (1: none is needed)
     rc = fn(qp, dt, qst, cache["k"].data_ptr(), cache["v"].data_ptr(), cst, cache["k_scale"].data_ptr(),
             cache["v_scale"].data_ptr(), sst, n_pages, page, block_tables.data_ptr(), tst, max_pages,
             lens.data_ptr(), B, Hq, Hkv, D, default_scale if sm_scale is None else sm_scale,
-            out.data_ptr(), ost, ws.data_ptr(), nb, status.data_ptr(), _stream(dev))
+            out.data_ptr(), ost, ws.data_ptr() if nb > 1 else None, nb, status.data_ptr(), _stream(dev))
     if rc:
         check(rc, "hq_paged4_decode")
     return out

@@ -676,7 +676,8 @@ HQ_API int hq_rope_append_kv(
  * hq_paged4_decode: one query per sequence (q, out [B, Hq, 128]) over its lens[b]
  *   tokens (at most the table's); zeros where there are none.  B <= 1024, Hq /
  *   Hkv <= 128.  The workspace (hq_paged4_decode_workspace_bytes, 256-byte
- *   aligned, no initial contents) is not shared by launches that may overlap.  A
+ *   aligned, no initial contents; 1: none is needed, 0: unsupported) is not
+ *   shared by launches that may overlap.  A
  *   page that is none of the n_pages sets HQ_ERR_INVALID_ARGUMENT in `status`;
  *   that sequence's output has no meaning then.
  * hq_paged4_gather: rows cu_seqlens[b] + i of k_out / v_out [T, Hkv, 128] take

@@ -43,9 +43,9 @@ def test_append_argument_errors():
 
 def test_decode_argument_errors():
     L = _lib.lib()
-    nb = L.hq_paged4_decode_workspace_bytes(2, 4, 2, 16, 4, 128)
-    assert nb > 0
-    base = [256, 1, S2, 256, 256, C2, 256, 256, SC2, 5, 16, 256, 4, 4, 256, 2, 4, 2, 128, 0.1, 256, S2, 256, nb, None, None]
+    nb = L.hq_paged4_decode_workspace_bytes(2, 4, 2, 16, 128, 128)
+    assert nb > 1 == L.hq_paged4_decode_workspace_bytes(2, 4, 2, 16, 64, 128)   # 1024 tokens: none is needed
+    base = [256, 1, S2, 256, 256, C2, 256, 256, SC2, 5, 16, 256, 128, 128, 256, 2, 4, 2, 128, 0.1, 256, S2, 256, nb, None, None]
     refused(L.hq_paged4_decode, base, [
         (-1, dict(_0=None)), (-1, dict(_14=None)), (-1, dict(_20=None)), (-1, dict(_0=264)), (-1, dict(_15=-1)),
         (-1, dict(_16=0)), (-1, dict(_2=_lib.strides((512, 4), 2))), (-1, dict(_21=_lib.strides((0, 128), 2))),

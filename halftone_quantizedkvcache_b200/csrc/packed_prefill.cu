@@ -344,19 +344,29 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
   // Q, 16 lanes a row: K-major tiles of two 64-channel halves, 128-byte swizzle; rows past the last: zeros
   {
     constexpr int kEach = (kRows * 16 + kThreads - 1) / kThreads;
+    static_assert(kThreads % 16 == 0, "a half-warp per row");
     uint4 v[kEach];
+    const int c = tid & 15;
+    // row r's query and head, stepped from one of this thread's rows to the next
+    const uint32_t nrep = p.nrep, first = row0 + (tid >> 4);
+    uint32_t i = first / nrep, h = first - i * nrep;
+    const uint32_t di = kThreads / 16 / nrep, dh = kThreads / 16 - di * nrep;
+    const char* q = static_cast<const char*>(p.q) + 2 * (s.q0 * p.qs[0] + static_cast<int64_t>(kvh) * p.nrep * p.qs[1] + 8 * c);
 #pragma unroll
-    for (int n = 0; n < kEach; ++n) {     // (all loads in flight at once)
-      const int r = (tid + n * kThreads) >> 4, c = tid & 15;
-      v[n] = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int i = static_cast<uint32_t>(row0 + r) / static_cast<uint32_t>(p.nrep), h = kvh * p.nrep + row0 + r - i * p.nrep;
-        v[n] = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + 2 * ((s.q0 + static_cast<int64_t>(i)) * p.qs[0] + h * p.qs[1] + 8 * c));
+    for (int n = 0; n < kEach; ++n) {     // all loads in flight at once (rows past the last read the first)
+      const bool real = (tid >> 4) + n * (kThreads / 16) < rows;
+      v[n] = *reinterpret_cast<const uint4*>(q + (real ? 2 * (i * p.qs[0] + h * p.qs[1]) : 0));
+      i += di;
+      h += dh;
+      if (h >= nrep) {
+        h -= nrep;
+        ++i;
       }
     }
 #pragma unroll
     for (int n = 0; n < kEach; ++n) {
-      const int r = (tid + n * kThreads) >> 4, c = tid & 15;
+      const int r = (tid >> 4) + n * (kThreads / 16);
+      if (r >= rows) v[n] = make_uint4(0, 0, 0, 0);
       if (r < kRows) *reinterpret_cast<uint4*>(smem + (r >> 7) * kTileB + (c >> 3) * (kBN * 128) + sw128(r & 127, c & 7)) = v[n];
     }
   }
@@ -384,19 +394,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
       if (!ok) break;
       tc_fence_after();
       const int left = lim - j * kBN;     // keys of the tile that this row sees
-      bool spoiled = false, masked = false;
-      if (j >= jm) {
-        ok = wait_bar(clean_bar(j), clean_phase(j));
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint32_t* w = bad + 4 * (j & 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = min(max(left - 32 * i, 0), 32);
-          spoiled |= (w[i] & (n == 32 ? 0xffffffffu : (1u << n) - 1u)) != 0;
-        }
-        masked = __any_sync(0xffffffffu, left < kBN);
-      }
+      const bool masked = j >= jm && __any_sync(0xffffffffu, left < kBN);
+      bool spoiled = false;
       // the row: all of it in registers, or (half as many of those a thread) 32 scores at a time, twice
       constexpr int kHold = NT == 2 ? 128 : 32;
       uint32_t x[kHold];
@@ -471,9 +470,21 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
         }
         tmem_wait_st();
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar[C::kPFull + 2 * t + h]);
+        // spoiled V rows that this row sees (before the products may go on: they free V's stage, and with
+        // it the barrier's next phase and the flags)
+        if (h == 1 && j >= jm) {
+          ok = wait_bar(clean_bar(j), clean_phase(j));
+          const uint32_t* w = bad + 4 * (j & 1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int n = min(max(left - 32 * i, 0), 32);
+            spoiled |= (w[i] & (n == 32 ? 0xffffffffu : (1u << n) - 1u)) != 0;
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok && lane == 0) mbar_arrive(&bar[C::kPFull + 2 * t + h]);
       }
+      if (!ok) break;
       float a, e;
       f2_split(f2_add(sum, sum1), a, e);
       l += a + e;
@@ -518,13 +529,23 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
       __syncwarp();
       if (p.n_split == 1) {               // 16 lanes a row
         const int c = lane & 15;
+        const uint32_t nrep = p.nrep;
+        int r2 = 32 * (warp & 3) + (lane >> 4);
+        const uint32_t first = row0 + 128 * t + r2, i0 = first / nrep;
+        uint32_t h = first - i0 * nrep;
+        char* dst = static_cast<char*>(p.out) + 2 * ((s.q0 + static_cast<int64_t>(i0)) * p.os[0] + (kvh * p.nrep + static_cast<int64_t>(h)) * p.os[1] + 8 * c);
+        // two rows on: the next query's where its heads end
+        const int64_t step = 2 * (nrep == 1 ? 2 * p.os[0] : 2 * p.os[1]), wrap = 2 * (p.os[0] - static_cast<int64_t>(nrep) * p.os[1]);
 #pragma unroll 4
-        for (int k = 0; k < 16; ++k) {
-          const int r2 = 32 * (warp & 3) + 2 * k + (lane >> 4), row = 128 * t + r2;
-          if (row >= rows) break;
-          const int i = static_cast<uint32_t>(row0 + row) / static_cast<uint32_t>(p.nrep), h = kvh * p.nrep + row0 + row - i * p.nrep;
-          *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + 2 * ((s.q0 + static_cast<int64_t>(i)) * p.os[0] + h * p.os[1] + 8 * c)) =
-              *reinterpret_cast<const uint4*>(q_tile + r2 * 256 + ((c ^ (r2 & 7)) << 4));
+        for (int k = 0; k < 16; ++k, r2 += 2) {
+          if (128 * t + r2 >= rows) break;
+          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(q_tile + r2 * 256 + ((c ^ (r2 & 7)) << 4));
+          dst += step;
+          h += 2;
+          if (nrep > 1 && h >= nrep) {
+            h -= nrep;
+            dst += wrap;
+          }
         }
       }
     }

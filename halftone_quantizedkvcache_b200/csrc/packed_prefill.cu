@@ -9,13 +9,12 @@
 // every K and V tile of 128 keys.  Where that leaves SMs idle the keys are split over several blocks,
 // whose states (m, l, O) join_kernel puts together.  Blocks with the most keys start first.
 //
-// Roles of a block (12 warps): two groups of 4 softmax warps, a thread per row; one warp that issues
-// the products; one that loads K and V by TMA; two that look over the V tiles of masked steps.
-// S = Q K^T goes to tensor memory; the softmax thread takes its row into registers, and writes P in
-// 16 bits over the S it came from; O += P V reads P from there.  While one tile is in its softmax the
-// other's products run.  The running maximum moves only when it grows by more than 8 (P <= 2^8), so O
-// is rarely rescaled; sums are float32.  P is rounded to the model's type (2^-9 of each weight in
-// bf16, 2^-12 in float16: what the output itself is rounded by).
+// Roles of a block: softmax warps, 4 or 8 a row tile; one warp that issues the products; one that loads K
+// and V by TMA; two that look over the V tiles of masked steps.  S = Q K^T goes to tensor memory; the
+// softmax threads take it into registers and write P in 16 bits over it; O += P V reads P from there.
+// While one tile is in its softmax the other's products run.  The running maximum moves only when it grows
+// by more than 8 (P <= 2^8), so O is rarely rescaled; sums are float32.  P is rounded to the model's type
+// (2^-9 of each weight in bf16, 2^-12 in float16: what the output itself is rounded by).
 //
 // A V row holding an infinity or NaN spoils the rows that see it and no others: 0 x NaN is NaN in the
 // product, so on steps where some row does not see every key such rows are zeroed in shared memory
@@ -44,16 +43,23 @@ constexpr int kMaxSplit = 16;
 template <int NT>
 struct Cfg {
   static constexpr int kRows = 128 * NT;
-  static constexpr int kSoft = 128 * NT, kThreads = kSoft + 128;
-  // registers a thread after the split (softmax warps, the others) of 168 or 128 at launch
-  static constexpr int kSoftRegs = NT == 2 ? 208 : 176, kOtherRegs = NT == 2 ? 88 : 80;
+  // Softmax threads: one a row with 128 keys, or (one row tile, where nothing hides a step's length) two with
+  // 64 each, which tell each other their maxima.  One tile: 64 sequences of up to 200 tokens 52 us with two,
+  // 57 with one; one of 512 15.2 and 16.5.  Two tiles: 2 x 8192 549 us with two, 465 with one.
+  static constexpr int kH = NT == 1 ? 2 : 1, kKeys = 128 / kH;
+  static_assert(NT * kH <= 2, "places for one pair of threads a row");
+  static constexpr int kSoft = 128 * NT * kH, kThreads = kSoft + 128;
+  // registers a thread after the split (softmax warps, the others) of 168 at launch; 0: no split
+  static constexpr int kSoftRegs = NT == 2 ? 208 : 0, kOtherRegs = NT == 2 ? 88 : 0;
+  static constexpr int kPCol = 64 / (3 - kH);           // P of a tile's keys 64 .. : behind those before, or over their S
   static constexpr int kStages = 2 * NT;                // K, V, ..
   static constexpr int kOffKv = NT * kTileB;            // behind the Q tiles
   static constexpr int kOffBar = kOffKv + kStages * kTileB;
   static constexpr int kFull = 0, kEmpty = kFull + kStages, kSFull = kEmpty + kStages, kPFull = kSFull + NT,
-                       kOFull = kPFull + 2 * NT, kClean = kOFull + NT, kDrain = kClean + 2, kBars = kDrain + 1;
+                       kOFull = kPFull + 2 * NT, kPair = kOFull + NT, kClean = kPair + 4, kDrain = kClean + 2, kBars = kDrain + 1;
   static constexpr int kOffBad = kOffBar + (kBars * 8 + 15) / 16 * 16;  // [2][4] words of spoiled V rows
-  static constexpr int kOffMisc = kOffBad + 32;
+  static constexpr int kOffHalf = kOffBad + 32;          // [2][kH][128] what the threads of a row tell each other
+  static constexpr int kOffMisc = kOffHalf + (kH == 2 ? 2048 : 0);
   static constexpr int kSmem = 1024 + kOffMisc + 48;
   static constexpr uint32_t kColO = 128 * NT;           // tensor memory: S tiles, then O tiles
   static constexpr uint32_t kCols = 256 * NT;
@@ -168,6 +174,28 @@ __device__ __forceinline__ void tmem_stw32(uint32_t taddr, const uint32_t (&r)[3
       "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
       "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_ldw16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15"
+      "}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  tmem_ldw16(taddr, r);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
+  uint32_t r[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[i]);
+  tmem_stw16(taddr, r);
 }
 
 template <int DT>
@@ -288,6 +316,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
       mbar_init(&bar[C::kPFull + 2 * t + 1], 4);
       mbar_init(&bar[C::kOFull + t], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&bar[C::kPair + i], 2);
     for (int i = 0; i < 2; ++i) mbar_init(&bar[C::kClean + i], kCleanWarps);
     mbar_init(&bar[C::kDrain], 1);
     fence_mbar_init();
@@ -377,14 +406,28 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
   const uint32_t tmem = static_cast<uint32_t>(misc[8]);
   bool ok = true;
 
-  if (warp >= kSoftWarps) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+  if constexpr (C::kSoftRegs > 0) {
+    if (warp >= kSoftWarps) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
+  }
   if (warp < kSoftWarps) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
-    // ------------------------------------------------------------ softmax: a thread per row
-    const int t = warp >> 2, r = 128 * t + 32 * (warp & 3) + lane;
+    // ------------------------------------------------------------ softmax: kH threads a row, kKeys keys each
+    constexpr int kH = C::kH, kKeys = C::kKeys, kO = kH == 1 ? 32 : 16;  // (O's columns at a time)
+    const int t = warp / (4 * kH), hf = kH == 2 ? warp >> 2 & 1 : 0, lr = 32 * (warp & 3) + lane, r = 128 * t + lr;
     const int lim = limit_of(p, s, row0 + min(r, rows - 1));
-    const uint32_t s_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + 128 * t;
-    const uint32_t o_addr = s_addr - 128 * t + C::kColO + 128 * t;
+    const uint32_t tile = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+    const uint32_t s_addr = tile + 128 * t + kKeys * hf, o_addr = tile + C::kColO + 128 * t + kKeys * hf;
+    // the other thread's value for this one's.  The place written turns from one call to the next, and the
+    // second next one's comes when both have read: a step's products wait for both threads.
+    auto exchange = [&](float v, int n) {
+      float* at = reinterpret_cast<float*>(smem + C::kOffHalf) + 256 * (n & 1) + lr;
+      uint64_t* pair = &bar[C::kPair + (warp & 3)];
+      at[128 * hf] = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair);
+      ok = wait_bar(pair, n & 1);
+      return at[128 * (hf ^ 1)];
+    };
     float m = -INFINITY, l = 0.0f;        // m: of the raw scores
     const int jt = min(j1, nt[t]);
 #pragma unroll 1
@@ -393,11 +436,11 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const int left = lim - j * kBN;     // keys of the tile that this row sees
-      const bool masked = j >= jm && __any_sync(0xffffffffu, left < kBN);
+      const int left = lim - j * kBN - kKeys * hf;  // keys of this thread's that its row sees
+      const bool masked = j >= jm && __any_sync(0xffffffffu, left < kKeys);
       bool spoiled = false;
-      // the row: all of it in registers, or (half as many of those a thread) 32 scores at a time, twice
-      constexpr int kHold = NT == 2 ? 128 : 32;
+      // the scores: all of them in registers, or (fewer of those a thread) 32 at a time, twice
+      constexpr int kHold = kH == 1 ? 128 : 32;
       uint32_t x[kHold];
       auto load = [&](int c) {
         if constexpr (kHold == 128) tmem_ld128(s_addr, x);
@@ -409,7 +452,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
       };
       float top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 128 / kHold; ++c) {
+      for (int c = 0; c < kKeys / kHold; ++c) {
         load(c);
         float m0 = fmaxf(top, __uint_as_float(x[0])), m1 = __uint_as_float(x[1]);
 #pragma unroll
@@ -418,6 +461,11 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
           m1 = max3(m1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
         }
         top = max3(fmaxf(m0, m1), __uint_as_float(x[kHold - 2]), __uint_as_float(x[kHold - 1]));
+      }
+      if constexpr (kH == 2) {
+        top = fmaxf(top, exchange(top, j - j0));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
       }
       if (j == j0) {
         m = top;
@@ -428,61 +476,57 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
         m = m_new;
         l *= f;
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          float o[32];
-          tmem_ld32(o_addr + 32 * i, o);
+        for (int i = 0; i < kKeys / kO; ++i) {
+          float o[kO];
+          if constexpr (kO == 32) tmem_ld32(o_addr + 32 * i, o);
+          else tmem_ld16(o_addr + 16 * i, o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= f;
-          tmem_st32(o_addr + 32 * i, o);
+          for (int e = 0; e < kO; ++e) o[e] *= f;
+          if constexpr (kO == 32) tmem_st32(o_addr + 32 * i, o);
+          else tmem_st16(o_addr + 16 * i, o);
         }
         tmem_wait_st();
       }
       const float mc = m == -INFINITY ? 0.0f : m * p.c;
       const F2 c2 = f2_make(p.c, p.c), n2 = f2_make(-mc, -mc);
       F2 sum = f2_make(0.0f, 0.0f), sum1 = sum;
-      // 2 n scores from x[at] on as weights of the model's type
-      auto weights = [&](int at, int n, uint32_t* w) {
+      // weights, over scores of this thread's that are read no more: those of the tile's keys 0 .. 63 at its
+      // columns 0 .. 31, the others' from column kPCol on
+      constexpr int kPiece = kHold == 32 ? 32 : 64;  // keys at a time
 #pragma unroll
-        for (int i = 0; i < n; ++i) {
+      for (int c = 0; c < kKeys / kPiece; ++c) {
+        if constexpr (kHold == 32) load(c);
+        constexpr int kAt = kHold == 32 ? 0 : kPiece;
+        uint32_t w[kPiece / 2];
+#pragma unroll
+        for (int i = 0; i < kPiece / 2; ++i) {
           float a, e;
-          f2_split(f2_fma(f2_make(__uint_as_float(x[at + 2 * i]), __uint_as_float(x[at + 2 * i + 1])), c2, n2), a, e);
+          f2_split(f2_fma(f2_make(__uint_as_float(x[kAt * c + 2 * i]), __uint_as_float(x[kAt * c + 2 * i + 1])), c2, n2), a, e);
           a = ex2_ftz(a);
           e = ex2_ftz(e);
           if (i & 1) sum = f2_add(sum, f2_make(a, e));
           else sum1 = f2_add(sum1, f2_make(a, e));
           w[i] = pack2<DT>(a, e);
         }
-      };
+        if constexpr (kPiece == 64) tmem_stw32(s_addr + 32 * c, w);
+        else tmem_stw16(s_addr + 16 * c, w);
+        if (kPiece == 64 || c == 1) {     // 64 keys' weights are there
+          tmem_wait_st();
+          tc_fence_before();
+          // spoiled V rows that this row sees (before the products may go on: they free V's stage, and with
+          // it the barrier's next phase and the flags)
+          if (c == kKeys / kPiece - 1 && j >= jm) {
+            ok = wait_bar(clean_bar(j), clean_phase(j));
+            const uint32_t* bits = bad + 4 * (j & 1) + 2 * hf;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (kHold == 128) {
-          uint32_t w[32];
-          weights(64 * h, 32, w);
-          tmem_stw32(s_addr + 32 * h, w);
-        } else {
-#pragma unroll
-          for (int c = 2 * h; c < 2 * h + 2; ++c) {
-            load(c);
-            uint32_t w[16];
-            weights(0, 16, w);
-            tmem_stw16(s_addr + 16 * c, w);
+            for (int i = 0; i < kKeys / 32; ++i) {
+              const int n = min(max(left - 32 * i, 0), 32);
+              spoiled |= (bits[i] & (n == 32 ? 0xffffffffu : (1u << n) - 1u)) != 0;
+            }
           }
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok && lane == 0) mbar_arrive(&bar[C::kPFull + 2 * t + (kH == 1 ? c : hf)]);
         }
-        tmem_wait_st();
-        tc_fence_before();
-        // spoiled V rows that this row sees (before the products may go on: they free V's stage, and with
-        // it the barrier's next phase and the flags)
-        if (h == 1 && j >= jm) {
-          ok = wait_bar(clean_bar(j), clean_phase(j));
-          const uint32_t* w = bad + 4 * (j & 1);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int n = min(max(left - 32 * i, 0), 32);
-            spoiled |= (w[i] & (n == 32 ? 0xffffffffu : (1u << n) - 1u)) != 0;
-          }
-        }
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok && lane == 0) mbar_arrive(&bar[C::kPFull + 2 * t + h]);
       }
       if (!ok) break;
       float a, e;
@@ -492,7 +536,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
     }
     // ---- the rows' results
     if (ok && jt > j0) {
-      ok = wait_bar(&bar[C::kOFull + t], 0);
+      if constexpr (kH == 2) l += exchange(l, jt - j0);
+      ok = ok && wait_bar(&bar[C::kOFull + t], 0);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
@@ -501,48 +546,54 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
       const float inv = has ? 1.0f / l : 0.0f;  // (a NaN stays)
       // a partial row's 4 channels c lie beside those of the other rows
       float4* prt = reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(item) * p.n_split + split) * kRows * kPartRow);
-      if (p.n_split > 1 && live) prt[r] = make_float4(has && m != -INFINITY ? m * p.c : -INFINITY, has ? l : 0.0f, 0.0f, 0.0f);
-      // this tile's Q is read no more (its last product has been awaited): its rows' place
+      if (p.n_split > 1 && live && hf == 0)
+        prt[r] = make_float4(has && m != -INFINITY ? m * p.c : -INFINITY, has ? l : 0.0f, 0.0f, 0.0f);
+      // this tile's Q is read no more (its last product has been awaited): its rows' place, in halves of 128
+      // bytes
       unsigned char* q_tile = smem + t * kTileB;
-      const int lr = r & 127;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float o[32];
-        tmem_ld32(o_addr + 32 * c, o);
+      for (int c = kKeys / kO * hf; c < kKeys / kO * (hf + 1); ++c) {
+        float o[kO];
+        if constexpr (kO == 32) tmem_ld32(tile + C::kColO + 128 * t + 32 * c, o);
+        else tmem_ld16(tile + C::kColO + 128 * t + 16 * c, o);
         if (p.n_split > 1) {
           if (live)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              prt[(1 + 8 * c + e) * kRows + r] =
+            for (int e = 0; e < kO / 4; ++e)
+              prt[(1 + kO / 4 * c + e) * kRows + r] =
                   has ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_float4(0, 0, 0, 0);
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < kO / 8; ++e) {
             uint4 w = make_uint4(0, 0, 0, 0);
             if (has)
               w = make_uint4(pack2<DT>(o[8 * e] * inv, o[8 * e + 1] * inv), pack2<DT>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
                              pack2<DT>(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2<DT>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
-            *reinterpret_cast<uint4*>(q_tile + lr * 256 + (((4 * c + e) ^ (lr & 7)) << 4)) = w;
+            const int at = kO / 8 * c + e;  // of the row's 16 pieces
+            *reinterpret_cast<uint4*>(q_tile + (at >> 3) * (kTileB / 2) + sw128(lr, at & 7)) = w;
           }
         }
       }
       __syncwarp();
-      if (p.n_split == 1) {               // 16 lanes a row
-        const int c = lane & 15;
+      if (p.n_split == 1) {               // 16 / kH lanes a row
+        constexpr uint32_t kLanes = 16 / kH, kStep = 32 / kLanes;
+        const int c = lane % kLanes + 8 * hf;  // 16 bytes of the row
         const uint32_t nrep = p.nrep;
-        int r2 = 32 * (warp & 3) + (lane >> 4);
+        int r2 = 32 * (warp & 3) + lane / kLanes;
         const uint32_t first = row0 + 128 * t + r2, i0 = first / nrep;
         uint32_t h = first - i0 * nrep;
         char* dst = static_cast<char*>(p.out) + 2 * ((s.q0 + static_cast<int64_t>(i0)) * p.os[0] + (kvh * p.nrep + static_cast<int64_t>(h)) * p.os[1] + 8 * c);
-        // two rows on: the next query's where its heads end
-        const int64_t step = 2 * (nrep == 1 ? 2 * p.os[0] : 2 * p.os[1]), wrap = 2 * (p.os[0] - static_cast<int64_t>(nrep) * p.os[1]);
+        const unsigned char* src = q_tile + (c >> 3) * (kTileB / 2);
+        // kStep rows on: di queries and dh heads, or one query more where its heads end
+        const uint32_t di = kStep / nrep, dh = kStep - di * nrep;
+        const int64_t step = 2 * (di * p.os[0] + dh * p.os[1]), wrap = 2 * (p.os[0] - static_cast<int64_t>(nrep) * p.os[1]);
 #pragma unroll 4
-        for (int k = 0; k < 16; ++k, r2 += 2) {
+        for (int k = 0; k < 32 / static_cast<int>(kStep); ++k, r2 += kStep) {
           if (128 * t + r2 >= rows) break;
-          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(q_tile + r2 * 256 + ((c ^ (r2 & 7)) << 4));
+          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src + sw128(r2, c & 7));
           dst += step;
-          h += 2;
-          if (nrep > 1 && h >= nrep) {
+          h += dh;
+          if (h >= nrep) {
             h -= nrep;
             dst += wrap;
           }
@@ -592,12 +643,13 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           ok = ok && wait_bar(&bar[C::kPFull + 2 * t + h], n & 1);
+          if (C::kH == 2 && h == 0) ok = ok && wait_bar(&bar[C::kPFull + 2 * t + 1], n & 1);  // (both rescale O)
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-            mma_ts(lead, tmem + C::kColO + 128 * t, tmem + 128 * t + 8 * kk, v + (kk * 16 * 128 >> 4), v_hi, id_o, n > 0 || kk > 0);
+            mma_ts(lead, tmem + C::kColO + 128 * t, tmem + 128 * t + C::kPCol * h + 8 * (kk & 3), v + (kk * 16 * 128 >> 4), v_hi, id_o, n > 0 || kk > 0);
         }
         if (!ok) break;
         if (j + 1 < min(j1, nt[t])) score(t, ks);
@@ -776,13 +828,6 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, cudaSt
   using C = Cfg<NT>;
   static std::atomic<uint64_t> ready{0};
   auto kern = packed_kernel<DT, NT>;
-  // an increase beyond the registers of the launch would wait for ever
-  static const bool fits = [&] {
-    cudaFuncAttributes a;
-    return cudaFuncGetAttributes(&a, kern) == cudaSuccess &&
-           a.numRegs * C::kThreads >= C::kSoft * C::kSoftRegs + (C::kThreads - C::kSoft) * C::kOtherRegs;
-  }();
-  if (!fits) return HQ_ERR_UNSUPPORTED;
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
@@ -790,6 +835,14 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, cudaSt
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     ready.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  if (C::kSoftRegs > 0) {  // an increase beyond the registers of the launch would wait for ever
+    static const bool fits = [&] {
+      cudaFuncAttributes a;
+      return cudaFuncGetAttributes(&a, kern) == cudaSuccess &&
+             a.numRegs * C::kThreads >= C::kSoft * C::kSoftRegs + (C::kThreads - C::kSoft) * C::kOtherRegs;
+    }();
+    if (!fits) return HQ_ERR_UNSUPPORTED;
   }
   kern<<<p.units * p.n_split, C::kThreads, C::kSmem, st>>>(p, km, vm);
   cudaError_t e = cudaGetLastError();

@@ -7,12 +7,15 @@
 // what crosses a block's border leaves partial states (m, l, o) that join_kernel puts together, always
 // in the order of the line.
 //
-// Bound by the cache's bytes and, close behind, by issue slots: 144 bytes a token and head are 256
-// codes to unpack.  Both products are whole-number products on bytes (mma.sync m16n8k32, exact), the
-// codes being the 16-row operand, since a word of 8 codes becomes bytes with two masks and a shift:
+// 64 sequences of 4096 to 8192 tokens, 8 kv heads of 2 rows: 105 us, 4.3 TB/s of cache.  What holds it
+// back is the work between loads (issue slots 49 %, arithmetic units 44 %, the matrix units 25 %, DRAM 49 %
+// at half that size): 144 bytes a token and head are 256 codes to unpack, twice.  Both products are
+// whole-number products on bytes (mma.sync m16n8k32, exact), the codes being the 16-row operand, since a
+// word of 8 codes becomes bytes with two masks and a shift (matrix instructions that take their operands
+// from shared memory would want those bytes written there first: three times the tile's traffic):
 //   * Q K^T: q is a 22-bit whole number per channel (of the row's largest |q|: 2^-22 of it is lost) in
-//     three base-256 digits, two columns and a third in a second product that starts at -8 sum(q) for
-//     the codes' offset; one product is one group of 32 channels, its scale joins in float32.
+//     three base-256 digits, two columns and a third in a second product, and -8 sum(q) added for the
+//     codes' offset; one product is one group of 32 channels, its scale joins in float32.
 //   * P V: p relative to the tile's maximum, times the token's group scale relative to the tile's
 //     largest, is a 16-bit whole number (2^-16 of the tile's largest weight is lost) in two digits,
 //     transposed in registers by movmatrix; four tokens' bytes are turned with permutes.  A tile's sums
@@ -58,6 +61,7 @@ struct DecodeParams {
 
 template <int NT>
 struct Cfg {
+  // 64 x 8192 tokens: 105 us; 12 warps of 168 registers 113 (spilled), tiles of 32 tokens 113
   static constexpr int kWarps = 8;
   static constexpr int kStages = 2;
   static constexpr int kRows = 4 * NT;

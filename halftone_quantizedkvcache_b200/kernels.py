@@ -1602,10 +1602,10 @@ def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None
     sqrt(mean(x^2) + eps)``; ``inv_freq`` float32 ``[rotary_dim / 2]`` (``rope_inv_freq``;
     rotary_dim a multiple of 16) turns its first channels, half-split or ``interleaved``, cos and sin
     times ``factor``.  Both happen in float32 and are rounded once.  K is coded from the unrounded
-    rotated values, codes and scales those of exact arithmetic; V as it came.
+    rotated values, codes and scales as float64 arithmetic finds them; V as it came.
 
-    Returns the new q (``q_out``, which may be q; rows behind the last sequence stay what they were
-    there, or are q's in a result made by this call); ``k_out [T,Hkv,128]`` (memory of its own) takes the
+    Returns the new q (``q_out``, which may be q; rows of no sequence stay what they were there,
+    or are q's in a result made by this call); ``k_out [T,Hkv,128]`` (memory of its own) takes the
     new k, for the prompt's own attention.  K and V of real tokens are finite (others spoil their group).  A
     sequence whose tokens do not fit its table, and a token whose page is no page of the cache, are
     not written and set ``ragged_status()``; no two new tokens may go to the same place.
@@ -1720,8 +1720,8 @@ def paged4_decode_attn(q, cache, block_tables, lens, *, sm_scale=None, out=None)
     its first ``lens[b]`` tokens (at most those its table holds), and gives zeros where there are
     none.  What pages hold past them does not matter.  Returns the output in q's layout and dtype (or
     writes ``out [B,Hq,128]``).  Nothing depends on ``lens`` on the host: a captured call replays while
-    sequences grow.  Scores and sums are float32; q and the weights are split in two bf16 parts (2^-17
-    of each).  A page number outside the cache sets ``ragged_status()``, and that sequence's output
+    sequences grow.  Sums are float32; of q 2^-22 of its row's largest value is rounded off, of the
+    weights 2^-16 of the largest of 64 tokens.  A page number outside the cache sets ``ragged_status()``, and that sequence's output
     has no meaning.
     """
     what = "paged4_decode_attn"
@@ -1791,7 +1791,8 @@ def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, 
     Row ``cu_seqlens[b] + i`` takes token ``first[b] + i`` (``first`` int32 ``[B]``, default 0) of
     sequence b, as long as that is below ``lens[b]`` and the row below ``cu_seqlens[b+1]``: what a
     chunk over a cached past attends (``packed_prefill_attn``), or with ``first`` the new tokens as
-    later steps will see them.  Values are ``scale * code``, rounded once.  Rows that no token goes to
+    later steps will see them.  Values are ``scale * code``, rounded once (beyond float16's range:
+    infinities).  Rows that no token goes to
     are zeros, or what they were in ``k_out`` / ``v_out``.  A page number outside the cache sets
     ``ragged_status()``; that token's row counts as one that no token goes to.
     """
@@ -1848,6 +1849,8 @@ def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, 
             if t.device != dev:
                 raise ValueError(f"{what}: {n} is on {t.device}, the cache on {dev}")
             _packed_out(what, n, t, (rows, Hkv, 128), k_out)
+        if rows and k_out.data_ptr() == v_out.data_ptr():
+            raise ValueError(f"{what}: k_out and v_out must have memory of their own")
         kst, vst = _lib.strides(k_out.stride()[:2], 2), _lib.strides(v_out.stride()[:2], 2)
     if rows == 0:
         return k_out, v_out

@@ -668,9 +668,9 @@ HQ_API int hq_rope_append_kv(
  *   are normed where there are weights ([128], of x_dtype or F32): w x /
  *   sqrt(mean(x^2) + eps); then their first rotary_dim channels (a multiple of
  *   16; 0: none) are turned as in hq_rope_append_kv.  q_out takes q' (may be q),
- *   k_out (or NULL; memory of its own) k', both rounded once; K is coded from the unrounded k', V as
- *   it came.  Codes are those of exact arithmetic.  Rows behind the last sequence
- *   are left as they were (q_out with copy_rest: q's).  A sequence whose tokens do
+ *   k_out (or NULL; memory of its own) k', both rounded once; K is coded from the
+ *   unrounded k', V as it came, codes and scales as float64 arithmetic finds them.
+ *   Rows of no sequence are left as they were (q_out with copy_rest: q's).  A sequence whose tokens do
  *   not fit its table, or a token whose page is none of the n_pages, is not
  *   written to the cache and sets HQ_ERR_INVALID_ARGUMENT in `status`.
  * hq_paged4_decode: one query per sequence (q, out [B, Hq, 128]) over its lens[b]

@@ -146,3 +146,21 @@ def test_strides():
     one = dense[1][:, :1].expand(191, 2, D)
     assert torch.equal(kernels.packed_prefill_attn(dense[0], one, dense[2], cum(nq)),
                        kernels.packed_prefill_attn(dense[0], one.contiguous(), dense[2], cum(nq)))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n,m", [(1, 4096), (64, 900), (300, 9000)])
+def test_many_small_weights_beside_a_large_one(dtype, n, m):
+    # key 0 has weight 1, each other 2^-25.4, which float16 would round to nothing: together they carry
+    # V.  float16's weights lose at most 2^-32 of the largest each.
+    from halftone_quantizedkvcache_b200 import kernels
+    q, k, v = (torch.zeros((x, 1, D), device="cuda") for x in (n, m, m))
+    q[:, :, 3], k[0, :, 3] = 16.0, 25.4 * math.log(2.0) / 16.0 * math.sqrt(D)
+    v[1:] = 4096.0
+    q, k, v = (x.to(DT[dtype]) for x in (q, k, v))
+    out = kernels.packed_prefill_attn(q, k, v, cum([n]), cum([m]), causal=False)
+    ref, mag = plain.attend(*(x.transpose(0, 1) for x in (q, k, v)), seen_of(n, m, False), None)
+    half = torch.finfo(DT[dtype]).eps / 2
+    err = (out.transpose(0, 1).double() - ref).abs()
+    assert float(ref.min()) > 0.05
+    assert not (~(err <= half * ref.abs() * 1.01 + (half + 2.0 ** -13) * mag + 2.0 ** -32 * m * 4096)).any(), float(err.max())

@@ -60,10 +60,10 @@ def test_decode_argument_errors():
 
 
 def test_gather_argument_errors():
-    base = [256, 256, C2, 256, 256, SC2, 5, 16, 256, 4, 4, 256, None, 256, 7, 2, 2, 128, 256, 256, 1, S2, S2, 0, None, None]
+    base = [256, 256, C2, 256, 256, SC2, 5, 16, 256, 4, 4, 256, None, 256, 7, 2, 2, 128, 256, 512, 1, S2, S2, 0, None, None]
     refused(_lib.lib().hq_paged4_gather, base, [
         (-1, dict(_0=None)), (-1, dict(_11=None)), (-1, dict(_13=None)), (-1, dict(_14=-1)), (-1, dict(_16=0)),
-        (-1, dict(_18=None)), (-1, dict(_19=264)), (-1, dict(_21=_lib.strides((0, 128), 2))),
+        (-1, dict(_18=None)), (-1, dict(_19=264)), (-1, dict(_19=256)), (-1, dict(_21=_lib.strides((0, 128), 2))),
         (-1, dict(_22=_lib.strides((512, 4), 2))), (-2, dict(_17=64)), (-2, dict(_20=0)), (-2, dict(_7=17)),
     ])
     assert _lib.lib().hq_paged4_gather(*changed(base, _14=0)) == 0

@@ -336,6 +336,7 @@ def test_refusals():
     no(TypeError, gat, cache, tables, lens, cu, 1.5)
     no(ValueError, gat, cache, tables, lens, cu[:3], 4)
     no(ValueError, gat, cache, tables, lens, cu, 4, k_out=k)
+    no(ValueError, gat, cache, tables, lens, cu, 4, k_out=k, v_out=k)
     no(ValueError, gat, cache, tables, lens, cu, 4, k_out=k, v_out=bf(3, 2, D))
     no(ValueError, gat, cache, tables, lens, cu, 4, first=lens[:2])
     # packed attention

@@ -886,7 +886,7 @@ using namespace hq;
 extern "C" size_t hq_packed_prefill_workspace_bytes(int T, int Tk, int B, int Hq, int Hkv, int D) {
   if (T <= 0 || Tk < 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D != pk::kD) return 0;
   pk::Plan pl{};
-  return pk::plan(pl, T, Tk, B, Hkv, Hq / Hkv) ? std::max<size_t>(pl.bytes, 256) : 0;
+  return pk::plan(pl, T, Tk, B, Hkv, Hq / Hkv) ? std::max<size_t>(pl.bytes, 1) : 0;
 }
 
 extern "C" int hq_packed_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t q_strides[2],

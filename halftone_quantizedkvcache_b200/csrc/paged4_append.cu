@@ -9,9 +9,9 @@
 //
 // Codes are those that float64 arithmetic finds.  P * inv_freq, its cos and its sin are formed in float64
 // (once a token, kept as two float32 parts in shared memory); norms and turns are float32, off by at most
-// kSlack of |x w| + |o w_o|.  The k rows with a quotient or a scale closer to a rounding border than that
-// (one in 40) are listed, and formed again in float64 at the end of the block, its half-warps sharing them
-// (on the spot, one by one, they took a tenth of the time: 149 us against 131, sizes as below).  V's codes
+// kSlack of the pair's larger value.  The k rows with a quotient or a scale closer to a rounding border than
+// that (one in 60) are listed, and formed again in float64 at the end of the block, a warp a row (8 of the
+// 124 us below; a half-warp a row 15, on the spot one by one 30).  V's codes
 // come from its 16-bit values: an 11-bit x over an 11-bit s is 2^-13 away from a border unless it lies on
 // it, and one corrected division finds both cases.
 //
@@ -19,9 +19,11 @@
 // (8 channels, 16 bytes, each); a half-warp takes one token and all of its rows, 7 of them in flight
 // through shared memory (the next row in registers instead: 179 us).
 //
-// 8 x 4096 tokens of 16 q heads and 8 kv heads, both norms, full rotation, k kept: 131 us, 3.9 TB/s of
+// 8 x 4096 tokens of 16 q heads and 8 kv heads, both norms, full rotation, k kept: 124 us, 4.1 TB/s of
 // bytes moved.  Bound by issue slots (65 % of them taken; arithmetic units 39 %, DRAM 31 % at half that
-// size): for a lane and row of k a reduction of 128 squares, the turn and the codes.
+// size): for a lane and row of k a reduction of 128 squares, the turn and the codes.  (8 lanes a row, both
+// values of a pair in one lane, take 27 % fewer instructions but 96 registers: 131 us, the 20 warps an SM hide
+// less.)
 #include <algorithm>
 
 #include "paged4.cuh"
@@ -59,10 +61,11 @@ struct AppendParams {
   int rows_per_block, groups;
 };
 
-// Error of the float32 route, relative to |x w| + |o w_o| (times r and the factor), in units of 2^-24:
-// half that of a sum of 128 squares (4 in a lane's half, the halves, 4 rounds) 4, the mean 1 and r 1, cos
-// or sin 1, their weight 1 and factor 1, the turn's two products and sum 2, r's product 1: 12.
-constexpr float kSlack = 12.0f / 16777216.0f;
+// Error of the float32 route, relative to |x w cos| + |o w_o sin| (times r and the factor), in units of 2^-24:
+// half that of the mean (squares are exact; 3 sums in a lane's half, the halves, 4 rounds, eps: 9) 4.5 and
+// that of its root's correction 2.5, cos or sin 1, their weight 1 and factor 1, the turn's product 1 and sum
+// 1, r's product 1: 13.  The sum is at most the pair's length, sqrt(2) times the larger of its turned values.
+constexpr float kSlack = 1.4143f * 13.0f / 16777216.0f;
 
 template <int DT>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
@@ -120,6 +123,11 @@ __device__ __forceinline__ void quotients(const F2 (&x)[4], float s, float rs, F
   }
 }
 template <int DT>
+__device__ __forceinline__ float2 unpack16(uint32_t w) {
+  if constexpr (DT == HQ_DTYPE_BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <int DT>
 __device__ __forceinline__ void unpack_pairs(const uint4& w, F2 (&x)[4]) {
   float f[8];
   Vec16<DT>::unpack(w, f);
@@ -144,73 +152,87 @@ __device__ __forceinline__ uint4 pack_row(const F2 (&y)[4]) {
   return make_uint4(pack16<DT>(a[0], a[1]), pack16<DT>(a[2], a[3]), pack16<DT>(a[4], a[5]), pack16<DT>(a[6], a[7]));
 }
 
-// One k row in float64 (all 16 lanes of the half-warp `mask`): this lane's word and group's scale.
-struct Exact {
-  uint32_t word;
-  __half scale;
-};
+// The chunk of 8 channels that chunk c is turned with (itself: interleaved pairs, or not turned).
+__device__ __forceinline__ int partner_of(const AppendParams& p, int c) {
+  const int h8 = p.rot / 16;
+  return p.inter || c >= 2 * h8 ? c : c < h8 ? c + h8 : c - h8;
+}
 template <int DT>
-__device__ __noinline__ Exact exact_row(const AppendParams& p, const uint4& x, unsigned mask, int partner,
-                                        const float4* turn, int l) {
-  float f[8];
-  Vec16<DT>::unpack(x, f);
-  const int d0 = 8 * l, half = p.rot / 2;
-  double y[8], r = 1.0;
+__device__ __forceinline__ float weight_at(const AppendParams& p, const void* w, int d) {
+  if (!w) return 1.0f;
+  return p.w_f32 ? static_cast<const float*>(w)[d] : Elem<DT>::to_f32(static_cast<const typename Elem<DT>::T*>(w)[d]);
+}
+
+// A k row in float64 (a warp, 4 channels a lane): its codes and scales.
+template <int DT>
+__device__ __forceinline__ void exact_row(const AppendParams& p, const unsigned char* row, const float4* turn, uint8_t* codes,
+                                          __half* scales, int place) {
+  const int lane = threadIdx.x & 31, c = lane >> 1, half = p.rot / 2;
+  const int d0 = 4 * lane, o0 = 8 * partner_of(p, c) + 4 * (lane & 1);  // (interleaved: partners e ^ 1)
+  auto unpack = [](const uint2& w, float (&f)[4]) {
+    const float2 a = unpack16<DT>(w.x), b = unpack16<DT>(w.y);
+    f[0] = a.x;
+    f[1] = a.y;
+    f[2] = b.x;
+    f[3] = b.y;
+  };
+  float f[4], g[4], wt[4], wo[4];
+  const uint2 x = *reinterpret_cast<const uint2*>(row + 2 * d0), xo = *reinterpret_cast<const uint2*>(row + 2 * o0);
+  float4 t[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int d = d0 + e, eo = p.inter ? e ^ 1 : e;
+    wt[e] = weight_at<DT>(p, p.kw, d);
+    wo[e] = weight_at<DT>(p, p.kw, o0 + eo);
+    t[e] = turn[d >= p.rot ? 0 : p.inter ? d / 2 : d < half ? d : d - half];
+  }
+  unpack(x, f);
+  unpack(xo, g);
+  double r = 1.0;
   if (p.kw) {
-    double s = 0.0;
+    double s = fma(static_cast<double>(f[0]), static_cast<double>(f[0]), static_cast<double>(f[1]) * f[1]) +
+               fma(static_cast<double>(f[2]), static_cast<double>(f[2]), static_cast<double>(f[3]) * f[3]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), s);
-#pragma unroll
-    for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor_sync(mask, s, m);
-    s = s / kD + static_cast<double>(p.eps);
+    for (int m = 16; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+    s = s * (1.0 / kD) + static_cast<double>(p.eps);
     r = rsqrtf(static_cast<float>(s));
     r = r * fma(-0.5 * s * r, r, 1.5);    // 2^-22 becomes 2^-43
   }
+  double z[4], amax = 0.0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float w = 1.0f;
-    if (p.kw) w = p.w_f32 ? static_cast<const float*>(p.kw)[d0 + e]
-                          : Elem<DT>::to_f32(static_cast<const typename Elem<DT>::T*>(p.kw)[d0 + e]);
-    y[e] = f[e] * r * static_cast<double>(w);
-  }
-  double amax = 0.0, z[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const double o = p.inter ? y[e ^ 1] : __shfl_sync(mask, y[e], partner);
-    const int d = d0 + e;
-    z[e] = y[e];
-    if (d < p.rot) {
-      const float4 t = turn[p.inter ? d / 2 : d < half ? d : d - half];
-      const double c = static_cast<double>(t.x) + t.z, s = static_cast<double>(t.y) + t.w;
-      z[e] = ((p.inter ? !(d & 1) : d < half) ? y[e] * c - o * s : y[e] * c + o * s) * static_cast<double>(p.factor);
+  for (int e = 0; e < 4; ++e) {
+    z[e] = f[e] * r * static_cast<double>(wt[e]);
+    if (d0 < p.rot) {
+      const double o = (p.inter ? g[e ^ 1] : g[e]) * r * static_cast<double>(wo[e]);
+      const double cs = static_cast<double>(t[e].x) + t[e].z, sn = static_cast<double>(t[e].y) + t[e].w;
+      z[e] = ((p.inter ? !(e & 1) : d0 < half) ? z[e] * cs - o * sn : z[e] * cs + o * sn) * static_cast<double>(p.factor);
     }
     amax = fmax(amax, fabs(z[e]));
   }
-  amax = fmax(amax, __shfl_xor_sync(mask, amax, 1));
-  amax = fmax(amax, __shfl_xor_sync(mask, amax, 2));
-  Exact out;
-  out.scale = group_scale(static_cast<float>(amax * (2.0 / 15.0)));
-  const float s = __half2float(out.scale);
+  float a75 = static_cast<float>(amax * (2.0 / 15.0));
+#pragma unroll
+  for (int m = 4; m >= 1; m >>= 1) a75 = max_nan(a75, __shfl_xor_sync(0xffffffffu, a75, m));
+  const __half sc = group_scale(a75);
+  const float s = __half2float(sc);
   double rs = 0.0;
   if (s > 0.0f) {
     rs = rcp(s);
     rs = rs * fma(-static_cast<double>(s), rs, 2.0);
   }
-  F2 k[4];
+  uint32_t word = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {           // (channels that are not turned can lie on a border: corrected, exact there)
-    const double t = z[e] * rs;
-    z[e] = rint(fma(fma(-t, static_cast<double>(s), z[e]), rs, t));
+  for (int e = 0; e < 4; ++e) {           // (channels that are not turned can lie on a border: corrected, exact there)
+    const double q = z[e] * rs;
+    const float k = static_cast<float>(rint(fma(fma(-q, static_cast<double>(s), z[e]), rs, q)));
+    word |= static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(k, -8.0f), 7.0f)) + 8) << (4 * e);
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) k[e] = f2_make(static_cast<float>(z[e]), static_cast<float>(z[e + 4]));
-  out.word = pack_codes(k);
-  return out;
+  const int g4 = lane >> 3, j = c & 3;
+  *reinterpret_cast<uint16_t*>(codes + word_at(place, g4, j) + 2 * (lane & 1)) = static_cast<uint16_t>(word);
+  if ((lane & 7) == 0) scales[g4] = sc;
 }
 
 template <int DT>
 __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_constant__ AppendParams p) {
-  using T16 = typename Elem<DT>::T;
   __shared__ uint4 ring[kTok][kRing * 16];
   __shared__ float4 turn[kTok][kD / 2];   // cos and sin, and what is left of them
   extern __shared__ uint32_t again[];     // k rows to form again: token of the block, head
@@ -293,8 +315,7 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
     float wt[8], c[8], g[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      wt[e] = 1.0f;
-      if (w) wt[e] = p.w_f32 ? static_cast<const float*>(w)[d0 + e] : Elem<DT>::to_f32(static_cast<const T16*>(w)[d0 + e]);
+      wt[e] = weight_at<DT>(p, w, d0 + e);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -392,8 +413,7 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
       const float s = __half2float(sc), rs = s > 0.0f ? rcp(s) : 0.0f;
       bool near = false;
       if (!plain_k) {
-        // |x w| + |o w_o| is at most twice the larger of the pair's turned values
-        const float err = 2.0f * kSlack * fmaxf(a, p.inter ? a : __shfl_sync(0xffffffffu, a, partner));
+        const float err = kSlack * fmaxf(a, p.inter ? a : __shfl_sync(0xffffffffu, a, partner));
         const float e75 = __fmaf_rn(err, 0.13333334f, a75 * 1.2e-7f);
         // the scale is the same for all a75 that this one may stand for
         near = a75 < INFINITY && __half_as_ushort(group_scale(a75 + e75)) != __half_as_ushort(group_scale(fmaxf(a75 - e75, 0.0f)));
@@ -451,13 +471,11 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
   // ---- rows whose codes float32 could not tell
   if (plain_k || r1 <= p.Hq || r0 >= p.Hq + p.Hkv) return;
   __syncthreads();
-  for (int i = sub; i < n_again; i += kTok) {
+  for (int i = tid >> 5; i < n_again; i += kThreads / 32) {
     const int of = again[i] >> 16, h = again[i] & 0xffff;
     const int4 w = where[of];             // token, page, place
-    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.k) + 2 * (w.x * p.ks[0] + h * p.ks[1] + d0));
-    const Exact ex = exact_row<DT>(p, x, mask, partner, turn[of], l);
-    *reinterpret_cast<uint32_t*>(p.pg.k + w.y * p.pg.cp + h * p.pg.ch + w.z * kRowB + word_at(w.z, l >> 2, l & 3)) = ex.word;
-    if ((l & 3) == 0) p.pg.ksc[w.y * p.pg.sp + h * p.pg.sh + w.z * 4 + (l >> 2)] = ex.scale;
+    exact_row<DT>(p, static_cast<const unsigned char*>(p.k) + 2 * (w.x * p.ks[0] + h * p.ks[1]), turn[of],
+                  p.pg.k + w.y * p.pg.cp + h * p.pg.ch + w.z * kRowB, p.pg.ksc + w.y * p.pg.sp + h * p.pg.sh + w.z * 4, w.z);
   }
 }
 

@@ -1906,13 +1906,13 @@ def packed_prefill_attn(q, k, v, cu_q, cu_k=None, *, causal=True, sm_scale=None,
             return _rows_strided(t) and all(st > 0 or n <= 1 for n, st in zip(t.shape, t.stride()))
         rising = [t.shape[1] > 1 and t.stride(1) > t.stride(0) for t in (k, v)]
         with _on_device(dev):
-            nb = 0 if T == 0 or B == 0 else _ws_size(what, dev, _lib.lib().hq_packed_prefill_workspace_bytes(
+            nb = 1 if T == 0 or B == 0 else _ws_size(what, dev, _lib.lib().hq_packed_prefill_workspace_bytes(
                 T, Tk, B, Hq, Hkv, D))
-        plan = _keep(key, (dev, T, Tk, B, Hq, Hkv, _DT[q.dtype], 1 if causal else 0, _rows_strided(q),
+        plan = _keep(key, (dev, T, Tk, B, Hq, Hkv, _DT[q.dtype], 1 if causal else 0, _rows_strided(q), q.is_contiguous(),
                            tma(k) and tma(v) and rising[0] == rising[1],
                            *[_lib.strides(x.stride()[:2], 2) for x in (q, k, v)], nb, (nb + 3) // 4,
                            _lib.strides((Hq * D, D), 2), 1.0 / math.sqrt(D), _lib.lib().hq_packed_prefill))
-    (dev, T, Tk, B, Hq, Hkv, dt, causal, q_ok, kv_ok, qst, kst, vst, nb, nw, ost, default_scale,
+    (dev, T, Tk, B, Hq, Hkv, dt, causal, q_ok, dense, kv_ok, qst, kst, vst, nb, nw, ost, default_scale,
      fn) = plan
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
@@ -1929,7 +1929,7 @@ def packed_prefill_attn(q, k, v, cu_q, cu_k=None, *, causal=True, sm_scale=None,
         kst, vst = (_lib.strides(t.stride()[:2], 2) for t in (k, v))
     rest = out is None
     if rest:
-        out = q.new_empty((T, Hq, 128))
+        out = torch.empty_like(q) if dense else q.new_empty((T, Hq, 128))
     else:
         _packed_out(what, "out", out, (T, Hq, 128), q)
         ost = _lib.strides(out.stride()[:2], 2)
@@ -1938,10 +1938,10 @@ def packed_prefill_attn(q, k, v, cu_q, cu_k=None, *, causal=True, sm_scale=None,
     if B == 0:
         return out.zero_() if rest else out
     status = _status_word(dev)
-    ws = status.new_empty(nw)
+    ws = status.new_empty(nw) if nb > 1 else None  # (1: none is needed)
     rc = fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, qst, kst, vst, cu_q.data_ptr(),
             cu_k.data_ptr(), T, Tk, B, Hq, Hkv, 128, causal, sm_scale, out.data_ptr(), ost,
-            1 if rest else 0, ws.data_ptr(), nb, status.data_ptr(), _stream(dev))
+            1 if rest else 0, ws.data_ptr() if nb > 1 else None, nb, status.data_ptr(), _stream(dev))
     if rc:
         check(rc, "hq_packed_prefill")
     return out

@@ -691,8 +691,8 @@ HQ_API int hq_rope_append_kv(
  *   have the larger stride at the same place.  A V row that holds an infinity or
  *   NaN spoils the rows that see it.  Rows before the first sequence and behind
  *   the last are left as they were, or with zero_rest become zeros.  The workspace
- *   (hq_packed_prefill_workspace_bytes, 16-byte aligned) holds partial states
- *   where keys are split over blocks.
+ *   (hq_packed_prefill_workspace_bytes, 16-byte aligned; 1: none is needed, 0:
+ *   unsupported) holds partial states where keys are split over blocks.
  */
 HQ_API int hq_paged4_append(const void* q, const void* k_new, const void* v_new, int x_dtype,
                             const int64_t q_strides[2], const int64_t k_strides[2],

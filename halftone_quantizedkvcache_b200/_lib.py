@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -19,12 +20,11 @@ OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_DEVICE_TIMEOUT = 0
 
 _i64_4 = ctypes.c_int64 * 4
 _i64_3 = ctypes.c_int64 * 3
-_i64_2 = ctypes.c_int64 * 2
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _Z = ctypes.c_size_t
 _F = ctypes.c_float
-_L = ctypes.c_int64
+_S = ctypes.c_char_p  # the bytes of a struct of arguments
 _A4 = ctypes.POINTER(ctypes.c_int64)
 
 # name -> (restype, argtypes), in the order of include/halftone_b200.h
@@ -91,19 +91,22 @@ SIGNATURES = {
                                    _A4, _P, _Z, _P, _P]),
     "hq_rope_append_kv": (_I, [_P, _P, _P, _I, _A4, _A4, _A4, _I, _I, _I, _I, _I, _P, _I, _I, _F,
                                _P, _P, _P, _P, _I, _A4, _P, _P, _A4, _P, _A4, _I, _P, _A4, _P, _P]),
-    "hq_paged4_append": (_I, [_P, _P, _P, _I, _A4, _A4, _A4, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P,
-                              _I, _F, _P, _I, _I, _F, _P, _P, _A4, _P, _P, _A4, _I, _I, _P, _L, _I, _P,
-                              _A4, _P, _A4, _I, _P, _P]),
+    "hq_paged4_append": (_I, [_S]),
     "hq_paged4_decode_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
-    "hq_paged4_decode": (_I, [_P, _I, _A4, _P, _P, _A4, _P, _P, _A4, _I, _I, _P, _L, _I, _P, _I, _I, _I,
-                              _I, _F, _P, _A4, _P, _Z, _P, _P]),
-    "hq_paged4_gather": (_I, [_P, _P, _A4, _P, _P, _A4, _I, _I, _P, _L, _I, _P, _P, _P, _I, _I, _I, _I,
-                              _P, _P, _I, _A4, _A4, _I, _P, _P]),
+    "hq_paged4_decode": (_I, [_S]),
+    "hq_paged4_gather": (_I, [_S]),
     "hq_packed_prefill_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
-    "hq_packed_prefill": (_I, [_P, _P, _P, _I, _A4, _A4, _A4, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P,
-                               _A4, _I, _P, _Z, _P, _P]),
+    "hq_packed_prefill": (_I, [_S]),
     "hq_read_status": (_I, [_P, _P]),
     "hq_set_plan_sms": (_I, [_I, _I]),
+}
+
+# the entries that take their arguments in a struct: its fields that a call sets, and those of a plan
+ARGS = {
+    "hq_paged4_append": (struct.Struct("@18P4q2f2i"), struct.Struct("@11q11i4x")),
+    "hq_paged4_decode": (struct.Struct("@11P4qf4x"), struct.Struct("@5qN8i")),
+    "hq_paged4_gather": (struct.Struct("@12P4q2i"), struct.Struct("@5q7i4x")),
+    "hq_packed_prefill": (struct.Struct("@9P8qfi"), struct.Struct("@N8i")),
 }
 
 _lib = None
@@ -149,7 +152,7 @@ def check(status: int, what: str) -> None:
 
 @functools.lru_cache(maxsize=8192)
 def _strides_cached(seq: tuple, n: int) -> ctypes.Array:
-    arr = (_i64_4 if n == 4 else _i64_3 if n == 3 else _i64_2)()
+    arr = (_i64_4 if n == 4 else _i64_3)()
     for i, v in enumerate(seq):
         arr[i] = int(v)
     return arr

@@ -889,60 +889,58 @@ extern "C" size_t hq_packed_prefill_workspace_bytes(int T, int Tk, int B, int Hq
   return pk::plan(pl, T, Tk, B, Hkv, Hq / Hkv) ? std::max<size_t>(pl.bytes, 1) : 0;
 }
 
-extern "C" int hq_packed_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t q_strides[2],
-                                 const int64_t k_strides[2], const int64_t v_strides[2], const int* cu_q,
-                                 const int* cu_k, int T, int Tk, int B, int Hq, int Hkv, int D, int causal,
-                                 float sm_scale, void* out, const int64_t out_strides[2], int zero_rest,
-                                 void* workspace, size_t workspace_bytes, int* status, hq_stream_t stream) {
-  if (T < 0 || Tk < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || !q_strides || !k_strides || !v_strides || !out_strides ||
-      !(sm_scale > 0.0f) || !(sm_scale < INFINITY))
+extern "C" int hq_packed_prefill(const hq_packed_prefill_args* args) {
+  if (!args) return HQ_ERR_INVALID_ARGUMENT;
+  const hq_packed_prefill_args& a = *args;
+  if (a.T < 0 || a.Tk < 0 || a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || !(a.sm_scale > 0.0f) || !(a.sm_scale < INFINITY))
     return HQ_ERR_INVALID_ARGUMENT;
-  if (D != pk::kD || Hq % Hkv || (dtype != HQ_DTYPE_BF16 && dtype != HQ_DTYPE_F16)) return HQ_ERR_UNSUPPORTED;
-  if (T == 0 || (B == 0 && !zero_rest)) return HQ_OK;
+  if (a.D != pk::kD || a.Hq % a.Hkv || (a.dtype != HQ_DTYPE_BF16 && a.dtype != HQ_DTYPE_F16)) return HQ_ERR_UNSUPPORTED;
+  if (a.T == 0 || (a.B == 0 && !a.zero_rest)) return HQ_OK;
   auto al = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
-  if (!q || !out || !cu_q || !cu_k || (Tk > 0 && (!k || !v)) || !al(q) || !al(k) || !al(v) || !al(out))
+  if (!a.q || !a.out || !a.cu_q || !a.cu_k || (a.Tk > 0 && (!a.k || !a.v)) || !al(a.q) || !al(a.k) || !al(a.v) || !al(a.out))
     return HQ_ERR_INVALID_ARGUMENT;
-  const int64_t* in[4] = {q_strides, k_strides, v_strides, out_strides};
+  const int64_t* in[4] = {a.q_strides, a.k_strides, a.v_strides, a.out_strides};
   for (const int64_t* s : in)
     if (s[0] % 8 || s[1] % 8 || s[0] < 0 || s[1] < 0) return HQ_ERR_INVALID_ARGUMENT;
-  if ((T > 1 && out_strides[0] == 0) || (Hq > 1 && out_strides[1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
+  if ((a.T > 1 && a.out_strides[0] == 0) || (a.Hq > 1 && a.out_strides[1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
   // TMA takes no stride of 0
-  for (int i = 1; i < 3 && Tk > 0; ++i)
-    if ((Tk > 1 && in[i][0] == 0) || (Hkv > 1 && in[i][1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
+  for (int i = 1; i < 3 && a.Tk > 0; ++i)
+    if ((a.Tk > 1 && in[i][0] == 0) || (a.Hkv > 1 && in[i][1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
   pk::Plan pl{};
-  if (!pk::plan(pl, T, Tk, std::max(B, 1), Hkv, Hq / Hkv)) return HQ_ERR_UNSUPPORTED;
-  if (pl.bytes && (!workspace || workspace_bytes < pl.bytes || !al(workspace))) return HQ_ERR_WORKSPACE;
+  if (!pk::plan(pl, a.T, a.Tk, std::max(a.B, 1), a.Hkv, a.Hq / a.Hkv)) return HQ_ERR_UNSUPPORTED;
+  if (pl.bytes && (!a.workspace || a.workspace_bytes < pl.bytes || !al(a.workspace))) return HQ_ERR_WORKSPACE;
   pk::Params p{};
-  p.q = q;
-  p.out = out;
+  p.q = a.q;
+  p.out = a.out;
   for (int i = 0; i < 2; ++i) {
-    p.qs[i] = q_strides[i];
-    p.os[i] = out_strides[i];
+    p.qs[i] = a.q_strides[i];
+    p.os[i] = a.out_strides[i];
   }
-  p.cu_q = cu_q;
-  p.cu_k = cu_k;
-  p.T = T;
-  p.Tk = Tk;
-  p.B = B;
-  p.Hkv = Hkv;
-  p.nrep = Hq / Hkv;
-  p.causal = causal;
-  p.c = sm_scale * 1.4426950408889634f;
+  p.cu_q = a.cu_q;
+  p.cu_k = a.cu_k;
+  p.T = a.T;
+  p.Tk = a.Tk;
+  p.B = a.B;
+  p.Hkv = a.Hkv;
+  p.nrep = a.Hq / a.Hkv;
+  p.causal = a.causal;
+  p.c = a.sm_scale * 1.4426950408889634f;
   p.n_split = pl.n_split;
   p.units = pl.units;
-  p.zero_rest = zero_rest;
-  p.part = static_cast<float*>(workspace);
-  p.status = status;
+  p.zero_rest = a.zero_rest;
+  p.part = static_cast<float*>(a.workspace);
+  p.status = a.status;
   CUtensorMap km{}, vm{};
-  if (Tk > 0) {
+  if (a.Tk > 0) {
     // strides in rising order, K's and V's alike
-    p.swap = Hkv > 1 && k_strides[1] > k_strides[0];
-    if (Hkv > 1 && (v_strides[1] > v_strides[0]) != (p.swap != 0)) return HQ_ERR_INVALID_ARGUMENT;
-    int64_t ks[2] = {Tk > 1 ? k_strides[0] : int64_t(Hkv) * pk::kD, k_strides[1]}, vs[2] = {Tk > 1 ? v_strides[0] : int64_t(Hkv) * pk::kD, v_strides[1]};
-    int rc = pk::encode(&km, k, dtype, ks, Tk, Hkv, p.swap);
-    if (rc == HQ_OK) rc = pk::encode(&vm, v, dtype, vs, Tk, Hkv, p.swap);
+    p.swap = a.Hkv > 1 && a.k_strides[1] > a.k_strides[0];
+    if (a.Hkv > 1 && (a.v_strides[1] > a.v_strides[0]) != (p.swap != 0)) return HQ_ERR_INVALID_ARGUMENT;
+    const int64_t one = int64_t(a.Hkv) * pk::kD;
+    const int64_t ks[2] = {a.Tk > 1 ? a.k_strides[0] : one, a.k_strides[1]}, vs[2] = {a.Tk > 1 ? a.v_strides[0] : one, a.v_strides[1]};
+    int rc = pk::encode(&km, a.k, a.dtype, ks, a.Tk, a.Hkv, p.swap);
+    if (rc == HQ_OK) rc = pk::encode(&vm, a.v, a.dtype, vs, a.Tk, a.Hkv, p.swap);
     if (rc != HQ_OK) return rc;
   }
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == HQ_DTYPE_BF16 ? pk::launch<HQ_DTYPE_BF16>(p, pl.nt, km, vm, st) : pk::launch<HQ_DTYPE_F16>(p, pl.nt, km, vm, st);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
+  return a.dtype == HQ_DTYPE_BF16 ? pk::launch<HQ_DTYPE_BF16>(p, pl.nt, km, vm, st) : pk::launch<HQ_DTYPE_F16>(p, pl.nt, km, vm, st);
 }

@@ -502,72 +502,62 @@ int launch_append(AppendParams p, cudaStream_t st) {
 
 using namespace hq;
 
-extern "C" int hq_paged4_append(const void* q, const void* k_new, const void* v_new, int x_dtype,
-                                const int64_t q_strides[2], const int64_t k_strides[2],
-                                const int64_t v_strides[2], int T, int B, int Hq, int Hkv, int D,
-                                const int* cu_seqlens, const int* lens, const int* pos_offset,
-                                const void* q_weight, const void* k_weight, int w_dtype, float eps,
-                                const float* inv_freq, int rotary_dim, int interleaved, float factor,
-                                uint8_t* k_codes, uint8_t* v_codes, const int64_t code_strides[2],
-                                void* k_scale, void* v_scale, const int64_t scale_strides[2],
-                                int n_pages, int page_size, const int* tables, int64_t table_stride,
-                                int max_pages, void* q_out, const int64_t qo_strides[2], void* k_out,
-                                const int64_t ko_strides[2], int copy_rest, int* status,
-                                hq_stream_t stream) {
-  if (T < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || rotary_dim < 0 || rotary_dim > D || (rotary_dim > 0 && !inv_freq) ||
-      !q_strides || !k_strides || !v_strides || !qo_strides || (k_out && !ko_strides) || !(eps >= 0.0f) ||
-      (!cu_seqlens && T != B))
+extern "C" int hq_paged4_append(const hq_paged4_append_args* args) {
+  if (!args) return HQ_ERR_INVALID_ARGUMENT;
+  const hq_paged4_append_args& a = *args;
+  if (a.T < 0 || a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.rotary_dim < 0 || a.rotary_dim > a.D ||
+      (a.rotary_dim > 0 && !a.inv_freq) || !(a.eps >= 0.0f) || (!a.cu_seqlens && a.T != a.B))
     return HQ_ERR_INVALID_ARGUMENT;
-  if (D != p4::kD || rotary_dim % 16 || (x_dtype != HQ_DTYPE_BF16 && x_dtype != HQ_DTYPE_F16) ||
-      (w_dtype != x_dtype && w_dtype != HQ_DTYPE_F32) || static_cast<int64_t>(Hq) + 2 * static_cast<int64_t>(Hkv) > 65535)
+  if (a.D != p4::kD || a.rotary_dim % 16 || (a.x_dtype != HQ_DTYPE_BF16 && a.x_dtype != HQ_DTYPE_F16) ||
+      (a.w_dtype != a.x_dtype && a.w_dtype != HQ_DTYPE_F32) || static_cast<int64_t>(a.Hq) + 2 * static_cast<int64_t>(a.Hkv) > 65535)
     return HQ_ERR_UNSUPPORTED;
-  const int rc = p4::check_pages(k_codes, v_codes, k_scale, v_scale, code_strides, scale_strides, n_pages,
-                                 page_size, tables, table_stride, max_pages, B, Hkv);
+  const int rc = p4::check_pages(a.k_codes, a.v_codes, a.k_scale, a.v_scale, a.code_strides, a.scale_strides, a.n_pages,
+                                 a.page_size, a.tables, a.table_stride, a.max_pages, a.B, a.Hkv);
   if (rc != HQ_OK) return rc;
-  if (T == 0 || B == 0) return T == 0 || !copy_rest ? HQ_OK : HQ_ERR_INVALID_ARGUMENT;
-  if (!q || !k_new || !v_new || !q_out || !lens) return HQ_ERR_INVALID_ARGUMENT;
+  if (a.T == 0 || a.B == 0) return a.T == 0 || !a.copy_rest ? HQ_OK : HQ_ERR_INVALID_ARGUMENT;
+  if (!a.q || !a.k_new || !a.v_new || !a.q_out || !a.lens) return HQ_ERR_INVALID_ARGUMENT;
   auto al = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
-  if (!al(q) || !al(k_new) || !al(v_new) || !al(q_out) || !al(k_out)) return HQ_ERR_INVALID_ARGUMENT;
-  if (k_out == k_new) return HQ_ERR_INVALID_ARGUMENT;  // (rows of k are read a second time)
-  const int64_t* all[5] = {q_strides, k_strides, v_strides, qo_strides, k_out ? ko_strides : qo_strides};
+  if (!al(a.q) || !al(a.k_new) || !al(a.v_new) || !al(a.q_out) || !al(a.k_out)) return HQ_ERR_INVALID_ARGUMENT;
+  if (a.k_out == a.k_new) return HQ_ERR_INVALID_ARGUMENT;  // (rows of k are read a second time)
+  const int64_t* all[5] = {a.q_strides, a.k_strides, a.v_strides, a.qo_strides, a.k_out ? a.ko_strides : a.qo_strides};
   for (const int64_t* s : all)
     if (s[0] % 8 || s[1] % 8) return HQ_ERR_INVALID_ARGUMENT;
   // what is written has rows of its own
-  const int heads[2] = {Hq, Hkv};
-  for (int i = 0; i < (k_out ? 2 : 1); ++i)
-    if ((T > 1 && all[3 + i][0] == 0) || (heads[i] > 1 && all[3 + i][1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
+  const int heads[2] = {a.Hq, a.Hkv};
+  for (int i = 0; i < (a.k_out ? 2 : 1); ++i)
+    if ((a.T > 1 && all[3 + i][0] == 0) || (heads[i] > 1 && all[3 + i][1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
   p4::AppendParams p{};
-  p.pg = p4::make_pages(k_codes, v_codes, k_scale, v_scale, code_strides, scale_strides, n_pages, page_size,
-                        tables, table_stride, max_pages);
-  p.q = q;
-  p.k = k_new;
-  p.v = v_new;
+  p.pg = p4::make_pages(a.k_codes, a.v_codes, a.k_scale, a.v_scale, a.code_strides, a.scale_strides, a.n_pages, a.page_size,
+                        a.tables, a.table_stride, a.max_pages);
+  p.q = a.q;
+  p.k = a.k_new;
+  p.v = a.v_new;
   for (int i = 0; i < 2; ++i) {
-    p.qs[i] = q_strides[i];
-    p.ks[i] = k_strides[i];
-    p.vs[i] = v_strides[i];
-    p.qos[i] = qo_strides[i];
-    p.kos[i] = k_out ? ko_strides[i] : 0;
+    p.qs[i] = a.q_strides[i];
+    p.ks[i] = a.k_strides[i];
+    p.vs[i] = a.v_strides[i];
+    p.qos[i] = a.qo_strides[i];
+    p.kos[i] = a.k_out ? a.ko_strides[i] : 0;
   }
-  p.T = T;
-  p.B = B;
-  p.Hq = Hq;
-  p.Hkv = Hkv;
-  p.cu = cu_seqlens;
-  p.lens = lens;
-  p.pos_offset = pos_offset;
-  p.qw = q_weight;
-  p.kw = k_weight;
-  p.w_f32 = w_dtype == HQ_DTYPE_F32;
-  p.eps = eps;
-  p.inv_freq = inv_freq;
-  p.rot = rotary_dim;
-  p.inter = interleaved;
-  p.factor = factor;
-  p.q_out = q_out;
-  p.k_out = k_out;
-  p.copy_rest = copy_rest;
-  p.status = status;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return x_dtype == HQ_DTYPE_BF16 ? p4::launch_append<HQ_DTYPE_BF16>(p, st) : p4::launch_append<HQ_DTYPE_F16>(p, st);
+  p.T = a.T;
+  p.B = a.B;
+  p.Hq = a.Hq;
+  p.Hkv = a.Hkv;
+  p.cu = a.cu_seqlens;
+  p.lens = a.lens;
+  p.pos_offset = a.pos_offset;
+  p.qw = a.q_weight;
+  p.kw = a.k_weight;
+  p.w_f32 = a.w_dtype == HQ_DTYPE_F32;
+  p.eps = a.eps;
+  p.inv_freq = a.inv_freq;
+  p.rot = a.rotary_dim;
+  p.inter = a.interleaved;
+  p.factor = a.factor;
+  p.q_out = a.q_out;
+  p.k_out = a.k_out;
+  p.copy_rest = a.copy_rest;
+  p.status = a.status;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
+  return a.x_dtype == HQ_DTYPE_BF16 ? p4::launch_append<HQ_DTYPE_BF16>(p, st) : p4::launch_append<HQ_DTYPE_F16>(p, st);
 }

@@ -777,49 +777,46 @@ extern "C" size_t hq_paged4_decode_workspace_bytes(int B, int Hq, int Hkv, int p
   return p4::plan_decode(pl, B, Hkv, Hq / Hkv, int64_t(page_size) * max_pages) ? pl.bytes : 0;
 }
 
-extern "C" int hq_paged4_decode(const void* q, int q_dtype, const int64_t q_strides[2], const uint8_t* k_codes,
-                                const uint8_t* v_codes, const int64_t code_strides[2], const void* k_scale,
-                                const void* v_scale, const int64_t scale_strides[2], int n_pages, int page_size,
-                                const int* tables, int64_t table_stride, int max_pages, const int* lens, int B,
-                                int Hq, int Hkv, int D, float sm_scale, void* out, const int64_t out_strides[2],
-                                void* workspace, size_t workspace_bytes, int* status, hq_stream_t stream) {
-  if (B < 0 || Hq <= 0 || Hkv <= 0 || !q_strides || !out_strides) return HQ_ERR_INVALID_ARGUMENT;
-  if (D != p4::kD || Hq % Hkv || (q_dtype != HQ_DTYPE_BF16 && q_dtype != HQ_DTYPE_F16)) return HQ_ERR_UNSUPPORTED;
-  const int rc = p4::check_pages(k_codes, v_codes, k_scale, v_scale, code_strides, scale_strides, n_pages,
-                                 page_size, tables, table_stride, max_pages, B, Hkv);
+extern "C" int hq_paged4_decode(const hq_paged4_decode_args* args) {
+  if (!args) return HQ_ERR_INVALID_ARGUMENT;
+  const hq_paged4_decode_args& a = *args;
+  if (a.B < 0 || a.Hq <= 0 || a.Hkv <= 0) return HQ_ERR_INVALID_ARGUMENT;
+  if (a.D != p4::kD || a.Hq % a.Hkv || (a.q_dtype != HQ_DTYPE_BF16 && a.q_dtype != HQ_DTYPE_F16)) return HQ_ERR_UNSUPPORTED;
+  const int rc = p4::check_pages(a.k_codes, a.v_codes, a.k_scale, a.v_scale, a.code_strides, a.scale_strides, a.n_pages,
+                                 a.page_size, a.tables, a.table_stride, a.max_pages, a.B, a.Hkv);
   if (rc != HQ_OK) return rc;
-  if (B == 0) return HQ_OK;
-  auto al = [](const void* x, uintptr_t a) { return reinterpret_cast<uintptr_t>(x) % a == 0; };
-  if (!q || !out || !lens || !al(q, 16) || !al(out, 8) || q_strides[0] % 8 || q_strides[1] % 8 ||
-      out_strides[0] % 4 || out_strides[1] % 4 || (B > 1 && out_strides[0] == 0) || (Hq > 1 && out_strides[1] == 0))
+  if (a.B == 0) return HQ_OK;
+  auto al = [](const void* x, uintptr_t n) { return reinterpret_cast<uintptr_t>(x) % n == 0; };
+  if (!a.q || !a.out || !a.lens || !al(a.q, 16) || !al(a.out, 8) || a.q_strides[0] % 8 || a.q_strides[1] % 8 ||
+      a.out_strides[0] % 4 || a.out_strides[1] % 4 || (a.B > 1 && a.out_strides[0] == 0) || (a.Hq > 1 && a.out_strides[1] == 0))
     return HQ_ERR_INVALID_ARGUMENT;
   p4::DecodePlan pl{};
-  if (!p4::plan_decode(pl, B, Hkv, Hq / Hkv, int64_t(page_size) * max_pages) || int64_t(B) * Hq > 0x7fffffff)
+  if (!p4::plan_decode(pl, a.B, a.Hkv, a.Hq / a.Hkv, int64_t(a.page_size) * a.max_pages) || int64_t(a.B) * a.Hq > 0x7fffffff)
     return HQ_ERR_UNSUPPORTED;
-  if (!pl.by_unit && (!workspace || workspace_bytes < pl.bytes || !al(workspace, 256))) return HQ_ERR_WORKSPACE;
+  if (!pl.by_unit && (!a.workspace || a.workspace_bytes < pl.bytes || !al(a.workspace, 256))) return HQ_ERR_WORKSPACE;
   p4::DecodeParams p{};
-  p.pg = p4::make_pages(k_codes, v_codes, k_scale, v_scale, code_strides, scale_strides, n_pages, page_size,
-                        tables, table_stride, max_pages);
-  p.q = q;
-  p.out = out;
+  p.pg = p4::make_pages(a.k_codes, a.v_codes, a.k_scale, a.v_scale, a.code_strides, a.scale_strides, a.n_pages, a.page_size,
+                        a.tables, a.table_stride, a.max_pages);
+  p.q = a.q;
+  p.out = a.out;
   for (int i = 0; i < 2; ++i) {
-    p.qs[i] = q_strides[i];
-    p.os[i] = out_strides[i];
+    p.qs[i] = a.q_strides[i];
+    p.os[i] = a.out_strides[i];
   }
-  p.B = B;
-  p.Hkv = Hkv;
-  p.nrep = Hq / Hkv;
+  p.B = a.B;
+  p.Hkv = a.Hkv;
+  p.nrep = a.Hq / a.Hkv;
   p.n_rt = pl.n_rt;
-  p.lens = lens;
-  p.qk_scale = sm_scale * 1.4426950408889634f;
+  p.lens = a.lens;
+  p.qk_scale = a.sm_scale * 1.4426950408889634f;
   if (!pl.by_unit) {
-    p.cum = static_cast<int*>(workspace);
-    p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.cum_bytes);
-    p.ends = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.cum_bytes + pl.part_bytes);
+    p.cum = static_cast<int*>(a.workspace);
+    p.part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + pl.cum_bytes);
+    p.ends = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + pl.cum_bytes + pl.part_bytes);
   }
   p.grid = pl.grid;
   p.by_unit = pl.by_unit;
-  p.status = status;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return pl.nt == 1 ? p4::launch_decode<1>(p, q_dtype, pl, st) : p4::launch_decode<2>(p, q_dtype, pl, st);
+  p.status = a.status;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
+  return pl.nt == 1 ? p4::launch_decode<1>(p, a.q_dtype, pl, st) : p4::launch_decode<2>(p, a.q_dtype, pl, st);
 }

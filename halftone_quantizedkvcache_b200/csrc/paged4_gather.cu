@@ -97,53 +97,49 @@ __global__ void __launch_bounds__(kGThreads) gather_kernel(const __grid_constant
 
 using namespace hq;
 
-extern "C" int hq_paged4_gather(const uint8_t* k_codes, const uint8_t* v_codes, const int64_t code_strides[2],
-                                const void* k_scale, const void* v_scale, const int64_t scale_strides[2],
-                                int n_pages, int page_size, const int* tables, int64_t table_stride,
-                                int max_pages, const int* lens, const int* first, const int* cu_seqlens,
-                                int T, int B, int Hkv, int D, void* k_out, void* v_out, int out_dtype,
-                                const int64_t k_strides[2], const int64_t v_strides[2], int zero_rest,
-                                int* status, hq_stream_t stream) {
-  if (T < 0 || B < 0 || Hkv <= 0 || !k_strides || !v_strides || !cu_seqlens) return HQ_ERR_INVALID_ARGUMENT;
-  if (D != p4::kD || (out_dtype != HQ_DTYPE_BF16 && out_dtype != HQ_DTYPE_F16) || Hkv > 65535) return HQ_ERR_UNSUPPORTED;
-  const int rc = p4::check_pages(k_codes, v_codes, k_scale, v_scale, code_strides, scale_strides, n_pages,
-                                 page_size, tables, table_stride, max_pages, B, Hkv);
+extern "C" int hq_paged4_gather(const hq_paged4_gather_args* args) {
+  if (!args) return HQ_ERR_INVALID_ARGUMENT;
+  const hq_paged4_gather_args& a = *args;
+  if (a.T < 0 || a.B < 0 || a.Hkv <= 0 || !a.cu_seqlens) return HQ_ERR_INVALID_ARGUMENT;
+  if (a.D != p4::kD || (a.out_dtype != HQ_DTYPE_BF16 && a.out_dtype != HQ_DTYPE_F16) || a.Hkv > 65535) return HQ_ERR_UNSUPPORTED;
+  const int rc = p4::check_pages(a.k_codes, a.v_codes, a.k_scale, a.v_scale, a.code_strides, a.scale_strides, a.n_pages,
+                                 a.page_size, a.tables, a.table_stride, a.max_pages, a.B, a.Hkv);
   if (rc != HQ_OK) return rc;
-  if (T == 0) return HQ_OK;
+  if (a.T == 0) return HQ_OK;
   auto al = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
-  if (!k_out || !v_out || k_out == v_out || (B > 0 && !lens) || !al(k_out) || !al(v_out) || k_strides[0] % 8 || k_strides[1] % 8 ||
-      v_strides[0] % 8 || v_strides[1] % 8)
+  if (!a.k_out || !a.v_out || a.k_out == a.v_out || (a.B > 0 && !a.lens) || !al(a.k_out) || !al(a.v_out) ||
+      a.k_strides[0] % 8 || a.k_strides[1] % 8 || a.v_strides[0] % 8 || a.v_strides[1] % 8)
     return HQ_ERR_INVALID_ARGUMENT;
-  const int64_t* w[2] = {k_strides, v_strides};
+  const int64_t* w[2] = {a.k_strides, a.v_strides};
   for (const int64_t* s : w)
-    if ((T > 1 && s[0] == 0) || (Hkv > 1 && s[1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
+    if ((a.T > 1 && s[0] == 0) || (a.Hkv > 1 && s[1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
   p4::GatherParams p{};
-  p.pg = p4::make_pages(k_codes, v_codes, k_scale, v_scale, code_strides, scale_strides, n_pages, page_size,
-                        tables, table_stride, max_pages);
-  p.T = T;
-  p.B = B;
-  p.Hkv = Hkv;
-  p.cu = cu_seqlens;
-  p.lens = lens;
-  p.first = first;
-  p.k_out = k_out;
-  p.v_out = v_out;
+  p.pg = p4::make_pages(a.k_codes, a.v_codes, a.k_scale, a.v_scale, a.code_strides, a.scale_strides, a.n_pages, a.page_size,
+                        a.tables, a.table_stride, a.max_pages);
+  p.T = a.T;
+  p.B = a.B;
+  p.Hkv = a.Hkv;
+  p.cu = a.cu_seqlens;
+  p.lens = a.lens;
+  p.first = a.first;
+  p.k_out = a.k_out;
+  p.v_out = a.v_out;
   for (int i = 0; i < 2; ++i) {
-    p.ks[i] = k_strides[i];
-    p.vs[i] = v_strides[i];
+    p.ks[i] = a.k_strides[i];
+    p.vs[i] = a.v_strides[i];
   }
-  p.zero_rest = zero_rest;
-  p.status = status;
-  const int64_t blocks = (static_cast<int64_t>(T) + p4::kGRows - 1) / p4::kGRows;
+  p.zero_rest = a.zero_rest;
+  p.status = a.status;
+  const int64_t blocks = (static_cast<int64_t>(a.T) + p4::kGRows - 1) / p4::kGRows;
   // a row's heads stay together as long as that leaves 4 blocks an SM
   const int64_t want = std::max<int64_t>(1, 4LL * current_sm_count() / blocks);
-  const int groups = static_cast<int>(std::min<int64_t>(Hkv, want));
-  p.heads_per_block = (Hkv + groups - 1) / groups;
-  p.groups = (Hkv + p.heads_per_block - 1) / p.heads_per_block;
+  const int groups = static_cast<int>(std::min<int64_t>(a.Hkv, want));
+  p.heads_per_block = (a.Hkv + groups - 1) / groups;
+  p.groups = (a.Hkv + p.heads_per_block - 1) / p.heads_per_block;
   if (blocks * p.groups > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   const unsigned grid = static_cast<unsigned>(blocks * p.groups);
-  if (out_dtype == HQ_DTYPE_BF16) p4::gather_kernel<HQ_DTYPE_BF16><<<grid, p4::kGThreads, 0, st>>>(p);
+  if (a.out_dtype == HQ_DTYPE_BF16) p4::gather_kernel<HQ_DTYPE_BF16><<<grid, p4::kGThreads, 0, st>>>(p);
   else p4::gather_kernel<HQ_DTYPE_F16><<<grid, p4::kGThreads, 0, st>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? HQ_OK : static_cast<int>(e);

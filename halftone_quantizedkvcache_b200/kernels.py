@@ -1486,6 +1486,10 @@ def rope_append_kv(q, k_new, v_new, inv_freq, k_cache, v_cache, k_sc, v_sc_cache
 
 # ---------------------------------------------------------------- paged cache in 4 bits
 PAGED4_SIZES = (16, 32, 64, 128, 256)
+_APPEND, _APPEND_PLAN = _lib.ARGS["hq_paged4_append"]
+_DECODE, _DECODE_PLAN = _lib.ARGS["hq_paged4_decode"]
+_GATHER, _GATHER_PLAN = _lib.ARGS["hq_paged4_gather"]
+_PREFILL, _PREFILL_PLAN = _lib.ARGS["hq_packed_prefill"]
 
 
 def paged4_alloc(n_pages: int, n_kv_heads: int, *, page_size: int = 64, head_dim: int = 128,
@@ -1511,8 +1515,8 @@ def paged4_alloc(n_pages: int, n_kv_heads: int, *, page_size: int = 64, head_dim
 
 
 def _paged4_cache(what: str, cache: dict, tables, B: int, dev):
-    """Checks a paged cache and its block tables; returns (Hkv, page size, C arguments after the
-    codes' and scales' pointers: strides, page count, page size; table stride, pages per table)."""
+    """Checks a paged cache and its block tables; returns (Hkv, strides of codes' and scales'
+    pages and heads and of the tables' rows, page count, page size, pages per table)."""
     try:
         k, v, ks, vs = cache["k"], cache["v"], cache["k_scale"], cache["v_scale"]
     except (TypeError, KeyError):
@@ -1547,8 +1551,7 @@ def _paged4_cache(what: str, cache: dict, tables, B: int, dev):
                          f"{tables.dtype} {tuple(tables.shape)}")
     if tables.shape[1] * page > 1 << 30:
         raise ValueError(f"{what}: a table of more than 2^30 tokens")
-    return (Hkv, _lib.strides(cs[:2], 2), _lib.strides(ss[:2], 2), P, page, max(tables.stride(0), 0),
-            tables.shape[1])
+    return Hkv, (*cs[:2], *ss[:2], max(tables.stride(0), 0)), P, page, tables.shape[1]
 
 
 def _paged4_key(cache: dict, tables) -> tuple:
@@ -1635,7 +1638,7 @@ def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None
         if lens.dim() != 1:
             raise ValueError(f"{what}: lens must be int32 [B]")
         B = lens.shape[0]
-        Hkv, *pages = _paged4_cache(what, cache, block_tables, B, dev)
+        Hkv, pst, n_pages, page, max_pages = _paged4_cache(what, cache, block_tables, B, dev)
         _packed(what, "k_new", k_new, dev, q.dtype, T, Hkv)
         _packed(what, "v_new", v_new, dev, q.dtype, T, Hkv)
         _lens_ok(what, "lens", lens, B, dev)
@@ -1662,12 +1665,13 @@ def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None
                 raise ValueError(f"{what}: inv_freq must be contiguous float32 on q's device, for a "
                                  f"rotary_dim of 16, 32, .. {D}")
         in_place = _rows_strided(q) and _rows_strided(k_new) and _rows_strided(v_new)
-        plan = _keep(key, (dev, T, B, Hq, Hkv, in_place, q.is_contiguous(), _DT[q.dtype],
-                           _DT[wdt or q.dtype], rot,
-                           *[_lib.strides(x.stride()[:2], 2) for x in (q, k_new, v_new)], *pages,
-                           _lib.strides((Hq * D, D), 2), _lib.lib().hq_paged4_append))
-    (dev, T, B, Hq, Hkv, in_place, dense, dt, wdt, rot, qst, kst, vst, cst, sst, n_pages, page, tst,
-     max_pages, ost, fn) = plan
+        rows = (pst, (T, B, Hq, Hkv, D, _DT[q.dtype], _DT[wdt or q.dtype], rot, n_pages, page, max_pages))
+
+        def tail(*x):
+            return _APPEND_PLAN.pack(*[st for t in x for st in t.stride()[:2]], *rows[0], *rows[1])
+        plan = _keep(key, (dev, T, B, Hkv, in_place, q.is_contiguous(), (Hq * D, D),
+                           tail(q, k_new, v_new) if in_place else b"", tail, _lib.lib().hq_paged4_append))
+    dev, T, B, Hkv, in_place, dense, ost, args, tail, fn = plan
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return paged4_append(q, k_new, v_new, cache, block_tables, lens, cu_seqlens=cu_seqlens,
@@ -1679,34 +1683,33 @@ def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None
     qp, kp, vp = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr()
     if not in_place or (qp | kp | vp) % 16:  # rows that the kernel cannot read in place
         q, k_new, v_new = _aligned_rows(q), _aligned_rows(k_new), _aligned_rows(v_new)
-        qst, kst, vst = (_lib.strides(x.stride()[:2], 2) for x in (q, k_new, v_new))
+        args = tail(q, k_new, v_new)
         qp, kp, vp = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr()
     rest = q_out is None
     if rest:
         q_out = torch.empty_like(q) if dense else q.new_empty(q.shape)
     else:
         _packed_out(what, "q_out", q_out, q.shape, q)
-        ost = _lib.strides(q_out.stride()[:2], 2)
-    kop, kost = None, None
+        ost = q_out.stride()[:2]
+    kop, kost = 0, ost
     if k_out is not None:
         _packed_out(what, "k_out", k_out, (T, Hkv, 128), q)
-        kop, kost = k_out.data_ptr(), _lib.strides(k_out.stride()[:2], 2)
+        kop, kost = k_out.data_ptr(), k_out.stride()[:2]
         if T and kop == kp:
             raise ValueError(f"{what}: k_out must not be k_new")
     if T == 0:
         return q_out
     if B == 0:
         return q_out.copy_(q) if rest else q_out
-    rc = fn(qp, kp, vp, dt, qst, kst, vst, T, B, Hq, Hkv, 128,
-            cu_seqlens.data_ptr() if cu_seqlens is not None else None, lens.data_ptr(),
-            pos_offset.data_ptr() if pos_offset is not None else None,
-            q_weight.data_ptr() if q_weight is not None else None,
-            k_weight.data_ptr() if k_weight is not None else None, wdt, eps,
-            inv_freq.data_ptr() if rot else None, rot, 1 if interleaved else 0, factor,
-            cache["k"].data_ptr(), cache["v"].data_ptr(), cst, cache["k_scale"].data_ptr(),
-            cache["v_scale"].data_ptr(), sst, n_pages, page, block_tables.data_ptr(), tst, max_pages,
-            q_out.data_ptr(), ost, kop, kost, 1 if rest else 0, _status_word(dev).data_ptr(),
-            _stream(dev))
+    rc = fn(_APPEND.pack(
+        qp, kp, vp, cu_seqlens.data_ptr() if cu_seqlens is not None else 0, lens.data_ptr(),
+        pos_offset.data_ptr() if pos_offset is not None else 0,
+        q_weight.data_ptr() if q_weight is not None else 0,
+        k_weight.data_ptr() if k_weight is not None else 0,
+        inv_freq.data_ptr() if inv_freq is not None else 0, cache["k"].data_ptr(), cache["v"].data_ptr(),
+        cache["k_scale"].data_ptr(), cache["v_scale"].data_ptr(), block_tables.data_ptr(),
+        q_out.data_ptr(), kop, _status_word(dev).data_ptr(), _stream(dev), *ost, *kost, eps, factor,
+        1 if interleaved else 0, 1 if rest else 0) + args)
     if rc:
         check(rc, "hq_paged4_append")
     return q_out
@@ -1741,20 +1744,20 @@ def paged4_decode_attn(q, cache, block_tables, lens, *, sm_scale=None, out=None)
             raise ValueError(f"{what}: q must be [B,Hq,128] or [B,Hq,1,128], got {tuple(q.shape)}")
         B, Hq, D = q.shape[0], q.shape[1], 128
         dev = q.device
-        Hkv, *pages = _paged4_cache(what, cache, block_tables, B, dev)
+        Hkv, pst, n_pages, page, max_pages = _paged4_cache(what, cache, block_tables, B, dev)
         _attn_common(what, q, Hq, Hkv)
         _lens_ok(what, "lens", lens, B, dev)
         qb = q if q.dim() == 3 else q[:, :, 0]
         in_place = _rows_strided(qb)
-        ost = _lib.strides((Hq * D, D), 2)
+        ost = (Hq * D, D)
         with _on_device(dev):
             nb = _ws_size(what, dev, _lib.lib().hq_paged4_decode_workspace_bytes(
-                max(B, 1), Hq, Hkv, pages[3], pages[5], D))
-        plan = _keep(key, (dev, (B, Hq, D), q.shape, in_place and q.is_contiguous(), _DT[q.dtype],
-                           _lib.strides(qb.stride()[:2], 2) if in_place else ost, in_place, Hkv, *pages,
-                           nb, (nb + 3) // 4, ost, 1.0 / math.sqrt(D), _lib.lib().hq_paged4_decode))
-    (dev, (B, Hq, D), shape, dense, dt, qst, in_place, Hkv, cst, sst, n_pages, page, tst, max_pages, nb,
-     nw, ost, default_scale, fn) = plan
+                max(B, 1), Hq, Hkv, page, max_pages, D))
+        args = _DECODE_PLAN.pack(*pst, nb, B, Hq, Hkv, D, _DT[q.dtype], n_pages, page, max_pages)
+        plan = _keep(key, (dev, (B, Hq, D), q.shape, in_place and q.is_contiguous(),
+                           qb.stride()[:2] if in_place else ost, in_place, (nb + 3) // 4 if nb > 1 else 0,
+                           ost, 1.0 / math.sqrt(D), args, _lib.lib().hq_paged4_decode))
+    dev, rows, shape, dense, qst, in_place, nw, ost, default_scale, args, fn = plan
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return paged4_decode_attn(q, cache, block_tables, lens, sm_scale=sm_scale, out=out)
@@ -1764,20 +1767,20 @@ def paged4_decode_attn(q, cache, block_tables, lens, *, sm_scale=None, out=None)
         qp = q.data_ptr()
     if out is None:
         out = torch.empty_like(q) if dense else q.new_empty(shape)
-        ost = _lib.strides((Hq * D, D), 2)
     else:
-        _out_like(what, out, (B, Hq, D), q)
+        _out_like(what, out, rows, q)
         if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
             raise ValueError(f"{what}: out must have rows of its own")
-        ost = _lib.strides(out.stride()[:2], 2)
-    if B == 0:
+        ost = out.stride()[:2]
+    if rows[0] == 0:
         return out
     status = _status_word(dev)
-    ws = status.new_empty(nw) if nb > 1 else None  # (1: none is needed)
-    rc = fn(qp, dt, qst, cache["k"].data_ptr(), cache["v"].data_ptr(), cst, cache["k_scale"].data_ptr(),
-            cache["v_scale"].data_ptr(), sst, n_pages, page, block_tables.data_ptr(), tst, max_pages,
-            lens.data_ptr(), B, Hq, Hkv, D, default_scale if sm_scale is None else sm_scale,
-            out.data_ptr(), ost, ws.data_ptr() if nb > 1 else None, nb, status.data_ptr(), _stream(dev))
+    ws = status.new_empty(nw) if nw else None
+    rc = fn(_DECODE.pack(
+        qp, cache["k"].data_ptr(), cache["v"].data_ptr(), cache["k_scale"].data_ptr(),
+        cache["v_scale"].data_ptr(), block_tables.data_ptr(), lens.data_ptr(), out.data_ptr(),
+        ws.data_ptr() if nw else 0, status.data_ptr(), _stream(dev), *qst, *ost,
+        default_scale if sm_scale is None else sm_scale) + args)
     if rc:
         check(rc, "hq_paged4_decode")
     return out
@@ -1823,13 +1826,14 @@ def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, 
         if lens.dim() != 1:
             raise ValueError(f"{what}: lens must be int32 [B]")
         B = lens.shape[0]
-        Hkv, *pages = _paged4_cache(what, cache, block_tables, B, dev)
+        Hkv, pst, n_pages, page, max_pages = _paged4_cache(what, cache, block_tables, B, dev)
         _lens_ok(what, "lens", lens, B, dev)
         _lens_ok(what, "cu_seqlens", cu_seqlens, B + 1, dev)
         _lens_ok(what, "first", first, B, dev)
-        plan = _keep(key, (dev, rows, B, Hkv, *pages, _lib.strides((Hkv * 128, 128), 2),
+        plan = _keep(key, (dev, rows, Hkv, (Hkv * 128, 128),
+                           _GATHER_PLAN.pack(*pst, rows, B, Hkv, 128, n_pages, page, max_pages),
                            _lib.lib().hq_paged4_gather))
-    dev, rows, B, Hkv, cst, sst, n_pages, page, tst, max_pages, ost, fn = plan
+    dev, rows, Hkv, ost, args, fn = plan
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, first=first, dtype=dtype,
@@ -1837,7 +1841,8 @@ def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, 
     kst = vst = ost
     made = k_out is None and v_out is None
     if made:
-        k_out, v_out = lens.new_empty((2, rows, Hkv, 128), dtype=dtype).unbind(0)
+        k_out = torch.empty_strided((rows, Hkv, 128), (*ost, 1), dtype=dtype, device=dev)
+        v_out = torch.empty_like(k_out)
     else:
         if k_out is None or v_out is None:
             raise ValueError(f"{what}: k_out and v_out come together")
@@ -1851,14 +1856,15 @@ def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, 
             _packed_out(what, n, t, (rows, Hkv, 128), k_out)
         if rows and k_out.data_ptr() == v_out.data_ptr():
             raise ValueError(f"{what}: k_out and v_out must have memory of their own")
-        kst, vst = _lib.strides(k_out.stride()[:2], 2), _lib.strides(v_out.stride()[:2], 2)
+        kst, vst = k_out.stride()[:2], v_out.stride()[:2]
     if rows == 0:
         return k_out, v_out
-    rc = fn(cache["k"].data_ptr(), cache["v"].data_ptr(), cst, cache["k_scale"].data_ptr(),
-            cache["v_scale"].data_ptr(), sst, n_pages, page, block_tables.data_ptr(), tst, max_pages,
-            lens.data_ptr(), first.data_ptr() if first is not None else None, cu_seqlens.data_ptr(),
-            rows, B, Hkv, 128, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype], kst, vst,
-            1 if made else 0, _status_word(dev).data_ptr(), _stream(dev))
+    rc = fn(_GATHER.pack(
+        cache["k"].data_ptr(), cache["v"].data_ptr(), cache["k_scale"].data_ptr(),
+        cache["v_scale"].data_ptr(), block_tables.data_ptr(), lens.data_ptr(),
+        first.data_ptr() if first is not None else 0, cu_seqlens.data_ptr(), k_out.data_ptr(),
+        v_out.data_ptr(), _status_word(dev).data_ptr(), _stream(dev), *kst, *vst, _DT[dtype],
+        1 if made else 0) + args)
     if rc:
         check(rc, "hq_paged4_gather")
     return k_out, v_out
@@ -1908,12 +1914,13 @@ def packed_prefill_attn(q, k, v, cu_q, cu_k=None, *, causal=True, sm_scale=None,
         with _on_device(dev):
             nb = 1 if T == 0 or B == 0 else _ws_size(what, dev, _lib.lib().hq_packed_prefill_workspace_bytes(
                 T, Tk, B, Hq, Hkv, D))
-        plan = _keep(key, (dev, T, Tk, B, Hq, Hkv, _DT[q.dtype], 1 if causal else 0, _rows_strided(q), q.is_contiguous(),
+        args = _PREFILL_PLAN.pack(nb, T, Tk, B, Hq, Hkv, D, _DT[q.dtype], 1 if causal else 0)
+        plan = _keep(key, (dev, T, B, _rows_strided(q), q.is_contiguous(),
                            tma(k) and tma(v) and rising[0] == rising[1],
-                           *[_lib.strides(x.stride()[:2], 2) for x in (q, k, v)], nb, (nb + 3) // 4,
-                           _lib.strides((Hq * D, D), 2), 1.0 / math.sqrt(D), _lib.lib().hq_packed_prefill))
-    (dev, T, Tk, B, Hq, Hkv, dt, causal, q_ok, dense, kv_ok, qst, kst, vst, nb, nw, ost, default_scale,
-     fn) = plan
+                           *[x.stride()[:2] for x in (q, k, v)], (nb + 3) // 4 if nb > 1 else 0,
+                           (T, Hq, D), (Hq * D, D), 1.0 / math.sqrt(D), args,
+                           _lib.lib().hq_packed_prefill))
+    (dev, T, B, q_ok, dense, kv_ok, qst, kst, vst, nw, shape, ost, default_scale, args, fn) = plan
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return packed_prefill_attn(q, k, v, cu_q, cu_k, causal=causal, sm_scale=sm_scale, out=out)
@@ -1922,26 +1929,26 @@ def packed_prefill_attn(q, k, v, cu_q, cu_k=None, *, causal=True, sm_scale=None,
     elif not 0 < sm_scale < math.inf:
         raise ValueError(f"{what}: sm_scale must be positive and finite")
     if not q_ok or q.data_ptr() % 16:  # rows that the kernel cannot read in place
-        q = q.clone(memory_format=torch.contiguous_format)
-        qst = _lib.strides(q.stride()[:2], 2)
+        q, qst = q.clone(memory_format=torch.contiguous_format), ost
     if not kv_ok or (k.data_ptr() | v.data_ptr()) % 16:
         k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
-        kst, vst = (_lib.strides(t.stride()[:2], 2) for t in (k, v))
+        kst, vst = k.stride()[:2], v.stride()[:2]
     rest = out is None
     if rest:
-        out = torch.empty_like(q) if dense else q.new_empty((T, Hq, 128))
+        out = torch.empty_like(q) if dense else q.new_empty(shape)
     else:
-        _packed_out(what, "out", out, (T, Hq, 128), q)
-        ost = _lib.strides(out.stride()[:2], 2)
+        _packed_out(what, "out", out, shape, q)
+        ost = out.stride()[:2]
     if T == 0:
         return out
     if B == 0:
         return out.zero_() if rest else out
     status = _status_word(dev)
-    ws = status.new_empty(nw) if nb > 1 else None  # (1: none is needed)
-    rc = fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, qst, kst, vst, cu_q.data_ptr(),
-            cu_k.data_ptr(), T, Tk, B, Hq, Hkv, 128, causal, sm_scale, out.data_ptr(), ost,
-            1 if rest else 0, ws.data_ptr() if nb > 1 else None, nb, status.data_ptr(), _stream(dev))
+    ws = status.new_empty(nw) if nw else None
+    rc = fn(_PREFILL.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
+        ws.data_ptr() if nw else 0, status.data_ptr(), _stream(dev), *qst, *kst, *vst, *ost, sm_scale,
+        1 if rest else 0) + args)
     if rc:
         check(rc, "hq_packed_prefill")
     return out

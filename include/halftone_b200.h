@@ -694,43 +694,77 @@ HQ_API int hq_rope_append_kv(
  *   (hq_packed_prefill_workspace_bytes, 16-byte aligned; 1: none is needed, 0:
  *   unsupported) holds partial states where keys are split over blocks.
  */
-HQ_API int hq_paged4_append(const void* q, const void* k_new, const void* v_new, int x_dtype,
-                            const int64_t q_strides[2], const int64_t k_strides[2],
-                            const int64_t v_strides[2], int T, int B, int Hq, int Hkv, int D,
-                            const int* cu_seqlens, const int* lens, const int* pos_offset,
-                            const void* q_weight, const void* k_weight, int w_dtype, float eps,
-                            const float* inv_freq, int rotary_dim, int interleaved, float factor,
-                            uint8_t* k_codes, uint8_t* v_codes, const int64_t code_strides[2],
-                            void* k_scale, void* v_scale, const int64_t scale_strides[2],
-                            int n_pages, int page_size, const int* tables, int64_t table_stride,
-                            int max_pages, void* q_out, const int64_t qo_strides[2], void* k_out,
-                            const int64_t ko_strides[2], int copy_rest, int* status,
-                            hq_stream_t stream);
+/* Their arguments come in a struct (by name; and a caller through a foreign-function
+ * interface pays for each argument of a call).  Every field is set, unused pointers
+ * to NULL. */
+typedef struct hq_paged4_append_args {
+  const void *q, *k_new, *v_new;
+  const int *cu_seqlens, *lens, *pos_offset;
+  const void *q_weight, *k_weight;
+  const float* inv_freq;
+  uint8_t *k_codes, *v_codes;
+  void *k_scale, *v_scale;
+  const int* tables;
+  void *q_out, *k_out;
+  int* status;
+  hq_stream_t stream;
+  int64_t qo_strides[2], ko_strides[2];
+  float eps, factor;
+  int interleaved, copy_rest;
+  int64_t q_strides[2], k_strides[2], v_strides[2];
+  int64_t code_strides[2], scale_strides[2], table_stride;
+  int T, B, Hq, Hkv, D, x_dtype, w_dtype, rotary_dim, n_pages, page_size, max_pages, pad;
+} hq_paged4_append_args;
+
+typedef struct hq_paged4_decode_args {
+  const void* q;
+  const uint8_t *k_codes, *v_codes;
+  const void *k_scale, *v_scale;
+  const int *tables, *lens;
+  void *out, *workspace;
+  int* status;
+  hq_stream_t stream;
+  int64_t q_strides[2], out_strides[2];
+  float sm_scale;
+  int pad;
+  int64_t code_strides[2], scale_strides[2], table_stride;
+  size_t workspace_bytes;
+  int B, Hq, Hkv, D, q_dtype, n_pages, page_size, max_pages;
+} hq_paged4_decode_args;
+
+typedef struct hq_paged4_gather_args {
+  const uint8_t *k_codes, *v_codes;
+  const void *k_scale, *v_scale;
+  const int *tables, *lens, *first, *cu_seqlens;
+  void *k_out, *v_out;
+  int* status;
+  hq_stream_t stream;
+  int64_t k_strides[2], v_strides[2];
+  int out_dtype, zero_rest;
+  int64_t code_strides[2], scale_strides[2], table_stride;
+  int T, B, Hkv, D, n_pages, page_size, max_pages, pad;
+} hq_paged4_gather_args;
+
+typedef struct hq_packed_prefill_args {
+  const void *q, *k, *v;
+  const int *cu_q, *cu_k;
+  void *out, *workspace;
+  int* status;
+  hq_stream_t stream;
+  int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2];
+  float sm_scale;
+  int zero_rest;
+  size_t workspace_bytes;
+  int T, Tk, B, Hq, Hkv, D, dtype, causal;
+} hq_packed_prefill_args;
+
+HQ_API int hq_paged4_append(const hq_paged4_append_args* args);
 HQ_API size_t hq_paged4_decode_workspace_bytes(int B, int Hq, int Hkv, int page_size, int max_pages,
                                                int D);
-HQ_API int hq_paged4_decode(const void* q, int q_dtype, const int64_t q_strides[2],
-                            const uint8_t* k_codes, const uint8_t* v_codes,
-                            const int64_t code_strides[2], const void* k_scale, const void* v_scale,
-                            const int64_t scale_strides[2], int n_pages, int page_size,
-                            const int* tables, int64_t table_stride, int max_pages, const int* lens,
-                            int B, int Hq, int Hkv, int D, float sm_scale, void* out,
-                            const int64_t out_strides[2], void* workspace, size_t workspace_bytes,
-                            int* status, hq_stream_t stream);
-HQ_API int hq_paged4_gather(const uint8_t* k_codes, const uint8_t* v_codes,
-                            const int64_t code_strides[2], const void* k_scale, const void* v_scale,
-                            const int64_t scale_strides[2], int n_pages, int page_size,
-                            const int* tables, int64_t table_stride, int max_pages, const int* lens,
-                            const int* first, const int* cu_seqlens, int T, int B, int Hkv, int D,
-                            void* k_out, void* v_out, int out_dtype, const int64_t k_strides[2],
-                            const int64_t v_strides[2], int zero_rest, int* status,
-                            hq_stream_t stream);
+HQ_API int hq_paged4_decode(const hq_paged4_decode_args* args);
+HQ_API int hq_paged4_gather(const hq_paged4_gather_args* args);
 HQ_API size_t hq_packed_prefill_workspace_bytes(int T, int Tk, int B, int Hq, int Hkv, int D);
-HQ_API int hq_packed_prefill(const void* q, const void* k, const void* v, int dtype,
-                             const int64_t q_strides[2], const int64_t k_strides[2],
-                             const int64_t v_strides[2], const int* cu_q, const int* cu_k, int T,
-                             int Tk, int B, int Hq, int Hkv, int D, int causal, float sm_scale,
-                             void* out, const int64_t out_strides[2], int zero_rest, void* workspace,
-                             size_t workspace_bytes, int* status, hq_stream_t stream);
+HQ_API int hq_packed_prefill(const hq_packed_prefill_args* args);
 
 /* ------------------------------------------------------------------------
  * Reads (and synchronises `stream` for) the device status word at the start

@@ -799,12 +799,13 @@ inline bool plan(Plan& pl, int64_t T, int64_t Tk, int B, int Hkv, int nrep) {
   if (T * nrep > 0x3fffffff || Tk > 0x3fffffff) return false;
   const int sms = current_sm_count();
   // One row tile a block where sequences are short, in rows and in keys: 64 sequences of up to 200
-  // tokens 52 us against 60, one of 512 16.4 against 17.2; with more of either, K and V are better
-  // shared: one of 2048 39 us against 40, 2 x 8192 467 against 529, 3 x 77 queries over 4022 keys 22
-  // against 25.
+  // tokens 50 us against 54, one of 512 14.6 against 15.4 (8 of 512 34 against 31); with more of either, K
+  // and V are better shared: one of 2048 38 us against 40, 2 x 8192 465 against 529, 3 x 77 queries over
+  // 4022 keys 23 against 26.
   pl.nt = T * nrep <= 1024LL * B && Tk <= 1024LL * B ? 1 : 2;
   const int rows = 128 * pl.nt;
-  const int64_t units = ((T * nrep + rows - 1) / rows + B) * Hkv;
+  // n rows are (n - 1) / rows + 1 pieces, rounded down; so are all sequences' at most
+  const int64_t full = std::min<int64_t>(B, T), units = ((T * nrep - full) / rows + full) * Hkv;
   if (units * kMaxSplit > 0x7fffffff) return false;
   // With fewer blocks than fit the GPU each piece's keys go to several, down to 4 key tiles of an average
   // sequence a block (3 x 77 queries over 4022 keys: 57 us unsplit, 22 split; one of 512: 16.4 unsplit,

@@ -20,7 +20,7 @@
 // through shared memory (the next row in registers instead: 179 us).
 //
 // 8 x 4096 tokens of 16 q heads and 8 kv heads, both norms, full rotation, k kept: 124 us, 4.1 TB/s of
-// bytes moved.  Bound by issue slots (65 % of them taken; arithmetic units 39 %, DRAM 31 % at half that
+// bytes moved.  Bound by issue slots (70 % of them taken; arithmetic units 45 %, DRAM 36 % at half that
 // size): for a lane and row of k a reduction of 128 squares, the turn and the codes.  (8 lanes a row, both
 // values of a pair in one lane, take 27 % fewer instructions but 96 registers: 131 us, the 20 warps an SM hide
 // less.)

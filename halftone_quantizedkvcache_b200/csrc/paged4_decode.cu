@@ -325,9 +325,10 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
     const int row0 = (cur.idx - kvh * p.n_rt) * C::kRows;
     const int b = cur.e, len = cur.len;
     const bool whole = t0 == 0 && t1 == cur.nt;
-    // B fragments of q: columns 2 r, 2 r + 1 are the upper two digits of row r (first product), 2 r the
-    // lowest (second); a lane's bytes are the channels 8 c4 + {0, 2, 4, 6} and + {1, 3, 5, 7} of a group
-    uint32_t bq[NT][4][2][2];
+    // B fragments of q: columns 2 r, 2 r + 1 are the upper two digits of row 4 nt + r (a product for each
+    // nt), 2 r + nt its lowest (one more); a lane's bytes are the channels 8 c4 + {0, 2, 4, 6} and
+    // + {1, 3, 5, 7} of a group
+    uint32_t bq[NT][4][2], bl[4][2] = {};
     int off[NT][4];                       // -8 sum(q) of row c4
     float qk[NT];
 #pragma unroll
@@ -361,19 +362,28 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int x = __float2int_rn(f[e] * fix), y = (x + 128) >> 8, z = (y + 128) >> 8;
-          const uint32_t d = (n8 & 1 ? y - 256 * z : z) & 0xff, d0 = n8 & 1 ? 0 : (x - 256 * y) & 0xff;
+          const uint32_t d = (n8 & 1 ? y - 256 * z : z) & 0xff, d0 = (x - 256 * y) & 0xff;
           top[e & 1] |= d << (8 * (e >> 1));
           low[e & 1] |= d0 << (8 * (e >> 1));
         }
-        bq[nt][g][0][0] = top[0];
-        bq[nt][g][0][1] = top[1];
-        bq[nt][g][1][0] = low[0];
-        bq[nt][g][1][1] = low[1];
-        constexpr uint32_t k8 = 0x08080808u;
-        int u[4], w[4];
-        mma_u8s8(u, k8, k8, k8, k8, top[0], top[1], kZero);
-        mma_u8s8(w, k8, k8, k8, k8, low[0], low[1], kZero);
-        off[nt][g] = -((u[0] * 256 + u[1]) * 256 + w[0]);
+        bq[nt][g][0] = top[0];
+        bq[nt][g][1] = top[1];
+        if ((n8 & 1) == nt) {
+          bl[g][0] = low[0];
+          bl[g][1] = low[1];
+        }
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      constexpr uint32_t k8 = 0x08080808u;
+      int w[4];
+      mma_u8s8(w, k8, k8, k8, k8, bl[g][0], bl[g][1], kZero);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        int u[4];
+        mma_u8s8(u, k8, k8, k8, k8, bq[nt][g][0], bq[nt][g][1], kZero);
+        off[nt][g] = -((u[0] * 256 + u[1]) * 256 + w[nt]);
       }
     }
     float m_run[NT], l_run[NT], o[NT][4][2][2];
@@ -420,14 +430,15 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
         for (int g = 0; g < 4; ++g) {
           constexpr uint32_t kLow = 0x0f0f0f0fu;
           const uint32_t x0 = a0[g] & kLow, x1 = (a0[g] >> 4) & kLow, y0 = a1[g] & kLow, y1 = (a1[g] >> 4) & kLow;
+          int w[4];
+          mma_u8s8(w, x0, y0, x1, y1, bl[g][0], bl[g][1], kZero);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            int u[4], w[4];
-            mma_u8s8(u, x0, y0, x1, y1, bq[nt][g][0][0], bq[nt][g][0][1], kZero);
-            mma_u8s8(w, x0, y0, x1, y1, bq[nt][g][1][0], bq[nt][g][1][1], kZero);
+            int u[4];
+            mma_u8s8(u, x0, y0, x1, y1, bq[nt][g][0], bq[nt][g][1], kZero);
             // 32 x 8 x 2^21 is 2^29: whole numbers all the way
-            sc[nt][2 * blk] = __fmaf_rn(s0[g], static_cast<float>((u[0] * 256 + u[1]) * 256 + (w[0] + off[nt][g])), sc[nt][2 * blk]);
-            sc[nt][2 * blk + 1] = __fmaf_rn(s1[g], static_cast<float>((u[2] * 256 + u[3]) * 256 + (w[2] + off[nt][g])), sc[nt][2 * blk + 1]);
+            sc[nt][2 * blk] = __fmaf_rn(s0[g], static_cast<float>((u[0] * 256 + u[1]) * 256 + (w[nt] + off[nt][g])), sc[nt][2 * blk]);
+            sc[nt][2 * blk + 1] = __fmaf_rn(s1[g], static_cast<float>((u[2] * 256 + u[3]) * 256 + (w[2 + nt] + off[nt][g])), sc[nt][2 * blk + 1]);
           }
         }
         const int tk = blk * 16 + slot_tok;

@@ -7,7 +7,7 @@
 // what crosses a block's border leaves partial states (m, l, o) that join_kernel puts together, always
 // in the order of the line.
 //
-// 64 sequences of 4096 to 8192 tokens, 8 kv heads of 2 rows: 105 us, 4.3 TB/s of cache.  What holds it
+// 64 sequences of 4096 to 8192 tokens, 8 kv heads of 2 rows: 103 us, 4.4 TB/s of cache.  What holds it
 // back is the work between loads (issue slots 49 %, arithmetic units 44 %, the matrix units 25 %, DRAM 49 %
 // at half that size): 144 bytes a token and head are 256 codes to unpack, twice.  Both products are
 // whole-number products on bytes (mma.sync m16n8k32, exact), the codes being the 16-row operand, since a
@@ -61,7 +61,7 @@ struct DecodeParams {
 
 template <int NT>
 struct Cfg {
-  // 64 x 8192 tokens: 105 us; 12 warps of 168 registers 113 (spilled), tiles of 32 tokens 113
+  // 64 x 8192 tokens: 103 us; 9 to 12 warps, their registers spilled, 113 to 123, tiles of 32 tokens 113
   static constexpr int kWarps = 8;
   static constexpr int kStages = 2;
   static constexpr int kRows = 4 * NT;

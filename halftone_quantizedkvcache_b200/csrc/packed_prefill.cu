@@ -17,7 +17,8 @@
 // (2^-9 of each weight in bf16, 2^-12 in float16: what the output itself is rounded by; in float16 also
 // 2^-32 of the largest).
 //
-// 2 x 8192 tokens of 16 q heads and 8 kv heads, bf16: 465 us, 1180 TFLOP/s.  Neither unit is full (1 x 8192:
+// 2 x 8192 tokens of 16 q heads and 8 kv heads, bf16: 454 us, 1210 TFLOP/s in a burst (530 in a
+// run of calls, at 990 W and 1.64 GHz).  Neither unit is full (1 x 8192:
 // tensor 57 %, exponentials 58 %, issue slots 37 %): a row tile's scores, softmax and products follow one
 // another, and two tiles a block leave gaps where both wait.  (Two threads a row 549 us; a quarter of the
 // exponentials as polynomials no change, half of them 513.)
@@ -51,7 +52,7 @@ struct Cfg {
   static constexpr int kRows = 128 * NT;
   // Softmax threads: one a row with 128 keys, or (one row tile, where nothing hides a step's length) two with
   // 64 each, which tell each other their maxima.  One tile: 64 sequences of up to 200 tokens 52 us with two,
-  // 57 with one; one of 512 15.2 and 16.5.  Two tiles: 2 x 8192 549 us with two, 465 with one.
+  // 57 with one; one of 512 15.2 and 16.5.  Two tiles: 2 x 8192 549 us with two, 460 with one.
   static constexpr int kH = NT == 1 ? 2 : 1, kKeys = 128 / kH;
   static_assert(NT * kH <= 2, "places for one pair of threads a row");
   static constexpr int kSoft = 128 * NT * kH, kThreads = kSoft + 128;
@@ -62,7 +63,7 @@ struct Cfg {
   static constexpr int kOffKv = NT * kTileB;            // behind the Q tiles
   static constexpr int kOffBar = kOffKv + kStages * kTileB;
   static constexpr int kFull = 0, kEmpty = kFull + kStages, kSFull = kEmpty + kStages, kPFull = kSFull + NT,
-                       kOFull = kPFull + 2 * NT, kPair = kOFull + NT, kClean = kPair + 4, kDrain = kClean + 2, kBars = kDrain + 1;
+                       kOFull = kPFull + 2 * NT, kPair = kOFull + NT, kClean = kPair + 4, kDrain = kClean + 2, kQ = kDrain + 1, kBars = kQ + 1;
   static constexpr int kOffBad = kOffBar + (kBars * 8 + 15) / 16 * 16;  // [2][4] words of spoiled V rows
   static constexpr int kOffHalf = kOffBad + 32;          // [2][kH][128] what the threads of a row tell each other
   static constexpr int kOffMisc = kOffHalf + (kH == 2 ? 2048 : 0);
@@ -82,6 +83,7 @@ struct Params {
   float c;                                // sm_scale log2(e)
   int n_split, units;                     // units: an upper bound of (sequence, piece of its rows, kv head)
   int swap;                               // tensor maps: (channel, token, head) instead of (channel, head, token)
+  int q_tma;                              // Q tiles by tensor map: n_rep divides 128
   int zero_rest;
   float* part;
   int* status;
@@ -275,7 +277,8 @@ __device__ __forceinline__ int limit_of(const Params& p, const Seq& s, int r) {
 
 template <int DT, int NT>
 __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
-    packed_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm) {
+    packed_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                  const __grid_constant__ CUtensorMap vm) {
   using C = Cfg<NT>;
   constexpr int kRows = C::kRows, kThreads = C::kThreads, kStages = C::kStages, kSoftWarps = C::kSoft / 32;
   extern __shared__ unsigned char smem_raw[];
@@ -325,6 +328,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
     for (int i = 0; i < 4; ++i) mbar_init(&bar[C::kPair + i], 2);
     for (int i = 0; i < 2; ++i) mbar_init(&bar[C::kClean + i], kCleanWarps);
     mbar_init(&bar[C::kDrain], 1);
+    mbar_init(&bar[C::kQ], 1);
     fence_mbar_init();
   }
   __syncthreads();
@@ -357,27 +361,40 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&misc[8])), "r"(C::kCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  auto box = [&](const CUtensorMap* map, unsigned char* to, int x, int y, int z, uint64_t* full) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(to)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(full))
+        : "memory");
+  };
   // K and V tiles, in turn
   const int copies = 2 * (j1 - j0);
   auto copy = [&](int n) {
     const int st = n % kStages;
-    unsigned char* to = smem + C::kOffKv + st * kTileB;
-    const CUtensorMap* map = n & 1 ? &vm : &km;
     const int key = s.k0 + (j0 + (n >> 1)) * kBN;
     mbar_arrive_expect_tx(&bar[C::kFull + st], kTileB);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      asm volatile(
-          "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-              smem_u32(to + h * (kBN * 128))),
-          "l"(reinterpret_cast<uint64_t>(map)), "r"(64 * h), "r"(p.swap ? key : kvh), "r"(p.swap ? kvh : key),
-          "r"(smem_u32(&bar[C::kFull + st]))
-          : "memory");
+      box(n & 1 ? &vm : &km, smem + C::kOffKv + st * kTileB + h * (kBN * 128), 64 * h, p.swap ? key : kvh, p.swap ? kvh : key,
+          &bar[C::kFull + st]);
   };
-  if (warp == kSoftWarps + 1 && lane == 0)
+  if (warp == kSoftWarps + 1 && lane == 0) {
+    if (p.q_tma && copies) {  // 128 / n_rep queries a tile, all heads of each: its rows in order
+      const int tiles = (rows + 127) / 128;
+      mbar_arrive_expect_tx(&bar[C::kQ], tiles * kTileB);
+      for (int t = 0; t < tiles; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          box(&qm, smem + t * kTileB + h * (kBN * 128), 64 * h, kvh * p.nrep, s.q0 + (row0 + 128 * t) / p.nrep, &bar[C::kQ]);
+    }
     for (int n = 0; n < min(copies, kStages); ++n) copy(n);
-  // Q, 16 lanes a row: K-major tiles of two 64-channel halves, 128-byte swizzle; rows past the last: zeros
-  {
+  }
+  // Q, 16 lanes a row: K-major tiles of two 64-channel halves, 128-byte swizzle; rows past the last: zeros.
+  // (By tensor
+  // map, where n_rep divides 128, a block starts up to 1.5 us earlier: 64 sequences of up to 200 tokens 46 us
+  // against 50, 2 x 8192 454 against 460.  Rows past the last are then whatever follows: no row sees another.)
+  if (!p.q_tma) {
     constexpr int kEach = (kRows * 16 + kThreads - 1) / kThreads;
     static_assert(kThreads % 16 == 0, "a half-warp per row");
     uint4 v[kEach];
@@ -628,6 +645,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
     };
     if (j0 < j1) {
       ok = wait_bar(&bar[C::kFull], 0);
+      if (p.q_tma) ok = ok && wait_bar(&bar[C::kQ], 0);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
 #pragma unroll
@@ -675,7 +693,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
     // ------------------------------------------------------------ copies
     int n = min(copies, kStages);
     if (lane == 0) {
-      for (; n < copies; ++n) {
+      if (p.q_tma && copies) ok = wait_bar(&bar[C::kQ], 0);
+      for (; ok && n < copies; ++n) {
         const int st = n % kStages;
         if (!(ok = wait_bar(&bar[C::kEmpty + st], (n / kStages - 1) & 1))) break;
         copy(n);
@@ -800,7 +819,7 @@ inline bool plan(Plan& pl, int64_t T, int64_t Tk, int B, int Hkv, int nrep) {
   const int sms = current_sm_count();
   // One row tile a block where sequences are short, in rows and in keys: 64 sequences of up to 200
   // tokens 50 us against 54, one of 512 14.6 against 15.4 (8 of 512 34 against 31); with more of either, K
-  // and V are better shared: one of 2048 38 us against 40, 2 x 8192 465 against 529, 3 x 77 queries over
+  // and V are better shared: one of 2048 38 us against 40, 2 x 8192 460 against 529, 3 x 77 queries over
   // 4022 keys 23 against 26.
   pl.nt = T * nrep <= 1024LL * B && Tk <= 1024LL * B ? 1 : 2;
   const int rows = 128 * pl.nt;
@@ -818,14 +837,15 @@ inline bool plan(Plan& pl, int64_t T, int64_t Tk, int B, int Hkv, int nrep) {
   return true;
 }
 
-// [T, H, 128] in boxes of 128 tokens x 64 channels, 128-byte swizzle, zeros past the end
-inline int encode(CUtensorMap* m, const void* base, int dt, const int64_t st[2], int T, int H, int swap) {
+// [T, H, 128] in boxes of 64 channels, 128-byte swizzle, zeros past the end: of 128 tokens of a head, or of
+// n_rep heads of 128 / n_rep tokens
+inline int encode(CUtensorMap* m, const void* base, int dt, const int64_t st[2], int T, int H, int swap, int heads) {
   auto enc = dec::encode_fn();
   if (!enc) return HQ_ERR_UNSUPPORTED;
   const cuuint64_t ts = 2 * st[0], hs = H > 1 ? 2 * st[1] : (swap ? 2 * st[0] : 2 * kD);
   const cuuint64_t dims[3] = {kD, static_cast<cuuint64_t>(swap ? T : H), static_cast<cuuint64_t>(swap ? H : T)};
   const cuuint64_t strides[2] = {swap ? ts : hs, swap ? hs : ts};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(swap ? kBN : 1), static_cast<cuuint32_t>(swap ? 1 : kBN)};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(swap ? kBN : heads), static_cast<cuuint32_t>(swap ? 1 : kBN / heads)};
   const cuuint32_t es[3] = {1, 1, 1};
   const CUresult r = enc(m, dt == HQ_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                          const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -834,7 +854,7 @@ inline int encode(CUtensorMap* m, const void* base, int dt, const int64_t st[2],
 }
 
 template <int DT, int NT>
-int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+int launch(const Params& p, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
   using C = Cfg<NT>;
   static std::atomic<uint64_t> ready{0};
   auto kern = packed_kernel<DT, NT>;
@@ -854,7 +874,7 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, cudaSt
     }();
     if (!fits) return HQ_ERR_UNSUPPORTED;
   }
-  kern<<<p.units * p.n_split, C::kThreads, C::kSmem, st>>>(p, km, vm);
+  kern<<<p.units * p.n_split, C::kThreads, C::kSmem, st>>>(p, qm, km, vm);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.n_split == 1) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};
@@ -875,8 +895,8 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, cudaSt
   return HQ_OK;
 }
 template <int DT>
-int launch(const Params& p, int nt, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
-  return nt == 1 ? launch<DT, 1>(p, km, vm, st) : launch<DT, 2>(p, km, vm, st);
+int launch(const Params& p, int nt, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+  return nt == 1 ? launch<DT, 1>(p, qm, km, vm, st) : launch<DT, 2>(p, qm, km, vm, st);
 }
 
 }  // namespace pk
@@ -931,17 +951,22 @@ extern "C" int hq_packed_prefill(const hq_packed_prefill_args* args) {
   p.zero_rest = a.zero_rest;
   p.part = static_cast<float*>(a.workspace);
   p.status = a.status;
-  CUtensorMap km{}, vm{};
+  CUtensorMap qm{}, km{}, vm{};
   if (a.Tk > 0) {
     // strides in rising order, K's and V's alike
     p.swap = a.Hkv > 1 && a.k_strides[1] > a.k_strides[0];
     if (a.Hkv > 1 && (a.v_strides[1] > a.v_strides[0]) != (p.swap != 0)) return HQ_ERR_INVALID_ARGUMENT;
     const int64_t one = int64_t(a.Hkv) * pk::kD;
     const int64_t ks[2] = {a.Tk > 1 ? a.k_strides[0] : one, a.k_strides[1]}, vs[2] = {a.Tk > 1 ? a.v_strides[0] : one, a.v_strides[1]};
-    int rc = pk::encode(&km, a.k, a.dtype, ks, a.Tk, a.Hkv, p.swap);
-    if (rc == HQ_OK) rc = pk::encode(&vm, a.v, a.dtype, vs, a.Tk, a.Hkv, p.swap);
+    int rc = pk::encode(&km, a.k, a.dtype, ks, a.Tk, a.Hkv, p.swap, 1);
+    if (rc == HQ_OK) rc = pk::encode(&vm, a.v, a.dtype, vs, a.Tk, a.Hkv, p.swap, 1);
+    // Q's rows in order come by tensor map: heads within tokens, no strides of 0
+    const int64_t qs[2] = {a.T > 1 ? a.q_strides[0] : int64_t(a.Hq) * pk::kD, a.q_strides[1]};
+    p.q_tma = 128 % p.nrep == 0 && qs[0] > 0 && (a.Hq == 1 || (qs[1] > 0 && qs[1] <= qs[0]));
+    if (rc == HQ_OK && p.q_tma) rc = pk::encode(&qm, a.q, a.dtype, qs, a.T, a.Hq, 0, p.nrep);
     if (rc != HQ_OK) return rc;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
-  return a.dtype == HQ_DTYPE_BF16 ? pk::launch<HQ_DTYPE_BF16>(p, pl.nt, km, vm, st) : pk::launch<HQ_DTYPE_F16>(p, pl.nt, km, vm, st);
+  return a.dtype == HQ_DTYPE_BF16 ? pk::launch<HQ_DTYPE_BF16>(p, pl.nt, qm, km, vm, st)
+                                  : pk::launch<HQ_DTYPE_F16>(p, pl.nt, qm, km, vm, st);
 }

@@ -164,3 +164,17 @@ def test_many_small_weights_beside_a_large_one(dtype, n, m):
     err = (out.transpose(0, 1).double() - ref).abs()
     assert float(ref.min()) > 0.05
     assert not (~(err <= half * ref.abs() * 1.01 + (half + 2.0 ** -13) * mag + 2.0 ** -32 * m * 4096)).any(), float(err.max())
+
+
+def test_queries_that_share_memory_and_neighbours_that_are_no_numbers():
+    from halftone_quantizedkvcache_b200 import kernels
+    nq = [5, 130, 60]
+    for rep in (2, 3, 128):
+        q, k, v = make(nq, nq, 1, rep, torch.bfloat16, 9)
+        for shared in (q[:, :1].expand_as(q), q[:1].expand_as(q)):
+            out = kernels.packed_prefill_attn(shared, k, v, cum(nq))
+            assert torch.equal(out, kernels.packed_prefill_attn(shared.contiguous(), k, v, cum(nq)))
+        out = kernels.packed_prefill_attn(q, k, v, cum(nq))
+        q[5:135], k[5:135], v[5:135] = math.nan, math.inf, math.nan
+        bad = kernels.packed_prefill_attn(q, k, v, cum(nq))
+        assert torch.equal(bad[:5], out[:5]) and torch.equal(bad[135:], out[135:]) and bad[5:135].isnan().all()

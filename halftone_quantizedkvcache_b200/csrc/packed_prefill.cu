@@ -818,10 +818,10 @@ inline bool plan(Plan& pl, int64_t T, int64_t Tk, int B, int Hkv, int nrep) {
   if (T * nrep > 0x3fffffff || Tk > 0x3fffffff) return false;
   const int sms = current_sm_count();
   // One row tile a block where sequences are short, in rows and in keys: 64 sequences of up to 200
-  // tokens 50 us against 54, one of 512 14.6 against 15.4 (8 of 512 34 against 31); with more of either, K
-  // and V are better shared: one of 2048 38 us against 40, 2 x 8192 460 against 529, 3 x 77 queries over
-  // 4022 keys 23 against 26.
-  pl.nt = T * nrep <= 1024LL * B && Tk <= 1024LL * B ? 1 : 2;
+  // tokens 45 us against 50 (32 of up to 300, 4 q heads a kv head, 85 and 85); with more of either, K and V
+  // are better shared: 8 of 512 29 us against 32 (one of 512 14.7 and 14.4), one of 2048 38 against 40,
+  // 2 x 8192 460 against 529, 3 x 77 queries over 4022 keys 23 against 26.
+  pl.nt = T * nrep <= 512LL * B && Tk <= 1024LL * B ? 1 : 2;
   const int rows = 128 * pl.nt;
   // n rows are (n - 1) / rows + 1 pieces, rounded down; so are all sequences' at most
   const int64_t full = std::min<int64_t>(B, T), units = ((T * nrep - full) / rows + full) * Hkv;

@@ -178,3 +178,17 @@ def test_queries_that_share_memory_and_neighbours_that_are_no_numbers():
         q[5:135], k[5:135], v[5:135] = math.nan, math.inf, math.nan
         bad = kernels.packed_prefill_attn(q, k, v, cum(nq))
         assert torch.equal(bad[:5], out[:5]) and torch.equal(bad[135:], out[135:]) and bad[5:135].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n,m", [(250, 250), (4, 1024), (5, 1000), (256, 1024)])
+def test_short_sequences_with_a_maximum_that_keeps_growing(dtype, n, m):
+    # blocks of one row tile, a row's keys shared by two threads; their keys split over blocks or not
+    from halftone_quantizedkvcache_b200 import kernels
+    q, k, v = make([n], [m], 1, 2, DT[dtype], 26)
+    for ramp in (torch.linspace(-30, 30, m, device="cuda"), torch.linspace(30, -30, m, device="cuda")):
+        k[:, 0, 0] = ramp.to(k.dtype)
+        q[..., 0] = 20.0
+        # (sum |q k| up to 700, as above)
+        check(kernels.packed_prefill_attn(q, k, v, cum([n]), cum([m])), q, k, v, [n], [m])
+    assert kernels.ragged_status() == 0

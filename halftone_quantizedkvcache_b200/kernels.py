@@ -1617,10 +1617,10 @@ def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None
     try:
         key = (what, q.shape, q.stride(), q.dtype, q.get_device(), k_new.shape, k_new.stride(),
                k_new.dtype, k_new.get_device(), v_new.shape, v_new.stride(), v_new.dtype,
-               v_new.get_device(), lens.shape, lens.stride(), lens.dtype, lens.get_device())
-        key += _paged4_key(cache, block_tables)
-        for t in (cu_seqlens, inv_freq, pos_offset, q_weight, k_weight):
-            key += _sig_opt(t)
+               v_new.get_device(), lens.shape, lens.stride(), lens.dtype, lens.get_device(),
+               _paged4_key(cache, block_tables),
+               *[None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+                 for t in (cu_seqlens, inv_freq, pos_offset, q_weight, k_weight)])
     except (AttributeError, TypeError, KeyError):
         _tensors(what, q=q, k_new=k_new, v_new=v_new, lens=lens)
         for t, n in ((cu_seqlens, "cu_seqlens"), (inv_freq, "inv_freq"), (pos_offset, "pos_offset"),
@@ -1730,8 +1730,7 @@ def paged4_decode_attn(q, cache, block_tables, lens, *, sm_scale=None, out=None)
     what = "paged4_decode_attn"
     try:
         key = (what, q.shape, q.stride(), q.dtype, q.get_device(), lens.shape, lens.stride(), lens.dtype,
-               lens.get_device())
-        key += _paged4_key(cache, block_tables)
+               lens.get_device(), _paged4_key(cache, block_tables))
     except (AttributeError, TypeError, KeyError):
         _tensors(what, q=q, lens=lens)
         _paged4_cache(what, cache, block_tables, q.shape[0] if q.dim() else 0, q.device)
@@ -1802,9 +1801,8 @@ def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, 
     what = "paged4_gather"
     try:
         key = (what, n_rows, dtype, lens.shape, lens.stride(), lens.dtype, lens.get_device(),
-               cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.get_device())
-        key += _paged4_key(cache, block_tables)
-        key += _sig_opt(first)
+               cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.get_device(),
+               _paged4_key(cache, block_tables), _sig_opt(first))
     except (AttributeError, TypeError, KeyError):
         _tensors(what, lens=lens, cu_seqlens=cu_seqlens)
         if first is not None:

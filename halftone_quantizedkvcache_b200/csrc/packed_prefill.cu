@@ -960,11 +960,11 @@ extern "C" int hq_packed_prefill(const hq_packed_prefill_args* args) {
     const int64_t ks[2] = {a.Tk > 1 ? a.k_strides[0] : one, a.k_strides[1]}, vs[2] = {a.Tk > 1 ? a.v_strides[0] : one, a.v_strides[1]};
     int rc = pk::encode(&km, a.k, a.dtype, ks, a.Tk, a.Hkv, p.swap, 1);
     if (rc == HQ_OK) rc = pk::encode(&vm, a.v, a.dtype, vs, a.Tk, a.Hkv, p.swap, 1);
+    if (rc != HQ_OK) return rc;
     // Q's rows in order come by tensor map: heads within tokens, no strides of 0
     const int64_t qs[2] = {a.T > 1 ? a.q_strides[0] : int64_t(a.Hq) * pk::kD, a.q_strides[1]};
-    p.q_tma = 128 % p.nrep == 0 && qs[0] > 0 && (a.Hq == 1 || (qs[1] > 0 && qs[1] <= qs[0]));
-    if (rc == HQ_OK && p.q_tma) rc = pk::encode(&qm, a.q, a.dtype, qs, a.T, a.Hq, 0, p.nrep);
-    if (rc != HQ_OK) return rc;
+    p.q_tma = 128 % p.nrep == 0 && qs[0] > 0 && (a.Hq == 1 || (qs[1] > 0 && qs[1] <= qs[0])) &&
+              pk::encode(&qm, a.q, a.dtype, qs, a.T, a.Hq, 0, p.nrep) == HQ_OK;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   return a.dtype == HQ_DTYPE_BF16 ? pk::launch<HQ_DTYPE_BF16>(p, pl.nt, qm, km, vm, st)

@@ -1576,6 +1576,9 @@ def _packed(what: str, name: str, t, dev, dtype, rows=None, heads=None) -> None:
 
 
 def _packed_out(what: str, name: str, t, shape, q) -> None:
+    if type(t) is torch.Tensor and t.shape == shape and t.stride() == (shape[1] * 128, 128, 1) and (
+            t.dtype == q.dtype and t.get_device() == q.get_device() and t.data_ptr() % 16 == 0):
+        return  # (the usual one, in a microsecond less)
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape) or t.dtype != q.dtype or (
             t.device != q.device) or not _rows_ok(t):
         raise ValueError(f"{what}: {name} must be {tuple(shape)} of q's dtype and device, with "

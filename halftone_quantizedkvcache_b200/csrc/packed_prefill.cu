@@ -754,7 +754,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
 
 // Joins the pieces of a row tile, in order: block (piece of the line and kv head, 32 rows, 16 channels), a
 // warp 8 rows, 4 lanes a row, 4 channels each: one round of loads.
-template <int DT, int MOST>  // MOST: pieces at most (16 held the small calls up for 10 us)
+template <int DT, int MOST>  // MOST: pieces at most (7 pieces with room for 16: 3 x 77 over 4022 22 us against 19)
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p, int rows) {
   __shared__ int found[6];
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -826,12 +826,21 @@ inline bool plan(Plan& pl, int64_t T, int64_t Tk, int B, int Hkv, int nrep) {
   // n rows are (n - 1) / rows + 1 pieces, rounded down; so are all sequences' at most
   const int64_t full = std::min<int64_t>(B, T), units = ((T * nrep - full) / rows + full) * Hkv;
   if (units * kMaxSplit > 0x7fffffff) return false;
-  // With fewer blocks than fit the GPU each piece's keys go to several, down to 4 key tiles of an average
-  // sequence a block (3 x 77 queries over 4022 keys: 57 us unsplit, 22 split; one of 512: 16.4 unsplit,
-  // 17.2 in two).
-  const int64_t room = (3 - pl.nt) * sms;
-  pl.n_split = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, room / std::max<int64_t>(units, 1)),
-                                                   std::max<int64_t>(1, Tk / (4 * kBN * std::max<int64_t>(B, 1))), kMaxSplit}));
+  // With fewer blocks than fit the GPU each piece's keys go to several, as many as make the estimated time
+  // least: 2 us a key tile of an average sequence; for more than one 3 us of a second launch (more than 8: 5.5), and
+  // 0.15 ns a row and part for the states.  (Unsplit and split: 3 x 77 queries over 4022 keys 57 us and 19; 4 x 16 over 800 21
+  // and 14; one of 1000 with 8 q heads over 2 kv heads 22 and 18; one of 512 14.7 and 16.1, 2 of 784 18.5 and
+  // 20.3, which stay whole.)
+  const int64_t room = sms / std::max<int64_t>(units, 1);
+  const int64_t tiles = (Tk + kBN * static_cast<int64_t>(B) - 1) / (kBN * static_cast<int64_t>(B));
+  int64_t best = INT64_MAX;
+  for (int64_t n = 1; n <= std::max<int64_t>(1, std::min<int64_t>({room, tiles, kMaxSplit})); ++n) {
+    const int64_t ns = 2000 * ((tiles + n - 1) / n) + (n > 1 ? 3000 + 3 * T * nrep * Hkv * n / 20 : 0) + (n > 8 ? 2500 : 0);
+    if (ns < best) {
+      best = ns;
+      pl.n_split = static_cast<int>(n);
+    }
+  }
   pl.units = static_cast<int>(units);
   pl.bytes = pl.n_split > 1 ? sizeof(float) * static_cast<size_t>(units) * pl.n_split * rows * kPartRow : 0;
   return true;
@@ -886,8 +895,9 @@ int launch(const Params& p, const CUtensorMap& qm, const CUtensorMap& km, const 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = p.n_split <= 4 ? cudaLaunchKernelEx(&cfg, join_kernel<DT, 4>, p, C::kRows)
-                     : cudaLaunchKernelEx(&cfg, join_kernel<DT, kMaxSplit>, p, C::kRows);
+  e = p.n_split <= 4   ? cudaLaunchKernelEx(&cfg, join_kernel<DT, 4>, p, C::kRows)
+      : p.n_split <= 8 ? cudaLaunchKernelEx(&cfg, join_kernel<DT, 8>, p, C::kRows)
+                       : cudaLaunchKernelEx(&cfg, join_kernel<DT, kMaxSplit>, p, C::kRows);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return static_cast<int>(e);

@@ -566,6 +566,11 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
       ok = ok && wait_bar(&bar[C::kOFull + t], 0);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
+    } else if (ok && p.q_tma && copies) {
+      // a tile whose rows see no key here has awaited nothing: its Q, copied for the block's other tile's sake,
+      // has to be there before zeros go over it
+      ok = wait_bar(&bar[C::kQ], 0);
+      ok = __all_sync(0xffffffffu, ok);
     }
     if (ok && 128 * t + 32 * (warp & 3) < rows) {
       const bool live = r < rows, has = jt > j0 && !(l <= 0.0f);
@@ -574,8 +579,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
       float4* prt = reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(item) * p.n_split + split) * kRows * kPartRow);
       if (p.n_split > 1 && live && hf == 0)
         prt[r] = make_float4(has && m != -INFINITY ? m * p.c : -INFINITY, has ? l : 0.0f, 0.0f, 0.0f);
-      // this tile's Q is read no more (its last product has been awaited): its rows' place, in halves of 128
-      // bytes
+      // this tile's Q is read no more (its last product has been awaited, or its copy where there is none): its
+      // rows' place, in halves of 128 bytes
       unsigned char* q_tile = smem + t * kTileB;
 #pragma unroll 1
       for (int c = kKeys / kO * hf; c < kKeys / kO * (hf + 1); ++c) {

@@ -192,3 +192,23 @@ def test_short_sequences_with_a_maximum_that_keeps_growing(dtype, n, m):
         # (sum |q k| up to 700, as above)
         check(kernels.packed_prefill_attn(q, k, v, cum([n]), cum([m])), q, k, v, [n], [m])
     assert kernels.ragged_status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("nq,nk,Hkv,rep", [
+    ([600], [500], 8, 2), ([1100, 600], [700, 470], 8, 1), ([2010], [100], 4, 8), ([700, 900, 3], [532, 0, 3], 2, 4),
+    ([650], [500], 3, 3),
+])
+def test_blocks_whose_first_row_tile_sees_no_key(dtype, nq, nk, Hkv, rep):
+    # More queries than keys: in some block of two row tiles the first one's rows see nothing, the second's do.
+    # The zeros of the first leave by the memory that its Q is copied to.
+    from halftone_quantizedkvcache_b200 import kernels
+    q, k, v = make(nq, nk, Hkv, rep, DT[dtype], 37)
+    blind = torch.cat([torch.arange(n, device="cuda") < n - m for n, m in zip(nq, nk)])
+    first = kernels.packed_prefill_attn(q, k, v, cum(nq), cum(nk))
+    check(first, q, k, v, nq, nk)
+    for _ in range(50):
+        out = kernels.packed_prefill_attn(q, k, v, cum(nq), cum(nk))
+        assert (out[blind] == 0).all()
+        assert torch.equal(out, first)
+    assert kernels.ragged_status() == 0

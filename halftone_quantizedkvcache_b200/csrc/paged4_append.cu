@@ -207,7 +207,7 @@ __device__ __forceinline__ void exact_row(const AppendParams& p, const unsigned 
       const double cs = static_cast<double>(t[e].x) + t[e].z, sn = static_cast<double>(t[e].y) + t[e].w;
       z[e] = ((p.inter ? !(e & 1) : d0 < half) ? z[e] * cs - o * sn : z[e] * cs + o * sn) * static_cast<double>(p.factor);
     }
-    amax = fmax(amax, fabs(z[e]));
+    if (fabs(z[e]) > amax || z[e] != z[e]) amax = fabs(z[e]);  // (NaN if any is: nothing is above it)
   }
   float a75 = static_cast<float>(amax * (2.0 / 15.0));
 #pragma unroll

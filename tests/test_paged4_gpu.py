@@ -378,3 +378,33 @@ def test_gather_bad_pages_and_short_rows():
     assert kernels.ragged_status() == -1
     kernels.reset_ragged_status()
     assert torch.equal(k[:16], ref[0][:16]) and (k[16:32] == 0).all() and torch.equal(k[32:40], ref[0][32:40])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("inter,rot", [(False, 128), (True, 128), (False, 96)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_append_turned_rows_that_hold_no_number(dtype, inter, rot, bad):
+    """A channel of K that is no number, in many turned rows (one in 60 is formed in float64 too): its group
+    and its partner's have scales that are none, the others what they would have."""
+    from halftone_quantizedkvcache_b200 import kernels
+    new, page = [2000, 1100], 64
+    q, k, v, cache, tables = append_case(new, [0, 0], 4, 1, DT[dtype], page, 15, fused=False)
+    g = gen(16)
+    T, H = k.shape[:2]
+    at = torch.randint(0, D, (T, H), generator=g, device="cuda")
+    k.scatter_(2, at[..., None], bad)
+    inv = kernels.rope_inv_freq(rot, 1e6)[0]
+    kernels.paged4_append(q, k, v, cache, tables, ints([0, 0]), cu_seqlens=cum(new), inv_freq=inv, interleaved=inter)
+    half = rot // 2
+    other = torch.where(at >= rot, at, at ^ 1 if inter else torch.where(at < half, at + half, at - half))
+    hit = torch.zeros((T, H, 4), dtype=torch.bool, device="cuda")
+    hit.scatter_(2, at[..., None] // 32, True).scatter_(2, other[..., None] // 32, True)
+    b = torch.repeat_interleave(torch.arange(2, device="cuda"), torch.tensor(new, device="cuda"))
+    i = torch.cat([torch.arange(n, device="cuda") for n in new])
+    codes, sc = plain.read_codes(cache, "k", tables.long()[b, i // page], i % page)
+    assert sc[hit].isnan().all(), int((~sc[hit].isnan()).sum())
+    # a group's codes are its own affair: zeros in the place of the channels that are no numbers
+    k.scatter_(2, at[..., None], 0.0)
+    want, wsc = plain.coded(plain.turned(k, None, i, inv, inter, 1.0, 0.0))
+    assert torch.equal(sc[~hit], wsc.double()[~hit])
+    assert torch.equal(codes.unflatten(-1, (4, 32))[~hit], want.unflatten(-1, (4, 32))[~hit])

@@ -7,7 +7,7 @@
 // what crosses a block's border leaves partial states (m, l, o) that join_kernel puts together, always
 // in the order of the line.
 //
-// 64 sequences of 4096 to 8192 tokens, 8 kv heads of 2 rows: 103 us, 4.4 TB/s of cache.  What holds it
+// 64 sequences of 4096 to 8192 tokens, 8 kv heads of 2 rows: 108 us, 4.2 TB/s of cache.  What holds it
 // back is the work between loads (issue slots 49 %, arithmetic units 44 %, the matrix units 25 %, DRAM 49 %
 // at half that size): 144 bytes a token and head are 256 codes to unpack, twice.  Both products are
 // whole-number products on bytes (mma.sync m16n8k32, exact), the codes being the 16-row operand, since a
@@ -16,9 +16,10 @@
 //   * Q K^T: q is a 22-bit whole number per channel (of the row's largest |q|: 2^-22 of it is lost) in
 //     three base-256 digits, two columns and a third in a second product, and -8 sum(q) added for the
 //     codes' offset; one product is one group of 32 channels, its scale joins in float32.
-//   * P V: p relative to the tile's maximum, times the token's group scale relative to the tile's
-//     largest, is a 16-bit whole number (2^-16 of the tile's largest weight is lost) in two digits,
-//     transposed in registers by movmatrix; four tokens' bytes are turned with permutes.  A tile's sums
+//   * P V: p times the token's group scale, relative to the row's largest such product of the tile, is a
+//     16-bit whole number (2^-16 of that product is lost of each; against the largest p and the largest
+//     scale, each by itself, the tile took 3 % less time, but a large scale without weight left the others
+//     no bits) in two digits, transposed in registers by movmatrix; four tokens' bytes are turned with permutes.  A tile's sums
 //     go into the float32 state with the tile's and the group's factor.
 // (As bf16 products, 7 to 12 instructions a word and twice the products, 64 x 8192 tokens took 138 us.)
 // Copies: every warp has its own ring of stages filled by bulk copies, one per page, side and kind,
@@ -61,7 +62,7 @@ struct DecodeParams {
 
 template <int NT>
 struct Cfg {
-  // 64 x 8192 tokens: 103 us; 9 to 12 warps, their registers spilled, 113 to 123, tiles of 32 tokens 113
+  // 64 x 8192 tokens: 9 to 12 warps, their registers spilled, took 10 to 19 % more time, tiles of 32 tokens 10 %
   static constexpr int kWarps = 8;
   static constexpr int kStages = 2;
   static constexpr int kRows = 4 * NT;
@@ -112,6 +113,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {  // of the magnitudes; NaN if any is
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -140,8 +146,10 @@ __device__ __forceinline__ void next_unit(Cursor& c, const int* lens, int per) {
 }
 // the whole number that a row's largest |q| becomes: below 2^21, and its upper digit below 32
 constexpr float kFixed = 2088960.0f;
-// and that a tile's largest weight becomes
+// and that a tile's largest weight becomes (taken to 2^-9 of itself: 32576 at most, 64 x 8 of them below 2^24)
 constexpr float kWeight = 32512.0f;
+// largest weights below this (2^-110 of p = 1 under a scale of 1) are taken for none
+constexpr float kNoWeight = 7.7037198e-34f;
 __device__ constexpr int kZero[4] = {0, 0, 0, 0};
 
 __device__ __forceinline__ uint32_t pack_pair(float a, float b, int dt) {
@@ -483,33 +491,48 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
       // ---- P V, two groups at a time: 2 gg in columns 2 r, 2 gg + 1 in 2 r + 1
 #pragma unroll
       for (int gg = 0; gg < 2; ++gg) {
-        // the tokens' V scales, and the largest
+        // the tokens' V scales, and the rows' largest weights p x scale (bf16: to 2^-9 of themselves)
         uint32_t u[kSets];
-        __half2 big = __float2half2_rn(0.0f);
+        float big[NT][2];
 #pragma unroll
-        for (int i = 0; i < kSets; ++i) {
-          const int tk = 8 * i + slot_tok;
-          u[i] = *reinterpret_cast<const uint32_t*>(s + kOffVs + tk * kScaleB + 4 * gg);
-          if (tk >= left) u[i] = 0;       // what no token wrote may be anything
-          big = __hmax2_nan(big, __habs2(*reinterpret_cast<const __half2*>(&u[i])));
+        for (int nt = 0; nt < NT; ++nt) big[nt][0] = big[nt][1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSets; i += 2) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int tk = 8 * (i + e) + slot_tok;
+            u[i + e] = *reinterpret_cast<const uint32_t*>(s + kOffVs + tk * kScaleB + 4 * gg);
+            if (tk >= left) u[i + e] = 0;   // what no token wrote may be anything
+          }
+          const float2 x = half2_of(u[i]), y = half2_of(u[i + 1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            big[nt][0] = max3_abs(big[nt][0], sc[nt][i] * x.x, sc[nt][i + 1] * y.x);
+            big[nt][1] = max3_abs(big[nt][1], sc[nt][i] * x.y, sc[nt][i + 1] * y.y);
+          }
         }
+        float2 top[NT], inv[NT];
 #pragma unroll
-        for (int d = 4; d <= 16; d <<= 1) big = __hmax2_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
-        const float2 top = __half22float2(big);
-        const float inv0 = top.x == 0.0f ? 0.0f : kWeight * rcp(top.x), inv1 = top.y == 0.0f ? 0.0f : kWeight * rcp(top.y);
+        for (int nt = 0; nt < NT; ++nt) {
+          __nv_bfloat162 both = __floats2bfloat162_rn(big[nt][0], big[nt][1]);
+#pragma unroll
+          for (int d = 4; d <= 16; d <<= 1) both = __hmax2_nan(both, __shfl_xor_sync(0xffffffffu, both, d));
+          top[nt] = __bfloat1622float2(both);
+          inv[nt].x = top[nt].x < kNoWeight ? 0.0f : kWeight * rcp(top[nt].x);
+          inv[nt].y = top[nt].y < kNoWeight ? 0.0f : kWeight * rcp(top[nt].y);
+        }
         // weights as whole numbers, then as operands: digits of 32 tokens each
         uint32_t hi[NT][kSets / 2], lo[NT][kSets / 2];
 #pragma unroll
         for (int i = 0; i < kSets / 2; ++i) {
           const float2 x = half2_of(u[2 * i]), y = half2_of(u[2 * i + 1]);
-          const float x0 = x.x * inv0, x1 = x.y * inv1, y0 = y.x * inv0, y1 = y.y * inv1;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             constexpr float kRound = 12582912.0f;  // 1.5 x 2^23: the whole number in the low bits
-            const uint32_t a = transpose8(prmt(__float_as_uint(__fmaf_rn(sc[nt][2 * i], x0, kRound)),
-                                               __float_as_uint(__fmaf_rn(sc[nt][2 * i], x1, kRound)), 0x5410u));
-            const uint32_t b2 = transpose8(prmt(__float_as_uint(__fmaf_rn(sc[nt][2 * i + 1], y0, kRound)),
-                                                __float_as_uint(__fmaf_rn(sc[nt][2 * i + 1], y1, kRound)), 0x5410u));
+            const uint32_t a = transpose8(prmt(__float_as_uint(__fmaf_rn(sc[nt][2 * i] * x.x, inv[nt].x, kRound)),
+                                               __float_as_uint(__fmaf_rn(sc[nt][2 * i] * x.y, inv[nt].y, kRound)), 0x5410u));
+            const uint32_t b2 = transpose8(prmt(__float_as_uint(__fmaf_rn(sc[nt][2 * i + 1] * y.x, inv[nt].x, kRound)),
+                                                __float_as_uint(__fmaf_rn(sc[nt][2 * i + 1] * y.y, inv[nt].y, kRound)), 0x5410u));
             lo[nt][i] = prmt(a, b2, 0x6420u);
             hi[nt][i] = prmt(a, b2, 0x7531u);
           }
@@ -527,7 +550,7 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
           }
         }
         // the groups' words of chunk vj of token slots 2 c4 and 2 c4 + 1, set by set: both groups' in one
-        // load, where there are registers for them (7 x 2501 tokens 10 us against 12; 64 x 8192 105 against 103)
+        // load, where there are registers for them (7 x 2501 tokens 10 us against 12; 64 x 8192 2 % more)
         uint2 vw[2 * kSets];
         if constexpr (NT == 1) {
 #pragma unroll
@@ -566,10 +589,10 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
                 mma_u8u8(q8[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][2 * k], lo[nt][2 * k + 1], k ? q8[nt][m] : cl[nt]);
               }
           }
-          // 64 x 8 x 32512 is below 2^24: exact in float32
+          // 64 x 8 x 32576 is below 2^24: exact in float32
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float w = f[nt] * ((e ? top.y : top.x) * (1.0f / kWeight));
+            const float w = f[nt] * ((e ? top[nt].y : top[nt].x) * (1.0f / kWeight));
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
               o[nt][g][m][0] = __fmaf_rn(w, static_cast<float>(h[nt][m][e] * 256 + q8[nt][m][e]), o[nt][g][m][0]);

@@ -1726,9 +1726,9 @@ def paged4_decode_attn(q, cache, block_tables, lens, *, sm_scale=None, out=None)
     its first ``lens[b]`` tokens (at most those its table holds), and gives zeros where there are
     none.  What pages hold past them does not matter.  Returns the output in q's layout and dtype (or
     writes ``out [B,Hq,128]``).  Nothing depends on ``lens`` on the host: a captured call replays while
-    sequences grow.  Sums are float32; of q 2^-22 of its row's largest value is rounded off, of the
-    weights 2^-16 of the largest of 64 tokens.  A page number outside the cache sets ``ragged_status()``, and that sequence's output
-    has no meaning.
+    sequences grow.  Sums are float32; of q 2^-22 of its row's largest value is rounded off, of each
+    weight times V scale 2^-16 of the row's largest such product among 64 tokens.  A page number
+    outside the cache sets ``ragged_status()``, and that sequence's output has no meaning.
     """
     what = "paged4_decode_attn"
     try:

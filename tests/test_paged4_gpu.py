@@ -408,3 +408,111 @@ def test_append_turned_rows_that_hold_no_number(dtype, inter, rot, bad):
     want, wsc = plain.coded(plain.turned(k, None, i, inv, inter, 1.0, 0.0))
     assert torch.equal(sc[~hit], wsc.double()[~hit])
     assert torch.equal(codes.unflatten(-1, (4, 32))[~hit], want.unflatten(-1, (4, 32))[~hit])
+
+
+def lost_weights(q, cache, tables, b, n, scale=None):
+    """What rounding p x scale to a 16-bit whole number does to the output at most: per row, group and tile of
+    64 tokens half a step, 1 / (2 x 32512), of the largest p x scale (taken to 2^-9 of itself), times
+    sum |code|.  q [Hkv, rep, D] -> [Hkv, rep, D]."""
+    page = cache["k"].shape[2]
+    k = plain.values(cache, "k", tables, b, n).transpose(0, 1)
+    p = torch.softmax(q.double() @ k.transpose(1, 2) * (scale if scale is not None else 1 / math.sqrt(D)), -1)
+    codes, sc = plain.read_codes(cache, "v", *plain.slots(tables, page, b, n))
+    pad = -n % 64
+    top = p[:, :, None] * sc.abs().permute(1, 2, 0)[:, None]                                   # [Hkv, rep, 4, n]
+    top = torch.nn.functional.pad(top, (0, pad)).unflatten(-1, (-1, 64)).amax(-1)
+    codes = torch.nn.functional.pad(codes.double().abs().permute(1, 2, 0), (0, pad)).unflatten(-1, (-1, 64)).sum(-1)
+    return torch.einsum("hrdt,hdt->hrd", top.repeat_interleave(32, 2), codes) * (1 + 2.0 ** -8) / (2 * 32512)
+
+
+def scored_cache(scores, Hkv, page, seed):
+    """One sequence whose token t has the score x scores[t] for a row of q that holds x throughout: all
+    codes of K are 7.  V: random codes, scales 0.1 .. 0.4."""
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(seed)
+    n = len(scores)
+    per = -(-n // page)
+    cache = plain.random_cache(kernels, per + 1, Hkv, page, g)
+    tables = plain.random_tables(1, per, per + 1, g)
+    cache["k"].fill_(0xff)
+    pg, t = plain.slots(tables, page, 0, n)
+    cache["k_scale"][pg, :, t] = (torch.tensor(scores, device="cuda").double() / (7 * math.sqrt(D))).half()[:, None, None]
+    return cache, tables, pg, t
+
+
+def check_scored(cache, tables, n, dt, rows):
+    """Rows of q that hold one number each, against the formula.  K's scales are the scores' only source."""
+    from halftone_quantizedkvcache_b200 import kernels
+    Hkv = cache["k"].shape[1]
+    q = torch.tensor(rows, device="cuda")[None, None, :, None].expand(1, Hkv, len(rows), D).reshape(1, -1, D).to(dt).contiguous()
+    out = kernels.paged4_decode_attn(q, cache, tables, ints([n]))
+    k, v = (plain.values(cache, x, tables, 0, n).transpose(0, 1) for x in ("k", "v"))
+    qq = q[0].view(Hkv, -1, D)
+    ref, mag = plain.attend(qq, k, v, torch.ones((1, n), dtype=torch.bool, device="cuda"))
+    # q is a whole number of steps here but for 2^-22 of itself; scores below 80: 2^-13 of a weight at most,
+    # twice.  Below its smallest normal number float16's step is 2^-24 whatever the value.
+    extra = mag * 2.0 ** -12 + lost_weights(qq, cache, tables, 0, n) + (2.0 ** -25 if dt == torch.float16 else 0.0)
+    near(out[0].view(ref.shape), ref, extra)
+    assert kernels.ragged_status() == 0
+    return out, ref
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("Hkv,rows,page", [(1, [1.0], 64), (2, [1.0, 0.5], 16), (1, [1.0, 0.75, 0.5, 0.25, 1.5], 128)])
+@pytest.mark.parametrize("ratio", [1e2, 1e3, 1e4, 2.0 ** 18])
+def test_decode_a_large_scale_without_weight_takes_no_bits(dtype, Hkv, rows, page, ratio):
+    """Tokens that no row heeds (p of 1e-12 and less for x = 1) with V scales `ratio` times those of the token
+    that all of them do."""
+    n = 200
+    scores = [0.0] * n
+    heeded = [7, 100, 150, 199]                 # one of each tile
+    for t in heeded:
+        scores[t] = 28.0
+    cache, tables, pg, t = scored_cache(scores, Hkv, page, 41)
+    v_scale = torch.full((n,), 2.0 ** -4 if ratio < 2e4 else 2.0 ** -10, device="cuda")
+    light = torch.ones(n, dtype=torch.bool, device="cuda")
+    light[heeded] = False
+    v_scale[light] *= ratio
+    cache["v_scale"][pg, :, t] = v_scale.half()[:, None, None]
+    check_scored(cache, tables, n, DT[dtype], rows)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("Hkv,rows,page", [(1, [1.0], 64), (2, [1.0, 0.5], 16), (1, [1.0, 0.75, 0.5, 0.25, 1.5], 128)])
+@pytest.mark.parametrize("sink", [0.0, 2.0 ** -24, 0.002])
+@pytest.mark.parametrize("n,far", [(64, 8.0), (500, 12.0), (3000, 20.0)])
+def test_decode_beside_a_token_that_takes_the_weight_and_has_no_values(dtype, Hkv, rows, page, sink, n, far):
+    """A first token with most of the softmax and V next to nothing, as sinks have it: the others' V is
+    what goes out, each with a weight of e^-far."""
+    cache, tables, pg, t = scored_cache([40.0] + [40.0 - far] * (n - 1), Hkv, page, 43)
+    cache["v_scale"][pg[0], :, t[0]] = sink
+    out, ref = check_scored(cache, tables, n, DT[dtype], rows)
+    assert float(ref.abs().max()) > 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [64, 1000, 5000])
+def test_decode_many_small_weights_beside_a_large_one(dtype, n):
+    """Key 0 has weight 1 and codes of zero under a scale like the others', each other key a weight of 2^-11:
+    one step in 32512 of 64 tokens' largest is what each may lose, and together they carry V."""
+    cache, tables, pg, t = scored_cache([40.0] + [40.0 - 11 * math.log(2.0)] * (n - 1), 1, 64, 44)
+    cache["v"][pg[0], :, t[0]] = 0x88
+    check_scored(cache, tables, n, DT[dtype], [1.0, 0.5])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_decode_scales_of_all_sizes(dtype):
+    """V scales from 2^-24 to 2^8 and scores within ten of each other, all at random."""
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(45)
+    lens = [900, 64, 1, 333]
+    cache = plain.random_cache(kernels, 70, 2, 64, g)
+    tables = plain.random_tables(4, 15, 70, g)
+    cache["v_scale"].copy_(2.0 ** torch.randint(-24, 9, cache["v_scale"].shape, generator=g, device="cuda").float())
+    q = torch.randn((4, 6, D), generator=g, device="cuda").to(DT[dtype])
+    out = kernels.paged4_decode_attn(q, cache, tables, ints(lens))
+    for b, n in enumerate(lens):
+        k, v = (plain.values(cache, x, tables, b, n).transpose(0, 1) for x in ("k", "v"))
+        qq = q[b].view(2, -1, D)
+        ref, mag = plain.attend(qq, k, v, torch.ones((1, n), dtype=torch.bool, device="cuda"))
+        near(out[b].view(ref.shape), ref, mag * 2.0 ** -12 + lost_weights(qq, cache, tables, b, n) + 2.0 ** -25)

@@ -11,7 +11,8 @@
 // (once a token, kept as two float32 parts in shared memory); norms and turns are float32, off by at most
 // kSlack of the pair's larger value.  The k rows with a quotient or a scale closer to a rounding border than
 // that (one in 60) are listed, and formed again in float64 at the end of the block, a warp a row (8 of the
-// 124 us below; a half-warp a row 15, on the spot one by one 30).  V's codes
+// 126 us below; a half-warp a row 15, on the spot one by one 30).  So are rows of q and k whose squares float32
+// does not hold (finding them takes 2 us: their bits are gathered, since a branch in q's loop took 5).  V's codes
 // come from its 16-bit values: an 11-bit x over an 11-bit s is 2^-13 away from a border unless it lies on
 // it, and one corrected division finds both cases.
 //
@@ -19,7 +20,7 @@
 // (8 channels, 16 bytes, each); a half-warp takes one token and all of its rows, 7 of them in flight
 // through shared memory (the next row in registers instead: 179 us).
 //
-// 8 x 4096 tokens of 16 q heads and 8 kv heads, both norms, full rotation, k kept: 124 us, 4.1 TB/s of
+// 8 x 4096 tokens of 16 q heads and 8 kv heads, both norms, full rotation, k kept: 126 us, 4.0 TB/s of
 // bytes moved.  Bound by issue slots (70 % of them taken; arithmetic units 45 %, DRAM 36 % at half that
 // size): for a lane and row of k a reduction of 128 squares, the turn and the codes.  (8 lanes a row, both
 // values of a pair in one lane, take 27 % fewer instructions but 96 registers: 131 us, the 20 warps an SM hide
@@ -36,6 +37,7 @@ namespace p4 {
 constexpr int kThreads = 128;
 constexpr int kTok = kThreads / 16;       // tokens per block
 constexpr int kRing = 8;                  // rows in flight for each, a power of two
+constexpr int kMostRows = 512;            // of a token for a block: its list takes 16 KB
 
 struct AppendParams {
   Pages pg;
@@ -62,10 +64,13 @@ struct AppendParams {
 };
 
 // Error of the float32 route, relative to |x w cos| + |o w_o sin| (times r and the factor), in units of 2^-24:
-// half that of the mean (squares are exact; 3 sums in a lane's half, the halves, 4 rounds, eps: 9) 4.5 and
+// half that of the mean (squares are exact but for 2^-150, below 2^-24 of it where it is a normal number; 3 sums
+// in a lane's half, the halves, 4 rounds, eps: 10) 5 and
 // that of its root's correction 2.5, cos or sin 1, their weight 1 and factor 1, the turn's product 1 and sum
-// 1, r's product 1: 13.  The sum is at most the pair's length, sqrt(2) times the larger of its turned values.
-constexpr float kSlack = 1.4143f * 13.0f / 16777216.0f;
+// 1, r's product 1: 13.5.  The sum is at most the pair's length, sqrt(2) times the larger of its turned values.
+constexpr float kSlack = 1.4143f * 13.5f / 16777216.0f;
+
+constexpr uint32_t kWhole = 0x80000000u;  // a listed row that float64 writes to q_out or k_out too
 
 template <int DT>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
@@ -90,6 +95,11 @@ __device__ __forceinline__ __half group_scale(float a75) {
 __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rsqrt_ftz(float x) {  // (infinity below the smallest normal number)
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 // a / 7.5 of a 16-bit a, correctly rounded: one correction of the product with 2 / 15
@@ -163,10 +173,11 @@ __device__ __forceinline__ float weight_at(const AppendParams& p, const void* w,
   return p.w_f32 ? static_cast<const float*>(w)[d] : Elem<DT>::to_f32(static_cast<const typename Elem<DT>::T*>(w)[d]);
 }
 
-// A k row in float64 (a warp, 4 channels a lane): its codes and scales.
+// A row of q or k in float64 (a warp, 4 channels a lane): `out` takes it and `codes` and `scales` its codes, where
+// they are not null.
 template <int DT>
-__device__ __forceinline__ void exact_row(const AppendParams& p, const unsigned char* row, const float4* turn, uint8_t* codes,
-                                          __half* scales, int place) {
+__device__ __forceinline__ void exact_row(const AppendParams& p, const void* weights, const char* row, const float4* turn,
+                                          char* out, uint8_t* codes, __half* scales, int place) {
   const int lane = threadIdx.x & 31, c = lane >> 1, half = p.rot / 2;
   const int d0 = 4 * lane, o0 = 8 * partner_of(p, c) + 4 * (lane & 1);  // (interleaved: partners e ^ 1)
   auto unpack = [](const uint2& w, float (&f)[4]) {
@@ -182,21 +193,24 @@ __device__ __forceinline__ void exact_row(const AppendParams& p, const unsigned 
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int d = d0 + e, eo = p.inter ? e ^ 1 : e;
-    wt[e] = weight_at<DT>(p, p.kw, d);
-    wo[e] = weight_at<DT>(p, p.kw, o0 + eo);
+    wt[e] = weight_at<DT>(p, weights, d);
+    wo[e] = weight_at<DT>(p, weights, o0 + eo);
     t[e] = turn[d >= p.rot ? 0 : p.inter ? d / 2 : d < half ? d : d - half];
   }
   unpack(x, f);
   unpack(xo, g);
   double r = 1.0;
-  if (p.kw) {
+  if (weights) {
     double s = fma(static_cast<double>(f[0]), static_cast<double>(f[0]), static_cast<double>(f[1]) * f[1]) +
                fma(static_cast<double>(f[2]), static_cast<double>(f[2]), static_cast<double>(f[3]) * f[3]);
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
     s = s * (1.0 / kD) + static_cast<double>(p.eps);
+    // (times 2^-200 or 2^200 where float32 would not hold it, its root by 2^-100 or 2^100)
+    const double by = s > 1e36 ? 0x1p-100 : s < 1e-30 ? 0x1p100 : 1.0;
+    s *= by * by;
     r = rsqrtf(static_cast<float>(s));
-    r = r * fma(-0.5 * s * r, r, 1.5);    // 2^-22 becomes 2^-43
+    r = r * fma(-0.5 * s * r, r, 1.5) * by;  // 2^-22 becomes 2^-43
   }
   double z[4], amax = 0.0;
 #pragma unroll
@@ -209,6 +223,10 @@ __device__ __forceinline__ void exact_row(const AppendParams& p, const unsigned 
     }
     if (fabs(z[e]) > amax || z[e] != z[e]) amax = fabs(z[e]);  // (NaN if any is: nothing is above it)
   }
+  if (out)
+    *reinterpret_cast<uint2*>(out + 2 * d0) = make_uint2(pack16<DT>(static_cast<float>(z[0]), static_cast<float>(z[1])),
+                                                         pack16<DT>(static_cast<float>(z[2]), static_cast<float>(z[3])));
+  if (!codes) return;                     // (the same for all lanes)
   float a75 = static_cast<float>(amax * (2.0 / 15.0));
 #pragma unroll
   for (int m = 4; m >= 1; m >>= 1) a75 = max_nan(a75, __shfl_xor_sync(0xffffffffu, a75, m));
@@ -235,7 +253,7 @@ template <int DT>
 __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ uint4 ring[kTok][kRing * 16];
   __shared__ float4 turn[kTok][kD / 2];   // cos and sin, and what is left of them
-  extern __shared__ uint32_t again[];     // k rows to form again: token of the block, head
+  extern __shared__ uint32_t again[];     // rows to form again: kWhole or 0, token of the block, row
   __shared__ int n_again;
   __shared__ int4 where[kTok];
   const int tid = threadIdx.x, lane = tid & 31, sub = tid >> 4, l = lane & 15, d0 = 8 * l;
@@ -265,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
   const int place = static_cast<int>(at) & (p.pg.page - 1);
   const double pos = static_cast<double>(at + (live && p.pos_offset ? p.pos_offset[b] : 0));
   const bool plain_k = !p.kw && p.rot == 0;  // k is coded as it came: no rounding before the codes
-  if (l == 0) where[sub] = make_int4(tok, pid, place, 0);
+  if (l == 0) where[sub] = make_int4(tok, pid, place, fits);
   if (tid == 0) n_again = 0;
   __syncthreads();
   const int half = p.rot / 2;
@@ -344,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
       row_of(x);
     }
   };
-  auto norm_of = [&](const F2 (&f)[4]) {
+  auto mean_square = [&](const F2 (&f)[4]) {
     F2 s2 = f2_mul(f[0], f[0]);
 #pragma unroll
     for (int e = 1; e < 4; ++e) s2 = f2_fma(f[e], f[e], s2);
@@ -353,11 +371,10 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
     s += s1;
 #pragma unroll
     for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-    s = __fmaf_rn(s, 1.0f / kD, p.eps);
-    const float r = rsqrtf(s);
-    return r * __fmaf_rn(-0.5f * s * r, r, 1.5f);
+    return __fmaf_rn(s, 1.0f / kD, p.eps);
   };
-  // normed and turned row
+  // Normed and turned row; whether float32 holds its norm: bf16's largest and smallest rows have a mean square that
+  // is infinite or no normal number in float32.  Their 1 / root is then infinite or NaN, and so is all of the row.
   auto turned_row = [&](const uint4& x, bool norm, F2 (&y)[4]) {
     F2 f[4], o[4];
     unpack_pairs<DT>(x, f);
@@ -373,24 +390,35 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = f2_fma(f[e], cs[e], f2_mul(o[e], sg[e]));
-    if (norm) {
-      const float r = norm_of(f);
+    if (!norm) return true;
+    const float s = mean_square(f);
+    float r = rsqrt_ftz(s);
+    r *= __fmaf_rn(-0.5f * s * r, r, 1.5f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = f2_mul(y[e], f2_make(r, r));
-    }
+    for (int e = 0; e < 4; ++e) y[e] = f2_mul(y[e], f2_make(r, r));
+    return fabsf(r) < INFINITY;
   };
+  auto list = [&](int row, uint32_t whole) { again[atomicAdd(&n_again, 1)] = whole | static_cast<uint32_t>(sub << 16 | row); };
 
   if (r0 < p.Hq) {
     factors(p.qw);
     char* to = static_cast<char*>(p.q_out) + 2 * (tok * p.qos[0] + r0 * p.qos[1] + d0);
     const bool store = live || (here && p.copy_rest);
-    each(r0, min(r1, p.Hq), [&](const uint4& x) {
-      F2 y[4];
-      turned_row(x, p.qw, y);
-      const uint4 w = live ? pack_row<DT>(y) : x;
-      if (store) *reinterpret_cast<uint4*>(to) = w;
-      to += 2 * p.qos[1];
-    });
+#pragma unroll 1
+    for (int c = r0; c < min(r1, p.Hq); c += 32) {
+      const int end = min(c + 32, min(r1, p.Hq));
+      uint32_t odd = 0;                   // the rows for float64, the last in bit 0
+      each(c, end, [&](const uint4& x) {
+        F2 y[4];
+        const bool held = turned_row(x, p.qw, y);
+        const uint4 w = live ? pack_row<DT>(y) : x;
+        if (store && (held || !live)) *reinterpret_cast<uint4*>(to) = w;  // (others stay what they were: q_out may be q)
+        odd = 2 * odd + !held;
+        to += 2 * p.qos[1];
+      });
+      if (live && l == 0)
+        for (; odd; odd &= odd - 1) list(end - __ffs(odd), kWhole);
+    }
   }
   // a lane's word and its group's scale in a head's page
   const int64_t code_at = pid * p.pg.cp + place * kRowB + word_at(place, l >> 2, l & 3);
@@ -415,8 +443,9 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
       if (!plain_k) {
         const float err = kSlack * fmaxf(a, p.inter ? a : __shfl_sync(0xffffffffu, a, partner));
         const float e75 = __fmaf_rn(err, 0.13333334f, a75 * 1.2e-7f);
-        // the scale is the same for all a75 that this one may stand for
-        near = a75 < INFINITY && __half_as_ushort(group_scale(a75 + e75)) != __half_as_ushort(group_scale(fmaxf(a75 - e75, 0.0f)));
+        // the scale is the same for all a75 that this one may stand for; or the row's norm is for float64 (or it
+        // holds no numbers)
+        near = !(a75 < INFINITY) || __half_as_ushort(group_scale(a75 + e75)) != __half_as_ushort(group_scale(fmaxf(a75 - e75, 0.0f)));
         const F2 r2 = f2_make(rs, rs), big = f2_make(12582912.0f, 12582912.0f);  // 1.5 x 2^23
         float far = 0.0f;
 #pragma unroll
@@ -433,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
       }
       const uint32_t word = pack_codes(k);
       if (live) {
-        if (__any_sync(mask, near && fits) && l == 0) again[atomicAdd(&n_again, 1)] = static_cast<uint32_t>(sub << 16 | h);
+        if (__any_sync(mask, near) && l == 0) list(p.Hq + h, a75 < INFINITY ? 0 : kWhole);
         if (fits) {
           *reinterpret_cast<uint32_t*>(codes) = word;
           if ((l & 3) == 0) *scales = sc;
@@ -468,14 +497,23 @@ __global__ void __launch_bounds__(kThreads, 7) append_kernel(const __grid_consta
       scales += p.pg.sh;
     });
   }
-  // ---- rows whose codes float32 could not tell
-  if (plain_k || r1 <= p.Hq || r0 >= p.Hq + p.Hkv) return;
+  // ---- rows whose norm float32 does not hold, or whose codes it could not tell
+  const bool lists = (r0 < p.Hq && p.qw) || (r1 > p.Hq && r0 < p.Hq + p.Hkv && !plain_k);
+  if (!lists) return;
   __syncthreads();
   for (int i = tid >> 5; i < n_again; i += kThreads / 32) {
-    const int of = again[i] >> 16, h = again[i] & 0xffff;
-    const int4 w = where[of];             // token, page, place
-    exact_row<DT>(p, static_cast<const unsigned char*>(p.k) + 2 * (w.x * p.ks[0] + h * p.ks[1]), turn[of],
-                  p.pg.k + w.y * p.pg.cp + h * p.pg.ch + w.z * kRowB, p.pg.ksc + w.y * p.pg.sp + h * p.pg.sh + w.z * 4, w.z);
+    const uint32_t entry = again[i];
+    const int of = entry >> 16 & 0xff, row = entry & 0xffff, h = row - p.Hq;
+    const int4 w = where[of];             // token, page, place, whether it has one
+    const bool of_q = row < p.Hq;
+    const int64_t* from = of_q ? p.qs : p.ks;
+    const int64_t* to = of_q ? p.qos : p.kos;
+    const int head = of_q ? row : h;
+    char* out = static_cast<char*>(of_q ? p.q_out : p.k_out);
+    exact_row<DT>(p, of_q ? p.qw : p.kw, static_cast<const char*>(of_q ? p.q : p.k) + 2 * (w.x * from[0] + head * from[1]), turn[of],
+                  out && entry & kWhole ? out + 2 * (w.x * to[0] + head * to[1]) : nullptr,
+                  !of_q && w.w ? p.pg.k + w.y * p.pg.cp + h * p.pg.ch + w.z * kRowB : nullptr,
+                  p.pg.ksc + w.y * p.pg.sp + h * p.pg.sh + w.z * 4, w.z);
   }
 }
 
@@ -487,11 +525,10 @@ int launch_append(AppendParams p, cudaStream_t st) {
   // warps an SM; below, they are split, down to one row each
   const int64_t want = std::max<int64_t>(1, 8LL * current_sm_count() / blocks);
   const int groups = static_cast<int>(std::min<int64_t>(rows, want));
-  p.rows_per_block = (rows + groups - 1) / groups;
+  p.rows_per_block = std::min((rows + groups - 1) / groups, kMostRows);
   p.groups = (rows + p.rows_per_block - 1) / p.rows_per_block;
   if (blocks * p.groups > 0x7fffffff) return HQ_ERR_UNSUPPORTED;
-  const int list = kTok * std::min(p.rows_per_block, p.Hkv) * 4;  // a block's k rows
-  if (list > 16384) return HQ_ERR_UNSUPPORTED;
+  const int list = kTok * std::min(p.rows_per_block, p.Hq + p.Hkv) * 4;  // a block's q and k rows
   append_kernel<DT><<<static_cast<unsigned>(blocks * p.groups), kThreads, list, st>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? HQ_OK : static_cast<int>(e);

@@ -516,3 +516,64 @@ def test_decode_scales_of_all_sizes(dtype):
         qq = q[b].view(2, -1, D)
         ref, mag = plain.attend(qq, k, v, torch.ones((1, n), dtype=torch.bool, device="cuda"))
         near(out[b].view(ref.shape), ref, mag * 2.0 ** -12 + lost_weights(qq, cache, tables, b, n) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-30, 1e-6])
+@pytest.mark.parametrize("inter,f32", [(False, True), (True, False)])
+def test_append_norms_of_rows_whose_squares_float32_does_not_hold(eps, inter, f32):
+    """Rows from bf16's smallest numbers to its largest, normed and turned: q, k, codes and scales are the
+    float64 form's."""
+    from halftone_quantizedkvcache_b200 import kernels
+    new = [1500]
+    q, k, v, cache, tables = append_case(new, [5], 2, 2, torch.bfloat16, 64, 51, fused=False)
+    g = gen(52)
+    powers = torch.tensor([-126, -100, -75, -62, -50, -49, 0, 49, 50, 59, 60, 62, 64, 100, 120, 124], device="cuda")
+    for x in (q, k):
+        by = powers[torch.randint(0, len(powers), x.shape[:2], generator=g, device="cuda")]
+        x.copy_((x.double() * 2.0 ** by.double()[..., None]).to(torch.bfloat16))
+    x[7, :, ::3] = 0                                     # (and some channels much smaller than their row's)
+    x[8, :, 1:] *= 2.0 ** -60
+    assert x.isfinite().all() and (x[:, :, 0] != 0).any()
+    before = {n: y.clone() for n, y in cache.items()}
+    inv = kernels.rope_inv_freq(128, 1e6)[0]
+    w = [torch.empty(D, device="cuda").uniform_(0.2, 2.0, generator=g).to(torch.float32 if f32 else torch.bfloat16) for _ in range(2)]
+    k_out = torch.zeros_like(k)
+    got = kernels.paged4_append(q, k, v, cache, tables, ints([5]), cu_seqlens=cum(new), inv_freq=inv, interleaved=inter,
+                                q_weight=w[0], k_weight=w[1], eps=eps, k_out=k_out)
+    eps32 = float(torch.tensor(eps, dtype=torch.float32))
+    check_append(q, k, v, cache, tables, new, [5], before, got, k_out, inv, w, inter, eps=eps32)
+
+
+def test_append_norm_without_eps_of_rows_that_are_zero_or_no_number():
+    from halftone_quantizedkvcache_b200 import kernels
+    q, k, v, cache, tables = append_case([4], [0], 1, 1, torch.bfloat16, 16, 53, fused=False)
+    k[1] = 0                                             # 0 / 0
+    k[2, 0, 40] = math.nan
+    w = torch.ones(D, device="cuda")
+    kernels.paged4_append(q, k, v, cache, tables, ints([0]), cu_seqlens=ints([0, 4]), q_weight=w, k_weight=w, eps=0.0)
+    kv, _ = kernels.paged4_gather(cache, tables, ints([4]), ints([0, 4]), 4)
+    assert kv[1:3].isnan().all() and kv[0].isfinite().all() and kv[3].isfinite().all()
+    kernels.paged4_append(q, k, v, cache, tables, ints([0]), cu_seqlens=ints([0, 4]), q_weight=w, k_weight=w, eps=1e-6)
+    kv, _ = kernels.paged4_gather(cache, tables, ints([4]), ints([0, 4]), 4)
+    assert (kv[1] == 0).all() and kv[2].isnan().all()
+
+
+def test_append_norms_in_place_over_many_heads_and_rows_behind_the_last_sequence():
+    """As above, 40 q heads a token in one block, q turned in its own memory; rows of no sequence stay."""
+    from halftone_quantizedkvcache_b200 import kernels
+    new = [9000, 597]
+    q, k, v, cache, tables = append_case(new + [3], [0, 0, 0], 2, 20, torch.bfloat16, 64, 54, fused=True)
+    tables = tables[:2].contiguous()
+    g = gen(55)
+    for x in (q, k):
+        x.mul_(torch.where(torch.rand(x.shape[:2], generator=g, device="cuda") < 0.1, 2.0 ** 70, 1.0).to(torch.bfloat16)[..., None])
+    before = {n: y.clone() for n, y in cache.items()}
+    inv = kernels.rope_inv_freq(128, 1e6)[0]
+    w = [torch.empty(D, device="cuda").uniform_(0.2, 2.0, generator=g) for _ in range(2)]
+    q0 = q.clone()
+    apart = kernels.paged4_append(q, k, v, cache, tables, ints([0, 0]), cu_seqlens=cum(new), inv_freq=inv, q_weight=w[0], k_weight=w[1])
+    assert torch.equal(q, q0)
+    assert kernels.paged4_append(q, k, v, cache, tables, ints([0, 0]), cu_seqlens=cum(new), inv_freq=inv, q_weight=w[0],
+                                 k_weight=w[1], q_out=q) is q
+    assert torch.equal(q, apart) and torch.equal(q[-3:], q0[-3:])
+    check_append(q0, k, v, cache, tables, new, [0, 0], before, q, None, inv, w)

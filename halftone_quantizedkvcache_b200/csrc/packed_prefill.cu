@@ -30,6 +30,7 @@
 #include <atomic>
 
 #include "decode_common.cuh"
+#include "rows.cuh"
 #include "umma.cuh"
 
 namespace hq {
@@ -938,7 +939,6 @@ extern "C" int hq_packed_prefill(const hq_packed_prefill_args* args) {
   const int64_t* in[4] = {a.q_strides, a.k_strides, a.v_strides, a.out_strides};
   for (const int64_t* s : in)
     if (s[0] % 8 || s[1] % 8 || s[0] < 0 || s[1] < 0) return HQ_ERR_INVALID_ARGUMENT;
-  if ((a.T > 1 && a.out_strides[0] == 0) || (a.Hq > 1 && a.out_strides[1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
   // TMA takes no stride of 0
   for (int i = 1; i < 3 && a.Tk > 0; ++i)
     if ((a.Tk > 1 && in[i][0] == 0) || (a.Hkv > 1 && in[i][1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
@@ -966,6 +966,11 @@ extern "C" int hq_packed_prefill(const hq_packed_prefill_args* args) {
   p.zero_rest = a.zero_rest;
   p.part = static_cast<float*>(a.workspace);
   p.status = a.status;
+  // what is written has memory of its own (but for q's: a block reads no rows of others)
+  const Rows out = packed_rows(a.out, a.T, a.Hq, a.out_strides), q = packed_rows(a.q, a.T, a.Hq, a.q_strides);
+  if (rows_meet(out) || (!same_rows(out, q) && rows_meet(out, q)) || rows_meet(out, packed_rows(a.k, a.Tk, a.Hkv, a.k_strides)) ||
+      rows_meet(out, packed_rows(a.v, a.Tk, a.Hkv, a.v_strides)))
+    return HQ_ERR_INVALID_ARGUMENT;
   CUtensorMap qm{}, km{}, vm{};
   if (a.Tk > 0) {
     // strides in rising order, K's and V's alike

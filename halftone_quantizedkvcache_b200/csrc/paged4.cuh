@@ -17,6 +17,7 @@
 #include <cmath>
 
 #include "hq_common.cuh"
+#include "rows.cuh"
 
 namespace hq {
 namespace p4 {
@@ -77,6 +78,14 @@ inline int check_pages(const void* k, const void* v, const void* ks, const void*
       return HQ_ERR_INVALID_ARGUMENT;
   }
   return HQ_OK;
+}
+// Pages and heads of K and V (codes or scales: a row of `row` bytes per token, strides in units of `unit`
+// bytes) that share no memory.
+inline bool own_memory(const void* k, const void* v, const int64_t st[2], int unit, int row, int n_pages, int Hkv, int page) {
+  const Rows a = rows_of(k, n_pages, Hkv, unit * st[0], unit * st[1], int64_t(row) * page);
+  Rows b = a;
+  b.base = v;
+  return !rows_meet(a) && !rows_meet(a, b);
 }
 inline Pages make_pages(const void* k, const void* v, const void* ks, const void* vs, const int64_t cs[2],
                         const int64_t ss[2], int n_pages, int page, const int* tables, int64_t tstride,

@@ -555,14 +555,22 @@ extern "C" int hq_paged4_append(const hq_paged4_append_args* args) {
   if (!a.q || !a.k_new || !a.v_new || !a.q_out || !a.lens) return HQ_ERR_INVALID_ARGUMENT;
   auto al = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
   if (!al(a.q) || !al(a.k_new) || !al(a.v_new) || !al(a.q_out) || !al(a.k_out)) return HQ_ERR_INVALID_ARGUMENT;
-  if (a.k_out == a.k_new) return HQ_ERR_INVALID_ARGUMENT;  // (rows of k are read a second time)
   const int64_t* all[5] = {a.q_strides, a.k_strides, a.v_strides, a.qo_strides, a.k_out ? a.ko_strides : a.qo_strides};
   for (const int64_t* s : all)
     if (s[0] % 8 || s[1] % 8) return HQ_ERR_INVALID_ARGUMENT;
-  // what is written has rows of its own
-  const int heads[2] = {a.Hq, a.Hkv};
-  for (int i = 0; i < (a.k_out ? 2 : 1); ++i)
-    if ((a.T > 1 && all[3 + i][0] == 0) || (heads[i] > 1 && all[3 + i][1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
+  // What is written has memory of its own, apart from the inputs', which other blocks may still read and this one
+  // reads a second time; but q_out may be q, whose rows one block reads and writes.
+  const Rows q = packed_rows(a.q, a.T, a.Hq, a.q_strides), k = packed_rows(a.k_new, a.T, a.Hkv, a.k_strides),
+             v = packed_rows(a.v_new, a.T, a.Hkv, a.v_strides), qo = packed_rows(a.q_out, a.T, a.Hq, a.qo_strides);
+  if (rows_meet(qo) || (!same_rows(qo, q) && rows_meet(qo, q)) || rows_meet(qo, k) || rows_meet(qo, v))
+    return HQ_ERR_INVALID_ARGUMENT;
+  if (a.k_out) {
+    const Rows ko = packed_rows(a.k_out, a.T, a.Hkv, a.ko_strides);
+    if (rows_meet(ko) || rows_meet(ko, q) || rows_meet(ko, k) || rows_meet(ko, v) || rows_meet(ko, qo)) return HQ_ERR_INVALID_ARGUMENT;
+  }
+  if (!p4::own_memory(a.k_codes, a.v_codes, a.code_strides, 1, p4::kRowB, a.n_pages, a.Hkv, a.page_size) ||
+      !p4::own_memory(a.k_scale, a.v_scale, a.scale_strides, 2, p4::kScaleB, a.n_pages, a.Hkv, a.page_size))
+    return HQ_ERR_INVALID_ARGUMENT;
   p4::AppendParams p{};
   p.pg = p4::make_pages(a.k_codes, a.v_codes, a.k_scale, a.v_scale, a.code_strides, a.scale_strides, a.n_pages, a.page_size,
                         a.tables, a.table_stride, a.max_pages);

@@ -822,12 +822,15 @@ extern "C" int hq_paged4_decode(const hq_paged4_decode_args* args) {
   if (a.B == 0) return HQ_OK;
   auto al = [](const void* x, uintptr_t n) { return reinterpret_cast<uintptr_t>(x) % n == 0; };
   if (!a.q || !a.out || !a.lens || !al(a.q, 16) || !al(a.out, 8) || a.q_strides[0] % 8 || a.q_strides[1] % 8 ||
-      a.out_strides[0] % 4 || a.out_strides[1] % 4 || (a.B > 1 && a.out_strides[0] == 0) || (a.Hq > 1 && a.out_strides[1] == 0))
+      a.out_strides[0] % 4 || a.out_strides[1] % 4)
     return HQ_ERR_INVALID_ARGUMENT;
   p4::DecodePlan pl{};
   if (!p4::plan_decode(pl, a.B, a.Hkv, a.Hq / a.Hkv, int64_t(a.page_size) * a.max_pages) || int64_t(a.B) * a.Hq > 0x7fffffff)
     return HQ_ERR_UNSUPPORTED;
   if (!pl.by_unit && (!a.workspace || a.workspace_bytes < pl.bytes || !al(a.workspace, 256))) return HQ_ERR_WORKSPACE;
+  // the output has rows of its own (but for q's: a unit's are read before they are written)
+  const Rows out = packed_rows(a.out, a.B, a.Hq, a.out_strides), q = packed_rows(a.q, a.B, a.Hq, a.q_strides);
+  if (rows_meet(out) || (!same_rows(out, q) && rows_meet(out, q))) return HQ_ERR_INVALID_ARGUMENT;
   p4::DecodeParams p{};
   p.pg = p4::make_pages(a.k_codes, a.v_codes, a.k_scale, a.v_scale, a.code_strides, a.scale_strides, a.n_pages, a.page_size,
                         a.tables, a.table_stride, a.max_pages);

@@ -122,12 +122,11 @@ extern "C" int hq_paged4_gather(const hq_paged4_gather_args* args) {
   if (rc != HQ_OK) return rc;
   if (a.T == 0) return HQ_OK;
   auto al = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
-  if (!a.k_out || !a.v_out || a.k_out == a.v_out || (a.B > 0 && !a.lens) || !al(a.k_out) || !al(a.v_out) ||
+  if (!a.k_out || !a.v_out || (a.B > 0 && !a.lens) || !al(a.k_out) || !al(a.v_out) ||
       a.k_strides[0] % 8 || a.k_strides[1] % 8 || a.v_strides[0] % 8 || a.v_strides[1] % 8)
     return HQ_ERR_INVALID_ARGUMENT;
-  const int64_t* w[2] = {a.k_strides, a.v_strides};
-  for (const int64_t* s : w)
-    if ((a.T > 1 && s[0] == 0) || (a.Hkv > 1 && s[1] == 0)) return HQ_ERR_INVALID_ARGUMENT;
+  const Rows ko = packed_rows(a.k_out, a.T, a.Hkv, a.k_strides), vo = packed_rows(a.v_out, a.T, a.Hkv, a.v_strides);
+  if (rows_meet(ko) || rows_meet(vo) || rows_meet(ko, vo)) return HQ_ERR_INVALID_ARGUMENT;
   p4::GatherParams p{};
   p.pg = p4::make_pages(a.k_codes, a.v_codes, a.k_scale, a.v_scale, a.code_strides, a.scale_strides, a.n_pages, a.page_size,
                         a.tables, a.table_stride, a.max_pages);

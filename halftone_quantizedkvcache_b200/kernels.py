@@ -1587,6 +1587,12 @@ def _packed_out(what: str, name: str, t, shape, q) -> None:
         raise ValueError(f"{what}: {name} must have rows of its own")
 
 
+def _apart(what: str, rc: int, names: str) -> None:
+    """What is left for the C entry to refuse as an argument, once the checks here have passed."""
+    if rc == -1:
+        raise ValueError(f"{what}: {names} must have memory of their own, apart from the inputs'")
+
+
 def _need16(what: str, q) -> None:
     _cuda(q, f"{what} q")
     if q.dtype not in (torch.bfloat16, torch.float16):
@@ -1714,6 +1720,7 @@ def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None
         q_out.data_ptr(), kop, _status_word(dev).data_ptr(), _stream(dev), *ost, *kost, eps, factor,
         1 if interleaved else 0, 1 if rest else 0) + args)
     if rc:
+        _apart(what, rc, "q_out, k_out and the cache's pages")
         check(rc, "hq_paged4_append")
     return q_out
 
@@ -1784,6 +1791,7 @@ def paged4_decode_attn(q, cache, block_tables, lens, *, sm_scale=None, out=None)
         ws.data_ptr() if nw else 0, status.data_ptr(), _stream(dev), *qst, *ost,
         default_scale if sm_scale is None else sm_scale) + args)
     if rc:
+        _apart(what, rc, "out")
         check(rc, "hq_paged4_decode")
     return out
 
@@ -1867,6 +1875,7 @@ def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, 
         v_out.data_ptr(), _status_word(dev).data_ptr(), _stream(dev), *kst, *vst, _DT[dtype],
         1 if made else 0) + args)
     if rc:
+        _apart(what, rc, "k_out and v_out")
         check(rc, "hq_paged4_gather")
     return k_out, v_out
 
@@ -1951,5 +1960,6 @@ def packed_prefill_attn(q, k, v, cu_q, cu_k=None, *, causal=True, sm_scale=None,
         ws.data_ptr() if nw else 0, status.data_ptr(), _stream(dev), *qst, *kst, *vst, *ost, sm_scale,
         1 if rest else 0) + args)
     if rc:
+        _apart(what, rc, "out")
         check(rc, "hq_packed_prefill")
     return out

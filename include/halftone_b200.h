@@ -659,7 +659,10 @@ HQ_API int hq_rope_append_kv(
  * = 0 .. 7, as code + 8 in bits 4 i .. 4 i + 3.  tables int32 [B, max_pages]
  * (row stride table_stride): the pages of sequence b, in order; pages past a
  * sequence's tokens are not read.  Packed arrays [T, H, 128] have strides
- * {token, head} in elements (rows contiguous, 16-byte aligned).
+ * {token, head} in elements (rows contiguous, 16-byte aligned).  Rows that a call
+ * writes (and append's pages of K and of V) share no byte with one another, nor
+ * with other rows or inputs of the call (HQ_ERR_INVALID_ARGUMENT); only a q_out,
+ * or the attentions' out, may be q itself, rows and strides alike.
  *
  * hq_paged4_append: new tokens, in one launch.  Packed rows cu_seqlens[b] ..
  *   cu_seqlens[b + 1] - 1 (int32 [B + 1]; NULL: T == B, one row each) are new

@@ -162,3 +162,47 @@ def test_alloc_and_arguments_of_the_wrong_kind():
         kernels.paged4_gather(cache, None, lens, lens, 4)
     with pytest.raises(ValueError):
         kernels.packed_prefill_attn(q, q, None, lens)
+
+
+# ---- outputs that share memory with one another or with what a call reads
+def test_outputs_that_overlap_are_refused():
+    M = 1 << 20
+    st = (512, 128)                                        # [T, 4, 128]; two heads of it: half a token's row
+    append = dict(q=1 * M, k_new=2 * M, v_new=3 * M, x_dtype=1, q_strides=st, k_strides=(256, 128), v_strides=(256, 128), T=30, B=2,
+                  Hq=4, Hkv=2, D=128, cu_seqlens=256, lens=256, pos_offset=None, q_weight=None, k_weight=None, w_dtype=1, eps=1e-6,
+                  inv_freq=256, rotary_dim=128, interleaved=0, factor=1.0, k_codes=4 * M, v_codes=5 * M, code_strides=C2,
+                  k_scale=6 * M, v_scale=7 * M, scale_strides=SC2, n_pages=5, page_size=16, tables=256, table_stride=4, max_pages=4,
+                  q_out=8 * M, qo_strides=st, k_out=9 * M, ko_strides=(256, 128), copy_rest=0, status=None, stream=None)
+    refused("hq_paged4_append", append, [
+        (-1, dict(k_out=2 * M)), (-1, dict(k_out=2 * M + 512)), (-1, dict(k_out=2 * M + 16)), (-1, dict(k_out=2 * M - 29 * 512)),
+        (-1, dict(k_out=3 * M + 512)), (-1, dict(k_out=1 * M)), (-1, dict(k_out=8 * M + 1024 * 29)),
+        (-1, dict(k_out=2 * M + 256, ko_strides=(512, 128))),
+        (-1, dict(k_out=9 * M, ko_strides=(128, 128))),     # tokens that share heads
+        (-1, dict(q_out=1 * M + 1024)), (-1, dict(q_out=1 * M, qo_strides=(1024, 128))), (-1, dict(q_out=2 * M)), (-1, dict(q_out=3 * M - 16)),
+        (-1, dict(q_out=8 * M, qo_strides=(512, 64))), (-1, dict(q_out=8 * M, qo_strides=(128, 128))),
+        (-1, dict(v_codes=4 * M)), (-1, dict(v_codes=4 * M + 1024)), (-1, dict(code_strides=(1024, 1024))),
+        (-1, dict(v_scale=6 * M + 128 * 9)), (-1, dict(scale_strides=(64, 64))),
+    ])
+    decode = dict(q=1 * M, q_dtype=1, q_strides=st, k_codes=2 * M, v_codes=3 * M, code_strides=C2, k_scale=4 * M, v_scale=5 * M,
+                  scale_strides=SC2, n_pages=5, page_size=16, tables=256, table_stride=4, max_pages=4, lens=256, B=20, Hq=4, Hkv=2,
+                  D=128, sm_scale=0.1, out=6 * M, out_strides=st, workspace=None, workspace_bytes=0, status=None, stream=None)
+    refused("hq_paged4_decode", decode, [
+        (-1, dict(out=1 * M + 1024)), (-1, dict(out=1 * M + 8)), (-1, dict(out=1 * M, out_strides=(256, 128))),
+        (-1, dict(out_strides=(128, 128))), (-1, dict(out_strides=(512, 64))), (-1, dict(out_strides=(0, 128))),
+    ])
+    gather = dict(k_codes=2 * M, v_codes=3 * M, code_strides=C2, k_scale=4 * M, v_scale=5 * M, scale_strides=SC2, n_pages=5,
+                  page_size=16, tables=256, table_stride=4, max_pages=4, lens=256, first=None, cu_seqlens=256, T=70, B=2, Hkv=2,
+                  D=128, k_out=6 * M, v_out=7 * M, out_dtype=1, k_strides=(256, 128), v_strides=(256, 128), zero_rest=0, status=None,
+                  stream=None)
+    refused("hq_paged4_gather", gather, [
+        (-1, dict(v_out=6 * M)), (-1, dict(v_out=6 * M + 512)), (-1, dict(v_out=6 * M + 256)), (-1, dict(v_out=6 * M - 69 * 512)),
+        (-1, dict(k_strides=(512, 128), v_strides=(512, 128), v_out=6 * M + 256)),
+        (-1, dict(k_strides=(128, 128))), (-1, dict(v_strides=(128, 256))), (-1, dict(v_strides=(256, 0))),
+    ])
+    prefill = dict(q=1 * M, k=2 * M, v=3 * M, dtype=1, q_strides=st, k_strides=(256, 128), v_strides=(256, 128), cu_q=256, cu_k=256,
+                   T=160, Tk=160, B=1, Hq=4, Hkv=2, D=128, causal=1, sm_scale=0.1, out=6 * M, out_strides=st, zero_rest=0,
+                   workspace=16 * M, workspace_bytes=1 << 30, status=None, stream=None)
+    refused("hq_packed_prefill", prefill, [
+        (-1, dict(out=2 * M)), (-1, dict(out=3 * M + 159 * 512)), (-1, dict(out=1 * M + 1024)), (-1, dict(out=1 * M, out_strides=(1024, 128))),
+        (-1, dict(out_strides=(128, 128))), (-1, dict(out_strides=(0, 128))), (-1, dict(out_strides=(512, 0))),
+    ])

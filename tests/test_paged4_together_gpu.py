@@ -356,3 +356,60 @@ def test_refusals():
     assert dec(q[:0], cache, tables[:0], none).shape == (0, 4, D)
     assert gat(cache, tables[:0], none, cu[:1], 3)[0].abs().sum() == 0
     assert torch.equal(app(q, k, k, cache, tables[:0], none, cu_seqlens=cu[:1]), q)
+
+
+def test_outputs_in_one_memory_side_by_side():
+    """Rows of q, k and v, of K and V, and of all outputs lie within one another's ranges, but share no byte:
+    such calls give what calls on separate memory give, and those that share some are refused."""
+    from halftone_quantizedkvcache_b200 import kernels
+    T, Hq, H, page, n = 90, 6, 2, 16, 8
+    g = gen(61)
+    lens, cu, now = ints([0, 0]), ints([0, 50, 90]), ints([50, 40])
+    tables = plain.random_tables(2, 4, n, g)
+    inv = kernels.rope_inv_freq(D, 1e6)[0]
+    qkv = torch.randn((T, Hq + 2 * H, D), generator=g, device="cuda").to(torch.bfloat16)
+    q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + H], qkv[:, Hq + H:]
+    plainly = kernels.paged4_alloc(n, H, page_size=page)
+    k16 = torch.empty((T, H, D), dtype=torch.bfloat16, device="cuda")
+    q2 = kernels.paged4_append(q, k, v, plainly, tables, lens, cu_seqlens=cu, inv_freq=inv, k_out=k16)
+    # pages of K and V in turn, q in its place, the new k beside other columns
+    codes = torch.zeros((n, 2, H, page, 64), dtype=torch.uint8, device="cuda")
+    scales = torch.zeros((n, 2, H, page, 4), dtype=torch.float16, device="cuda")
+    cache = {"k": codes[:, 0], "v": codes[:, 1], "k_scale": scales[:, 0], "v_scale": scales[:, 1]}
+    wide = torch.zeros((T, 3 * H, D), dtype=torch.bfloat16, device="cuda")
+    x = qkv.clone()
+    xq, xk, xv = x[:, :Hq], x[:, Hq:Hq + H], x[:, Hq + H:]
+    assert kernels.paged4_append(xq, xk, xv, cache, tables, lens, cu_seqlens=cu, inv_freq=inv, q_out=xq, k_out=wide[:, H:2 * H]) is xq
+    assert torch.equal(xq, q2) and torch.equal(wide[:, H:2 * H], k16) and torch.equal(x[:, Hq:], qkv[:, Hq:])
+    assert all(torch.equal(cache[c], plainly[c]) for c in cache) and (wide[:, :H] == 0).all()
+    kg, vg = kernels.paged4_gather(plainly, tables, now, cu, T)
+    kernels.paged4_gather(cache, tables, now, cu, T, k_out=wide[:, :H], v_out=wide[:, 2 * H:])
+    assert torch.equal(wide[:, :H], kg) and torch.equal(wide[:, 2 * H:], vg) and torch.equal(wide[:, H:2 * H], k16)
+    out = kernels.packed_prefill_attn(q2, k16, v, cu)
+    assert kernels.packed_prefill_attn(xq, wide[:, H:2 * H], xv, cu, out=xq) is xq and torch.equal(xq, out)
+    step = kernels.paged4_decode_attn(q2[:2], plainly, tables, now)
+    y = q2.clone()
+    assert torch.equal(kernels.paged4_decode_attn(y[:2], cache, tables, now, out=y[:2]), step) and torch.equal(y[2:], q2[2:])
+    assert kernels.ragged_status() == 0
+    # shared in part
+    big = torch.zeros((T + 1, Hq, D), dtype=torch.bfloat16, device="cuda")
+    bad = [
+        lambda: kernels.paged4_append(q, k, v, plainly, tables, lens, cu_seqlens=cu, k_out=qkv[:, Hq + 1:Hq + 1 + H]),
+        lambda: kernels.paged4_append(q, k, v, plainly, tables, lens, cu_seqlens=cu, q_out=qkv[:, 1:Hq + 1]),
+        lambda: kernels.paged4_append(big[:T], k, v, plainly, tables, lens, cu_seqlens=cu, q_out=big[1:]),
+        lambda: kernels.paged4_append(q, k, v, plainly, tables, lens, cu_seqlens=cu, q_out=big[1:], k_out=big[:T, :H]),
+        lambda: kernels.paged4_append(q, k, v, {**cache, "v": cache["k"]}, tables, lens, cu_seqlens=cu),
+        lambda: kernels.paged4_append(q, k, v, {**cache, "v_scale": cache["k_scale"]}, tables, lens, cu_seqlens=cu),
+        lambda: kernels.paged4_gather(plainly, tables, now, cu, T, k_out=big[:T, :H], v_out=big[1:, :H]),
+        lambda: kernels.paged4_gather(plainly, tables, now, cu, T, k_out=big[:T, :H], v_out=big[:T, 1:H + 1]),
+        lambda: kernels.packed_prefill_attn(big[:T], k, v, cu, out=big[1:]),
+        lambda: kernels.packed_prefill_attn(q, big[:T, :H], v, cu, out=big[:T]),
+        lambda: kernels.packed_prefill_attn(q, k, big[1:, Hq - H:], cu, out=big[:T]),
+        lambda: kernels.paged4_decode_attn(big[:2], plainly, tables, now, out=big[1:3]),
+        lambda: kernels.paged4_decode_attn(q2[:2], plainly, tables, now, out=torch.as_strided(big, (2, Hq, D), (D, D, 1))),
+    ]
+    saved = {c: t.clone() for c, t in plainly.items()}
+    for call in bad:
+        with pytest.raises(ValueError, match="memory of their own"):
+            call()
+    assert all(torch.equal(plainly[c], saved[c]) for c in saved) and (big == 0).all()

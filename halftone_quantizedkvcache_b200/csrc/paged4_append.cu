@@ -21,7 +21,7 @@
 // through shared memory (the next row in registers instead: 179 us).
 //
 // 8 x 4096 tokens of 16 q heads and 8 kv heads, both norms, full rotation, k kept: 126 us, 4.0 TB/s of
-// bytes moved.  Bound by issue slots (70 % of them taken; arithmetic units 45 %, DRAM 36 % at half that
+// bytes moved.  Bound by issue slots (72 % of them taken; arithmetic units 45 %, DRAM 36 % at half that
 // size): for a lane and row of k a reduction of 128 squares, the turn and the codes.  (8 lanes a row, both
 // values of a pair in one lane, take 27 % fewer instructions but 96 registers: 131 us, the 20 warps an SM hide
 // less.)
@@ -223,6 +223,7 @@ __device__ __forceinline__ void exact_row(const AppendParams& p, const void* wei
     }
     if (fabs(z[e]) > amax || z[e] != z[e]) amax = fabs(z[e]);  // (NaN if any is: nothing is above it)
   }
+  __syncwarp();                           // (the row has been read, by all lanes: out may be its memory)
   if (out)
     *reinterpret_cast<uint2*>(out + 2 * d0) = make_uint2(pack16<DT>(static_cast<float>(z[0]), static_cast<float>(z[1])),
                                                          pack16<DT>(static_cast<float>(z[2]), static_cast<float>(z[3])));

@@ -412,7 +412,7 @@ def test_append_turned_rows_that_hold_no_number(dtype, inter, rot, bad):
 
 def lost_weights(q, cache, tables, b, n, scale=None):
     """What rounding p x scale to a 16-bit whole number does to the output at most: per row, group and tile of
-    64 tokens half a step, 1 / (2 x 32512), of the largest p x scale (taken to 2^-9 of itself), times
+    64 tokens half a step, 1 / (2 x 32512), of the largest p x scale (taken to 2^-8 of itself), times
     sum |code|.  q [Hkv, rep, D] -> [Hkv, rep, D]."""
     page = cache["k"].shape[2]
     k = plain.values(cache, "k", tables, b, n).transpose(0, 1)
@@ -577,3 +577,20 @@ def test_append_norms_in_place_over_many_heads_and_rows_behind_the_last_sequence
                                  k_weight=w[1], q_out=q) is q
     assert torch.equal(q, apart) and torch.equal(q[-3:], q0[-3:])
     check_append(q0, k, v, cache, tables, new, [0, 0], before, q, None, inv, w)
+
+
+@pytest.mark.parametrize("rot,inter", [(0, False), (32, False), (96, True), (128, True)])
+def test_append_norms_in_place_with_part_of_the_channels_turned(rot, inter):
+    """Every row for float64, in its own memory: some lanes wait for their partners' channels, others do not."""
+    from halftone_quantizedkvcache_b200 import kernels
+    new = [700, 33]
+    q, k, v, cache, tables = append_case(new, [3, 9], 2, 4, torch.bfloat16, 32, 56)
+    for x in (q, k):
+        x.mul_(2.0 ** 66)
+    before = {n: y.clone() for n, y in cache.items()}
+    inv = kernels.rope_inv_freq(rot, 1e6)[0] if rot else None
+    w = [torch.empty(D, device="cuda").uniform_(0.2, 2.0, generator=gen(57)) for _ in range(2)]
+    q0 = q.clone()
+    kernels.paged4_append(q, k, v, cache, tables, ints([3, 9]), cu_seqlens=cum(new), inv_freq=inv, interleaved=inter, q_weight=w[0],
+                          k_weight=w[1], q_out=q)
+    check_append(q0, k, v, cache, tables, new, [3, 9], before, q, None, inv, w, inter)

@@ -7,21 +7,26 @@
 // Work.  Row r of a unit (sequence, kv head) is q head kvh n_rep + r % n_rep of query r / n_rep; 128
 // rows are the lanes of a tile in tensor memory, and a block takes two tiles, 256 rows, that share
 // every K and V tile of 128 keys.  Where that leaves SMs idle the keys are split over several blocks,
-// whose states (m, l, O) join_kernel puts together.  Blocks with the most keys start first.
+// whose states (m, l, O) join_kernel puts together.  How many is one number for the whole call, from averages
+// that the host has: one long past beside many short sequences keeps its keys in one piece (plan()).  Blocks
+// start from the end of the packed order, so of one sequence the pieces with the most keys come first; of
+// several that is so where the last are the longest (16 sequences of 256 to 4096 tokens: 406 us in rising
+// order, 407 to 419 in falling).  Every block looks for its sequence through all starts, 32 at a time: 64 sequences of
+// one token 23 us, 1024 of them 420.
 //
 // Roles of a block: softmax warps, 4 or 8 a row tile; one warp that issues the products; one that loads K
 // and V by TMA; two that look over the V tiles of masked steps.  S = Q K^T goes to tensor memory; the
 // softmax threads take it into registers and write P in 16 bits over it; O += P V reads P from there.
 // While one tile is in its softmax the other's products run.  The running maximum moves only when it grows
 // by more than 8 (P <= 2^8), so O is rarely rescaled; sums are float32.  P is rounded to the model's type
-// (2^-9 of each weight in bf16, 2^-12 in float16: what the output itself is rounded by; in float16 also
+// (2^-8 of each weight in bf16, 2^-11 in float16: what the output itself is rounded by; in float16 also
 // 2^-32 of the largest).
 //
-// 2 x 8192 tokens of 16 q heads and 8 kv heads, bf16: 454 us, 1210 TFLOP/s in a burst (530 in a
-// run of calls, at 990 W and 1.64 GHz).  Neither unit is full (1 x 8192:
+// 2 x 8192 tokens of 16 q heads and 8 kv heads, bf16: 530 to 540 us in a run of calls, at 990 W and 1.64 GHz
+// (455 to 462, 1200 TFLOP/s, in a burst).  Neither unit is full (1 x 8192:
 // tensor 57 %, exponentials 58 %, issue slots 37 %): a row tile's scores, softmax and products follow one
-// another, and two tiles a block leave gaps where both wait.  (Two threads a row 549 us; a quarter of the
-// exponentials as polynomials no change, half of them 513.)
+// another, and two tiles a block leave gaps where both wait.  (Two threads a row take 19 % more; a quarter of the
+// exponentials as polynomials no change, half of them 12 % more.)
 //
 // A V row holding an infinity or NaN spoils the rows that see it and no others: 0 x NaN is NaN in the
 // product, so on steps where some row does not see every key such rows are zeroed in shared memory
@@ -52,8 +57,8 @@ template <int NT>
 struct Cfg {
   static constexpr int kRows = 128 * NT;
   // Softmax threads: one a row with 128 keys, or (one row tile, where nothing hides a step's length) two with
-  // 64 each, which tell each other their maxima.  One tile: 64 sequences of up to 200 tokens 52 us with two,
-  // 57 with one; one of 512 15.2 and 16.5.  Two tiles: 2 x 8192 549 us with two, 460 with one.
+  // 64 each, which tell each other their maxima.  One tile: 64 sequences of up to 200 tokens take 9 % less time
+  // with two than with one, one of 512 8 %.  Two tiles: 2 x 8192 19 % more with two.
   static constexpr int kH = NT == 1 ? 2 : 1, kKeys = 128 / kH;
   static_assert(NT * kH <= 2, "places for one pair of threads a row");
   static constexpr int kSoft = 128 * NT * kH, kThreads = kSoft + 128;
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
     }
   }
   if (warp == 0) {
-    // heavy (last) pieces first
+    // from the end: the last pieces of a sequence have the most keys
     const int item = p.units - 1 - static_cast<int>(blockIdx.x) / p.n_split;
     int b, y;
     Seq s{};
@@ -392,9 +397,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 3 - NT)
     for (int n = 0; n < min(copies, kStages); ++n) copy(n);
   }
   // Q, 16 lanes a row: K-major tiles of two 64-channel halves, 128-byte swizzle; rows past the last: zeros.
-  // (By tensor
-  // map, where n_rep divides 128, a block starts up to 1.5 us earlier: 64 sequences of up to 200 tokens 46 us
-  // against 50, 2 x 8192 454 against 460.  Rows past the last are then whatever follows: no row sees another.)
+  // (By tensor map, where n_rep divides 128, a block starts up to 1.5 us earlier: 64 sequences of up to 200
+  // tokens take 8 % less time, 2 x 8192 1 %.  Rows past the last are then whatever follows: no row sees another.)
   if (!p.q_tma) {
     constexpr int kEach = (kRows * 16 + kThreads - 1) / kThreads;
     static_assert(kThreads % 16 == 0, "a half-warp per row");
@@ -824,9 +828,9 @@ inline bool plan(Plan& pl, int64_t T, int64_t Tk, int B, int Hkv, int nrep) {
   if (T * nrep > 0x3fffffff || Tk > 0x3fffffff) return false;
   const int sms = current_sm_count();
   // One row tile a block where sequences are short, in rows and in keys: 64 sequences of up to 200
-  // tokens 45 us against 50 (32 of up to 300, 4 q heads a kv head, 85 and 85); with more of either, K and V
-  // are better shared: 8 of 512 29 us against 32 (one of 512 14.7 and 14.4), one of 2048 38 against 40,
-  // 2 x 8192 460 against 529, 3 x 77 queries over 4022 keys 23 against 26.
+  // tokens 45 us against 49 (32 of up to 300, 4 q heads a kv head, 85 and 85); with more of either, K and V
+  // are better shared: 8 of 512 29 us against 32 (one of 512 14.9 and 14.4), one of 2048 38 against 40,
+  // 2 x 8192 459 against 535, 3 x 77 queries over 4022 keys 19.5 against 21.5.
   pl.nt = T * nrep <= 512LL * B && Tk <= 1024LL * B ? 1 : 2;
   const int rows = 128 * pl.nt;
   // n rows are (n - 1) / rows + 1 pieces, rounded down; so are all sequences' at most
@@ -836,7 +840,8 @@ inline bool plan(Plan& pl, int64_t T, int64_t Tk, int B, int Hkv, int nrep) {
   // least: 2 us a key tile of an average sequence; for more than one 3 us of a second launch (more than 8: 5.5), and
   // 0.15 ns a row and part for the states.  (Unsplit and split: 3 x 77 queries over 4022 keys 57 us and 19; 4 x 16 over 800 21
   // and 14; one of 1000 with 8 q heads over 2 kv heads 22 and 18; one of 512 14.7 and 16.1, 2 of 784 18.5 and
-  // 20.3, which stay whole.)
+  // 20.3, which stay whole.  What averages miss: 16 queries over 32768 keys are split in 16 and take 39 us alone,
+  // but 397 beside 16 sequences of one token, whose units leave the call unsplit.)
   const int64_t room = sms / std::max<int64_t>(units, 1);
   const int64_t tiles = (Tk + kBN * static_cast<int64_t>(B) - 1) / (kBN * static_cast<int64_t>(B));
   int64_t best = INT64_MAX;

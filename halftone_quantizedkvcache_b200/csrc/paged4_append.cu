@@ -64,10 +64,10 @@ struct AppendParams {
 };
 
 // Error of the float32 route, relative to |x w cos| + |o w_o sin| (times r and the factor), in units of 2^-24:
-// half that of the mean (squares are exact but for 2^-150, below 2^-24 of it where it is a normal number; 3 sums
-// in a lane's half, the halves, 4 rounds, eps: 10) 5 and
-// that of its root's correction 2.5, cos or sin 1, their weight 1 and factor 1, the turn's product 1 and sum
-// 1, r's product 1: 13.5.  The sum is at most the pair's length, sqrt(2) times the larger of its turned values.
+// half that of the mean (squares are exact but for 2^-150, below 2^-24 of it where it is a normal number; 3
+// sums in a lane's half, the halves, 4 rounds, eps: 10) 5 and that of its root's correction 2.5, cos or sin 1,
+// their weight 1 and factor 1, the turn's product 1 and sum 1, r's product 1: 13.5.  The sum is at most the
+// pair's length, sqrt(2) times the larger of its turned values.
 constexpr float kSlack = 1.4143f * 13.5f / 16777216.0f;
 
 constexpr uint32_t kWhole = 0x80000000u;  // a listed row that float64 writes to q_out or k_out too

@@ -7,9 +7,10 @@
 // what crosses a block's border leaves partial states (m, l, o) that join_kernel puts together, always
 // in the order of the line.
 //
-// 64 sequences of 4096 to 8192 tokens, 8 kv heads of 2 rows: 108 us, 4.2 TB/s of cache.  What holds it
-// back is the work between loads (issue slots 49 %, arithmetic units 44 %, the matrix units 25 %, DRAM 49 %
-// at half that size): 144 bytes a token and head are 256 codes to unpack, twice.  Both products are
+// 64 sequences of 4096 to 8192 tokens, 8 kv heads of 2 rows: 108 us, 4.2 TB/s of cache.  No unit is full
+// (issue slots 49 %, arithmetic units 44 %, the matrix units 24 %, DRAM 47 % at half that size): the 8 warps
+// that an SM has registers for do not hide the latency of a tile's chain of products, reductions and
+// transpositions, and 144 bytes a token and head are 256 codes to unpack, twice.  Both products are
 // whole-number products on bytes (mma.sync m16n8k32, exact), the codes being the 16-row operand, since a
 // word of 8 codes becomes bytes with two masks and a shift (matrix instructions that take their operands
 // from shared memory would want those bytes written there first: three times the tile's traffic):
@@ -19,9 +20,12 @@
 //   * P V: p times the token's group scale, relative to the row's largest such product of the tile, is a
 //     16-bit whole number (2^-16 of that product is lost of each; against the largest p and the largest
 //     scale, each by itself, the tile took 3 % less time, but a large scale without weight left the others
-//     no bits) in two digits, transposed in registers by movmatrix; four tokens' bytes are turned with permutes.  A tile's sums
-//     go into the float32 state with the tile's and the group's factor.
+//     no bits) in two digits, transposed in registers by movmatrix; four tokens' bytes are turned with
+//     permutes.  A tile's sums go into the float32 state with the tile's and the group's factor.
 // (As bf16 products, 7 to 12 instructions a word and twice the products, 64 x 8192 tokens took 138 us.)
+// Up to 4 rows a kv head share one pass over its codes, up to 8 another that takes 1.5 times as long; more rows
+// take a pass for every 8 of them (64 x 8192 whole tokens, 8 kv heads: 2 and 4 rows 136 us, 8 rows 207, 16
+// rows 392, 128 rows 2861).
 // Copies: every warp has its own ring of stages filled by bulk copies, one per page, side and kind,
 // issued by one lane each.
 #include <algorithm>
@@ -146,7 +150,7 @@ __device__ __forceinline__ void next_unit(Cursor& c, const int* lens, int per) {
 }
 // the whole number that a row's largest |q| becomes: below 2^21, and its upper digit below 32
 constexpr float kFixed = 2088960.0f;
-// and that a tile's largest weight becomes (taken to 2^-9 of itself: 32576 at most, 64 x 8 of them below 2^24)
+// and that a tile's largest weight becomes (taken to 2^-8 of itself: 32640 at most, 64 x 8 of them below 2^24)
 constexpr float kWeight = 32512.0f;
 // largest weights below this (2^-110 of p = 1 under a scale of 1) are taken for none
 constexpr float kNoWeight = 7.7037198e-34f;
@@ -491,7 +495,7 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
       // ---- P V, two groups at a time: 2 gg in columns 2 r, 2 gg + 1 in 2 r + 1
 #pragma unroll
       for (int gg = 0; gg < 2; ++gg) {
-        // the tokens' V scales, and the rows' largest weights p x scale (bf16: to 2^-9 of themselves)
+        // the tokens' V scales, and the rows' largest weights p x scale (bf16: to 2^-8 of themselves)
         uint32_t u[kSets];
         float big[NT][2];
 #pragma unroll
@@ -589,7 +593,7 @@ __global__ void __launch_bounds__(32 * Cfg<NT>::kWarps, 1) decode_kernel(const _
                 mma_u8u8(q8[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][2 * k], lo[nt][2 * k + 1], k ? q8[nt][m] : cl[nt]);
               }
           }
-          // 64 x 8 x 32576 is below 2^24: exact in float32
+          // 64 x 8 x 32640 is below 2^24: exact in float32
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const float w = f[nt] * ((e ? top[nt].y : top[nt].x) * (1.0f / kWeight));

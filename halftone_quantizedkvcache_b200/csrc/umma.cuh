@@ -2,7 +2,8 @@
 // shared-memory layout and its matrix descriptor, the kind::f16 instruction
 // descriptor, issue and commit of an MMA, the proxy and thread-sync fences,
 // 32-column tensor-memory loads and stores, and a bounded wait.  Used by
-// prefill_attn.cu and ragged_attn.cu.
+// prefill_attn.cu, ragged_attn.cu and packed_prefill.cu; paged4_decode.cu
+// takes the wait.
 #pragma once
 
 #include "hq_common.cuh"

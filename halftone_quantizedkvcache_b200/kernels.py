@@ -1497,8 +1497,8 @@ def paged4_alloc(n_pages: int, n_kv_heads: int, *, page_size: int = 64, head_dim
     """Pages of a cache held in 4 bits (``paged4_append`` / ``paged4_decode_attn`` /
     ``paged4_gather``): codes ``k`` / ``v`` uint8 ``[n_pages,Hkv,page_size,64]`` and scales
     ``k_scale`` / ``v_scale`` float16 ``[n_pages,Hkv,page_size,4]``, 144 bytes per token and kv head.
-    Per token 4 groups of 32 channels: ``s = f16(amax / 7.5)``, codes ``clamp(rint(x / s), -8, 7)``
-    (the byte order within a row is the kernels' own, include/halftone_b200.h; ``paged4_gather``
+    Per token 4 groups of 32 channels: ``s = f16(amax / 7.5)``, at most 65504 (larger values
+    saturate), codes ``clamp(rint(x / s), -8, 7)`` (the byte order within a row is the kernels' own, include/halftone_b200.h; ``paged4_gather``
     reads it).  Which pages a sequence has is the caller's block table."""
     if page_size not in PAGED4_SIZES:
         raise ValueError(f"paged4: page_size must be one of {PAGED4_SIZES}")
@@ -1617,9 +1617,10 @@ def paged4_append(q, k_new, v_new, cache, block_tables, lens, *, cu_seqlens=None
     rotated values, codes and scales as float64 arithmetic finds them; V as it came.
 
     Returns the new q (``q_out``, which may be q; rows of no sequence stay what they were there,
-    or are q's in a result made by this call); ``k_out [T,Hkv,128]`` (memory of its own) takes the
-    new k, for the prompt's own attention.  K and V of real tokens are finite (others spoil their group).  A
-    sequence whose tokens do not fit its table, and a token whose page is no page of the cache, are
+    or are q's in a result made by this call); ``k_out [T,Hkv,128]`` takes the new k, for the
+    prompt's own attention.  ``q_out``, ``k_out`` and the pages of K and of V have memory of their
+    own (ValueError).  K and V of real tokens are finite (others spoil their group, with a norm
+    their row).  A sequence whose tokens do not fit its table, and a token whose page is no page of the cache, are
     not written and set ``ragged_status()``; no two new tokens may go to the same place.
     """
     what = "paged4_append"
@@ -1732,8 +1733,8 @@ def paged4_decode_attn(q, cache, block_tables, lens, *, sm_scale=None, out=None)
     ``block_tables`` int32 ``[B,pages]`` and ``lens`` int32 ``[B]`` on the device: sequence b attends
     its first ``lens[b]`` tokens (at most those its table holds), and gives zeros where there are
     none.  What pages hold past them does not matter.  Returns the output in q's layout and dtype (or
-    writes ``out [B,Hq,128]``).  Nothing depends on ``lens`` on the host: a captured call replays while
-    sequences grow.  Sums are float32; of q 2^-22 of its row's largest value is rounded off, of each
+    writes ``out [B,Hq,128]``, which may be q and shares no memory with it otherwise).  Nothing depends
+    on ``lens`` on the host: a captured call replays while sequences grow.  Sums are float32; of q 2^-22 of its row's largest value is rounded off, of each
     weight times V scale 2^-16 of the row's largest such product among 64 tokens.  A page number
     outside the cache sets ``ragged_status()``, and that sequence's output has no meaning.
     """
@@ -1806,7 +1807,7 @@ def paged4_gather(cache, block_tables, lens, cu_seqlens, n_rows, *, first=None, 
     chunk over a cached past attends (``packed_prefill_attn``), or with ``first`` the new tokens as
     later steps will see them.  Values are ``scale * code``, rounded once (beyond float16's range:
     infinities).  Rows that no token goes to
-    are zeros, or what they were in ``k_out`` / ``v_out``.  A page number outside the cache sets
+    are zeros, or what they were in ``k_out`` / ``v_out`` (which share no memory).  A page number outside the cache sets
     ``ragged_status()``; that token's row counts as one that no token goes to.
     """
     what = "paged4_gather"
@@ -1888,9 +1889,11 @@ def packed_prefill_attn(q, k, v, cu_q, cu_k=None, *, causal=True, sm_scale=None,
     ``cu_q[b] .. cu_q[b+1]-1`` and the keys ``cu_k[b] .. cu_k[b+1]-1`` (int32 ``[B+1]`` on the device;
     ``cu_k`` defaults to ``cu_q``: whole prompts).  The queries stand at the last positions: query i
     of n sees keys ``j <= m - n + i`` of m (``causal=False``: all of them), and gives zeros where that
-    is none.  Returns ``[T,Hq,128]``; rows before the first sequence and behind the last are zeros, or are left
-    as they were in ``out``.  ``sm_scale`` (default 1/sqrt(128)) is positive.  Sums are float32, the weights rounded
-    to q's type.  A V row that holds an infinity or NaN spoils the rows that see it, and no others.
+    is none.  Returns ``[T,Hq,128]``; rows before the first sequence and behind the last are zeros, or
+    are left as they were in ``out`` (which may be q, and shares no memory with q, k or v otherwise).
+    ``sm_scale`` (default 1/sqrt(128)) is positive.  Sums are float32, the weights rounded to q's
+    type.  How keys are split over blocks follows from averages: a long past beside many short
+    sequences is better served by a call of its own.  A V row that holds an infinity or NaN spoils the rows that see it, and no others.
     """
     what = "packed_prefill_attn"
     if cu_k is None:

@@ -649,8 +649,9 @@ HQ_API int hq_rope_append_kv(
 
 /* ------------------------------------------------------------------------
  * A paged cache held in 4 bits.  Per token and kv head 128 channels in 4 groups
- * of 32: scale s = f16(amax / 7.5), codes clamp(rint(x / s), -8, 7), values s *
- * code.  k_codes / v_codes [n_pages, Hkv, page_size, 64] bytes and k_scale /
+ * of 32: scale s = f16(amax / 7.5), at most 65504 (larger values saturate; a
+ * group with an infinity or NaN has the scale NaN), codes clamp(rint(x / s), -8,
+ * 7), values s * code.  k_codes / v_codes [n_pages, Hkv, page_size, 64] bytes and k_scale /
  * v_scale [n_pages, Hkv, page_size, 4] float16, each page and head contiguous;
  * code_strides (bytes, multiples of 16) and scale_strides (elements, multiples
  * of 8) are {page, head}; page_size 16, 32, 64, 128 or 256.  A row's 64 bytes:

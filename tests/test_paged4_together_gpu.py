@@ -413,3 +413,26 @@ def test_outputs_in_one_memory_side_by_side():
         with pytest.raises(ValueError, match="memory of their own"):
             call()
     assert all(torch.equal(plainly[c], saved[c]) for c in saved) and (big == 0).all()
+
+
+@pytest.mark.parametrize("nq,nk,Hkv,rep", [([512], [512], 8, 2), ([2100, 900], [2100, 900], 2, 2), ([20, 48, 77], [1020, 2600, 4099], 2, 6),
+                                           ([64, 65, 63, 1], [64, 65, 63, 1], 2, 4), ([600], [500], 8, 2), ([300, 7], [300, 7], 1, 3)])
+def test_attention_over_its_queries(nq, nk, Hkv, rep):
+    """out is q: one and two row tiles a block, keys split or not, Q by tensor map or by loads."""
+    from halftone_quantizedkvcache_b200 import kernels
+    g = gen(62)
+    q = torch.randn((sum(nq), Hkv * rep, D), generator=g, device="cuda").to(torch.bfloat16)
+    k, v = (torch.randn((sum(nk), Hkv, D), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    ref = kernels.packed_prefill_attn(q, k, v, cum(nq), cum(nk))
+    for _ in range(10):
+        x = q.clone()
+        assert kernels.packed_prefill_attn(x, k, v, cum(nq), cum(nk), out=x) is x
+        assert torch.equal(x, ref)
+    cache = plain.random_cache(kernels, len(nk) * 65 + 1, Hkv, 64, g)
+    tables = plain.random_tables(len(nk), 65, len(nk) * 65 + 1, g)
+    y = q[:len(nk)].contiguous()
+    step = kernels.paged4_decode_attn(y, cache, tables, ints(nk))
+    for _ in range(10):
+        x = y.clone()
+        kernels.paged4_decode_attn(x, cache, tables, ints(nk), out=x)
+        assert torch.equal(x, step)
